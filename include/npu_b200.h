@@ -36,6 +36,13 @@ extern "C" {
 #define NPUB200_DTYPE_BF16 0
 #define NPUB200_DTYPE_F32 1
 
+/* Activations of npub200_gemm_act. */
+#define NPUB200_ACT_GELU 1       /* y/2 (1 + erf(y / sqrt 2)) */
+#define NPUB200_ACT_GELU_TANH 2  /* y/2 (1 + tanh(sqrt(2/pi) (y + 0.044715 y^3))) */
+#define NPUB200_ACT_QUICK_GELU 3 /* y sigmoid(1.702 y) */
+#define NPUB200_ACT_SILU 4       /* y sigmoid(y) */
+#define NPUB200_ACT_RELU 5       /* max(y, 0) */
+
 /* Library version (major * 10000 + minor * 100 + patch). */
 int npub200_version(void);
 
@@ -85,6 +92,14 @@ int npub200_gemm_w(const void* x, int64_t ldx, int64_t m, int64_t k, int64_t wei
 int npub200_gemm_residual(const void* x, int64_t ldx, int64_t m, int64_t k, const void* w, int64_t ldw, int64_t n,
                           const void* bias, int bias_dtype, const void* residual, int64_t ldr, void* out, int64_t ldo,
                           int out_dtype, void* workspace, size_t workspace_bytes, int variant, void* stream);
+/* GEMM with bias, activation and residual in its epilogue: out = act(x . W^T + bias) + residual, all of it in f32
+ * before the one rounding to the output type. activation: an NPUB200_ACT_* code; bias and residual may be NULL;
+ * residual bf16 [M, N] with row stride ldr (may be `out` itself when out is bf16). The feed-forward projection of a
+ * block without gating (the reference offloads the projection, npu/xdna1_gemm.py:428-448, and leaves the activation
+ * to the host). Otherwise as npub200_gemm. */
+int npub200_gemm_act(const void* x, int64_t ldx, int64_t m, int64_t k, const void* w, int64_t ldw, int64_t n,
+                     const void* bias, int bias_dtype, int activation, const void* residual, int64_t ldr, void* out,
+                     int64_t ldo, int out_dtype, void* workspace, size_t workspace_bytes, int variant, void* stream);
 /* GEGLU feed-forward projection in one kernel: W is [2n, K] (nn.Linear layout of SD1.5's GEGLU `proj`: the n
  * value rows, then the n gate rows), bias [2n] or NULL, and out[M, n] = (x.W[j] + b[j]) * gelu(x.W[n+j] + b[n+j])
  * with the exact (erf) GELU, f32 accumulation and gating, out f32 or bf16. The reference computes the projection

@@ -17,6 +17,7 @@ TORCH_OPS_PATH = os.path.join(HERE, "libnpub200_torch.so")
 
 OK, EINVAL, ECUDA, EUNSUPPORTED, EDEVICE = 0, -1, -2, -3, -4
 DTYPE_BF16, DTYPE_F32 = 0, 1
+ACTIVATIONS = {"gelu": 1, "gelu_tanh": 2, "quick_gelu": 3, "silu": 4, "relu": 5}  # NPUB200_ACT_*
 
 _c_i64 = ctypes.c_int64
 _c_p = ctypes.c_void_p
@@ -50,6 +51,9 @@ _SIGNATURES = {
     "npub200_gemm_residual": (ctypes.c_int, [_c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, ctypes.c_int,
                                              _c_p, _c_i64, _c_p, _c_i64, ctypes.c_int, _c_p, ctypes.c_size_t,
                                              ctypes.c_int, _c_p]),
+    "npub200_gemm_act": (ctypes.c_int, [_c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, ctypes.c_int,
+                                        ctypes.c_int, _c_p, _c_i64, _c_p, _c_i64, ctypes.c_int, _c_p, ctypes.c_size_t,
+                                        ctypes.c_int, _c_p]),
     "npub200_gemm_noalloc": (ctypes.c_int, [_c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, ctypes.c_int,
                                             _c_p, _c_i64, ctypes.c_int, ctypes.c_int, _c_p]),
     "npub200_gemm_w": (ctypes.c_int, [_c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, ctypes.c_int, _c_p, _c_i64,

@@ -171,7 +171,7 @@ size_t gemm_workspace_bytes(const void* x, int64_t ldx, int64_t m, int64_t k, co
 int gemm_with_workspace(const void* x, int64_t ldx, int64_t m, int64_t k, const void* w, int64_t ldw, int64_t n,
                         const CUtensorMap* w_map, const void* bias, int bias_dtype, void* out, int64_t ldo,
                         int out_dtype, void* workspace, size_t workspace_bytes, int variant, void* stream,
-                        int geglu, const void* residual, int64_t ldr) {
+                        int geglu, const void* residual, int64_t ldr, int act) {
   if (int rc = check_gemm_common(m, k, n, bias_dtype, out, ldo, out_dtype)) return rc;
   if (x == nullptr || w == nullptr) return fail(kErrInvalid, "GEMM operand pointer is null");
   if (ldx < k) return fail(kErrInvalid, "x row stride %lld < K=%lld", (long long)ldx, (long long)k);
@@ -199,6 +199,7 @@ int gemm_with_workspace(const void* x, int64_t ldx, int64_t m, int64_t k, const 
                                                   (long long)n);
   p.residual = residual;
   p.ldr = ldr;
+  p.act = act;
 
   const DeviceInfo* dev = nullptr;
   if (int rc = current_device_info(&dev)) return rc;
@@ -325,6 +326,16 @@ int npub200_gemm_residual(const void* x, int64_t ldx, int64_t m, int64_t k, cons
   if (residual == nullptr) return fail(kErrInvalid, "npub200_gemm_residual needs a residual");
   return gemm_with_workspace(x, ldx, m, k, w, ldw, n, nullptr, bias, bias_dtype, out, ldo, out_dtype, workspace,
                              workspace_bytes, variant, stream, 0, residual, ldr);
+}
+
+int npub200_gemm_act(const void* x, int64_t ldx, int64_t m, int64_t k, const void* w, int64_t ldw, int64_t n,
+                     const void* bias, int bias_dtype, int activation, const void* residual, int64_t ldr, void* out,
+                     int64_t ldo, int out_dtype, void* workspace, size_t workspace_bytes, int variant, void* stream) {
+  if (int rc = check_gemm_common(m, k, n, bias_dtype, out, ldo, out_dtype)) return rc;
+  if (activation < NPUB200_ACT_GELU || activation > NPUB200_ACT_RELU)
+    return fail(kErrInvalid, "unknown activation code %d", activation);
+  return gemm_with_workspace(x, ldx, m, k, w, ldw, n, nullptr, bias, bias_dtype, out, ldo, out_dtype, workspace,
+                             workspace_bytes, variant, stream, 0, residual, ldr, activation);
 }
 
 int npub200_gemm_geglu(const void* x, int64_t ldx, int64_t m, int64_t k, const void* w, int64_t ldw, int64_t n,

@@ -30,6 +30,7 @@
 #include <mutex>
 
 #include "internal.h"
+#include "npu_b200.h"
 
 namespace npub200 {
 
@@ -53,6 +54,7 @@ struct GemmArgs {
   int bias_img_pixels, bias_imgs;
   const void* residual;       // bf16 [M, N] added in the epilogue (row stride ldr), or null
   long long ldr;
+  int act;                    // activation form: NPUB200_ACT_* code applied between the bias and the residual
   int cv_w, cv_hw, cv_cblocks;  // 3x3 convolution form: image width, pixels per image, 64-channel blocks of Cin
   void* out;
   long long ldo;
@@ -198,6 +200,7 @@ __device__ __forceinline__ void add_residual32(const GemmArgs& a, int grow, int 
 constexpr int kModePlain = 0;
 constexpr int kModeGeglu = 1;
 constexpr int kModeConv3x3 = 2;
+constexpr int kModeAct = 3;  // plain GEMM with an activation between the bias and the residual
 
 // GELU with the error function (torch's default `F.gelu`, approximate='none'): y * Phi(y) = y/2 * (1 + erf(y/sqrt2)).
 // erf by Abramowitz & Stegun, Handbook of Mathematical Functions, formula 7.1.26 (Hastings' rational approximation,
@@ -213,6 +216,37 @@ __device__ __forceinline__ float gelu_erf(float y) {
   q = fmaf(q, t, 0.254829592f);
   const float tail = q * t * fast_exp2(-z * z * 1.4426950408889634f);  // 1 - erf(z)
   return 0.5f * y * (y >= 0.0f ? 2.0f - tail : tail);
+}
+
+// y * sigmoid(s) = y / (1 + 2^(-s log2 e)); a denominator past 2^126 gives 0 (the true value is below 1e-37 |y|).
+__device__ __forceinline__ float times_sigmoid(float y, float s) {
+  return __fdividef(y, 1.0f + fast_exp2(-1.4426950408889634f * s));
+}
+
+// The activation of NPUB200_ACT_* code `act` on 32 (or 4) values; the branch is uniform over the grid. The tanh form of
+// GELU is y sigmoid(2u) with u = sqrt(2/pi) (y + 0.044715 y^3), since (1 + tanh u) / 2 = sigmoid(2u): one exp2 and one
+// reciprocal, and no cancellation for negative y.
+template <int N>
+__device__ __forceinline__ void activate(int act, float (&v)[N]) {
+  if (act == NPUB200_ACT_GELU) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = gelu_erf(v[j]);
+  } else if (act == NPUB200_ACT_GELU_TANH) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float y = v[j];
+      v[j] = times_sigmoid(y, y * fmaf(1.5957691216057308f * 0.044715f * y, y, 1.5957691216057308f));
+    }
+  } else if (act == NPUB200_ACT_QUICK_GELU) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = times_sigmoid(v[j], 1.702f * v[j]);
+  } else if (act == NPUB200_ACT_SILU) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = times_sigmoid(v[j], v[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = v[j] < 0.0f ? 0.0f : v[j];  // a NaN stays one
+  }
 }
 
 __device__ __forceinline__ void tile_coords(const GemmArgs& a, int tile, int& m_blk, int& n_blk) {
@@ -621,6 +655,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             else
               b = load_bias_own(args, gcol, j, own);
             v[j] += b;
+          }
+          if constexpr (MODE == kModeAct) activate(args.act, v);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
             if (args.residual != nullptr && gcol + j < args.N)
               v[j] += __bfloat162float(static_cast<const __nv_bfloat16*>(args.residual)[(long long)grow * args.ldr +
                                                                                           gcol + j]);
@@ -717,6 +755,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
               fetch_bias(b, c, n0 + c);
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[j] += b[j];
+              if constexpr (MODE == kModeAct) activate(args.act, v);
               if (args.residual != nullptr) add_residual32(args, m0 + row, n0 + c, v);
             }
             if (chunk_tma) {
@@ -1023,6 +1062,7 @@ int gemm_launch(const GemmProblem& p, cudaStream_t stream) {
   const bool geglu = p.geglu != 0;
   if (p.variant && !gemm_variant_known(p.variant, geglu))
     return fail(kErrUnsupported, "no GEMM%s variant %d", geglu ? " (GEGLU)" : "", p.variant);
+  if (geglu && p.act) return fail(kErrInvalid, "the GEGLU form has its own activation");
   if (geglu && p.w_map_cache != nullptr) return fail(kErrInvalid, "the GEGLU form encodes its own weight map");
   GemmPlan plan = gemm_plan(p.M, geglu ? 2 * p.N : p.N, p.K, dev->sms, p.variant, geglu);
   const int bn = plan.bn;
@@ -1065,6 +1105,7 @@ int gemm_launch(const GemmProblem& p, cudaStream_t stream) {
   a.bias_n = int(geglu ? 2 * p.N : p.N);
   a.residual = geglu ? nullptr : p.residual;
   a.ldr = p.ldr;
+  a.act = p.act;
   a.out = p.out;
   a.ldo = p.ldo;
   a.out_f32 = p.out_f32;
@@ -1084,6 +1125,12 @@ int gemm_launch(const GemmProblem& p, cudaStream_t stream) {
         case 192: return launch_variant<192, 6, kModeGeglu, true>(mx, mw, mo, a, units, sms, stream, d);
         case 256: return launch_variant<256, 6, kModeGeglu, true>(mx, mw, mo, a, units, sms, stream, d);
       }
+    } else if (p.act) {
+      switch (bn) {
+        case 128: return launch_variant<128, 8, kModeAct, true>(mx, mw, mo, a, units, sms, stream, d);
+        case 192: return launch_variant<192, 6, kModeAct, true>(mx, mw, mo, a, units, sms, stream, d);
+        case 256: return launch_variant<256, 6, kModeAct, true>(mx, mw, mo, a, units, sms, stream, d);
+      }
     } else {
       switch (bn) {
         case 128: return launch_variant<128, 8, kModePlain, true>(mx, mw, mo, a, units, sms, stream, d);
@@ -1101,6 +1148,17 @@ int gemm_launch(const GemmProblem& p, cudaStream_t stream) {
       case 256: return launch_variant<256, 4, kModeGeglu>(mx, mw, mo, a, units, sms, stream, d);
     }
     return fail(kErrUnsupported, "no GEGLU GEMM variant with an N tile of %d", bn);
+  }
+  if (p.act) {
+    switch (bn) {
+      case 64: return launch_variant<64, 8, kModeAct>(mx, mw, mo, a, units, sms, stream, d);
+      case 96: return launch_variant<96, 6, kModeAct>(mx, mw, mo, a, units, sms, stream, d);
+      case 128: return launch_variant<128, 6, kModeAct>(mx, mw, mo, a, units, sms, stream, d);
+      case 160: return launch_variant<160, 5, kModeAct>(mx, mw, mo, a, units, sms, stream, d);
+      case 192: return launch_variant<192, 4, kModeAct>(mx, mw, mo, a, units, sms, stream, d);
+      case 256: return launch_variant<256, 4, kModeAct>(mx, mw, mo, a, units, sms, stream, d);
+    }
+    return fail(kErrUnsupported, "no activation GEMM variant with an N tile of %d", bn);
   }
   switch (bn) {
     case 64: return launch_variant<64, 8>(mx, mw, mo, a, units, sms, stream, d);

@@ -81,6 +81,7 @@ struct GemmProblem {
   int geglu;  // 1: W has 2N rows [a; gate] and out[:, j] = (x.W[j] + b[j]) * gelu(x.W[N+j] + b[N+j]); bias has 2N
   const void* residual;  // bf16 [M, N] added after the bias (row stride ldr), or null
   int64_t ldr;
+  int act;  // activation between the bias and the residual (NPUB200_ACT_*; 0 = none, not with geglu)
 };
 // Launch plan for a problem: the N tile and the split-K factor (what `variant == 0` resolves to).
 struct GemmPlan {
@@ -110,7 +111,7 @@ size_t gemm_workspace_bytes(const void* x, int64_t ldx, int64_t m, int64_t k, co
 int gemm_with_workspace(const void* x, int64_t ldx, int64_t m, int64_t k, const void* w, int64_t ldw, int64_t n,
                         const CUtensorMap* w_map, const void* bias, int bias_dtype, void* out, int64_t ldo,
                         int out_dtype, void* workspace, size_t workspace_bytes, int variant, void* stream,
-                        int geglu = 0, const void* residual = nullptr, int64_t ldr = 0);
+                        int geglu = 0, const void* residual = nullptr, int64_t ldr = 0, int act = 0);
 int gemm_launch(const GemmProblem& p, cudaStream_t stream);
 
 // 3x3 convolution, stride 1, zero padding 1, as an implicit GEMM on the GEMM kernel (its convolution form).

@@ -44,11 +44,11 @@ void check_operand(const at::Tensor& t, const at::Tensor& ref, const char* name)
 
 void* stream_of(const at::Tensor& t) { return at::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 
-// out[M, N] = x[M, K] . w[N, K]^T (+ bias) (+ residual); bf16 operands, f32 accumulation, bias in f32.
+// out[M, N] = act(x[M, K] . w[N, K]^T (+ bias)) (+ residual), act an NPUB200_ACT_* code or 0 for none; bf16 operands, f32 accumulation, bias in f32.
 // Replaces NpuGemm.matmul_t (npu/xdna1_gemm.py:349-422) / NpuProgram.submit_gemm (npu/xdna1_program.py:451-454).
 at::Tensor gemm(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias,
                 const std::optional<at::Tensor>& out, int64_t variant, std::optional<at::ScalarType> out_dtype,
-                int64_t weight_handle, const std::optional<at::Tensor>& residual) {
+                int64_t weight_handle, const std::optional<at::Tensor>& residual, int64_t activation) {
   check_operand(x, x, "x");
   check_operand(w, x, "w");
   TORCH_CHECK_VALUE(x.dim() == 2 && w.dim() == 2, "gemm takes 2-D x [M, K] and w [N, K]");
@@ -75,19 +75,32 @@ at::Tensor gemm(const at::Tensor& x, const at::Tensor& w, const std::optional<at
     b_ptr = b.data_ptr();
   }
   void* st = stream_of(x);
-  if (residual.has_value()) {
-    const at::Tensor& r = *residual;
-    check_operand(r, x, "residual");
-    TORCH_CHECK_VALUE(r.dim() == 2 && r.size(0) == M && r.size(1) == N, "residual must be [M, N]");
+  if (residual.has_value() || activation != 0) {
+    const void* r_ptr = nullptr;
+    int64_t ldr = 0;
+    if (residual.has_value()) {
+      const at::Tensor& r = *residual;
+      check_operand(r, x, "residual");
+      TORCH_CHECK_VALUE(r.dim() == 2 && r.size(0) == M && r.size(1) == N, "residual must be [M, N]");
+      r_ptr = r.data_ptr();
+      ldr = r.stride(0);
+    }
     size_t ws_bytes = 0;
     check_rc(npub200_gemm_workspace_size(x.data_ptr(), x.stride(0), M, K, w.data_ptr(), w.stride(0), N,
                                          int(variant), &ws_bytes),
              "npub200::gemm");
     at::Tensor ws = at::empty({int64_t(ws_bytes)}, x.options().dtype(at::kByte));
-    check_rc(npub200_gemm_residual(x.data_ptr(), x.stride(0), M, K, w.data_ptr(), w.stride(0), N, b_ptr, b_code,
-                                   r.data_ptr(), r.stride(0), y.data_ptr(), y.stride(0), out_code,
-                                   ws_bytes ? ws.data_ptr() : nullptr, ws_bytes, int(variant), st),
-             "npub200::gemm");
+    void* ws_ptr = ws_bytes ? ws.data_ptr() : nullptr;
+    if (activation != 0)
+      check_rc(npub200_gemm_act(x.data_ptr(), x.stride(0), M, K, w.data_ptr(), w.stride(0), N, b_ptr, b_code,
+                                int(activation), r_ptr, ldr, y.data_ptr(), y.stride(0), out_code, ws_ptr, ws_bytes,
+                                int(variant), st),
+               "npub200::gemm");
+    else
+      check_rc(npub200_gemm_residual(x.data_ptr(), x.stride(0), M, K, w.data_ptr(), w.stride(0), N, b_ptr, b_code,
+                                     r_ptr, ldr, y.data_ptr(), y.stride(0), out_code, ws_ptr, ws_bytes, int(variant),
+                                     st),
+               "npub200::gemm");
     return y;
   }
   size_t ws_bytes = 0;
@@ -175,7 +188,7 @@ at::Tensor attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor&
 
 TORCH_LIBRARY(npub200, m) {
   m.def("gemm(Tensor x, Tensor w, Tensor? bias=None, Tensor? out=None, int variant=0, ScalarType? out_dtype=None, "
-        "int weight_handle=0, Tensor? residual=None) -> Tensor");
+        "int weight_handle=0, Tensor? residual=None, int activation=0) -> Tensor");
   m.def("attention(Tensor q, Tensor k, Tensor v, Tensor? out, int B, int H, int Sq, int Skv, int d, "
         "int q_row_stride, int kv_row_stride, int o_row_stride, bool head_major_in, bool head_major_out, "
         "float scale, int variant, ScalarType? out_dtype=None) -> Tensor");

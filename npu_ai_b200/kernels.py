@@ -94,9 +94,11 @@ def reset_workspaces() -> None:
 
 def gemm(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, out: torch.Tensor | None = None,
          out_dtype: torch.dtype = torch.float32, variant: int = 0, handle: int | None = None,
-         residual: torch.Tensor | None = None) -> torch.Tensor:
-    """out[M, N] = x[M, K] @ w[N, K]^T (+ bias) (+ residual) with bf16 operands and f32 accumulation.
+         residual: torch.Tensor | None = None, activation: str | None = None) -> torch.Tensor:
+    """out[M, N] = act(x[M, K] @ w[N, K]^T (+ bias)) (+ residual) with bf16 operands and f32 accumulation.
 
+    `activation` (None, "gelu" with the error function, "gelu_tanh", "quick_gelu", "silu" or "relu") is applied in
+    f32 in the kernel's epilogue, between the bias and the residual.
     x and w are bf16 CUDA matrices with a unit inner stride (any row stride); bias is bf16 or f32 [N]; residual a
     bf16 [M, N] matrix with unit inner stride (may be `out`). With `handle` (from register_weight for this very `w`)
     the cached weight descriptor is used.
@@ -122,9 +124,15 @@ def gemm(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, out
                 residual.stride(1) != 1:
             raise ValueError("residual must be a bf16 [M, N] matrix with contiguous rows")
         handle = None  # the residual entry point takes the weight itself
+    act = 0
+    if activation is not None:
+        act = _lib.ACTIVATIONS.get(activation, 0)
+        if not act:
+            raise ValueError(f"unknown activation {activation!r} (one of {', '.join(_lib.ACTIVATIONS)})")
+        handle = None  # and so does the activation's
     ops = _lib.torch_ops()
     if ops is not None:
-        return ops.gemm(x, w, bias, out, int(variant), None, int(handle or 0), residual)
+        return ops.gemm(x, w, bias, out, int(variant), None, int(handle or 0), residual, act)
     ws = _gemm_workspace(x, None if handle is not None else w, M, K, N, variant)
     args_tail = (ctypes.c_void_p(bias.data_ptr()) if bias is not None else None,
                  _DT[bias.dtype] if bias is not None else _lib.DTYPE_BF16,
@@ -132,7 +140,12 @@ def gemm(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, out
                  ctypes.c_void_p(ws.data_ptr()) if ws is not None else None, ws.numel() if ws is not None else 0,
                  int(variant), ctypes.c_void_p(_stream_ptr(x.device)))
     with torch.cuda.device(x.device):
-        if residual is not None:
+        if act:
+            _lib.call("npub200_gemm_act", ctypes.c_void_p(x.data_ptr()), x.stride(0), M, K,
+                      ctypes.c_void_p(w.data_ptr()), w.stride(0), N, args_tail[0], args_tail[1], act,
+                      ctypes.c_void_p(residual.data_ptr()) if residual is not None else None,
+                      residual.stride(0) if residual is not None else 0, *args_tail[2:])
+        elif residual is not None:
             _lib.call("npub200_gemm_residual", ctypes.c_void_p(x.data_ptr()), x.stride(0), M, K,
                       ctypes.c_void_p(w.data_ptr()), w.stride(0), N, args_tail[0], args_tail[1],
                       ctypes.c_void_p(residual.data_ptr()), residual.stride(0), *args_tail[2:])

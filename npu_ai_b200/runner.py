@@ -257,9 +257,10 @@ class NpuGemm:
         return b.contiguous()
 
     def matmul_t(self, x, w: NpuWeight, bias=None, out: torch.Tensor | None = None,
-                 out_dtype: torch.dtype | None = None, residual: torch.Tensor | None = None) -> torch.Tensor:
-        """x: (M, K) numpy/torch float -> (M, N) CUDA tensor = x @ W (+ bias); bf16 operands, f32 accumulation,
-        bias in f32 (npu/xdna1_gemm.py:349-422). f32 output unless `out_dtype`/`out` say otherwise."""
+                 out_dtype: torch.dtype | None = None, residual: torch.Tensor | None = None,
+                 activation: str | None = None) -> torch.Tensor:
+        """x: (M, K) numpy/torch float -> (M, N) CUDA tensor = act(x @ W (+ bias)); bf16 operands, f32 accumulation,
+        bias in f32 (npu/xdna1_gemm.py:349-422); `activation` as in kernels.gemm (None: none). f32 output unless `out_dtype`/`out` say otherwise."""
         t_start = time.perf_counter()
         x2 = self._x_device(x)
         if x2.dim() != 2:
@@ -268,7 +269,8 @@ class NpuGemm:
         assert K == w.K, f"K mismatch: x has {K}, weight has {w.K}"
         ev = self._events()
         y = kernels.gemm(x2, w.tensor[:, :K] if w.handle is None else w.tensor, self._bias_device(bias), out=out,
-                         out_dtype=out_dtype or self.out_dtype, handle=w.handle, residual=residual)
+                         out_dtype=out_dtype or self.out_dtype, handle=w.handle, residual=residual,
+                         activation=activation)
         self._close("gemm", ev)
         with self._lock:
             self.stats["calls"] += 1
@@ -282,15 +284,15 @@ class NpuGemm:
         return self.matmul_t(x, w, out_dtype=torch.float32).cpu().numpy()
 
     def linear(self, x, w: NpuWeight, bias=None, out_dtype: torch.dtype | None = None,
-               residual: torch.Tensor | None = None):
-        """x: (..., K) -> (..., N) = x @ W (+ bias) (+ residual, a bf16 (..., N) CUDA tensor added in the GEMM's
-        epilogue). torch in -> torch (CUDA) out, numpy in -> numpy out (npu/xdna1_gemm.py:428-448)."""
+               residual: torch.Tensor | None = None, activation: str | None = None):
+        """x: (..., K) -> (..., N) = act(x @ W (+ bias)) (+ residual, a bf16 (..., N) CUDA tensor); activation and
+        residual are applied in the GEMM's epilogue (`activation` as in kernels.gemm). torch in -> torch (CUDA) out, numpy in -> numpy out (npu/xdna1_gemm.py:428-448)."""
         is_torch = isinstance(x, torch.Tensor)
         xt = _as_tensor(x)
         shp = tuple(xt.shape)
         x2 = xt.reshape(-1, shp[-1])
         r2 = residual.reshape(-1, w.N) if residual is not None else None
-        y = self.matmul_t(x2, w, bias, out_dtype=out_dtype, residual=r2).view(*shp[:-1], w.N)
+        y = self.matmul_t(x2, w, bias, out_dtype=out_dtype, residual=r2, activation=activation).view(*shp[:-1], w.N)
         return y if is_torch else y.cpu().numpy()
 
     def linear_geglu(self, x, w: NpuWeight, bias=None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
