@@ -35,6 +35,7 @@ extern "C" {
 
 #define NPUB200_DTYPE_BF16 0
 #define NPUB200_DTYPE_F32 1
+#define NPUB200_DTYPE_BOOL 2 /* one byte per value, 0 or 1 (attention mask tensors only) */
 
 /* Activations of npub200_gemm_act. */
 #define NPUB200_ACT_GELU 1       /* y/2 (1 + erf(y / sqrt 2)) */
@@ -198,6 +199,54 @@ int npub200_attention(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, c
                       void* out, int64_t o_sb, int64_t o_ss, int64_t o_sh, int out_dtype, int64_t batch,
                       int64_t heads, int64_t sq, int64_t skv, int64_t head_dim, float scale, int variant,
                       void* stream);
+
+/* ----------------------------------------------------------------------------------------------------------
+ * Attention with masks, score modifiers and grouped key/value heads; the reference hands every such call to the CPU
+ * (its attention gate refuses masks and grouped heads, comfyui node :39-99). As npub200_attention, with
+ *   s_ij = scale q_i . k_j, then cap tanh(s / cap) when softcap > 0, then - slopes[h] |p_i - j| and
+ *          + distance_bias[h][clamp(j - p_i, -R, R) + R] and + mask_ij where given,
+ *   o_i  = sum_j softmax_j(s_ij) v_j over the keys j that row i may see; zeros for a row that sees none.
+ * p_i = q_start + i is query i's position among the keys. Row i may see key j of its sequence b when all of these hold:
+ *   j < kv_lens[b]; causal: j <= p_i or j < prefix; documents: i and j lie in the same document, document d of
+ *   sequence b being tokens [off[d], off[d + 1]) (tokens outside every document see nothing); a boolean mask is not 0.
+ * Keys that no row of the call may see under the lengths, causal and document rules are not read into the result,
+ * whatever they hold (NaN included); a key that some rows see and others do not has to be finite. An additive mask of
+ * -inf hides a key; a mask of the type's lowest finite value is a score like any other (a row with nothing else
+ * averages those keys). q: [batch, sq, heads, head_dim] strided as in npub200_attention, k and v with kv_heads heads:
+ * query head h reads key/value head h / (heads / kv_heads). All pointers are device memory; int32 values outside
+ * their range are clamped, never read past.
+ * variant: 0, or the number of parts that every row's keys are split into (1 ... 64). Few rows over many keys are
+ * split automatically; each part's partial result goes to `workspace` (npub200_attention_masked_workspace_size()
+ * bytes, 16-byte aligned, contents irrelevant) and a second kernel joins the parts in a fixed order. Calls that can run
+ * at the same time must not share a workspace. Deterministic; allocates nothing.
+ * ---------------------------------------------------------------------------------------------------------- */
+typedef struct npub200_attention_mods {
+  int32_t causal;                /* 1: row i sees keys up to its own position */
+  int32_t mask_dtype;            /* NPUB200_DTYPE_* of `mask` */
+  int64_t q_start;               /* position of query 0 among the keys */
+  const int32_t* q_starts;       /* [batch] positions instead of q_start, or NULL */
+  int64_t prefix;                /* causal only: keys below `prefix` are seen by every row */
+  const int32_t* prefixes;       /* [batch] prefixes instead of prefix, or NULL */
+  const int32_t* kv_lens;        /* [batch] valid keys of each sequence, or NULL (skv) */
+  const int32_t* doc_offsets;    /* [docs + 1] nondecreasing document borders (sq == skv only), or NULL */
+  int64_t docs;
+  int64_t doc_stride;            /* elements between the borders of consecutive sequences (0: shared by all) */
+  float softcap;                 /* > 0: cap of the scores; 0: none */
+  int32_t max_distance;          /* R: distance_bias has 2 R + 1 entries per head */
+  const float* slopes;           /* [heads], or NULL */
+  const float* distance_bias;    /* [heads][2 R + 1] dense, or NULL */
+  const void* mask;              /* bool (0 hides) or additive bf16/f32; element (b, h, i, j) at b*mask_sb + h*mask_sh +
+                                    i*mask_sq + j, strides >= 0 (0 broadcasts), or NULL */
+  int64_t mask_sb, mask_sh, mask_sq;
+} npub200_attention_mods;
+int npub200_attention_masked_workspace_size(int64_t batch, int64_t heads, int64_t kv_heads, int64_t sq, int64_t skv,
+                                            int64_t head_dim, int variant, size_t* bytes_out);
+int npub200_attention_masked(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, const void* k, int64_t k_sb,
+                             int64_t k_ss, int64_t k_sh, const void* v, int64_t v_sb, int64_t v_ss, int64_t v_sh,
+                             void* out, int64_t o_sb, int64_t o_ss, int64_t o_sh, int out_dtype, int64_t batch,
+                             int64_t heads, int64_t kv_heads, int64_t sq, int64_t skv, int64_t head_dim, float scale,
+                             const npub200_attention_mods* mods, void* workspace, size_t workspace_bytes, int variant,
+                             void* stream);
 
 /* ----------------------------------------------------------------------------------------------------------
  * Device status word (failure detection; the reference's RuntimeError from NpuProgram.wait,

@@ -16,11 +16,22 @@ LIB_PATH = os.path.join(HERE, "libnpub200.so")
 TORCH_OPS_PATH = os.path.join(HERE, "libnpub200_torch.so")
 
 OK, EINVAL, ECUDA, EUNSUPPORTED, EDEVICE = 0, -1, -2, -3, -4
-DTYPE_BF16, DTYPE_F32 = 0, 1
+DTYPE_BF16, DTYPE_F32, DTYPE_BOOL = 0, 1, 2
 ACTIVATIONS = {"gelu": 1, "gelu_tanh": 2, "quick_gelu": 3, "silu": 4, "relu": 5}  # NPUB200_ACT_*
 
 _c_i64 = ctypes.c_int64
 _c_p = ctypes.c_void_p
+
+
+class AttentionMods(ctypes.Structure):
+    """npub200_attention_mods (include/npu_b200.h)."""
+    _fields_ = [("causal", ctypes.c_int32), ("mask_dtype", ctypes.c_int32), ("q_start", _c_i64), ("q_starts", _c_p),
+                ("prefix", _c_i64), ("prefixes", _c_p), ("kv_lens", _c_p), ("doc_offsets", _c_p), ("docs", _c_i64),
+                ("doc_stride", _c_i64), ("softcap", ctypes.c_float), ("max_distance", ctypes.c_int32),
+                ("slopes", _c_p), ("distance_bias", _c_p), ("mask", _c_p), ("mask_sb", _c_i64), ("mask_sh", _c_i64),
+                ("mask_sq", _c_i64)]
+
+
 _SIGNATURES = {
     "npub200_version": (ctypes.c_int, []),
     "npub200_last_error": (ctypes.c_char_p, []),
@@ -61,6 +72,13 @@ _SIGNATURES = {
     "npub200_attention": (ctypes.c_int, [_c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_i64,
                                          _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_i64, ctypes.c_int, _c_i64, _c_i64,
                                          _c_i64, _c_i64, _c_i64, ctypes.c_float, ctypes.c_int, _c_p]),
+    "npub200_attention_masked_workspace_size": (ctypes.c_int, [_c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64,
+                                                               ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
+    "npub200_attention_masked": (ctypes.c_int, [_c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_i64,
+                                                _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_i64, ctypes.c_int, _c_i64,
+                                                _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_float,
+                                                ctypes.POINTER(AttentionMods), _c_p, ctypes.c_size_t, ctypes.c_int,
+                                                _c_p]),
     "npub200_status_read": (ctypes.c_int, [_c_p, ctypes.POINTER(ctypes.c_uint32), ctypes.c_int]),
     "npub200_set_wait_timeout_ns": (ctypes.c_int, [ctypes.c_uint64]),
     "npub200_set_debug_flags": (ctypes.c_int, [ctypes.c_uint32]),

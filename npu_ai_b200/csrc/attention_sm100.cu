@@ -37,13 +37,10 @@
 #include <cstdio>
 #include <cstring>
 
-#include "internal.h"
+#include "attention_sm100.cuh"
 
 namespace npub200 {
 
-constexpr int kAttnBM = 128;           // query rows per Q tile (one softmax warpgroup, one TMEM lane per row)
-constexpr int kSoftmaxWarps = 4;       // per Q tile
-constexpr int kAtomBytesPerRow = 128;  // one 128-byte swizzle atom row: 64 bf16
 // Of every 8 (key, key+1) pairs of a softmax row, this many take their exponentials from the FMA-pipe polynomial
 // (exp2_poly3_x2) instead of the MUFU. Measured: head dims up to 64 (the least MMA work per exponential) gain from
 // moving 2 of 8 to the FP32 pipe with one or two Q tiles per CTA; with four Q tiles per CTA the issue slots the
@@ -51,108 +48,6 @@ constexpr int kAtomBytesPerRow = 128;  // one 128-byte swizzle atom row: 64 bf16
 template <int DP, int QT>
 constexpr int exp_poly_pairs_per8() {
   return (DP <= 64 && QT <= 2) ? 2 : 0;
-}
-
-struct MapPos {
-  int s, h, b;  // position (1..3) of the seq / head / batch dimension in the tensor map
-};
-
-struct AttnArgs {
-  int Sq, Skv, H, nkv;
-  float scale_log2;     // scale * log2(e)
-  float rescale_thr;    // lazy-rescale threshold in log2 units
-  void* out;
-  long long o_sb, o_ss, o_sh;
-  int out_f32;
-  int D;                // true head dim (output columns)
-  MapPos pq, pk, pv;
-  KernelCtl ctl;
-};
-
-// Coordinates (dim, then the three outer dims in the map's order) of 64-column atom `atom` of row s of (b, h).
-__device__ __forceinline__ void map_coords(const MapPos& p, int atom, int s, int h, int b, int& c0, int& c1, int& c2,
-                                           int& c3) {
-  c0 = atom * 64;
-  c1 = p.s == 1 ? s : (p.h == 1 ? h : b);
-  c2 = p.s == 2 ? s : (p.h == 2 ? h : b);
-  c3 = p.s == 3 ? s : (p.h == 3 ? h : b);
-}
-
-// ---------------------------------------------------------------------------------------------------------------
-// Producer: K and V tiles of one (b, h) pair into STAGES-deep rings, K one tile ahead of V (K_j is needed a whole
-// softmax step before V_j). On an abort it waits for the loads it issued before returning, so shared memory is
-// not released under an in-flight copy.
-// ---------------------------------------------------------------------------------------------------------------
-template <int NA, int BN, int STAGES>
-__device__ __forceinline__ void kv_producer(const CUtensorMap* tm_k, const CUtensorMap* tm_v, const AttnArgs& args,
-                                            uint8_t* sK, uint8_t* sV, uint64_t* k_full, uint64_t* v_full,
-                                            uint64_t* k_empty, uint64_t* v_empty, volatile int* abort_flag, int hh,
-                                            int bb) {
-  constexpr int kAtom = BN * kAtomBytesPerRow;
-  constexpr int kTile = NA * kAtom;
-  const int nkv = args.nkv;
-  int issued_k = 0, issued_v = 0;
-  bool ok = true;
-  int c0, c1, c2, c3;
-  for (int j = 0; j <= nkv; ++j) {
-    if (j < nkv) {
-      const int st = j % STAGES;
-      if (!mbar_wait_bounded(&k_empty[st], (uint32_t(j / STAGES) & 1u) ^ 1u, abort_flag, args.ctl,
-                             kStatusTimeoutProducer)) {
-        ok = false;
-        break;
-      }
-      mbar_arrive_expect_tx(&k_full[st], kTile);
-      for (int a = 0; a < NA; ++a) {
-        map_coords(args.pk, a, j * BN, hh, bb, c0, c1, c2, c3);
-        tma_load_4d(tm_k, &k_full[st], sK + st * kTile + a * kAtom, c0, c1, c2, c3);
-      }
-      ++issued_k;
-    }
-    if (j >= 1) {
-      const int i = j - 1;
-      const int st = i % STAGES;
-      if (!mbar_wait_bounded(&v_empty[st], (uint32_t(i / STAGES) & 1u) ^ 1u, abort_flag, args.ctl,
-                             kStatusTimeoutProducer)) {
-        ok = false;
-        break;
-      }
-      mbar_arrive_expect_tx(&v_full[st], kTile);
-      for (int a = 0; a < NA; ++a) {
-        map_coords(args.pv, a, i * BN, hh, bb, c0, c1, c2, c3);
-        tma_load_4d(tm_v, &v_full[st], sV + st * kTile + a * kAtom, c0, c1, c2, c3);
-      }
-      ++issued_v;
-    }
-  }
-  if (!ok) {
-    for (int i = max(0, issued_k - STAGES); i < issued_k; ++i)
-      mbar_wait_drain(&k_full[i % STAGES], uint32_t(i / STAGES) & 1u, args.ctl);
-    for (int i = max(0, issued_v - STAGES); i < issued_v; ++i)
-      mbar_wait_drain(&v_full[i % STAGES], uint32_t(i / STAGES) & 1u, args.ctl);
-  }
-}
-
-// S = Q K_j^T for one Q tile: K-major over the head dim, atoms of 64 columns, +32 B per 16 columns in an atom.
-template <int DP, int BN>
-__device__ __forceinline__ void issue_s(uint32_t d_tmem, uint64_t q_desc, uint64_t k_desc, int q_atom_bytes,
-                                        int kv_atom_bytes) {
-  constexpr uint32_t kIdescS = idesc_bf16_f32(kAttnBM, BN, false);
-#pragma unroll
-  for (int kk = 0; kk < DP / 16; ++kk)
-    umma_f16_ss(d_tmem, q_desc + uint64_t(((kk >> 2) * q_atom_bytes + (kk & 3) * 32) >> 4),
-                k_desc + uint64_t(((kk >> 2) * kv_atom_bytes + (kk & 3) * 32) >> 4), kIdescS, kk > 0 ? 1u : 0u);
-}
-
-// O += P V_j: P from TMEM (16 keys = 8 columns of bf16 pairs per K step), V MN-major (head dim contiguous), 16 keys
-// = 16 rows of 128 B further per K step.
-template <int DP, int BN>
-__device__ __forceinline__ void issue_pv(uint32_t o_tmem, uint32_t p_tmem, uint64_t v_desc, bool accumulate) {
-  constexpr uint32_t kIdescO = idesc_bf16_f32(kAttnBM, DP, true);
-#pragma unroll
-  for (int kk = 0; kk < BN / 16; ++kk)
-    umma_f16_ts(o_tmem, p_tmem + uint32_t(kk * 8), v_desc + uint64_t((kk * 16 * kAtomBytesPerRow) >> 4), kIdescO,
-                (accumulate || kk > 0) ? 1u : 0u);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -229,80 +124,6 @@ __device__ __forceinline__ float softmax_step(uint32_t s_addr, int kv0, int Skv,
   l = l * alpha + (r0 + r1);
   m = m_new;
   return alpha;
-}
-
-// O row *= alpha (TMEM columns from o_addr). Warp-wide: lanes whose max did not move pass alpha = 1.
-template <int DP>
-__device__ __forceinline__ void rescale_o_row(uint32_t o_addr, float alpha) {
-#pragma unroll
-  for (int cc = 0; cc < DP; cc += 16) {
-    uint32_t r[16];
-    tmem_ld16(o_addr + uint32_t(cc), r);
-    tmem_wait_ld();
-#pragma unroll
-    for (int t = 0; t < 16; ++t) r[t] = __float_as_uint(__uint_as_float(r[t]) * alpha);
-    tmem_st16(o_addr + uint32_t(cc), r);
-  }
-  tmem_wait_st();
-}
-
-// Normalised O row (TMEM columns from o_addr) to the output: the first D columns of row `grow` of pair (bb, hh),
-// bf16 or f32, 16-byte vector stores where aligned. Rows past Sq only drain TMEM (tcgen05.ld is warp-wide).
-template <int DP>
-__device__ __forceinline__ void store_o_row(uint32_t o_addr, const AttnArgs& args, int grow, int bb, int hh,
-                                            float inv_l) {
-  const bool store = grow < args.Sq;
-  const long long obase = (long long)bb * args.o_sb + (long long)grow * args.o_ss + (long long)hh * args.o_sh;
-#pragma unroll
-  for (int cc = 0; cc < DP; cc += 16) {
-    uint32_t r[16];
-    tmem_ld16(o_addr + uint32_t(cc), r);
-    tmem_wait_ld();
-    if (store) {
-      float o[16];
-#pragma unroll
-      for (int t = 0; t < 16; ++t) o[t] = __uint_as_float(r[t]) * inv_l;
-      const int ncols = min(16, args.D - cc);
-      if (args.out_f32) {
-        float* dst = static_cast<float*>(args.out) + obase + cc;
-        if (ncols == 16 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-            reinterpret_cast<float4*>(dst)[t] = make_float4(o[4 * t], o[4 * t + 1], o[4 * t + 2], o[4 * t + 3]);
-        } else {
-#pragma unroll
-          for (int t = 0; t < 16; ++t)
-            if (t < ncols) dst[t] = o[t];
-        }
-      } else {
-        __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(args.out) + obase + cc;
-        if (ncols >= 8 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
-          uint4 v0;
-          v0.x = pack_bf16x2(o[0], o[1]);
-          v0.y = pack_bf16x2(o[2], o[3]);
-          v0.z = pack_bf16x2(o[4], o[5]);
-          v0.w = pack_bf16x2(o[6], o[7]);
-          reinterpret_cast<uint4*>(dst)[0] = v0;
-          if (ncols == 16) {
-            uint4 v1;
-            v1.x = pack_bf16x2(o[8], o[9]);
-            v1.y = pack_bf16x2(o[10], o[11]);
-            v1.z = pack_bf16x2(o[12], o[13]);
-            v1.w = pack_bf16x2(o[14], o[15]);
-            reinterpret_cast<uint4*>(dst)[1] = v1;
-          } else {
-#pragma unroll
-            for (int t = 8; t < 16; ++t)
-              if (t < ncols) dst[t] = __float2bfloat16_rn(o[t]);
-          }
-        } else {
-#pragma unroll
-          for (int t = 0; t < 16; ++t)
-            if (t < ncols) dst[t] = __float2bfloat16_rn(o[t]);
-        }
-      }
-    }
-  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -409,7 +230,7 @@ __global__ void __launch_bounds__(kAttn1Threads, Attn1Layout<DP, BN, STAGES>::kT
         tma_load_4d(&tm_q, q_full, sQ + a * L::kQAtom, c0, c1, c2, c3);
       }
       kv_producer<L::kNA, BN, STAGES>(&tm_k, &tm_v, args, sK, sV, k_full, v_full, k_empty, v_empty, abort_flag, hh,
-                                      bb);
+                                      bb, nkv);
       mbar_wait_drain(q_full, 0, args.ctl);
     }
   } else if (warp == 5) {
@@ -659,7 +480,7 @@ __global__ void __launch_bounds__(attn_mq_threads<QT>(), 1)
           tma_load_4d(&tm_q, q_full, sQ + w * L::kQBytes + a * L::kQAtom, c0, c1, c2, c3);
         }
       kv_producer<L::kNA, BN, STAGES>(&tm_k, &tm_v, args, sK, sV, k_full, v_full, k_empty, v_empty, abort_flag, hh,
-                                      bb);
+                                      bb, nkv);
       mbar_wait_drain(q_full, 0, args.ctl);
     }
   } else if (warp == kSWarp || warp == kPvWarp) {
@@ -794,10 +615,12 @@ struct DimStride {
   int which;       // 0 = seq, 1 = head, 2 = batch
 };
 
+}  // namespace
+
 // 4-D map (dim, then seq/head/batch sorted by stride) with a box of 64 dim-elements (one 128-byte swizzle atom) x
-// `rows` sequence rows. The dim extent is the true head dim: the columns of the atom past it read as zeros.
+// `rows` sequence rows x `heads` heads. The dim extent is the true head dim: the columns of the atom past it read as zeros.
 int encode_bshd_map(const void* base, int64_t D, int64_t S, int64_t H, int64_t B, int64_t ss, int64_t sh, int64_t sb,
-                    int rows, CUtensorMap* out, MapPos* pos) {
+                    int rows, CUtensorMap* out, MapPos* pos, int heads) {
   EncodeTiledFn enc = nullptr;
   if (int rc = encode_tiled_fn(&enc)) return rc;
   DimStride d[3] = {{S, ss, 0}, {H, sh, 1}, {B, sb, 2}};
@@ -820,6 +643,7 @@ int encode_bshd_map(const void* base, int64_t D, int64_t S, int64_t H, int64_t B
       box[i + 1] = cuuint32_t(rows);
       pos->s = i + 1;
     } else if (d[i].which == 1) {
+      box[i + 1] = cuuint32_t(heads);
       pos->h = i + 1;
     } else {
       pos->b = i + 1;
@@ -833,6 +657,8 @@ int encode_bshd_map(const void* base, int64_t D, int64_t S, int64_t H, int64_t B
                 int(r), (long long)D, (long long)S, (long long)H, (long long)B);
   return kOk;
 }
+
+namespace {
 
 template <typename Kern>
 int launch_kernel(Kern kern, int smem_bytes, int threads, bool* configured, const CUtensorMap& mq,

@@ -498,6 +498,32 @@ int npub200_attention(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, c
   return attention_launch(p, static_cast<cudaStream_t>(stream));
 }
 
+int npub200_attention_masked_workspace_size(int64_t batch, int64_t heads, int64_t kv_heads, int64_t sq, int64_t skv,
+                                            int64_t head_dim, int variant, size_t* bytes_out) {
+  if (bytes_out == nullptr) return fail(kErrInvalid, "null output pointer");
+  return attention_masked_workspace(batch, heads, kv_heads, sq, skv, head_dim, variant, bytes_out);
+}
+
+int npub200_attention_masked(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, const void* k, int64_t k_sb,
+                             int64_t k_ss, int64_t k_sh, const void* v, int64_t v_sb, int64_t v_ss, int64_t v_sh,
+                             void* out, int64_t o_sb, int64_t o_ss, int64_t o_sh, int out_dtype, int64_t batch,
+                             int64_t heads, int64_t kv_heads, int64_t sq, int64_t skv, int64_t head_dim, float scale,
+                             const npub200_attention_mods* mods, void* workspace, size_t workspace_bytes, int variant,
+                             void* stream) {
+  AttnMaskedProblem p;
+  memset(&p, 0, sizeof(p));
+  p.base = AttnProblem{q,    k,    v,    out,  q_sb, q_ss, q_sh, k_sb,  k_ss, k_sh, v_sb,     v_ss,  v_sh,
+                       o_sb, o_ss, o_sh, batch, heads, sq, skv, head_dim, scale, out_dtype == NPUB200_DTYPE_F32, variant,
+                       g_debug_flags.load()};
+  if (out_dtype != NPUB200_DTYPE_BF16 && out_dtype != NPUB200_DTYPE_F32)
+    return fail(kErrInvalid, "unknown output dtype code %d", out_dtype);
+  p.kv_heads = kv_heads;
+  p.mods = mods;
+  p.workspace = workspace;
+  p.workspace_bytes = workspace_bytes;
+  return attention_masked_launch(p, static_cast<cudaStream_t>(stream));
+}
+
 int npub200_status_read(void* stream, uint32_t* bits_out, int clear) {
   const DeviceInfo* d = nullptr;
   if (int rc = current_device_info(&d)) return rc;

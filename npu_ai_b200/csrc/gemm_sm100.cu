@@ -30,7 +30,6 @@
 #include <mutex>
 
 #include "internal.h"
-#include "npu_b200.h"
 
 namespace npub200 {
 

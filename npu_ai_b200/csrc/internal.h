@@ -8,6 +8,7 @@
 #include <string>
 #include <utility>
 
+#include "npu_b200.h"
 #include "sm100_ptx.cuh"
 
 namespace npub200 {
@@ -176,5 +177,18 @@ struct AttnProblem {
   uint32_t debug;
 };
 int attention_launch(const AttnProblem& p, cudaStream_t stream);
+
+// Masked attention (attention_masked.cu): AttnProblem plus grouped key/value heads and the score modifiers.
+struct AttnMaskedProblem {
+  AttnProblem base;  // variant: number of key splits (0 = automatic)
+  int64_t kv_heads;
+  const npub200_attention_mods* mods;  // null: none
+  void* workspace;
+  size_t workspace_bytes;
+};
+int attention_masked_launch(const AttnMaskedProblem& p, cudaStream_t stream);
+// Bytes of workspace the launch needs (partial results of split keys), 0 when the keys are not split.
+int attention_masked_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t sq, int64_t skv,
+                               int64_t head_dim, int variant, size_t* bytes);
 
 }  // namespace npub200

@@ -14,6 +14,7 @@
 
 #include <cmath>
 #include <optional>
+#include <type_traits>
 
 #include "npu_b200.h"
 
@@ -184,6 +185,97 @@ at::Tensor attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor&
   return o;
 }
 
+// A device vector of n values of a masked attention (lengths, positions, slopes): its pointer, or null when absent.
+template <typename T>
+const T* vector_ptr(const std::optional<at::Tensor>& t, const at::Tensor& q, int64_t n, const char* name) {
+  if (!t.has_value()) return nullptr;
+  const at::ScalarType want = std::is_same_v<T, float> ? at::kFloat : at::kInt;
+  TORCH_CHECK_VALUE(t->is_cuda() && t->device() == q.device() && t->scalar_type() == want && t->dim() == 1 &&
+                        t->size(0) == n && t->is_contiguous(),
+                    name, " must be a contiguous ", want, " vector of ", n, " values on ", q.device());
+  return static_cast<const T*>(t->data_ptr());
+}
+
+// Attention with masks, score modifiers and grouped key/value heads (npub200_attention_masked) into `out`: (B, S, H*d)
+// tensors, or (B, H, S, d) when head-major. The workspace of split keys comes from torch's allocator, one per call.
+at::Tensor attention_masked(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& out,
+                            int64_t heads, int64_t kv_heads, bool head_major_in, bool head_major_out, double scale,
+                            int64_t variant, bool causal, int64_t q_start, const std::optional<at::Tensor>& q_starts,
+                            int64_t prefix, const std::optional<at::Tensor>& prefixes,
+                            const std::optional<at::Tensor>& kv_lens, const std::optional<at::Tensor>& doc_offsets,
+                            double softcap, const std::optional<at::Tensor>& slopes,
+                            const std::optional<at::Tensor>& distance_bias, const std::optional<at::Tensor>& mask) {
+  check_operand(q, q, "q");
+  check_operand(k, q, "k");
+  check_operand(v, q, "v");
+  TORCH_CHECK_VALUE(heads > 0 && kv_heads > 0, "head counts must be positive");
+  TORCH_CHECK_VALUE(q.dim() == (head_major_in ? 4 : 3) && k.dim() == q.dim(), "attention operands have the wrong rank");
+  TORCH_CHECK_VALUE(head_major_in || q.size(2) % heads == 0, "q's last dimension is not a multiple of heads");
+  const int64_t B = q.size(0), Sq = q.size(head_major_in ? 2 : 1), Skv = k.size(head_major_in ? 2 : 1);
+  const int64_t d = head_major_in ? q.size(3) : q.size(2) / heads;
+  check_layout(q, head_major_in, B, heads, Sq, d, 0, "q");
+  check_layout(k, head_major_in, B, kv_heads, Skv, d, 0, "k");
+  check_layout(v, head_major_in, B, kv_heads, Skv, d, 0, "v");
+  check_layout(out, head_major_out, B, heads, Sq, d, 0, "out");
+  TORCH_CHECK_VALUE(out.is_cuda() && out.device() == q.device() && out.stride(-1) == 1,
+                    "out must be a CUDA tensor on q's device with a contiguous last dimension");
+  npub200_attention_mods m = {};
+  m.causal = causal ? 1 : 0;
+  m.q_start = q_start;
+  m.q_starts = vector_ptr<int32_t>(q_starts, q, B, "q_starts");
+  m.prefix = prefix;
+  m.prefixes = vector_ptr<int32_t>(prefixes, q, B, "prefixes");
+  m.kv_lens = vector_ptr<int32_t>(kv_lens, q, B, "kv_lens");
+  m.softcap = float(softcap);
+  m.slopes = vector_ptr<float>(slopes, q, heads, "slopes");
+  if (doc_offsets.has_value()) {
+    const at::Tensor& t = *doc_offsets;
+    TORCH_CHECK_VALUE(t.is_cuda() && t.device() == q.device() && t.scalar_type() == at::kInt && t.is_contiguous() &&
+                          (t.dim() == 1 || (t.dim() == 2 && t.size(0) == B)) && t.size(-1) >= 1,
+                      "doc_offsets must be a contiguous int32 [n + 1] or [B, n + 1] tensor on q's device");
+    m.doc_offsets = static_cast<const int32_t*>(t.data_ptr());
+    m.docs = t.size(-1) - 1;
+    m.doc_stride = t.dim() == 2 ? t.size(1) : 0;
+  }
+  if (distance_bias.has_value()) {
+    const at::Tensor& t = *distance_bias;
+    TORCH_CHECK_VALUE(t.is_cuda() && t.device() == q.device() && t.scalar_type() == at::kFloat && t.is_contiguous() &&
+                          t.dim() == 2 && t.size(0) == heads && t.size(1) % 2 == 1 && t.size(1) <= (1 << 25),
+                      "distance_bias must be a contiguous f32 [heads, 2R + 1] tensor on q's device");
+    m.distance_bias = static_cast<const float*>(t.data_ptr());
+    m.max_distance = int32_t(t.size(1) / 2);
+  }
+  if (mask.has_value()) {
+    const at::Tensor& t = *mask;
+    TORCH_CHECK_VALUE(t.is_cuda() && t.device() == q.device() && t.dim() == 4 && (t.size(0) == 1 || t.size(0) == B) &&
+                          (t.size(1) == 1 || t.size(1) == heads) && (t.size(2) == 1 || t.size(2) == Sq) &&
+                          t.size(3) == Skv && (Skv == 1 || t.stride(3) == 1),
+                      "mask must be a 4-D tensor on q's device that broadcasts to (B, heads, Sq, Skv), keys contiguous");
+    m.mask = t.data_ptr();
+    m.mask_dtype = t.scalar_type() == at::kBool ? NPUB200_DTYPE_BOOL : dtype_code(t, "mask");
+    m.mask_sb = t.size(0) > 1 ? t.stride(0) : 0;
+    m.mask_sh = t.size(1) > 1 ? t.stride(1) : 0;
+    m.mask_sq = t.size(2) > 1 ? t.stride(2) : 0;
+  }
+  const c10::cuda::CUDAGuard guard(q.device());
+  size_t ws_bytes = 0;
+  check_rc(npub200_attention_masked_workspace_size(B, heads, kv_heads, Sq, Skv, d, int(variant), &ws_bytes),
+           "npub200::attention_masked");
+  at::Tensor ws;
+  if (ws_bytes) ws = at::empty({int64_t(ws_bytes)}, q.options().dtype(at::kByte));
+  int64_t qs[3], ks[3], vs[3], os[3];
+  bsh_strides(q, head_major_in, d, &qs[0], &qs[1], &qs[2]);
+  bsh_strides(k, head_major_in, d, &ks[0], &ks[1], &ks[2]);
+  bsh_strides(v, head_major_in, d, &vs[0], &vs[1], &vs[2]);
+  bsh_strides(out, head_major_out, d, &os[0], &os[1], &os[2]);
+  check_rc(npub200_attention_masked(q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(),
+                                    vs[0], vs[1], vs[2], out.data_ptr(), os[0], os[1], os[2], dtype_code(out, "out"), B,
+                                    heads, kv_heads, Sq, Skv, d, float(scale), &m, ws_bytes ? ws.data_ptr() : nullptr,
+                                    ws_bytes, int(variant), stream_of(q)),
+           "npub200::attention_masked");
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(npub200, m) {
@@ -192,9 +284,14 @@ TORCH_LIBRARY(npub200, m) {
   m.def("attention(Tensor q, Tensor k, Tensor v, Tensor? out, int B, int H, int Sq, int Skv, int d, "
         "int q_row_stride, int kv_row_stride, int o_row_stride, bool head_major_in, bool head_major_out, "
         "float scale, int variant, ScalarType? out_dtype=None) -> Tensor");
+  m.def("attention_masked(Tensor q, Tensor k, Tensor v, Tensor(a!) out, int heads, int kv_heads, bool head_major_in, "
+        "bool head_major_out, float scale, int variant, bool causal, int q_start, Tensor? q_starts, int prefix, "
+        "Tensor? prefixes, Tensor? kv_lens, Tensor? doc_offsets, float softcap, Tensor? slopes, Tensor? distance_bias, "
+        "Tensor? mask) -> Tensor(a!)");
 }
 
 TORCH_LIBRARY_IMPL(npub200, CUDA, m) {
   m.impl("gemm", &gemm);
   m.impl("attention", &attention);
+  m.impl("attention_masked", &attention_masked);
 }

@@ -376,14 +376,39 @@ def _bshd_strides(t: torch.Tensor, head_major: bool) -> tuple[int, int, int]:
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, scale: float | None = None,
               head_major_in: bool = False, head_major_out: bool = False, out_dtype: torch.dtype = torch.float32,
-              out: torch.Tensor | None = None, variant: int = 0) -> torch.Tensor:
+              out: torch.Tensor | None = None, variant: int = 0, *, kv_heads: int | None = None, causal: bool = False,
+              q_start: int | torch.Tensor | None = None, prefix_len: int | torch.Tensor | None = None,
+              kv_lens: torch.Tensor | None = None, doc_offsets: torch.Tensor | None = None,
+              softcap: float | None = None, slopes: torch.Tensor | None = None,
+              distance_bias: torch.Tensor | None = None, mask: torch.Tensor | None = None) -> torch.Tensor:
     """softmax(q k^T * scale) v for every (batch, head) pair in one launch.
 
     q/k/v: bf16 CUDA tensors, (B, S, H*D) or (B, H, S, D) when head_major_in; the output (B, Sq, H*D) or
     (B, H, Sq, D) when head_major_out. Strides may be padded (views), the last dimension must be contiguous.
     variant: key tile (0 = automatic, 64, 96, 128) + 1000 x query tiles of 128 rows per CTA (0 = automatic, 1, 2,
     or 4 with 64-key tiles for head dims up to 64); e.g. 2128 = two query tiles with 128-key tiles.
+
+    The keyword arguments select masked attention; a row that may see no key is zero. Query i of sequence b has the
+    position p = q_start + i among the keys (default Skv - Sq + i: the last query meets the last key; an int, or int32
+    [B]). Device tensors are read when the call runs, so a captured graph follows their contents.
+    kv_heads:      k and v hold this many heads, a divisor of `heads` (default: what k's shape says); query head h reads
+                   head h // (heads // kv_heads).
+    causal:        query p sees keys j <= p; with prefix_len (an int, or int32 [B]) also every key j < prefix_len.
+    kv_lens:       int32 [B], the valid keys of each sequence; what lies behind them is never used.
+    doc_offsets:   int32 [n + 1] or [B, n + 1], nondecreasing borders of packed documents (Sq == Skv): a token sees its
+                   own document only; tokens outside every document see nothing.
+    softcap:       scores become softcap * tanh(score / softcap).
+    slopes:        f32 [heads], adds -slopes[h] * |p - j|.
+    distance_bias: f32 [heads, 2R + 1], adds distance_bias[h, clamp(j - p, -R, R) + R].
+    mask:          bool (False hides) or additive bf16/f32, [Sq, Skv] or 4-D broadcastable to [B, heads, Sq, Skv], with
+                   contiguous keys. A key has to be finite unless kv_lens, causal or doc_offsets hide it from every row.
+    variant is then the number of parts each row's keys are split into (0 = automatic).
     """
+    if (causal or kv_lens is not None or mask is not None or doc_offsets is not None or softcap is not None
+            or slopes is not None or distance_bias is not None or prefix_len is not None
+            or (kv_heads is not None and int(kv_heads) != (q.shape[1] if head_major_in else int(heads)))):
+        return _attention_masked(q, k, v, heads, scale, head_major_in, head_major_out, out_dtype, out, variant, kv_heads,
+                                 causal, q_start, prefix_len, kv_lens, doc_offsets, softcap, slopes, distance_bias, mask)
     for name, t in (("q", q), ("k", k), ("v", v)):
         _require_cuda(t, name)
         if t.dtype != torch.bfloat16:
@@ -423,6 +448,126 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, sca
                   ctypes.c_void_p(q.data_ptr()), *qs, ctypes.c_void_p(k.data_ptr()), *ks,
                   ctypes.c_void_p(v.data_ptr()), *vs, ctypes.c_void_p(out.data_ptr()), *os_, _DT[out.dtype],
                   B, H, Sq, Skv, D, ctypes.c_float(scale), int(variant), ctypes.c_void_p(_stream_ptr(q.device)))
+    return out
+
+
+def _per_batch(t, name: str, B: int, device: torch.device, dtype: torch.dtype = torch.int32):
+    """Checks a [B] (or [heads]) device vector given for a masked attention."""
+    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != B or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of {B} values on {device} "
+                         f"(got {t.dtype} {tuple(t.shape)} on {t.device})")
+    return t
+
+
+def _attention_masked(q, k, v, heads, scale, head_major_in, head_major_out, out_dtype, out, variant, kv_heads, causal,
+                      q_start, prefix_len, kv_lens, doc_offsets, softcap, slopes, distance_bias, mask):
+    dims = 4 if head_major_in else 3
+    dev = q.device
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _require_cuda(t, name)
+        if t.dtype != torch.bfloat16:
+            raise ValueError(f"attention {name} must be bf16")
+        if t.dim() != dims or t.stride(-1) != 1 or t.device != dev:
+            raise ValueError(f"attention {name} must be {'(B, H, S, D)' if head_major_in else '(B, S, H*D)'} with a "
+                             f"contiguous last dimension on {dev}")
+    H = int(heads)
+    if head_major_in:
+        B, Hq, Sq, D = q.shape
+        if Hq != H:
+            raise ValueError(f"q has {Hq} heads, not {H}")
+        Hk, Skv = k.shape[1], k.shape[2]
+        want = (B, Hk, Skv, D)
+    else:
+        B, Sq, inner = q.shape
+        if H <= 0 or inner % H:
+            raise ValueError(f"q's last dimension {inner} is not a multiple of heads={heads}")
+        D = inner // H
+        if D == 0 or k.shape[2] % D:
+            raise ValueError(f"k's last dimension {k.shape[2]} is not a multiple of the head dim {D}")
+        Hk, Skv = k.shape[2] // D, k.shape[1]
+        want = (B, Skv, Hk * D)
+    if k.shape != want or v.shape != want:
+        raise ValueError(f"k/v shapes {tuple(k.shape)}, {tuple(v.shape)} do not match q")
+    if (kv_heads is not None and int(kv_heads) != Hk) or Hk <= 0 or H % Hk:
+        raise ValueError(f"k/v hold {Hk} heads: kv_heads must be that, and a divisor of heads={H} (got {kv_heads})")
+    scale = D ** -0.5 if scale is None else float(scale)
+    shape = (B, H, Sq, D) if head_major_out else (B, Sq, H * D)
+    if out is None:
+        out = torch.empty(shape, dtype=out_dtype, device=dev)
+    elif out.dtype not in _DT or out.shape != shape or out.stride(-1) != 1 or out.device != dev:
+        raise ValueError(f"attention output must be bf16/f32 {shape} with a contiguous last dimension on {dev}")
+    start, starts = Skv - Sq, None
+    if isinstance(q_start, torch.Tensor):
+        starts = _per_batch(q_start, "q_start", B, dev)
+    elif q_start is not None:
+        start = int(q_start)
+    prefix, prefixes = 0, None
+    if prefix_len is not None:
+        if not causal:
+            raise ValueError("prefix_len needs causal=True")
+        if isinstance(prefix_len, torch.Tensor):
+            prefixes = _per_batch(prefix_len, "prefix_len", B, dev)
+        else:
+            prefix = int(prefix_len)
+    if kv_lens is not None:
+        _per_batch(kv_lens, "kv_lens", B, dev)
+    if doc_offsets is not None:
+        if Sq != Skv:
+            raise ValueError(f"doc_offsets need as many queries as keys (got {Sq} and {Skv})")
+        if doc_offsets.dtype != torch.int32 or doc_offsets.dim() not in (1, 2) or doc_offsets.shape[-1] < 1 or \
+                (doc_offsets.dim() == 2 and doc_offsets.shape[0] != B) or not doc_offsets.is_contiguous() or \
+                doc_offsets.device != dev:
+            raise ValueError(f"doc_offsets must be contiguous int32 [n + 1] or [B, n + 1] on {dev}")
+    cap = 0.0
+    if softcap is not None:
+        cap = float(softcap)
+        if not 0.0 < cap < 3e38:
+            raise ValueError(f"softcap must be positive and finite (got {softcap})")
+    if slopes is not None:
+        _per_batch(slopes, "slopes", H, dev, torch.float32)
+    if distance_bias is not None:
+        if distance_bias.dtype != torch.float32 or distance_bias.dim() != 2 or distance_bias.shape[0] != H or \
+                distance_bias.shape[1] % 2 == 0 or not distance_bias.is_contiguous() or distance_bias.device != dev:
+            raise ValueError(f"distance_bias must be a contiguous f32 [heads, 2R + 1] tensor on {dev}")
+    if mask is not None:
+        if mask.dtype not in (torch.bool, torch.bfloat16, torch.float32) or mask.dim() not in (2, 4) or \
+                mask.device != dev:
+            raise ValueError(f"mask must be a bool, bf16 or f32 tensor of 2 or 4 dimensions on {dev}")
+        if mask.dim() == 2:
+            mask = mask[None, None]
+        if any(n not in (1, m) for n, m in zip(mask.shape[:3], (B, H, Sq))) or mask.shape[3] != Skv or \
+                (Skv > 1 and mask.stride(3) != 1):
+            raise ValueError(f"mask {tuple(mask.shape)} does not broadcast to {(B, H, Sq, Skv)} with contiguous keys")
+    ops = _lib.torch_ops()
+    if ops is not None:
+        return ops.attention_masked(q, k, v, out, H, Hk, head_major_in, head_major_out, scale, int(variant), causal,
+                                    start, starts, prefix, prefixes, kv_lens, doc_offsets, cap, slopes, distance_bias,
+                                    mask)
+    mods = _lib.AttentionMods(causal=int(causal), q_start=start, prefix=prefix, softcap=cap)
+    for name, t in (("q_starts", starts), ("prefixes", prefixes), ("kv_lens", kv_lens), ("doc_offsets", doc_offsets),
+                    ("slopes", slopes), ("distance_bias", distance_bias), ("mask", mask)):
+        setattr(mods, name, None if t is None else t.data_ptr())
+    if doc_offsets is not None:
+        mods.docs = doc_offsets.shape[-1] - 1
+        mods.doc_stride = doc_offsets.shape[1] if doc_offsets.dim() == 2 else 0
+    if distance_bias is not None:
+        mods.max_distance = distance_bias.shape[1] // 2
+    if mask is not None:
+        mods.mask_dtype = _lib.DTYPE_BOOL if mask.dtype == torch.bool else _DT[mask.dtype]
+        mods.mask_sb, mods.mask_sh, mods.mask_sq = (s if n > 1 else 0 for n, s in zip(mask.shape, mask.stride()[:3]))
+    qs, ks, vs, os_ = ((t.stride(0), t.stride(2), t.stride(1)) if hm else (t.stride(0), t.stride(1), D)
+                       for t, hm in ((q, head_major_in), (k, head_major_in), (v, head_major_in), (out, head_major_out)))
+    with torch.cuda.device(dev):
+        nbytes = ctypes.c_size_t(0)
+        _lib.call("npub200_attention_masked_workspace_size", B, H, Hk, Sq, Skv, D, int(variant), ctypes.byref(nbytes))
+        # a workspace of this call's own: calls on other streams and captured graphs never share one
+        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev) if nbytes.value else None
+        _lib.call("npub200_attention_masked",
+                  ctypes.c_void_p(q.data_ptr()), *qs, ctypes.c_void_p(k.data_ptr()), *ks,
+                  ctypes.c_void_p(v.data_ptr()), *vs, ctypes.c_void_p(out.data_ptr()), *os_, _DT[out.dtype],
+                  B, H, Hk, Sq, Skv, D, ctypes.c_float(scale), ctypes.byref(mods),
+                  ctypes.c_void_p(ws.data_ptr()) if ws is not None else None, nbytes.value, int(variant),
+                  ctypes.c_void_p(_stream_ptr(dev)))
     return out
 
 
