@@ -39,8 +39,21 @@ constexpr int kGemmBK = 64;  // one 128-byte swizzle atom of bf16 along K
 // (32 accumulator rows) and take alternate output chunks, so one warp's TMEM-load and store latencies overlap the
 // other's arithmetic.
 constexpr int kGemmEpiWarps = 8;
-constexpr int kGemmEpiThreads = kGemmEpiWarps * 32;
-constexpr int kGemmThreads = 64 + kGemmEpiThreads;
+constexpr int kGemmThreads = 64 + kGemmEpiWarps * 32;
+
+constexpr int kModePlain = 0;
+constexpr int kModeGeglu = 1;
+constexpr int kModeConv3x3 = 2;
+constexpr int kModeAct = 3;  // plain GEMM with an activation between the bias and the residual
+
+// Epilogue warps of an instantiation. The activation form's wide tiles take 16, in two sets of 8 that serve alternate
+// tiles (one accumulator buffer each): its epilogue is longer than the main loop, and with two tiles in work one set's
+// arithmetic overlaps the other's loads and stores. Measured at 65536 x 320 x 1280 with gelu and residual: 8 warps 126
+// us, one set of 16 109 us, two sets 106 us (relu 86 us; 124 us for the plain form's epilogue with residual alone).
+template <int BN, int MODE>
+constexpr int gemm_epi_warps() {
+  return MODE == kModeAct && BN >= 128 ? 16 : kGemmEpiWarps;
+}
 
 struct GemmArgs {
   int M, N, K;
@@ -58,6 +71,7 @@ struct GemmArgs {
   void* out;
   long long ldo;
   int out_f32;
+  int tma_residual;  // activation form, bf16 output: the residual is read through TMA
   int tma_store;  // 1: the output goes out through TMA stores (aligned output), 0: direct predicated stores
   // Split-K: `splits` CTAs, one cluster, share an output tile, each over `kb_per_split` K blocks. Each parks its
   // f32 partial in its own shared memory; after all have, each sums a slice of the tile over every CTA's partial
@@ -67,7 +81,8 @@ struct GemmArgs {
 };
 
 // BROWS: rows of the B tile this CTA holds per stage (BN, or BN/2 for one CTA of a pair).
-template <int BN, int STAGES, int BROWS = BN>
+// EPIW: epilogue warps.
+template <int BN, int STAGES, int BROWS = BN, int EPIW = kGemmEpiWarps>
 struct GemmLayout {
   static constexpr int kABytes = kGemmBM * kGemmBK * 2;  // 16 KB
   static constexpr int kBBytes = BROWS * kGemmBK * 2;
@@ -75,14 +90,15 @@ struct GemmLayout {
   static constexpr int kTmemCols = (2 * BN <= 64) ? 64 : (2 * BN <= 128) ? 128 : (2 * BN <= 256) ? 256 : 512;
   // Epilogue staging: per epilogue warp one 32-row x 128-byte tile (128-byte swizzle) for the TMA stores.
   static constexpr int kStagingOffset = STAGES * kStageBytes;
-  static constexpr int kStagingBytes = kGemmEpiWarps * 32 * 128;
+  static constexpr int kStagingBytes = EPIW * 32 * 128;
   static constexpr int kBarOffset = kStagingOffset + kStagingBytes;
-  // full[S], empty[S], acc_full[2], acc_empty[2], drain, bias_full, bias_free, parts_ready
-  static constexpr int kNumBars = 2 * STAGES + 8;
+  // full[S], empty[S], acc_full[2], acc_empty[2], drain, bias_full, bias_free, parts_ready, res_full[2 EPIW]
+  static constexpr int kNumBars = 2 * STAGES + 8 + 2 * EPIW;
   static constexpr int kMiscOffset = kBarOffset + kNumBars * 8;
-  // The tile's bias in f32 (BN entries: the output columns', then in the GEGLU form the gate columns').
+  // The tile's bias in f32 (BN entries: the output columns', then in the GEGLU form the gate columns'); with 16 epilogue
+  // warps room for two 32-value slots per warp as well.
   static constexpr int kBiasOffset = (kMiscOffset + 16 + 15) / 16 * 16;
-  static constexpr int kSmemBytes = kBiasOffset + BN * 4 + 1024;  // + slack to align the base to 1 KB
+  static constexpr int kSmemBytes = kBiasOffset + BN * 4 + (EPIW > kGemmEpiWarps ? EPIW * 256 : 0) + 1024;  // + slack to align the base to 1 KB
   static_assert(kBBytes % 1024 == 0, "B stage must keep 1 KB alignment for the 128-byte swizzle");
   static_assert(BN % 32 == 0 && BN >= 32 && BN <= 256, "N tile: a multiple of 32 (UMMA N for M=128 <= 256)");
   static_assert(kSmemBytes <= 232448, "shared memory budget of one CTA");
@@ -196,11 +212,6 @@ __device__ __forceinline__ void add_residual32(const GemmArgs& a, int grow, int 
   }
 }
 
-constexpr int kModePlain = 0;
-constexpr int kModeGeglu = 1;
-constexpr int kModeConv3x3 = 2;
-constexpr int kModeAct = 3;  // plain GEMM with an activation between the bias and the residual
-
 // GELU with the error function (torch's default `F.gelu`, approximate='none'): y * Phi(y) = y/2 * (1 + erf(y/sqrt2)).
 // erf by Abramowitz & Stegun, Handbook of Mathematical Functions, formula 7.1.26 (Hastings' rational approximation,
 // |error| <= 1.5e-7): for z >= 0, erf(z) = 1 - t (a1 + t (a2 + t (a3 + t (a4 + t a5)))) exp(-z^2), t = 1 / (1 + p z).
@@ -217,34 +228,97 @@ __device__ __forceinline__ float gelu_erf(float y) {
   return 0.5f * y * (y >= 0.0f ? 2.0f - tail : tail);
 }
 
-// y * sigmoid(s) = y / (1 + 2^(-s log2 e)); a denominator past 2^126 gives 0 (the true value is below 1e-37 |y|).
-__device__ __forceinline__ float times_sigmoid(float y, float s) {
-  return __fdividef(y, 1.0f + fast_exp2(-1.4426950408889634f * s));
+// Activations of two values at a time (packed f32x2 arithmetic halves the issue slots of the FMA-pipe work; the
+// exponentials and reciprocals go to the MUFU one by one).
+
+// Reciprocals of two pairs, (1 / d0, 1 / d1) and (1 / d2, 1 / d3), from one MUFU reciprocal of their product (which
+// must not overflow): 9 FMA-pipe slots against 24 MUFU cycles a warp.
+__device__ __forceinline__ void rcp4(uint64_t da, uint64_t db, uint64_t& ra, uint64_t& rb) {
+  float d0, d1, d2, d3;
+  f2_unpack(da, d0, d1);
+  f2_unpack(db, d2, d3);
+  const float pa = d0 * d1, pb = d2 * d3;
+  const float r = fast_rcp(pa * pb);
+  const float qa = r * pb, qb = r * pa;
+  ra = f2_mul(f2_pack(d1, d0), f2_pack(qa, qa));
+  rb = f2_mul(f2_pack(d3, d2), f2_pack(qb, qb));
 }
 
-// The activation of NPUB200_ACT_* code `act` on 32 (or 4) values; the branch is uniform over the grid. The tanh form of
-// GELU is y sigmoid(2u) with u = sqrt(2/pi) (y + 0.044715 y^3), since (1 + tanh u) / 2 = sigmoid(2u): one exp2 and one
+// y sigmoid(s) = y / (1 + 2^t) of two pairs, t = -s log2 e capped at 30: below s = -20.8 the sigmoid stays at 2^-30,
+// an error under 1e-9 |y| (and the product of four denominators stays finite).
+__device__ __forceinline__ void times_sigmoid4(uint64_t& ya, uint64_t& yb, uint64_t ta, uint64_t tb) {
+  float t0, t1, t2, t3;
+  f2_unpack(ta, t0, t1);
+  f2_unpack(tb, t2, t3);
+  const uint64_t one = f2_pack(1.0f, 1.0f);
+  uint64_t ra, rb;
+  rcp4(f2_add(f2_pack(fast_exp2(fminf(t0, 30.0f)), fast_exp2(fminf(t1, 30.0f))), one),
+       f2_add(f2_pack(fast_exp2(fminf(t2, 30.0f)), fast_exp2(fminf(t3, 30.0f))), one), ra, rb);
+  ya = f2_mul(ya, ra);
+  yb = f2_mul(yb, rb);
+}
+
+// gelu(y) = y/2 (1 + erf(y/sqrt2)) = max(y, 0) - |y|/2 (1 - erf(|y|/sqrt2)) of two pairs, the tail 1 - erf by the formula
+// of gelu_erf (the halves folded into its coefficients). |y| is capped at 64, where the tail is 0, so an infinity meets
+// no 0 * inf.
+__device__ __forceinline__ uint64_t gelu_cap(uint64_t y) {
+  float y0, y1;
+  f2_unpack(y, y0, y1);
+  return f2_pack(fminf(fabsf(y0), 64.0f), fminf(fabsf(y1), 64.0f));
+}
+__device__ __forceinline__ uint64_t gelu_finish(uint64_t y, uint64_t a, uint64_t t) {
+  constexpr float kE = -0.5f * 1.4426950408889634f;
+  float y0, y1, e0, e1;
+  f2_unpack(y, y0, y1);
+  f2_unpack(f2_mul(f2_mul(a, a), f2_pack(kE, kE)), e0, e1);
+  const uint64_t e = f2_pack(fast_exp2(e0), fast_exp2(e1));
+  // minus half the polynomial's coefficients: the result is max(y, 0) + a * (q t e)
+  uint64_t q = f2_fma(f2_pack(-0.5307027145f, -0.5307027145f), t, f2_pack(0.7265760135f, 0.7265760135f));
+  q = f2_fma(q, t, f2_pack(-0.7107068705f, -0.7107068705f));
+  q = f2_fma(q, t, f2_pack(0.142248368f, 0.142248368f));
+  q = f2_fma(q, t, f2_pack(-0.127414796f, -0.127414796f));
+  return f2_fma(f2_mul(f2_mul(q, t), e), a, f2_pack(relu_nan(y0), relu_nan(y1)));
+}
+__device__ __forceinline__ void gelu_erf4(uint64_t& ya, uint64_t& yb) {
+  constexpr float kP = 0.3275911f * 0.70710678118654752f;
+  const uint64_t one = f2_pack(1.0f, 1.0f), p = f2_pack(kP, kP);
+  const uint64_t aa = gelu_cap(ya), ab = gelu_cap(yb);
+  uint64_t ta, tb;
+  rcp4(f2_fma(aa, p, one), f2_fma(ab, p, one), ta, tb);
+  ya = gelu_finish(ya, aa, ta);
+  yb = gelu_finish(yb, ab, tb);
+}
+
+// The activation of NPUB200_ACT_* code `act` on N pairs; the branch is uniform over the grid. The tanh form of GELU is
+// y sigmoid(2u) with u = sqrt(2/pi) (y + 0.044715 y^3), since (1 + tanh u) / 2 = sigmoid(2u): one exp2 and one
 // reciprocal, and no cancellation for negative y.
 template <int N>
-__device__ __forceinline__ void activate(int act, float (&v)[N]) {
+__device__ __forceinline__ void activate(int act, uint64_t (&v)[N]) {
+  constexpr float kLog2e = 1.4426950408889634f;
+  static_assert(N % 2 == 0, "pairs go two by two");
   if (act == NPUB200_ACT_GELU) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = gelu_erf(v[j]);
+    for (int j = 0; j < N; j += 2) gelu_erf4(v[j], v[j + 1]);
   } else if (act == NPUB200_ACT_GELU_TANH) {
+    constexpr float kA = -2.0f * 0.79788456080286536f * kLog2e, kB = 0.044715f * kA;
+    const uint64_t a = f2_pack(kA, kA), b = f2_pack(kB, kB);
+#pragma unroll
+    for (int j = 0; j < N; j += 2)
+      times_sigmoid4(v[j], v[j + 1], f2_mul(v[j], f2_fma(f2_mul(v[j], v[j]), b, a)),
+                     f2_mul(v[j + 1], f2_fma(f2_mul(v[j + 1], v[j + 1]), b, a)));
+  } else if (act == NPUB200_ACT_RELU) {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const float y = v[j];
-      v[j] = times_sigmoid(y, y * fmaf(1.5957691216057308f * 0.044715f * y, y, 1.5957691216057308f));
+      float y0, y1;
+      f2_unpack(v[j], y0, y1);
+      v[j] = f2_pack(relu_nan(y0), relu_nan(y1));
     }
-  } else if (act == NPUB200_ACT_QUICK_GELU) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = times_sigmoid(v[j], 1.702f * v[j]);
-  } else if (act == NPUB200_ACT_SILU) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = times_sigmoid(v[j], v[j]);
   } else {
+    const float k = act == NPUB200_ACT_SILU ? -kLog2e : -1.702f * kLog2e;
+    const uint64_t k2 = f2_pack(k, k);
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = v[j] < 0.0f ? 0.0f : v[j];  // a NaN stays one
+    for (int j = 0; j < N; j += 2)
+      times_sigmoid4(v[j], v[j + 1], f2_mul(v[j], k2), f2_mul(v[j + 1], k2));
   }
 }
 
@@ -263,10 +337,15 @@ __device__ __forceinline__ void tile_coords(const GemmArgs& a, int tile, int& m_
 // the MMAs, whose commits arrive on both CTAs' barriers; each CTA's epilogue drains its own 128 accumulator rows.
 // Per SM that is 16 KB + BN/2 x 128 B of operands per K block instead of 16 KB + BN x 128 B.
 template <int BN, int STAGES, int MODE, bool PAIR>
-__global__ void __launch_bounds__(kGemmThreads, 1)
+__global__ void __launch_bounds__(64 + 32 * gemm_epi_warps<BN, MODE>(), 1)
     gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
-                             const __grid_constant__ CUtensorMap tm_out, const GemmArgs args) {
-  using L = GemmLayout<BN, STAGES, PAIR ? BN / 2 : BN>;
+                             const __grid_constant__ CUtensorMap tm_out, const __grid_constant__ CUtensorMap tm_res,
+                             const GemmArgs args) {
+  constexpr int kEpiWarps = gemm_epi_warps<BN, MODE>();
+  constexpr int kSets = kEpiWarps / kGemmEpiWarps;
+  constexpr int kEpiThreads = kGemmEpiWarps * 32;  // threads of a set
+  constexpr int kParts = kGemmEpiWarps / 4;        // a set's warps per TMEM lane quarter
+  using L = GemmLayout<BN, STAGES, PAIR ? BN / 2 : BN, kEpiWarps>;
   constexpr bool GEGLU = MODE == kModeGeglu;
   static_assert(!PAIR || (BN % 32 == 0 && BN >= 64), "a pair splits the weight rows of a tile in two 16-row multiples");
   const uint32_t rank = PAIR ? cluster_ctarank() : 0u;  // CTA rank in the pair (0 = leader)
@@ -326,6 +405,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   uint64_t* bias_full = drain + 1;  // the epilogue warps have written this tile's bias table
   uint64_t* bias_free = drain + 2;  // the epilogue warps are done reading the previous tile's table
   uint64_t* parts_ready = drain + 3;  // split K: every CTA of the cluster has parked its partial tile
+  uint64_t* res_full = drain + 4;     // activation form: a residual tile has landed, two per epilogue warp
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMiscOffset);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMiscOffset + 4);
 
@@ -342,8 +422,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       mbar_init(&acc_empty[a], PAIR ? 2 * kGemmEpiWarps : kGemmEpiWarps);  // one arrival per epilogue warp
     }
     mbar_init(drain, 1);
-    mbar_init(bias_full, kGemmEpiThreads);  // one arrival per epilogue thread
-    mbar_init(bias_free, kGemmEpiThreads);
+    mbar_init(bias_full, kEpiThreads);  // one arrival per epilogue thread
+    mbar_init(bias_free, kEpiThreads);
+    for (int i = 0; MODE == kModeAct && i < 2 * kEpiWarps; ++i) mbar_init(&res_full[i], 1);
     mbar_init(parts_ready, uint32_t(args.splits));  // one arrival from each CTA of a split-K cluster
     *abort_flag = 0;
     fence_barrier_init();
@@ -542,7 +623,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   } else {
     // ------------------------------------------------------------------ epilogue (warps 2..9)
     const int quarter = warp & 3;  // TMEM lanes this warp may access: [32*quarter, 32*quarter + 32)
-    const int half = (warp - 2) >> 2;  // which of the quarter's two warps: output chunks half, half + 2, ...
+    const int set = (warp - 2) / kGemmEpiWarps;  // serves the CTA's units set, set + kSets, ...
+    const int half = ((warp - 2) >> 2) & 1;  // which of the quarter's kParts warps: output chunks half, half + kParts, ...
     const int row = quarter * 32 + lane;
     // Output goes out in chunks of 128-byte rows (64 bf16 or 32 f32 columns) through a staging tile per warp,
     // laid out with the 128-byte swizzle so the row-per-thread writes hit distinct banks; the quarter's two warps
@@ -551,16 +633,59 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     uint8_t* sb = smem + L::kStagingOffset + (warp - 2) * (32 * 128);
     const int cw = args.out_f32 ? 32 : 64;
     const int splits = args.splits;
-    int local = 0;
+    int local = set;
     // One bias row for the whole output: read from a per-tile table in shared memory. A bias row per image is read
     // by each thread for its own row.
-    const bool table_bias = args.bias != nullptr && args.bias_img_stride == 0;
+    // (The activation form uses it for split K only: a barrier over the epilogue warps in every tile held them in step.
+    // Its warps keep the 32 values of a group in a slot of their own, requested a group ahead.)
+    const bool table_bias = args.bias != nullptr && args.bias_img_stride == 0 && (MODE != kModeAct || splits > 1);
     float* bias_tab = reinterpret_cast<float*>(smem + L::kBiasOffset);
+    // Activation form: a tile's columns go in groups of 32, group g to the quarter's warp g % kParts, through two
+    // alternating 2 KB staging tiles per warp (bf16, 64-byte rows with the 64-byte swizzle; f32: one 4 KB tile), so one
+    // group's output leaves while the next is computed: with a single one the stores, bound by the write bandwidth,
+    // and the arithmetic took turns. A bf16 residual that TMA can address is loaded into the staging tile that its
+    // output replaces, one group ahead.
+    uint64_t* my_res = res_full + 2 * (warp - 2);
+    int group = 0;                          // groups this warp has processed (staging tile group & 1)
+    uint32_t res_phase = 0, res_pending = 0;  // per staging tile: the barrier's next parity, whether a load is in flight
+    auto request_residual = [&](int buf, int rm0, int gcol) {  // lane 0 only issues; the state is warp-uniform
+      if (gcol >= args.N || rm0 + quarter * 32 >= args.M) return;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&my_res[buf], 32 * 64);
+        tma_load_2d(&tm_res, &my_res[buf], sb + buf * 2048, gcol, rm0 + quarter * 32);
+      }
+      res_pending |= 1u << buf;
+    };
+    // Coordinates of the set's next tile, stepped without a division.
+    int next_mb = 0, next_nb = 0;
+    const int inner = args.n_fastest ? args.num_n_blk : args.num_m_blk;
+    const int step_outer = kSets * unit_stride / inner, step_inner = kSets * unit_stride - step_outer * inner;
+    auto step_tile = [&](int& tmb, int& tnb) {
+      int& fast = args.n_fastest ? tnb : tmb;
+      int& slow = args.n_fastest ? tmb : tnb;
+      fast += step_inner;
+      slow += step_outer;
+      if (fast >= inner) {
+        fast -= inner;
+        ++slow;
+      }
+    };
+    float* bias_slot = reinterpret_cast<float*>(smem + L::kBiasOffset) + (kSets > 1 ? BN + (warp - 2) * 64 : 0);
+    auto bias_value = [&](int col) {  // lane's value of a group of 32 columns
+      if (args.bias == nullptr || col >= args.N) return 0.0f;
+      return args.bias_f32 ? __ldg(static_cast<const float*>(args.bias) + col)
+                           : __bfloat162float(static_cast<const __nv_bfloat16*>(args.bias)[col]);
+    };
     pdl_wait();  // the previous kernel may still read (or write) the output / bias
-    for (int unit = unit0; unit < num_units; unit += unit_stride, ++local) {
+    if constexpr (MODE == kModeAct) {
+      tile_coords(args, unit0 / splits + set * unit_stride, next_mb, next_nb);
+      if (kSets > 1 && splits == 1) bias_slot[lane] = bias_value(next_nb * BN + half * 32 + lane);
+      __syncwarp();
+    }
+    for (int unit = unit0 + set * unit_stride; unit < num_units; unit += kSets * unit_stride, local += kSets) {
       const int acc = local & 1;
       const uint32_t acc_phase = (local >> 1) & 1;
-      if (args.bias != nullptr && warp == 2) {
+      if (kEpiWarps == kGemmEpiWarps && args.bias != nullptr && warp == 2) {
         // Pull this tile's bias into L2 while the main loop runs (one 128-byte line per lane).
         int pmb, pnb;
         tile_coords(args, unit / splits, pmb, pnb);
@@ -575,13 +700,22 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       const int tile = unit / splits;
       const int split = unit % splits;
       int mb, nb;
-      tile_coords(args, tile, mb, nb);
+      if constexpr (MODE == kModeAct) {
+        mb = next_mb;
+        nb = next_nb;
+        if (splits == 1) step_tile(next_mb, next_nb);
+      } else {
+        tile_coords(args, tile, mb, nb);
+      }
       const int m0 = mb * kTileM + int(rank) * kGemmBM;  // this CTA's 128 rows of the tile
       const int n0 = nb * kOutCols;
+      if constexpr (MODE == kModeAct) {
+        if (args.tma_residual && local == set && half * 32 < BN) request_residual(0, m0, n0 + half * 32);
+      }
       if (table_bias) {
         // This tile's bias table: each epilogue thread fetches up to two entries (requested before any wait),
         // stores them once every warp is done with the previous tile's table, then all wait for the full table.
-        static_assert(BN <= kGemmEpiThreads, "one bias table entry per epilogue thread");
+        static_assert(BN <= kEpiThreads, "one bias table entry per epilogue thread");
         const int i = int(threadIdx.x) - 64;
         const int col = i < kOutCols ? n0 + i : args.N + n0 + (i - kOutCols);
         const float e = (i < BN && col < args.bias_n)
@@ -606,7 +740,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         constexpr int kPS = BN + 4;
         float* part = reinterpret_cast<float*>(smem);
 #pragma unroll 1
-        for (int c = half * 32; c < BN; c += 64) {
+        for (int c = half * 32; c < BN; c += 32 * kParts) {
           uint32_t r[32];
           tmem_ld32(t_row + uint32_t(c), r);
           tmem_wait_ld();
@@ -616,7 +750,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             dst[j] = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]),
                                  __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
         }
-        named_barrier_sync(1, kGemmEpiThreads);
+        named_barrier_sync(1, kEpiThreads);
         if (threadIdx.x == 64) {
           fence_acq_rel_cluster();
           for (int s2 = 0; s2 < splits; ++s2) mbar_arrive_cluster(cluster_smem_addr(parts_ready, uint32_t(s2)));
@@ -626,7 +760,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         const int r1 = (kGemmBM * (split + 1)) / splits;
         const int items = (r1 - r0) * (BN / 4);
 #pragma unroll 1
-        for (int it = int(threadIdx.x) - 64; it < items; it += kGemmEpiThreads) {
+        for (int it = int(threadIdx.x) - 64; it < items; it += kEpiThreads) {
           const int rr = r0 + it / (BN / 4);
           const int cc = (it % (BN / 4)) * 4;
           const float* mine = part + rr * kPS + cc;
@@ -655,7 +789,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
               b = load_bias_own(args, gcol, j, own);
             v[j] += b;
           }
-          if constexpr (MODE == kModeAct) activate(args.act, v);
+          if constexpr (MODE == kModeAct) {
+            uint64_t v2[2] = {f2_pack(v[0], v[1]), f2_pack(v[2], v[3])};
+            activate(args.act, v2);
+            f2_unpack(v2[0], v[0], v[1]);
+            f2_unpack(v2[1], v[2], v[3]);
+          }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             if (args.residual != nullptr && gcol + j < args.N)
@@ -682,6 +821,114 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             }
           }
         }
+      } else if constexpr (MODE == kModeAct) {
+        bool ok = true;
+#pragma unroll 1
+        for (int c = half * 32; c < BN; c += 32 * kParts, ++group) {
+          const int buf = args.out_f32 ? 0 : group & 1;
+          uint32_t r[32];
+          tmem_ld32(t_row + uint32_t(c), r);
+          // The next group of this warp: in this tile or in its set's next one.
+          const bool here = c + 32 * kParts < BN;
+          const bool more = here || unit + kSets * unit_stride < num_units;
+          const int next_m0 = here ? m0 : next_mb * kTileM + int(rank) * kGemmBM;
+          const int next_col = here ? n0 + c + 32 * kParts : next_nb * BN + half * 32;
+          const float bias_next = kSets > 1 && more ? bias_value(next_col + lane) : 0.0f;
+          tmem_wait_ld();
+          if (!here) {  // the accumulator is read: the MMA warp may refill it under this group's arithmetic
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              if constexpr (PAIR)
+                mbar_arrive_cluster(cluster_smem_addr(&acc_empty[acc], 0));
+              else
+                mbar_arrive(&acc_empty[acc]);
+            }
+          }
+          uint64_t v2[16];
+          if (args.bias != nullptr) {
+            float own[kSets > 1 ? 1 : 32];
+            if constexpr (kSets == 1) load_bias32(args, n0 + c, own);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              float4 b4;
+              if constexpr (kSets > 1)
+                b4 = reinterpret_cast<const float4*>(bias_slot + 32 * (group & 1))[j];
+              else
+                b4 = make_float4(own[4 * j], own[4 * j + 1], own[4 * j + 2], own[4 * j + 3]);
+              v2[2 * j] = f2_add(f2_pack(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1])), f2_pack(b4.x, b4.y));
+              v2[2 * j + 1] =
+                  f2_add(f2_pack(__uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3])), f2_pack(b4.z, b4.w));
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v2[j] = f2_pack(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+          }
+          activate(args.act, v2);
+          const bool staged = (res_pending >> buf) & 1u;
+          if (args.tma_residual) {
+            // The other staging tile's output has left it: it takes the next group's residual (of this tile, or of the
+            // set's next tile).
+            if (lane == 0) bulk_wait_read<0>();
+            if (more) request_residual(buf ^ 1, next_m0, next_col);
+          } else if (lane == 0) {
+            // The output that last used this staging tile has left it.
+            if (args.out_f32)
+              bulk_wait_read<0>();
+            else
+              bulk_wait_read<1>();
+          }
+          if (kSets > 1) bias_slot[32 * ((group & 1) ^ 1) + lane] = bias_next;
+          __syncwarp();
+          uint8_t* rowp = sb + buf * 2048 + lane * 64;
+          const int sw = (lane >> 1) & 3;
+          if (staged) {
+            if (!mbar_wait_bounded_warp(&my_res[buf], (res_phase >> buf) & 1u, abort_flag, args.ctl,
+                                        kStatusTimeoutEpilogue)) {
+              ok = false;
+              break;
+            }
+            res_phase ^= 1u << buf;
+            res_pending &= ~(1u << buf);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint4 t = *reinterpret_cast<const uint4*>(rowp + (j ^ sw) * 16);
+              const uint32_t w4[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                v2[4 * j + e] = f2_add(v2[4 * j + e], f2_pack(__uint_as_float(w4[e] << 16),
+                                                             __uint_as_float(w4[e] & 0xFFFF0000u)));
+            }
+          }
+          float v[32];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) f2_unpack(v2[j], v[2 * j], v[2 * j + 1]);
+          if (args.residual != nullptr && !args.tma_residual) add_residual32(args, m0 + row, n0 + c, v);
+          if (!args.tma_store) {
+            store_row32_direct(args, m0 + row, n0 + c, v);
+            continue;
+          }
+          if (args.out_f32) {
+            uint8_t* row4 = sb + lane * 128;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              *reinterpret_cast<float4*>(row4 + (j ^ (lane & 7)) * 16) =
+                  make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              *reinterpret_cast<uint4*>(rowp + (j ^ sw) * 16) =
+                  make_uint4(pack_bf16x2(v[8 * j], v[8 * j + 1]), pack_bf16x2(v[8 * j + 2], v[8 * j + 3]),
+                             pack_bf16x2(v[8 * j + 4], v[8 * j + 5]), pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (n0 + c < args.N && m0 + quarter * 32 < args.M) tma_store_2d(&tm_out, sb + buf * 2048, n0 + c, m0 + quarter * 32);
+            bulk_commit();  // an empty group too: bulk_wait_read<1> counts one group per staging tile
+          }
+        }
+        if (!ok) break;
       } else {
 #pragma unroll 1
         for (int c0 = half * cw; c0 < kOutCols; c0 += 2 * cw) {
@@ -754,7 +1001,6 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
               fetch_bias(b, c, n0 + c);
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[j] += b[j];
-              if constexpr (MODE == kModeAct) activate(args.act, v);
               if (args.residual != nullptr) add_residual32(args, m0 + row, n0 + c, v);
             }
             if (chunk_tma) {
@@ -796,7 +1042,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) {
+      if (lane == 0 && (MODE != kModeAct || splits > 1)) {  // the activation form has arrived already
         if constexpr (PAIR)
           mbar_arrive_cluster(cluster_smem_addr(&acc_empty[acc], 0));  // the leader's MMA waits on it
         else
@@ -804,6 +1050,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       }
       if (table_bias) mbar_arrive(bias_free);
     }
+    for (int i = 0; i < 2; ++i)  // after an abort: residual loads still in flight
+      if ((res_pending >> i) & 1u) mbar_wait_drain(&my_res[i], (res_phase >> i) & 1u, args.ctl);
     if (args.tma_store && lane == 0) bulk_wait_read<0>();  // staging must not be released while being read
   }
 
@@ -832,8 +1080,9 @@ namespace {
 // cluster of `splits` CTAs per output tile, one unit per CTA.
 template <int BN, int STAGES, int MODE = kModePlain, bool PAIR = false>
 int launch_variant(const CUtensorMap& mx, const CUtensorMap& mw, const CUtensorMap& mo, const GemmArgs& args,
-                   int64_t units, int sms, cudaStream_t st, int device) {
-  using L = GemmLayout<BN, STAGES, PAIR ? BN / 2 : BN>;
+                   int64_t units, int sms, cudaStream_t st, int device, const CUtensorMap* mr = nullptr) {
+  constexpr int kEpiWarps = gemm_epi_warps<BN, MODE>();
+  using L = GemmLayout<BN, STAGES, PAIR ? BN / 2 : BN, kEpiWarps>;
   static bool configured[64] = {false};
   static int resident_clusters[64][kGemmMaxSplits + 1] = {};
   auto kern = gemm_bf16_tcgen05_kernel<BN, STAGES, MODE, PAIR>;
@@ -848,7 +1097,7 @@ int launch_variant(const CUtensorMap& mx, const CUtensorMap& mw, const CUtensorM
   }
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
-  cfg.blockDim = dim3(kGemmThreads);
+  cfg.blockDim = dim3(64 + 32 * kEpiWarps);
   cfg.dynamicSmemBytes = L::kSmemBytes;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -877,7 +1126,7 @@ int launch_variant(const CUtensorMap& mx, const CUtensorMap& mw, const CUtensorM
   }
   if (grid > INT32_MAX) return fail(kErrInvalid, "GEMM grid too large");
   cfg.gridDim = dim3(unsigned(grid));
-  return check_cuda(cudaLaunchKernelEx(&cfg, kern, mx, mw, mo, args), "gemm kernel launch");
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, mx, mw, mo, mr != nullptr ? *mr : mo, args), "gemm kernel launch");
 }
 
 int encode_kmajor_map(const void* base, int64_t rows, int64_t k, int64_t ld, int box_rows, CUtensorMap* out) {
@@ -897,16 +1146,18 @@ int encode_kmajor_map(const void* base, int64_t rows, int64_t k, int64_t ld, int
 }
 
 // Output map for the TMA-store epilogue: boxes of 32 rows x 128 bytes (64 bf16 or 32 f32), 128-byte swizzle.
-int encode_out_map(void* out, int64_t M, int64_t N, int64_t ldo, bool f32, CUtensorMap* map) {
+// narrow: boxes of 32 columns, which in bf16 are 64 bytes with the 64-byte swizzle (the activation form's tiles).
+int encode_out_map(void* out, int64_t M, int64_t N, int64_t ldo, bool f32, CUtensorMap* map, bool narrow = false) {
   EncodeTiledFn enc = nullptr;
   if (int rc = encode_tiled_fn(&enc)) return rc;
   const int esz = f32 ? 4 : 2;
   cuuint64_t dims[2] = {cuuint64_t(N), cuuint64_t(M)};
   cuuint64_t strides[1] = {cuuint64_t(ldo) * esz};
-  cuuint32_t box[2] = {cuuint32_t(128 / esz), 32};
+  cuuint32_t box[2] = {cuuint32_t(narrow ? 32 : 128 / esz), 32};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = enc(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, out, dims, strides,
-                   box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   narrow && !f32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                    CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? kOk : kErrInvalid;
 }
@@ -1081,10 +1332,18 @@ int gemm_launch(const GemmProblem& p, cudaStream_t stream) {
   memset(&mo, 0, sizeof(mo));
   const int esz = p.out_f32 ? 4 : 2;
   bool tma_store = (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && (p.ldo * esz) % 16 == 0;
-  if (tma_store && encode_out_map(p.out, p.M, p.N, p.ldo, p.out_f32 != 0, &mo) != kOk) tma_store = false;
+  if (tma_store && encode_out_map(p.out, p.M, p.N, p.ldo, p.out_f32 != 0, &mo, p.act != 0) != kOk) tma_store = false;
+
+  // The activation form reads a bf16 residual through TMA, in boxes laid out as the output's (bf16 output tiles).
+  CUtensorMap mr;
+  memset(&mr, 0, sizeof(mr));
+  const bool tma_residual = p.act != 0 && p.residual != nullptr && !p.out_f32 && tma_store && plan.splits == 1 &&
+                            (reinterpret_cast<uintptr_t>(p.residual) & 15) == 0 && p.ldr % 8 == 0 &&
+                            encode_out_map(const_cast<void*>(p.residual), p.M, p.N, p.ldr, false, &mr, true) == kOk;
 
   GemmArgs a;
   memset(&a, 0, sizeof(a));
+  a.tma_residual = tma_residual ? 1 : 0;
   a.tma_store = tma_store ? 1 : 0;
   a.M = int(p.M);
   a.N = int(p.N);
@@ -1126,9 +1385,9 @@ int gemm_launch(const GemmProblem& p, cudaStream_t stream) {
       }
     } else if (p.act) {
       switch (bn) {
-        case 128: return launch_variant<128, 8, kModeAct, true>(mx, mw, mo, a, units, sms, stream, d);
-        case 192: return launch_variant<192, 6, kModeAct, true>(mx, mw, mo, a, units, sms, stream, d);
-        case 256: return launch_variant<256, 6, kModeAct, true>(mx, mw, mo, a, units, sms, stream, d);
+        case 128: return launch_variant<128, 6, kModeAct, true>(mx, mw, mo, a, units, sms, stream, d, &mr);
+        case 192: return launch_variant<192, 4, kModeAct, true>(mx, mw, mo, a, units, sms, stream, d, &mr);
+        case 256: return launch_variant<256, 4, kModeAct, true>(mx, mw, mo, a, units, sms, stream, d, &mr);
       }
     } else {
       switch (bn) {
@@ -1150,12 +1409,12 @@ int gemm_launch(const GemmProblem& p, cudaStream_t stream) {
   }
   if (p.act) {
     switch (bn) {
-      case 64: return launch_variant<64, 8, kModeAct>(mx, mw, mo, a, units, sms, stream, d);
-      case 96: return launch_variant<96, 6, kModeAct>(mx, mw, mo, a, units, sms, stream, d);
-      case 128: return launch_variant<128, 6, kModeAct>(mx, mw, mo, a, units, sms, stream, d);
-      case 160: return launch_variant<160, 5, kModeAct>(mx, mw, mo, a, units, sms, stream, d);
-      case 192: return launch_variant<192, 4, kModeAct>(mx, mw, mo, a, units, sms, stream, d);
-      case 256: return launch_variant<256, 4, kModeAct>(mx, mw, mo, a, units, sms, stream, d);
+      case 64: return launch_variant<64, 8, kModeAct>(mx, mw, mo, a, units, sms, stream, d, &mr);
+      case 96: return launch_variant<96, 6, kModeAct>(mx, mw, mo, a, units, sms, stream, d, &mr);
+      case 128: return launch_variant<128, 4, kModeAct>(mx, mw, mo, a, units, sms, stream, d, &mr);
+      case 160: return launch_variant<160, 4, kModeAct>(mx, mw, mo, a, units, sms, stream, d, &mr);
+      case 192: return launch_variant<192, 3, kModeAct>(mx, mw, mo, a, units, sms, stream, d, &mr);
+      case 256: return launch_variant<256, 3, kModeAct>(mx, mw, mo, a, units, sms, stream, d, &mr);
     }
     return fail(kErrUnsupported, "no activation GEMM variant with an N tile of %d", bn);
   }
