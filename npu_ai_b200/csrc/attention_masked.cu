@@ -1,872 +1,141 @@
-// attention_masked.cu - attention with masks, score modifiers and grouped key/value heads on B200:
-//   o_i = sum_j softmax_j(s_ij) v_j over the keys j that row i may see (zeros if none),
-//   s_ij = cap tanh(scale q_i.k_j / cap) - slope_h |p_i - j| + table_h[clamp(j - p_i)] + mask_ij.
-// The reference sends every such call to the CPU (its attention gate, comfyui node :39-99); here prompts and single
-// tokens run on the tensor cores.
-//
-// Every rule but the mask tensor leaves a row ONE interval [lo, hi) of keys: lengths, causal (hi = p + 1), prefix
-// (hi = max(p + 1, prefix)), documents ([start, end) of the row's document). A softmax thread owns one row, so its mask
-// is two registers; the CTA walks only the key tiles of the union of its rows' intervals, and only tiles that some row
-// of a warp sees in part pay for masking (two compares a score). A warp none of whose rows sees a tile writes P = 0
-// without reading S.
-//
-// One kernel, one 128-row Q tile per CTA, 64-key tiles, up to two CTAs per SM (the structure of
-// attention_fwd_tcgen05_kernel with eight softmax warps, a TMA producer warp and an MMA warp):
-//   * Two softmax warps share a lane quarter (32 rows): each takes 32 of the tile's 64 keys, they exchange their row
-//     maxima through shared memory, keep a partial sum each, and rescale and store half of the O columns each. Short
-//     prompts and tokens are bound by the latency of a softmax step, which this nearly halves.
-//   * Q rows: `pack` query heads x T positions. With few queries the heads of a group that share a K/V head fill the
-//     tile together (one TMA box of pack heads x T positions), so the cache is read once per group, not once per head.
-//   * Keys beyond the union inside its last (or before it inside its first) tile may be stale cache memory: their V
-//     rows are zeroed in shared memory before the P V product, since P = 0 times a NaN would be a NaN. Their scores are
-//     replaced, not added to.
-//   * Split keys (grid z): when the row tiles leave most SMs idle, each CTA takes an equal part of its tile's keys and
-//     writes its unnormalised O row, max and sum to the workspace; attention_join_kernel joins the parts in part order.
-// Rounding: P is rounded to bf16 for the tensor core (relative 2^-9, as in the unmasked kernel); the sums, the maxima,
-// the modifiers and O are f32.
+// attention_masked.cu - host side of the masked attention (attention_masked.cuh holds the kernel and its reasons): argument
+// checks, the launch plan, and the kernel that joins split keys.
 #include <algorithm>
 #include <cfloat>
 #include <cstring>
 
-#include "attention_sm100.cuh"
+#include "attention_masked.cuh"
 
 namespace npub200 {
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kMaskedBN = 64;        // keys per tile
-constexpr int kHalf = kMaskedBN / 2;  // keys per softmax thread: two warps share the rows of a TMEM lane quarter
-constexpr int kSoftWarps = 2 * kSoftmaxWarps;
-constexpr int kProducerWarp = kSoftWarps, kMmaWarp = kSoftWarps + 1;
-constexpr int kMaskedThreads = (kSoftWarps + 2) * 32;
-constexpr int kMaxSplits = 64;
-constexpr int kTableMargin = 128;     // repeated ends of the distance bias in shared memory, either side
-constexpr int kTableSmemMax = 10240;  // bytes: keeps two CTAs per SM
+// Joins the split parts of a row: with M = max of the parts' maxima, o = sum_z 2^(m_z - M) O_z / sum_z 2^(m_z - M) l_z.
+// WARPS warps take a row's parts in turn (4: few rows, a block each; 1: many rows, four a block), all loads of a warp
+// issued before the weights are known: the join is bound by latency (two round trips to L2), not by its few KB a row.
+// Measured: 160 rows of 27 parts, a token step 18.2 -> 12.4 us with four warps a row; 16384 rows of 2 parts 40 us with
+// a block each, 5 us with a warp each. The sum runs in a fixed order.
+constexpr int kJoinBlockWarps = 4;
+constexpr int kJoinFewRows = 2048;  // about two waves of blocks
 
-struct MaskedArgs {
-  AttnArgs a;
-  int G;              // query heads per key/value head
-  int pack, T;        // a Q tile holds `pack` heads x T positions
-  int inv_row;        // 65536 / (pack or T), rounded up: the divisor of a tile row
-  int head_fast;      // tile row r = position * pack + head (1) or head * T + position (0)
-  int q_bytes;        // bytes of one 64-column atom of the Q box
-  int tiles;          // Q tiles along the positions
-  int pairs, groups;  // (batch, head group) pairs, groups of a sequence: the grid is pairs x tiles x splits
-  int splits;
-  float* part_o;      // [splits][pairs][tiles][128][D] unnormalised O rows
-  float2* part_ml;    // [splits][pairs][tiles][128] (max in log2 units, sum)
-  int causal;
-  long long q_start;
-  const int* q_starts;
-  long long prefix;
-  const int* prefixes;
-  const int* kv_lens;
-  const int* docs;
-  int ndocs;
-  long long doc_stride;
-  float cap_in, cap_out;  // capped score in log2 units = cap_out x tanh(cap_in x raw score)
-  const float* slopes;
-  const float* table;
-  int max_dist;
-  const void* mask;
-  int mask_kind;  // 0 none, 1 bool, 2 bf16, 3 f32
-  int mask_vec;   // rows can be read in 16-byte words
-  int mask_row;   // the rows of a warp share one mask row
-  int table_smem; // the tile's head has its distance bias in shared memory
-  int out_vec;    // output rows can be written in 16-byte words
-  long long m_sb, m_sh, m_sq;
-};
-
-// What a softmax thread knows of its row.
-struct Row {
-  int lo, hi;       // keys it may see
-  int p;            // its position among the keys
-  bool valid;       // a row of the output
-  int head, i, b;
-  float slope;      // slopes[head] * log2 e
-};
-
-__device__ __forceinline__ int clamp_pos(long long x) {
-  return int(min(max(x, -(1ll << 30)), 1ll << 30));
-}
-
-// The document [lo, hi) that token i lies in; false outside every document. Few borders: the warp reads them together and
-// every lane looks at each; many: a binary search. Documents of no tokens are passed over.
-__device__ __forceinline__ bool document_of(const int* off, int docs, int i, int lane, int& lo, int& hi) {
-  lo = hi = 0;
-  int below = 0;  // borders at or below i
-  if (docs < 64) {
-    bool above = false;
-    for (int base = 0; base <= docs; base += 32) {
-      const int v = off[min(base + lane, docs)];
-      for (int k = 0; k < 32 && base + k <= docs; ++k) {
-        const int o = __shfl_sync(0xffffffffu, v, k);
-        if (o <= i) {
-          lo = o;
-          ++below;
-        } else if (!above) {
-          hi = o;
-          above = true;
-        }
-      }
-    }
-  } else {
-    int right = docs + 1;  // off[below - 1] <= i < off[right]
-    while (below < right) {
-      const int mid = (below + right) >> 1;
-      if (off[mid] <= i)
-        below = mid + 1;
-      else
-        right = mid;
-    }
-    if (below >= 1 && below <= docs) {
-      lo = off[below - 1];
-      hi = off[below];
-    }
-  }
-  return below >= 1 && below <= docs;
-}
-
-// The row of thread r of the tile (whole warps call it).
-__device__ __forceinline__ Row row_of(const MaskedArgs& m, int r, int tile, int h0, int b) {
-  Row w;
-  // r / pack or r / T by a multiplication (both at most 128, so the reciprocal rounded up is exact for r < 128)
-  const int q = (r * m.inv_row) >> 16;
-  const int s = m.head_fast ? q : r - q * m.T;
-  const int g = m.head_fast ? r - q * m.pack : q;
-  w.i = tile * m.T + s;
-  w.head = h0 + g;
-  w.b = b;
-  w.valid = r < m.pack * m.T && w.i < m.a.Sq;
-  if (!w.valid) w.head = h0;
-  const int len = m.kv_lens != nullptr ? m.kv_lens[b] : m.a.Skv;
-  const long long start = m.q_starts != nullptr ? (long long)m.q_starts[b] : m.q_start;
-  const long long prefix = m.prefixes != nullptr ? (long long)m.prefixes[b] : m.prefix;
-  w.slope = m.slopes != nullptr ? m.slopes[w.head] * kLog2e : 0.0f;
-  w.p = w.valid ? clamp_pos(start + w.i) : 0;
-  int lo = 0, hi = min(m.a.Skv, len);
-  if (m.causal) hi = min(hi, max(w.p + 1, clamp_pos(prefix)));
-  if (m.docs != nullptr) {
-    int d0, d1;
-    const bool in = document_of(m.docs + b * m.doc_stride, m.ndocs, w.i, r & 31, d0, d1);
-    lo = max(d0, 0);
-    hi = in ? min(hi, d1) : 0;
-  }
-  const bool any = w.valid && hi > lo;  // a row that sees nothing leaves the union alone
-  w.lo = any ? lo : 0;
-  w.hi = any ? hi : 0;
-  return w;
-}
-
-// tanh(y) / y as a polynomial in z = y^2, |y| <= 1 (fit_tanh_poly.py beside this file; relative error 7e-7). Scalar: its
-// constants are immediate operands, which the packed form has to keep or rebuild in register pairs.
-__device__ __forceinline__ float tanh_ratio(float z) {
-  float p = fmaf(-3.074449487e-03f, z, 1.676048711e-02f);
-  p = fmaf(p, z, -5.161965266e-02f);
-  p = fmaf(p, z, 1.328188479e-01f);
-  p = fmaf(p, z, -3.332909346e-01f);
-  p = fmaf(p, z, 9.999994040e-01f);
-  return p;
-}
-
-// Tile-wide values a softmax step needs besides the scores: the mask words or values requested before the wait for S.
-struct MaskAhead {
-  uint4 words[2];  // bool rows of a thread's own: 32 bytes
-  float e;         // one row for the warp: key kv0 + lane in log2 units
-  bool have;
-};
-
-// A mask value in log2 units: -inf hides; any finite value, however low, stays finite.
-__device__ __forceinline__ float mask_log2(float e) { return e == -INFINITY ? e : fmaxf(e * kLog2e, -FLT_MAX); }
-
-__device__ __forceinline__ void request_mask(const MaskedArgs& m, const Row& w, int kv0, int lane, MaskAhead& a) {
-  a.have = false;
-  if (m.mask_kind == 0) return;
-  const long long off = (long long)w.b * m.m_sb + (long long)w.head * m.m_sh + (long long)(w.valid ? w.i : 0) * m.m_sq + kv0;
-  if (m.mask_row) {
-    float e = -INFINITY;
-    if (kv0 + lane < m.a.Skv) {
-      if (m.mask_kind == 1)
-        e = __ldg(static_cast<const uint8_t*>(m.mask) + off + lane) != 0 ? 0.0f : -INFINITY;
-      else if (m.mask_kind == 2)
-        e = mask_log2(__uint_as_float(uint32_t(__ldg(static_cast<const unsigned short*>(m.mask) + off + lane)) << 16));
-      else
-        e = mask_log2(__ldg(static_cast<const float*>(m.mask) + off + lane));
-    }
-    a.e = e;
-    a.have = true;
-  } else if (m.mask_kind == 1 && m.mask_vec && kv0 + kHalf <= m.a.Skv) {
-    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(m.mask) + off);
-#pragma unroll
-    for (int k = 0; k < 2; ++k) a.words[k] = __ldg(p + k);
-    a.have = true;
-  }
-}
-
-// Raw scores -> log2 units with the cap, the biases and the mask tensor applied.
-template <int BN>
-__device__ __forceinline__ void modify_scores(const MaskedArgs& m, const Row& w, int kv0, const MaskAhead& ahead,
-                                              const float* s_table, float* s_mask, int lane, float (&s)[BN]) {
-  if (m.cap_in != 0.0f) {
-    float big = 0.0f;
-#pragma unroll
-    for (int t = 0; t < BN; t += 2) big = fmax3(big, fabsf(s[t]), fabsf(s[t + 1]));
-    if (__all_sync(0xffffffffu, big * m.cap_in <= 1.0f)) {  // the usual case: all on the FMA pipe
-#pragma unroll
-      for (int t = 0; t < BN; ++t) {
-        const float y = s[t] * m.cap_in;
-        s[t] = y * m.cap_out * tanh_ratio(y * y);
-      }
-    } else {
-      // tanh(y) = 1 - 2 / (1 + e^(2y)); the absolute error of a few 2^-23 stays that small next to the cap.
-      const float k = 2.0f * kLog2e * m.cap_in;
-#pragma unroll
-      for (int t = 0; t < BN; ++t)
-        s[t] = m.cap_out * fmaf(-2.0f, fast_rcp(1.0f + fast_exp2(k * s[t])), 1.0f);
-    }
-  } else {
-#pragma unroll
-    for (int t = 0; t < BN; ++t) s[t] *= m.a.scale_log2;
-  }
-  if (m.slopes != nullptr) {
-    const float rel = float(w.p - kv0);
-#pragma unroll
-    for (int t = 0; t < BN; ++t) s[t] = fmaf(-w.slope, fabsf(float(t) - rel), s[t]);
-  }
-  if (m.table != nullptr) {
-    const int R = m.max_dist;
-    const float* tab = m.table + (long long)w.head * (2 * R + 1) + R;
-    const int d0 = kv0 - w.p;
-    if (__all_sync(0xffffffffu, !w.valid || d0 >= R || d0 + BN - 1 <= -R)) {  // past the table's end on either side
-      const float e = __ldg(tab + (d0 >= R ? R : -R)) * kLog2e;
-#pragma unroll
-      for (int t = 0; t < BN; ++t) s[t] += e;
-    } else if (m.table_smem) {
-      // Log2 units, the ends repeated: no clamp a score. Rows of a warp lie within 32 positions, so some row in reach
-      // keeps all within the margin; rows that are no output rows read a row's place in reach.
-      const float* e = s_table + R + kTableMargin + min(max(d0, -R - kTableMargin), R + kTableMargin - BN + 1);
-#pragma unroll
-      for (int t = 0; t < BN; ++t) s[t] += e[t];
-    } else {
-#pragma unroll
-      for (int t = 0; t < BN; ++t) s[t] = fmaf(__ldg(tab + min(max(d0 + t, -R), R)), kLog2e, s[t]);
-    }
-  }
-  if (m.mask_kind == 0) return;
-  if (m.mask_row) {  // one mask row for the warp: broadcast from shared memory
-    s_mask[lane] = ahead.e;
-    const bool low = ahead.e < -1e37f && ahead.e != -INFINITY;
-    if (!__any_sync(0xffffffffu, low)) {  // (orders the writes before the reads, too)
-      __syncwarp();
-#pragma unroll
-      for (int t = 0; t < BN; t += 4) {
-        const float4 e = *reinterpret_cast<const float4*>(s_mask + t);
-        s[t] += e.x;
-        s[t + 1] += e.y;
-        s[t + 2] += e.z;
-        s[t + 3] += e.w;
-      }
-    } else {
-      __syncwarp();
-#pragma unroll
-      for (int t = 0; t < BN; ++t) {
-        const float e = s_mask[t];
-        s[t] = e == -INFINITY ? e : fmaxf(s[t] + e, -FLT_MAX);
-      }
-    }
-    return;
-  }
-  const long long off = (long long)w.b * m.m_sb + (long long)w.head * m.m_sh + (long long)(w.valid ? w.i : 0) * m.m_sq + kv0;
-  const int n = m.a.Skv - kv0;  // readable keys from here
-  // -inf hides; any finite value, however low, stays finite in log2 units.
-  auto add = [](float x, float e) { return e == -INFINITY ? -INFINITY : fmaxf(fmaf(e, kLog2e, x), -FLT_MAX); };
-  if (m.mask_kind == 1) {
-    const uint8_t* p = static_cast<const uint8_t*>(m.mask) + off;
-    if (ahead.have) {
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const uint32_t q[4] = {ahead.words[c].x, ahead.words[c].y, ahead.words[c].z, ahead.words[c].w};
-#pragma unroll
-        for (int t = 0; t < 16; ++t)
-          if ((q[t / 4] & (0xffu << (8 * (t % 4)))) == 0) s[16 * c + t] = -INFINITY;
-      }
-    } else {
-#pragma unroll
-      for (int t = 0; t < BN; ++t)
-        if (t >= n || __ldg(p + t) == 0) s[t] = -INFINITY;
-    }
-  } else if (m.mask_kind == 2) {
-    const unsigned short* p = static_cast<const unsigned short*>(m.mask) + off;
-    if (m.mask_vec && n >= BN) {
-#pragma unroll
-      for (int c = 0; c < BN; c += 8) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p + c));
-        const uint32_t q[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int t = 0; t < 8; ++t)
-          s[c + t] = add(s[c + t], __uint_as_float(t & 1 ? q[t / 2] & 0xFFFF0000u : q[t / 2] << 16));
-      }
-    } else {
-#pragma unroll
-      for (int t = 0; t < BN; ++t)
-        s[t] = t < n ? add(s[t], __uint_as_float(uint32_t(__ldg(p + t)) << 16)) : -INFINITY;
-    }
-  } else {
-    const float* p = static_cast<const float*>(m.mask) + off;
-    if (m.mask_vec && n >= BN) {
-#pragma unroll
-      for (int c = 0; c < BN; c += 4) {
-        const float4 v = __ldg(reinterpret_cast<const float4*>(p + c));
-        s[c] = add(s[c], v.x);
-        s[c + 1] = add(s[c + 1], v.y);
-        s[c + 2] = add(s[c + 2], v.z);
-        s[c + 3] = add(s[c + 3], v.w);
-      }
-    } else {
-#pragma unroll
-      for (int t = 0; t < BN; ++t) s[t] = t < n ? add(s[t], __ldg(p + t)) : -INFINITY;
-    }
-  }
-}
-
-// Whether no row of the warp sees the key tile at kv0 (the same in both warps of the rows: neither reads S then, nor
-// takes the step's barrier).
-__device__ __forceinline__ bool hidden_tile(const Row& w, int kv0) {
-  return __all_sync(0xffffffffu, w.hi <= kv0 || w.lo >= kv0 + kMaskedBN);
-}
-
-// One online-softmax step over the key tile at kv0 for this thread's row and its half of the keys: P as bf16 pairs over
-// the first columns of the S buffer, the running max `mx` (log2 units, -inf while the row has seen nothing) moved only
-// when the tile's max beats it by more than 8 (see softmax_step of the unmasked kernel), the running sum of this half.
-// The two warps of the rows exchange their maxima through s_max[2][128] (a buffer for alternate tiles); the barrier
-// also orders one warp's reads of S before the other's P over the same columns. Returns the factor for O; `move`:
-// whether the max moved (the same in both warps).
-template <bool SCORES>
-__device__ __forceinline__ float masked_softmax_step(const MaskedArgs& m, const Row& w, uint32_t s_addr, int kv0, int half,
-                                                     int row, int lane, const MaskAhead& ahead, const float* s_table,
-                                                     float* s_mask, float* s_max, float& run_max, float& run_sum,
-                                                     bool& move) {
-  move = false;
-  const uint32_t p_addr = s_addr + uint32_t(half * (kHalf / 2));
-  if (hidden_tile(w, kv0)) {
-    const uint32_t z[16] = {};
-    tmem_st16(p_addr, z);
-    return 1.0f;
-  }
-  const int key0 = kv0 + half * kHalf;
-  float s[kHalf];
-  {
-    uint32_t r[32];
-    tmem_ld32(s_addr + uint32_t(half * kHalf), r);
-    tmem_wait_ld();
-#pragma unroll
-    for (int t = 0; t < kHalf; ++t) s[t] = __uint_as_float(r[t]);
-  }
-  if constexpr (SCORES) modify_scores<kHalf>(m, w, key0, ahead, s_table, s_mask, lane, s);
-  if (__any_sync(0xffffffffu, w.valid && (w.lo > key0 || w.hi < key0 + kHalf))) {
-    const int a = w.lo - key0, z = w.hi - key0;
-#pragma unroll
-    for (int t = 0; t < kHalf; ++t)
-      if (t < a || t >= z) s[t] = -INFINITY;
-  }
-  float mx8[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) mx8[e] = fmax3(s[e], s[8 + e], s[16 + e]);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) mx8[e] = fmaxf(mx8[e], s[24 + e]);
-  const float c = SCORES ? 1.0f : m.a.scale_log2;
-  float mx = fmax3(fmax3(mx8[0], mx8[1], mx8[2]), fmax3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])) * c;
-  s_max[half * kAttnBM + row] = mx;
-  named_barrier_sync(1 + (row >> 5), 64);
-  mx = fmaxf(mx, s_max[(half ^ 1) * kAttnBM + row]);
-  move = mx > run_max + m.a.rescale_thr;
-  const float m_new = move ? mx : run_max;
-  const float alpha = move ? fast_exp2(run_max - m_new) : 1.0f;  // 0 on the first tile with a key
-  const float neg_m = m_new == -INFINITY ? 0.0f : -m_new;        // nothing seen yet: every P is 2^-inf = 0
-  const uint64_t c2 = f2_pack(c, c);
-  const uint64_t nm2 = f2_pack(neg_m, neg_m);
-  uint64_t rs2[4] = {0ull, 0ull, 0ull, 0ull};
-  uint32_t pk[16];
-#pragma unroll
-  for (int e2 = 0; e2 < 16; ++e2) {
-    float x0, x1;
-    const uint64_t sv = f2_pack(s[2 * e2], s[2 * e2 + 1]);
-    f2_unpack(SCORES ? f2_add(sv, nm2) : f2_fma(sv, c2, nm2), x0, x1);
-    const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
-    rs2[e2 & 3] = f2_add(rs2[e2 & 3], f2_pack(p0, p1));
-    pk[e2] = pack_bf16x2(p0, p1);
-  }
-  tmem_st16(p_addr, pk);
-  rs2[0] = f2_add(rs2[0], rs2[2]);
-  rs2[1] = f2_add(rs2[1], rs2[3]);
-  float r0, r1;
-  f2_unpack(f2_add(rs2[0], rs2[1]), r0, r1);
-  run_sum = run_sum * alpha + (r0 + r1);
-  run_max = m_new;
-  return alpha;
-}
-
-// The O columns [begin, end) of a padded head dim that each of the two warps of a row rescales and stores: halves in
-// units of 16 columns.
-template <int DP>
-struct OColumns {
-  static constexpr int kFirst = (DP / 16 + 1) / 2 * 16;  // columns of the first warp, where the second's begin
-  static constexpr int kSecond = DP - kFirst;
-};
-
-__device__ __forceinline__ void st_global_v4(uint64_t to, const uint4& v) {
-  asm volatile("st.global.v4.b32 [%0], {%1, %2, %3, %4};" ::"l"(to), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-}
-
-// The warp's 32 O rows x inv (zeros where `zero`) to `dst` (each lane's own row, null: no row): `cols` columns from
-// o_addr on (a multiple of 8) as f32 or bf16. A lane holds a row, so rows go through shared memory (`stage`, an odd
-// number of 16-byte words apart) and out in 16-byte words along them. Rolled loops: this runs once a tile, and
-// straight-line code for every head dim and type was paid for in instruction fetches.
-__device__ __forceinline__ void store_rows(uint32_t o_addr, uint8_t* stage, int cols, bool f32, uint8_t* dst, float inv,
-                                           bool zero, int lane) {
-  const int words = cols * (f32 ? 4 : 2) / 16;  // 16-byte words of a row
-  const int pitch = (words | 1) * 16;
-  uint8_t* mine = stage + lane * pitch;
-#pragma unroll 1
-  for (int c = 0; c < cols; c += 8) {
-    uint32_t r[8];
-    tmem_ld8(o_addr + uint32_t(c), r);
-    tmem_wait_ld();
-    float o[8];
-#pragma unroll
-    for (int t = 0; t < 8; ++t) o[t] = zero ? 0.0f : __uint_as_float(r[t]) * inv;
-    if (f32) {
-      *reinterpret_cast<float4*>(mine + c * 4) = make_float4(o[0], o[1], o[2], o[3]);
-      *reinterpret_cast<float4*>(mine + c * 4 + 16) = make_float4(o[4], o[5], o[6], o[7]);
-    } else {
-      *reinterpret_cast<uint4*>(mine + c * 2) = make_uint4(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]),
-                                                           pack_bf16x2(o[4], o[5]), pack_bf16x2(o[6], o[7]));
-    }
-  }
-  __syncwarp();
-  int row = lane / words, c = lane - row * words;
-  const int step_row = 32 / words, step_c = 32 - step_row * words;
-#pragma unroll 1
-  for (int k = 0; k < words; k += 4) {  // four words in flight a lane
-    uint64_t to[4];
-    uint4 v[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      to[e] = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(dst), row & 31);
-      if (k + e >= words) to[e] = 0;
-      v[e] = to[e] != 0 ? *reinterpret_cast<const uint4*>(stage + row * pitch + c * 16) : make_uint4(0u, 0u, 0u, 0u);
-      if (to[e] != 0) to[e] += uint64_t(c) * 16;
-      row += step_row;
-      c += step_c;
-      if (c >= words) {
-        c -= words;
-        ++row;
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (to[e] != 0) st_global_v4(to[e], v[e]);
-  }
-}
-
-template <int DP, int STAGES>
-struct MaskedLayout {
-  static constexpr int BN = kMaskedBN;
-  static constexpr int kNA = (DP + 63) / 64;
-  static constexpr int kQAtom = kAttnBM * kAtomBytesPerRow;
-  static constexpr int kKVAtom = BN * kAtomBytesPerRow;
-  static constexpr int kQBytes = kNA * kQAtom;
-  static constexpr int kKVBytes = kNA * kKVAtom;
-  static constexpr int kKOff = kQBytes;
-  static constexpr int kVOff = kKOff + STAGES * kKVBytes;
-  static constexpr int kBarOff = kVOff + STAGES * kKVBytes;
-  // q_full, k_full[S], v_full[S], k_empty[S], v_empty[S], s_full[2], p_full[2], pv_done[2], drain
-  static constexpr int kNumBars = 1 + 4 * STAGES + 6 + 1;
-  static constexpr int kMiscOff = kBarOff + kNumBars * 8;   // TMEM slot, abort flag, the warps' unions
-  static constexpr int kMaskOff = (kMiscOff + 16 + 4 * 8 + 15) / 16 * 16;  // the warp's part of a mask row, per softmax warp
-  static constexpr int kMaxOff = kMaskOff + kSoftWarps * kHalf * 4;        // row maxima [tile parity][half][row]
-  static constexpr int kTableOff = kMaxOff + 2 * 2 * kAttnBM * 4;          // the head's distance bias (launch-sized)
-  static constexpr int kSmemBytes = kTableOff + 1024;
-  // The output rows' staging (f32 rows of up to 256 columns, an odd number of words apart) reuses Q, K and V.
-  static_assert(kBarOff >= 2 * kAttnBM * ((DP / 16 + 1) / 2 * 16 * 4 + 16), "staging of the output rows");
-  static constexpr int kOCol = 2 * BN;
-  static constexpr int kTmemUsed = kOCol + DP;
-  static constexpr int kTmemCols = (kTmemUsed <= 256) ? 256 : 512;
-  static constexpr bool kTwoPerSm = kSmemBytes <= 113 * 1024 && kTmemCols <= 256;
-  static_assert(DP % 16 == 0 && DP >= 16 && DP <= 256, "padded head dim must be a multiple of 16 in [16, 256]");
-  static_assert(kSmemBytes <= 232448, "shared memory budget");
-};
-
-template <int DP, int STAGES, bool SCORES>
-__global__ void __launch_bounds__(kMaskedThreads, MaskedLayout<DP, STAGES>::kTwoPerSm ? 2 : 1)
-    attention_masked_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                                    const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ MaskedArgs m) {
-  using L = MaskedLayout<DP, STAGES>;
-  using O = OColumns<DP>;
-  constexpr int BN = L::BN;
-  const AttnArgs& args = m.a;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sQ = smem;
-  uint8_t* sK = smem + L::kKOff;
-  uint8_t* sV = smem + L::kVOff;
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
-  uint64_t* k_full = q_full + 1;
-  uint64_t* v_full = k_full + STAGES;
-  uint64_t* k_empty = v_full + STAGES;
-  uint64_t* v_empty = k_empty + STAGES;
-  uint64_t* s_full = v_empty + STAGES;
-  uint64_t* p_full = s_full + 2;
-  uint64_t* pv_done = p_full + 2;
-  uint64_t* drain = pv_done + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMiscOff);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMiscOff + 4);
-  int* s_union = reinterpret_cast<int*>(smem + L::kMiscOff + 16);  // lo[4], hi[4]
-  float* s_table = reinterpret_cast<float*>(smem + L::kTableOff);
-
-  const int warp = threadIdx.x >> 5;
-  const int lane = threadIdx.x & 31;
-  // All pairs' tiles of one place before the next place; causal rows see more the later they come, so those start first.
-  const int pair = int(blockIdx.x);
-  const int tile = m.causal ? m.tiles - 1 - int(blockIdx.y) : int(blockIdx.y);
-  const int bb = pair / m.groups;
-  const int h0 = (pair - bb * m.groups) * m.pack;
-  const int kvh = m.pack > 1 ? pair - bb * m.groups : h0 / m.G;
-  const int split = int(blockIdx.z);
-
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&k_full[s], 1);
-      mbar_init(&v_full[s], 1);
-      mbar_init(&k_empty[s], 1);
-      mbar_init(&v_empty[s], 1);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], kSoftWarps);
-      mbar_init(&pv_done[i], 1);
-    }
-    mbar_init(drain, 1);
-    *abort_flag = 0;
-    fence_barrier_init();
-  }
-  if (warp == kMmaWarp) {
-    tmem_alloc(tmem_slot, L::kTmemCols);
-    tmem_relinquish();
-    tc_fence_before();
-  }
-  if (warp == kProducerWarp && lane == 0) {
-    mbar_init(q_full, 1);  // by the thread that loads Q, which does not wait for the barriers' owner
-    fence_barrier_init();
-    fence_proxy_async_smem();
-    tma_prefetch_desc(&tm_q);
-    tma_prefetch_desc(&tm_k);
-    tma_prefetch_desc(&tm_v);
-  }
-  pdl_launch_dependents();
-  pdl_wait();  // q, k, v, the lengths, borders and masks may be the previous kernel's outputs; it may read out
-  Row w = {};
-  if (warp == kProducerWarp && lane == 0) {  // Q needs nothing but the tile
-    int c0, c1, c2, c3;
-    mbar_arrive_expect_tx(q_full, uint32_t(L::kNA * m.q_bytes));
-    for (int a = 0; a < L::kNA; ++a) {
-      map_coords(args.pq, a, tile * m.T, h0, bb, c0, c1, c2, c3);
-      tma_load_4d(&tm_q, q_full, sQ + a * L::kQAtom, c0, c1, c2, c3);
-    }
-  }
-  if (SCORES && m.table_smem) {
-    const int R = m.max_dist;
-    const float* tab = m.table + (long long)h0 * (2 * R + 1) + R;
-    for (int k = int(threadIdx.x); k < 2 * (R + kTableMargin) + 1; k += kMaskedThreads)
-      s_table[k] = __ldg(tab + min(max(k - R - kTableMargin, -R), R)) * kLog2e;
-  }
-  const int row = int(threadIdx.x) & (kAttnBM - 1);  // softmax threads: row of the tile and half of the keys
-  const int half = int(threadIdx.x) >> 7;
-  if (warp < kSoftWarps) {
-    w = row_of(m, row, tile, h0, bb);
-    const int lo = __reduce_min_sync(0xffffffffu, w.hi > w.lo ? w.lo : INT_MAX);
-    const int hi = __reduce_max_sync(0xffffffffu, w.hi);
-    if (lane == 0 && half == 0) {
-      s_union[warp] = lo;
-      s_union[4 + warp] = hi;
-    }
-  }
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
-  // The keys [key_lo, key_hi) that some row of the tile sees, and this part's tiles of them.
-  const int key_lo = min(min(s_union[0], s_union[1]), min(s_union[2], s_union[3]));
-  const int key_hi = max(max(s_union[4], s_union[5]), max(s_union[6], s_union[7]));
-  int first = 0, nkv = 0;
-  if (key_hi > key_lo) {
-    const int t0 = key_lo / BN, t1 = (key_hi + BN - 1) / BN;
-    const int per = (t1 - t0 + m.splits - 1) / m.splits;
-    first = t0 + split * per;
-    nkv = max(0, min(t1 - first, per));
-  }
-
-  if (warp == kProducerWarp) {
-    // ------------------------------------------------------------------ TMA producer
-    if (lane == 0) {
-      if (nkv > 0)
-        kv_producer<L::kNA, BN, STAGES>(&tm_k, &tm_v, args, sK, sV, k_full, v_full, k_empty, v_empty, abort_flag, kvh,
-                                        bb, nkv, first);
-      mbar_wait_drain(q_full, 0, args.ctl);
-    }
-  } else if (nkv > 0 && warp == kMmaWarp) {
-    // ------------------------------------------------------------------ MMA issuer (whole warp, one elected lane issues)
-    bool ok = true;
-    if (args.ctl.debug & 1u) {
-      if (!mbar_wait_bounded_warp(drain, 0, abort_flag, args.ctl, kStatusForced)) ok = false;
-    }
-    if (ok && !mbar_wait_bounded_warp(q_full, 0, abort_flag, args.ctl, kStatusTimeoutMma)) ok = false;
-    tc_fence_after();
-    const uint64_t q_desc = smem_desc_kmajor_sw128(smem_u32(sQ));
-    const uint64_t k_desc = smem_desc_kmajor_sw128(smem_u32(sK));
-    const uint64_t v_desc = smem_desc_mnmajor_sw128(smem_u32(sV), L::kKVAtom);
-    auto pv_step = [&](int i) -> bool {
-      const int st = i % STAGES;
-      const int buf = i & 1;
-      if (!mbar_wait_bounded_warp(&v_full[st], uint32_t(i / STAGES) & 1u, abort_flag, args.ctl, kStatusTimeoutMma))
-        return false;
-      // V rows of this tile that no row sees: zeros, whatever the cache holds there.
-      const int kv0 = (first + i) * BN;
-      const int live0 = max(key_lo - kv0, 0), live1 = min(key_hi - kv0, BN), end = min(args.Skv - kv0, BN);
-      if (live0 > 0 || live1 < end) {
-        for (int c = lane; c < BN * L::kNA * 8; c += 32) {
-          const int row = (c >> 3) % BN;
-          if (row < live0 || row >= live1)
-            *reinterpret_cast<uint4*>(sV + st * L::kKVBytes + (c >> 3) / BN * L::kKVAtom + row * kAtomBytesPerRow +
-                                      (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-      }
-      if (!mbar_wait_bounded_warp(&p_full[buf], uint32_t(i >> 1) & 1u, abort_flag, args.ctl, kStatusTimeoutMma))
-        return false;
-      tc_fence_after();
-      if (elect_one()) {
-        issue_pv<DP, BN>(tmem_base + L::kOCol, tmem_base + uint32_t(buf * BN),
-                         v_desc + uint64_t((st * L::kKVBytes) >> 4), i > 0);
-        umma_commit(&pv_done[buf]);
-        umma_commit(&v_empty[st]);
-      }
-      __syncwarp();
-      return true;
-    };
-    for (int j = 0; ok && j < nkv; ++j) {
-      const int st = j % STAGES;
-      const int buf = j & 1;
-      if (!mbar_wait_bounded_warp(&k_full[st], uint32_t(j / STAGES) & 1u, abort_flag, args.ctl, kStatusTimeoutMma)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      if (elect_one()) {
-        issue_s<DP, BN>(tmem_base + uint32_t(buf * BN), q_desc, k_desc + uint64_t((st * L::kKVBytes) >> 4), L::kQAtom,
-                        L::kKVAtom);
-        umma_commit(&s_full[buf]);
-        umma_commit(&k_empty[st]);
-      }
-      __syncwarp();
-      if (j >= 1 && !pv_step(j - 1)) {
-        ok = false;
-        break;
-      }
-    }
-    if (ok && !pv_step(nkv - 1)) ok = false;
-    if (!ok) {
-      if (elect_one()) umma_commit(drain);
-      __syncwarp();
-      mbar_wait_drain(drain, 0u, args.ctl);
-    }
-  } else if (warp < kSoftWarps) {
-    // ------------------------------------------------------------------ softmax / correction / epilogue
-    const uint32_t lane_base = tmem_base + (uint32_t((warp & 3) * 32) << 16);
-    const uint32_t o_addr = lane_base + uint32_t(L::kOCol);
-    float* s_mask = reinterpret_cast<float*>(smem + L::kMaskOff) + warp * kHalf;
-    float* s_max = reinterpret_cast<float*>(smem + L::kMaxOff);
-    float run_max = -INFINITY, run_sum = 0.0f;
-    bool ok = true;
-    for (int j = 0; j < nkv; ++j) {
-      const int buf = j & 1;
-      const int kv0 = (first + j) * BN;
-      MaskAhead ahead;
-      if constexpr (SCORES) request_mask(m, w, kv0 + half * kHalf, lane, ahead);
-      if (ok && !mbar_wait_bounded_warp(&s_full[buf], uint32_t(j >> 1) & 1u, abort_flag, args.ctl,
-                                        kStatusTimeoutEpilogue))
-        ok = false;
-      if (!ok) {  // aborted: the other warp of the rows may still come to this step's barrier
-        if (!hidden_tile(w, kv0)) named_barrier_sync(1 + (row >> 5), 64);
-        continue;
-      }
-      tc_fence_after();
-      bool move;
-      const float alpha =
-          masked_softmax_step<SCORES>(m, w, lane_base + uint32_t(buf * BN), kv0, half, row, lane, ahead, s_table, s_mask,
-                                      s_max + buf * 2 * kAttnBM, run_max, run_sum, move);
-      if (j > 0 && __any_sync(0xffffffffu, move)) {
-        if (!mbar_wait_bounded_warp(&pv_done[(j - 1) & 1], uint32_t((j - 1) >> 1) & 1u, abort_flag, args.ctl,
-                                    kStatusTimeoutEpilogue)) {
-          ok = false;
-          continue;
-        }
-        tc_fence_after();
-#pragma unroll 1
-        for (int c = half == 0 ? 0 : O::kFirst; c < (half == 0 ? O::kFirst : DP); c += 16)
-          rescale_o_row<16>(o_addr + uint32_t(c), alpha);
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[buf]);
-    }
-    if (ok && nkv > 0)
-      ok = mbar_wait_bounded_warp(&pv_done[(nkv - 1) & 1], uint32_t((nkv - 1) >> 1) & 1u, abort_flag, args.ctl,
-                                  kStatusTimeoutEpilogue);
-    // The row's sum is both halves'. (Aborted warps take the barrier, too.)
-    float* s_sum = s_max + (nkv & 1) * 2 * kAttnBM;
-    s_sum[half * kAttnBM + row] = run_sum;
-    named_barrier_sync(1 + (row >> 5), 64);
-    if (ok && __any_sync(0xffffffffu, w.valid)) {
-      tc_fence_after();
-      run_sum += s_sum[(half ^ 1) * kAttnBM + row];
-      const bool empty = run_max == -INFINITY;       // the row has seen no key
-      const bool wide = m.splits > 1 || args.out_f32;  // f32 rows
-      const int esz = wide ? 4 : 2;
-      const int begin = half == 0 ? 0 : O::kFirst;
-      const int cols = min(args.D - begin, half == 0 ? O::kFirst : O::kSecond);  // this warp's, maybe none
-      const long long obase =
-          (long long)bb * args.o_sb + (long long)w.i * args.o_ss + (long long)w.head * args.o_sh + begin;
-      uint8_t* stage = smem + warp * 32 * ((O::kFirst * esz / 16) | 1) * 16;
-      uint8_t* dst = nullptr;
-      if (m.splits > 1) {
-        const long long at = (((long long)split * m.pairs + pair) * m.tiles + tile) * kAttnBM + row;
-        if (w.valid && half == 0) m.part_ml[at] = make_float2(run_max, empty ? 0.0f : run_sum);
-        if (w.valid && !empty) dst = reinterpret_cast<uint8_t*>(m.part_o + at * args.D + begin);
-      } else if (w.valid) {
-        dst = static_cast<uint8_t*>(args.out) + obase * esz;
-      }
-      const float inv = m.splits > 1 ? 1.0f : 1.0f / run_sum;
-      if (cols <= 0) {
-        // nothing of the true head dim in this half
-      } else if (nkv > 0 && (m.splits > 1 || m.out_vec)) {
-        store_rows(o_addr + uint32_t(begin), stage, cols, wide, dst, inv, empty, lane);
-      } else if (m.splits == 1) {
-        // Output rows that 16-byte words do not reach, and tiles whose rows see nothing at all.
-        for (int c = 0; c < cols; c += 8) {
-          float o[8] = {};
-          if (nkv > 0) {
-            uint32_t r[8];
-            tmem_ld8(o_addr + uint32_t(begin + c), r);
-            tmem_wait_ld();
-#pragma unroll
-            for (int t = 0; t < 8; ++t) o[t] = empty ? 0.0f : __uint_as_float(r[t]) * inv;
-          }
-          if (w.valid) {
-#pragma unroll
-            for (int t = 0; t < 8; ++t) {
-              if (wide)
-                reinterpret_cast<float*>(dst)[c + t] = o[t];
-              else
-                reinterpret_cast<__nv_bfloat16*>(dst)[c + t] = __float2bfloat16_rn(o[t]);
-            }
-          }
-        }
-      }
-    }
-    tc_fence_before();
-  }
-
-  __syncthreads();
-  if (warp == kMmaWarp) {
-    tc_fence_after();
-    tmem_dealloc(tmem_base, L::kTmemCols);
-  }
-}
-
-// Joins the split parts of a row: with M = max of the parts' maxima, o = sum_z 2^(m_z - M) O_z / sum_z 2^(m_z - M) l_z in
-// part order. One warp per row; a few KB per row from L2.
-__global__ void __launch_bounds__(128) attention_join_kernel(const __grid_constant__ MaskedArgs m, int rows) {
+template <int WARPS>
+__global__ void __launch_bounds__(32 * kJoinBlockWarps)
+    attention_join_kernel(const __grid_constant__ MaskedArgs m, int rows) {
+  constexpr int kJoinWarps = WARPS;
+  __shared__ float s_acc[WARPS][256];
   pdl_launch_dependents();
   pdl_wait();
   const AttnArgs& args = m.a;
-  const int lane = threadIdx.x & 31;
-  const int row = int(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (row >= rows) return;
+  const int lane = threadIdx.x & 31, warp = WARPS > 1 ? int(threadIdx.x >> 5) : 0;
+  const int out_row = WARPS > 1 ? int(blockIdx.x) : int(blockIdx.x) * kJoinBlockWarps + int(threadIdx.x >> 5);
+  if (out_row >= rows) return;  // (whole warps, and only where they share nothing)
   // rows run (b, i, h), h fastest
-  const int h = row % args.H;
-  const int i = row / args.H % args.Sq;
-  const int b = row / args.H / args.Sq;
-  const int groups = args.H / m.pack;
+  const int h = out_row % args.H;
+  const int bi = out_row / args.H;
+  const int b = bi / args.Sq, i = bi - b * args.Sq;
   const int g = h % m.pack;
   const int tile = i / m.T, s = i - tile * m.T;
   const int r = m.head_fast ? s * m.pack + g : g * m.T + s;
-  const long long at = (((long long)(b * groups + h / m.pack)) * m.tiles + tile) * kAttnBM + r;
+  const long long at = (((long long)(b * m.groups + h / m.pack)) * m.tiles + tile) * kAttnBM + r;
   const long long step = (long long)m.pairs * m.tiles * kAttnBM;  // rows between parts
   float mz[2], lz[2];
-  float top = -INFINITY;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const int z = lane + 32 * k;
     const float2 ml = z < m.splits ? m.part_ml[at + z * step] : make_float2(-INFINITY, 0.0f);
     mz[k] = ml.x;
     lz[k] = ml.y;
-    top = fmaxf(top, ml.x);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const int c = lane * 8;  // this lane's columns
+  float acc[8] = {};
   float wz[2], sum = 0.0f;
+  for (int z0 = warp; z0 < m.splits; z0 += 8 * kJoinWarps) {
+    float4 v[8][2];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    wz[k] = mz[k] == -INFINITY ? 0.0f : fast_exp2(mz[k] - top);
-    sum += wz[k] * lz[k];
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-  const long long obase = (long long)b * args.o_sb + (long long)i * args.o_ss + (long long)h * args.o_sh;
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int c = half * 128 + lane * 4;
-    if (half * 128 >= args.D) break;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int z0 = 0; z0 < m.splits; z0 += 8) {  // eight parts' rows in flight
-      float4 v[8];
-      float wt[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int z = min(z0 + k, kMaxSplits - 1);
-        wt[k] = __shfl_sync(0xffffffffu, z < 32 ? wz[0] : wz[1], z & 31);  // 0 past the last part
-        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        // parts that saw nothing wrote no O
-        if (wt[k] != 0.0f && c < args.D && z0 + k < m.splits)
-          v[k] = *reinterpret_cast<const float4*>(m.part_o + (at + z * step) * args.D + c);
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        acc.x = fmaf(wt[k], v[k].x, acc.x);
-        acc.y = fmaf(wt[k], v[k].y, acc.y);
-        acc.z = fmaf(wt[k], v[k].z, acc.z);
-        acc.w = fmaf(wt[k], v[k].w, acc.w);
+    for (int k = 0; k < 8; ++k) {
+      const int z = z0 + k * kJoinWarps;
+      v[k][0] = v[k][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (z < m.splits && c < args.D) {
+        const float4* p = reinterpret_cast<const float4*>(m.part_o + (at + z * step) * args.D + c);
+        v[k][0] = p[0];
+        v[k][1] = p[1];
       }
     }
-    if (c < args.D) {
-      const float v[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
-      if (m.out_vec && args.out_f32) {
-        *reinterpret_cast<float4*>(static_cast<float*>(args.out) + obase + c) = make_float4(v[0], v[1], v[2], v[3]);
-      } else if (m.out_vec) {
-        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(args.out) + obase + c) =
-            make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-      } else {
+    if (z0 == warp) {
+      float top = fmaxf(mz[0], mz[1]);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          if (args.out_f32)
-            static_cast<float*>(args.out)[obase + c + t] = v[t];
-          else
-            static_cast<__nv_bfloat16*>(args.out)[obase + c + t] = __float2bfloat16_rn(v[t]);
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll
+      for (int k = 0; k < 2; ++k) wz[k] = mz[k] == -INFINITY ? 0.0f : fast_exp2(mz[k] - top);
+      sum = fmaf(wz[0], lz[0], wz[1] * lz[1]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int z = z0 + k * kJoinWarps;
+      const float wt = z < m.splits ? __shfl_sync(0xffffffffu, z < 32 ? wz[0] : wz[1], z & 31) : 0.0f;
+      if (wt != 0.0f) {  // a part that saw nothing wrote no O: whatever was read there is dropped
+        const float* e = &v[k][0].x;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) acc[t] = fmaf(wt, e[t], acc[t]);
+      }
+    }
+  }
+  const long long obase = (long long)b * args.o_sb + (long long)i * args.o_ss + (long long)h * args.o_sh;
+  if constexpr (WARPS == 1) {
+    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    if (c < args.D) {
+#pragma unroll
+      for (int t = 0; t < 8; ++t) acc[t] *= inv;
+      if (args.out_f32) {
+        float* dst = static_cast<float*>(args.out) + obase + c;
+        if (m.out_vec) {
+          reinterpret_cast<float4*>(dst)[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+          reinterpret_cast<float4*>(dst)[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+        } else {
+#pragma unroll
+          for (int t = 0; t < 8; ++t) dst[t] = acc[t];
         }
+      } else {
+        __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(args.out) + obase + c;
+        if (m.out_vec) {
+          *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]),
+                                                      pack_bf16x2(acc[4], acc[5]), pack_bf16x2(acc[6], acc[7]));
+        } else {
+#pragma unroll
+          for (int t = 0; t < 8; ++t) dst[t] = __float2bfloat16_rn(acc[t]);
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int t = 0; t < 8; ++t) s_acc[warp][c + t] = acc[t];
+    __syncthreads();
+    // (a warp without a part has no sum: warp 0 always has one)
+    __shared__ float s_inv;
+    if (threadIdx.x == 0) s_inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    __syncthreads();
+    const int col = int(threadIdx.x) * 2;
+    if (col < args.D) {
+      float o[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        float x = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kJoinWarps; ++k) x += s_acc[k][col + t];
+        o[t] = x * s_inv;
+      }
+      if (args.out_f32) {
+        float* dst = static_cast<float*>(args.out) + obase + col;
+        dst[0] = o[0];
+        dst[1] = o[1];
+      } else if (m.out_vec) {
+        *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(args.out) + obase + col) = pack_bf16x2(o[0], o[1]);
+      } else {
+        __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(args.out) + obase + col;
+        dst[0] = __float2bfloat16_rn(o[0]);
+        dst[1] = __float2bfloat16_rn(o[1]);
       }
     }
   }
@@ -924,8 +193,11 @@ int plan_masked(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Skv, int64
     p.splits = variant;
   } else if (2 * ctas <= slots && key_tiles >= 8) {
     // Fill the slots; several waves where the parts stay long (32 tiles at one wave), which evens out ragged lengths.
+    // With many rows the partial results are worth their traffic only in parts of at least 16 tiles (16384 rows of 1024
+    // keys: 30 us whole, 33 us in two parts).
     const int64_t want = key_tiles * ctas >= 32 * slots ? 5 * slots / (2 * ctas) : slots / ctas;
-    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>({want, key_tiles, kMaxSplits}));
+    const int64_t most = B * H * Sq <= kJoinFewRows ? key_tiles : key_tiles / 16;
+    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>({want, most, kMaxSplits}));
     const int64_t per = (key_tiles + parts - 1) / parts;
     p.splits = int((key_tiles + per - 1) / per);
   }
@@ -938,40 +210,6 @@ int plan_masked(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Skv, int64
   }
   *out = p;
   return kOk;
-}
-
-template <int DP, int STAGES, bool SCORES>
-int launch_masked(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const MaskedArgs& m, dim3 grid,
-                  cudaStream_t st, int device) {
-  static bool configured[64] = {false};
-  auto kern = attention_masked_tcgen05_kernel<DP, STAGES, SCORES>;
-  using L = MaskedLayout<DP, STAGES>;
-  static_assert(L::kSmemBytes + kTableSmemMax <= (L::kTwoPerSm ? 113 * 1024 : 232448), "room for the distance bias");
-  const int smem = L::kSmemBytes + (m.table_smem ? (2 * (m.max_dist + kTableMargin) + 1) * 4 : 0);
-  if (!configured[device]) {
-    if (int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 L::kSmemBytes + kTableSmemMax),
-                            "cudaFuncSetAttribute(masked attention smem)"))
-      return rc;
-    configured[device] = true;
-  }
-  return check_cuda(launch_pdl(kern, grid, dim3(kMaskedThreads), smem, st, mq, mk, mv, m),
-                    "masked attention kernel launch");
-}
-
-template <bool SCORES>
-int launch_masked_for(int64_t D, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
-                      const MaskedArgs& m, dim3 grid, cudaStream_t st, int dev) {
-  // The padded head dims with a kernel; the columns between D and its pad are TMA zeros.
-  if (D <= 32) return launch_masked<32, 5, SCORES>(mq, mk, mv, m, grid, st, dev);
-  if (D <= 48) return launch_masked<48, 5, SCORES>(mq, mk, mv, m, grid, st, dev);
-  if (D <= 64) return launch_masked<64, 5, SCORES>(mq, mk, mv, m, grid, st, dev);
-  if (D <= 80) return launch_masked<80, 2, SCORES>(mq, mk, mv, m, grid, st, dev);
-  if (D <= 96) return launch_masked<96, 2, SCORES>(mq, mk, mv, m, grid, st, dev);
-  if (D <= 128) return launch_masked<128, 2, SCORES>(mq, mk, mv, m, grid, st, dev);
-  if (D <= 160) return launch_masked<160, 2, SCORES>(mq, mk, mv, m, grid, st, dev);
-  if (D <= 192) return launch_masked<192, 2, SCORES>(mq, mk, mv, m, grid, st, dev);
-  return launch_masked<256, 2, SCORES>(mq, mk, mv, m, grid, st, dev);
 }
 
 }  // namespace
@@ -1093,13 +331,20 @@ int attention_masked_launch(const AttnMaskedProblem& mp, cudaStream_t stream) {
     m.mask_row = (o.mask_sq == 0 || p.Sq == 1) && (o.mask_sh == 0 || m.pack == 1);
   }
   const dim3 grid{unsigned(plan.pairs), unsigned(plan.tiles), unsigned(plan.splits)};
-  const bool scores = o.softcap > 0.0f || o.slopes != nullptr || o.distance_bias != nullptr || o.mask != nullptr;
-  if (int rc = scores ? launch_masked_for<true>(p.D, mq, mk, mv, m, grid, stream, dev->device)
-                      : launch_masked_for<false>(p.D, mq, mk, mv, m, grid, stream, dev->device))
-    return rc;
+  const int feats = (o.softcap > 0.0f ? kFeatCap : 0) | (o.slopes || o.distance_bias ? kFeatDistance : 0) |
+                    (o.mask ? kFeatMask : 0);
+  auto launch = feats == 0               ? launch_masked_for<0>
+                : feats == kFeatCap      ? launch_masked_for<kFeatCap>
+                : feats == kFeatDistance ? launch_masked_for<kFeatDistance>
+                : feats == kFeatMask     ? launch_masked_for<kFeatMask>
+                                         : launch_masked_for<kFeatAny>;
+  if (int rc = launch(p.D, mq, mk, mv, m, grid, stream, dev->device)) return rc;
   if (plan.splits == 1) return kOk;
-  const int64_t rows = p.B * p.H * p.Sq;
-  return check_cuda(launch_pdl(attention_join_kernel, dim3(unsigned((rows + 3) / 4)), dim3(128), 0, stream, m, int(rows)),
+  const int rows = int(p.B * p.H * p.Sq);
+  const bool few = rows <= kJoinFewRows;
+  return check_cuda(launch_pdl(few ? attention_join_kernel<4> : attention_join_kernel<1>,
+                               dim3(unsigned(few ? rows : (rows + kJoinBlockWarps - 1) / kJoinBlockWarps)),
+                               dim3(32 * kJoinBlockWarps), 0, stream, m, rows),
                     "attention join kernel launch");
 }
 

@@ -112,25 +112,23 @@ bool tma_rows_ok(const void* p, int64_t ld, int64_t cols) { return aligned16(p) 
 
 int64_t round_up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
-// Workspace layout: [4 KiB reserved][split bytes the plan reports][repacked x][repacked W]. Split K reduces inside a
-// cluster's shared memory, so plans report no split bytes and the workspace holds only operands that TMA cannot
-// read as given, repacked; the leading region stays reserved so the layout does not depend on the plan.
+// Workspace layout: [4 KiB reserved][repacked x][repacked W]. Split K reduces inside a cluster's shared memory, so the
+// workspace holds only operands that TMA cannot read as given, repacked, whatever the launch plan (which is not worked
+// out here: it took 1.3 us of every call).
 constexpr size_t kCounterRegion = 4096;
 struct WsLayout {
-  size_t split_bytes = 0;
   size_t x_off = 0, x_bytes = 0;
   size_t w_off = 0, w_bytes = 0;
   size_t total = 0;
 };
 
 WsLayout gemm_ws_layout(const void* x, int64_t ldx, int64_t m, int64_t k, const void* w, int64_t ldw, int64_t n,
-                        int variant, int sms, int geglu = 0) {
+                        int geglu = 0) {
   WsLayout L;
   const int64_t kp = round_up(k, 8);
   const bool pad_k = (k % 8) != 0;
   const int64_t w_rows = geglu ? 2 * n : n;
-  L.split_bytes = (sms > 0 && !geglu) ? gemm_plan(m, n, kp, sms, variant).split_ws_bytes : 0;  // counters + partials
-  size_t off = L.split_bytes > 0 ? L.split_bytes : kCounterRegion;
+  size_t off = kCounterRegion;
   if (pad_k || !tma_rows_ok(x, ldx, k)) {
     L.x_off = off;
     L.x_bytes = size_t(round_up(m * kp * 2, 256));
@@ -141,7 +139,7 @@ WsLayout gemm_ws_layout(const void* x, int64_t ldx, int64_t m, int64_t k, const 
     L.w_bytes = size_t(round_up(w_rows * kp * 2, 256));
     off += L.w_bytes;
   }
-  L.total = (L.split_bytes > 0 || L.x_bytes > 0 || L.w_bytes > 0) ? off : 0;
+  L.total = (L.x_bytes > 0 || L.w_bytes > 0) ? off : 0;
   return L;
 }
 
@@ -165,7 +163,9 @@ namespace npub200 {
 
 size_t gemm_workspace_bytes(const void* x, int64_t ldx, int64_t m, int64_t k, const void* w, int64_t ldw, int64_t n,
                             int variant, int sms, int geglu) {
-  return gemm_ws_layout(x, ldx, m, k, w, ldw, n, variant, sms, geglu).total;
+  (void)variant;
+  (void)sms;
+  return gemm_ws_layout(x, ldx, m, k, w, ldw, n, geglu).total;
 }
 
 int gemm_with_workspace(const void* x, int64_t ldx, int64_t m, int64_t k, const void* w, int64_t ldw, int64_t n,
@@ -206,7 +206,7 @@ int gemm_with_workspace(const void* x, int64_t ldx, int64_t m, int64_t k, const 
   const bool pad_k = (k % 8) != 0;
   const bool x_ok = !pad_k && tma_rows_ok(x, ldx, k);
   const bool w_ok = !pad_k && tma_rows_ok(w, ldw, k);
-  const WsLayout L = gemm_ws_layout(x, ldx, m, k, w_map ? nullptr : w, ldw, n, variant, dev->sms, geglu);
+  const WsLayout L = gemm_ws_layout(x, ldx, m, k, w_map ? nullptr : w, ldw, n, geglu);
   if (workspace != nullptr && !aligned16(workspace)) return fail(kErrInvalid, "workspace must be 16-byte aligned");
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const int64_t kp = round_up(k, 8);
@@ -227,11 +227,6 @@ int gemm_with_workspace(const void* x, int64_t ldx, int64_t m, int64_t k, const 
       p.w_map_cache = nullptr;
     }
     if (pad_k) p.K = kp;
-  }
-  // Split-K bytes the plan asked for (none: split K reduces inside a cluster).
-  if (ws != nullptr && L.split_bytes > 0 && workspace_bytes >= L.split_bytes) {
-    p.ws_split = ws;
-    p.ws_split_bytes = L.split_bytes;
   }
   return gemm_launch(p, st);
 }
@@ -297,7 +292,7 @@ int npub200_gemm_workspace_size(const void* x, int64_t ldx, int64_t m, int64_t k
   if (m <= 0 || k <= 0 || n <= 0) return fail(kErrInvalid, "GEMM sizes must be positive");
   const DeviceInfo* d = nullptr;
   if (int rc = current_device_info(&d)) return rc;
-  *bytes_out = gemm_ws_layout(x, ldx, m, k, w, ldw, n, variant, d->sms).total;
+  *bytes_out = gemm_ws_layout(x, ldx, m, k, w, ldw, n).total;
   return kOk;
 }
 

@@ -90,7 +90,8 @@ at::Tensor gemm(const at::Tensor& x, const at::Tensor& w, const std::optional<at
     check_rc(npub200_gemm_workspace_size(x.data_ptr(), x.stride(0), M, K, w.data_ptr(), w.stride(0), N,
                                          int(variant), &ws_bytes),
              "npub200::gemm");
-    at::Tensor ws = at::empty({int64_t(ws_bytes)}, x.options().dtype(at::kByte));
+    at::Tensor ws;
+    if (ws_bytes) ws = at::empty({int64_t(ws_bytes)}, x.options().dtype(at::kByte));
     void* ws_ptr = ws_bytes ? ws.data_ptr() : nullptr;
     if (activation != 0)
       check_rc(npub200_gemm_act(x.data_ptr(), x.stride(0), M, K, w.data_ptr(), w.stride(0), N, b_ptr, b_code,
@@ -108,7 +109,8 @@ at::Tensor gemm(const at::Tensor& x, const at::Tensor& w, const std::optional<at
   check_rc(npub200_gemm_workspace_size(x.data_ptr(), x.stride(0), M, K, weight_handle ? nullptr : w.data_ptr(),
                                        w.stride(0), N, int(variant), &ws_bytes),
            "npub200::gemm");
-  at::Tensor ws = at::empty({int64_t(ws_bytes)}, x.options().dtype(at::kByte));
+  at::Tensor ws;
+  if (ws_bytes) ws = at::empty({int64_t(ws_bytes)}, x.options().dtype(at::kByte));
   void* ws_ptr = ws_bytes ? ws.data_ptr() : nullptr;
   if (weight_handle != 0) {
     check_rc(npub200_gemm_w(x.data_ptr(), x.stride(0), M, K, weight_handle, b_ptr, b_code, y.data_ptr(), y.stride(0),
@@ -196,11 +198,14 @@ const T* vector_ptr(const std::optional<at::Tensor>& t, const at::Tensor& q, int
   return static_cast<const T*>(t->data_ptr());
 }
 
-// Attention with masks, score modifiers and grouped key/value heads (npub200_attention_masked) into `out`: (B, S, H*d)
-// tensors, or (B, H, S, d) when head-major. The workspace of split keys comes from torch's allocator, one per call.
-at::Tensor attention_masked(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& out,
+// Attention with masks, score modifiers and grouped key/value heads (npub200_attention_masked): (B, S, H*d) tensors, or
+// (B, H, S, d) when head-major. Defaults: kv_heads 0 what k's shape says, scale <= 0 d^-0.5, no q_start the last query at
+// the last key, softcap 0 none. The workspace of split keys comes from torch's allocator, one per call.
+at::Tensor attention_masked(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                            const std::optional<at::Tensor>& out_arg, std::optional<at::ScalarType> out_dtype,
                             int64_t heads, int64_t kv_heads, bool head_major_in, bool head_major_out, double scale,
-                            int64_t variant, bool causal, int64_t q_start, const std::optional<at::Tensor>& q_starts,
+                            int64_t variant, bool causal, std::optional<int64_t> q_start,
+                            const std::optional<at::Tensor>& q_starts,
                             int64_t prefix, const std::optional<at::Tensor>& prefixes,
                             const std::optional<at::Tensor>& kv_lens, const std::optional<at::Tensor>& doc_offsets,
                             double softcap, const std::optional<at::Tensor>& slopes,
@@ -208,20 +213,40 @@ at::Tensor attention_masked(const at::Tensor& q, const at::Tensor& k, const at::
   check_operand(q, q, "q");
   check_operand(k, q, "k");
   check_operand(v, q, "v");
-  TORCH_CHECK_VALUE(heads > 0 && kv_heads > 0, "head counts must be positive");
-  TORCH_CHECK_VALUE(q.dim() == (head_major_in ? 4 : 3) && k.dim() == q.dim(), "attention operands have the wrong rank");
-  TORCH_CHECK_VALUE(head_major_in || q.size(2) % heads == 0, "q's last dimension is not a multiple of heads");
+  TORCH_CHECK_VALUE(q.dim() == (head_major_in ? 4 : 3) && k.dim() == q.dim() && v.dim() == q.dim(),
+                    "attention operands must be ", head_major_in ? "(B, H, S, d)" : "(B, S, H*d)");
+  TORCH_CHECK_VALUE(heads > 0 && (head_major_in || q.size(2) % heads == 0), "q's last dimension is not a multiple of heads=",
+                    heads);
   const int64_t B = q.size(0), Sq = q.size(head_major_in ? 2 : 1), Skv = k.size(head_major_in ? 2 : 1);
   const int64_t d = head_major_in ? q.size(3) : q.size(2) / heads;
+  const int64_t Hk = head_major_in ? k.size(1) : (d > 0 && k.size(2) % d == 0 ? k.size(2) / d : 0);
+  TORCH_CHECK_VALUE(Hk > 0 && heads % Hk == 0 && (kv_heads <= 0 || kv_heads == Hk), "k/v hold ", Hk,
+                    " heads: kv_heads must be that, and a divisor of heads=", heads, " (got ", kv_heads, ")");
+  kv_heads = Hk;
+  TORCH_CHECK_VALUE(k.size(0) == B && k.size(-1) == (head_major_in ? d : Hk * d) && v.sizes() == k.sizes(), "k/v shapes ",
+                    k.sizes(), ", ", v.sizes(), " do not match q's ", q.sizes());
   check_layout(q, head_major_in, B, heads, Sq, d, 0, "q");
   check_layout(k, head_major_in, B, kv_heads, Skv, d, 0, "k");
   check_layout(v, head_major_in, B, kv_heads, Skv, d, 0, "v");
-  check_layout(out, head_major_out, B, heads, Sq, d, 0, "out");
-  TORCH_CHECK_VALUE(out.is_cuda() && out.device() == q.device() && out.stride(-1) == 1,
-                    "out must be a CUDA tensor on q's device with a contiguous last dimension");
+  const c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor out;
+  if (out_arg.has_value()) {
+    out = *out_arg;
+    check_layout(out, head_major_out, B, heads, Sq, d, 0, "attention output");
+    TORCH_CHECK_VALUE(out.is_cuda() && out.device() == q.device() && out.stride(-1) == 1,
+                      "attention output must be a CUDA tensor on q's device with a contiguous last dimension");
+  } else {
+    const auto opts = q.options().dtype(out_dtype.value_or(at::kFloat));
+    out = head_major_out ? at::empty({B, heads, Sq, d}, opts) : at::empty({B, Sq, heads * d}, opts);
+  }
+  const int out_code = dtype_code(out, "attention output");
+  if (scale <= 0) {
+    TORCH_CHECK_VALUE(scale == 0, "attention scale must be positive (got ", scale, ")");
+    scale = 1.0 / std::sqrt(double(d));
+  }
   npub200_attention_mods m = {};
   m.causal = causal ? 1 : 0;
-  m.q_start = q_start;
+  m.q_start = q_start.value_or(Skv - Sq);
   m.q_starts = vector_ptr<int32_t>(q_starts, q, B, "q_starts");
   m.prefix = prefix;
   m.prefixes = vector_ptr<int32_t>(prefixes, q, B, "prefixes");
@@ -247,17 +272,21 @@ at::Tensor attention_masked(const at::Tensor& q, const at::Tensor& k, const at::
   }
   if (mask.has_value()) {
     const at::Tensor& t = *mask;
-    TORCH_CHECK_VALUE(t.is_cuda() && t.device() == q.device() && t.dim() == 4 && (t.size(0) == 1 || t.size(0) == B) &&
-                          (t.size(1) == 1 || t.size(1) == heads) && (t.size(2) == 1 || t.size(2) == Sq) &&
-                          t.size(3) == Skv && (Skv == 1 || t.stride(3) == 1),
-                      "mask must be a 4-D tensor on q's device that broadcasts to (B, heads, Sq, Skv), keys contiguous");
+    TORCH_CHECK_VALUE(t.is_cuda() && t.device() == q.device() && (t.dim() == 4 || t.dim() == 2),
+                      "mask must be a tensor of 2 or 4 dimensions on q's device");
+    const int64_t off = t.dim() - 4;  // a 2-D mask is [Sq, Skv]
+    const auto size = [&](int64_t i) { return i + off < 0 ? int64_t(1) : t.size(i + off); };
+    const auto stride = [&](int64_t i) { return size(i) > 1 ? t.stride(i + off) : int64_t(0); };
+    TORCH_CHECK_VALUE((size(0) == 1 || size(0) == B) && (size(1) == 1 || size(1) == heads) &&
+                          (size(2) == 1 || size(2) == Sq) && size(3) == Skv && (Skv == 1 || t.stride(-1) == 1),
+                      "mask ", t.sizes(), " does not broadcast to (", B, ", ", heads, ", ", Sq, ", ", Skv,
+                      ") with contiguous keys");
     m.mask = t.data_ptr();
     m.mask_dtype = t.scalar_type() == at::kBool ? NPUB200_DTYPE_BOOL : dtype_code(t, "mask");
-    m.mask_sb = t.size(0) > 1 ? t.stride(0) : 0;
-    m.mask_sh = t.size(1) > 1 ? t.stride(1) : 0;
-    m.mask_sq = t.size(2) > 1 ? t.stride(2) : 0;
+    m.mask_sb = stride(0);
+    m.mask_sh = stride(1);
+    m.mask_sq = stride(2);
   }
-  const c10::cuda::CUDAGuard guard(q.device());
   size_t ws_bytes = 0;
   check_rc(npub200_attention_masked_workspace_size(B, heads, kv_heads, Sq, Skv, d, int(variant), &ws_bytes),
            "npub200::attention_masked");
@@ -269,7 +298,7 @@ at::Tensor attention_masked(const at::Tensor& q, const at::Tensor& k, const at::
   bsh_strides(v, head_major_in, d, &vs[0], &vs[1], &vs[2]);
   bsh_strides(out, head_major_out, d, &os[0], &os[1], &os[2]);
   check_rc(npub200_attention_masked(q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(),
-                                    vs[0], vs[1], vs[2], out.data_ptr(), os[0], os[1], os[2], dtype_code(out, "out"), B,
+                                    vs[0], vs[1], vs[2], out.data_ptr(), os[0], os[1], os[2], out_code, B,
                                     heads, kv_heads, Sq, Skv, d, float(scale), &m, ws_bytes ? ws.data_ptr() : nullptr,
                                     ws_bytes, int(variant), stream_of(q)),
            "npub200::attention_masked");
@@ -284,10 +313,11 @@ TORCH_LIBRARY(npub200, m) {
   m.def("attention(Tensor q, Tensor k, Tensor v, Tensor? out, int B, int H, int Sq, int Skv, int d, "
         "int q_row_stride, int kv_row_stride, int o_row_stride, bool head_major_in, bool head_major_out, "
         "float scale, int variant, ScalarType? out_dtype=None) -> Tensor");
-  m.def("attention_masked(Tensor q, Tensor k, Tensor v, Tensor(a!) out, int heads, int kv_heads, bool head_major_in, "
-        "bool head_major_out, float scale, int variant, bool causal, int q_start, Tensor? q_starts, int prefix, "
-        "Tensor? prefixes, Tensor? kv_lens, Tensor? doc_offsets, float softcap, Tensor? slopes, Tensor? distance_bias, "
-        "Tensor? mask) -> Tensor(a!)");
+  m.def("attention_masked(Tensor q, Tensor k, Tensor v, Tensor? out, ScalarType? out_dtype, int heads, int kv_heads=0, "
+        "bool head_major_in=False, bool head_major_out=False, float scale=0., int variant=0, bool causal=False, "
+        "int? q_start=None, Tensor? q_starts=None, int prefix=0, Tensor? prefixes=None, Tensor? kv_lens=None, "
+        "Tensor? doc_offsets=None, float softcap=0., Tensor? slopes=None, Tensor? distance_bias=None, "
+        "Tensor? mask=None) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(npub200, CUDA, m) {

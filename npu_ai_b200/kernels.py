@@ -112,9 +112,13 @@ def gemm(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, out
     N, K2 = w.shape
     if K != K2:
         raise AssertionError(f"K mismatch: x has {K}, weight has {K2}")
+    ops = _lib.torch_ops()
     if out is None:
-        out = torch.empty((M, N), dtype=out_dtype, device=x.device)
-    if out.dtype not in _DT or out.stride(1) != 1 or tuple(out.shape) != (M, N):
+        if out_dtype not in _DT:
+            raise ValueError("out must be an [M, N] bf16/f32 matrix with contiguous rows")
+        if ops is None:
+            out = torch.empty((M, N), dtype=out_dtype, device=x.device)
+    elif out.dtype not in _DT or out.stride(1) != 1 or tuple(out.shape) != (M, N):
         raise ValueError("out must be an [M, N] bf16/f32 matrix with contiguous rows")
     if bias is not None:
         if bias.dtype not in _DT or bias.numel() != N or not bias.is_contiguous():
@@ -130,9 +134,8 @@ def gemm(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, out
         if not act:
             raise ValueError(f"unknown activation {activation!r} (one of {', '.join(_lib.ACTIVATIONS)})")
         handle = None  # and so does the activation's
-    ops = _lib.torch_ops()
     if ops is not None:
-        return ops.gemm(x, w, bias, out, int(variant), None, int(handle or 0), residual, act)
+        return ops.gemm(x, w, bias, out, int(variant), out_dtype, int(handle or 0), residual, act)
     ws = _gemm_workspace(x, None if handle is not None else w, M, K, N, variant)
     args_tail = (ctypes.c_void_p(bias.data_ptr()) if bias is not None else None,
                  _DT[bias.dtype] if bias is not None else _lib.DTYPE_BF16,
@@ -461,6 +464,22 @@ def _per_batch(t, name: str, B: int, device: torch.device, dtype: torch.dtype = 
 
 def _attention_masked(q, k, v, heads, scale, head_major_in, head_major_out, out_dtype, out, variant, kv_heads, causal,
                       q_start, prefix_len, kv_lens, doc_offsets, softcap, slopes, distance_bias, mask):
+    ops = _lib.torch_ops()
+    if ops is not None:  # the operator checks every tensor itself
+        if not (q.is_cuda and k.is_cuda and v.is_cuda):
+            raise ValueError(f"q, k and v must be CUDA tensors (got {q.device}, {k.device}, {v.device})")
+        starts = q_start if isinstance(q_start, torch.Tensor) else None
+        prefixes = prefix_len if isinstance(prefix_len, torch.Tensor) else None
+        if prefix_len is not None and not causal:
+            raise ValueError("prefix_len needs causal=True")
+        if softcap is not None and not 0.0 < softcap < 3e38:
+            raise ValueError(f"softcap must be positive and finite (got {softcap})")
+        if scale is not None and not scale > 0.0:
+            raise ValueError(f"attention scale must be positive (got {scale})")
+        return ops.attention_masked(q, k, v, out, out_dtype, heads, kv_heads or 0, head_major_in, head_major_out,
+                                    scale or 0.0, variant, causal, q_start if starts is None else None, starts,
+                                    prefix_len or 0 if prefixes is None else 0, prefixes, kv_lens, doc_offsets,
+                                    softcap or 0.0, slopes, distance_bias, mask)
     dims = 4 if head_major_in else 3
     dev = q.device
     for name, t in (("q", q), ("k", k), ("v", v)):
@@ -538,11 +557,6 @@ def _attention_masked(q, k, v, heads, scale, head_major_in, head_major_out, out_
         if any(n not in (1, m) for n, m in zip(mask.shape[:3], (B, H, Sq))) or mask.shape[3] != Skv or \
                 (Skv > 1 and mask.stride(3) != 1):
             raise ValueError(f"mask {tuple(mask.shape)} does not broadcast to {(B, H, Sq, Skv)} with contiguous keys")
-    ops = _lib.torch_ops()
-    if ops is not None:
-        return ops.attention_masked(q, k, v, out, H, Hk, head_major_in, head_major_out, scale, int(variant), causal,
-                                    start, starts, prefix, prefixes, kv_lens, doc_offsets, cap, slopes, distance_bias,
-                                    mask)
     mods = _lib.AttentionMods(causal=int(causal), q_start=start, prefix=prefix, softcap=cap)
     for name, t in (("q_starts", starts), ("prefixes", prefixes), ("kv_lens", kv_lens), ("doc_offsets", doc_offsets),
                     ("slopes", slopes), ("distance_bias", distance_bias), ("mask", mask)):
