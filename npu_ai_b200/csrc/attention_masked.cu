@@ -314,6 +314,7 @@ int attention_masked_launch(const AttnMaskedProblem& mp, cudaStream_t stream) {
   if (o.softcap > 0.0f) {
     m.cap_in = p.scale / o.softcap;
     m.cap_out = o.softcap * kLog2e;
+    for (int i = 0; i < 6; ++i) m.cap_poly[i] = m.cap_out * kTanhRatio[i];
   }
   m.slopes = o.slopes;
   m.table = o.distance_bias;

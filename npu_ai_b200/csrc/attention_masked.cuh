@@ -66,6 +66,7 @@ struct MaskedArgs {
   int ndocs;
   long long doc_stride;
   float cap_in, cap_out;  // capped score in log2 units = cap_out x tanh(cap_in x raw score)
+  float cap_poly[6];      // cap_out x kTanhRatio: operands straight from the constant bank
   const float* slopes;
   const float* table;
   int max_dist;
@@ -85,6 +86,10 @@ struct Row {
   bool valid;       // a row of the output
   int head, i, b;
   float slope;      // slopes[head] * log2 e
+  const uint8_t* mask;  // its mask row
+  // Over the warp's rows that see something (output rows for the positions): what a tile is to all of them is decided
+  // from these, without a vote.
+  int lo_min, lo_max, hi_min, hi_max, p_min, p_max;
 };
 
 __device__ __forceinline__ int clamp_pos(long long x) {
@@ -156,19 +161,21 @@ __device__ __forceinline__ Row row_of(const MaskedArgs& m, int r, int tile, int 
   const bool any = w.valid && hi > lo;  // a row that sees nothing leaves the union alone
   w.lo = any ? lo : 0;
   w.hi = any ? hi : 0;
+  w.lo_min = __reduce_min_sync(0xffffffffu, any ? lo : INT_MAX);
+  w.lo_max = __reduce_max_sync(0xffffffffu, any ? lo : 0);
+  w.hi_min = __reduce_min_sync(0xffffffffu, any ? hi : (w.valid ? 0 : INT_MAX));  // a row that sees nothing is masked
+  w.hi_max = __reduce_max_sync(0xffffffffu, any ? hi : 0);
+  w.p_min = __reduce_min_sync(0xffffffffu, w.valid ? w.p : INT_MAX);
+  w.p_max = __reduce_max_sync(0xffffffffu, w.valid ? w.p : -INT_MAX);
+  const int esz = m.mask_kind == 3 ? 4 : m.mask_kind;
+  w.mask = static_cast<const uint8_t*>(m.mask) +
+           ((long long)b * m.m_sb + (long long)w.head * m.m_sh + (long long)(w.valid ? w.i : 0) * m.m_sq) * esz;
   return w;
 }
 
-// tanh(y) / y as a polynomial in z = y^2, |y| <= 1 (fit_tanh_poly.py beside this file; relative error 7e-7). Scalar: its
-// constants are immediate operands, which the packed form has to keep or rebuild in register pairs.
-__device__ __forceinline__ float tanh_ratio(float z) {
-  float p = fmaf(-3.074449487e-03f, z, 1.676048711e-02f);
-  p = fmaf(p, z, -5.161965266e-02f);
-  p = fmaf(p, z, 1.328188479e-01f);
-  p = fmaf(p, z, -3.332909346e-01f);
-  p = fmaf(p, z, 9.999994040e-01f);
-  return p;
-}
+// tanh(y) / y as a polynomial in y^2, |y| <= 1 (fit_tanh_poly.py beside this file; relative error 7e-7).
+constexpr float kTanhRatio[6] = {9.999994040e-01f, -3.332909346e-01f, 1.328188479e-01f,
+                                 -5.161965266e-02f, 1.676048711e-02f, -3.074449487e-03f};
 
 // What a kernel instantiation does to the scores: nothing, one of these, or any of them as the arguments say. (One
 // kernel with every branch spent as long on instruction fetches as on the instructions.)
@@ -189,19 +196,21 @@ __device__ __forceinline__ bool has_mask(const MaskedArgs& m) {
 // A mask value in log2 units: -inf hides; any finite value, however low, stays finite.
 __device__ __forceinline__ float mask_log2(float e) { return e == -INFINITY ? e : fmaxf(e * kLog2e, -FLT_MAX); }
 
-// Element offset of this thread's mask row at key kv0.
-__device__ __forceinline__ long long mask_offset(const MaskedArgs& m, const Row& w, int kv0) {
-  return (long long)w.b * m.m_sb + (long long)w.head * m.m_sh + (long long)(w.valid ? w.i : 0) * m.m_sq + kv0;
+// All bits the sign bit of byte `i` (a constant) of x.
+__device__ __forceinline__ uint32_t replicate_sign(uint32_t x, uint32_t i) {
+  uint32_t r;
+  asm("prmt.b32 %0, %1, 0, %2;" : "=r"(r) : "r"(x), "r"(0x8888u + 0x1111u * i));
+  return r;
 }
 
 // One mask row for the warp: this lane's value, key kv0 + lane, in log2 units, requested before the wait for S.
 __device__ __forceinline__ float mask_row_value(const MaskedArgs& m, const Row& w, int kv0, int lane) {
   if (kv0 + lane >= m.a.Skv) return -INFINITY;
-  const long long at = mask_offset(m, w, kv0) + lane;
-  if (m.mask_kind == 1) return __ldg(static_cast<const uint8_t*>(m.mask) + at) != 0 ? 0.0f : -INFINITY;
+  const int at = kv0 + lane;
+  if (m.mask_kind == 1) return __ldg(w.mask + at) != 0 ? 0.0f : -INFINITY;
   if (m.mask_kind == 2)
-    return mask_log2(__uint_as_float(uint32_t(__ldg(static_cast<const unsigned short*>(m.mask) + at)) << 16));
-  return mask_log2(__ldg(static_cast<const float*>(m.mask) + at));
+    return mask_log2(__uint_as_float(uint32_t(__ldg(reinterpret_cast<const unsigned short*>(w.mask) + at)) << 16));
+  return mask_log2(__ldg(reinterpret_cast<const float*>(w.mask) + at));
 }
 
 // Rows of their own: the next tile's part of this thread's row into L1 while this tile is worked on (kHalf values of
@@ -209,7 +218,7 @@ __device__ __forceinline__ float mask_row_value(const MaskedArgs& m, const Row& 
 __device__ __forceinline__ void prefetch_mask(const MaskedArgs& m, const Row& w, int kv0) {
   if (kv0 + kHalf > m.a.Skv) return;
   const int esz = m.mask_kind == 3 ? 4 : m.mask_kind;
-  const uint8_t* p = static_cast<const uint8_t*>(m.mask) + mask_offset(m, w, kv0) * esz;
+  const uint8_t* p = w.mask + (long long)kv0 * esz;
   for (int k = 0; k < esz; ++k) asm volatile("prefetch.global.L1 [%0];" ::"l"(p + 32 * k));
 }
 
@@ -221,31 +230,32 @@ __device__ __forceinline__ float modify_scores(const MaskedArgs& m, const Row& w
                                                const float* s_table, float* s_mask, int lane, float (&s)[BN]) {
   float k = m.a.scale_log2;
   if (has_cap<FEAT>(m)) {
-    // tanh(y) = 1 - 2 / (1 + e^(2y)) on the MUFU (its absolute error of a few 2^-23 is that small next to the cap), for
-    // every other score by the polynomial on the FMA pipe where all are small enough, the usual case.
-    const float e = 2.0f * kLog2e * m.cap_in;
     float big = 0.0f;
 #pragma unroll
-    for (int t = 0; t < BN; t += 4) big = fmax3(big, fabsf(s[t]), fabsf(s[t + 2]));
+    for (int t = 0; t < BN; t += 2) big = fmax3(big, fabsf(s[t]), fabsf(s[t + 1]));
     if (__all_sync(0xffffffffu, big * m.cap_in <= 1.0f)) {
+      // The usual case, on the FMA pipe (the MUFU has the softmax's exponentials to do): cap tanh(y) = y P(y^2).
 #pragma unroll
-      for (int t = 0; t < BN; t += 2) {
-        const float y = s[t] * m.cap_in;
-        s[t] = y * m.cap_out * tanh_ratio(y * y);
+      for (int t = 0; t < BN; ++t) {
+        const float y = s[t] * m.cap_in, z = y * y;
+        float p = fmaf(m.cap_poly[5], z, m.cap_poly[4]);
+        p = fmaf(p, z, m.cap_poly[3]);
+        p = fmaf(p, z, m.cap_poly[2]);
+        p = fmaf(p, z, m.cap_poly[1]);
+        p = fmaf(p, z, m.cap_poly[0]);
+        s[t] = y * p;
       }
     } else {
+      // tanh(y) = 1 - 2 / (1 + e^(2y)); the absolute error of a few 2^-23 stays that small next to the cap.
+      const float e = 2.0f * kLog2e * m.cap_in;
 #pragma unroll
-      for (int t = 0; t < BN; t += 2)
-        s[t] = fmaf(-2.0f * m.cap_out, fast_rcp(1.0f + fast_exp2(e * s[t])), m.cap_out);
+      for (int t = 0; t < BN; ++t) s[t] = fmaf(-2.0f * m.cap_out, fast_rcp(1.0f + fast_exp2(e * s[t])), m.cap_out);
     }
-#pragma unroll
-    for (int t = 1; t < BN; t += 2)
-      s[t] = fmaf(-2.0f * m.cap_out, fast_rcp(1.0f + fast_exp2(e * s[t])), m.cap_out);
     k = 1.0f;
   }
   if (has_distance<FEAT>(m) && m.slopes != nullptr) {
     const float rel = float(w.p - kv0);
-    if (__all_sync(0xffffffffu, !w.valid || w.p >= kv0 + BN - 1)) {  // all keys at or before their rows: linear in t
+    if (w.p_min >= kv0 + BN - 1) {  // all keys at or before their rows: linear in t
       const float base = -w.slope * rel;
 #pragma unroll
       for (int t = 0; t < BN; ++t) s[t] = fmaf(w.slope, float(t), fmaf(s[t], k, base));
@@ -259,8 +269,8 @@ __device__ __forceinline__ float modify_scores(const MaskedArgs& m, const Row& w
     const int R = m.max_dist;
     const float* tab = m.table + (long long)w.head * (2 * R + 1) + R;
     const int d0 = kv0 - w.p;
-    if (__all_sync(0xffffffffu, !w.valid || d0 >= R || d0 + BN - 1 <= -R)) {  // past the table's end on either side
-      const float e = __ldg(tab + (d0 >= R ? R : -R)) * kLog2e;
+    if (kv0 - w.p_max >= R || kv0 + BN - 1 - w.p_min <= -R) {  // past the table's end on either side, for every row
+      const float e = __ldg(tab + (kv0 - w.p_max >= R ? R : -R)) * kLog2e;
 #pragma unroll
       for (int t = 0; t < BN; ++t) s[t] = fmaf(s[t], k, e);
     } else if (m.table_smem) {
@@ -299,20 +309,22 @@ __device__ __forceinline__ float modify_scores(const MaskedArgs& m, const Row& w
     }
     return 1.0f;
   }
-  const long long off = mask_offset(m, w, kv0);
   const int n = m.a.Skv - kv0;  // readable keys from here
   // -inf hides; any finite value, however low, stays finite in log2 units.
   auto add = [k](float x, float e) { return e == -INFINITY ? -INFINITY : fmaxf(fmaf(x, k, e * kLog2e), -FLT_MAX); };
   if (m.mask_kind == 1) {
-    const uint8_t* p = static_cast<const uint8_t*>(m.mask) + off;
+    const uint8_t* p = w.mask + kv0;
     if (m.mask_vec && n >= BN) {
 #pragma unroll
       for (int c = 0; c < BN / 16; ++c) {
         const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + c);
         const uint32_t q[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int t = 0; t < 16; ++t)
-          if ((q[t / 4] & (0xffu << (8 * (t % 4)))) == 0) s[16 * c + t] = -INFINITY;
+        for (int t = 0; t < 16; ++t) {
+          // The byte (0 or 1) as all zeros or all ones: its low bit moved to the sign and that replicated.
+          const uint32_t keep = replicate_sign(q[t / 4] << 7, t % 4);
+          s[16 * c + t] = __uint_as_float((__float_as_uint(s[16 * c + t]) & keep) | (0xff800000u & ~keep));
+        }
       }
     } else {
 #pragma unroll
@@ -320,7 +332,7 @@ __device__ __forceinline__ float modify_scores(const MaskedArgs& m, const Row& w
         if (t >= n || __ldg(p + t) == 0) s[t] = -INFINITY;
     }
   } else if (m.mask_kind == 2) {
-    const unsigned short* p = static_cast<const unsigned short*>(m.mask) + off;
+    const unsigned short* p = reinterpret_cast<const unsigned short*>(w.mask) + kv0;
     if (m.mask_vec && n >= BN) {
 #pragma unroll
       for (int c = 0; c < BN; c += 8) {
@@ -336,7 +348,7 @@ __device__ __forceinline__ float modify_scores(const MaskedArgs& m, const Row& w
         s[t] = t < n ? add(s[t], __uint_as_float(uint32_t(__ldg(p + t)) << 16)) : -INFINITY;
     }
   } else {
-    const float* p = static_cast<const float*>(m.mask) + off;
+    const float* p = reinterpret_cast<const float*>(w.mask) + kv0;
     if (m.mask_vec && n >= BN) {
 #pragma unroll
       for (int c = 0; c < BN; c += 4) {
@@ -357,7 +369,7 @@ __device__ __forceinline__ float modify_scores(const MaskedArgs& m, const Row& w
 // Whether no row of the warp sees the key tile at kv0 (the same in both warps of the rows: neither reads S then, nor
 // takes the step's barrier).
 __device__ __forceinline__ bool hidden_tile(const Row& w, int kv0) {
-  return __all_sync(0xffffffffu, w.hi <= kv0 || w.lo >= kv0 + kMaskedBN);
+  return w.hi_max <= kv0 || w.lo_min >= kv0 + kMaskedBN;
 }
 
 // One online-softmax step over the key tile at kv0 for this thread's row and its half of the keys: P as bf16 pairs over
@@ -389,7 +401,7 @@ __device__ __forceinline__ float masked_softmax_step(const MaskedArgs& m, const 
   }
   float c = m.a.scale_log2;
   if constexpr (FEAT != 0) c = modify_scores<FEAT, kHalf>(m, w, key0, row_mask, s_table, s_mask, lane, s);
-  if (__any_sync(0xffffffffu, w.valid && (w.lo > key0 || w.hi < key0 + kHalf))) {
+  if (w.lo_max > key0 || w.hi_min < key0 + kHalf) {
     const int a = w.lo - key0, z = w.hi - key0;
 #pragma unroll
     for (int t = 0; t < kHalf; ++t)
@@ -616,11 +628,9 @@ __global__ void __launch_bounds__(kMaskedThreads, MaskedLayout<DP, STAGES>::kTwo
   const int half = int(threadIdx.x) >> 7;
   if (warp < kSoftWarps) {
     w = row_of(m, row, tile, h0, bb);
-    const int lo = __reduce_min_sync(0xffffffffu, w.hi > w.lo ? w.lo : INT_MAX);
-    const int hi = __reduce_max_sync(0xffffffffu, w.hi);
     if (lane == 0 && half == 0) {
-      s_union[warp] = lo;
-      s_union[4 + warp] = hi;
+      s_union[warp] = w.lo_min;
+      s_union[4 + warp] = w.hi_max;
     }
   }
   __syncthreads();

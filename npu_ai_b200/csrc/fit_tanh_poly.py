@@ -1,4 +1,4 @@
-"""Fits the polynomial behind the capped scores of the masked attention (tanh_ratio() in attention_masked.cuh).
+"""Fits the polynomial behind the capped scores of the masked attention (kTanhRatio in attention_masked.cuh).
 
 tanh(y) = y p(y^2) on |y| <= 1 with p of degree 5, chosen to minimise the maximum RELATIVE error |y p(y^2) / tanh(y) - 1|
 over a dense grid: a linear program in the coefficients and the error (minimax fit by linear programming). The

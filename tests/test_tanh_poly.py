@@ -1,4 +1,4 @@
-"""The capped scores' polynomial (tanh_ratio in attention_masked.cuh): its constants are the ones the committed fit
+"""The capped scores' polynomial (kTanhRatio in attention_masked.cuh): its constants are the ones the committed fit
 produces, and evaluated in f32 the way the kernel does it, its relative error stays below 1e-6 on the kernel's range."""
 import importlib.util
 import pathlib
@@ -18,9 +18,9 @@ def _fit_module():
 
 def _kernel_coeffs():
     src = (CSRC / "attention_masked.cuh").read_text()
-    body = src[src.index("float tanh_ratio("):]
-    body = body[:body.index("\n}")]
-    return np.float32([float(v) for v in re.findall(r"(-?[0-9]\.[0-9]+e[-+][0-9]+)f", body)][::-1])
+    body = src[src.index("float kTanhRatio[6]"):]
+    body = body[:body.index("};")]
+    return np.float32([float(v) for v in re.findall(r"(-?[0-9]\.[0-9]+e[-+][0-9]+)f", body)])
 
 
 def test_kernel_constants_match_fit():
