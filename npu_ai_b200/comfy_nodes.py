@@ -12,8 +12,11 @@ What changes: the model runs on the GPU, so calls route by device `cuda` (the re
 NPU, node :150, :174). The attention gate no longer chooses between the accelerator and the CPU: it chooses
 between kernel variants of the fused attention (query tiles per CTA x key tile) by timing each once per shape, and still
 checks the first result of every shape against the model's own attention (max relative error <= 0.1, else
-RuntimeError, node :225-232). Shapes with a mask or GQA (which the fused kernel does not implement) and
-attention mode "off" (the reference's "cpu") run the model's own attention function, logged once per shape.
+RuntimeError, node :225-232). Calls with a mask (bool or additive, 2-D or 4-D) or grouped key/value heads run the
+masked attention kernel, checked the same way (the reference leaves them to the CPU, node :39-99); masks of other
+forms and attention mode "off" (the reference's "cpu") run the model's own attention function, logged once per shape.
+Linears of a Sequential that an activation follows (feed-forward projections without gating) apply it in the GEMM's
+epilogue.
 """
 from __future__ import annotations
 
@@ -51,7 +54,8 @@ def _mode(m: str) -> str:
 
 @dataclass
 class ShapeRecord:
-    """The gate's knowledge of one attention shape, keyed (batch, query tokens, key tokens, heads, head dim)."""
+    """The gate's knowledge of one attention shape, keyed (batch, query tokens, key tokens, heads, head dim), for masked
+    and grouped-query calls also by what the mask is."""
     variant_ms: dict[int, float] = field(default_factory=dict)  # timed once per variant on the first call
     model_ms: float | None = None        # the model's own attention, timed after one warm-up call
     variant: int | None = None           # the fused-kernel variant this shape runs
@@ -76,10 +80,10 @@ class AttentionGate:
     Mode ``auto`` times every variant the head dim allows once, on the shape's first call, and keeps the fastest;
     ``gpu`` keeps the kernel's own automatic variant; ``off`` (the reference's ``cpu``) hands every call to the
     model's own attention. In every mode the first fused result of a shape is compared with the model's own
-    attention (max relative error <= 0.1, else RuntimeError). The model's attention also serves the calls the
-    kernel does not implement: an attention mask or grouped-query heads. ``min_tokens`` (default 1, so every SD1.5
-    self- and cross-attention, the 64-token middle block included, stays on the kernel) sends shorter query
-    sequences there too; each such shape is logged once with its reason.
+    attention (max relative error <= 0.1, else RuntimeError). Calls with a mask or grouped-query heads that the
+    masked kernel takes have one variant; the model's attention serves what it does not take. ``min_tokens``
+    (default 1, so every SD1.5 self- and cross-attention, the 64-token middle block included, stays on the kernel)
+    sends shorter query sequences there too; each such shape is logged once with its reason.
     """
 
     def __init__(self, mode: str = "auto", min_tokens: int = 1):
@@ -156,6 +160,7 @@ class B200Runtime:
         # Linears on the GEMM kernel: weights[id] = (resident NpuWeight, f32 bias on the device or None, name).
         self.weights: dict[int, tuple] = {}
         self.geglu_modules: set[int] = set()     # GEGLU modules routed to the fused projection + gating kernel
+        self.act_modules: set[int] = set()       # Sequentials with a Linear and its activation in one kernel
         # Sibling projections fed the same input (self-attention q/k/v, cross-attention k/v) run as ONE GEMM over
         # the concatenated weight: leader id -> (fused NpuWeight, fused bias | None, [(member id, column slice)]),
         # member id -> leader id; `pending` holds the member outputs of the last leader call until consumed.
@@ -244,6 +249,11 @@ class B200Runtime:
                     and id(mod) not in self.patched and proj.out_features % 2 == 0):
                 self.geglu_modules.add(id(mod))
                 self._patch(mod, _gpu_geglu_forward)
+        # Linear -> activation pairs of a Sequential (feed-forward blocks without gating): one kernel.
+        for mod in diffusion_model.modules():
+            if id(mod) not in self.patched and _linear_act_pairs(mod, self):
+                self.act_modules.add(id(mod))
+                self._patch(mod, _gpu_linear_act_forward)
         return n_new
 
     def _fuse_projections(self, diffusion_model: torch.nn.Module) -> None:
@@ -391,6 +401,7 @@ class B200Runtime:
         self.patched.clear()
         self.weights.clear()
         self.geglu_modules.clear()
+        self.act_modules.clear()
         self.enabled = False
 
 
@@ -448,6 +459,46 @@ def _gpu_geglu_forward(self, x: torch.Tensor) -> torch.Tensor:
     out_dtype = x.dtype if x.dtype in (torch.bfloat16, torch.float32) else torch.float32
     y = rt.gemm.linear_geglu(x, w, bias, out_dtype=out_dtype)
     return y if y.dtype == x.dtype else y.to(dtype=x.dtype)
+
+
+def _activation_name(mod) -> str | None:
+    """The GEMM epilogue activation that a module is, or None."""
+    if type(mod) is torch.nn.GELU:
+        return {"none": "gelu", "tanh": "gelu_tanh"}.get(mod.approximate)
+    return {torch.nn.SiLU: "silu", torch.nn.ReLU: "relu"}.get(type(mod))
+
+
+def _linear_act_pairs(mod, rt) -> list[int]:
+    """The places of a Sequential's taken-over Linears that an activation of the GEMM's epilogue follows. Linears that
+    serve others' products (q/k/v groups) and modules with hooks, which would be passed by, are left out."""
+    if type(mod) is not torch.nn.Sequential:
+        return []
+    items = list(mod)
+    return [i for i, (a, b) in enumerate(zip(items, items[1:]))
+            if isinstance(a, torch.nn.Linear) and id(a) in rt.weights and _activation_name(b) is not None
+            and id(a) not in rt.fused_member and id(a) not in rt.fused_groups
+            and not any(m._forward_hooks or m._forward_pre_hooks for m in (a, b))]
+
+
+def _gpu_linear_act_forward(self, x):
+    """Sequential.forward with each Linear -> activation pair as one GEMM whose epilogue applies the activation to the
+    f32 sums (one launch and one activation round trip fewer); the other modules run as they are, and so does a pair
+    wherever its Linear would fall back (runtime off, discovery pass, too few tokens, CPU tensors)."""
+    rt = _RUNTIME
+    items = list(self)
+    pairs = set(_linear_act_pairs(self, rt)) if _runtime_on(rt) and id(self) in rt.act_modules else ()
+    i = 0
+    while i < len(items):
+        tokens = x.numel() // x.shape[-1] if isinstance(x, torch.Tensor) and x.dim() and x.numel() else 0
+        if i in pairs and tokens >= max(rt.min_tokens, 1) and x.device.type == "cuda":
+            w, bias, _name = rt.weights[id(items[i])]
+            out_dtype = x.dtype if x.dtype in (torch.bfloat16, torch.float32) else torch.float32
+            x = rt.gemm.linear(x, w, bias, out_dtype=out_dtype, activation=_activation_name(items[i + 1])).to(x.dtype)
+            i += 2
+        else:
+            x = items[i](x)
+            i += 1
+    return x
 
 
 def _out_linear(m):
@@ -768,6 +819,21 @@ def _gpu_resblock_forward(self, x, emb, *args, **kwargs):
     return out
 
 
+def _kernel_mask(mask, b: int, h: int, tq: int, tk: int, device):
+    """The mask as the masked attention kernel reads it, or None when the call stays with the model: bool, bf16 or f32
+    (f16 is widened; f64 would lose its finite extremes), [tq, tk] or 4-D broadcastable to [b, h, tq, tk]. What the
+    leading dimension of a 3-D mask means differs between models."""
+    if not isinstance(mask, torch.Tensor) or mask.device != device or mask.dim() not in (2, 4) or mask.requires_grad:
+        return None
+    if mask.dtype == torch.float16:
+        mask = mask.float()
+    if mask.dtype not in (torch.bool, torch.bfloat16, torch.float32) or mask.shape[-1] != tk:
+        return None
+    if any(n not in (1, m) for n, m in zip(mask.shape[-2::-1], (tq, h, b))):
+        return None
+    return mask if tk == 1 or mask.stride(-1) == 1 else mask.contiguous()
+
+
 def _gpu_attention_override(func, q, k, v, heads, mask=None, attn_precision=None, skip_reshape=False,
                             skip_output_reshape=False, **kwargs):
     """transformer_options["optimized_attention_override"] (the reference's _npu_attention_override,
@@ -789,8 +855,17 @@ def _gpu_attention_override(func, q, k, v, heads, mask=None, attn_precision=None
         h, d = heads, inner // heads
         tk = k.shape[1]
     key = (b, tq, tk, h, d)
-    fits = rt.gemm.attention_fits(tq, tk, d, b * h)
-    why = gate.model_route_reason(key, mask is not None, bool(kwargs.get("enable_gqa", False)), fits)
+    gqa = bool(kwargs.get("enable_gqa", False))
+    masked = mask is not None or gqa
+    if masked:
+        fits = rt.gemm.attention_fused_fits(tq, tk, d, b * h)
+        hk = k.shape[1] if skip_reshape else k.shape[2] // d
+        kmask = _kernel_mask(mask, b, h, tq, tk, q.device) if mask is not None else None
+        key += ((f"{kmask.dtype} mask" if kmask is not None else "") + (f" {hk} kv heads" if gqa else ""),)
+        why = gate.model_route_reason(key, mask is not None and kmask is None, gqa and (hk <= 0 or h % hk != 0), fits)
+    else:
+        fits = rt.gemm.attention_fits(tq, tk, d, b * h)
+        why = gate.model_route_reason(key, False, False, fits)
     if why is not None or rt.record_only:
         t0 = time.perf_counter()
         out = model_attn()
@@ -803,6 +878,10 @@ def _gpu_attention_override(func, q, k, v, heads, mask=None, attn_precision=None
     def fused(variant):
         from . import kernels
         qd, kd, vd = (rt.gemm._attn_operand(t) for t in (q, k, v))
+        if masked:
+            return kernels.attention(qd, kd, vd, h, scale=scale, head_major_in=skip_reshape,
+                                     head_major_out=skip_output_reshape, out_dtype=out_dtype,
+                                     kv_heads=hk if gqa else None, mask=kmask)
         return kernels.attention(qd, kd, vd, h, scale=scale, head_major_in=skip_reshape,
                                  head_major_out=skip_output_reshape, out_dtype=out_dtype, variant=variant)
 
@@ -811,13 +890,17 @@ def _gpu_attention_override(func, q, k, v, heads, mask=None, attn_precision=None
         # First call of this shape: time the variants (each after one warm-up launch), then check the first
         # result against the model's own attention, also timed after a warm-up call.
         y = None
-        for var in (attn_variants(d) if gate.mode == "auto" else (0,)):
+        for var in (attn_variants(d) if gate.mode == "auto" and not masked else (0,)):
             fused(var)
             y_v, rec.variant_ms[var] = _time_gpu(lambda: fused(var), rt.gemm.device)
             y = y_v if y is None else y
         model_attn()
         ref, rec.model_ms = _time_gpu(model_attn, rt.gemm.device)
-        err = float((y.float() - ref.float()).abs().max() / (ref.float().abs().max() + 1e-12))
+        ref = ref.float()
+        if masked:  # rows whose mask hides every key: zeros here, NaN from a plain softmax
+            hidden = torch.isnan(ref) & (y == 0)
+            ref = torch.where(hidden, 0.0, ref)
+        err = float((y.float() - ref).abs().max() / (ref.abs().max() + 1e-12))
         rec.max_rel_err = err
         if not np.isfinite(err) or err > 0.1:
             raise RuntimeError(f"fused attention result for {key} does not match the model's attention "

@@ -220,7 +220,7 @@ at::Tensor attention_masked(const at::Tensor& q, const at::Tensor& k, const at::
   const int64_t B = q.size(0), Sq = q.size(head_major_in ? 2 : 1), Skv = k.size(head_major_in ? 2 : 1);
   const int64_t d = head_major_in ? q.size(3) : q.size(2) / heads;
   const int64_t Hk = head_major_in ? k.size(1) : (d > 0 && k.size(2) % d == 0 ? k.size(2) / d : 0);
-  TORCH_CHECK_VALUE(Hk > 0 && heads % Hk == 0 && (kv_heads <= 0 || kv_heads == Hk), "k/v hold ", Hk,
+  TORCH_CHECK_VALUE(Hk > 0 && heads % Hk == 0 && (kv_heads == 0 || kv_heads == Hk), "k/v hold ", Hk,
                     " heads: kv_heads must be that, and a divisor of heads=", heads, " (got ", kv_heads, ")");
   kv_heads = Hk;
   TORCH_CHECK_VALUE(k.size(0) == B && k.size(-1) == (head_major_in ? d : Hk * d) && v.sizes() == k.sizes(), "k/v shapes ",

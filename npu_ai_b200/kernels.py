@@ -476,7 +476,7 @@ def _attention_masked(q, k, v, heads, scale, head_major_in, head_major_out, out_
             raise ValueError(f"softcap must be positive and finite (got {softcap})")
         if scale is not None and not scale > 0.0:
             raise ValueError(f"attention scale must be positive (got {scale})")
-        return ops.attention_masked(q, k, v, out, out_dtype, heads, kv_heads or 0, head_major_in, head_major_out,
+        return ops.attention_masked(q, k, v, out, out_dtype, heads, 0 if kv_heads is None else kv_heads or -1, head_major_in, head_major_out,
                                     scale or 0.0, variant, causal, q_start if starts is None else None, starts,
                                     prefix_len or 0 if prefixes is None else 0, prefixes, kv_lens, doc_offsets,
                                     softcap or 0.0, slopes, distance_bias, mask)

@@ -9,6 +9,7 @@ the NPU runner (its ComfyUI node, its test scripts) run unchanged:
   linear(x, w, bias=None)                   xdna1_gemm.py:428-448
   prepare(shapes), dispatch_shapes(M,K,N)   xdna1_gemm.py:295-308
   attention(q, k, v, heads, scale=None, skip_reshape=False, skip_output_reshape=False)   xdna1_gemm.py:499-600
+                                            (also masked and with grouped key/value heads: kernels.attention)
   attention_fits / attention_warmup / attention_fused_fits                              xdna1_gemm.py:451-497
   summary(), stats, pool                    xdna1_gemm.py:201-209, :755-773
 
@@ -260,7 +261,8 @@ class NpuGemm:
                  out_dtype: torch.dtype | None = None, residual: torch.Tensor | None = None,
                  activation: str | None = None) -> torch.Tensor:
         """x: (M, K) numpy/torch float -> (M, N) CUDA tensor = act(x @ W (+ bias)); bf16 operands, f32 accumulation,
-        bias in f32 (npu/xdna1_gemm.py:349-422); `activation` as in kernels.gemm (None: none). f32 output unless `out_dtype`/`out` say otherwise."""
+        bias in f32 (npu/xdna1_gemm.py:349-422); `activation` as in kernels.gemm (None: none). f32 output unless
+        `out_dtype`/`out` say otherwise."""
         t_start = time.perf_counter()
         x2 = self._x_device(x)
         if x2.dim() != 2:
@@ -286,7 +288,8 @@ class NpuGemm:
     def linear(self, x, w: NpuWeight, bias=None, out_dtype: torch.dtype | None = None,
                residual: torch.Tensor | None = None, activation: str | None = None):
         """x: (..., K) -> (..., N) = act(x @ W (+ bias)) (+ residual, a bf16 (..., N) CUDA tensor); activation and
-        residual are applied in the GEMM's epilogue (`activation` as in kernels.gemm). torch in -> torch (CUDA) out, numpy in -> numpy out (npu/xdna1_gemm.py:428-448)."""
+        residual are applied in the GEMM's epilogue (`activation` as in kernels.gemm). torch in -> torch (CUDA) out,
+        numpy in -> numpy out (npu/xdna1_gemm.py:428-448)."""
         is_torch = isinstance(x, torch.Tensor)
         xt = _as_tensor(x)
         shp = tuple(xt.shape)
@@ -349,18 +352,24 @@ class NpuGemm:
 
     def attention(self, q, k, v, heads: int, scale: float | None = None, skip_reshape: bool = False,
                   skip_output_reshape: bool = False, out_dtype: torch.dtype | None = None, *,
-                  group=None) -> torch.Tensor:
+                  group=None, kv_heads: int | None = None, **masking) -> torch.Tensor:
         """softmax(Q K^T * scale) V for all (batch, head) pairs in ONE launch (bf16 in, f32 accumulate).
 
         q/k/v: (b, t, heads*d), or (b, heads, t, d) when skip_reshape. Returns (b, tq, heads*d) (or
         (b, heads, tq, d) when skip_output_reshape), f32 unless `out_dtype` (npu/xdna1_gemm.py:499-533).
         `group` (a torch.distributed process group, every rank holding the whole block on its GPU) splits the pairs
         over the group's ranks in contiguous ranges and all-gathers the result (npu_ai_b200.sharding).
+        `kv_heads` and `masking` (causal, q_start, prefix_len, kv_lens, doc_offsets, softcap, slopes, distance_bias,
+        mask) are those of kernels.attention, on any device; the FLOP count in `stats` is that of the unmasked call.
         """
         t_start = time.perf_counter()
         qd, kd, vd = (self._attn_operand(t) for t in (q, k, v))
         # Q read in place: the caller's device tensor itself reached the kernel (no host copy, cast or compaction)
         q_inplace = isinstance(q, torch.Tensor) and q.is_cuda and q.data_ptr() == qd.data_ptr() and q.dtype == qd.dtype
+        if group is not None and (kv_heads is not None or any(m is not None and m is not False for m in masking.values())):
+            raise ValueError("masked attention and grouped key/value heads are not split over a group")
+        masking = {name: m.detach().to(self.device) if isinstance(m, torch.Tensor) else m
+                   for name, m in masking.items()}
         if skip_reshape:
             b, h, tq, d = qd.shape
             tk = kd.shape[2]
@@ -379,7 +388,8 @@ class NpuGemm:
                                   head_major_out=skip_output_reshape, out_dtype=out_dtype or self.out_dtype)
         else:
             y = kernels.attention(qd, kd, vd, h, scale=scale, head_major_in=skip_reshape,
-                                  head_major_out=skip_output_reshape, out_dtype=out_dtype or self.out_dtype)
+                                  head_major_out=skip_output_reshape, out_dtype=out_dtype or self.out_dtype,
+                                  kv_heads=kv_heads, **masking)
         with self._lock:
             sh = self.stats["attn_by_shape"].setdefault(key, [0, 0.0, 0.0, 0.0, 0.0, 0, 0.0])
             self._close("attn", ev, key)
