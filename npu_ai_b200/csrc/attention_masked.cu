@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(32 * kJoinBlockWarps)
 // Host side
 // ---------------------------------------------------------------------------------------------------------------
 struct MaskedPlan {
-  int pack, T, splits;
+  int pack, T, splits, streams;
   int64_t tiles, pairs;
   size_t ml_bytes, bytes;  // workspace: (max, sum) pairs first, then the O rows
 };
@@ -189,6 +189,7 @@ int plan_masked(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Skv, int64
   const int64_t key_tiles = (Skv + kMaskedBN - 1) / kMaskedBN;
   const int64_t slots = (D <= 128 ? 2 : 1) * int64_t(sms);  // resident CTAs
   p.splits = 1;
+  p.streams = 1;
   if (variant > 0) {
     p.splits = variant;
   } else if (2 * ctas <= slots && key_tiles >= 8) {
@@ -201,6 +202,8 @@ int plan_masked(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Skv, int64
     const int64_t per = (key_tiles + parts - 1) / parts;
     p.splits = int((key_tiles + per - 1) / per);
   }
+  // Where an SM holds one CTA anyway, that CTA runs two streams of key tiles.
+  if (D <= 160 && (D > 128 || ctas * p.splits <= sms) && key_tiles >= 4 * p.splits) p.streams = 2;
   if (p.splits > 1) {
     if (B * H * Sq > INT32_MAX / kMaxSplits)
       return fail(kErrUnsupported, "too many rows to split their keys (%lld)", (long long)(B * H * Sq));
@@ -339,7 +342,7 @@ int attention_masked_launch(const AttnMaskedProblem& mp, cudaStream_t stream) {
                 : feats == kFeatDistance ? launch_masked_for<kFeatDistance>
                 : feats == kFeatMask     ? launch_masked_for<kFeatMask>
                                          : launch_masked_for<kFeatAny>;
-  if (int rc = launch(p.D, mq, mk, mv, m, grid, stream, dev->device)) return rc;
+  if (int rc = launch(p.D, plan.streams, mq, mk, mv, m, grid, stream, dev->device)) return rc;
   if (plan.splits == 1) return kOk;
   const int rows = int(p.B * p.H * p.Sq);
   const bool few = rows <= kJoinFewRows;

@@ -37,9 +37,7 @@ namespace npub200 {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaskedBN = 64;        // keys per tile
 constexpr int kHalf = kMaskedBN / 2;  // keys per softmax thread: two warps share the rows of a TMEM lane quarter
-constexpr int kSoftWarps = 2 * kSoftmaxWarps;
-constexpr int kProducerWarp = kSoftWarps, kMmaWarp = kSoftWarps + 1;
-constexpr int kMaskedThreads = (kSoftWarps + 2) * 32;
+constexpr int kSoftWarps = 2 * kSoftmaxWarps;  // of a stream of key tiles
 constexpr int kMaxSplits = 64;
 constexpr int kTableMargin = 128;     // repeated ends of the distance bias in shared memory, either side
 constexpr int kTableSmemMax = 10240;  // bytes: keeps two CTAs per SM
@@ -381,8 +379,8 @@ __device__ __forceinline__ bool hidden_tile(const Row& w, int kv0) {
 template <int FEAT>
 __device__ __forceinline__ float masked_softmax_step(const MaskedArgs& m, const Row& w, uint32_t s_addr, int kv0, int half,
                                                      int row, int lane, float row_mask, const float* s_table,
-                                                     float* s_mask, float* s_max, float& run_max, float& run_sum,
-                                                     bool& move) {
+                                                     float* s_mask, float* s_max, int barrier, float& run_max,
+                                                     float& run_sum, bool& move) {
   move = false;
   const uint32_t p_addr = s_addr + uint32_t(half * (kHalf / 2));
   if (hidden_tile(w, kv0)) {
@@ -414,7 +412,7 @@ __device__ __forceinline__ float masked_softmax_step(const MaskedArgs& m, const 
   for (int e = 0; e < 8; ++e) mx8[e] = fmaxf(mx8[e], s[24 + e]);
   float mx = fmax3(fmax3(mx8[0], mx8[1], mx8[2]), fmax3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])) * c;
   s_max[half * kAttnBM + row] = mx;
-  named_barrier_sync(1 + (row >> 5), 64);
+  named_barrier_sync(barrier, 64);
   mx = fmaxf(mx, s_max[(half ^ 1) * kAttnBM + row]);
   move = mx > run_max + m.a.rescale_thr;
   const float m_new = move ? mx : run_max;
@@ -443,24 +441,24 @@ __device__ __forceinline__ float masked_softmax_step(const MaskedArgs& m, const 
   return alpha;
 }
 
-// The O columns [begin, end) of a padded head dim that each of the two warps of a row rescales and stores: halves in
-// units of 16 columns.
-template <int DP>
+// The O columns of a padded head dim that each of PARTS warps of a row takes: parts in units of 16 columns.
+template <int DP, int PARTS>
 struct OColumns {
-  static constexpr int kFirst = (DP / 16 + 1) / 2 * 16;  // columns of the first warp, where the second's begin
-  static constexpr int kSecond = DP - kFirst;
+  static constexpr int kWidth = (DP / 16 + PARTS - 1) / PARTS * 16;  // the last parts may be narrower or empty
+  static __device__ __forceinline__ int begin(int part) { return min(part * kWidth, DP); }
 };
 
 __device__ __forceinline__ void st_global_v4(uint64_t to, const uint4& v) {
   asm volatile("st.global.v4.b32 [%0], {%1, %2, %3, %4};" ::"l"(to), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
-// The warp's 32 O rows x inv (zeros where `zero`; o_addr 0: no O, all zeros) to `dst` (each lane's own row, null: no
-// row): `cols` columns from o_addr on (a multiple of 8; the padded columns are whole sixteens) as f32 or bf16. A lane holds a row, so rows go through shared memory (`stage`, an odd
+// The warp's 32 O rows x inv (zeros where `zero`; o_addr 0: no O, all zeros; o_addr2 not 0: plus the rows there x inv2)
+// to `dst` (each lane's own row, null: no row): `cols` columns from o_addr on (a multiple of 8; the padded
+// columns are whole sixteens) as f32 or bf16. A lane holds a row, so rows go through shared memory (`stage`, an odd
 // number of 16-byte words apart) and out in 16-byte words along them. Rolled loops: this runs once a tile, and
 // straight-line code for every head dim and type was paid for in instruction fetches.
-__device__ __forceinline__ void store_rows(uint32_t o_addr, uint8_t* stage, int cols, bool f32, uint8_t* dst, float inv,
-                                           bool zero, int lane) {
+__device__ __forceinline__ void store_rows(uint32_t o_addr, uint32_t o_addr2, uint8_t* stage, int cols, bool f32,
+                                           uint8_t* dst, float inv, float inv2, bool zero, int lane) {
   const int words = cols * (f32 ? 4 : 2) / 16;  // 16-byte words of a row
   const int pitch = (words | 1) * 16;
   uint8_t* mine = stage + lane * pitch;
@@ -474,6 +472,12 @@ __device__ __forceinline__ void store_rows(uint32_t o_addr, uint8_t* stage, int 
     float o[16];
 #pragma unroll
     for (int t = 0; t < 16; ++t) o[t] = zero ? 0.0f : __uint_as_float(r[t]) * inv;
+    if (o_addr2 != 0) {
+      tmem_ld16(o_addr2 + uint32_t(c), r);
+      tmem_wait_ld();
+#pragma unroll
+      for (int t = 0; t < 16; ++t) o[t] = zero ? 0.0f : fmaf(__uint_as_float(r[t]), inv2, o[t]);
+    }
 #pragma unroll
     for (int e = 0; e < 16; e += 8) {
       if (c + e >= cols) break;
@@ -513,10 +517,12 @@ __device__ __forceinline__ void store_rows(uint32_t o_addr, uint8_t* stage, int 
   }
 }
 
-template <int DP, int STAGES>
+template <int DP, int STAGES, int STREAMS>
 struct MaskedLayout {
   static constexpr int BN = kMaskedBN;
   static constexpr int kNA = (DP + 63) / 64;
+  static constexpr int kThreads = (STREAMS * kSoftWarps + 2) * 32;
+  static constexpr int kBufs = STREAMS + 1;  // S tiles in TMEM
   static constexpr int kQAtom = kAttnBM * kAtomBytesPerRow;
   static constexpr int kKVAtom = BN * kAtomBytesPerRow;
   static constexpr int kQBytes = kNA * kQAtom;
@@ -524,30 +530,39 @@ struct MaskedLayout {
   static constexpr int kKOff = kQBytes;
   static constexpr int kVOff = kKOff + STAGES * kKVBytes;
   static constexpr int kBarOff = kVOff + STAGES * kKVBytes;
-  // q_full, k_full[S], v_full[S], k_empty[S], v_empty[S], s_full[2], p_full[2], pv_done[2], drain
-  static constexpr int kNumBars = 1 + 4 * STAGES + 6 + 1;
+  // q_full, k_full[S], v_full[S], k_empty[S], v_empty[S], s_full[kBufs], p_full[kBufs], pv_done[2], drain
+  static constexpr int kNumBars = 1 + 4 * STAGES + 2 * kBufs + 2 + 1;
   static constexpr int kMiscOff = kBarOff + kNumBars * 8;   // TMEM slot, abort flag, the warps' unions
   static constexpr int kMaskOff = (kMiscOff + 16 + 4 * 8 + 15) / 16 * 16;  // the warp's part of a mask row, per softmax warp
-  static constexpr int kMaxOff = kMaskOff + kSoftWarps * kHalf * 4;        // row maxima [tile parity][half][row]
-  static constexpr int kTableOff = kMaxOff + 2 * 2 * kAttnBM * 4;          // the head's distance bias (launch-sized)
+  // row maxima [stream][tile parity][half][row]
+  static constexpr int kMaxOff = kMaskOff + STREAMS * kSoftWarps * kHalf * 4;
+  // both streams' sums [stream][half][row] and maxima [stream][row]
+  static constexpr int kJoinOff = kMaxOff + STREAMS * 2 * 2 * kAttnBM * 4;
+  // the head's distance bias (launch-sized)
+  static constexpr int kTableOff = kJoinOff + (STREAMS > 1 ? 6 * kAttnBM * 4 : 0);
   static constexpr int kSmemBytes = kTableOff + 1024;
-  // The output rows' staging (f32 rows of up to 256 columns, an odd number of words apart) reuses Q, K and V.
-  static_assert(kBarOff >= 2 * kAttnBM * ((DP / 16 + 1) / 2 * 16 * 4 + 16), "staging of the output rows");
-  static constexpr int kOCol = 2 * BN;
-  static constexpr int kTmemUsed = kOCol + DP;
+  // The output rows' staging (f32 rows, an odd number of words apart) reuses Q, K and V.
+  static_assert(kBarOff >= STREAMS * kSoftWarps * 32 * (OColumns<DP, 2 * STREAMS>::kWidth * 4 + 16),
+                "staging of the output rows");
+  static constexpr int kOCol = kBufs * BN;
+  static constexpr int kTmemUsed = kOCol + STREAMS * DP;
+  static_assert(kTmemUsed <= 512, "TMEM columns");
   static constexpr int kTmemCols = (kTmemUsed <= 256) ? 256 : 512;
-  static constexpr bool kTwoPerSm = kSmemBytes <= 113 * 1024 && kTmemCols <= 256;
+  static constexpr bool kTwoPerSm = STREAMS == 1 && kSmemBytes <= 113 * 1024 && kTmemCols <= 256;
   static_assert(DP % 16 == 0 && DP >= 16 && DP <= 256, "padded head dim must be a multiple of 16 in [16, 256]");
   static_assert(kSmemBytes <= 232448, "shared memory budget");
 };
 
-template <int DP, int STAGES, int FEAT>
-__global__ void __launch_bounds__(kMaskedThreads, MaskedLayout<DP, STAGES>::kTwoPerSm ? 2 : 1)
+template <int DP, int STAGES, int STREAMS, int FEAT>
+__global__ void __launch_bounds__(MaskedLayout<DP, STAGES, STREAMS>::kThreads,
+                                  MaskedLayout<DP, STAGES, STREAMS>::kTwoPerSm ? 2 : 1)
     attention_masked_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ MaskedArgs m) {
-  using L = MaskedLayout<DP, STAGES>;
-  using O = OColumns<DP>;
+  using L = MaskedLayout<DP, STAGES, STREAMS>;
+  using OHalf = OColumns<DP, 2>;            // a stream's O, rescaled by the two warps of a row
+  using OPart = OColumns<DP, 2 * STREAMS>;  // the output row, stored by all warps of a row
   constexpr int BN = L::BN;
+  constexpr int kProducerWarp = STREAMS * kSoftWarps, kMmaWarp = kProducerWarp + 1;
   const AttnArgs& args = m.a;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -560,8 +575,8 @@ __global__ void __launch_bounds__(kMaskedThreads, MaskedLayout<DP, STAGES>::kTwo
   uint64_t* k_empty = v_full + STAGES;
   uint64_t* v_empty = k_empty + STAGES;
   uint64_t* s_full = v_empty + STAGES;
-  uint64_t* p_full = s_full + 2;
-  uint64_t* pv_done = p_full + 2;
+  uint64_t* p_full = s_full + L::kBufs;
+  uint64_t* pv_done = p_full + L::kBufs;
   uint64_t* drain = pv_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMiscOff);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMiscOff + 4);
@@ -585,11 +600,11 @@ __global__ void __launch_bounds__(kMaskedThreads, MaskedLayout<DP, STAGES>::kTwo
       mbar_init(&k_empty[s], 1);
       mbar_init(&v_empty[s], 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < L::kBufs; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], kSoftWarps);
-      mbar_init(&pv_done[i], 1);
     }
+    for (int i = 0; i < 2; ++i) mbar_init(&pv_done[i], 1);
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_barrier_init();
@@ -621,14 +636,16 @@ __global__ void __launch_bounds__(kMaskedThreads, MaskedLayout<DP, STAGES>::kTwo
   if ((FEAT & kFeatDistance) && m.table_smem) {
     const int R = m.max_dist;
     const float* tab = m.table + (long long)h0 * (2 * R + 1) + R;
-    for (int k = int(threadIdx.x); k < 2 * (R + kTableMargin) + 1; k += kMaskedThreads)
+    for (int k = int(threadIdx.x); k < 2 * (R + kTableMargin) + 1; k += L::kThreads)
       s_table[k] = __ldg(tab + min(max(k - R - kTableMargin, -R), R)) * kLog2e;
   }
-  const int row = int(threadIdx.x) & (kAttnBM - 1);  // softmax threads: row of the tile and half of the keys
-  const int half = int(threadIdx.x) >> 7;
-  if (warp < kSoftWarps) {
+  // Softmax threads: row of the tile, half of the keys, stream of key tiles.
+  const int row = int(threadIdx.x) & (kAttnBM - 1);
+  const int half = (int(threadIdx.x) >> 7) & 1;
+  const int stream = int(threadIdx.x) >> 8;
+  if (warp < STREAMS * kSoftWarps) {
     w = row_of(m, row, tile, h0, bb);
-    if (lane == 0 && half == 0) {
+    if (lane == 0 && warp < kSoftmaxWarps) {
       s_union[warp] = w.lo_min;
       s_union[4 + warp] = w.hi_max;
     }
@@ -668,7 +685,7 @@ __global__ void __launch_bounds__(kMaskedThreads, MaskedLayout<DP, STAGES>::kTwo
     const uint64_t v_desc = smem_desc_mnmajor_sw128(smem_u32(sV), L::kKVAtom);
     auto pv_step = [&](int i) -> bool {
       const int st = i % STAGES;
-      const int buf = i & 1;
+      const int buf = i % L::kBufs;
       if (!mbar_wait_bounded_warp(&v_full[st], uint32_t(i / STAGES) & 1u, abort_flag, args.ctl, kStatusTimeoutMma))
         return false;
       // V rows of this tile that no row sees: zeros, whatever the cache holds there.
@@ -684,13 +701,13 @@ __global__ void __launch_bounds__(kMaskedThreads, MaskedLayout<DP, STAGES>::kTwo
         fence_proxy_async_smem();
         __syncwarp();
       }
-      if (!mbar_wait_bounded_warp(&p_full[buf], uint32_t(i >> 1) & 1u, abort_flag, args.ctl, kStatusTimeoutMma))
+      if (!mbar_wait_bounded_warp(&p_full[buf], uint32_t(i / L::kBufs) & 1u, abort_flag, args.ctl, kStatusTimeoutMma))
         return false;
       tc_fence_after();
       if (elect_one()) {
-        issue_pv<DP, BN>(tmem_base + L::kOCol, tmem_base + uint32_t(buf * BN),
-                         v_desc + uint64_t((st * L::kKVBytes) >> 4), i > 0);
-        umma_commit(&pv_done[buf]);
+        issue_pv<DP, BN>(tmem_base + L::kOCol + uint32_t(i % STREAMS * DP), tmem_base + uint32_t(buf * BN),
+                         v_desc + uint64_t((st * L::kKVBytes) >> 4), i >= STREAMS);
+        umma_commit(&pv_done[i & 1]);
         umma_commit(&v_empty[st]);
       }
       __syncwarp();
@@ -698,7 +715,7 @@ __global__ void __launch_bounds__(kMaskedThreads, MaskedLayout<DP, STAGES>::kTwo
     };
     for (int j = 0; ok && j < nkv; ++j) {
       const int st = j % STAGES;
-      const int buf = j & 1;
+      const int buf = j % L::kBufs;
       if (!mbar_wait_bounded_warp(&k_full[st], uint32_t(j / STAGES) & 1u, abort_flag, args.ctl, kStatusTimeoutMma)) {
         ok = false;
         break;
@@ -711,106 +728,128 @@ __global__ void __launch_bounds__(kMaskedThreads, MaskedLayout<DP, STAGES>::kTwo
         umma_commit(&k_empty[st]);
       }
       __syncwarp();
-      if (j >= 1 && !pv_step(j - 1)) {
+      if (j >= STREAMS && !pv_step(j - STREAMS)) {
         ok = false;
         break;
       }
     }
-    if (ok && !pv_step(nkv - 1)) ok = false;
+    for (int i = max(nkv - STREAMS, 0); ok && i < nkv; ++i) ok = pv_step(i);
     if (!ok) {
       if (elect_one()) umma_commit(drain);
       __syncwarp();
       mbar_wait_drain(drain, 0u, args.ctl);
     }
-  } else if (warp < kSoftWarps) {
+  } else if (warp < STREAMS * kSoftWarps) {
     // ------------------------------------------------------------------ softmax / correction / epilogue
     const uint32_t lane_base = tmem_base + (uint32_t((warp & 3) * 32) << 16);
     const uint32_t o_addr = lane_base + uint32_t(L::kOCol);
+    const int barrier = 1 + stream * 4 + (warp & 3);  // of the row's two warps in a stream
     float* s_mask = reinterpret_cast<float*>(smem + L::kMaskOff) + warp * kHalf;
-    float* s_max = reinterpret_cast<float*>(smem + L::kMaxOff);
+    float* s_max = reinterpret_cast<float*>(smem + L::kMaxOff) + stream * 4 * kAttnBM;
     float run_max = -INFINITY, run_sum = 0.0f;
     bool ok = true;
-    for (int j = 0; j < nkv; ++j) {
-      const int buf = j & 1;
+    for (int j = stream; j < nkv; j += STREAMS) {
+      const int buf = j % L::kBufs;
       const int kv0 = (first + j) * BN;
       float row_mask = 0.0f;
       if (has_mask<FEAT>(m)) {
         if (m.mask_row)
           row_mask = mask_row_value(m, w, kv0 + half * kHalf, lane);
         else
-          prefetch_mask(m, w, kv0 + BN + half * kHalf);
+          prefetch_mask(m, w, kv0 + STREAMS * BN + half * kHalf);
       }
-      if (ok && !mbar_wait_bounded_warp(&s_full[buf], uint32_t(j >> 1) & 1u, abort_flag, args.ctl,
+      if (ok && !mbar_wait_bounded_warp(&s_full[buf], uint32_t(j / L::kBufs) & 1u, abort_flag, args.ctl,
                                         kStatusTimeoutEpilogue))
         ok = false;
       if (!ok) {  // aborted: the other warp of the rows may still come to this step's barrier
-        if (!hidden_tile(w, kv0)) named_barrier_sync(1 + (row >> 5), 64);
+        if (!hidden_tile(w, kv0)) named_barrier_sync(barrier, 64);
         continue;
       }
       tc_fence_after();
       bool move;
       const float alpha =
           masked_softmax_step<FEAT>(m, w, lane_base + uint32_t(buf * BN), kv0, half, row, lane, row_mask, s_table, s_mask,
-                                      s_max + buf * 2 * kAttnBM, run_max, run_sum, move);
-      if (j > 0 && __any_sync(0xffffffffu, move)) {
-        if (!mbar_wait_bounded_warp(&pv_done[(j - 1) & 1], uint32_t((j - 1) >> 1) & 1u, abort_flag, args.ctl,
+                                      s_max + (j / STREAMS & 1) * 2 * kAttnBM, barrier, run_max, run_sum, move);
+      if (j >= STREAMS && __any_sync(0xffffffffu, move)) {
+        if (!mbar_wait_bounded_warp(&pv_done[(j - STREAMS) & 1], uint32_t((j - STREAMS) >> 1) & 1u, abort_flag, args.ctl,
                                     kStatusTimeoutEpilogue)) {
           ok = false;
           continue;
         }
         tc_fence_after();
 #pragma unroll 1
-        for (int c = half == 0 ? 0 : O::kFirst; c < (half == 0 ? O::kFirst : DP); c += 16)
-          rescale_o_row<16>(o_addr + uint32_t(c), alpha);
+        for (int c = OHalf::begin(half); c < OHalf::begin(half + 1); c += 16)
+          rescale_o_row<16>(o_addr + uint32_t(stream * DP + c), alpha);
       }
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[buf]);
     }
-    // The last P V; without a tile the Q load, which the rows' staging would race with.
-    if (ok)
-      ok = nkv > 0 ? mbar_wait_bounded_warp(&pv_done[(nkv - 1) & 1], uint32_t((nkv - 1) >> 1) & 1u, abort_flag, args.ctl,
-                                            kStatusTimeoutEpilogue)
-                   : mbar_wait_bounded_warp(q_full, 0, abort_flag, args.ctl, kStatusTimeoutEpilogue);
-    // The row's sum is both halves'. (Aborted warps take the barrier, too.)
-    float* s_sum = s_max + (nkv & 1) * 2 * kAttnBM;
-    s_sum[half * kAttnBM + row] = run_sum;
-    named_barrier_sync(1 + (row >> 5), 64);
+    // The last P V of each stream; without a tile the Q load, which the rows' staging would race with.
+    if (ok && nkv == 0) ok = mbar_wait_bounded_warp(q_full, 0, abort_flag, args.ctl, kStatusTimeoutEpilogue);
+    for (int i = max(nkv - STREAMS, 0); ok && i < nkv; ++i)
+      ok = mbar_wait_bounded_warp(&pv_done[i & 1], uint32_t(i >> 1) & 1u, abort_flag, args.ctl, kStatusTimeoutEpilogue);
+    // The row's sum is both halves', and with two streams the row is joined: with M the larger maximum, 2^(m - M) weighs
+    // each stream's O and sum. (Aborted warps take the barrier, too.)
+    float weight[2] = {1.0f, 0.0f};
+    if constexpr (STREAMS == 1) {
+      float* s_sum = s_max + (nkv & 1) * 2 * kAttnBM;
+      s_sum[half * kAttnBM + row] = run_sum;
+      named_barrier_sync(barrier, 64);
+      run_sum += s_sum[(half ^ 1) * kAttnBM + row];
+    } else {
+      float* s_join = reinterpret_cast<float*>(smem + L::kJoinOff) + row;
+      s_join[(2 * stream + half) * kAttnBM] = run_sum;
+      s_join[(4 + stream) * kAttnBM] = run_max;  // the same in both halves
+      named_barrier_sync(1 + 8 + (warp & 3), 128);
+      run_max = fmaxf(s_join[4 * kAttnBM], s_join[5 * kAttnBM]);
+      run_sum = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float top = s_join[(4 + e) * kAttnBM];
+        weight[e] = top == -INFINITY ? 0.0f : fast_exp2(top - run_max);
+        run_sum = fmaf(s_join[2 * e * kAttnBM] + s_join[(2 * e + 1) * kAttnBM], weight[e], run_sum);
+      }
+    }
     if (ok && __any_sync(0xffffffffu, w.valid)) {
       tc_fence_after();
-      run_sum += s_sum[(half ^ 1) * kAttnBM + row];
       const bool empty = run_max == -INFINITY;       // the row has seen no key
       const bool wide = m.splits > 1 || args.out_f32;  // f32 rows
       const int esz = wide ? 4 : 2;
-      const int begin = half == 0 ? 0 : O::kFirst;
-      const int cols = min(args.D - begin, half == 0 ? O::kFirst : O::kSecond);  // this warp's, maybe none
+      const int part = 2 * stream + half;
+      const int begin = OPart::begin(part);
+      const int cols = min(args.D, OPart::begin(part + 1)) - begin;  // this warp's, maybe none
       const long long obase =
           (long long)bb * args.o_sb + (long long)w.i * args.o_ss + (long long)w.head * args.o_sh + begin;
-      uint8_t* stage = smem + warp * 32 * ((O::kFirst * esz / 16) | 1) * 16;
+      uint8_t* stage = smem + warp * 32 * ((OPart::kWidth * esz / 16) | 1) * 16;
       uint8_t* dst = nullptr;
       if (m.splits > 1) {
         const long long at = (((long long)split * m.pairs + pair) * m.tiles + tile) * kAttnBM + row;
-        if (w.valid && half == 0) m.part_ml[at] = make_float2(run_max, empty ? 0.0f : run_sum);
+        if (w.valid && part == 0) m.part_ml[at] = make_float2(run_max, empty ? 0.0f : run_sum);
         if (w.valid && !empty) dst = reinterpret_cast<uint8_t*>(m.part_o + at * args.D + begin);
       } else if (w.valid) {
         dst = static_cast<uint8_t*>(args.out) + obase * esz;
       }
       const float inv = m.splits > 1 ? 1.0f : 1.0f / run_sum;
+      const uint32_t o_at = nkv > 0 ? o_addr + uint32_t(begin) : 0u;
+      const uint32_t o_at2 = STREAMS > 1 && nkv > 1 ? o_addr + uint32_t(DP + begin) : 0u;
       if (cols <= 0) {
         // nothing of the true head dim in this half
       } else if (m.splits > 1 ? nkv > 0 : m.out_vec != 0) {
-        store_rows(nkv > 0 ? o_addr + uint32_t(begin) : 0u, stage, cols, wide, dst, inv, empty, lane);
+        store_rows(o_at, o_at2, stage, cols, wide, dst, inv * weight[0], inv * weight[1], empty, lane);
       } else if (m.splits == 1) {
         // Output rows that 16-byte words do not reach.
         for (int c = 0; c < cols; c += 8) {
           float o[8] = {};
-          if (nkv > 0) {
+#pragma unroll
+          for (int e = 0; e < STREAMS; ++e) {
+            if ((e == 0 ? o_at : o_at2) == 0) break;
             uint32_t r[8];
-            tmem_ld8(o_addr + uint32_t(begin + c), r);
+            tmem_ld8((e == 0 ? o_at : o_at2) + uint32_t(c), r);
             tmem_wait_ld();
 #pragma unroll
-            for (int t = 0; t < 8; ++t) o[t] = empty ? 0.0f : __uint_as_float(r[t]) * inv;
+            for (int t = 0; t < 8; ++t) o[t] = empty ? 0.0f : fmaf(__uint_as_float(r[t]), inv * weight[e], o[t]);
           }
           if (w.valid) {
 #pragma unroll
@@ -834,12 +873,12 @@ __global__ void __launch_bounds__(kMaskedThreads, MaskedLayout<DP, STAGES>::kTwo
   }
 }
 
-template <int DP, int STAGES, int FEAT>
+template <int DP, int STAGES, int STREAMS, int FEAT>
 int launch_masked(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const MaskedArgs& m, dim3 grid,
                   cudaStream_t st, int device) {
   static bool configured[64] = {false};
-  auto kern = attention_masked_tcgen05_kernel<DP, STAGES, FEAT>;
-  using L = MaskedLayout<DP, STAGES>;
+  auto kern = attention_masked_tcgen05_kernel<DP, STAGES, STREAMS, FEAT>;
+  using L = MaskedLayout<DP, STAGES, STREAMS>;
   static_assert(L::kSmemBytes + kTableSmemMax <= (L::kTwoPerSm ? 113 * 1024 : 232448), "room for the distance bias");
   const int smem = L::kSmemBytes + (m.table_smem ? (2 * (m.max_dist + kTableMargin) + 1) * 4 : 0);
   if (!configured[device]) {
@@ -849,35 +888,40 @@ int launch_masked(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMa
       return rc;
     configured[device] = true;
   }
-  return check_cuda(launch_pdl(kern, grid, dim3(kMaskedThreads), smem, st, mq, mk, mv, m),
-                    "masked attention kernel launch");
+  return check_cuda(launch_pdl(kern, grid, dim3(L::kThreads), smem, st, mq, mk, mv, m), "masked attention kernel launch");
 }
 
 template <int FEAT>
-int launch_masked_for(int64_t D, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
+int launch_masked_for(int64_t D, int streams, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
                       const MaskedArgs& m, dim3 grid, cudaStream_t st, int dev) {
+  if (streams == 2) {
+    if (D <= 64) return launch_masked<64, 5, 2, FEAT>(mq, mk, mv, m, grid, st, dev);
+    if (D <= 96) return launch_masked<96, 4, 2, FEAT>(mq, mk, mv, m, grid, st, dev);
+    if (D <= 128) return launch_masked<128, 4, 2, FEAT>(mq, mk, mv, m, grid, st, dev);
+    return launch_masked<160, 3, 2, FEAT>(mq, mk, mv, m, grid, st, dev);
+  }
   // The padded head dims with a kernel; the columns between D and its pad are TMA zeros.
-  if (D <= 32) return launch_masked<32, 5, FEAT>(mq, mk, mv, m, grid, st, dev);
-  if (D <= 48) return launch_masked<48, 5, FEAT>(mq, mk, mv, m, grid, st, dev);
-  if (D <= 64) return launch_masked<64, 5, FEAT>(mq, mk, mv, m, grid, st, dev);
-  if (D <= 80) return launch_masked<80, 2, FEAT>(mq, mk, mv, m, grid, st, dev);
-  if (D <= 96) return launch_masked<96, 2, FEAT>(mq, mk, mv, m, grid, st, dev);
-  if (D <= 128) return launch_masked<128, 2, FEAT>(mq, mk, mv, m, grid, st, dev);
-  if (D <= 160) return launch_masked<160, 2, FEAT>(mq, mk, mv, m, grid, st, dev);
-  if (D <= 192) return launch_masked<192, 2, FEAT>(mq, mk, mv, m, grid, st, dev);
-  return launch_masked<256, 2, FEAT>(mq, mk, mv, m, grid, st, dev);
+  if (D <= 32) return launch_masked<32, 5, 1, FEAT>(mq, mk, mv, m, grid, st, dev);
+  if (D <= 48) return launch_masked<48, 5, 1, FEAT>(mq, mk, mv, m, grid, st, dev);
+  if (D <= 64) return launch_masked<64, 5, 1, FEAT>(mq, mk, mv, m, grid, st, dev);
+  if (D <= 80) return launch_masked<80, 2, 1, FEAT>(mq, mk, mv, m, grid, st, dev);
+  if (D <= 96) return launch_masked<96, 2, 1, FEAT>(mq, mk, mv, m, grid, st, dev);
+  if (D <= 128) return launch_masked<128, 2, 1, FEAT>(mq, mk, mv, m, grid, st, dev);
+  if (D <= 160) return launch_masked<160, 2, 1, FEAT>(mq, mk, mv, m, grid, st, dev);
+  if (D <= 192) return launch_masked<192, 2, 1, FEAT>(mq, mk, mv, m, grid, st, dev);
+  return launch_masked<256, 2, 1, FEAT>(mq, mk, mv, m, grid, st, dev);
 }
 
 // The instantiations (attention_masked.cu and attention_masked_*.cu, one set of features each).
-extern template int launch_masked_for<0>(int64_t, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&,
+extern template int launch_masked_for<0>(int64_t, int, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&,
                                          const MaskedArgs&, dim3, cudaStream_t, int);
-extern template int launch_masked_for<kFeatCap>(int64_t, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&,
+extern template int launch_masked_for<kFeatCap>(int64_t, int, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&,
                                                 const MaskedArgs&, dim3, cudaStream_t, int);
-extern template int launch_masked_for<kFeatDistance>(int64_t, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&,
+extern template int launch_masked_for<kFeatDistance>(int64_t, int, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&,
                                                      const MaskedArgs&, dim3, cudaStream_t, int);
-extern template int launch_masked_for<kFeatMask>(int64_t, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&,
+extern template int launch_masked_for<kFeatMask>(int64_t, int, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&,
                                                  const MaskedArgs&, dim3, cudaStream_t, int);
-extern template int launch_masked_for<kFeatAny>(int64_t, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&,
+extern template int launch_masked_for<kFeatAny>(int64_t, int, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&,
                                                 const MaskedArgs&, dim3, cudaStream_t, int);
 
 }  // namespace npub200

@@ -3,7 +3,7 @@
 
 namespace npub200 {
 
-template int launch_masked_for<0>(int64_t, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&,
+template int launch_masked_for<0>(int64_t, int, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&,
                                   const MaskedArgs&, dim3, cudaStream_t, int);
 
 }  // namespace npub200
