@@ -233,15 +233,14 @@ __device__ __forceinline__ float modify_scores(const MaskedArgs& m, const Row& w
     for (int t = 0; t < BN; t += 2) big = fmax3(big, fabsf(s[t]), fabsf(s[t + 1]));
     if (__all_sync(0xffffffffu, big * m.cap_in <= 1.0f)) {
       // The usual case, on the FMA pipe (the MUFU has the softmax's exponentials to do): cap tanh(y) = y P(y^2).
+const uint64_t in2 = f2_pack(m.cap_in, m.cap_in);
 #pragma unroll
-      for (int t = 0; t < BN; ++t) {
-        const float y = s[t] * m.cap_in, z = y * y;
-        float p = fmaf(m.cap_poly[5], z, m.cap_poly[4]);
-        p = fmaf(p, z, m.cap_poly[3]);
-        p = fmaf(p, z, m.cap_poly[2]);
-        p = fmaf(p, z, m.cap_poly[1]);
-        p = fmaf(p, z, m.cap_poly[0]);
-        s[t] = y * p;
+      for (int t = 0; t < BN; t += 2) {
+        const uint64_t y = f2_mul(f2_pack(s[t], s[t + 1]), in2), z = f2_mul(y, y);
+        uint64_t p = f2_pack(m.cap_poly[5], m.cap_poly[5]);
+#pragma unroll
+        for (int e = 4; e >= 0; --e) p = f2_fma(p, z, f2_pack(m.cap_poly[e], m.cap_poly[e]));
+        f2_unpack(f2_mul(y, p), s[t], s[t + 1]);
       }
     } else {
       // tanh(y) = 1 - 2 / (1 + e^(2y)); the absolute error of a few 2^-23 stays that small next to the cap.
