@@ -399,10 +399,12 @@ __device__ __forceinline__ float masked_softmax_step(const MaskedArgs& m, const 
   float c = m.a.scale_log2;
   if constexpr (FEAT != 0) c = modify_scores<FEAT, kHalf>(m, w, key0, row_mask, s_table, s_mask, lane, s);
   if (w.lo_max > key0 || w.hi_min < key0 + kHalf) {
-    const int a = w.lo - key0, z = w.hi - key0;
+    // The keys [a, z) of this half as bits: a bit test a score instead of two comparisons.
+    const int a = max(w.lo - key0, 0), z = min(w.hi - key0, kHalf);
+    const uint32_t keep = a < z ? (0xffffffffu << a) & (0xffffffffu >> (32 - z)) : 0u;
+    static_assert(kHalf == 32, "a bit a key");
 #pragma unroll
-    for (int t = 0; t < kHalf; ++t)
-      if (t < a || t >= z) s[t] = -INFINITY;
+    for (int t = 0; t < kHalf; ++t) s[t] = (keep >> t) & 1u ? s[t] : -INFINITY;
   }
   float mx8[8];
 #pragma unroll
