@@ -236,11 +236,13 @@ int attention_masked_launch(const AttnMaskedProblem& mp, cudaStream_t stream) {
   if (p.q == nullptr || p.k == nullptr || p.v == nullptr || p.o == nullptr)
     return fail(kErrInvalid, "attention tensor pointer is null");
   if (int rc = check_masked_sizes(p.B, p.H, mp.kv_heads, p.Sq, p.Skv, p.D, p.variant)) return rc;
-  if (!(p.scale > 0.0f)) return fail(kErrInvalid, "attention scale must be positive (got %g)", double(p.scale));
+  if (!(p.scale > 0.0f && p.scale <= FLT_MAX))
+    return fail(kErrInvalid, "attention scale must be positive and finite (got %g)", double(p.scale));
   for (const void* ptr : {p.q, p.k, p.v})
     if (reinterpret_cast<uintptr_t>(ptr) & 15u) return fail(kErrInvalid, "q/k/v base addresses must be 16-byte aligned");
-  if (!(o.softcap >= 0.0f) || o.softcap > FLT_MAX)
-    return fail(kErrInvalid, "softcap must be 0 (none) or positive and finite (got %g)", double(o.softcap));
+  // (the cap and its reciprocal, times the scale and log2 e, have to stay normal numbers)
+  if (!(o.softcap == 0.0f || (o.softcap >= 1e-30f && o.softcap <= 1e30f)))
+    return fail(kErrInvalid, "softcap must be 0 (none) or positive, within [1e-30, 1e30] (got %g)", double(o.softcap));
   if (!o.causal && (o.prefix != 0 || o.prefixes != nullptr))
     return fail(kErrInvalid, "a prefix needs the causal mask");
   if (o.doc_offsets != nullptr) {

@@ -104,6 +104,15 @@ def gemm(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, out
     the cached weight descriptor is used.
     """
     _require_cuda(x, "x")
+    act = 0
+    if activation is not None:
+        act = _lib.ACTIVATIONS.get(activation, 0)
+        if not act:
+            raise ValueError(f"unknown activation {activation!r} (one of {', '.join(_lib.ACTIVATIONS)})")
+        handle = None  # the activation's entry point takes the weight itself
+        ops = _lib.torch_ops()
+        if ops is not None:  # the operator checks every tensor itself
+            return ops.gemm(x, w, bias, out, variant, out_dtype, 0, residual, act)
     if x.dtype != torch.bfloat16 or w.dtype != torch.bfloat16:
         raise ValueError("gemm operands must be bf16")
     if x.dim() != 2 or w.dim() != 2 or x.stride(1) != 1 or w.stride(1) != 1:
@@ -128,14 +137,8 @@ def gemm(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, out
                 residual.stride(1) != 1:
             raise ValueError("residual must be a bf16 [M, N] matrix with contiguous rows")
         handle = None  # the residual entry point takes the weight itself
-    act = 0
-    if activation is not None:
-        act = _lib.ACTIVATIONS.get(activation, 0)
-        if not act:
-            raise ValueError(f"unknown activation {activation!r} (one of {', '.join(_lib.ACTIVATIONS)})")
-        handle = None  # and so does the activation's
     if ops is not None:
-        return ops.gemm(x, w, bias, out, int(variant), out_dtype, int(handle or 0), residual, act)
+        return ops.gemm(x, w, bias, out, int(variant), out_dtype, int(handle or 0), residual)
     ws = _gemm_workspace(x, None if handle is not None else w, M, K, N, variant)
     args_tail = (ctypes.c_void_p(bias.data_ptr()) if bias is not None else None,
                  _DT[bias.dtype] if bias is not None else _lib.DTYPE_BF16,
@@ -400,7 +403,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, sca
     kv_lens:       int32 [B], the valid keys of each sequence; what lies behind them is never used.
     doc_offsets:   int32 [n + 1] or [B, n + 1], nondecreasing borders of packed documents (Sq == Skv): a token sees its
                    own document only; tokens outside every document see nothing.
-    softcap:       scores become softcap * tanh(score / softcap).
+    softcap:       scores become softcap * tanh(score / softcap); within [1e-30, 1e30].
     slopes:        f32 [heads], adds -slopes[h] * |p - j|.
     distance_bias: f32 [heads, 2R + 1], adds distance_bias[h, clamp(j - p, -R, R) + R].
     mask:          bool (False hides) or additive bf16/f32, [Sq, Skv] or 4-D broadcastable to [B, heads, Sq, Skv], with
@@ -472,13 +475,13 @@ def _attention_masked(q, k, v, heads, scale, head_major_in, head_major_out, out_
         prefixes = prefix_len if isinstance(prefix_len, torch.Tensor) else None
         if prefix_len is not None and not causal:
             raise ValueError("prefix_len needs causal=True")
-        if softcap is not None and not 0.0 < softcap < 3e38:
-            raise ValueError(f"softcap must be positive and finite (got {softcap})")
+        if softcap is not None and not 1e-30 <= softcap <= 1e30:
+            raise ValueError(f"softcap must be positive, within [1e-30, 1e30] (got {softcap})")
         if scale is not None and not scale > 0.0:
             raise ValueError(f"attention scale must be positive (got {scale})")
-        return ops.attention_masked(q, k, v, out, out_dtype, heads, 0 if kv_heads is None else kv_heads or -1, head_major_in, head_major_out,
-                                    scale or 0.0, variant, causal, q_start if starts is None else None, starts,
-                                    prefix_len or 0 if prefixes is None else 0, prefixes, kv_lens, doc_offsets,
+        return ops.attention_masked(q, k, v, out, out_dtype, heads, 0 if kv_heads is None else kv_heads or -1, head_major_in,
+                                    head_major_out, scale or 0.0, variant, causal, q_start if starts is None else None,
+                                    starts, prefix_len or 0 if prefixes is None else 0, prefixes, kv_lens, doc_offsets,
                                     softcap or 0.0, slopes, distance_bias, mask)
     dims = 4 if head_major_in else 3
     dev = q.device
@@ -540,8 +543,8 @@ def _attention_masked(q, k, v, heads, scale, head_major_in, head_major_out, out_
     cap = 0.0
     if softcap is not None:
         cap = float(softcap)
-        if not 0.0 < cap < 3e38:
-            raise ValueError(f"softcap must be positive and finite (got {softcap})")
+        if not 1e-30 <= cap <= 1e30:
+            raise ValueError(f"softcap must be positive, within [1e-30, 1e30] (got {softcap})")
     if slopes is not None:
         _per_batch(slopes, "slopes", H, dev, torch.float32)
     if distance_bias is not None:

@@ -39,6 +39,9 @@ def test_unsupported_requests(kw):
     (dict(softcap=-1.0), {}),
     (dict(softcap=float("nan")), {}),
     (dict(softcap=float("inf")), {}),
+    (dict(softcap=1e-31), {}),
+    (dict(softcap=2e38), {}),
+    ({}, dict(scale=float("inf"))),
     (dict(doc_offsets=16, docs=1), dict(Skv=9)),
     (dict(doc_offsets=16, docs=-1), {}),
     (dict(distance_bias=16, max_distance=-1), {}),

@@ -399,6 +399,31 @@ def test_ctypes_binding_gives_the_same(cuda_device, monkeypatch):
     assert torch.equal(c, kernels.attention(s, s, s, 2, **kd))
 
 
+@pytest.mark.parametrize("cap", [1e-30, 1e-6, 1e6, 1e30])
+def test_extreme_caps(cuda_device, cap):
+    """Caps that flatten every score and caps that change none, at the ends of the range."""
+    run(cuda_device, 2, 4, 2, 70, 300, 64, q_scale=3.0, softcap=cap, causal=True)
+
+
+@pytest.mark.parametrize("B,H,Hk,Sq,Skv,D", [
+    (1, 2, 2, 128, 256, 64), (1, 2, 2, 128, 255, 64), (1, 2, 2, 128, 320, 64), (3, 4, 2, 300, 321, 80), (2, 2, 1, 200, 449, 96),
+    (2, 4, 4, 130, 1000, 128), (2, 8, 4, 500, 500, 160), (2, 8, 8, 2100, 300, 136), (1, 4, 4, 777, 777, 40)])
+def test_two_streams_of_key_tiles(cuda_device, B, H, Hk, Sq, Skv, D):
+    """Few CTAs, or head dims of which an SM holds one CTA, over at least four key tiles: even and odd numbers of tiles,
+    rows that see a tile of one stream only, rows that see nothing."""
+    lens = ints(cuda_device, *[max(Skv - 130 * b, 1) for b in range(B)])
+    run(cuda_device, B, H, Hk, Sq, Skv, D, causal=True, kv_lens=lens, seed=Skv)
+    run(cuda_device, B, H, Hk, Sq, Skv, D, causal=True, q_start=-70, head_major=True, out_dtype=BF16, seed=Skv + 1)
+    run(cuda_device, B, H, Hk, Sq, Skv, D, softcap=3.0, q_scale=8.0, seed=Skv + 2)
+    one = torch.zeros(Sq, Skv, dtype=torch.bool, device=cuda_device)
+    one[torch.arange(Sq), torch.arange(Sq) * 7 % Skv] = True  # a single key a row
+    one[3] = False
+    run(cuda_device, B, H, Hk, Sq, Skv, D, mask=one, seed=Skv + 3)
+    slopes = torch.rand(H, device=cuda_device)
+    table = torch.randn(H, 41, device=cuda_device)
+    run(cuda_device, B, H, Hk, Sq, Skv, D, slopes=slopes, distance_bias=table, kv_lens=lens, seed=Skv + 4)
+
+
 def test_refusals(cuda_device):
     from npu_ai_b200 import kernels
     dev = cuda_device
