@@ -383,6 +383,25 @@ def test_forced_timeout_reports_status_and_recovers(cuda_device):
     run(cuda_device, 1, 2, 2, 256, 512, 40, causal=True)
 
 
+@pytest.mark.parametrize("variant", [1, 2])
+def test_forced_timeout_with_two_streams(cuda_device, variant):
+    """The same with two streams of key tiles in a CTA (eight tiles, whole and in two parts)."""
+    from npu_ai_b200 import kernels
+    q, k, v = _qkv(1, 2, 2, 256, 512, 64, 2, cuda_device)
+    mask = torch.ones(256, 512, dtype=torch.bool, device=cuda_device)
+    kernels.status(cuda_device)
+    kernels.set_wait_timeout_ns(2_000_000)
+    kernels.set_debug_flags(1)
+    try:
+        kernels.attention(q, k, v, 2, mask=mask, variant=variant)
+        with pytest.raises(RuntimeError, match="failure status"):
+            kernels.check_status(cuda_device)
+    finally:
+        kernels.set_debug_flags(0)
+        kernels.set_wait_timeout_ns(0)
+    run(cuda_device, 1, 2, 2, 256, 512, 64, mask=mask, variant=variant)
+
+
 def test_ctypes_binding_gives_the_same(cuda_device, monkeypatch):
     """Without the torch operators the same call goes through ctypes."""
     from npu_ai_b200 import _lib, kernels
