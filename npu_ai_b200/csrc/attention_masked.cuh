@@ -39,6 +39,7 @@ constexpr int kMaskedBN = 64;        // keys per tile
 constexpr int kHalf = kMaskedBN / 2;  // keys per softmax thread: two warps share the rows of a TMEM lane quarter
 constexpr int kSoftWarps = 2 * kSoftmaxWarps;  // of a stream of key tiles
 constexpr int kMaxSplits = 64;
+constexpr int kMaxCluster = 16;  // parts that are joined within a cluster of CTAs
 constexpr int kTableMargin = 128;     // repeated ends of the distance bias in shared memory, either side
 constexpr int kTableSmemMax = 10240;  // bytes: keeps two CTAs per SM
 
@@ -52,6 +53,7 @@ struct MaskedArgs {
   int tiles;          // Q tiles along the positions
   int pairs, groups;  // (batch, head group) pairs, groups of a sequence: the grid is pairs x tiles x splits
   int splits;
+  int cluster;        // the parts of a tile are a cluster, which joins them through its shared memory
   float* part_o;      // [splits][pairs][tiles][128][D] unnormalised O rows
   float2* part_ml;    // [splits][pairs][tiles][128] (max in log2 units, sum)
   int causal;
@@ -457,9 +459,10 @@ __device__ __forceinline__ void st_global_v4(uint64_t to, const uint4& v) {
 // to `dst` (each lane's own row, null: no row): `cols` columns from o_addr on (a multiple of 8; the padded
 // columns are whole sixteens) as f32 or bf16. A lane holds a row, so rows go through shared memory (`stage`, an odd
 // number of 16-byte words apart) and out in 16-byte words along them. Rolled loops: this runs once a tile, and
-// straight-line code for every head dim and type was paid for in instruction fetches.
+// straight-line code for every head dim and type was paid for in instruction fetches. `keep`: only staged.
 __device__ __forceinline__ void store_rows(uint32_t o_addr, uint32_t o_addr2, uint8_t* stage, int cols, bool f32,
-                                           uint8_t* dst, float inv, float inv2, bool zero, int lane) {
+                                           uint8_t* dst, float inv, float inv2, bool zero, int lane,
+                                           bool keep = false) {
   const int words = cols * (f32 ? 4 : 2) / 16;  // 16-byte words of a row
   const int pitch = (words | 1) * 16;
   uint8_t* mine = stage + lane * pitch;
@@ -492,6 +495,7 @@ __device__ __forceinline__ void store_rows(uint32_t o_addr, uint32_t o_addr2, ui
       }
     }
   }
+  if (keep) return;
   __syncwarp();
   int row = lane / words, c = lane - row * words;
   const int step_row = 32 / words, step_c = 32 - step_row * words;
@@ -518,6 +522,83 @@ __device__ __forceinline__ void store_rows(uint32_t o_addr, uint32_t o_addr2, ui
   }
 }
 
+// Eight columns of an output row, from element offset `at` on.
+__device__ __forceinline__ void write_columns(const MaskedArgs& m, long long at, const float (&o)[8]) {
+  if (m.a.out_f32) {
+    float* dst = static_cast<float*>(m.a.out) + at;
+    if (m.out_vec) {
+      reinterpret_cast<float4*>(dst)[0] = make_float4(o[0], o[1], o[2], o[3]);
+      reinterpret_cast<float4*>(dst)[1] = make_float4(o[4], o[5], o[6], o[7]);
+    } else {
+#pragma unroll
+      for (int t = 0; t < 8; ++t) dst[t] = o[t];
+    }
+  } else {
+    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(m.a.out) + at;
+    if (m.out_vec) {
+      *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]),
+                                                  pack_bf16x2(o[4], o[5]), pack_bf16x2(o[6], o[7]));
+    } else {
+#pragma unroll
+      for (int t = 0; t < 8; ++t) dst[t] = __float2bfloat16_rn(o[t]);
+    }
+  }
+}
+
+// Joins the parts of the tile's rows, which the CTAs of the cluster hold as staged rows and (max, sum) pairs in shared
+// memory: with M = max of the parts' maxima, o = sum_z 2^(m_z - M) O_z / sum_z 2^(m_z - M) l_z, in part order. CTA `rank`
+// takes every splits-th row, a thread eight columns.
+template <int DP, int STREAMS>
+__device__ __noinline__ void join_cluster(const MaskedArgs& m, const uint8_t* smem, const float2* s_ml, int tile, int h0,
+                                          int bb, int rank) {
+  using OPart = OColumns<DP, 2 * STREAMS>;
+  const AttnArgs& args = m.a;
+  const int chunks = args.D / 8, splits = m.splits;
+  const int items = (m.pack * m.T - rank + splits - 1) / splits * chunks;
+  for (int k = int(threadIdx.x); k < items; k += STREAMS * kSoftWarps * 32) {
+    const int r = rank + k / chunks * splits, c = k % chunks * 8;
+    const int q = (r * m.inv_row) >> 16;
+    const int i = tile * m.T + (m.head_fast ? q : r - q * m.T), head = h0 + (m.head_fast ? r - q * m.pack : q);
+    if (i >= args.Sq) continue;
+    float wz[kMaxCluster], lz[kMaxCluster];
+    float top = -INFINITY;
+#pragma unroll
+    for (int z = 0; z < kMaxCluster; ++z) {
+      wz[z] = -INFINITY;
+      lz[z] = 0.0f;
+      if (z < splits) ld_cluster_f32x2(cluster_smem_addr(s_ml + r, uint32_t(z)), wz[z], lz[z]);
+    }
+#pragma unroll
+    for (int z = 0; z < kMaxCluster; ++z) top = fmaxf(top, wz[z]);
+    float sum = 0.0f;
+#pragma unroll
+    for (int z = 0; z < kMaxCluster; ++z) {
+      wz[z] = wz[z] == -INFINITY ? 0.0f : fast_exp2(wz[z] - top);
+      sum = fmaf(wz[z], lz[z], sum);
+    }
+    const int part = c / OPart::kWidth, begin = OPart::begin(part);
+    const int cols = min(args.D, OPart::begin(part + 1)) - begin;
+    const int warp = (part >> 1) * kSoftWarps + (part & 1) * kSoftmaxWarps + (r >> 5);
+    const uint8_t* src = smem + warp * 32 * ((OPart::kWidth * 4 / 16) | 1) * 16 + (r & 31) * ((cols / 4) | 1) * 16 +
+                         (c - begin) * 4;
+    float o[8] = {};
+#pragma unroll
+    for (int z = 0; z < kMaxCluster; ++z) {
+      if (wz[z] != 0.0f) {  // a part that saw nothing staged no row
+        const uint32_t at = cluster_smem_addr(src, uint32_t(z));
+        const float4 a = ld_cluster_f32x4(at), b = ld_cluster_f32x4(at + 16);
+        const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int t = 0; t < 8; ++t) o[t] = fmaf(wz[z], v[t], o[t]);
+      }
+    }
+    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+    for (int t = 0; t < 8; ++t) o[t] *= inv;
+    write_columns(m, (long long)bb * args.o_sb + (long long)i * args.o_ss + (long long)head * args.o_sh + c, o);
+  }
+}
+
 template <int DP, int STAGES, int STREAMS>
 struct MaskedLayout {
   static constexpr int BN = kMaskedBN;
@@ -539,8 +620,10 @@ struct MaskedLayout {
   static constexpr int kMaxOff = kMaskOff + STREAMS * kSoftWarps * kHalf * 4;
   // both streams' sums [stream][half][row] and maxima [stream][row]
   static constexpr int kJoinOff = kMaxOff + STREAMS * 2 * 2 * kAttnBM * 4;
+  // the rows' (max, sum) for the other CTAs of a cluster
+  static constexpr int kMlOff = kJoinOff + (STREAMS > 1 ? 6 * kAttnBM * 4 : 0);
   // the head's distance bias (launch-sized)
-  static constexpr int kTableOff = kJoinOff + (STREAMS > 1 ? 6 * kAttnBM * 4 : 0);
+  static constexpr int kTableOff = kMlOff + kAttnBM * 8;
   static constexpr int kSmemBytes = kTableOff + 1024;
   // The output rows' staging (f32 rows, an odd number of words apart) reuses Q, K and V.
   static_assert(kBarOff >= STREAMS * kSoftWarps * 32 * (OColumns<DP, 2 * STREAMS>::kWidth * 4 + 16),
@@ -813,6 +896,8 @@ __global__ void __launch_bounds__(MaskedLayout<DP, STAGES, STREAMS>::kThreads,
         run_sum = fmaf(s_join[2 * e * kAttnBM] + s_join[(2 * e + 1) * kAttnBM], weight[e], run_sum);
       }
     }
+    float2* s_ml = reinterpret_cast<float2*>(smem + L::kMlOff);
+    if (m.cluster && warp < kSoftmaxWarps) s_ml[row] = make_float2(ok ? run_max : -INFINITY, run_sum);
     if (ok && __any_sync(0xffffffffu, w.valid)) {
       tc_fence_after();
       const bool empty = run_max == -INFINITY;       // the row has seen no key
@@ -825,11 +910,11 @@ __global__ void __launch_bounds__(MaskedLayout<DP, STAGES, STREAMS>::kThreads,
           (long long)bb * args.o_sb + (long long)w.i * args.o_ss + (long long)w.head * args.o_sh + begin;
       uint8_t* stage = smem + warp * 32 * ((OPart::kWidth * esz / 16) | 1) * 16;
       uint8_t* dst = nullptr;
-      if (m.splits > 1) {
+      if (m.splits > 1 && !m.cluster) {
         const long long at = (((long long)split * m.pairs + pair) * m.tiles + tile) * kAttnBM + row;
         if (w.valid && part == 0) m.part_ml[at] = make_float2(run_max, empty ? 0.0f : run_sum);
         if (w.valid && !empty) dst = reinterpret_cast<uint8_t*>(m.part_o + at * args.D + begin);
-      } else if (w.valid) {
+      } else if (w.valid && !m.cluster) {
         dst = static_cast<uint8_t*>(args.out) + obase * esz;
       }
       const float inv = m.splits > 1 ? 1.0f : 1.0f / run_sum;
@@ -838,7 +923,8 @@ __global__ void __launch_bounds__(MaskedLayout<DP, STAGES, STREAMS>::kThreads,
       if (cols <= 0) {
         // nothing of the true head dim in this half
       } else if (m.splits > 1 ? nkv > 0 : m.out_vec != 0) {
-        store_rows(o_at, o_at2, stage, cols, wide, dst, inv * weight[0], inv * weight[1], empty, lane);
+        store_rows(o_at, o_at2, stage, cols, wide, dst, inv * weight[0], inv * weight[1], empty, lane,
+                   m.cluster != 0);
       } else if (m.splits == 1) {
         // Output rows that 16-byte words do not reach.
         for (int c = 0; c < cols; c += 8) {
@@ -872,6 +958,12 @@ __global__ void __launch_bounds__(MaskedLayout<DP, STAGES, STREAMS>::kThreads,
     tc_fence_after();
     tmem_dealloc(tmem_base, L::kTmemCols);
   }
+  if (m.cluster) {  // (after TMEM is free: a CTA that waits for it elsewhere may belong to this cluster)
+    cluster_sync();
+    if (warp < STREAMS * kSoftWarps)
+      join_cluster<DP, STREAMS>(m, smem, reinterpret_cast<const float2*>(smem + L::kMlOff), tile, h0, bb, split);
+    cluster_sync();  // no CTA leaves while another reads its rows
+  }
 }
 
 template <int DP, int STAGES, int STREAMS, int FEAT>
@@ -887,9 +979,25 @@ int launch_masked(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMa
                                                  L::kSmemBytes + kTableSmemMax),
                             "cudaFuncSetAttribute(masked attention smem)"))
       return rc;
+    if (int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1),
+                            "cudaFuncSetAttribute(masked attention cluster)"))
+      return rc;
     configured[device] = true;
   }
-  return check_cuda(launch_pdl(kern, grid, dim3(L::kThreads), smem, st, mq, mk, mv, m), "masked attention kernel launch");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(L::kThreads);
+  cfg.dynamicSmemBytes = size_t(smem);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = grid.z;
+  cfg.attrs = attr;
+  cfg.numAttrs = m.cluster ? 2 : 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, mq, mk, mv, m), "masked attention kernel launch");
 }
 
 template <int FEAT>

@@ -251,6 +251,9 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t cluster_addr) {
                : "memory");
   return v;
 }
+__device__ __forceinline__ void ld_cluster_f32x2(uint32_t cluster_addr, float& x, float& y) {
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x), "=f"(y) : "r"(cluster_addr) : "memory");
+}
 // Every thread of both CTAs: shared-memory writes (barrier inits included) before it are visible to the pair after.
 // The non-.aligned forms, so threads of a warp may reach it at different times (roles run on single lanes).
 __device__ __forceinline__ void cluster_sync() {
