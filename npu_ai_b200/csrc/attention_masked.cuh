@@ -222,6 +222,52 @@ __device__ __forceinline__ void prefetch_mask(const MaskedArgs& m, const Row& w,
   for (int k = 0; k < esz; ++k) asm volatile("prefetch.global.L1 [%0];" ::"l"(p + 32 * k));
 }
 
+// 16 bytes from offset `o` (0 ... 15) of two consecutive 16-byte words.
+__device__ __forceinline__ uint4 bytes_at(const uint4& a, const uint4& b, uint32_t o) {
+  const bool two = o & 8u, one = o & 4u;
+  const uint32_t t[6] = {two ? a.z : a.x, two ? a.w : a.y, two ? b.x : a.z,
+                         two ? b.y : a.w, two ? b.z : b.x, two ? b.w : b.y};
+  uint32_t u[5];
+#pragma unroll
+  for (int e = 0; e < 5; ++e) u[e] = one ? t[e + 1] : t[e];
+  const uint32_t s = 8 * (o & 3u);
+  return make_uint4(__funnelshift_r(u[0], u[1], s), __funnelshift_r(u[1], u[2], s), __funnelshift_r(u[2], u[3], s),
+                    __funnelshift_r(u[3], u[4], s));
+}
+
+// A mask row's bytes from p on, 32 a call. `whole`: p is aligned and the bytes are all the row's. Otherwise the aligned
+// words that hold a byte of [p, end), put together (the first and the last may hold neighbours' bytes, which share their
+// 16 bytes and so their page); what lies behind the end is zeros or a neighbour's.
+struct MaskBytes {
+  const uint4* next;
+  const uint8_t* end;
+  uint32_t o;
+  bool whole;
+  uint4 word;
+  __device__ __forceinline__ MaskBytes(const uint8_t* p, const uint8_t* row_end, bool all) : end(row_end), whole(all) {
+    o = uint32_t(reinterpret_cast<uintptr_t>(p) & 15u);
+    next = reinterpret_cast<const uint4*>(p - o);
+    if (!whole) word = load();
+  }
+  __device__ __forceinline__ uint4 load() {
+    const uint4 v = reinterpret_cast<const uint8_t*>(next) < end ? __ldg(next) : make_uint4(0u, 0u, 0u, 0u);
+    ++next;
+    return v;
+  }
+  __device__ __forceinline__ void take(uint4 (&v)[2]) {
+    if (whole) {
+      v[0] = __ldg(next);
+      v[1] = __ldg(next + 1);
+      next += 2;
+    } else {
+      const uint4 a = load(), b = load();
+      v[0] = bytes_at(word, a, o);
+      v[1] = bytes_at(a, b, o);
+      word = b;
+    }
+  }
+};
+
 // The cap, the biases by distance and the mask tensor on 32 raw scores of keys from kv0 on. Returns the factor that
 // takes the result to log2 units: the scale, until something that is not a multiple of a score has been added (the
 // addition then carries it: one fused multiply-add a score).
@@ -308,58 +354,42 @@ const uint64_t in2 = f2_pack(m.cap_in, m.cap_in);
     }
     return 1.0f;
   }
-  const int n = m.a.Skv - kv0;  // readable keys from here
+  const int esz = m.mask_kind == 3 ? 4 : m.mask_kind;
+  // (scores of keys behind the last get any value here: no row sees them)
+  MaskBytes bytes(w.mask + (long long)kv0 * esz, w.mask + (long long)m.a.Skv * esz, m.mask_vec && m.a.Skv - kv0 >= BN);
   // -inf hides; any finite value, however low, stays finite in log2 units.
   auto add = [k](float x, float e) { return e == -INFINITY ? -INFINITY : fmaxf(fmaf(x, k, e * kLog2e), -FLT_MAX); };
   if (m.mask_kind == 1) {
-    const uint8_t* p = w.mask + kv0;
-    if (m.mask_vec && n >= BN) {
+    uint4 v[BN / 16];
+    bytes.take(v);
 #pragma unroll
-      for (int c = 0; c < BN / 16; ++c) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + c);
-        const uint32_t q[4] = {v.x, v.y, v.z, v.w};
+    for (int c = 0; c < BN; c += 16) {
+      const uint32_t q[4] = {v[c / 16].x, v[c / 16].y, v[c / 16].z, v[c / 16].w};
 #pragma unroll
-        for (int t = 0; t < 16; ++t) {
-          // The byte (0 or 1) as all zeros or all ones: its low bit moved to the sign and that replicated.
-          const uint32_t keep = replicate_sign(q[t / 4] << 7, t % 4);
-          s[16 * c + t] = __uint_as_float((__float_as_uint(s[16 * c + t]) & keep) | (0xff800000u & ~keep));
-        }
+      for (int t = 0; t < 16; ++t) {
+        // The byte (0 or 1) as all zeros or all ones: its low bit moved to the sign and that replicated.
+        const uint32_t keep = replicate_sign(q[t / 4] << 7, t % 4);
+        s[c + t] = __uint_as_float((__float_as_uint(s[c + t]) & keep) | (0xff800000u & ~keep));
       }
-    } else {
-#pragma unroll
-      for (int t = 0; t < BN; ++t)
-        if (t >= n || __ldg(p + t) == 0) s[t] = -INFINITY;
     }
   } else if (m.mask_kind == 2) {
-    const unsigned short* p = reinterpret_cast<const unsigned short*>(w.mask) + kv0;
-    if (m.mask_vec && n >= BN) {
 #pragma unroll
-      for (int c = 0; c < BN; c += 8) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p + c));
-        const uint32_t q[4] = {v.x, v.y, v.z, v.w};
+    for (int c = 0; c < BN; c += 16) {
+      uint4 v[2];
+      bytes.take(v);
+      const uint32_t q[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
 #pragma unroll
-        for (int t = 0; t < 8; ++t)
-          s[c + t] = add(s[c + t], __uint_as_float(t & 1 ? q[t / 2] & 0xFFFF0000u : q[t / 2] << 16));
-      }
-    } else {
-#pragma unroll
-      for (int t = 0; t < BN; ++t)
-        s[t] = t < n ? add(s[t], __uint_as_float(uint32_t(__ldg(p + t)) << 16)) : -INFINITY;
+      for (int t = 0; t < 16; ++t)
+        s[c + t] = add(s[c + t], __uint_as_float(t & 1 ? q[t / 2] & 0xFFFF0000u : q[t / 2] << 16));
     }
   } else {
-    const float* p = reinterpret_cast<const float*>(w.mask) + kv0;
-    if (m.mask_vec && n >= BN) {
 #pragma unroll
-      for (int c = 0; c < BN; c += 4) {
-        const float4 v = __ldg(reinterpret_cast<const float4*>(p + c));
-        s[c] = add(s[c], v.x);
-        s[c + 1] = add(s[c + 1], v.y);
-        s[c + 2] = add(s[c + 2], v.z);
-        s[c + 3] = add(s[c + 3], v.w);
-      }
-    } else {
+    for (int c = 0; c < BN; c += 8) {
+      uint4 v[2];
+      bytes.take(v);
+      const uint32_t q[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
 #pragma unroll
-      for (int t = 0; t < BN; ++t) s[t] = t < n ? add(s[t], __ldg(p + t)) : -INFINITY;
+      for (int t = 0; t < 8; ++t) s[c + t] = add(s[c + t], __uint_as_float(q[t]));
     }
   }
   return m.mask_kind == 1 ? k : 1.0f;

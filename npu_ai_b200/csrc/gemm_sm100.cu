@@ -25,6 +25,7 @@
 // bias row (conv bias + time embedding) and a residual tensor. The only layout requirement is TMA's: 16-byte aligned base and row strides (K % 8 == 0 for a
 // dense matrix); anything else is repacked by the host into a caller-provided workspace first.
 #include <algorithm>
+#include <climits>
 #include <cstdio>
 #include <cstring>
 #include <mutex>
@@ -66,6 +67,7 @@ struct GemmArgs {
   int bias_img_pixels, bias_imgs;
   const void* residual;       // bf16 [M, N] added in the epilogue (row stride ldr), or null
   long long ldr;
+  int res_vec;  // residual columns a lane reads at once where TMA does not bring them (activation form)
   int act;                    // activation form: NPUB200_ACT_* code applied between the bias and the residual
   int cv_w, cv_hw, cv_cblocks;  // 3x3 convolution form: image width, pixels per image, 64-channel blocks of Cin
   void* out;
@@ -152,6 +154,56 @@ __device__ __forceinline__ float load_bias_own(const GemmArgs& a, int gcol, int 
   if (a.bias == nullptr || gcol + j >= a.bias_n) return 0.0f;
   return a.bias_f32 ? __ldg(static_cast<const float*>(a.bias) + row_off + gcol + j)
                     : __bfloat162float(static_cast<const __nv_bfloat16*>(a.bias)[row_off + gcol + j]);
+}
+
+// A warp's 32 x 32 bf16 residual values into its staging tile (64-byte rows, 64-byte swizzle), E columns a lane: all loads
+// of a batch before its stores, which the compiler cannot reorder (each waited for the last: 6 us a group).
+template <int E>
+__device__ __forceinline__ void stage_residual(const unsigned short* from, long long ld, int rows, int cols, uint8_t* to,
+                                               int lane) {
+  constexpr int kBatch = E == 1 ? 16 : 32 / E;
+  const int c = lane % (32 / E) * E, r0 = lane / (32 / E);
+#pragma unroll 1
+  for (int b = 0; b < 32; b += kBatch * E) {
+    uint32_t v[kBatch][(E + 1) / 2];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int rr = b + k * E + r0;
+      const unsigned short* p = from + rr * ld + c;
+#pragma unroll
+      for (int e = 0; e < (E + 1) / 2; ++e) v[k][e] = 0u;
+      if (rr < rows && c + E <= cols) {
+        if constexpr (E == 8) {
+          const uint4 t = *reinterpret_cast<const uint4*>(p);
+          v[k][0] = t.x, v[k][1] = t.y, v[k][2] = t.z, v[k][3] = t.w;
+        } else if constexpr (E == 4) {
+          const uint2 t = *reinterpret_cast<const uint2*>(p);
+          v[k][0] = t.x, v[k][1] = t.y;
+        } else if constexpr (E == 2) {
+          v[k][0] = *reinterpret_cast<const uint32_t*>(p);
+        } else {
+          v[k][0] = *p;
+        }
+      } else if (rr < rows) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (c + e < cols) v[k][e / 2] |= uint32_t(p[e]) << (e % 2 * 16);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int rr = b + k * E + r0;
+      uint8_t* q = to + rr * 64 + ((c >> 3) ^ ((rr >> 1) & 3)) * 16 + (c & 7) * 2;
+      if constexpr (E == 8)
+        *reinterpret_cast<uint4*>(q) = make_uint4(v[k][0], v[k][1], v[k][2], v[k][3]);
+      else if constexpr (E == 4)
+        *reinterpret_cast<uint2*>(q) = make_uint2(v[k][0], v[k][1]);
+      else if constexpr (E == 2)
+        *reinterpret_cast<uint32_t*>(q) = v[k][0];
+      else
+        *reinterpret_cast<unsigned short*>(q) = static_cast<unsigned short>(v[k][0]);
+    }
+  }
 }
 
 // Direct-store epilogue for outputs TMA cannot address: 32 columns of one row, rows/columns predicated with
@@ -882,6 +934,26 @@ __global__ void __launch_bounds__(64 + 32 * gemm_epi_warps<BN, MODE>(), 1)
           __syncwarp();
           uint8_t* rowp = sb + buf * 2048 + lane * 64;
           const int sw = (lane >> 1) & 3;
+          // Rows that TMA cannot address (an odd N) go through the same tiles, a row of 32 columns at a time: one row a
+          // lane, as the accumulator lies, made every access 32 separate ones (45922 x 728 x 387 with gelu and residual
+          // 256 us).
+          const int g_rows = min(32, args.M - (m0 + quarter * 32)), g_col = n0 + c + lane;
+          const bool by_rows = args.residual != nullptr && !args.tma_residual;
+          if (by_rows) {
+            const unsigned short* from = static_cast<const unsigned short*>(args.residual) +
+                                         (long long)(m0 + quarter * 32) * args.ldr + n0 + c;
+            uint8_t* to = sb + buf * 2048;
+            const int g_cols = args.N - (n0 + c);
+            if (args.res_vec == 8)
+              stage_residual<8>(from, args.ldr, g_rows, g_cols, to, lane);
+            else if (args.res_vec == 4)
+              stage_residual<4>(from, args.ldr, g_rows, g_cols, to, lane);
+            else if (args.res_vec == 2)
+              stage_residual<2>(from, args.ldr, g_rows, g_cols, to, lane);
+            else
+              stage_residual<1>(from, args.ldr, g_rows, g_cols, to, lane);
+            __syncwarp();
+          }
           if (staged) {
             if (!mbar_wait_bounded_warp(&my_res[buf], (res_phase >> buf) & 1u, abort_flag, args.ctl,
                                         kStatusTimeoutEpilogue)) {
@@ -890,6 +962,8 @@ __global__ void __launch_bounds__(64 + 32 * gemm_epi_warps<BN, MODE>(), 1)
             }
             res_phase ^= 1u << buf;
             res_pending &= ~(1u << buf);
+          }
+          if (staged || by_rows) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const uint4 t = *reinterpret_cast<const uint4*>(rowp + (j ^ sw) * 16);
@@ -899,15 +973,11 @@ __global__ void __launch_bounds__(64 + 32 * gemm_epi_warps<BN, MODE>(), 1)
                 v2[4 * j + e] = f2_add(v2[4 * j + e], f2_pack(__uint_as_float(w4[e] << 16),
                                                              __uint_as_float(w4[e] & 0xFFFF0000u)));
             }
+            if (by_rows) __syncwarp();  // f32 output rows take the places of other lanes' residual rows
           }
           float v[32];
 #pragma unroll
           for (int j = 0; j < 16; ++j) f2_unpack(v2[j], v[2 * j], v[2 * j + 1]);
-          if (args.residual != nullptr && !args.tma_residual) add_residual32(args, m0 + row, n0 + c, v);
-          if (!args.tma_store) {
-            store_row32_direct(args, m0 + row, n0 + c, v);
-            continue;
-          }
           if (args.out_f32) {
             uint8_t* row4 = sb + lane * 128;
 #pragma unroll
@@ -920,6 +990,23 @@ __global__ void __launch_bounds__(64 + 32 * gemm_epi_warps<BN, MODE>(), 1)
               *reinterpret_cast<uint4*>(rowp + (j ^ sw) * 16) =
                   make_uint4(pack_bf16x2(v[8 * j], v[8 * j + 1]), pack_bf16x2(v[8 * j + 2], v[8 * j + 3]),
                              pack_bf16x2(v[8 * j + 4], v[8 * j + 5]), pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
+          }
+          if (!args.tma_store) {
+            __syncwarp();
+            if (g_col < args.N) {
+              const long long at = (long long)(m0 + quarter * 32) * args.ldo + g_col;
+#pragma unroll 4
+              for (int rr = 0; rr < g_rows; ++rr) {
+                if (args.out_f32)
+                  static_cast<float*>(args.out)[at + rr * args.ldo] = *reinterpret_cast<const float*>(
+                      sb + rr * 128 + ((lane >> 2) ^ (rr & 7)) * 16 + (lane & 3) * 4);
+                else
+                  static_cast<unsigned short*>(args.out)[at + rr * args.ldo] = *reinterpret_cast<const unsigned short*>(
+                      sb + buf * 2048 + rr * 64 + ((lane >> 3) ^ ((rr >> 1) & 3)) * 16 + (lane & 7) * 2);
+              }
+            }
+            __syncwarp();
+            continue;
           }
           fence_proxy_async_smem();
           __syncwarp();
@@ -1344,6 +1431,8 @@ int gemm_launch(const GemmProblem& p, cudaStream_t stream) {
   GemmArgs a;
   memset(&a, 0, sizeof(a));
   a.tma_residual = tma_residual ? 1 : 0;
+  const uintptr_t res_align = reinterpret_cast<uintptr_t>(p.residual) | uintptr_t(p.ldr * 2);
+  a.res_vec = res_align % 16 == 0 ? 8 : res_align % 8 == 0 ? 4 : res_align % 4 == 0 ? 2 : 1;
   a.tma_store = tma_store ? 1 : 0;
   a.M = int(p.M);
   a.N = int(p.N);
@@ -1544,12 +1633,20 @@ size_t conv3x3_workspace_bytes(int64_t n, int64_t h, int64_t w, int64_t cin, int
 // ---------------------------------------------------------------------------------------------------------------
 __global__ void repack_rows_bf16_kernel(const __nv_bfloat16* __restrict__ src, long long ld_src, long long rows,
                                         long long cols, __nv_bfloat16* __restrict__ dst, long long cols_pad) {
-  const long long total = rows * cols_pad;
+  // Eight columns (a 16-byte word of dst) a thread: one division and one store for them, the 2-byte loads of a warp
+  // within 512 bytes of a row.
+  const int chunks = int(cols_pad / 8);
+  const long long total = rows * chunks;
+  const unsigned short* from = reinterpret_cast<const unsigned short*>(src);
   for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total;
        i += (long long)gridDim.x * blockDim.x) {
-    const long long r = i / cols_pad;
-    const long long c = i - r * cols_pad;
-    dst[i] = c < cols ? src[r * ld_src + c] : __float2bfloat16_rn(0.0f);
+    const long long r = total <= INT_MAX ? int(i) / chunks : i / chunks;
+    const long long c = (i - r * chunks) * 8;
+    uint32_t w[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = c + e < cols ? from[r * ld_src + c + e] : 0u;
+    reinterpret_cast<uint4*>(dst)[i] =
+        make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
   }
 }
 
@@ -1557,7 +1654,9 @@ int repack_rows_bf16(const void* src, int64_t ld_src, int64_t rows, int64_t cols
                      cudaStream_t stream) {
   const DeviceInfo* dev = nullptr;
   if (int rc = current_device_info(&dev)) return rc;
-  const long long total = rows * cols_pad;
+  if (cols_pad % 8 != 0 || (reinterpret_cast<uintptr_t>(dst) & 15u) != 0)
+    return fail(kErrInvalid, "repacked rows must be whole 16-byte words");
+  const long long total = rows * (cols_pad / 8);
   const int threads = 256;
   const long long want = (total + threads - 1) / threads;
   const int grid = int(std::max<long long>(1, std::min<long long>(want, int64_t(dev->sms) * 8)));

@@ -77,6 +77,26 @@ def test_every_tile(cuda_device, variant):
         _check(_run(cuda_device, x, w, None, None, act, out_dtype=torch.float32, variant=variant), x, w, None, None, act)
 
 
+@pytest.mark.parametrize("M,K,N,out_dtype", [(700, 728, 387, torch.bfloat16), (700, 728, 387, torch.float32),
+                                             (129, 147, 99, torch.bfloat16), (33, 2360, 665, torch.float32),
+                                             (513, 3594, 73, torch.bfloat16), (20000, 72, 325, torch.bfloat16)])
+def test_rows_that_tma_does_not_address(cuda_device, M, K, N, out_dtype):
+    """Odd N: output and residual rows at any 2-byte address; K off a multiple of 8: repacked operands. What lies beside
+    the output rows stays as it was, and the residual may be the output."""
+    from npu_ai_b200 import kernels
+    x, w, b, r = _case(M, K, N, torch.float32, True, seed=M + N)
+    for act, res in (("gelu", r), ("silu", None)):
+        _check(_run(cuda_device, x, w, b, res, act, out_dtype=out_dtype), x, w, b, res, act)
+    buf = torch.full((M + 2, N + 6), 7.0, dtype=torch.bfloat16, device=cuda_device)
+    view = buf[1:M + 1, 3:N + 3]
+    view.copy_(r)
+    out = kernels.gemm(x.to(cuda_device), w.to(cuda_device), b.to(cuda_device), out=view, residual=view, activation="relu")
+    kernels.check_status(cuda_device)
+    _check(out.contiguous(), x, w, b, r, "relu")
+    buf[1:M + 1, 3:N + 3] = 7.0
+    assert bool((buf == 7.0).all())
+
+
 def test_strided_operands_and_in_place_residual(cuda_device):
     """Row strides past the row length for every operand; the residual may be the output itself; columns and rows
     outside the output view stay as they were."""
