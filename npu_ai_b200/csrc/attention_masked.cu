@@ -149,6 +149,12 @@ int check_masked_sizes(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Skv
   return kOk;
 }
 
+// Two streams of key tiles in a CTA where an SM holds one CTA anyway (by its size, or because there are no more) and each
+// stream has two tiles at least. 2x8x1024x1024x80 with a mask of its own rows: 32.5 us with one stream, 18.3 with two.
+bool two_streams(int64_t D, int64_t ctas, int64_t tiles, int sms) {
+  return D <= 160 && (D > 128 || ctas <= sms) && tiles >= 4;
+}
+
 int plan_masked(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Skv, int64_t D, int variant, int sms,
                 MaskedPlan* out) {
   const int64_t G = H / Hk;
@@ -171,25 +177,36 @@ int plan_masked(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Skv, int64
   const int64_t key_tiles = (Skv + kMaskedBN - 1) / kMaskedBN;
   const int64_t slots = (D <= 128 ? 2 : 1) * int64_t(sms);  // resident CTAs
   p.splits = 1;
-  p.streams = 1;
   if (variant > 0) {
     p.splits = variant;
-  } else if (2 * ctas <= slots && key_tiles >= 8) {
-    // Fill the slots; several waves where the parts stay long (32 tiles at one wave), which evens out ragged lengths.
-    // With many rows the partial results are worth their traffic only in parts of at least 16 tiles (16384 rows of 1024
-    // keys: 30 us whole, 33 us in two parts).
-    const int64_t want = key_tiles * ctas >= 32 * slots ? 5 * slots / (2 * ctas) : slots / ctas;
-    const int64_t most = B * H * Sq <= kJoinFewRows ? key_tiles : key_tiles / 16;
-    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>({want, most, kMaxSplits}));
-    const int64_t per = (key_tiles + parts - 1) / parts;
-    p.splits = int((key_tiles + per - 1) / per);
+  } else if (2 * ctas <= slots && key_tiles >= 4) {
+    if (key_tiles * ctas >= 32 * slots) {
+      // Many long rows: parts of at least 32 tiles, several waves of them, which evens out ragged lengths.
+      p.splits = int(std::min<int64_t>(5 * slots / (2 * ctas), kMaxSplits));
+    } else {
+      // The number of parts with the least time, in us: its tiles one after the other (0.7 with two streams, 1.3 without),
+      // and the partial results' way out and in (0.8 a MB) with what a join costs by itself. Measured against the
+      // choice: 1x4x1024x1024x64 16.1 us whole, 13.8 / 12.5 / 13.7 in 2 / 4 / 8 parts; 1x8x512x512x128 11.4 whole,
+      // 13.3 in 2; 8 pairs of 20 rows over 79 tiles 92.6 whole, 13.7 / 13.0 / 12.7 in 12 / 16 / 27.
+      double best = 0;
+      const int64_t most = std::min<int64_t>({slots / ctas, key_tiles, kMaxSplits});
+      for (int64_t parts = 1; parts <= most; ++parts) {
+        const int64_t per = (key_tiles + parts - 1) / parts;
+        if ((key_tiles + per - 1) / per != parts) continue;  // the same tiles a part in fewer parts
+        const double us = double(per) * (two_streams(D, ctas * parts, per, sms) ? 0.7 : 1.3) +
+                          (parts > 1 ? 1.5 + 0.8e-6 * double(B * H * Sq * parts * D * 4) : 0.0);
+        if (parts == 1 || us < best) {
+          best = us;
+          p.splits = int(parts);
+        }
+      }
+    }
   }
-  // Where an SM holds one CTA anyway, that CTA runs two streams of key tiles.
-  if (D <= 160 && (D > 128 || ctas * p.splits <= sms) && key_tiles >= 4 * p.splits) p.streams = 2;
-  // Few parts are joined by a cluster: no workspace, no second launch. The GPU time is the same (2 x 13 parts 6.8 us, with
-  // the second kernel 7.1), but the call takes some 4 us less on the host, which is what so small a call waits for. Larger
-  // ones run out of places for whole clusters: 8 x 16 parts take 21.7 us, through the workspace 13.0.
-  p.cluster = p.splits > 1 && p.splits <= kMaxCluster && 4 * ctas * p.splits <= sms;
+  p.streams = two_streams(D, ctas * p.splits, key_tiles / p.splits, sms) ? 2 : 1;
+  // Few parts are joined by a cluster: no workspace, no second launch. The GPU time is that of the second kernel or less
+  // (2 x 13 parts 6.8 us, with the second kernel 7.1), and the call takes some 4 us less on the host, which is what a
+  // small call waits for. Large clusters run out of places: 8 x 16 parts take 21.7 us, through the workspace 13.0.
+  p.cluster = p.splits > 1 && p.splits <= kMaxCluster && (p.splits <= 4 ? 1 : 4) * ctas * p.splits <= sms;
   if (p.splits > 1 && !p.cluster) {
     if (B * H * Sq > INT32_MAX / kMaxSplits)
       return fail(kErrUnsupported, "too many rows to split their keys (%lld)", (long long)(B * H * Sq));

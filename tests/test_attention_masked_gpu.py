@@ -418,6 +418,27 @@ def test_ctypes_binding_gives_the_same(cuda_device, monkeypatch):
     assert torch.equal(c, kernels.attention(s, s, s, 2, **kd))
 
 
+@pytest.mark.parametrize("B,H,Hk,Sq,Skv,D", [
+    (1, 2, 1, 1, 777, 64), (1, 4, 4, 300, 1100, 64), (1, 2, 2, 1000, 2000, 40), (1, 3, 3, 128, 600, 136), (2, 6, 2, 9, 450, 72),
+    (1, 1, 1, 40, 1000, 256), (1, 2, 2, 1, 800, 8), (3, 8, 1, 3, 300, 200)])
+@pytest.mark.parametrize("variant", [0, 2, 3, 4, 7, 13, 16])
+def test_parts_joined_by_a_cluster(cuda_device, B, H, Hk, Sq, Skv, D, variant):
+    """Few parts of few CTAs are joined through the shared memory of a cluster: parts without a tile, rows that a part
+    does not see, output rows of every alignment."""
+    from npu_ai_b200 import kernels
+    lens = ints(cuda_device, *[max(Skv - 200 * b, 1) for b in range(B)])
+    run(cuda_device, B, H, Hk, Sq, Skv, D, causal=True, kv_lens=lens, variant=variant, seed=Skv)
+    run(cuda_device, B, H, Hk, Sq, Skv, D, softcap=6.0, q_scale=4.0, head_major=True, out_dtype=BF16, variant=variant, seed=1)
+    q, k, v = _qkv(B, H, Hk, Sq, Skv, D, 2, cuda_device)
+    buf = torch.full((B, Sq, H * D + 3), 7.0, dtype=BF16, device=cuda_device)
+    view = buf[..., 1:H * D + 1]
+    kernels.attention(q, k, v, H, kv_heads=Hk, kv_lens=lens, out=view, variant=variant)
+    kernels.check_status(cuda_device)
+    check(view.contiguous(), *oracle(q, k, v, H, Hk, kv_lens=lens), H, False)
+    view.fill_(7.0)
+    assert bool((buf == 7.0).all())
+
+
 @pytest.mark.parametrize("cap", [1e-30, 1e-6, 1e6, 1e30])
 def test_extreme_caps(cuda_device, cap):
     """Caps that flatten every score and caps that change none, at the ends of the range."""
