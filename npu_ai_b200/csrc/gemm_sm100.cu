@@ -22,8 +22,11 @@
 // channels x a 128-pixel patch of whole image rows, shifted by the tap; the out-of-range rows and columns of the
 // shift are TMA zeros, which is the convolution's zero padding. The weights are [Cout, 3, 3, Cin] (K-major) and the
 // output tile is 128 consecutive NHWC pixels, so the epilogue is the GEMM's. The epilogue can also add a per-image
-// bias row (conv bias + time embedding) and a residual tensor. The only layout requirement is TMA's: 16-byte aligned base and row strides (K % 8 == 0 for a
-// dense matrix); anything else is repacked by the host into a caller-provided workspace first.
+// bias row (conv bias + time embedding) and a residual tensor.
+// Activation form (template mode): act(x . W^T + bias) + residual, all in f32 before the one rounding. Its epilogue works in
+// groups of 32 columns on packed f32 pairs; see gemm_epi_warps and the epilogue for what each step measured.
+// The only layout requirement is TMA's: 16-byte aligned base and row strides (K % 8 == 0 for a dense matrix); anything
+// else is repacked by the host into a caller-provided workspace first.
 #include <algorithm>
 #include <climits>
 #include <cstdio>
@@ -523,7 +526,9 @@ __global__ void __launch_bounds__(64 + 32 * gemm_epi_warps<BN, MODE>(), 1)
       int issued = 0;
       bool ok = true;
       // The weight never depends on the previous kernel on the stream: the first stages' W tiles are requested
-      // before waiting on it (programmatic dependent launch), so their fetch overlaps that kernel's tail.
+      // before waiting on it (programmatic dependent launch), so their fetch overlaps that kernel's tail. (Not in the
+      // activation form, which does not ask that of its weight.)
+      if constexpr (MODE == kModeAct) pdl_wait();
       int pre = 0;
       if (unit0 < num_units) {
         int mb, nb;

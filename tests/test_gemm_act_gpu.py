@@ -178,3 +178,21 @@ def test_refusals(cuda_device):
         kernels.gemm(x, w, b, residual=r[:8], activation="gelu")
     with pytest.raises(ValueError, match="bias"):
         kernels.gemm(x, w, b[:8], activation="gelu")
+
+
+def test_operands_of_the_kernel_before(cuda_device):
+    """x, w, bias and residual may each be what the kernel before on the stream has written (launches overlap)."""
+    from npu_ai_b200 import kernels
+    x, w, b, r = _case(512, 512, 512, torch.float32, True, seed=3)
+    xd, wd, bd, rd = (t.to(cuda_device) for t in (x, w, b, r))
+    eye = torch.eye(512, dtype=torch.bfloat16, device=cuda_device)
+    for _ in range(20):
+        w2 = torch.empty_like(wd).fill_(float("nan"))
+        kernels.gemm(wd, eye, out=w2)          # w again
+        y = kernels.gemm(xd, w2, bd, residual=rd, activation="silu", out_dtype=torch.float32)
+        r2 = torch.empty_like(rd).fill_(float("nan"))
+        kernels.gemm(rd, eye, out=r2)
+        z = kernels.gemm(xd, wd, bd, residual=r2, activation="silu", out_dtype=torch.float32)
+        kernels.check_status(cuda_device)
+        assert torch.equal(y, z)
+    _check(y, x, w, b, r, "silu")
