@@ -299,10 +299,15 @@ __device__ __forceinline__ void rcp4(uint64_t da, uint64_t db, uint64_t& ra, uin
   rb = f2_mul(f2_pack(d3, d2), f2_pack(qb, qb));
 }
 
-// y sigmoid(s) = y / (1 + 2^t) of two pairs, t = -s log2 e capped at 30: below s = -20.8 the sigmoid stays at 2^-30,
-// an error under 1e-9 |y| (and the product of four denominators stays finite).
-__device__ __forceinline__ void times_sigmoid4(uint64_t& ya, uint64_t& yb, uint64_t ta, uint64_t tb) {
-  float t0, t1, t2, t3;
+// y sigmoid(s) = y / (1 + 2^t) of two pairs, t = -s log2 e capped at 30 (the product of four denominators has to stay
+// finite, a NaN to keep out of it) and y, where t is 30 or more, at `least`: the result ends at least * 2^-30, -2e-8,
+// instead of falling to 0. (Without the cap on y it would grow with y again: -1000 at y = -1e12.)
+__device__ __forceinline__ void times_sigmoid4(uint64_t& ya, uint64_t& yb, uint64_t ta, uint64_t tb, float least) {
+  float t0, t1, t2, t3, y0, y1, y2, y3;
+  f2_unpack(ya, y0, y1);
+  f2_unpack(yb, y2, y3);
+  ya = f2_pack(max_nan(y0, least), max_nan(y1, least));
+  yb = f2_pack(max_nan(y2, least), max_nan(y3, least));
   f2_unpack(ta, t0, t1);
   f2_unpack(tb, t2, t3);
   const uint64_t one = f2_pack(1.0f, 1.0f);
@@ -360,7 +365,7 @@ __device__ __forceinline__ void activate(int act, uint64_t (&v)[N]) {
 #pragma unroll
     for (int j = 0; j < N; j += 2)
       times_sigmoid4(v[j], v[j + 1], f2_mul(v[j], f2_fma(f2_mul(v[j], v[j]), b, a)),
-                     f2_mul(v[j + 1], f2_fma(f2_mul(v[j + 1], v[j + 1]), b, a)));
+                     f2_mul(v[j + 1], f2_fma(f2_mul(v[j + 1], v[j + 1]), b, a)), -8.0f);
   } else if (act == NPUB200_ACT_RELU) {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
@@ -373,7 +378,7 @@ __device__ __forceinline__ void activate(int act, uint64_t (&v)[N]) {
     const uint64_t k2 = f2_pack(k, k);
 #pragma unroll
     for (int j = 0; j < N; j += 2)
-      times_sigmoid4(v[j], v[j + 1], f2_mul(v[j], k2), f2_mul(v[j + 1], k2));
+      times_sigmoid4(v[j], v[j + 1], f2_mul(v[j], k2), f2_mul(v[j + 1], k2), 30.0f / k);
   }
 }
 

@@ -486,12 +486,13 @@ __device__ __forceinline__ float fast_rcp(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// max(x, 0) that keeps a NaN.
-__device__ __forceinline__ float relu_nan(float x) {
+// max(x, c) and max(x, 0) that keep a NaN.
+__device__ __forceinline__ float max_nan(float x, float c) {
   float y;
-  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(y) : "f"(x));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(c));
   return y;
 }
+__device__ __forceinline__ float relu_nan(float x) { return max_nan(x, 0.0f); }
 
 // 2^x of two values on the FMA pipe (packed f32x2 arithmetic), so a share of a softmax's exponentials leaves the
 // MUFU (16 per clock per SM) for the FP32 pipe: x = n + f with n = round(x) (adding 1.5 * 2^23 leaves round(x) in the low mantissa bits) and

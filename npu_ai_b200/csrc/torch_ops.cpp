@@ -1,7 +1,8 @@
-// torch_ops.cpp - the GEMM and the fused attention as torch operators (torch.ops.npub200.gemm / .attention).
+// torch_ops.cpp - the GEMM, the fused and the masked attention as torch operators (torch.ops.npub200.gemm / .attention /
+// .attention_masked).
 //
 // The reference hands each request to its NPU as one XRT command: NpuProgram.submit_gemm / submit_attn
-// (npu/xdna1_program.py:441-473) with three buffer objects and 13 int32 parameters. Here the same two requests are
+// (npu/xdna1_program.py:441-473) with three buffer objects and 13 int32 parameters. Here the same requests are
 // operators registered with the torch dispatcher (TORCH_LIBRARY), so torch code, CUDA-graph capture and
 // torch.compile-free callers see them as ordinary ops on CUDA tensors. Each one checks its tensors, then calls
 // the library's C ABI (include/npu_b200.h) on at::cuda::getCurrentCUDAStream() of the tensors' device; nothing is
@@ -45,7 +46,8 @@ void check_operand(const at::Tensor& t, const at::Tensor& ref, const char* name)
 
 void* stream_of(const at::Tensor& t) { return at::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 
-// out[M, N] = act(x[M, K] . w[N, K]^T (+ bias)) (+ residual), act an NPUB200_ACT_* code or 0 for none; bf16 operands, f32 accumulation, bias in f32.
+// out[M, N] = act(x[M, K] . w[N, K]^T (+ bias)) (+ residual), act an NPUB200_ACT_* code or 0 for none; bf16 operands, f32
+// accumulation, bias in f32.
 // Replaces NpuGemm.matmul_t (npu/xdna1_gemm.py:349-422) / NpuProgram.submit_gemm (npu/xdna1_program.py:451-454).
 at::Tensor gemm(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias,
                 const std::optional<at::Tensor>& out, int64_t variant, std::optional<at::ScalarType> out_dtype,

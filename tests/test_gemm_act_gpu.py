@@ -180,6 +180,30 @@ def test_refusals(cuda_device):
         kernels.gemm(x, w, b[:8], activation="gelu")
 
 
+@pytest.mark.parametrize("act", ACTS)
+def test_values_of_every_size(cuda_device, act):
+    """One value a row from 2^-60 to 2^100, both signs, and infinities: sums that are those values exactly. For negative
+    ones the result falls to 0, which the kernel may miss by 2.8e-8 (30 x 2^-30). A NaN stays in its own place."""
+    from npu_ai_b200 import kernels
+    v = torch.tensor([s * m * 2.0 ** e for e in range(-60, 101) for m in (1.0, 1.5) for s in (1.0, -1.0)])
+    M = v.numel()
+    x = torch.zeros(M, 64, dtype=torch.bfloat16)
+    x[:, 0] = v.to(torch.bfloat16)
+    w = torch.zeros(128, 64, dtype=torch.bfloat16)
+    w[:, 0] = 1.0
+    y = v.double()[:, None].expand(M, 128)
+    out = kernels.gemm(x.to(cuda_device), w.to(cuda_device), activation=act)
+    ref = torch.where((y == -float("inf")) | (y < -1e4), 0.0, _act64(act, y))
+    assert bool(((out.double().cpu() - ref).abs() <= 2.0 ** -19 * ref.abs() + 2.8e-8 + 1.5e-7 * y.abs().clamp(max=64.0)).all())
+    # a bias carries the infinities and the NaN (0 x inf would be a NaN on the way)
+    b = torch.zeros(128)
+    b[5], b[6], b[7] = float("inf"), float("-inf"), float("nan")
+    out = kernels.gemm(torch.zeros_like(x).to(cuda_device), w.to(cuda_device), b.to(cuda_device), activation=act).cpu()
+    kernels.check_status(cuda_device)
+    assert bool((out[:, 5] == float("inf")).all()) and bool((out[:, 6].abs() <= 2.8e-8).all())
+    assert bool(out[:, 7].isnan().all()) and bool((out[:, [i for i in range(128) if i not in (5, 6, 7)]] == 0).all())
+
+
 def test_operands_of_the_kernel_before(cuda_device):
     """x, w, bias and residual may each be what the kernel before on the stream has written (launches overlap)."""
     from npu_ai_b200 import kernels
