@@ -767,9 +767,12 @@ def run_e2e(args, dist, device, total_flops) -> dict:
 def _kernel_kind(name: str) -> str:
     if "attention_fwd" in name:
         return "attention"
+    if "attention_masked" in name or "attention_join" in name:
+        return "masked attention"
     if "gemm_bf16_tcgen05" in name:
         mode = name.split("gemm_bf16_tcgen05_kernel<", 1)[-1].split(",")
-        return {"1": "GEGLU GEMM", "2": "3x3 convolution"}.get(mode[2].strip() if len(mode) > 2 else "", "GEMM")
+        kinds = {"1": "GEGLU GEMM", "2": "3x3 convolution", "3": "activation GEMM"}
+        return kinds.get(mode[2].strip() if len(mode) > 2 else "", "GEMM")
     for key, kind in (("gn_", "GroupNorm"), ("layer_norm", "LayerNorm"), ("concat_channels", "NHWC copy"),
                       ("upsample_nearest2x", "NHWC copy"), ("repack_rows", "GEMM operand repack")):
         if key in name:

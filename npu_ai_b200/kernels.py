@@ -1,9 +1,9 @@
 """Tensor-level calls into libnpub200: torch CUDA tensors in, pointers/strides through the C ABI, torch out.
 
 torch provides device memory and the current stream; the arithmetic runs in the sm_100a kernels of the
-library. The GEMM and the attention go through the library's torch operators (torch.ops.npub200.gemm /
-.attention, libnpub200_torch.so) when that layer is built, else straight through ctypes; both reach the same C ABI
-and kernels. Nothing here computes on the CPU, and there is no fallback when a kernel refuses a request.
+library. The GEMM and the attention go through the library's torch operators (torch.ops.npub200.gemm / .attention /
+.attention_masked, libnpub200_torch.so) when that layer is built, else straight through ctypes; both reach the same
+C ABI and kernels. Nothing here computes on the CPU, and there is no fallback when a kernel refuses a request.
 """
 from __future__ import annotations
 
