@@ -312,7 +312,7 @@ int attention_masked_launch(const AttnMaskedProblem& mp, cudaStream_t stream) {
   a.ctl.timeout_ns = wait_timeout_ns();
   a.ctl.debug = p.debug;
   m.causal = o.causal != 0;
-  m.q_start = o.q_start;
+  m.q_start = std::min<int64_t>(std::max<int64_t>(o.q_start, -(int64_t(1) << 40)), int64_t(1) << 40);  // + a query index
   m.q_starts = o.q_starts;
   m.prefix = o.prefix;
   m.prefixes = o.prefixes;

@@ -374,8 +374,8 @@ const uint64_t in2 = f2_pack(m.cap_in, m.cap_in);
       const uint32_t q[4] = {v[c / 16].x, v[c / 16].y, v[c / 16].z, v[c / 16].w};
 #pragma unroll
       for (int t = 0; t < 16; ++t) {
-        // The byte (0 or 1) as all zeros or all ones: its low bit moved to the sign and that replicated.
-        const uint32_t keep = replicate_sign(q[t / 4] << 7, t % 4);
+        // The byte as all zeros or all ones: any of its bits carried to the sign and that replicated.
+        const uint32_t keep = replicate_sign(((q[t / 4] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | q[t / 4], t % 4);
         s[c + t] = __uint_as_float((__float_as_uint(s[c + t]) & keep) | (0xff800000u & ~keep));
       }
     }

@@ -464,6 +464,50 @@ def test_two_streams_of_key_tiles(cuda_device, B, H, Hk, Sq, Skv, D):
     run(cuda_device, B, H, Hk, Sq, Skv, D, slopes=slopes, distance_bias=table, kv_lens=lens, seed=Skv + 4)
 
 
+@pytest.mark.parametrize("Skv", [320, 333])
+def test_bool_masks_of_any_byte(cuda_device, Skv):
+    """Any nonzero byte shows a key, in rows that 16-byte words divide and in others, for many rows and for one."""
+    from npu_ai_b200 import kernels
+    g = torch.Generator(device=cuda_device).manual_seed(Skv)
+    raw = torch.randint(0, 256, (200, Skv), generator=g, device=cuda_device, dtype=torch.uint8)
+    raw *= torch.randint(0, 2, (200, Skv), generator=g, device=cuda_device, dtype=torch.uint8)
+    raw[:, 7] = 2
+    q, k, v = _qkv(2, 4, 4, 200, Skv, 64, 1, cuda_device)
+    for bytes_ in (raw, raw[:1]):
+        out = kernels.attention(q, k, v, 4, mask=bytes_.view(torch.bool))
+        kernels.check_status(cuda_device)
+        check(out, *oracle(q, k, v, 4, 4, mask=(bytes_ != 0).expand(200, Skv)), 4, False)
+
+
+def test_positions_at_the_ends_of_64_bits(cuda_device):
+    from npu_ai_b200 import kernels
+    q, k, v = _qkv(1, 2, 2, 130, 100, 64, 1, cuda_device)
+    last = kernels.attention(q, k, v, 2, causal=True, q_start=2 ** 63 - 1)
+    first = kernels.attention(q, k, v, 2, causal=True, q_start=-2 ** 63)
+    far = kernels.attention(q, k, v, 2, causal=True, prefix_len=2 ** 63 - 1, q_start=-2 ** 63)
+    kernels.check_status(cuda_device)
+    ref = oracle(q, k, v, 2, 2)
+    check(last, *ref, 2, False)
+    check(far, *ref, 2, False)
+    assert bool((first == 0).all())
+
+
+def test_broadcast_and_odd_strides(cuda_device):
+    """A cache shared by the whole batch (stride 0), single-row dimensions with any stride."""
+    from npu_ai_b200 import kernels
+    q, k, v = _qkv(3, 4, 2, 5, 300, 64, 1, cuda_device)
+    try:
+        out = kernels.attention(q, k[:1].expand(3, -1, -1), v[:1].expand(3, -1, -1), 4, kv_heads=2, causal=True)
+    except (ValueError, RuntimeError):
+        out = None  # refused
+    if out is not None:
+        check(out, *oracle(q, k[:1].expand(3, -1, -1), v[:1].expand(3, -1, -1), 4, 2, causal=True), 4, False)
+    one = q[:1, :1].as_strided((1, 1, 256), (3, 5, 1))
+    out = kernels.attention(one, k[:1], v[:1], 4, kv_heads=2, causal=True)
+    kernels.check_status(cuda_device)
+    check(out, *oracle(q[:1, :1], k[:1], v[:1], 4, 2, causal=True), 4, False)
+
+
 def test_refusals(cuda_device):
     from npu_ai_b200 import kernels
     dev = cuda_device
