@@ -286,7 +286,7 @@ __device__ __forceinline__ float modify_scores(const MaskedArgs& m, const Row& w
     float big = 0.0f;
 #pragma unroll
     for (int t = 0; t < BN; t += 2) big = fmax3(big, fabsf(s[t]), fabsf(s[t + 1]));
-    if (__all_sync(0xffffffffu, big * m.cap_in <= 1.0f)) {
+    if (__all_sync(0xffffffffu, !w.valid || big * m.cap_in <= 1.0f)) {
       // The usual case, on the FMA pipe (the MUFU has the softmax's exponentials to do): cap tanh(y) = y P(y^2).
 const uint64_t in2 = f2_pack(m.cap_in, m.cap_in);
 #pragma unroll
@@ -435,13 +435,22 @@ __device__ __forceinline__ float masked_softmax_step(const MaskedArgs& m, const 
 #pragma unroll
     for (int t = 0; t < kHalf; ++t) s[t] = __uint_as_float(r[t]);
   }
+  // Partly seen: the keys [a, z) of this half as bits, a bit test a score instead of two comparisons.
+  const bool partial = w.lo_max > key0 || w.hi_min < key0 + kHalf;
+  uint32_t keep = 0xffffffffu;
+  if (partial) {
+    const int a = max(w.lo - key0, 0), z = min(w.hi - key0, kHalf);
+    keep = a < z ? (0xffffffffu << a) & (0xffffffffu >> (32 - z)) : 0u;
+    static_assert(kHalf == 32, "a bit a key");
+    if constexpr ((FEAT & kFeatCap) != 0) {
+      // The largest score chooses between the cap's two forms: stale memory must have no say in it.
+#pragma unroll
+      for (int t = 0; t < kHalf; ++t) s[t] = (keep >> t) & 1u ? s[t] : 0.0f;
+    }
+  }
   float c = m.a.scale_log2;
   if constexpr (FEAT != 0) c = modify_scores<FEAT, kHalf>(m, w, key0, row_mask, s_table, s_mask, lane, s);
-  if (w.lo_max > key0 || w.hi_min < key0 + kHalf) {
-    // The keys [a, z) of this half as bits: a bit test a score instead of two comparisons.
-    const int a = max(w.lo - key0, 0), z = min(w.hi - key0, kHalf);
-    const uint32_t keep = a < z ? (0xffffffffu << a) & (0xffffffffu >> (32 - z)) : 0u;
-    static_assert(kHalf == 32, "a bit a key");
+  if (partial) {
 #pragma unroll
     for (int t = 0; t < kHalf; ++t) s[t] = (keep >> t) & 1u ? s[t] : -INFINITY;
   }

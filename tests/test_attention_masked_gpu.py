@@ -493,19 +493,38 @@ def test_positions_at_the_ends_of_64_bits(cuda_device):
 
 
 def test_broadcast_and_odd_strides(cuda_device):
-    """A cache shared by the whole batch (stride 0), single-row dimensions with any stride."""
+    """A cache shared by the whole batch (stride 0) is refused; single-row dimensions may have any stride."""
     from npu_ai_b200 import kernels
     q, k, v = _qkv(3, 4, 2, 5, 300, 64, 1, cuda_device)
-    try:
-        out = kernels.attention(q, k[:1].expand(3, -1, -1), v[:1].expand(3, -1, -1), 4, kv_heads=2, causal=True)
-    except (ValueError, RuntimeError):
-        out = None  # refused
-    if out is not None:
-        check(out, *oracle(q, k[:1].expand(3, -1, -1), v[:1].expand(3, -1, -1), 4, 2, causal=True), 4, False)
+    with pytest.raises(ValueError, match="strides"):
+        kernels.attention(q, k[:1].expand(3, -1, -1), v[:1].expand(3, -1, -1), 4, kv_heads=2, causal=True)
     one = q[:1, :1].as_strided((1, 1, 256), (3, 5, 1))
     out = kernels.attention(one, k[:1], v[:1], 4, kv_heads=2, causal=True)
     kernels.check_status(cuda_device)
     check(out, *oracle(q[:1, :1], k[:1], v[:1], 4, 2, causal=True), 4, False)
+
+
+@pytest.mark.parametrize("Sq", [1, 5, 130])
+def test_stale_memory_has_no_say(cuda_device, Sq):
+    """Bit for bit the same whatever the cache holds behind the lengths and the kernel before left in shared memory."""
+    from npu_ai_b200 import kernels
+    q, k, v = _qkv(2, 8, 2, Sq, 700, 64, Sq, cuda_device)
+    lens = ints(cuda_device, 700, 333)
+    wild = [t * 300.0 for t in _qkv(4, 16, 4, 512, 512, 64, 3, cuda_device)]
+    calm = [t * 1e-3 for t in wild]
+    both = dict(kv_heads=2, causal=True, q_start=lens - Sq, kv_lens=lens, softcap=5.0,
+                slopes=torch.rand(8, device=cuda_device))
+    for drop in ("", "slopes", "softcap"):
+        kw = {n: a for n, a in both.items() if n != drop}
+        ref = None
+        for fill in (0.0, 1e4, -1e30, float("nan"), float("inf")):
+            k[1, 333:], v[1, 333:] = fill, fill
+            for before in (wild, calm):
+                kernels.attention(*before, 16, kv_heads=4, softcap=1.0)
+                out = kernels.attention(q, k, v, 8, **kw)
+                kernels.check_status(cuda_device)
+                ref = out if ref is None else ref
+                assert torch.equal(out, ref), (drop, fill)
 
 
 def test_refusals(cuda_device):
