@@ -37,22 +37,24 @@ __device__ __forceinline__ void map_coords(const MapPos& p, int atom, int s, int
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Producer: the nkv K and V tiles from tile `first` on of one (b, h) pair into STAGES-deep rings, K one tile ahead of V (K_j is needed a whole
-// softmax step before V_j). On an abort it waits for the loads it issued before returning, so shared memory is
-// not released under an in-flight copy.
+// Producer: the nkv K and V tiles from tile `first` on of one (b, h) pair into STAGES-deep rings, K one tile ahead
+// of V (K_j is needed a whole softmax step before V_j; `first_k_issued`: the first K is on its way). On an abort it
+// waits for the loads it issued before returning, so shared memory is not released under an in-flight copy.
 // ---------------------------------------------------------------------------------------------------------------
 template <int NA, int BN, int STAGES>
 __device__ __forceinline__ void kv_producer(const CUtensorMap* tm_k, const CUtensorMap* tm_v, const AttnArgs& args,
                                             uint8_t* sK, uint8_t* sV, uint64_t* k_full, uint64_t* v_full,
                                             uint64_t* k_empty, uint64_t* v_empty, volatile int* abort_flag, int hh,
-                                            int bb, int nkv, int first = 0) {
+                                            int bb, int nkv, int first = 0, bool first_k_issued = false) {
   constexpr int kAtom = BN * kAtomBytesPerRow;
   constexpr int kTile = NA * kAtom;
   int issued_k = 0, issued_v = 0;
   bool ok = true;
   int c0, c1, c2, c3;
   for (int j = 0; j <= nkv; ++j) {
-    if (j < nkv) {
+    if (j == 0 && first_k_issued) {
+      ++issued_k;
+    } else if (j < nkv) {
       const int st = j % STAGES;
       if (!mbar_wait_bounded(&k_empty[st], (uint32_t(j / STAGES) & 1u) ^ 1u, abort_flag, args.ctl,
                              kStatusTimeoutProducer)) {
