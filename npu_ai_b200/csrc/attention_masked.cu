@@ -155,6 +155,14 @@ bool two_streams(int64_t D, int64_t ctas, int64_t tiles, int sms) {
   return D <= 160 && (D > 128 || ctas <= sms) && tiles >= 4;
 }
 
+// Few parts are joined by a cluster: no workspace, no second launch. The GPU time is that of the second kernel or less
+// (2 x 13 parts 6.8 us, with the second kernel 7.1), and the call takes some 4 us less on the host, which is what a small
+// call waits for. Clusters that do not all find a place at once wait for a second wave: 35 x 4 parts of 32 tiles took 35 us,
+// through the workspace 25; 8 x 16 parts 21.7 and 13.0.
+bool in_cluster(int64_t ctas, int64_t parts, int sms) {
+  return parts > 1 && parts <= kMaxCluster && (parts <= 4 ? 8 : 28) * ctas * parts <= 7 * sms;
+}
+
 int plan_masked(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Skv, int64_t D, int variant, int sms,
                 MaskedPlan* out) {
   const int64_t G = H / Hk;
@@ -184,29 +192,28 @@ int plan_masked(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Skv, int64
       // Many long rows: parts of at least 32 tiles, several waves of them, which evens out ragged lengths.
       p.splits = int(std::min<int64_t>(5 * slots / (2 * ctas), kMaxSplits));
     } else {
-      // The number of parts with the least time, in us: its tiles one after the other (0.7 with two streams, 1.3 without),
-      // and the partial results' way out and in (0.8 a MB) with what a join costs by itself. Measured against the
-      // choice: 1x4x1024x1024x64 16.1 us whole, 13.8 / 12.5 / 13.7 in 2 / 4 / 8 parts; 1x8x512x512x128 11.4 whole,
-      // 13.3 in 2; 8 pairs of 20 rows over 79 tiles 92.6 whole, 13.7 / 13.0 / 12.7 in 12 / 16 / 27.
+      // The number of parts with the least time, in us: a tile after the other 1.2, 1.5 where two streams share the SM's
+      // units; a join 2.8, and 0.4 a MB of partial results within a cluster, 0.8 through the workspace. Measured against
+      // the choice: 1x4x1024x1024x64 16.0 us whole, 13.7 / 12.4 / 13.7 in 2 / 4 / 8 parts; 1x8x512x512x128 11.2 whole,
+      // 13.1 in 2; 3x16/8x16x410x72 9.7 whole, 10.8 / 9.5 in 2 / 4; 7x10/5x1x8124x64 30.5 / 25.3 in 4 / 8; 8 pairs of 20
+      // rows over 79 tiles 92.6 whole, 13.7 / 13.0 / 12.7 in 12 / 16 / 27.
       double best = 0;
       const int64_t most = std::min<int64_t>({slots / ctas, key_tiles, kMaxSplits});
-      for (int64_t parts = 1; parts <= most; ++parts) {
-        const int64_t per = (key_tiles + parts - 1) / parts;
-        if ((key_tiles + per - 1) / per != parts) continue;  // the same tiles a part in fewer parts
-        const double us = double(per) * (two_streams(D, ctas * parts, per, sms) ? 0.7 : 1.3) +
-                          (parts > 1 ? 1.5 + 0.8e-6 * double(B * H * Sq * parts * D * 4) : 0.0);
-        if (parts == 1 || us < best) {
+      for (int wish : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {  // (every number would take a microsecond)
+        const int per = int((key_tiles + std::min<int64_t>(wish, most) - 1) / std::min<int64_t>(wish, most));
+        const int64_t parts = (int(key_tiles) + per - 1) / per;  // no part without a tile
+        double us = two_streams(D, ctas * parts, per, sms) ? 1.5 * ((per + 1) / 2) : 1.2 * per;
+        if (parts > 1) us += 2.8 + (in_cluster(ctas, parts, sms) ? 0.4e-6 : 0.8e-6) * double(B * H * Sq * parts * D * 4);
+        if (wish == 1 || us < best) {
           best = us;
           p.splits = int(parts);
         }
+        if (wish >= most) break;
       }
     }
   }
   p.streams = two_streams(D, ctas * p.splits, key_tiles / p.splits, sms) ? 2 : 1;
-  // Few parts are joined by a cluster: no workspace, no second launch. The GPU time is that of the second kernel or less
-  // (2 x 13 parts 6.8 us, with the second kernel 7.1), and the call takes some 4 us less on the host, which is what a
-  // small call waits for. Large clusters run out of places: 8 x 16 parts take 21.7 us, through the workspace 13.0.
-  p.cluster = p.splits > 1 && p.splits <= kMaxCluster && (p.splits <= 4 ? 1 : 4) * ctas * p.splits <= sms;
+  p.cluster = in_cluster(ctas, p.splits, sms);
   if (p.splits > 1 && !p.cluster) {
     if (B * H * Sq > INT32_MAX / kMaxSplits)
       return fail(kErrUnsupported, "too many rows to split their keys (%lld)", (long long)(B * H * Sq));
