@@ -859,7 +859,7 @@ def _gpu_attention_override(func, q, k, v, heads, mask=None, attn_precision=None
     masked = mask is not None or gqa
     if masked:
         fits = rt.gemm.attention_fused_fits(tq, tk, d, b * h)
-        hk = k.shape[1] if skip_reshape else k.shape[2] // d
+        hk = k.shape[1] if skip_reshape else k.shape[2] // max(d, 1)
         kmask = _kernel_mask(mask, b, h, tq, tk, q.device) if mask is not None else None
         key += ((f"{kmask.dtype} mask" if kmask is not None else "") + (f" {hk} kv heads" if gqa else ""),)
         why = gate.model_route_reason(key, mask is not None and kmask is None, gqa and (hk <= 0 or h % hk != 0), fits)
