@@ -298,12 +298,16 @@ int attention_masked_launch(const AttnMaskedProblem& mp, cudaStream_t stream) {
   m.tiles = int(plan.tiles);
   m.pairs = int(plan.pairs);
   m.groups = int(p.H / plan.pack);
-  m.out_vec = ((reinterpret_cast<uintptr_t>(p.o) | uintptr_t(p.o_sb * (p.out_f32 ? 4 : 2)) |
-                uintptr_t(p.o_ss * (p.out_f32 ? 4 : 2)) | uintptr_t(p.o_sh * (p.out_f32 ? 4 : 2))) & 15u) == 0;
+  const int out_size = p.out_f32 ? 4 : 2;
+  const uintptr_t out_align = reinterpret_cast<uintptr_t>(p.o) | uintptr_t(p.o_sb * out_size) | uintptr_t(p.o_ss * out_size) |
+                              uintptr_t(p.o_sh * out_size);
+  m.out_vec = (out_align & 15u) == 0;
   m.splits = plan.splits;
   m.cluster = plan.cluster;
   m.part_ml = static_cast<float2*>(mp.workspace);
   m.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(mp.workspace) + plan.ml_bytes);
+  m.out_sectors = plan.splits > 1 ? p.D % 8 == 0 && ((reinterpret_cast<uintptr_t>(m.part_o) | uintptr_t(p.D * 4)) & 31u) == 0
+                                  : (out_align & 31u) == 0;
   a.Sq = int(p.Sq);
   a.Skv = int(p.Skv);
   a.H = int(p.H);

@@ -83,6 +83,7 @@ struct MaskedArgs {
   int mask_row;   // the rows of a warp share one mask row
   int table_smem; // the tile's head has its distance bias in shared memory
   int out_vec;    // output rows can be written in 16-byte words
+  int out_sectors;  // and in 32-byte ones (with split keys: the partial rows)
   long long m_sb, m_sh, m_sq;
 };
 
@@ -497,74 +498,64 @@ struct OColumns {
   static __device__ __forceinline__ int begin(int part) { return min(part * kWidth, DP); }
 };
 
-__device__ __forceinline__ void st_global_v4(uint64_t to, const uint4& v) {
-  asm volatile("st.global.v4.b32 [%0], {%1, %2, %3, %4};" ::"l"(to), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+// 32 aligned bytes, a whole sector, to global memory.
+__device__ __forceinline__ void st_global_v8(void* to, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
 }
 
-// The warp's 32 O rows x inv (zeros where `zero`; o_addr 0: no O, all zeros; o_addr2 not 0: plus the rows there x inv2)
-// to `dst` (each lane's own row, null: no row): `cols` columns from o_addr on (a multiple of 8; the padded
-// columns are whole sixteens) as f32 or bf16. A lane holds a row, so rows go through shared memory (`stage`, an odd
-// number of 16-byte words apart) and out in 16-byte words along them. Rolled loops: this runs once a tile, and
-// straight-line code for every head dim and type was paid for in instruction fetches. `keep`: only staged.
-__device__ __forceinline__ void store_rows(uint32_t o_addr, uint32_t o_addr2, uint8_t* stage, int cols, bool f32,
-                                           uint8_t* dst, float inv, float inv2, bool zero, int lane,
-                                           bool keep = false) {
-  const int words = cols * (f32 ? 4 : 2) / 16;  // 16-byte words of a row
-  const int pitch = (words | 1) * 16;
-  uint8_t* mine = stage + lane * pitch;
+// The warp's 32 O rows x inv (zeros where `zero`; o_addr 0: no O, all zeros; o_addr2 not 0: plus the rows there x inv2):
+// `cols` columns from o_addr on (a multiple of 8; the padded columns are whole sixteens) as f32 or bf16 to `dst`, each
+// lane's own row (null: no row). A lane holds a row and writes it itself, in whole sectors (`sectors`) or in 16-byte words:
+// through shared memory and out along the rows, with the index arithmetic that takes, was slower (2x12x77x77x64 causal 4.95
+// us, 4.80 in 16-byte words, 4.62 in sectors; 5 tokens against 5001 keys 12.65, 11.8, 11.6). Rolled: it runs once a tile, and
+// straight-line code for every head dim and type was paid for in instruction fetches.
+__device__ __forceinline__ void store_rows(uint32_t o_addr, uint32_t o_addr2, int cols, bool f32, uint8_t* dst, float inv,
+                                           float inv2, bool zero, bool sectors) {
 #pragma unroll 1
   for (int c = 0; c < cols; c += 16) {
-    uint32_t r[16] = {};
-    if (o_addr != 0) {
-      tmem_ld16(o_addr + uint32_t(c), r);
-      tmem_wait_ld();
-    }
+    uint32_t r[16] = {}, r2[16] = {};
+    if (o_addr != 0) tmem_ld16(o_addr + uint32_t(c), r);
+    if (o_addr2 != 0) tmem_ld16(o_addr2 + uint32_t(c), r2);
+    tmem_wait_ld();
     float o[16];
 #pragma unroll
-    for (int t = 0; t < 16; ++t) o[t] = zero ? 0.0f : __uint_as_float(r[t]) * inv;
-    if (o_addr2 != 0) {
-      tmem_ld16(o_addr2 + uint32_t(c), r);
-      tmem_wait_ld();
+    for (int t = 0; t < 16; ++t) {
+      o[t] = __uint_as_float(r[t]) * inv;
+      if (o_addr2 != 0) o[t] = fmaf(__uint_as_float(r2[t]), inv2, o[t]);
+      if (zero) o[t] = 0.0f;
+    }
+    if (dst == nullptr) continue;
+    if (sectors && c + 16 <= cols) {
+      uint32_t w[8];
+      if (f32) {
 #pragma unroll
-      for (int t = 0; t < 16; ++t) o[t] = zero ? 0.0f : fmaf(__uint_as_float(r[t]), inv2, o[t]);
+        for (int h = 0; h < 16; h += 8) {
+#pragma unroll
+          for (int t = 0; t < 8; ++t) w[t] = __float_as_uint(o[h + t]);
+          st_global_v8(dst + (c + h) * 4, w);
+        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < 8; ++t) w[t] = pack_bf16x2(o[2 * t], o[2 * t + 1]);
+        st_global_v8(dst + c * 2, w);
+      }
+      continue;
     }
 #pragma unroll
     for (int e = 0; e < 16; e += 8) {
       if (c + e >= cols) break;
       if (f32) {
-        *reinterpret_cast<float4*>(mine + (c + e) * 4) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-        *reinterpret_cast<float4*>(mine + (c + e) * 4 + 16) = make_float4(o[e + 4], o[e + 5], o[e + 6], o[e + 7]);
+        float4* to = reinterpret_cast<float4*>(dst + (c + e) * 4);
+        to[0] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        to[1] = make_float4(o[e + 4], o[e + 5], o[e + 6], o[e + 7]);
       } else {
-        *reinterpret_cast<uint4*>(mine + (c + e) * 2) =
+        *reinterpret_cast<uint4*>(dst + (c + e) * 2) =
             make_uint4(pack_bf16x2(o[e], o[e + 1]), pack_bf16x2(o[e + 2], o[e + 3]), pack_bf16x2(o[e + 4], o[e + 5]),
                        pack_bf16x2(o[e + 6], o[e + 7]));
       }
     }
-  }
-  if (keep) return;
-  __syncwarp();
-  int row = lane / words, c = lane - row * words;
-  const int step_row = 32 / words, step_c = 32 - step_row * words;
-#pragma unroll 1
-  for (int k = 0; k < words; k += 4) {  // four words in flight a lane
-    uint64_t to[4];
-    uint4 v[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      to[e] = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(dst), row & 31);
-      if (k + e >= words) to[e] = 0;
-      v[e] = to[e] != 0 ? *reinterpret_cast<const uint4*>(stage + row * pitch + c * 16) : make_uint4(0u, 0u, 0u, 0u);
-      if (to[e] != 0) to[e] += uint64_t(c) * 16;
-      row += step_row;
-      c += step_c;
-      if (c >= words) {
-        c -= words;
-        ++row;
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (to[e] != 0) st_global_v4(to[e], v[e]);
   }
 }
 
@@ -969,7 +960,7 @@ __global__ void __launch_bounds__(MaskedLayout<DP, STAGES, STREAMS>::kThreads,
       const int cols = min(args.D, OPart::begin(part + 1)) - begin;  // this warp's, maybe none
       const long long obase =
           (long long)bb * args.o_sb + (long long)w.i * args.o_ss + (long long)w.head * args.o_sh + begin;
-      uint8_t* stage = smem + warp * 32 * ((OPart::kWidth * esz / 16) | 1) * 16;
+      uint8_t* stage = smem + warp * 32 * ((OPart::kWidth * 4 / 16) | 1) * 16;
       uint8_t* dst = nullptr;
       if (m.splits > 1 && !m.cluster) {
         const long long at = (((long long)split * m.pairs + pair) * m.tiles + tile) * kAttnBM + row;
@@ -984,8 +975,9 @@ __global__ void __launch_bounds__(MaskedLayout<DP, STAGES, STREAMS>::kThreads,
       if (cols <= 0) {
         // nothing of the true head dim in this half
       } else if (m.splits > 1 ? nkv > 0 : m.out_vec != 0) {
-        store_rows(o_at, o_at2, stage, cols, wide, dst, inv * weight[0], inv * weight[1], empty, lane,
-                   m.cluster != 0);
+        // (in a cluster to the staged rows in shared memory, from where the other CTAs read them)
+        store_rows(o_at, o_at2, cols, wide, m.cluster ? stage + lane * ((cols / 4) | 1) * 16 : dst, inv * weight[0],
+                   inv * weight[1], empty, !m.cluster && m.out_sectors);
       } else if (m.splits == 1) {
         // Output rows that 16-byte words do not reach.
         for (int c = 0; c < cols; c += 8) {
