@@ -527,6 +527,29 @@ def test_stale_memory_has_no_say(cuda_device, Sq):
                 assert torch.equal(out, ref), (drop, fill)
 
 
+@pytest.mark.parametrize("Sq,variant", [(70, 0), (1, 0), (1, 40), (70, 2)])
+def test_offsets_past_32_bits(cuda_device, Sq, variant):
+    """Sequences more than 2^31 elements (and 2^32 bytes) apart: queries, cache, mask and output in one large buffer."""
+    from npu_ai_b200 import kernels
+    H, Hk, Skv, D, far = 4, 2, 300, 64, 2 ** 31 + 4096
+    if torch.cuda.mem_get_info(cuda_device)[0] < 16 << 30:
+        pytest.skip("needs 16 GB")
+    big = torch.empty(far + (1 << 20), dtype=BF16, device=cuda_device)
+    src = _qkv(2, H, Hk, Sq, Skv, D, 5, cuda_device)
+    bias = torch.randn(2, 1, Sq, Skv, device=cuda_device).to(BF16)
+    views, at = [], 0
+    for t in (*src, bias, torch.zeros_like(src[0])):
+        n = t[0].numel()
+        v = big.as_strided(t.shape, (far, *t[0].stride()), at)
+        v.copy_(t)
+        views.append(v)
+        at += (n + 63) // 64 * 64
+    q, k, v, mask, out = views
+    kernels.attention(q, k, v, H, kv_heads=Hk, causal=True, mask=mask, out=out, variant=variant)
+    kernels.check_status(cuda_device)
+    check(out, *oracle(*src, H, Hk, causal=True, mask=bias), H, False)
+
+
 def test_refusals(cuda_device):
     from npu_ai_b200 import kernels
     dev = cuda_device

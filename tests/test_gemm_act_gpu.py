@@ -204,6 +204,22 @@ def test_values_of_every_size(cuda_device, act):
     assert bool(out[:, 7].isnan().all()) and bool((out[:, [i for i in range(128) if i not in (5, 6, 7)]] == 0).all())
 
 
+@pytest.mark.parametrize("shift", [0, 1])
+def test_rows_far_apart(cuda_device, shift):
+    """Output and residual rows more than 2^32 bytes from the first to the last, aligned (TMA) and not."""
+    from npu_ai_b200 import kernels
+    M, K, N, ld = 40, 72, 96, 2 ** 26
+    if torch.cuda.mem_get_info(cuda_device)[0] < 16 << 30:
+        pytest.skip("needs 16 GB")
+    x, w, b, r = _case(M, K, N, torch.float32, True, seed=4)
+    big = torch.empty(M * ld, dtype=torch.bfloat16, device=cuda_device)
+    out, res = big.as_strided((M, N), (ld, 1), shift), big.as_strided((M, N), (ld, 1), 4096 + shift)
+    res.copy_(r)
+    kernels.gemm(x.to(cuda_device), w.to(cuda_device), b.to(cuda_device), out=out, residual=res, activation="gelu")
+    kernels.check_status(cuda_device)
+    _check(out.contiguous(), x, w, b, r, "gelu")
+
+
 def test_operands_of_the_kernel_before(cuda_device):
     """x, w, bias and residual may each be what the kernel before on the stream has written (launches overlap)."""
     from npu_ai_b200 import kernels
