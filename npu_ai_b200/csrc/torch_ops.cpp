@@ -201,7 +201,7 @@ const T* vector_ptr(const std::optional<at::Tensor>& t, const at::Tensor& q, int
 }
 
 // Attention with masks, score modifiers and grouped key/value heads (npub200_attention_masked): (B, S, H*d) tensors, or
-// (B, H, S, d) when head-major. Defaults: kv_heads 0 what k's shape says, scale <= 0 d^-0.5, no q_start the last query at
+// (B, H, S, d) when head-major. Defaults: kv_heads 0 what k's shape says, scale 0 d^-0.5, no q_start the last query at
 // the last key, softcap 0 none. The workspace of split keys comes from torch's allocator, one per call.
 at::Tensor attention_masked(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                             const std::optional<at::Tensor>& out_arg, std::optional<at::ScalarType> out_dtype,
