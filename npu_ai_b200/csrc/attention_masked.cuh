@@ -734,6 +734,8 @@ __global__ void __launch_bounds__(MaskedLayout<DP, STAGES, STREAMS>::kThreads,
     tmem_alloc(tmem_slot, L::kTmemCols);
     tmem_relinquish();
     tc_fence_before();
+    // Only now may the next kernel's blocks come: one that took the TMEM this block still needs would wait for this grid.
+    pdl_launch_dependents();
   }
   if (warp == kProducerWarp && lane == 0) {
     mbar_init(q_full, 1);  // by the thread that loads Q, which does not wait for the barriers' owner
@@ -744,7 +746,6 @@ __global__ void __launch_bounds__(MaskedLayout<DP, STAGES, STREAMS>::kThreads,
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
   }
-  pdl_launch_dependents();
   pdl_wait();  // q, k, v, the lengths, borders and masks may be the previous kernel's outputs; it may read out
   Row w = {};
   // Q needs nothing but the tile, and neither does the first K tile where no rule hides the first keys: both are on their
