@@ -205,7 +205,8 @@ int npub200_attention(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, c
  * (its attention gate refuses masks and grouped heads, comfyui node :39-99). As npub200_attention, with
  *   s_ij = scale q_i . k_j, then cap tanh(s / cap) when softcap > 0, then - slopes[h] |p_i - j| and
  *          + distance_bias[h][clamp(j - p_i, -R, R) + R] and + mask_ij where given,
- *   o_i  = sum_j softmax_j(s_ij) v_j over the keys j that row i may see; zeros for a row that sees none.
+ *   o_i  = sum_j softmax_j(s_ij) v_j over the keys j that row i may see; zeros for a row that sees none, NaN for one that
+ *          sees a NaN score (of q, k or the mask).
  * p_i = q_start + i is query i's position among the keys. Row i may see key j of its sequence b when all of these hold:
  *   j < kv_lens[b]; causal: j <= p_i or j < prefix; documents: i and j lie in the same document, document d of
  *   sequence b being tokens [off[d], off[d + 1]) (tokens outside every document see nothing); a boolean mask is not 0.

@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(32 * kJoinBlockWarps)
   }
   const long long obase = (long long)b * args.o_sb + (long long)i * args.o_ss + (long long)h * args.o_sh;
   if constexpr (WARPS == 1) {
-    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // (a NaN sum makes the row NaN, whatever its parts' weights)
     if (c < args.D) {
 #pragma unroll
       for (int t = 0; t < 8; ++t) acc[t] *= inv;
@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(32 * kJoinBlockWarps)
     __syncthreads();
     // (a warp without a part has no sum: warp 0 always has one)
     __shared__ float s_inv;
-    if (threadIdx.x == 0) s_inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    if (threadIdx.x == 0) s_inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     __syncthreads();
     const int col = int(threadIdx.x) * 2;
     if (col < args.D) {

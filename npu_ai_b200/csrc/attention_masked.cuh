@@ -201,8 +201,8 @@ __device__ __forceinline__ bool has_mask(const MaskedArgs& m) {
   return FEAT == kFeatMask || (FEAT == kFeatAny && m.mask_kind != 0);
 }
 
-// A mask value in log2 units: -inf hides; any finite value, however low, stays finite.
-__device__ __forceinline__ float mask_log2(float e) { return e == -INFINITY ? e : fmaxf(e * kLog2e, -FLT_MAX); }
+// A mask value in log2 units: -inf hides; any finite value, however low, stays finite; a NaN stays.
+__device__ __forceinline__ float mask_log2(float e) { return e == -INFINITY ? e : max_nan(e * kLog2e, -FLT_MAX); }
 
 // All bits the sign bit of byte `i` (a constant) of x.
 __device__ __forceinline__ uint32_t replicate_sign(uint32_t x, uint32_t i) {
@@ -357,7 +357,7 @@ const uint64_t in2 = f2_pack(m.cap_in, m.cap_in);
 #pragma unroll
       for (int t = 0; t < BN; ++t) {
         const float e = s_mask[t];
-        s[t] = e == -INFINITY ? e : fmaxf(fmaf(s[t], k, e), -FLT_MAX);
+        s[t] = e == -INFINITY ? e : max_nan(fmaf(s[t], k, e), -FLT_MAX);
       }
     }
     return 1.0f;
@@ -365,8 +365,8 @@ const uint64_t in2 = f2_pack(m.cap_in, m.cap_in);
   const int esz = m.mask_kind == 3 ? 4 : m.mask_kind;
   // (scores of keys behind the last get any value here: no row sees them)
   MaskBytes bytes(w.mask + (long long)kv0 * esz, w.mask + (long long)m.a.Skv * esz, m.mask_vec && m.a.Skv - kv0 >= BN);
-  // -inf hides; any finite value, however low, stays finite in log2 units.
-  auto add = [k](float x, float e) { return e == -INFINITY ? -INFINITY : fmaxf(fmaf(x, k, e * kLog2e), -FLT_MAX); };
+  // -inf hides; any finite value, however low, stays finite in log2 units; a NaN, of the score or the mask, stays.
+  auto add = [k](float x, float e) { return e == -INFINITY ? -INFINITY : max_nan(fmaf(x, k, e * kLog2e), -FLT_MAX); };
   if (m.mask_kind == 1) {
     uint4 v[BN / 16];
     bytes.take(v);
@@ -415,6 +415,8 @@ __device__ __forceinline__ bool hidden_tile(const Row& w, int kv0) {
 // The two warps of the rows exchange their maxima through s_max[2][128] (a buffer for alternate tiles); the barrier
 // also orders one warp's reads of S before the other's P over the same columns. Returns the factor for O; `move`:
 // whether the max moved (the same in both warps).
+// A NaN score makes its P and from then on the sum and O NaN (the maximum passes it over): the sum carries it to the end,
+// through the joins too, where 0 x NaN is NaN whatever weight the part has.
 template <int FEAT>
 __device__ __forceinline__ float masked_softmax_step(const MaskedArgs& m, const Row& w, uint32_t s_addr, int kv0, int half,
                                                      int row, int lane, float row_mask, const float* s_table,
@@ -629,7 +631,7 @@ __device__ __noinline__ void join_cluster(const MaskedArgs& m, const uint8_t* sm
         for (int t = 0; t < 8; ++t) o[t] = fmaf(wz[z], v[t], o[t]);
       }
     }
-    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // (a NaN sum makes the row NaN, whatever its parts' weights)
 #pragma unroll
     for (int t = 0; t < 8; ++t) o[t] *= inv;
     write_columns(m, (long long)bb * args.o_sb + (long long)i * args.o_ss + (long long)head * args.o_sh + c, o);
@@ -953,7 +955,8 @@ __global__ void __launch_bounds__(MaskedLayout<DP, STAGES, STREAMS>::kThreads,
     if (m.cluster && warp < kSoftmaxWarps) s_ml[row] = make_float2(ok ? run_max : -INFINITY, run_sum);
     if (ok && __any_sync(0xffffffffu, w.valid)) {
       tc_fence_after();
-      const bool empty = run_max == -INFINITY;       // the row has seen no key
+      // The row has seen no key. (A score that is NaN leaves the maximum alone, but not the sum: such a row is NaN.)
+      const bool empty = run_max == -INFINITY && run_sum == 0.0f;
       const bool wide = m.splits > 1 || args.out_f32;  // f32 rows
       const int esz = wide ? 4 : 2;
       const int part = 2 * stream + half;

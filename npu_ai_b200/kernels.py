@@ -394,7 +394,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, sca
     variant: key tile (0 = automatic, 64, 96, 128) + 1000 x query tiles of 128 rows per CTA (0 = automatic, 1, 2,
     or 4 with 64-key tiles for head dims up to 64); e.g. 2128 = two query tiles with 128-key tiles.
 
-    The keyword arguments select masked attention; a row that may see no key is zero. Query i of sequence b has the
+    The keyword arguments select masked attention; a row that may see no key is zero, one that sees a NaN score NaN. Query i of sequence b has the
     position p = q_start + i among the keys (default Skv - Sq + i: the last query meets the last key; an int, or int32
     [B]). Device tensors are read when the call runs, so a captured graph follows their contents.
     kv_heads:      k and v hold this many heads, a divisor of `heads` (default: what k's shape says); query head h reads
