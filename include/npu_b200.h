@@ -211,9 +211,9 @@ int npub200_attention(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, c
  *   j < kv_lens[b]; causal: j <= p_i or j < prefix; documents: i and j lie in the same document, document d of
  *   sequence b being tokens [off[d], off[d + 1]) (tokens outside every document see nothing); a boolean mask is not 0.
  * Keys that no row of the call may see under the lengths, causal and document rules are not read into the result,
- * whatever they hold (NaN included); a key that some rows see and others do not has to be finite. An additive mask of
- * -inf hides a key; a mask of the type's lowest finite value is a score like any other (a row with nothing else
- * averages those keys). q: [batch, sq, heads, head_dim] strided as in npub200_attention, k and v with kv_heads heads:
+ * whatever they hold (NaN included). Of the others the scores count where the key is seen and nowhere else, whatever they
+ * are; v has to be finite (a hidden key's weight is 0). An additive mask of -inf hides a key; a mask of the type's lowest
+ * finite value is a score like any other (a row with nothing else averages those keys; below -2.36e38 all are lowest). q: [batch, sq, heads, head_dim] strided as in npub200_attention, k and v with kv_heads heads:
  * query head h reads key/value head h / (heads / kv_heads). All pointers are device memory; int32 values outside
  * their range are clamped, never read past.
  * variant: 0, or the number of parts that every row's keys are split into (1 ... 64). Few rows over many keys are

@@ -439,20 +439,32 @@ __device__ __forceinline__ float masked_softmax_step(const MaskedArgs& m, const 
     for (int t = 0; t < kHalf; ++t) s[t] = __uint_as_float(r[t]);
   }
   // Partly seen: the keys [a, z) of this half as bits, a bit test a score instead of two comparisons.
-  const bool partial = w.lo_max > key0 || w.hi_min < key0 + kHalf;
+  bool partial = w.lo_max > key0 || w.hi_min < key0 + kHalf;
   uint32_t keep = 0xffffffffu;
   if (partial) {
     const int a = max(w.lo - key0, 0), z = min(w.hi - key0, kHalf);
     keep = a < z ? (0xffffffffu << a) & (0xffffffffu >> (32 - z)) : 0u;
     static_assert(kHalf == 32, "a bit a key");
-    if constexpr ((FEAT & kFeatCap) != 0) {
-      // The largest score chooses between the cap's two forms: stale memory must have no say in it.
+  }
+  // What a mask row of the whole warp hides goes the same way: its -inf added to a NaN or an infinite score would not
+  // hide it.
+  uint32_t hidden = 0u;
+  if (has_mask<FEAT>(m) && m.mask_row) {
+    hidden = __ballot_sync(0xffffffffu, row_mask == -INFINITY);
+    keep &= ~hidden;
+    partial = partial || hidden != 0;
+  }
+  if constexpr ((FEAT & kFeatCap) != 0) {
+    // The largest score chooses between the cap's two forms: stale memory must have no say in it.
+    if (partial) {
 #pragma unroll
       for (int t = 0; t < kHalf; ++t) s[t] = (keep >> t) & 1u ? s[t] : 0.0f;
     }
   }
   float c = m.a.scale_log2;
-  if constexpr (FEAT != 0) c = modify_scores<FEAT, kHalf>(m, w, key0, row_mask, s_table, s_mask, lane, s);
+  if constexpr (FEAT != 0) {
+    if (hidden != 0xffffffffu) c = modify_scores<FEAT, kHalf>(m, w, key0, row_mask, s_table, s_mask, lane, s);
+  }
   if (partial) {
 #pragma unroll
     for (int t = 0; t < kHalf; ++t) s[t] = (keep >> t) & 1u ? s[t] : -INFINITY;

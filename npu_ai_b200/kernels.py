@@ -407,7 +407,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, sca
     slopes:        f32 [heads], adds -slopes[h] * |p - j|.
     distance_bias: f32 [heads, 2R + 1], adds distance_bias[h, clamp(j - p, -R, R) + R].
     mask:          bool (False hides) or additive bf16/f32, [Sq, Skv] or 4-D broadcastable to [B, heads, Sq, Skv], with
-                   contiguous keys. A key has to be finite unless kv_lens, causal or doc_offsets hide it from every row.
+                   contiguous keys. v has to be finite at every key that kv_lens, causal and doc_offsets leave to some row.
     variant is then the number of parts each row's keys are split into (0 = automatic).
     """
     if (causal or kv_lens is not None or mask is not None or doc_offsets is not None or softcap is not None
