@@ -331,6 +331,7 @@ int attention_masked_launch(const AttnMaskedProblem& mp, cudaStream_t stream) {
   m.docs = o.doc_offsets;
   m.ndocs = int(o.docs);
   m.doc_stride = o.doc_stride;
+  m.gaps = o.doc_offsets != nullptr && o.causal && (o.q_starts != nullptr || o.q_start < 0);
   if (o.softcap > 0.0f) {
     m.cap_in = p.scale / o.softcap;
     m.cap_out = o.softcap * kLog2e;
@@ -352,8 +353,9 @@ int attention_masked_launch(const AttnMaskedProblem& mp, cudaStream_t stream) {
     m.mask_row = (o.mask_sq == 0 || p.Sq == 1) && (o.mask_sh == 0 || m.pack == 1);
   }
   const dim3 grid{unsigned(plan.pairs), unsigned(plan.tiles), unsigned(plan.splits)};
-  const int feats = (o.softcap > 0.0f ? kFeatCap : 0) | (o.slopes || o.distance_bias ? kFeatDistance : 0) |
-                    (o.mask ? kFeatMask : 0);
+  const int feats = m.gaps ? kFeatAny
+                           : (o.softcap > 0.0f ? kFeatCap : 0) | (o.slopes || o.distance_bias ? kFeatDistance : 0) |
+                                 (o.mask ? kFeatMask : 0);
   auto launch = feats == 0               ? launch_masked_for<0>
                 : feats == kFeatCap      ? launch_masked_for<kFeatCap>
                 : feats == kFeatDistance ? launch_masked_for<kFeatDistance>

@@ -72,6 +72,7 @@ struct MaskedArgs {
   const int* docs;
   int ndocs;
   long long doc_stride;
+  int gaps;           // documents may end in keys that no row sees: causal, and a start that may be below 0
   float cap_in, cap_out;  // capped score in log2 units = cap_out x tanh(cap_in x raw score)
   float cap_poly[6];      // cap_out x kTanhRatio: operands straight from the constant bank
   const float* slopes;
@@ -179,6 +180,27 @@ __device__ __forceinline__ Row row_of(const MaskedArgs& m, int r, int tile, int 
   w.mask = static_cast<const uint8_t*>(m.mask) +
            ((long long)b * m.m_sb + (long long)w.head * m.m_sh + (long long)(w.valid ? w.i : 0) * m.m_sq) * esz;
   return w;
+}
+
+// Which of the 64 keys of the tile at kv0 no row of the Q tile sees, as bits, with documents and causal (whole warps call
+// it). From position 0 on every key of a document is seen by its own row or by a later one of the Q tile; a start below 0
+// takes each document's last keys from all its rows. Only the kernel for any modifier has this code, and those calls go
+// there: even out of line it cost the others 2% (1x32/8x4096x128 causal 128.7 us without, 131.5 with it).
+static __device__ __noinline__ uint64_t unseen_keys(const MaskedArgs& m, int b, int tile, int kv0, int lane) {
+  const long long start = m.q_starts != nullptr ? (long long)m.q_starts[b] : m.q_start;
+  const long long prefix = m.prefixes != nullptr ? (long long)m.prefixes[b] : m.prefix;
+  const int i0 = tile * m.T, i1 = min(i0 + m.T, m.a.Sq);
+  uint64_t bits = 0;
+  if (start >= 0) return bits;
+  for (int k = 0; k < kMaskedBN; k += 32) {
+    const int key = kv0 + k + lane;
+    int d0, d1;
+    const bool in = document_of(m.docs + b * m.doc_stride, m.ndocs, key, lane, d0, d1);
+    const int last = min(d1, i1) - 1;  // the document's last row in the Q tile sees the most
+    const bool seen = in && last >= max(d0, i0) && (key <= clamp_pos(start + last) || key < prefix);
+    bits |= uint64_t(__ballot_sync(0xffffffffu, !seen)) << k;
+  }
+  return bits;
 }
 
 // tanh(y) / y as a polynomial in y^2, |y| <= 1 (fit_tanh_poly.py beside this file; relative error 7e-7).
@@ -840,10 +862,14 @@ __global__ void __launch_bounds__(MaskedLayout<DP, STAGES, STREAMS>::kThreads,
       // V rows of this tile that no row sees: zeros, whatever the cache holds there.
       const int kv0 = (first + i) * BN;
       const int live0 = max(key_lo - kv0, 0), live1 = min(key_hi - kv0, BN), end = min(args.Skv - kv0, BN);
-      if (live0 > 0 || live1 < end) {
+      uint64_t gaps = 0;  // between those keys
+      if constexpr (FEAT == kFeatAny) {
+        if (m.gaps) gaps = unseen_keys(m, bb, tile, kv0, lane);
+      }
+      if (live0 > 0 || live1 < end || gaps != 0) {
         for (int c = lane; c < BN * L::kNA * 8; c += 32) {
           const int row = (c >> 3) % BN;
-          if (row < live0 || row >= live1)
+          if (row < live0 || row >= live1 || (gaps >> row & 1u) != 0)
             *reinterpret_cast<uint4*>(sV + st * L::kKVBytes + (c >> 3) / BN * L::kKVAtom + row * kAtomBytesPerRow +
                                       (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
         }
