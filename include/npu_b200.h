@@ -232,7 +232,7 @@ typedef struct npub200_attention_mods {
   const int32_t* doc_offsets;    /* [docs + 1] nondecreasing document borders (sq == skv only), or NULL */
   int64_t docs;
   int64_t doc_stride;            /* elements between the borders of consecutive sequences (0: shared by all) */
-  float softcap;                 /* 1e-30 ... 1e30: cap of the scores; 0: none */
+  float softcap;                 /* 1e-30 ... 1e30, scale / softcap within [1.2e-38, 1.1e38]: cap of the scores; 0: none */
   int32_t max_distance;          /* R: distance_bias has 2 R + 1 entries per head */
   const float* slopes;           /* [heads], or NULL */
   const float* distance_bias;    /* [heads][2 R + 1] dense, or NULL */

@@ -246,13 +246,18 @@ int attention_masked_launch(const AttnMaskedProblem& mp, cudaStream_t stream) {
   if (p.q == nullptr || p.k == nullptr || p.v == nullptr || p.o == nullptr)
     return fail(kErrInvalid, "attention tensor pointer is null");
   if (int rc = check_masked_sizes(p.B, p.H, mp.kv_heads, p.Sq, p.Skv, p.D, p.variant)) return rc;
-  if (!(p.scale > 0.0f && p.scale <= FLT_MAX))
-    return fail(kErrInvalid, "attention scale must be positive and finite (got %g)", double(p.scale));
+  if (!(p.scale > 0.0f && p.scale * kLog2e <= FLT_MAX))
+    return fail(kErrInvalid, "attention scale must be positive and finite, times log2 e too (got %g)", double(p.scale));
   for (const void* ptr : {p.q, p.k, p.v})
     if (reinterpret_cast<uintptr_t>(ptr) & 15u) return fail(kErrInvalid, "q/k/v base addresses must be 16-byte aligned");
-  // (the cap and its reciprocal, times the scale and log2 e, have to stay normal numbers)
   if (!(o.softcap == 0.0f || (o.softcap >= 1e-30f && o.softcap <= 1e30f)))
     return fail(kErrInvalid, "softcap must be 0 (none) or positive, within [1e-30, 1e30] (got %g)", double(o.softcap));
+  // What the kernel computes with has to be a normal number: the cap times log2 e and its polynomial's coefficients are
+  // within that range, the scale over the cap, and that times 2 log2 e, only for scales that belong to the cap.
+  const float cap_in = o.softcap > 0.0f ? p.scale / o.softcap : 1.0f;
+  if (!(cap_in >= FLT_MIN && 2.0f * kLog2e * cap_in <= FLT_MAX))
+    return fail(kErrInvalid, "attention scale %g over softcap %g is not a normal number", double(p.scale),
+                double(o.softcap));
   if (!o.causal && (o.prefix != 0 || o.prefixes != nullptr))
     return fail(kErrInvalid, "a prefix needs the causal mask");
   if (o.doc_offsets != nullptr) {
@@ -333,7 +338,7 @@ int attention_masked_launch(const AttnMaskedProblem& mp, cudaStream_t stream) {
   m.doc_stride = o.doc_stride;
   m.gaps = o.doc_offsets != nullptr && o.causal && (o.q_starts != nullptr || o.q_start < 0);
   if (o.softcap > 0.0f) {
-    m.cap_in = p.scale / o.softcap;
+    m.cap_in = cap_in;
     m.cap_out = o.softcap * kLog2e;
     for (int i = 0; i < 6; ++i) m.cap_poly[i] = m.cap_out * kTanhRatio[i];
   }

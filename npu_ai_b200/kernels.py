@@ -403,7 +403,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, sca
     kv_lens:       int32 [B], the valid keys of each sequence; what lies behind them is never used.
     doc_offsets:   int32 [n + 1] or [B, n + 1], nondecreasing borders of packed documents (Sq == Skv): a token sees its
                    own document only; tokens outside every document see nothing.
-    softcap:       scores become softcap * tanh(score / softcap); within [1e-30, 1e30].
+    softcap:       scores become softcap * tanh(score / softcap); within [1e-30, 1e30], scale / softcap a normal f32.
     slopes:        f32 [heads], adds -slopes[h] * |p - j|.
     distance_bias: f32 [heads, 2R + 1], adds distance_bias[h, clamp(j - p, -R, R) + R].
     mask:          bool (False hides) or additive bf16/f32, [Sq, Skv] or 4-D broadcastable to [B, heads, Sq, Skv], with

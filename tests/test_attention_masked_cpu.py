@@ -85,3 +85,17 @@ def test_struct_matches_the_header(tmp_path):
     subprocess.run(["gcc", f"-I{root}/include", str(c), "-o", str(exe)], check=True)
     got = [int(x) for x in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
     assert got == [getattr(_lib.AttentionMods, n).offset for n in fields] + [ctypes.sizeof(_lib.AttentionMods)]
+
+
+@pytest.mark.parametrize("softcap,scale", [(1e30, 1e-16), (1e30, 1e-9), (1e-30, 1e9), (1e-30, 2e8), (0.0, 3e38)])
+def test_scales_that_leave_32_bits(softcap, scale):
+    """scale / softcap and scale log2 e have to be normal f32 numbers: 0 would average every key, infinity gives NaN."""
+    with pytest.raises(ValueError, match="scale"):
+        _call(_lib.AttentionMods(softcap=softcap), scale=scale)
+
+
+@pytest.mark.parametrize("softcap,scale", [(1e30, 1.2e-8), (1e-30, 5e7), (0.0, 2e38), (0.0, 1e-30)])
+def test_scales_at_the_ends_of_the_range_pass_the_check(softcap, scale):
+    """The next check, of the mask's type, is the one that refuses these calls."""
+    with pytest.raises(ValueError, match="mask dtype"):
+        _call(_lib.AttentionMods(softcap=softcap, mask=16, mask_dtype=5), scale=scale)
