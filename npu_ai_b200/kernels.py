@@ -412,7 +412,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, sca
     """
     if (causal or kv_lens is not None or mask is not None or doc_offsets is not None or softcap is not None
             or slopes is not None or distance_bias is not None or prefix_len is not None
-            or (kv_heads is not None and int(kv_heads) != (q.shape[1] if head_major_in else int(heads)))):
+            or (kv_heads is not None and int(kv_heads) != (q.shape[1] if head_major_in else int(heads)))
+            or _grouped(q, k, head_major_in)):
         return _attention_masked(q, k, v, heads, scale, head_major_in, head_major_out, out_dtype, out, variant, kv_heads,
                                  causal, q_start, prefix_len, kv_lens, doc_offsets, softcap, slopes, distance_bias, mask)
     for name, t in (("q", q), ("k", k), ("v", v)):
@@ -455,6 +456,12 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, sca
                   ctypes.c_void_p(v.data_ptr()), *vs, ctypes.c_void_p(out.data_ptr()), *os_, _DT[out.dtype],
                   B, H, Sq, Skv, D, ctypes.c_float(scale), int(variant), ctypes.c_void_p(_stream_ptr(q.device)))
     return out
+
+
+def _grouped(q: torch.Tensor, k: torch.Tensor, head_major: bool) -> bool:
+    """Whether k holds another number of heads than q."""
+    dim = 1 if head_major else 2
+    return q.dim() == k.dim() == (4 if head_major else 3) and k.shape[dim] != q.shape[dim]
 
 
 def _per_batch(t, name: str, B: int, device: torch.device, dtype: torch.dtype = torch.int32):

@@ -70,6 +70,9 @@ def attention_shard(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: in
         if H <= 0 or inner % H:
             raise ValueError(f"q's last dimension {inner} is not a multiple of heads={heads}")
         D = inner // H
+    if any(t.dim() != q.dim() or t.shape[0] != B or t.shape[1 if head_major_in else 2] != q.shape[1 if head_major_in else 2]
+           for t in (k, v)):  # a rank's slice of grouped heads would pair queries with the wrong key/value heads
+        raise ValueError(f"k/v shapes {tuple(k.shape)}, {tuple(v.shape)} do not hold q's batch and heads")
     pairs = B * H
     lo, hi = pair_range(pairs, world, rank)
     width = pair_width(pairs, world)

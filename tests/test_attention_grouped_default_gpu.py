@@ -1,0 +1,23 @@
+"""Grouped key/value heads without kv_heads and without another modifier: k's shape says how many there are."""
+import pytest
+import torch
+
+from test_attention_masked_gpu import BF16, _qkv, check, oracle
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("Hk", [1, 2, 8])
+@pytest.mark.parametrize("head_major", [False, True])
+@pytest.mark.parametrize("Sq,Skv", [(1, 400), (130, 300)])
+def test_kv_heads_by_the_shape_of_k(cuda_device, Hk, head_major, Sq, Skv):
+    from npu_ai_b200 import kernels
+    from npu_ai_b200.runner import NpuGemm
+    q, k, v = _qkv(2, 8, Hk, Sq, Skv, 64, Sq, cuda_device, head_major=head_major)
+    ref = oracle(q, k, v, 8, Hk, head_major)
+    out = kernels.attention(q, k, v, 8, head_major_in=head_major, head_major_out=head_major, out_dtype=BF16)
+    kernels.check_status(cuda_device)
+    check(out, *ref, 8, head_major)
+    g = NpuGemm(device=cuda_device, verbose=False)
+    out = g.attention(q, k, v, 8, skip_reshape=head_major, skip_output_reshape=head_major)
+    check(out, *ref, 8, head_major)
