@@ -411,7 +411,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, sca
     variant is then the number of parts each row's keys are split into (0 = automatic).
     """
     if (causal or kv_lens is not None or mask is not None or doc_offsets is not None or softcap is not None
-            or slopes is not None or distance_bias is not None or prefix_len is not None
+            or slopes is not None or distance_bias is not None or prefix_len is not None or q_start is not None
             or (kv_heads is not None and int(kv_heads) != (q.shape[1] if head_major_in else int(heads)))
             or _grouped(q, k, head_major_in)):
         return _attention_masked(q, k, v, heads, scale, head_major_in, head_major_out, out_dtype, out, variant, kv_heads,

@@ -40,6 +40,11 @@ def test_fewer_key_heads_than_query_heads(route):
         assert route(q, q, q, 8, head_major_in=hm, kv_heads=8) == "unmasked"
 
 
+def test_a_start_position_is_checked_with_the_others(route):
+    q = torch.zeros(2, 9, 512, dtype=BF16)
+    assert route(q, q, q, 8, q_start=0) == "masked"
+
+
 @pytest.mark.parametrize("head_major", [False, True])
 def test_a_group_refuses_grouped_heads(head_major):
     """Slicing the pairs of a rank out of k and v needs one head each for every query head."""

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from test_attention_masked_gpu import BF16, _qkv, check, oracle
+from test_attention_masked_gpu import BF16, _qkv, check, ints, oracle
 
 pytestmark = pytest.mark.gpu
 
@@ -21,3 +21,14 @@ def test_kv_heads_by_the_shape_of_k(cuda_device, Hk, head_major, Sq, Skv):
     g = NpuGemm(device=cuda_device, verbose=False)
     out = g.attention(q, k, v, 8, skip_reshape=head_major, skip_output_reshape=head_major)
     check(out, *ref, 8, head_major)
+
+
+def test_a_start_position_alone_is_checked(cuda_device):
+    """It changes nothing without a rule that looks at positions, and a bad one is refused all the same."""
+    from npu_ai_b200 import kernels
+    q, k, v = _qkv(2, 4, 4, 20, 30, 64, 1, cuda_device)
+    check(kernels.attention(q, k, v, 4, q_start=ints(cuda_device, 3, 7)), *oracle(q, k, v, 4, 4), 4, False)
+    with pytest.raises(ValueError, match="q_start"):
+        kernels.attention(q, k, v, 4, q_start=torch.zeros(2, device=cuda_device))
+    with pytest.raises(ValueError, match="heads"):
+        kernels.attention(q, k[..., :192], v[..., :192], 4)
