@@ -37,7 +37,9 @@ extern "C" {
 #define NPUB200_DTYPE_F32 1
 #define NPUB200_DTYPE_BOOL 2 /* one byte per value, 0 or 1 (attention mask tensors only) */
 
-/* Activations of npub200_gemm_act. */
+/* Activations of npub200_gemm_act. The sigmoid forms are accurate to a few f32 roundings relative to their value, down to
+ * f32's smallest normal numbers; erf is a formula with an absolute error of 1.5e-7, so gelu is off by up to 7.5e-8 |y|
+ * (below -4 that is the larger part of an f32 result). */
 #define NPUB200_ACT_GELU 1       /* y/2 (1 + erf(y / sqrt 2)) */
 #define NPUB200_ACT_GELU_TANH 2  /* y/2 (1 + tanh(sqrt(2/pi) (y + 0.044715 y^3))) */
 #define NPUB200_ACT_QUICK_GELU 3 /* y sigmoid(1.702 y) */

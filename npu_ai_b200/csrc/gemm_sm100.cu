@@ -28,6 +28,7 @@
 // The only layout requirement is TMA's: 16-byte aligned base and row strides (K % 8 == 0 for a dense matrix); anything
 // else is repacked by the host into a caller-provided workspace first.
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 #include <cstdio>
 #include <cstring>
@@ -299,15 +300,10 @@ __device__ __forceinline__ void rcp4(uint64_t da, uint64_t db, uint64_t& ra, uin
   rb = f2_mul(f2_pack(d3, d2), f2_pack(qb, qb));
 }
 
-// y sigmoid(s) = y / (1 + 2^t) of two pairs, t = -s log2 e capped at 30 (the product of four denominators has to stay
-// finite, a NaN to keep out of it) and y, where t is 30 or more, at `least`: the result ends at least * 2^-30, -2e-8,
-// instead of falling to 0. (Without the cap on y it would grow with y again: -1000 at y = -1e12.)
-__device__ __forceinline__ void times_sigmoid4(uint64_t& ya, uint64_t& yb, uint64_t ta, uint64_t tb, float least) {
-  float t0, t1, t2, t3, y0, y1, y2, y3;
-  f2_unpack(ya, y0, y1);
-  f2_unpack(yb, y2, y3);
-  ya = f2_pack(max_nan(y0, least), max_nan(y1, least));
-  yb = f2_pack(max_nan(y2, least), max_nan(y3, least));
+// y sigmoid(s) = y / (1 + 2^t) of two pairs, t = -s log2 e at most 30: the product of four denominators stays finite. (The
+// minimum keeps a NaN out of it; y carries it to its own result.)
+__device__ __forceinline__ void times_sigmoid4(uint64_t& ya, uint64_t& yb, uint64_t ta, uint64_t tb) {
+  float t0, t1, t2, t3;
   f2_unpack(ta, t0, t1);
   f2_unpack(tb, t2, t3);
   const uint64_t one = f2_pack(1.0f, 1.0f);
@@ -316,6 +312,28 @@ __device__ __forceinline__ void times_sigmoid4(uint64_t& ya, uint64_t& yb, uint6
        f2_add(f2_pack(fast_exp2(fminf(t2, 30.0f)), fast_exp2(fminf(t3, 30.0f))), one), ra, rb);
   ya = f2_mul(ya, ra);
   yb = f2_mul(yb, rb);
+}
+
+// The same of one pair for any t, a reciprocal each: a lane that holds a value further out takes this for all of its
+// values, so the far negative side falls to 0 as it should and is rarely paid for. -inf ends there, too (no -inf * 0).
+__device__ __forceinline__ uint64_t times_sigmoid_far(uint64_t y, uint64_t t) {
+  float y0, y1, t0, t1;
+  f2_unpack(y, y0, y1);
+  f2_unpack(t, t0, t1);
+  return f2_pack(max_nan(y0, -FLT_MAX) * fast_rcp(1.0f + fast_exp2(t0)),
+                 max_nan(y1, -FLT_MAX) * fast_rcp(1.0f + fast_exp2(t1)));
+}
+
+template <int N>
+__device__ __forceinline__ bool any_below(const uint64_t (&v)[N], float least) {
+  float low = 0.0f;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    float y0, y1;
+    f2_unpack(v[j], y0, y1);
+    low = fmin3(low, y0, y1);
+  }
+  return low < least;
 }
 
 // gelu(y) = y/2 (1 + erf(y/sqrt2)) = max(y, 0) - |y|/2 (1 - erf(|y|/sqrt2)) of two pairs, the tail 1 - erf by the formula
@@ -362,10 +380,15 @@ __device__ __forceinline__ void activate(int act, uint64_t (&v)[N]) {
   } else if (act == NPUB200_ACT_GELU_TANH) {
     constexpr float kA = -2.0f * 0.79788456080286536f * kLog2e, kB = 0.044715f * kA;
     const uint64_t a = f2_pack(kA, kA), b = f2_pack(kB, kB);
+    if (any_below(v, -5.5f)) {  // t = 29.8 there
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] = times_sigmoid_far(v[j], f2_mul(v[j], f2_fma(f2_mul(v[j], v[j]), b, a)));
+      return;
+    }
 #pragma unroll
     for (int j = 0; j < N; j += 2)
       times_sigmoid4(v[j], v[j + 1], f2_mul(v[j], f2_fma(f2_mul(v[j], v[j]), b, a)),
-                     f2_mul(v[j + 1], f2_fma(f2_mul(v[j + 1], v[j + 1]), b, a)), -8.0f);
+                     f2_mul(v[j + 1], f2_fma(f2_mul(v[j + 1], v[j + 1]), b, a)));
   } else if (act == NPUB200_ACT_RELU) {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
@@ -376,9 +399,13 @@ __device__ __forceinline__ void activate(int act, uint64_t (&v)[N]) {
   } else {
     const float k = act == NPUB200_ACT_SILU ? -kLog2e : -1.702f * kLog2e;
     const uint64_t k2 = f2_pack(k, k);
+    if (any_below(v, 30.0f / k)) {
 #pragma unroll
-    for (int j = 0; j < N; j += 2)
-      times_sigmoid4(v[j], v[j + 1], f2_mul(v[j], k2), f2_mul(v[j + 1], k2), 30.0f / k);
+      for (int j = 0; j < N; ++j) v[j] = times_sigmoid_far(v[j], f2_mul(v[j], k2));
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < N; j += 2) times_sigmoid4(v[j], v[j + 1], f2_mul(v[j], k2), f2_mul(v[j + 1], k2));
   }
 }
 

@@ -455,6 +455,12 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   return r;
 }
 
+__device__ __forceinline__ float fmin3(float a, float b, float c) {
+  float r;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // Two f32 lanes in one 64-bit register and the sm_100 packed f32x2 arithmetic on them (one FMA-pipe instruction
 // for two results).
 __device__ __forceinline__ uint64_t f2_pack(float lo, float hi) {

@@ -98,7 +98,8 @@ def gemm(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, out
     """out[M, N] = act(x[M, K] @ w[N, K]^T (+ bias)) (+ residual) with bf16 operands and f32 accumulation.
 
     `activation` (None, "gelu" with the error function, "gelu_tanh", "quick_gelu", "silu" or "relu") is applied in
-    f32 in the kernel's epilogue, between the bias and the residual.
+    f32 in the kernel's epilogue, between the bias and the residual. "gelu" is off by up to 7.5e-8 |y| there (its erf is a
+    formula of 1.5e-7), the others by a few f32 roundings relative to their value.
     x and w are bf16 CUDA matrices with a unit inner stride (any row stride); bias is bf16 or f32 [N]; residual a
     bf16 [M, N] matrix with unit inner stride (may be `out`). With `handle` (from register_weight for this very `w`)
     the cached weight descriptor is used.
