@@ -834,6 +834,13 @@ def _kernel_mask(mask, b: int, h: int, tq: int, tk: int, device):
     return mask if tk == 1 or mask.stride(-1) == 1 else mask.contiguous()
 
 
+def _rows_without_a_key(mask, b: int, h: int, tq: int, d: int, head_major: bool) -> torch.Tensor:
+    """Which rows of the output the mask leaves no key, laid out like it: (b, h, tq, 1) or (b, tq, h * d)."""
+    none = (~mask if mask.dtype == torch.bool else mask == -float("inf")).all(-1)
+    none = (none if none.dim() == 3 else none[None, None]).expand(b, h, tq)
+    return none[..., None] if head_major else none.transpose(1, 2).repeat_interleave(d, -1)
+
+
 def _gpu_attention_override(func, q, k, v, heads, mask=None, attn_precision=None, skip_reshape=False,
                             skip_output_reshape=False, **kwargs):
     """transformer_options["optimized_attention_override"] (the reference's _npu_attention_override,
@@ -857,6 +864,7 @@ def _gpu_attention_override(func, q, k, v, heads, mask=None, attn_precision=None
     key = (b, tq, tk, h, d)
     gqa = bool(kwargs.get("enable_gqa", False))
     masked = mask is not None or gqa
+    kmask = None
     if masked:
         fits = rt.gemm.attention_fused_fits(tq, tk, d, b * h)
         hk = k.shape[1] if skip_reshape else k.shape[2] // max(d, 1)
@@ -897,9 +905,9 @@ def _gpu_attention_override(func, q, k, v, heads, mask=None, attn_precision=None
         model_attn()
         ref, rec.model_ms = _time_gpu(model_attn, rt.gemm.device)
         ref = ref.float()
-        if masked:  # rows whose mask hides every key: zeros here, NaN from a plain softmax
-            hidden = torch.isnan(ref) & (y == 0)
-            ref = torch.where(hidden, 0.0, ref)
+        if kmask is not None:  # rows whose mask hides every key: zeros here, NaN from a plain softmax
+            none = _rows_without_a_key(kmask, b, h, tq, d, skip_output_reshape)
+            ref = torch.where(none & torch.isnan(ref), 0.0, ref)
         err = float((y.float() - ref).abs().max() / (ref.abs().max() + 1e-12))
         rec.max_rel_err = err
         if not np.isfinite(err) or err > 0.1:

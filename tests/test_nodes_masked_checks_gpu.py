@@ -1,0 +1,69 @@
+"""The ComfyUI node's first-call check of masked attention and the calls that stay with the model, on the GPU."""
+import pytest
+import torch
+
+from test_attention_masked_gpu import BF16
+from test_nodes_masked_gpu import _call, _check, _qkv, model_attention, runtime  # noqa: F401 (a fixture)
+
+pytestmark = pytest.mark.gpu
+
+INF, NAN = float("inf"), float("nan")
+
+
+def _plain_model(q, k, v, heads, mask=None, skip_output_reshape=False, **kw):
+    """A softmax in f32 of head-major operands, NaN where the mask leaves nothing (what SDPA gives there is its backend's)."""
+    n = q.shape[1] // k.shape[1]
+    s = q.float() @ k.float().repeat_interleave(n, 1).transpose(-1, -2) * q.shape[-1] ** -0.5
+    if mask is not None:
+        s = s.masked_fill(~mask, -INF) if mask.dtype == torch.bool else s + mask.float()
+    o = (s.softmax(-1) @ v.float().repeat_interleave(n, 1)).to(q.dtype)
+    return o if skip_output_reshape else o.transpose(1, 2).flatten(2)
+
+
+@pytest.mark.parametrize("kind", ["bool", "additive", "pad", "grouped"])
+@pytest.mark.parametrize("head_major_out", [False, True])
+def test_nan_in_a_query_raises_on_the_first_call(runtime, cuda_device, kind, head_major_out):
+    """As for an unmasked call: a result that is not finite is not checked, so the shape is not accepted."""
+    from npu_ai_b200 import comfy_nodes as cn
+    q, k, v = _qkv(cuda_device, 2, 8, 2 if kind == "grouped" else 8, 64, 64, 64, True)
+    mask = torch.ones(64, 64, dtype=torch.bool, device=cuda_device).tril(8)
+    mask[9] = False  # and a row that the mask does hide
+    kw = {"bool": dict(mask=mask), "additive": dict(mask=torch.where(mask, 0.0, -INF).to(BF16)),
+          "pad": dict(mask=torch.zeros(2, 1, 1, 64, device=cuda_device, dtype=BF16)), "grouped": dict(enable_gqa=True)}[kind]
+    good = q.clone()
+    q[1, 3, 40] = NAN
+    kw.update(skip_reshape=True, skip_output_reshape=head_major_out)
+    for bad in (q, torch.full_like(q, NAN)):
+        with pytest.raises(RuntimeError, match="does not match"):
+            cn._gpu_attention_override(_plain_model, bad, k, v, 8, **kw)
+        assert all(r.variant is None for r in runtime.attn.shapes.values())
+    before = runtime.attn.fused_calls
+    y = cn._gpu_attention_override(_plain_model, good, k, v, 8, **kw)
+    assert runtime.attn.fused_calls == before + 1
+    _check(y, good, k, v, 2 if kind == "grouped" else 8, kw.get("mask"), True, head_major_out)
+
+
+@pytest.mark.parametrize("shape", [(64, 64), (2, 1, 1, 64), (1, 8, 64, 64), (2, 8, 64, 64)])
+@pytest.mark.parametrize("dtype", [torch.bool, BF16, torch.float32])
+@pytest.mark.parametrize("head_major_out", [False, True])
+def test_rows_that_the_mask_hides_are_told_from_the_others(runtime, cuda_device, shape, dtype, head_major_out):
+    """Each form of mask with some rows hidden: accepted, and zeros there, whatever the model gives (NaN)."""
+    q, k, v = _qkv(cuda_device, 2, 8, 8, 64, 64, 40, False)
+    mask = torch.ones(shape, dtype=torch.bool, device=cuda_device)
+    mask[..., 50:] = False
+    (mask[7] if len(shape) == 2 else mask[-1, -1, min(7, shape[2] - 1)])[:] = False
+    if dtype != torch.bool:
+        mask = torch.where(mask, 0.0, -INF).to(dtype)
+
+    def nan_model(*a, **kw):  # a plain softmax: rows without a key are NaN
+        o = model_attention(*a, **kw)
+        m4 = mask if mask.dim() == 4 else mask[None, None]
+        none = (~m4 if dtype == torch.bool else m4 == -INF).all(-1).expand(2, 8, 64)
+        hm = o if head_major_out else o.unflatten(-1, (8, 40)).transpose(1, 2)
+        hm = torch.where(none[..., None], NAN, hm)
+        return hm if head_major_out else hm.transpose(1, 2).flatten(2)
+    from npu_ai_b200 import comfy_nodes as cn
+    y = cn._gpu_attention_override(nan_model, q, k, v, 8, mask=mask, skip_output_reshape=head_major_out)
+    (rec,) = runtime.attn.shapes.values()
+    assert rec.variant == 0 and rec.max_rel_err < 0.1
+    _check(y, q, k, v, 8, mask, False, head_major_out)
