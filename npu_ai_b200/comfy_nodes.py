@@ -55,7 +55,7 @@ def _mode(m: str) -> str:
 @dataclass
 class ShapeRecord:
     """The gate's knowledge of one attention shape, keyed (batch, query tokens, key tokens, heads, head dim), for masked
-    and grouped-query calls also by what the mask is."""
+    and grouped-query calls also by what the mask is: its form, type and the key/value heads."""
     variant_ms: dict[int, float] = field(default_factory=dict)  # timed once per variant on the first call
     model_ms: float | None = None        # the model's own attention, timed after one warm-up call
     variant: int | None = None           # the fused-kernel variant this shape runs
@@ -834,6 +834,13 @@ def _kernel_mask(mask, b: int, h: int, tq: int, tk: int, device):
     return mask if tk == 1 or mask.stride(-1) == 1 else mask.contiguous()
 
 
+def _mask_form(mask) -> str:
+    """Which of (batch, head, query) a mask differs over, as letters ("bhq", "b11", "11q" for a 2-D one): the kernel reads
+    one row for all queries another way than one per query."""
+    shape = (1,) * (4 - mask.dim()) + tuple(mask.shape)
+    return "".join(c if n > 1 else "1" for c, n in zip("bhq", shape))
+
+
 def _rows_without_a_key(mask, b: int, h: int, tq: int, d: int, head_major: bool) -> torch.Tensor:
     """Which rows of the output the mask leaves no key, laid out like it: (b, h, tq, 1) or (b, tq, h * d)."""
     none = (~mask if mask.dtype == torch.bool else mask == -float("inf")).all(-1)
@@ -869,7 +876,8 @@ def _gpu_attention_override(func, q, k, v, heads, mask=None, attn_precision=None
         fits = rt.gemm.attention_fused_fits(tq, tk, d, b * h)
         hk = k.shape[1] if skip_reshape else k.shape[2] // max(d, 1)
         kmask = _kernel_mask(mask, b, h, tq, tk, q.device) if mask is not None else None
-        key += ((f"{kmask.dtype} mask" if kmask is not None else "") + (f" {hk} kv heads" if gqa else ""),)
+        key += ((f"{_mask_form(kmask)} {kmask.dtype} mask" if kmask is not None else "")
+                + (f" {hk} kv heads" if gqa else ""),)
         why = gate.model_route_reason(key, mask is not None and kmask is None, gqa and (hk <= 0 or h % hk != 0), fits)
     else:
         fits = rt.gemm.attention_fits(tq, tk, d, b * h)

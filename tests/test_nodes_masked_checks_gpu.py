@@ -67,3 +67,17 @@ def test_rows_that_the_mask_hides_are_told_from_the_others(runtime, cuda_device,
     (rec,) = runtime.attn.shapes.values()
     assert rec.variant == 0 and rec.max_rel_err < 0.1
     _check(y, q, k, v, 8, mask, False, head_major_out)
+
+
+def test_each_form_of_mask_is_checked(runtime, cuda_device):
+    """The kernel reads a mask row for all queries another way than one per query: a check of one form does not vouch for
+    another."""
+    q, k, v = _qkv(cuda_device, 2, 8, 8, 64, 64, 64, False)
+    for n, shape in enumerate([(64, 64), (2, 1, 1, 64), (1, 1, 1, 64), (1, 8, 1, 64), (2, 8, 64, 64), (2, 1, 64, 64)]):
+        mask = torch.zeros(shape, dtype=BF16, device=cuda_device)
+        for _ in range(2):
+            _call(runtime, q, k, v, 8, mask=mask)
+        assert len(runtime.attn.shapes) == n + 1
+    assert all(r.max_rel_err is not None for r in runtime.attn.shapes.values())
+    _call(runtime, q, k, v, 8, mask=torch.zeros(1, 1, 64, 64, dtype=BF16, device=cuda_device))  # as [64, 64]
+    assert len(runtime.attn.shapes) == 6
