@@ -345,8 +345,9 @@ class NpuGemm:
 
     def _attn_operand(self, t) -> torch.Tensor:
         t = self._x_device(t)
-        # TMA addressing: 16-byte aligned base and strides in multiples of 8 elements, else one compact copy.
-        if t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:-1]):
+        # TMA addressing: 16-byte aligned base and positive strides in multiples of 8 elements, else one compact copy (of
+        # expanded operands, too).
+        if t.data_ptr() % 16 or any(s % 8 or (s <= 0 and n > 1) for s, n in zip(t.stride()[:-1], t.shape)):
             t = t.contiguous()
         return t
 

@@ -81,3 +81,17 @@ def test_each_form_of_mask_is_checked(runtime, cuda_device):
     assert all(r.max_rel_err is not None for r in runtime.attn.shapes.values())
     _call(runtime, q, k, v, 8, mask=torch.zeros(1, 1, 64, 64, dtype=BF16, device=cuda_device))  # as [64, 64]
     assert len(runtime.attn.shapes) == 6
+
+
+@pytest.mark.parametrize("head_major", [False, True])
+@pytest.mark.parametrize("masked", [False, True])
+def test_keys_shared_by_the_batch(runtime, cuda_device, head_major, masked):
+    """k and v expanded over the batch (stride 0), which TMA does not address: through the node and the runner."""
+    q, k, v = _qkv(cuda_device, 2, 8, 8, 64, 77, 40, head_major)
+    k, v = (t[:1].expand(2, *t.shape[1:]) for t in (k, v))
+    mask = torch.ones(64, 77, dtype=torch.bool, device=cuda_device).tril(20) if masked else None
+    y, _, fused, _ = _call(runtime, q, k, v, 8, mask=mask, skip_reshape=head_major, skip_output_reshape=head_major)
+    assert fused == 1
+    _check(y, q, k, v, 8, mask, head_major, head_major)
+    y = runtime.gemm.attention(q, k, v, 8, skip_reshape=head_major, skip_output_reshape=head_major, mask=mask)
+    _check(y, q, k, v, 8, mask, head_major, head_major)
