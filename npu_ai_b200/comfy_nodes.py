@@ -12,9 +12,10 @@ What changes: the model runs on the GPU, so calls route by device `cuda` (the re
 NPU, node :150, :174). The attention gate no longer chooses between the accelerator and the CPU: it chooses
 between kernel variants of the fused attention (query tiles per CTA x key tile) by timing each once per shape, and still
 checks the first result of every shape against the model's own attention (max relative error <= 0.1, else
-RuntimeError, node :225-232). Calls with a mask (bool or additive, 2-D or 4-D) or grouped key/value heads run the
-masked attention kernel, checked the same way (the reference leaves them to the CPU, node :39-99); masks of other
-forms and attention mode "off" (the reference's "cpu") run the model's own attention function, logged once per shape.
+RuntimeError, node :225-232). bf16 calls with a mask (bool or additive, 2-D or 4-D) or grouped key/value heads
+run the masked attention kernel, checked the same way (the reference leaves them to the CPU, node :39-99). Masked and
+grouped calls of other types, masks of other forms and attention mode "off" (the reference's "cpu") run the model's own
+attention function, logged once per shape.
 Linears of a Sequential that an activation follows (feed-forward projections without gating) apply it in the GEMM's
 epilogue.
 """
@@ -102,11 +103,13 @@ class AttentionGate:
             rec = self.shapes[key] = ShapeRecord()
         return rec
 
-    def model_route_reason(self, key: tuple, masked: bool, gqa: bool, fits: bool) -> str | None:
-        """Why this call must run the model's own attention, or None when the fused kernel takes it."""
+    def model_route_reason(self, key: tuple, masked: bool, gqa: bool, fits: bool, bits: bool = False) -> str | None:
+        """Why this call must run the model's own attention, or None when the fused kernel takes it. `bits`: a masked or
+        grouped call whose operands would lose bits in the kernel."""
         rules = ((self.mode == "off", "attention mode = off"),
                  (masked, "masked attention"),
                  (gqa, "grouped-query attention"),
+                 (bits, "masked or grouped, and not in bf16"),
                  (not fits, "outside the fused kernel's range"),
                  (key[1] < self.min_tokens, f"fewer than {self.min_tokens} query tokens"))
         why = next((text for hit, text in rules if hit), None)
@@ -878,7 +881,8 @@ def _gpu_attention_override(func, q, k, v, heads, mask=None, attn_precision=None
         kmask = _kernel_mask(mask, b, h, tq, tk, q.device) if mask is not None else None
         key += ((f"{_mask_form(kmask)} {kmask.dtype} mask" if kmask is not None else "")
                 + (f" {hk} kv heads" if gqa else ""),)
-        why = gate.model_route_reason(key, mask is not None and kmask is None, gqa and (hk <= 0 or h % hk != 0), fits)
+        why = gate.model_route_reason(key, mask is not None and kmask is None, gqa and (hk <= 0 or h % hk != 0), fits,
+                                      any(t.dtype != torch.bfloat16 for t in (q, k, v)))
     else:
         fits = rt.gemm.attention_fits(tq, tk, d, b * h)
         why = gate.model_route_reason(key, False, False, fits)

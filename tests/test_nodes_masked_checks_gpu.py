@@ -95,3 +95,24 @@ def test_keys_shared_by_the_batch(runtime, cuda_device, head_major, masked):
     _check(y, q, k, v, 8, mask, head_major, head_major)
     y = runtime.gemm.attention(q, k, v, 8, skip_reshape=head_major, skip_output_reshape=head_major, mask=mask)
     _check(y, q, k, v, 8, mask, head_major, head_major)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("case", ["mask", "grouped", "mixed"])
+def test_operands_of_more_bits_stay_with_the_model(runtime, cuda_device, dtype, case):
+    """Masked and grouped calls are computed in the caller's type: bit for bit the model's result."""
+    q, k, v = (t.to(dtype) for t in _qkv(cuda_device, 2, 8, 2 if case == "grouped" else 8, 64, 64, 64, True))
+    if case == "mixed":
+        q, k = q.to(BF16), k.to(BF16)
+
+    def func(q, k, v, *a, **kw):
+        return model_attention(q.to(v.dtype), k.to(v.dtype), v, *a, **kw)
+    kw = dict(enable_gqa=True) if case == "grouped" else \
+        dict(mask=torch.ones(64, 64, dtype=torch.bool, device=cuda_device).tril(8))
+    from npu_ai_b200 import comfy_nodes as cn
+    before = runtime.attn.fused_calls
+    for _ in range(2):
+        y = cn._gpu_attention_override(func, q, k, v, 8, skip_reshape=True, **kw)
+        assert torch.equal(y, func(q, k, v, 8, skip_reshape=True, **kw)) and y.dtype == dtype
+    assert runtime.attn.fused_calls == before
+    assert any("bf16" in (r.model_reason or "") for r in runtime.attn.shapes.values())
