@@ -837,6 +837,18 @@ def _kernel_mask(mask, b: int, h: int, tq: int, tk: int, device):
     return mask if tk == 1 or mask.stride(-1) == 1 else mask.contiguous()
 
 
+def _kernel_operands(q, k, v, h: int, head_major: bool, scale) -> bool:
+    """Whether the masked kernel takes these operands and loses nothing of them: k and v of one shape with q's batch and
+    head dim, nothing to differentiate, a positive scale. The model's own attention serves what does not fit."""
+    if k.dim() != q.dim() or v.shape != k.shape or k.shape[0] != q.shape[0]:
+        return False
+    if q.shape[3] != k.shape[3] if head_major else (q.shape[2] % h != 0 or k.shape[2] % (q.shape[2] // h) != 0):
+        return False
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
+        return False
+    return scale is None or (isinstance(scale, (int, float)) and 0.0 < scale < float("inf"))
+
+
 def _mask_form(mask) -> str:
     """Which of (batch, head, query) a mask differs over, as letters ("bhq", "b11", "11q" for a 2-D one): the kernel reads
     one row for all queries another way than one per query."""
@@ -876,7 +888,8 @@ def _gpu_attention_override(func, q, k, v, heads, mask=None, attn_precision=None
     masked = mask is not None or gqa
     kmask = None
     if masked:
-        fits = rt.gemm.attention_fused_fits(tq, tk, d, b * h)
+        fits = (rt.gemm.attention_fused_fits(tq, tk, d, b * h)
+                and _kernel_operands(q, k, v, h, skip_reshape, kwargs.get("scale")))
         hk = k.shape[1] if skip_reshape else k.shape[2] // max(d, 1)
         kmask = _kernel_mask(mask, b, h, tq, tk, q.device) if mask is not None else None
         key += ((f"{_mask_form(kmask)} {kmask.dtype} mask" if kmask is not None else "")

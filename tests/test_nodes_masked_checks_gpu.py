@@ -116,3 +116,37 @@ def test_operands_of_more_bits_stay_with_the_model(runtime, cuda_device, dtype, 
         assert torch.equal(y, func(q, k, v, 8, skip_reshape=True, **kw)) and y.dtype == dtype
     assert runtime.attn.fused_calls == before
     assert any("bf16" in (r.model_reason or "") for r in runtime.attn.shapes.values())
+
+
+def _stays(rt, func, q, k, v, heads, **kw):
+    """The call runs the model's own attention, twice, bit for bit."""
+    from npu_ai_b200 import comfy_nodes as cn
+    before = rt.attn.fused_calls
+    for _ in range(2):
+        assert torch.equal(cn._gpu_attention_override(func, q, k, v, heads, **kw), func(q, k, v, heads, **kw))
+    assert rt.attn.fused_calls == before
+
+
+def test_operands_that_the_kernel_does_not_take_stay_with_the_model(runtime, cuda_device):
+    """v of another width, k and v of one batch entry broadcast by the model, a scale of the model's own, no queries."""
+    q, k, v = _qkv(cuda_device, 2, 8, 8, 64, 64, 64, True)
+    mask = torch.ones(64, 64, dtype=torch.bool, device=cuda_device).tril(8)
+    kw = dict(mask=mask, skip_reshape=True, skip_output_reshape=True)
+    _stays(runtime, model_attention, q, k, v[..., :40], 8, **kw)
+    _stays(runtime, model_attention, q, k[:1], v[:1], 8, **kw)
+    _stays(runtime, model_attention, q, k, v, 8, scale=-0.125, **kw)
+    _stays(runtime, model_attention, q, k, v, 8, scale=torch.tensor(0.125).item() * 0.0, **kw)
+    assert all(r.variant is None for r in runtime.attn.shapes.values())
+
+
+def test_gradients_stay_with_the_model(runtime, cuda_device):
+    from npu_ai_b200 import comfy_nodes as cn
+    q, k, v = _qkv(cuda_device, 2, 8, 8, 64, 64, 64, False)
+    mask = torch.ones(64, 64, dtype=torch.bool, device=cuda_device).tril(8)
+    k.requires_grad_()
+    y = cn._gpu_attention_override(model_attention, q, k, v, 8, mask=mask)
+    y.float().square().sum().backward()
+    assert k.grad is not None and bool(k.grad.abs().sum() > 0)
+    with torch.no_grad():  # nothing to lose: the kernel
+        y, _, fused, _ = _call(runtime, q, k, v, 8, mask=mask)
+    assert fused == 1
