@@ -150,3 +150,40 @@ def test_gradients_stay_with_the_model(runtime, cuda_device):
     with torch.no_grad():  # nothing to lose: the kernel
         y, _, fused, _ = _call(runtime, q, k, v, 8, mask=mask)
     assert fused == 1
+
+
+@pytest.mark.parametrize("dtype", [torch.bool, BF16, torch.float32])
+def test_models_with_other_rows_without_a_key(runtime, cuda_device, dtype):
+    """A model that fills with a finite value gives the average of v where its mask leaves nothing; a model that casts f32's
+    lowest value to bf16 gives NaN where the kernel gives the average. Their calls stay with them instead of failing."""
+    from npu_ai_b200 import comfy_nodes as cn
+    q, k, v = _qkv(cuda_device, 2, 8, 8, 64, 64, 64, True)
+    mask = torch.ones(64, 64, dtype=torch.bool, device=cuda_device)
+    mask[5] = False
+    hide = mask
+    if dtype == BF16:
+        mask = torch.where(mask, 0.0, -INF).to(BF16)
+    elif dtype == torch.float32:
+        mask = torch.where(mask, 0.0, torch.finfo(torch.float32).min)
+
+    def func(q, k, v, heads, mask=None, **kw):
+        s = (q.float() @ k.float().transpose(-1, -2)) * 0.125
+        s = s + mask.to(BF16).float() if dtype == torch.float32 else s.masked_fill(~hide, -1e30)
+        return (s.softmax(-1) @ v.float()).to(BF16)
+    before = runtime.attn.fused_calls
+    for _ in range(2):
+        y = cn._gpu_attention_override(func, q, k, v, 8, mask=mask, skip_reshape=True, skip_output_reshape=True)
+        ref = func(q, k, v, 8, mask=mask)
+        assert torch.equal(torch.nan_to_num(y), torch.nan_to_num(ref)) and torch.equal(y.isnan(), ref.isnan())
+    assert runtime.attn.fused_calls == before
+    (rec,) = runtime.attn.shapes.values()
+    assert "no key" in rec.model_reason
+    # any other difference is still an error
+
+    def wrong(*a, **kw):
+        o = func(*a, **kw).clone()
+        o[:, :, 9] += 5.0
+        return o
+    runtime.attn.reset()
+    with pytest.raises(RuntimeError, match="does not match"):
+        cn._gpu_attention_override(wrong, q, k, v, 8, mask=mask, skip_reshape=True, skip_output_reshape=True)
