@@ -83,7 +83,8 @@ class AttentionGate:
     ``gpu`` keeps the kernel's own automatic variant; ``off`` (the reference's ``cpu``) hands every call to the
     model's own attention. In every mode the first fused result of a shape is compared with the model's own
     attention (max relative error <= 0.1, else RuntimeError). Calls with a mask or grouped-query heads that the
-    masked kernel takes have one variant; the model's attention serves what it does not take. ``min_tokens``
+    masked kernel takes have one variant; the model's attention serves what it does not take and, in mode ``auto``, the
+    shapes that it is clearly faster on. ``min_tokens``
     (default 1, so every SD1.5 self- and cross-attention, the 64-token middle block included, stays on the kernel)
     sends shorter query sequences there too; each such shape is logged once with its reason.
     """
@@ -940,6 +941,13 @@ def _gpu_attention_override(func, q, k, v, heads, mask=None, attn_precision=None
         model_y, rec.model_ms = _time_gpu(model_attn, rt.gemm.device)
         ref, other = model_y.float(), y.float()
         stay = None
+        if masked and gate.mode == "auto":
+            # These calls were the model's: one that is clearly faster (a tenth and 10 us, best of three) keeps them.
+            for _ in range(2):
+                rec.variant_ms[0] = min(rec.variant_ms[0], _time_gpu(lambda: fused(0), rt.gemm.device)[1])
+                rec.model_ms = min(rec.model_ms, _time_gpu(model_attn, rt.gemm.device)[1])
+            if rec.model_ms < 0.9 * rec.variant_ms[0] and rec.model_ms + 0.01 < rec.variant_ms[0]:
+                stay = "the model's attention is faster"
         if kmask is not None:
             # What a row without a key gives is the model's own convention: zeros here, NaN from a plain softmax, an average
             # where hidden keys have a finite score. NaN stands for zeros; a model with another convention keeps its calls.

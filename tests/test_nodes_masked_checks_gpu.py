@@ -187,3 +187,33 @@ def test_models_with_other_rows_without_a_key(runtime, cuda_device, dtype):
     runtime.attn.reset()
     with pytest.raises(RuntimeError, match="does not match"):
         cn._gpu_attention_override(wrong, q, k, v, 8, mask=mask, skip_reshape=True, skip_output_reshape=True)
+
+
+def test_shapes_on_which_the_model_is_faster_stay_with_it(runtime, cuda_device):
+    """Auto mode keeps a masked shape with the model's attention when that took clearly less time; gpu mode does not."""
+    from npu_ai_b200 import comfy_nodes as cn
+    q, k, v = _qkv(cuda_device, 2, 8, 8, 4096, 4096, 40, True)
+    mask = torch.zeros(4096, 4096, dtype=BF16, device=cuda_device)
+    ref = model_attention(q, k, v, 8, mask=mask, skip_reshape=True, skip_output_reshape=True)
+
+    def func(*a, **kw):  # a model as fast as can be
+        return ref
+    for _ in range(2):
+        before = runtime.attn.fused_calls, runtime.attn.model_calls
+        y = cn._gpu_attention_override(func, q, k, v, 8, mask=mask, skip_reshape=True, skip_output_reshape=True)
+        assert y is ref and (runtime.attn.fused_calls, runtime.attn.model_calls) == (before[0], before[1] + 1)
+    (rec,) = runtime.attn.shapes.values()
+    assert "faster" in rec.model_reason and rec.model_ms < rec.variant_ms[0]
+    runtime.attn.reset()
+    runtime.attn.mode = "gpu"
+    before = runtime.attn.fused_calls
+    y = cn._gpu_attention_override(func, q, k, v, 8, mask=mask, skip_reshape=True, skip_output_reshape=True)
+    assert runtime.attn.fused_calls == before + 1 and y is not ref
+
+
+def test_shapes_on_which_the_kernel_is_faster_use_it(runtime, cuda_device):
+    q, k, v = _qkv(cuda_device, 2, 8, 8, 1024, 1024, 80, True)
+    mask = torch.rand(1024, 1024, device=cuda_device) < 0.5
+    mask[:, 0] = True
+    y, _, fused, _ = _call(runtime, q, k, v, 8, mask=mask, skip_reshape=True, skip_output_reshape=True)
+    assert fused == 1
