@@ -475,16 +475,24 @@ def _activation_name(mod) -> str | None:
     return {torch.nn.SiLU: "silu", torch.nn.ReLU: "relu"}.get(type(mod))
 
 
+def _forward_is_known(mod) -> bool:
+    """Whether the module's forward is its class's or the node's own for Linears."""
+    own = mod.__dict__.get("forward")
+    return own is None or getattr(own, "__func__", None) is _gpu_linear_forward
+
+
 def _linear_act_pairs(mod, rt) -> list[int]:
     """The places of a Sequential's taken-over Linears that an activation of the GEMM's epilogue follows. Linears that
-    serve others' products (q/k/v groups) and modules with hooks, which would be passed by, are left out."""
+    serve others' products (q/k/v groups) and modules with hooks or a forward that somebody else put on them, which would
+    be passed by, are left out."""
     if type(mod) is not torch.nn.Sequential:
         return []
     items = list(mod)
     return [i for i, (a, b) in enumerate(zip(items, items[1:]))
             if isinstance(a, torch.nn.Linear) and id(a) in rt.weights and _activation_name(b) is not None
             and id(a) not in rt.fused_member and id(a) not in rt.fused_groups
-            and not any(m._forward_hooks or m._forward_pre_hooks for m in (a, b))]
+            and not any(m._forward_hooks or m._forward_pre_hooks for m in (a, b))
+            and _forward_is_known(a) and _forward_is_known(b)]
 
 
 def _gpu_linear_act_forward(self, x):
