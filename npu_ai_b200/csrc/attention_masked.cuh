@@ -311,7 +311,7 @@ __device__ __forceinline__ float modify_scores(const MaskedArgs& m, const Row& w
     for (int t = 0; t < BN; t += 2) big = fmax3(big, fabsf(s[t]), fabsf(s[t + 1]));
     if (__all_sync(0xffffffffu, !w.valid || big * m.cap_in <= 1.0f)) {
       // The usual case, on the FMA pipe (the MUFU has the softmax's exponentials to do): cap tanh(y) = y P(y^2).
-const uint64_t in2 = f2_pack(m.cap_in, m.cap_in);
+      const uint64_t in2 = f2_pack(m.cap_in, m.cap_in);
 #pragma unroll
       for (int t = 0; t < BN; t += 2) {
         const uint64_t y = f2_mul(f2_pack(s[t], s[t + 1]), in2), z = f2_mul(y, y);

@@ -161,11 +161,8 @@ int check_gemm_common(int64_t m, int64_t k, int64_t n, int bias_dtype, const voi
 
 namespace npub200 {
 
-size_t gemm_workspace_bytes(const void* x, int64_t ldx, int64_t m, int64_t k, const void* w, int64_t ldw, int64_t n,
-                            int variant, int sms, int geglu) {
-  (void)variant;
-  (void)sms;
-  return gemm_ws_layout(x, ldx, m, k, w, ldw, n, geglu).total;
+size_t gemm_workspace_bytes(const void* x, int64_t ldx, int64_t m, int64_t k, const void* w, int64_t ldw, int64_t n) {
+  return gemm_ws_layout(x, ldx, m, k, w, ldw, n).total;
 }
 
 int gemm_with_workspace(const void* x, int64_t ldx, int64_t m, int64_t k, const void* w, int64_t ldw, int64_t n,
@@ -351,6 +348,8 @@ int npub200_conv3x3(const void* x, int64_t n, int64_t h, int64_t w, int64_t cin,
   if (bias_dtype != NPUB200_DTYPE_BF16 && bias_dtype != NPUB200_DTYPE_F32)
     return fail(kErrInvalid, "unknown bias dtype code %d", bias_dtype);
   if (bias_img_stride < 0) return fail(kErrInvalid, "negative bias row stride");
+  (void)workspace;  // split K reduces inside a cluster
+  (void)workspace_bytes;
   ConvProblem p;
   memset(&p, 0, sizeof(p));
   p.x = x;
@@ -370,8 +369,6 @@ int npub200_conv3x3(const void* x, int64_t n, int64_t h, int64_t w, int64_t cin,
   p.out_f32 = out_dtype == NPUB200_DTYPE_F32;
   p.variant = variant;
   p.debug = g_debug_flags.load();
-  p.ws_split = workspace;
-  p.ws_split_bytes = workspace_bytes;
   return conv3x3_launch(p, static_cast<cudaStream_t>(stream));
 }
 
@@ -407,10 +404,11 @@ int npub200_group_norm_scratch_size(int64_t n, int64_t groups, size_t* bytes_out
 
 int npub200_conv3x3_workspace_size(int64_t n, int64_t h, int64_t w, int64_t cin, int64_t cout, int variant,
                                    size_t* bytes_out) {
+  (void)n, (void)h, (void)w, (void)cin, (void)cout, (void)variant;
   if (bytes_out == nullptr) return fail(kErrInvalid, "null output pointer");
   const DeviceInfo* d = nullptr;
   if (int rc = current_device_info(&d)) return rc;
-  *bytes_out = conv3x3_workspace_bytes(n, h, w, cin, cout, variant, d->sms);
+  *bytes_out = 0;  // split K reduces inside a cluster
   return kOk;
 }
 

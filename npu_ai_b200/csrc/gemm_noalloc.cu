@@ -66,7 +66,7 @@ extern "C" int npub200_gemm_noalloc(const void* x, int64_t ldx, int64_t m, int64
                 (long long)n);
   const DeviceInfo* dev = nullptr;
   if (int rc = current_device_info(&dev)) return rc;
-  const size_t need = gemm_workspace_bytes(x, ldx, m, k, w, ldw, n, variant, dev->sms);
+  const size_t need = gemm_workspace_bytes(x, ldx, m, k, w, ldw, n);
   if (need > size_t(NPUB200_NOALLOC_SCRATCH_BYTES))
     return fail(kErrInvalid,
                 "npub200_gemm_noalloc: this GEMM (M=%lld K=%lld N=%lld) needs %zu bytes of scratch, above the "

@@ -1402,7 +1402,6 @@ GemmPlan gemm_plan(int64_t M, int64_t N, int64_t K, int sms, int variant, bool g
         best.bn = bn;
         best.splits = sp;
         best.kb_per_split = kps;
-        best.split_ws_bytes = 0;  // split K reduces through distributed shared memory: no workspace
       }
     }
   }
@@ -1658,11 +1657,6 @@ int conv3x3_launch(const ConvProblem& p, cudaStream_t stream) {
     case 256: return launch_variant<256, 4, kModeConv3x3>(mx, mw, mo, a, units, sms, stream, d);
   }
   return fail(kErrUnsupported, "no conv3x3 variant with an output-channel tile of %d", bn);
-}
-
-size_t conv3x3_workspace_bytes(int64_t n, int64_t h, int64_t w, int64_t cin, int64_t cout, int variant, int sms) {
-  if (n <= 0 || h <= 0 || w <= 0 || cin <= 0 || cout <= 0 || sms <= 0) return 0;
-  return gemm_plan(n * h * w, cout, 9 * cin, sms, variant, false, false).split_ws_bytes;
 }
 
 // ---------------------------------------------------------------------------------------------------------------

@@ -76,8 +76,6 @@ struct GemmProblem {
   int64_t M, N, K;
   int variant;       // 0 = automatic, else a forced N tile (64, 96, 128, 160, 192, 256)
   const CUtensorMap* w_map_cache;  // optional cached B tensor map (matching the chosen tile), may be null
-  void* ws_split;                  // caller workspace (split K needs none: it reduces inside a cluster)
-  size_t ws_split_bytes;
   uint32_t debug;
   int geglu;  // 1: W has 2N rows [a; gate] and out[:, j] = (x.W[j] + b[j]) * gelu(x.W[N+j] + b[N+j]); bias has 2N
   const void* residual;  // bf16 [M, N] added after the bias (row stride ldr), or null
@@ -89,7 +87,6 @@ struct GemmPlan {
   int bn;
   int splits;
   int kb_per_split;
-  size_t split_ws_bytes;  // bytes of split-K workspace the plan needs (0: split K reduces inside a cluster)
   bool pair;              // 256-row tiles on a two-CTA cluster (tcgen05 cta_group::2)
 };
 // Tile variants: BN (64 ... 256) for one CTA per tile, kGemmPairVariant + BN (128, 192, 256) for a CTA pair.
@@ -105,9 +102,8 @@ inline int gemm_plan_variant(const GemmPlan& p) { return p.pair ? kGemmPairVaria
 // Weight rows per TMA box: BN, or BN/2 for the GEGLU form (a and gate halves) and for one CTA of a pair.
 inline int gemm_plan_box_rows(const GemmPlan& p, bool geglu) { return (p.pair || geglu) ? p.bn / 2 : p.bn; }
 int gemm_encode_b_map(const void* w, int64_t ldw, int64_t N, int64_t K, int box_rows, CUtensorMap* out);
-// Bytes of workspace the GEMM entry points use for a problem (split-K counters + partials, repack buffers).
-size_t gemm_workspace_bytes(const void* x, int64_t ldx, int64_t m, int64_t k, const void* w, int64_t ldw, int64_t n,
-                            int variant, int sms, int geglu = 0);
+// Bytes of workspace the GEMM entry points use for a problem: repacked operands (split K reduces inside a cluster).
+size_t gemm_workspace_bytes(const void* x, int64_t ldx, int64_t m, int64_t k, const void* w, int64_t ldw, int64_t n);
 // The GEMM entry point's body with a caller-given workspace (argument checks, repacking, split-K, launch).
 int gemm_with_workspace(const void* x, int64_t ldx, int64_t m, int64_t k, const void* w, int64_t ldw, int64_t n,
                         const CUtensorMap* w_map, const void* bias, int bias_dtype, void* out, int64_t ldo,
@@ -131,8 +127,6 @@ struct ConvProblem {
   int out_f32;
   int variant;                // 0 or a forced output-channel tile
   uint32_t debug;
-  void* ws_split;             // caller workspace (split K needs none: it reduces inside a cluster)
-  size_t ws_split_bytes;
 };
 int conv3x3_launch(const ConvProblem& p, cudaStream_t stream);
 // GroupNorm (+ SiLU) over NHWC bf16: x, out [n][hw][c]; gamma, beta f32 [c]; stats: group_norm_scratch_bytes()
@@ -154,8 +148,6 @@ int upsample_nearest2x_launch(const void* x, int64_t n, int64_t h, int64_t w, in
                               cudaStream_t stream);
 int concat_channels_launch(const void* a, int64_t lda, int64_t ca, const void* b, int64_t ldb, int64_t cb,
                            int64_t pixels, void* out, int64_t ldo, cudaStream_t stream);
-// Split-K workspace bytes the convolution's fastest plan uses (0: none).
-size_t conv3x3_workspace_bytes(int64_t n, int64_t h, int64_t w, int64_t cin, int64_t cout, int variant, int sms);
 // bf16 copy of a row-strided matrix into a dense [rows, cols_pad] buffer, zero-filling the pad columns.
 int repack_rows_bf16(const void* src, int64_t ld_src, int64_t rows, int64_t cols, void* dst, int64_t cols_pad,
                      cudaStream_t stream);
