@@ -1378,7 +1378,7 @@ GemmPlan gemm_plan(int64_t M, int64_t N, int64_t K, int sms, int variant, bool g
   // split into a and gate halves of 32-column multiples are candidates. `variant` (when not 0) forces one tile:
   // BN, or kGemmPairVariant + BN for the paired form.
   const int64_t kb = (K + kGemmBK - 1) / kGemmBK;
-  GemmPlan best{128, 1, int(kb), 0, false};
+  GemmPlan best{128, 1, int(kb), false};
   double best_cost = 1e300;
   for (int bn : kTileChoices) {
     if (variant && bn != variant) continue;
@@ -1415,7 +1415,7 @@ GemmPlan gemm_plan(int64_t M, int64_t N, int64_t K, int sms, int variant, bool g
     const double cost = plan_cost_pair(M, N, kb, bn, sms);
     if (variant || cost < best_cost * 0.999) {
       best_cost = cost;
-      best = GemmPlan{bn, 1, int(kb), 0, true};
+      best = GemmPlan{bn, 1, int(kb), true};
     }
   }
   return best;
