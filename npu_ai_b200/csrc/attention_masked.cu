@@ -360,11 +360,12 @@ int attention_masked_launch(const AttnMaskedProblem& mp, cudaStream_t stream) {
   const dim3 grid{unsigned(plan.pairs), unsigned(plan.tiles), unsigned(plan.splits)};
   const int feats = m.gaps ? kFeatAny
                            : (o.softcap > 0.0f ? kFeatCap : 0) | (o.slopes || o.distance_bias ? kFeatDistance : 0) |
-                                 (o.mask ? kFeatMask : 0);
+                                 (o.mask == nullptr ? 0 : m.mask_row ? kFeatMaskRow : kFeatMask);
   auto launch = feats == 0               ? launch_masked_for<0>
                 : feats == kFeatCap      ? launch_masked_for<kFeatCap>
                 : feats == kFeatDistance ? launch_masked_for<kFeatDistance>
                 : feats == kFeatMask     ? launch_masked_for<kFeatMask>
+                : feats == kFeatMaskRow  ? launch_masked_for<kFeatMaskRow>
                                          : launch_masked_for<kFeatAny>;
   if (int rc = launch(p.D, plan.streams, mq, mk, mv, m, grid, stream, dev->device)) return rc;
   if (plan.splits == 1 || plan.cluster) return kOk;

@@ -209,7 +209,10 @@ constexpr float kTanhRatio[6] = {9.999994040e-01f, -3.332909346e-01f, 1.32818847
 
 // What a kernel instantiation does to the scores: nothing, one of these, or any of them as the arguments say. (One
 // kernel with every branch spent as long on instruction fetches as on the instructions.)
-constexpr int kFeatCap = 1, kFeatDistance = 2, kFeatMask = 4, kFeatAny = 7;
+// A mask tensor with a row of its own for each query and one whose row a warp shares are two kinds: in one kernel a few
+// instructions more in either moved the other by 10% (1x24x4608x4608x128 with a bool mask of its own rows 431 us before the
+// NaN tests, 465 with them, 408 in a kernel of its own).
+constexpr int kFeatCap = 1, kFeatDistance = 2, kFeatMask = 4, kFeatMaskRow = 8, kFeatAny = 15;
 template <int FEAT>
 __device__ __forceinline__ bool has_cap(const MaskedArgs& m) {
   return FEAT == kFeatCap || (FEAT == kFeatAny && m.cap_in != 0.0f);
@@ -220,7 +223,11 @@ __device__ __forceinline__ bool has_distance(const MaskedArgs& m) {
 }
 template <int FEAT>
 __device__ __forceinline__ bool has_mask(const MaskedArgs& m) {
-  return FEAT == kFeatMask || (FEAT == kFeatAny && m.mask_kind != 0);
+  return FEAT == kFeatMask || FEAT == kFeatMaskRow || (FEAT == kFeatAny && m.mask_kind != 0);
+}
+template <int FEAT>
+__device__ __forceinline__ bool has_mask_row(const MaskedArgs& m) {
+  return FEAT == kFeatMaskRow || (FEAT == kFeatAny && m.mask_row);
 }
 
 // A mask value in log2 units: -inf hides; any finite value, however low, stays finite; a NaN stays.
@@ -361,7 +368,14 @@ __device__ __forceinline__ float modify_scores(const MaskedArgs& m, const Row& w
     k = 1.0f;
   }
   if (!has_mask<FEAT>(m)) return k;
-  if (m.mask_row) {  // one mask row for the warp: broadcast from shared memory
+  if (has_mask_row<FEAT>(m)) {  // one mask row for the warp: broadcast from shared memory
+    // What it hides is replaced: -inf added to a NaN or an infinite score would not hide it.
+    const uint32_t hidden = __ballot_sync(0xffffffffu, row_mask == -INFINITY);
+    if (hidden == 0xffffffffu) {
+#pragma unroll
+      for (int t = 0; t < BN; ++t) s[t] = -INFINITY;
+      return 1.0f;
+    }
     s_mask[lane] = row_mask;
     const bool low = row_mask < -1e37f && row_mask != -INFINITY;
     const bool lows = __any_sync(0xffffffffu, low);
@@ -374,6 +388,10 @@ __device__ __forceinline__ float modify_scores(const MaskedArgs& m, const Row& w
         s[t + 1] = fmaf(s[t + 1], k, e.y);
         s[t + 2] = fmaf(s[t + 2], k, e.z);
         s[t + 3] = fmaf(s[t + 3], k, e.w);
+      }
+      if (hidden != 0u) {
+#pragma unroll
+        for (int t = 0; t < BN; ++t) s[t] = (hidden >> t) & 1u ? -INFINITY : s[t];
       }
     } else {
 #pragma unroll
@@ -388,7 +406,10 @@ __device__ __forceinline__ float modify_scores(const MaskedArgs& m, const Row& w
   // (scores of keys behind the last get any value here: no row sees them)
   MaskBytes bytes(w.mask + (long long)kv0 * esz, w.mask + (long long)m.a.Skv * esz, m.mask_vec && m.a.Skv - kv0 >= BN);
   // -inf hides; any finite value, however low, stays finite in log2 units; a NaN, of the score or the mask, stays.
-  auto add = [k](float x, float e) { return e == -INFINITY ? -INFINITY : max_nan(fmaf(x, k, e * kLog2e), -FLT_MAX); };
+  auto add = [k](float x, float e) {
+    const float r = fmaf(x, k, e * kLog2e);
+    return e == -INFINITY ? -INFINITY : r < -FLT_MAX ? -FLT_MAX : r;
+  };
   if (m.mask_kind == 1) {
     uint4 v[BN / 16];
     bytes.take(v);
@@ -461,32 +482,20 @@ __device__ __forceinline__ float masked_softmax_step(const MaskedArgs& m, const 
     for (int t = 0; t < kHalf; ++t) s[t] = __uint_as_float(r[t]);
   }
   // Partly seen: the keys [a, z) of this half as bits, a bit test a score instead of two comparisons.
-  bool partial = w.lo_max > key0 || w.hi_min < key0 + kHalf;
+  const bool partial = w.lo_max > key0 || w.hi_min < key0 + kHalf;
   uint32_t keep = 0xffffffffu;
   if (partial) {
     const int a = max(w.lo - key0, 0), z = min(w.hi - key0, kHalf);
     keep = a < z ? (0xffffffffu << a) & (0xffffffffu >> (32 - z)) : 0u;
     static_assert(kHalf == 32, "a bit a key");
-  }
-  // What a mask row of the whole warp hides goes the same way: its -inf added to a NaN or an infinite score would not
-  // hide it.
-  uint32_t hidden = 0u;
-  if (has_mask<FEAT>(m) && m.mask_row) {
-    hidden = __ballot_sync(0xffffffffu, row_mask == -INFINITY);
-    keep &= ~hidden;
-    partial = partial || hidden != 0;
-  }
-  if constexpr ((FEAT & kFeatCap) != 0) {
-    // The largest score chooses between the cap's two forms: stale memory must have no say in it.
-    if (partial) {
+    if constexpr ((FEAT & kFeatCap) != 0) {
+      // The largest score chooses between the cap's two forms: stale memory must have no say in it.
 #pragma unroll
       for (int t = 0; t < kHalf; ++t) s[t] = (keep >> t) & 1u ? s[t] : 0.0f;
     }
   }
   float c = m.a.scale_log2;
-  if constexpr (FEAT != 0) {
-    if (hidden != 0xffffffffu) c = modify_scores<FEAT, kHalf>(m, w, key0, row_mask, s_table, s_mask, lane, s);
-  }
+  if constexpr (FEAT != 0) c = modify_scores<FEAT, kHalf>(m, w, key0, row_mask, s_table, s_mask, lane, s);
   if (partial) {
 #pragma unroll
     for (int t = 0; t < kHalf; ++t) s[t] = (keep >> t) & 1u ? s[t] : -INFINITY;
@@ -928,7 +937,7 @@ __global__ void __launch_bounds__(MaskedLayout<DP, STAGES, STREAMS>::kThreads,
       const int kv0 = (first + j) * BN;
       float row_mask = 0.0f;
       if (has_mask<FEAT>(m)) {
-        if (m.mask_row)
+        if (has_mask_row<FEAT>(m))
           row_mask = mask_row_value(m, w, kv0 + half * kHalf, lane);
         else
           prefetch_mask(m, w, kv0 + STREAMS * BN + half * kHalf);
@@ -1125,6 +1134,8 @@ extern template int launch_masked_for<kFeatDistance>(int64_t, int, const CUtenso
                                                      const MaskedArgs&, dim3, cudaStream_t, int);
 extern template int launch_masked_for<kFeatMask>(int64_t, int, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&,
                                                  const MaskedArgs&, dim3, cudaStream_t, int);
+extern template int launch_masked_for<kFeatMaskRow>(int64_t, int, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&,
+                                                    const MaskedArgs&, dim3, cudaStream_t, int);
 extern template int launch_masked_for<kFeatAny>(int64_t, int, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&,
                                                 const MaskedArgs&, dim3, cudaStream_t, int);
 

@@ -1,4 +1,4 @@
-// attention_masked_tensor.cu - the masked attention kernels with a mask tensor.
+// attention_masked_tensor.cu - the masked attention kernels with a mask tensor that has a row for each query.
 #include "attention_masked.cuh"
 
 namespace npub200 {
