@@ -17,7 +17,7 @@
 //     chain of waits (TMEM load, maximum, exchange, exponentials, store) of which the instructions are half.
 //   * Two streams of key tiles where an SM holds one CTA (two_streams in attention_masked.cu): sixteen warps, eight on the
 //     even and eight on the odd tiles with running maxima, sums and O accumulators of their own, joined at the end. One
-//     stream's waits are the other's work: 2x8x1024x1024x80 with a bool mask 32.5 -> 18.3 us (now 19.1, any byte a true).
+//     stream's waits are the other's work: 2x8x1024x1024x80 with a bool mask 32.5 -> 18.3 us (now 17.9).
 //   * Q rows: `pack` query heads x T positions. With few queries the heads of a group that share a K/V head fill the
 //     tile together (one TMA box of pack heads x T positions), so the cache is read once per group, not once per head.
 //   * Keys beyond the union inside its last (or before it inside its first) tile may be stale cache memory: their V
@@ -27,8 +27,9 @@
 //     parts are a cluster, which joins them through its shared memory; otherwise each CTA writes its unnormalised O row,
 //     max and sum to the workspace and attention_join_kernel joins the parts, either way in part order.
 // What bounds it: a token against a long cache, memory (16x32/8 over 16384 keys of 128: 134 us, 6.1 of 6.5 TB/s); a long
-// prompt, the softmax step and the shared-memory port together (1x32/8x4096x4096x128 causal: 131 us, 1.05 PFLOP/s, tensor
-// pipe 53%, issue 56%); everything between, the step's latency, 0.7 - 1.3 us a tile, and 2.5 - 4 us of a CTA's start and end.
+// prompt, the waits of the softmax step's chain (1x32/8x4096x4096x128 causal: 130 us, 1.05 PFLOP/s; no pipe is full: tensor
+// 54%, MUFU 55%, issue 55%, loads and stores of shared memory 11%); everything between, the same chain, 0.7 - 1.3 us a
+// tile, and 2.5 - 4 us of a CTA's start and end.
 // Rounding: P is rounded to bf16 for the tensor core (relative 2^-8, as in the unmasked kernel); the sums, the maxima,
 // the modifiers and O are f32.
 #pragma once

@@ -54,7 +54,7 @@ constexpr int kModeAct = 3;  // plain GEMM with an activation between the bias a
 // Epilogue warps of an instantiation. The activation form's wide tiles take 16, in two sets of 8 that serve alternate
 // tiles (one accumulator buffer each): its epilogue is longer than the main loop, and with two tiles in work one set's
 // arithmetic overlaps the other's loads and stores. Measured at 65536 x 320 x 1280 with gelu and residual: 8 warps 126
-// us, one set of 16 109 us, two sets 106 us (relu 86 us; 124 us for the plain form's epilogue with residual alone).
+// us, one set of 16 109 us, two sets 107 us (relu 86 us; 124 us for the plain form's epilogue with residual alone).
 template <int BN, int MODE>
 constexpr int gemm_epi_warps() {
   return MODE == kModeAct && BN >= 128 ? 16 : kGemmEpiWarps;
