@@ -851,14 +851,14 @@ def _kernel_mask(mask, b: int, h: int, tq: int, tk: int, device):
 
 def _kernel_operands(q, k, v, h: int, head_major: bool, scale) -> bool:
     """Whether the masked kernel takes these operands and loses nothing of them: k and v of one shape with q's batch and
-    head dim, nothing to differentiate, a positive scale. The model's own attention serves what does not fit."""
+    head dim, nothing to differentiate, a positive scale within f32. The model's own attention serves what does not fit."""
     if k.dim() != q.dim() or v.shape != k.shape or k.shape[0] != q.shape[0]:
         return False
     if q.shape[3] != k.shape[3] if head_major else (q.shape[2] % h != 0 or k.shape[2] % (q.shape[2] // h) != 0):
         return False
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
         return False
-    return scale is None or (isinstance(scale, (int, float)) and 0.0 < scale < float("inf"))
+    return scale is None or (isinstance(scale, (int, float)) and 1e-37 <= scale <= 1e38)
 
 
 def _mask_form(mask) -> str:
