@@ -252,6 +252,79 @@ int npub200_attention_masked(const void* q, int64_t q_sb, int64_t q_ss, int64_t 
                              void* stream);
 
 /* ----------------------------------------------------------------------------------------------------------
+ * Rotary positions: what a text model does with its queries and keys before their scores (the reference runs no text
+ * model; its host would do this around the offloaded projections). Pair j of a head's first rot_dim values, (j, j +
+ * rot_dim / 2) or, interleaved, (2j, 2j + 1), at position p:
+ *   u' = m (u cos a - v sin a), v' = m (v cos a + u sin a), a = p freqs[j];
+ * the other values are copied. With `inverse` the pair turns by -a: with magnitude 1 that undoes the rotation, and with the
+ * rotation's own magnitude it is its gradient (dy to dx). Angles in 64 bits, the rotation in f32, one rounding.
+ * x and out: [batch, seq, heads, head_dim] strided as in npub200_attention, any strides >= 0, bf16 or f32 each; out may be
+ * x itself (same strides and type) and shares no element with it otherwise. head_dim even, up to 1024. The position of
+ * token (b, s): positions[b * pos_sb + s * pos_ss], or starts[b] + s, or start + s (in this order, where given; both
+ * pointers: NPUB200_EINVAL). Any int32 is a position. batch, seq or heads 0: nothing is done. Allocates nothing.
+ * ---------------------------------------------------------------------------------------------------------- */
+typedef struct npub200_rotation {
+  const double* freqs; /* [rot_dim / 2] radians a position, in device memory */
+  int64_t rot_dim;     /* even, 0 ... head_dim */
+  int32_t interleaved;
+  int32_t inverse;
+  float magnitude;     /* m: 1 without scaling */
+} npub200_rotation;
+int npub200_rope(const void* x, int64_t x_sb, int64_t x_ss, int64_t x_sh, int x_dtype, void* out, int64_t o_sb,
+                 int64_t o_ss, int64_t o_sh, int out_dtype, int64_t batch, int64_t seq, int64_t heads, int64_t head_dim,
+                 const npub200_rotation* rotation, int64_t start, const int32_t* starts, const int32_t* positions,
+                 int64_t pos_sb, int64_t pos_ss, void* stream);
+
+/* ----------------------------------------------------------------------------------------------------------
+ * A key/value cache in pages, which a batch of sequences shares: sequence b's position p lies in slot p % page_size of
+ * page table[b * table_stride + p / page_size]. Element (page, slot, head, e) of the keys at page*k_sp + slot*k_ss +
+ * head*k_sh + e, so both orders of slots and heads are strided views; bf16. A page may stand in several tables. A page id
+ * outside [0, pages) is a page that is not there: nothing is written to it and its keys are seen by no row. A sequence's
+ * pages hold at most 2^30 tokens.
+ * ---------------------------------------------------------------------------------------------------------- */
+typedef struct npub200_paged_cache {
+  void* k;
+  int64_t k_sp, k_ss, k_sh;
+  void* v;
+  int64_t v_sp, v_ss, v_sh;
+  int64_t pages, page_size, kv_heads, head_dim;
+  const int32_t* table; /* device memory */
+  int64_t table_stride, table_width;
+} npub200_paged_cache;
+
+/* Appends the keys and values of new tokens to the cache: token (b, s) goes to position starts[b] + s when s < counts[b]
+ * (counts NULL: all) and that position lies within the table (0 ... table_width * page_size - 1); other tokens write
+ * nothing. With a rotation the keys turn by their positions first (as npub200_rope), and so do the queries in the same
+ * launch: q_out [batch, seq, heads, head_dim] bf16, every row, whatever counts says (heads 0: no queries; q_out may be q
+ * itself). q, k and v are of one type, bf16 or f32, strided as in npub200_attention; k and v hold the cache's heads. No two
+ * tokens of a call may have the same slot (which of them stays is then undefined). Allocates nothing. */
+int npub200_paged_append(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, void* q_out, int64_t o_sb, int64_t o_ss,
+                         int64_t o_sh, int64_t heads, const void* k, int64_t k_sb, int64_t k_ss, int64_t k_sh,
+                         const void* v, int64_t v_sb, int64_t v_ss, int64_t v_sh, int dtype,
+                         const npub200_paged_cache* cache, const int32_t* starts, const int32_t* counts, int64_t batch,
+                         int64_t seq, const npub200_rotation* rotation, void* stream);
+
+/* Attention of a few new tokens of each sequence over its pages: npub200_attention_masked with key j of sequence b read from
+ * position j of its table. Row i of sequence b stands at p_i = q_starts[b] + i (NULL: kv_lens[b] - sq + i) and sees the
+ * keys j < kv_lens[b], with causal those of them with j <= p_i, on pages that are there; scores are scale q_i . k_j, then
+ * softcap tanh(s / softcap) when softcap > 0, then - slopes[h] |p_i - j| when given. A row that sees no key is zeros, one that
+ * sees a NaN score is NaN. kv_lens are clamped to 0 ... table_width * page_size; keys behind them are not read. V has to be
+ * finite at every key that some row sees. q: bf16, strides in multiples of 8 elements and a 16-byte aligned base, as the
+ * pages'; out: bf16 or f32, any strides. Head dims in multiples of 8 up to 256; any sq (made for few: a prompt's attention
+ * belongs to npub200_attention_masked). The keys of the whole batch are split evenly over the GPU on the device, from
+ * kv_lens: nothing but the sizes given here decides the launch, so a captured graph follows growing lengths. Partial results
+ * go to `workspace` (npub200_attention_paged_workspace_size() bytes, 16-byte aligned, contents irrelevant) and a second
+ * kernel joins them in a fixed order: deterministic. Calls that can run at the same time must not share a workspace.
+ * variant: 0, or the least number of 16-key tiles of one split (1 ... 2^20). Allocates nothing. */
+int npub200_attention_paged_workspace_size(int64_t heads, int64_t kv_heads, int64_t sq, int64_t head_dim,
+                                           size_t* bytes_out);
+int npub200_attention_paged(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, const npub200_paged_cache* cache,
+                            const int32_t* kv_lens, void* out, int64_t o_sb, int64_t o_ss, int64_t o_sh, int out_dtype,
+                            int64_t batch, int64_t heads, int64_t sq, float scale, int causal, const int32_t* q_starts,
+                            float softcap, const float* slopes, void* workspace, size_t workspace_bytes, int variant,
+                            void* stream);
+
+/* ----------------------------------------------------------------------------------------------------------
  * Device status word (failure detection; the reference's RuntimeError from NpuProgram.wait,
  * npu/xdna1_program.py:475-479). Synchronises `stream`, returns the OR of the status bits kernels on the current
  * device reported since the last clear (0 = healthy), and clears them when `clear` is non-zero.

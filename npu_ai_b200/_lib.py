@@ -32,6 +32,19 @@ class AttentionMods(ctypes.Structure):
                 ("mask_sq", _c_i64)]
 
 
+class Rotation(ctypes.Structure):
+    """npub200_rotation (include/npu_b200.h)."""
+    _fields_ = [("freqs", _c_p), ("rot_dim", _c_i64), ("interleaved", ctypes.c_int32), ("inverse", ctypes.c_int32),
+                ("magnitude", ctypes.c_float)]
+
+
+class PagedCache(ctypes.Structure):
+    """npub200_paged_cache (include/npu_b200.h)."""
+    _fields_ = [("k", _c_p), ("k_sp", _c_i64), ("k_ss", _c_i64), ("k_sh", _c_i64), ("v", _c_p), ("v_sp", _c_i64),
+                ("v_ss", _c_i64), ("v_sh", _c_i64), ("pages", _c_i64), ("page_size", _c_i64), ("kv_heads", _c_i64),
+                ("head_dim", _c_i64), ("table", _c_p), ("table_stride", _c_i64), ("table_width", _c_i64)]
+
+
 _SIGNATURES = {
     "npub200_version": (ctypes.c_int, []),
     "npub200_last_error": (ctypes.c_char_p, []),
@@ -79,6 +92,19 @@ _SIGNATURES = {
                                                 _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_float,
                                                 ctypes.POINTER(AttentionMods), _c_p, ctypes.c_size_t, ctypes.c_int,
                                                 _c_p]),
+    "npub200_rope": (ctypes.c_int, [_c_p, _c_i64, _c_i64, _c_i64, ctypes.c_int, _c_p, _c_i64, _c_i64, _c_i64, ctypes.c_int,
+                                    _c_i64, _c_i64, _c_i64, _c_i64, ctypes.POINTER(Rotation), _c_i64, _c_p, _c_p, _c_i64,
+                                    _c_i64, _c_p]),
+    "npub200_paged_append": (ctypes.c_int, [_c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_i64,
+                                            _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_i64, ctypes.c_int,
+                                            ctypes.POINTER(PagedCache), _c_p, _c_p, _c_i64, _c_i64,
+                                            ctypes.POINTER(Rotation), _c_p]),
+    "npub200_attention_paged_workspace_size": (ctypes.c_int, [_c_i64, _c_i64, _c_i64, _c_i64,
+                                                              ctypes.POINTER(ctypes.c_size_t)]),
+    "npub200_attention_paged": (ctypes.c_int, [_c_p, _c_i64, _c_i64, _c_i64, ctypes.POINTER(PagedCache), _c_p, _c_p, _c_i64,
+                                               _c_i64, _c_i64, ctypes.c_int, _c_i64, _c_i64, _c_i64, ctypes.c_float,
+                                               ctypes.c_int, _c_p, ctypes.c_float, _c_p, _c_p, ctypes.c_size_t, ctypes.c_int,
+                                               _c_p]),
     "npub200_status_read": (ctypes.c_int, [_c_p, ctypes.POINTER(ctypes.c_uint32), ctypes.c_int]),
     "npub200_set_wait_timeout_ns": (ctypes.c_int, [ctypes.c_uint64]),
     "npub200_set_debug_flags": (ctypes.c_int, [ctypes.c_uint32]),
@@ -118,7 +144,7 @@ _ops = None
 
 
 def torch_ops():
-    """torch.ops.npub200: the GEMM and the fused attention as torch operators (libnpub200_torch.so, a thin
+    """torch.ops.npub200: the GEMM, the attentions and the paged cache as torch operators (libnpub200_torch.so, a thin
     TORCH_LIBRARY layer over this same C ABI, running on torch's current CUDA stream), or None when that library
     is not built. Loads libnpub200.so first, so both bindings share one instance of the kernel library."""
     global _ops

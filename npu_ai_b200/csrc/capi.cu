@@ -517,6 +517,42 @@ int npub200_attention_masked(const void* q, int64_t q_sb, int64_t q_ss, int64_t 
   return attention_masked_launch(p, static_cast<cudaStream_t>(stream));
 }
 
+int npub200_rope(const void* x, int64_t x_sb, int64_t x_ss, int64_t x_sh, int x_dtype, void* out, int64_t o_sb,
+                 int64_t o_ss, int64_t o_sh, int out_dtype, int64_t batch, int64_t seq, int64_t heads, int64_t head_dim,
+                 const npub200_rotation* rotation, int64_t start, const int32_t* starts, const int32_t* positions,
+                 int64_t pos_sb, int64_t pos_ss, void* stream) {
+  const RopeProblem p = {x,    x_sb, x_ss,  x_sh,     x_dtype,  out,   o_sb,   o_ss,      o_sh,   out_dtype, batch,
+                         seq,  heads, head_dim, rotation, start, starts, positions, pos_sb, pos_ss};
+  return rope_launch(p, static_cast<cudaStream_t>(stream));
+}
+
+int npub200_paged_append(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, void* q_out, int64_t o_sb, int64_t o_ss,
+                         int64_t o_sh, int64_t heads, const void* k, int64_t k_sb, int64_t k_ss, int64_t k_sh,
+                         const void* v, int64_t v_sb, int64_t v_ss, int64_t v_sh, int dtype,
+                         const npub200_paged_cache* cache, const int32_t* starts, const int32_t* counts, int64_t batch,
+                         int64_t seq, const npub200_rotation* rotation, void* stream) {
+  const PagedAppendProblem p = {q,    q_sb, q_ss, q_sh, q_out, o_sb,  o_ss,  o_sh,   heads,  k,     k_sb, k_ss,
+                                k_sh, v,    v_sb, v_ss, v_sh,  dtype, cache, starts, counts, batch, seq,  rotation};
+  return paged_append_launch(p, static_cast<cudaStream_t>(stream));
+}
+
+int npub200_attention_paged_workspace_size(int64_t heads, int64_t kv_heads, int64_t sq, int64_t head_dim,
+                                           size_t* bytes_out) {
+  if (bytes_out == nullptr) return fail(kErrInvalid, "null output pointer");
+  return attention_paged_workspace(heads, kv_heads, sq, head_dim, bytes_out);
+}
+
+int npub200_attention_paged(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, const npub200_paged_cache* cache,
+                            const int32_t* kv_lens, void* out, int64_t o_sb, int64_t o_ss, int64_t o_sh, int out_dtype,
+                            int64_t batch, int64_t heads, int64_t sq, float scale, int causal, const int32_t* q_starts,
+                            float softcap, const float* slopes, void* workspace, size_t workspace_bytes, int variant,
+                            void* stream) {
+  const AttnPagedProblem p = {q,     q_sb,   q_ss,     q_sh,    cache,  kv_lens,   out,             o_sb,
+                              o_ss,  o_sh,   out_dtype, batch,  heads,  sq,        scale,           causal,
+                              q_starts, softcap, slopes, workspace, workspace_bytes, variant, g_debug_flags.load()};
+  return attention_paged_launch(p, static_cast<cudaStream_t>(stream));
+}
+
 int npub200_status_read(void* stream, uint32_t* bits_out, int clear) {
   const DeviceInfo* d = nullptr;
   if (int rc = current_device_info(&d)) return rc;

@@ -183,4 +183,63 @@ int attention_masked_launch(const AttnMaskedProblem& p, cudaStream_t stream);
 int attention_masked_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t sq, int64_t skv,
                                int64_t head_dim, int variant, size_t* bytes);
 
+// ---- rotary positions and the paged cache --------------------------------------------------------------------------
+struct RopeProblem {
+  const void* x;  // element (b, s, h, e) at b*sb + s*ss + h*sh + e
+  int64_t x_sb, x_ss, x_sh;
+  int in_dtype;
+  void* out;
+  int64_t o_sb, o_ss, o_sh;
+  int out_dtype;
+  int64_t batch, seq, heads, head_dim;
+  const npub200_rotation* rotation;
+  int64_t start;             // position of token 0 where neither of these is given
+  const int32_t* starts;     // [batch]
+  const int32_t* positions;  // (b, s) at b*pos_sb + s*pos_ss
+  int64_t pos_sb, pos_ss;
+};
+int rope_launch(const RopeProblem& p, cudaStream_t stream);
+
+struct PagedAppendProblem {
+  const void* q;  // heads == 0: none
+  int64_t q_sb, q_ss, q_sh;
+  void* q_out;
+  int64_t o_sb, o_ss, o_sh;
+  int64_t heads;
+  const void* k;
+  int64_t k_sb, k_ss, k_sh;
+  const void* v;
+  int64_t v_sb, v_ss, v_sh;
+  int in_dtype;
+  const npub200_paged_cache* cache;
+  const int32_t* starts;
+  const int32_t* counts;
+  int64_t batch, seq;
+  const npub200_rotation* rotation;
+};
+int check_paged_cache(const npub200_paged_cache* cache, int64_t batch, const char* what);
+int paged_append_launch(const PagedAppendProblem& p, cudaStream_t stream);
+
+struct AttnPagedProblem {
+  const void* q;
+  int64_t q_sb, q_ss, q_sh;
+  const npub200_paged_cache* cache;
+  const int32_t* kv_lens;
+  void* out;
+  int64_t o_sb, o_ss, o_sh;
+  int out_dtype;
+  int64_t batch, heads, sq;
+  float scale;
+  int causal;
+  const int32_t* q_starts;
+  float softcap;
+  const float* slopes;
+  void* workspace;
+  size_t workspace_bytes;
+  int variant;
+  uint32_t debug;
+};
+int attention_paged_launch(const AttnPagedProblem& p, cudaStream_t stream);
+int attention_paged_workspace(int64_t heads, int64_t kv_heads, int64_t sq, int64_t head_dim, size_t* bytes);
+
 }  // namespace npub200

@@ -1,5 +1,5 @@
-// torch_ops.cpp - the GEMM, the fused and the masked attention as torch operators (torch.ops.npub200.gemm / .attention /
-// .attention_masked).
+// torch_ops.cpp - the GEMM, the fused and the masked attention, rotary positions and the paged cache as torch operators
+// (torch.ops.npub200.gemm / .attention / .attention_masked / .rope / .paged_append / .attention_paged).
 //
 // The reference hands each request to its NPU as one XRT command: NpuProgram.submit_gemm / submit_attn
 // (npu/xdna1_program.py:441-473) with three buffer objects and 13 int32 parameters. Here the same requests are
@@ -9,6 +9,7 @@
 // computed here and there is no CPU kernel (CPU tensors are refused by the dispatcher). Errors raise like the
 // reference's runner: an invalid request is a ValueError, anything else a RuntimeError.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
@@ -16,6 +17,7 @@
 #include <cmath>
 #include <optional>
 #include <type_traits>
+#include <vector>
 
 #include "npu_b200.h"
 
@@ -307,6 +309,220 @@ at::Tensor attention_masked(const at::Tensor& q, const at::Tensor& k, const at::
   return out;
 }
 
+// (batch, seq, head) element strides of a tensor of heads, and the checks of its shape: (B, S, heads * d), or (B, heads, S, d)
+// when head-major. A dimension of one element has no stride of its own.
+struct HeadRows {
+  int64_t sb, ss, sh;
+};
+HeadRows head_rows(const at::Tensor& t, const at::Tensor& ref, bool head_major, int64_t heads, int64_t d, const char* name) {
+  TORCH_CHECK_VALUE(t.is_cuda() && t.device() == ref.device(), name, " must be a CUDA tensor on ", ref.device());
+  const bool ok = head_major ? t.dim() == 4 && t.size(1) == heads && t.size(3) == d
+                             : t.dim() == 3 && t.size(2) == heads * d;
+  TORCH_CHECK_VALUE(ok && heads > 0, name, " must be ", head_major ? "(B, heads, S, d)" : "(B, S, heads*d)", " with ", heads,
+                    " heads of ", d, ", got ", t.sizes());
+  TORCH_CHECK_VALUE(t.size(-1) <= 1 || t.stride(-1) == 1, name, " must have a contiguous last dimension");
+  const auto stride = [&](int64_t dim) { return t.size(dim) > 1 ? t.stride(dim) : int64_t(0); };
+  return head_major ? HeadRows{stride(0), stride(2), stride(1)} : HeadRows{stride(0), stride(1), d};
+}
+
+// Positions of the tokens: none (a plain start), int32 [B] (of each sequence's first token) or int32 [B, S].
+struct Positions {
+  const int32_t* starts = nullptr;
+  const int32_t* each = nullptr;
+  int64_t sb = 0, ss = 0;
+};
+Positions positions_of(const std::optional<at::Tensor>& t, const at::Tensor& x, int64_t B, int64_t S) {
+  Positions p;
+  if (!t.has_value()) return p;
+  TORCH_CHECK_VALUE(t->is_cuda() && t->device() == x.device() && t->scalar_type() == at::kInt &&
+                        ((t->dim() == 1 && t->size(0) == B && (B <= 1 || t->stride(0) == 1)) ||
+                         (t->dim() == 2 && t->size(0) == B && t->size(1) == S)),
+                    "positions must be int32, contiguous [", B, "] or [", B, ", ", S, "], on ", x.device(), ", got ",
+                    t->scalar_type(), " ", t->sizes(), " on ", t->device());
+  const int32_t* ptr = static_cast<const int32_t*>(t->data_ptr());
+  if (t->dim() == 1) {
+    p.starts = ptr;
+  } else {
+    p.each = ptr;
+    p.sb = t->stride(0);
+    p.ss = t->stride(1);
+  }
+  return p;
+}
+
+npub200_rotation rotation_of(const at::Tensor& freqs, const at::Tensor& x, bool interleaved, bool inverse, double magnitude) {
+  TORCH_CHECK_VALUE(freqs.is_cuda() && freqs.device() == x.device() && freqs.scalar_type() == at::kDouble &&
+                        freqs.dim() == 1 && freqs.is_contiguous(),
+                    "freqs must be a contiguous float64 vector (radians a position of each pair) on ", x.device(), ", got ",
+                    freqs.scalar_type(), " ", freqs.sizes(), " on ", freqs.device());
+  npub200_rotation r = {};
+  r.freqs = static_cast<const double*>(freqs.data_ptr());
+  r.rot_dim = 2 * freqs.numel();
+  r.interleaved = interleaved ? 1 : 0;
+  r.inverse = inverse ? 1 : 0;
+  r.magnitude = float(magnitude);
+  return r;
+}
+
+// A tensor that a kernel writes: no element twice, and `from` itself or nothing of it.
+void check_written(const at::Tensor& t, const char* name, const at::Tensor* from = nullptr) {
+  TORCH_CHECK_VALUE(at::has_internal_overlap(t) != at::MemOverlap::Yes, name, " must not hold an element twice");
+  TORCH_CHECK_VALUE(from == nullptr || at::get_overlap_status(t, *from) != at::MemOverlapStatus::Partial, name,
+                    " must be the input itself or share no element with it");
+}
+
+// Rotary positions (npub200_rope): x (B, S, heads * d), or (B, heads, S, d) when head-major, like the result.
+at::Tensor rope(const at::Tensor& x, const at::Tensor& freqs, int64_t heads, const std::optional<at::Tensor>& out_arg,
+                std::optional<at::ScalarType> out_dtype, int64_t start, const std::optional<at::Tensor>& positions,
+                bool interleaved, double magnitude, bool inverse, bool head_major) {
+  TORCH_CHECK_VALUE(heads > 0 && x.dim() == (head_major ? 4 : 3) && (head_major || x.size(2) % heads == 0),
+                    "x must be ", head_major ? "(B, heads, S, d)" : "(B, S, heads*d)", " with heads=", heads, ", got ",
+                    x.sizes());
+  const int64_t d = head_major ? x.size(3) : x.size(2) / heads;
+  const int64_t B = x.size(0), S = x.size(head_major ? 2 : 1);
+  const HeadRows xr = head_rows(x, x, head_major, heads, d, "x");
+  const int x_code = dtype_code(x, "x");
+  const npub200_rotation r = rotation_of(freqs, x, interleaved, inverse, magnitude);
+  const Positions p = positions_of(positions, x, B, S);
+  const c10::cuda::CUDAGuard guard(x.device());
+  at::Tensor out;
+  if (out_arg.has_value()) {
+    out = *out_arg;
+    TORCH_CHECK_VALUE(out.sizes() == x.sizes(), "out must have x's shape ", x.sizes(), ", got ", out.sizes());
+    check_written(out, "out", &x);
+  } else {
+    out = at::empty(x.sizes(), x.options().dtype(out_dtype.value_or(x.scalar_type())));
+  }
+  const HeadRows orr = head_rows(out, x, head_major, heads, d, "out");
+  check_rc(npub200_rope(x.data_ptr(), xr.sb, xr.ss, xr.sh, x_code, out.data_ptr(), orr.sb, orr.ss, orr.sh,
+                        dtype_code(out, "out"), B, S, heads, d, &r, start, p.starts, p.each, p.sb, p.ss, stream_of(x)),
+           "npub200::rope");
+  return out;
+}
+
+// The pages of a cache: [pages, page_size, kv_heads, d] bf16 views of any strides, and each sequence's table of them.
+npub200_paged_cache cache_of(const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table, int64_t B) {
+  TORCH_CHECK_VALUE(k_pages.is_cuda() && k_pages.dim() == 4 && k_pages.scalar_type() == at::kBFloat16 &&
+                        v_pages.device() == k_pages.device() && v_pages.scalar_type() == at::kBFloat16 &&
+                        v_pages.sizes() == k_pages.sizes(),
+                    "k_pages and v_pages must be bf16 CUDA tensors [pages, page_size, kv_heads, d] of one shape, got ",
+                    k_pages.scalar_type(), " ", k_pages.sizes(), " and ", v_pages.scalar_type(), " ", v_pages.sizes());
+  TORCH_CHECK_VALUE(k_pages.size(3) <= 1 || (k_pages.stride(3) == 1 && v_pages.stride(3) == 1),
+                    "k_pages and v_pages must have a contiguous last dimension");
+  TORCH_CHECK_VALUE(table.is_cuda() && table.device() == k_pages.device() && table.scalar_type() == at::kInt &&
+                        table.dim() == 2 && table.size(0) == B && (table.size(1) <= 1 || table.stride(1) == 1),
+                    "page_table must be int32 [", B, ", pages] with contiguous rows on ", k_pages.device(), ", got ",
+                    table.scalar_type(), " ", table.sizes(), " on ", table.device());
+  const auto stride = [](const at::Tensor& t, int64_t dim) { return t.size(dim) > 1 ? t.stride(dim) : int64_t(0); };
+  npub200_paged_cache c = {};
+  c.k = k_pages.data_ptr();
+  c.k_sp = stride(k_pages, 0), c.k_ss = stride(k_pages, 1), c.k_sh = stride(k_pages, 2);
+  c.v = v_pages.data_ptr();
+  c.v_sp = stride(v_pages, 0), c.v_ss = stride(v_pages, 1), c.v_sh = stride(v_pages, 2);
+  c.pages = k_pages.size(0);
+  c.page_size = k_pages.size(1);
+  c.kv_heads = k_pages.size(2);
+  c.head_dim = k_pages.size(3);
+  c.table = static_cast<const int32_t*>(table.data_ptr());
+  c.table_stride = stride(table, 0);
+  c.table_width = table.size(1);
+  return c;
+}
+
+// Appends new keys and values to the pages, keys and queries rotated on the way (npub200_paged_append). Returns the rotated
+// queries, or nothing without them.
+std::optional<at::Tensor> paged_append(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_pages,
+                                       const at::Tensor& v_pages, const at::Tensor& page_table, const at::Tensor& starts,
+                                       const std::optional<at::Tensor>& counts, const std::optional<at::Tensor>& q,
+                                       int64_t heads, const std::optional<at::Tensor>& q_out,
+                                       const std::optional<at::Tensor>& freqs, bool interleaved, double magnitude,
+                                       bool head_major) {
+  TORCH_CHECK_VALUE(k.dim() == (head_major ? 4 : 3), "k must be ", head_major ? "(B, heads, S, d)" : "(B, S, heads*d)",
+                    ", got ", k.sizes());
+  const int64_t B = k.size(0), S = k.size(head_major ? 2 : 1);
+  const npub200_paged_cache c = cache_of(k_pages, v_pages, page_table, B);
+  const HeadRows kr = head_rows(k, k_pages, head_major, c.kv_heads, c.head_dim, "k");
+  const HeadRows vr = head_rows(v, k_pages, head_major, c.kv_heads, c.head_dim, "v");
+  const int code = dtype_code(k, "k");
+  TORCH_CHECK_VALUE(v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type(), "v must have k's shape and type, got ",
+                    v.scalar_type(), " ", v.sizes());
+  check_written(k_pages, "k_pages");
+  check_written(v_pages, "v_pages");
+  const int32_t* starts_ptr = vector_ptr<int32_t>(starts, k_pages, B, "starts");
+  const int32_t* counts_ptr = vector_ptr<int32_t>(counts, k_pages, B, "counts");
+  npub200_rotation r = {};
+  if (freqs.has_value()) r = rotation_of(*freqs, k_pages, interleaved, false, magnitude);
+  const c10::cuda::CUDAGuard guard(k_pages.device());
+  std::optional<at::Tensor> out;
+  HeadRows qr = {}, orr = {};
+  if (q.has_value()) {
+    TORCH_CHECK_VALUE(freqs.has_value(), "q is taken to be rotated: it needs freqs");
+    qr = head_rows(*q, k_pages, head_major, heads, c.head_dim, "q");
+    TORCH_CHECK_VALUE(q->size(0) == B && q->size(head_major ? 2 : 1) == S && q->scalar_type() == k.scalar_type(),
+                      "q must have k's batch, tokens and type, got ", q->scalar_type(), " ", q->sizes());
+    if (q_out.has_value()) {
+      TORCH_CHECK_VALUE(q_out->sizes() == q->sizes() && q_out->scalar_type() == at::kBFloat16,
+                        "q_out must be bf16 with q's shape ", q->sizes(), ", got ", q_out->scalar_type(), " ", q_out->sizes());
+      check_written(*q_out, "q_out", &*q);
+      out = *q_out;
+    } else {
+      out = at::empty(q->sizes(), k_pages.options());
+    }
+    orr = head_rows(*out, k_pages, head_major, heads, c.head_dim, "q_out");
+  } else {
+    TORCH_CHECK_VALUE(!q_out.has_value(), "q_out is given without q");
+  }
+  check_rc(npub200_paged_append(q.has_value() ? q->data_ptr() : nullptr, qr.sb, qr.ss, qr.sh,
+                                q.has_value() ? out->data_ptr() : nullptr, orr.sb, orr.ss, orr.sh, q.has_value() ? heads : 0,
+                                k.data_ptr(), kr.sb, kr.ss, kr.sh, v.data_ptr(), vr.sb, vr.ss, vr.sh, code, &c, starts_ptr,
+                                counts_ptr, B, S, freqs.has_value() ? &r : nullptr, stream_of(k_pages)),
+           "npub200::paged_append");
+  return out;
+}
+
+// Attention over a cache in pages (npub200_attention_paged). Defaults: scale 0 d^-0.5, softcap 0 none. The workspace comes
+// from torch's allocator, one per call.
+at::Tensor attention_paged(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages,
+                           const at::Tensor& page_table, const at::Tensor& kv_lens, const std::optional<at::Tensor>& out_arg,
+                           std::optional<at::ScalarType> out_dtype, int64_t heads, double scale, bool causal,
+                           const std::optional<at::Tensor>& q_starts, double softcap,
+                           const std::optional<at::Tensor>& slopes, bool head_major_in, bool head_major_out,
+                           int64_t variant) {
+  TORCH_CHECK_VALUE(q.scalar_type() == at::kBFloat16 && q.dim() == (head_major_in ? 4 : 3), "q must be bf16 ",
+                    head_major_in ? "(B, heads, S, d)" : "(B, S, heads*d)", ", got ", q.scalar_type(), " ", q.sizes());
+  const int64_t B = q.size(0), S = q.size(head_major_in ? 2 : 1);
+  const npub200_paged_cache c = cache_of(k_pages, v_pages, page_table, B);
+  const int64_t d = c.head_dim;
+  const HeadRows qr = head_rows(q, k_pages, head_major_in, heads, d, "q");
+  TORCH_CHECK_VALUE(scale >= 0, "attention scale must be positive (got ", scale, ")");
+  if (scale == 0) scale = 1.0 / std::sqrt(double(d));
+  const c10::cuda::CUDAGuard guard(k_pages.device());
+  at::Tensor out;
+  const auto shape = head_major_out ? std::vector<int64_t>{B, heads, S, d} : std::vector<int64_t>{B, S, heads * d};
+  if (out_arg.has_value()) {
+    out = *out_arg;
+    TORCH_CHECK_VALUE(out.sizes() == at::IntArrayRef(shape), "attention output must be ", at::IntArrayRef(shape), ", got ",
+                      out.sizes());
+    check_written(out, "out");
+  } else {
+    out = at::empty(shape, q.options().dtype(out_dtype.value_or(at::kFloat)));
+  }
+  const HeadRows orr = head_rows(out, k_pages, head_major_out, heads, d, "attention output");
+  const int out_code = dtype_code(out, "attention output");
+  const int32_t* lens = vector_ptr<int32_t>(kv_lens, k_pages, B, "kv_lens");
+  const int32_t* starts = vector_ptr<int32_t>(q_starts, k_pages, B, "q_start");
+  const float* slopes_ptr = vector_ptr<float>(slopes, k_pages, heads, "slopes");
+  if (B == 0 || S == 0) return out;
+  size_t ws_bytes = 0;
+  check_rc(npub200_attention_paged_workspace_size(heads, c.kv_heads, S, d, &ws_bytes), "npub200::attention_paged");
+  const at::Tensor ws = at::empty({int64_t(ws_bytes)}, q.options().dtype(at::kByte));
+  check_rc(npub200_attention_paged(q.data_ptr(), qr.sb, qr.ss, qr.sh, &c, lens, out.data_ptr(), orr.sb, orr.ss, orr.sh,
+                                   out_code, B, heads, S, float(scale), causal ? 1 : 0, starts, float(softcap), slopes_ptr,
+                                   ws.data_ptr(), ws_bytes, int(variant), stream_of(k_pages)),
+           "npub200::attention_paged");
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(npub200, m) {
@@ -320,10 +536,22 @@ TORCH_LIBRARY(npub200, m) {
         "int? q_start=None, Tensor? q_starts=None, int prefix=0, Tensor? prefixes=None, Tensor? kv_lens=None, "
         "Tensor? doc_offsets=None, float softcap=0., Tensor? slopes=None, Tensor? distance_bias=None, "
         "Tensor? mask=None) -> Tensor");
+  m.def("rope(Tensor x, Tensor freqs, int heads, Tensor? out=None, ScalarType? out_dtype=None, int start=0, "
+        "Tensor? positions=None, bool interleaved=False, float magnitude=1., bool inverse=False, "
+        "bool head_major=False) -> Tensor");
+  m.def("paged_append(Tensor k, Tensor v, Tensor k_pages, Tensor v_pages, Tensor page_table, Tensor starts, "
+        "Tensor? counts=None, Tensor? q=None, int heads=0, Tensor? q_out=None, Tensor? freqs=None, "
+        "bool interleaved=False, float magnitude=1., bool head_major=False) -> Tensor?");
+  m.def("attention_paged(Tensor q, Tensor k_pages, Tensor v_pages, Tensor page_table, Tensor kv_lens, Tensor? out, "
+        "ScalarType? out_dtype, int heads, float scale=0., bool causal=True, Tensor? q_starts=None, float softcap=0., "
+        "Tensor? slopes=None, bool head_major_in=False, bool head_major_out=False, int variant=0) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(npub200, CUDA, m) {
   m.impl("gemm", &gemm);
   m.impl("attention", &attention);
   m.impl("attention_masked", &attention_masked);
+  m.impl("rope", &rope);
+  m.impl("paged_append", &paged_append);
+  m.impl("attention_paged", &attention_paged);
 }

@@ -3,11 +3,12 @@
 torch provides device memory and the current stream; the arithmetic runs in the sm_100a kernels of the
 library. The GEMM and the attention go through the library's torch operators (torch.ops.npub200.gemm / .attention /
 .attention_masked, libnpub200_torch.so) when that layer is built, else straight through ctypes; both reach the same
-C ABI and kernels. Nothing here computes on the CPU, and there is no fallback when a kernel refuses a request.
+C ABI and kernels. Rotary positions and the paged cache need that layer. Nothing here computes on the CPU, and there is no fallback when a kernel refuses a request.
 """
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 
@@ -594,6 +595,129 @@ def _attention_masked(q, k, v, heads, scale, head_major_in, head_major_out, out_
                   ctypes.c_void_p(ws.data_ptr()) if ws is not None else None, nbytes.value, int(variant),
                   ctypes.c_void_p(_stream_ptr(dev)))
     return out
+
+
+def _operators():
+    """torch.ops.npub200, for the calls that have no other route."""
+    ops = _lib.torch_ops()
+    if ops is None:
+        raise _lib.KernelLibraryMissing(
+            f"{_lib.TORCH_OPS_PATH} is missing: build it with `python -m npu_ai_b200.build` (there is no CPU fallback)")
+    return ops
+
+
+def rope_frequencies(rot_dim: int, base: float = 10000.0, scaling: str | None = None, factor: float = 1.0,
+                     original_length: int = 4096, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                     device: torch.device | str | None = None) -> tuple[torch.Tensor, float]:
+    """(freqs, magnitude) of `rope` and `paged_append`: float64 [rot_dim / 2] radians a position, base^(-2j / rot_dim), and
+    the factor of the rotated values.
+
+    scaling for contexts `factor` times longer than the model was trained on:
+      None      none.
+      "linear"  positions divided by the factor.
+      "ntk"     the base times factor^(rot_dim / (rot_dim - 2)): the last pair slows down by the factor, the first not.
+      "yarn"    pairs that turn more than beta_fast times over original_length keep their frequency, those that turn less
+                than beta_slow times have it divided by the factor, a linear ramp over the logarithm of their turns between;
+                magnitude 0.1 ln(factor) + 1 (for factors above 1).
+    """
+    if rot_dim <= 0 or rot_dim % 2:
+        raise ValueError(f"rot_dim must be positive and even (got {rot_dim})")
+    if not base > 1.0 or not factor >= 1.0 or original_length <= 0 or not beta_fast > beta_slow > 0.0:
+        raise ValueError("rope_frequencies needs base > 1, factor >= 1, original_length > 0 and beta_fast > beta_slow > 0")
+    j = torch.arange(0, rot_dim, 2, dtype=torch.float64)
+    magnitude = 1.0
+    if scaling == "ntk":
+        if rot_dim == 2:
+            raise ValueError("ntk scaling needs more than one pair")
+        base = base * factor ** (rot_dim / (rot_dim - 2))
+    f = torch.tensor(float(base), dtype=torch.float64) ** (-j / rot_dim)
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "yarn":
+        turns = original_length * f / (2.0 * math.pi)
+        keep = ((turns / beta_slow).log() / math.log(beta_fast / beta_slow)).clamp(0.0, 1.0)
+        f = f * keep + f / factor * (1.0 - keep)
+        magnitude = 0.1 * math.log(factor) + 1.0
+    elif scaling not in (None, "ntk"):
+        raise ValueError(f"unknown scaling {scaling!r} (None, 'linear', 'ntk' or 'yarn')")
+    return f.to(device) if device is not None else f, magnitude
+
+
+def rope(x: torch.Tensor, freqs: torch.Tensor, heads: int, positions: int | torch.Tensor = 0, *, interleaved: bool = False,
+         magnitude: float = 1.0, inverse: bool = False, head_major: bool = False, out: torch.Tensor | None = None,
+         out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """Rotary positions: pair j of each head's first 2 * len(freqs) values turned by position * freqs[j], the rest copied.
+
+    x: bf16 or f32 (B, S, heads*D), or (B, heads, S, D) when head_major, any strides with a contiguous last dimension, so the
+    query and key heads of a fused projection are one call. Returns a tensor of the same layout, of x's type unless
+    `out_dtype` (or `out`, which may be x itself) says otherwise.
+    freqs:       float64 [r / 2] on the device (rope_frequencies), radians a position; D even, up to 1024.
+    positions:   of the tokens: an int (token s stands at positions + s), int32 [B] (at positions[b] + s) or int32 [B, S].
+                 Device tensors are read when the call runs, so a captured graph follows their contents.
+    interleaved: pairs (2j, 2j + 1) instead of (j, j + r / 2).
+    magnitude:   factor of the rotated values.
+    inverse:     turn by -position * freqs[j]: undoes the rotation (with magnitude 1 / m), and with the same magnitude takes
+                 the gradient of a rotation's output to that of its input.
+    Angles are worked out in 64 bits, the rotation in f32, with one rounding.
+    """
+    _require_cuda(x, "x")
+    at = positions if isinstance(positions, torch.Tensor) else None
+    return _operators().rope(x, freqs, heads, out, out_dtype, positions if at is None else 0, at, interleaved, magnitude,
+                             inverse, head_major)
+
+
+def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                 starts: torch.Tensor, *, counts: torch.Tensor | None = None, q: torch.Tensor | None = None,
+                 heads: int | None = None, q_out: torch.Tensor | None = None, freqs: torch.Tensor | None = None,
+                 interleaved: bool = False, magnitude: float = 1.0, head_major: bool = False) -> torch.Tensor | None:
+    """Appends new keys and values to a cache in pages, keys and queries rotated on the way, in one launch.
+
+    k, v:             bf16 or f32 (B, S, kv_heads*D), or (B, kv_heads, S, D) when head_major; any strides.
+    k_pages, v_pages: bf16 [pages, page_size, kv_heads, D], any strides (a pool with heads before slots is passed
+                      transposed). Position p of sequence b lies in slot p % page_size of page page_table[b, p // page_size].
+    page_table:       int32 [B, width]. A page id outside the pool is a page that is not there: nothing is written to it.
+    starts:           int32 [B]; token s goes to position starts[b] + s, if that lies within the table.
+    counts:           int32 [B], the tokens of each sequence that are appended (default: all); nothing is written for the
+                      others, the padding of a ragged batch.
+    freqs, interleaved, magnitude: as in rope; without freqs k is stored as it is.
+    q, heads:         queries of k's type and layout with `heads` heads, rotated by the same positions (every row); needs
+                      freqs. Returned in bf16, in `q_out` if given (which may be q itself).
+    Keys are rotated in f32 and rounded once. No two tokens may share a slot.
+    """
+    _require_cuda(k, "k")
+    if q is not None and heads is None:
+        raise ValueError("q needs heads")
+    return _operators().paged_append(k, v, k_pages, v_pages, page_table, starts, counts, q, heads or 0, q_out, freqs,
+                                     interleaved, magnitude, head_major)
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                    kv_lens: torch.Tensor, heads: int, scale: float | None = None, *, causal: bool = True,
+                    q_start: torch.Tensor | None = None, softcap: float | None = None, slopes: torch.Tensor | None = None,
+                    head_major_in: bool = False, head_major_out: bool = False, out_dtype: torch.dtype = torch.float32,
+                    out: torch.Tensor | None = None, variant: int = 0) -> torch.Tensor:
+    """softmax(q k^T * scale) v of a few new tokens of each sequence over its keys in the pages of a cache.
+
+    q:          bf16 (B, Sq, heads*D), or (B, heads, Sq, D) when head_major_in; strides in multiples of 8 elements. The output
+                (B, Sq, heads*D), or (B, heads, Sq, D) when head_major_out, f32 unless `out_dtype` or `out` says otherwise.
+    k_pages, v_pages, page_table: as in paged_append (strides in multiples of 8 elements); query head h reads head
+                h // (heads // kv_heads). Keys on a page that is not there are seen by no row.
+    kv_lens:    int32 [B], the valid keys of each sequence, its new tokens among them (clamped to the table). Device tensors
+                are read when the call runs, so a captured graph follows their contents.
+    q_start:    int32 [B], the position of query 0 (default kv_lens - Sq: the last query meets the last key).
+    causal:     query i sees the keys up to its position q_start + i; otherwise all of kv_lens.
+    softcap, slopes: as in attention. A row that may see no key is zero, one that sees a NaN score NaN; v has to be finite
+                at every key that some row sees.
+    The batch's keys are split evenly over the GPU whatever the lengths. Made for few tokens; the attention of a prompt is
+    `attention`, on its own keys. variant: the least number of 16-key tiles of one split (0 = automatic).
+    """
+    _require_cuda(q, "q")
+    if softcap is not None and not 1e-30 <= softcap <= 1e30:
+        raise ValueError(f"softcap must be positive, within [1e-30, 1e30] (got {softcap})")
+    if scale is not None and not scale > 0.0:
+        raise ValueError(f"attention scale must be positive (got {scale})")
+    return _operators().attention_paged(q, k_pages, v_pages, page_table, kv_lens, out, out_dtype, heads, scale or 0.0, causal,
+                                        q_start, softcap or 0.0, slopes, head_major_in, head_major_out, variant)
 
 
 def status(device: torch.device | int | None = None, clear: bool = True) -> int:

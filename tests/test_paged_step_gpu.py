@@ -1,0 +1,84 @@
+"""A decoder's cached steps as a user runs them: the fused q/k/v projection, the append with the rotation, the attention over
+the pages, the output projection. A ragged prompt and its continuation, token by token, eagerly and as a replayed graph, give
+what a contiguous cache gives with rope and kernels.attention on the same tensors, within the attention's tolerance."""
+import pytest
+import torch
+
+from test_attention_masked_gpu import BF16, check, oracle
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("heads,kv_heads,page,interleaved", [(8, 2, 16, False), (4, 4, 7, True), (8, 1, 64, False)])
+def test_prompt_and_continuation(cuda_device, heads, kv_heads, page, interleaved):
+    from npu_ai_b200 import kernels
+    dev, d, B, T, steps = cuda_device, 64, 3, 77, 6
+    C, most = heads * d, 77 + 6
+    g = torch.Generator(device=dev).manual_seed(heads)
+    w_qkv, w_out = ((torch.randn(n, C, generator=g, device=dev) * C ** -0.5).to(BF16) for n in ((heads + 2 * kv_heads) * d, C))
+    freqs, magnitude = kernels.rope_frequencies(d, scaling="yarn", factor=4.0, device=dev)
+    turn = dict(interleaved=interleaved, magnitude=magnitude)
+    width = -(-most // page)
+    k_pages, v_pages = (torch.full((B * width, page, kv_heads, d), float("nan"), dtype=BF16, device=dev) for _ in range(2))
+    table = torch.randperm(B * width, generator=g, device=dev).view(B, width).to(torch.int32)
+    flat = [torch.zeros(B, most, kv_heads * d, dtype=BF16, device=dev) for _ in range(2)]  # the same cache in one piece
+
+    def layer(x, starts, lens, counts=None):
+        n = x.shape[1]
+        y = kernels.gemm(x.view(-1, C), w_qkv, out_dtype=BF16).view(B, n, -1)
+        q, k, v = y.split((heads * d, kv_heads * d, kv_heads * d), -1)
+        q = kernels.paged_append(k, v, k_pages, v_pages, table, starts, counts=counts, q=q, heads=heads, freqs=freqs, **turn)
+        o = kernels.paged_attention(q, k_pages, v_pages, table, lens, heads, q_start=starts, out_dtype=BF16)
+        return y, q, o, kernels.gemm(o.view(-1, C), w_out, out_dtype=BF16, residual=x.reshape(-1, C)).view(B, n, C)
+
+    def verify(y, q, o, starts, lens):
+        n = y.shape[1]
+        nq, nk = heads * d, kv_heads * d
+        assert torch.equal(q, kernels.rope(y[..., :nq], freqs, heads, starts, **turn))
+        new = kernels.rope(y[..., nq:nq + nk], freqs, kv_heads, starts, **turn), y[..., nq + nk:]
+        for f, t in zip(flat, new):
+            for b in range(B):
+                s, e = int(starts[b]), int(lens[b])
+                f[b, s:e] = t[b, :e - s]
+        own = torch.arange(n, device=dev) < (lens - starts)[:, None]  # a sequence's own tokens, not its padding
+        ref, tol = oracle(q, *flat, heads, kv_heads, causal=True, q_start=starts, kv_lens=lens)
+        check(o, ref, tol, heads, False)
+        base = kernels.attention(q, *flat, heads, kv_heads=kv_heads, causal=True, q_start=starts, kv_lens=lens, out_dtype=BF16)
+        check(base, ref, tol, heads, False)
+        assert bool(torch.isfinite(o[own]).all())
+
+    lens = torch.tensor([77, 40, 1], dtype=torch.int32, device=dev)
+    zero = torch.zeros_like(lens)
+    x = torch.randn(B, T, C, generator=g, device=dev).to(BF16)
+    y, q, o, _ = layer(x, zero, lens, counts=lens)
+    kernels.check_status(dev)
+    verify(y, q, o, zero, lens)
+    pages = [t.clone() for t in (k_pages, v_pages)]
+    tokens = torch.randn(steps, B, 1, C, generator=g, device=dev).to(BF16)
+
+    starts = lens.clone()
+    eager = []
+    for tok in tokens:
+        y, q, o, out = layer(tok, starts, starts + 1)
+        verify(y, q, o, starts, starts + 1)
+        eager.append(out)
+        starts.add_(1)
+    kernels.check_status(dev)
+
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        tok = tokens[0].clone()
+        starts.copy_(lens)
+        layer(tok, starts, starts + 1)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = layer(tok, starts, starts + 1)[3]
+            starts.add_(1)
+        for t, p in zip((k_pages, v_pages), pages):
+            t.copy_(p)
+        starts.copy_(lens)
+        for t, want in zip(tokens, eager):
+            tok.copy_(t)
+            graph.replay()
+            assert torch.equal(out, want)
