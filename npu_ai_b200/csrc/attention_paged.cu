@@ -12,12 +12,15 @@
 //     rows take one warp, more share the keys of one load among 2 or 4 warps. Rows of 16 waste the matrix instruction's
 //     rows, not time: mma.sync m16n8k16 on registers keeps the whole softmax in one warp, without the round trips through
 //     TMEM and shared memory that a tcgen05 tile of 128 rows would add to each tile of keys.
-//   * Every worker takes an equal run of 16-key tiles of the whole batch, found on the device from kv_lens, so ragged
-//     lengths leave no worker idle and a captured graph follows them. A run starts and ends anywhere in a sequence; parts
-//     of a row's keys go to the workspace and the join kernel adds them up in order of keys.
-//   * A tile's 16 keys and 16 values are 32 rows anywhere in memory, one bulk copy a lane (`cp.async.bulk`, which takes any
-//     page size and layout), into a ring of 3 to 6 tiles a warp. Rows in shared memory are 16 bytes longer than the head,
-//     so that ldmatrix reads 8 of them without a bank conflict.
+//   * Every worker takes an equal run of tiles of 16 wr keys of the whole batch, found on the device from kv_lens, so
+//     ragged lengths leave no worker idle and a captured graph follows them. A run starts and ends anywhere in a sequence;
+//     parts of a row's keys go to the workspace and the join kernel adds them up in order of keys.
+//   * A tile's keys and values are rows anywhere in memory: cp.async of 16 bytes a lane takes any page size and layout,
+//     into a ring of 3 to 6 tiles. (A bulk copy a row, one instruction a lane, was the first form: the copy engine takes
+//     one in about 17 cycles, 16 bytes a cycle at 128 columns where 23 are the memory's rate.) Rows in shared memory are
+//     16 bytes longer than the head, so that ldmatrix reads 8 of them without a bank conflict.
+#include <algorithm>
+#include <atomic>
 #include <cfloat>
 #include <cmath>
 #include <cstring>
@@ -30,8 +33,8 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kWarps = 4;      // of a block
-constexpr int kTileKeys = 16;  // of a tile
-constexpr int kMaxStages = 6;  // of a warp's ring
+constexpr int kSub = 16;       // keys of one step of the matrix instructions; a tile is `wr` of them
+constexpr int kMaxStages = 6;  // of a ring
 constexpr int kJoinWarps = 8;
 // The row maximum moves only when a tile's beats it by this much (log2 units): P stays within 2^8 of 1, which bf16 holds
 // with the same relative rounding, and the O registers are rescaled once in a while instead of once a tile.
@@ -57,13 +60,15 @@ struct PagedArgs {
   float scale_log2;     // scores to log2 units
   float cap_in, cap_out;  // softcap: cap_out tanh(cap_in q.k), cap_out 0: none
   const float* slopes;
-  int wr, workers, stages;  // warps of a worker, workers of the grid, stages of a worker's ring
+  int workers;              // of the grid
   int rows, row_tiles, slot_rows;  // rows of a (sequence, kv head), tiles of 16 wr rows, rows of a part in the workspace
   int min_span;             // least tiles of a worker's run
-  int4* rec;                // [workers] the item whose first part the worker holds: sequence, kv head and row tile, parts
+  // What there is to join: of each item where there are no more items than workers, else of the item that begins in each
+  // worker's run and goes on behind it. (sequence, kv head and row tile, parts or 0, worker of the first)
+  int4* rec;
+  int rec_items;
   float2* part_ml;          // [2 workers][slot_rows] (m, l); part 0 of a worker continues an item, part 1 begins one
   float* part_o;            // [2 workers][slot_rows][D]
-  KernelCtl ctl;
 };
 
 __device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t (&r)[4]) {
@@ -85,22 +90,27 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// `bytes` (a multiple of 16) from global to shared memory, counted on the barrier; all addresses on 16-byte boundaries.
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
+// 16 bytes from global to shared memory, or zeros where `ok` is false.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {  // all but the last N groups of this thread are there
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Layout of a block's shared memory for head dims up to DP.
-template <int DP>
+// Layout of a block's shared memory for head dims up to DP and workers of WR warps.
+template <int DP, int WR>
 struct PagedLayout {
+  static constexpr int kTile = kSub * WR;                // keys of a tile
   static constexpr int kRow = DP * 2 + 16;               // bytes of a key's (value's) row
-  static constexpr int kStage = 2 * kTileKeys * kRow;    // 16 keys, then their values
+  static constexpr int kStage = 2 * kTile * kRow;        // the keys, then their values
   static constexpr int kBlocks = DP <= 128 ? 2 : 1;      // resident on an SM
   // As many as 227 KB hold: 69 to 112 KB in flight on an SM, of which some 40 KB cover the latency at full rate.
   static constexpr int kStages = DP == 64 ? 6 : DP == 96 ? 4 : DP == 128 ? 3 : DP == 160 ? 5 : DP == 192 ? 4 : 3;
-  static constexpr int kSmem = kWarps * kStages * kStage;
+  static constexpr int kRing = kStages * kStage;
+  static constexpr int kSmem = kWarps / WR * kRing;
 };
 
 // The keys that row tile `rt` of a sequence sees at most, and the row's own bounds.
@@ -120,10 +130,14 @@ __device__ __forceinline__ int keys_seen(const PagedArgs& a, int len, long long 
   return a.causal ? int(max(0ll, min((long long)len, p + 1))) : len;
 }
 // A sequence without keys still has rows to write: it counts one tile.
-__device__ __forceinline__ int tiles_of(int len) { return max(1, (len + kTileKeys - 1) / kTileKeys); }
+template <int KT>
+__device__ __forceinline__ int tiles_of(int len) {
+  return max(1, (len + KT - 1) / KT);
+}
 
 // A worker's place in its run of tiles: the item (sequence b, rest = kv head * row_tiles + row tile) and the tiles of it
 // that belong to the run.
+template <int KT>
 struct Cursor {
   int b, rest;
   int t, t1;        // next tile, end of the run's tiles within the item
@@ -134,11 +148,11 @@ struct Cursor {
 
   __device__ __forceinline__ void enter(const PagedArgs& a, int t0, long long run) {
     seq = sequence_of(a, b);
-    tiles = tiles_of(seq.len);
+    tiles = tiles_of<KT>(seq.len);
     t = t0;
     t1 = int(min((long long)tiles, t0 + run));
     left = run - (t1 - t0);
-    const int last = min(a.rows, (rest % a.row_tiles + 1) * 16 * a.wr) - 1;
+    const int last = min(a.rows, (rest % a.row_tiles + 1) * KT) - 1;  // (a row tile has as many rows as a tile has keys)
     seen = keys_seen(a, seq.len, seq.p0 + last / a.G);
   }
   // The next item of the run; false when there is none.
@@ -152,61 +166,39 @@ struct Cursor {
     return true;
   }
   // End of the tiles that have a key to see.
-  __device__ __forceinline__ int visible_end() const { return min(t1, (seen + kTileKeys - 1) / kTileKeys); }
+  __device__ __forceinline__ int visible_end() const { return min(t1, (seen + KT - 1) / KT); }
 };
 
 __device__ __forceinline__ long long shfl_ll(long long v, int lane) { return __shfl_sync(0xffffffffu, v, lane); }
 
-template <int DP, bool MODS>
-__global__ void __launch_bounds__(kWarps * 32, PagedLayout<DP>::kBlocks) attention_paged_kernel(const PagedArgs a) {
-  using L = PagedLayout<DP>;
+template <int DP, int WR, bool MODS>
+__global__ void __launch_bounds__(kWarps * 32, PagedLayout<DP, WR>::kBlocks) attention_paged_kernel(const PagedArgs a) {
+  using L = PagedLayout<DP, WR>;
+  constexpr int KT = L::kTile;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ __align__(8) uint64_t s_full[kWarps * kMaxStages], s_empty[kWarps * kMaxStages], s_never;
-  __shared__ uint32_t s_valid[kWarps * kMaxStages];  // which of a stage's 16 keys are there
-  __shared__ int s_abort;
-  const int tid = int(threadIdx.x), lane = tid & 31, warp = tid >> 5;
-  const int role = warp % a.wr;                        // this warp's 16 rows of the worker's
-  const int worker = int(blockIdx.x) * (kWarps / a.wr) + warp / a.wr;
-  const int ring0 = (warp / a.wr) * a.stages;          // first stage of the worker's ring
-
-  if (tid == 0) {
-    for (int i = 0; i < kWarps * L::kStages; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&s_empty[i], uint32_t(a.wr));
-    }
-    mbar_init(&s_never, 1);
-    s_abort = 0;
-    fence_barrier_init();
-  }
-  // Columns of the keys behind the head dim: zeros once, no copy writes them. (The values' only reach columns of O that
-  // are not stored.)
-  if (a.D < DP) {
-    const int words = (DP - a.D) / 8;
-    for (int i = tid; i < kWarps * L::kStages * kTileKeys * words; i += kWarps * 32) {
-      const int row = i / words, c = i - row * words;
-      *reinterpret_cast<uint4*>(smem + (row / kTileKeys) * L::kStage + (row % kTileKeys) * L::kRow + (a.D + c * 8) * 2) =
-          make_uint4(0u, 0u, 0u, 0u);
-    }
-  }
-  __syncthreads();
+  __shared__ uint32_t s_valid[kWarps][kMaxStages][2];  // which of a stage's keys are there, as each warp found
+  const int lane = int(threadIdx.x) & 31, warp = int(threadIdx.x) >> 5;
+  const int role = warp % WR;  // this warp's 16 rows of the worker's
+  const int worker = int(blockIdx.x) * (kWarps / WR) + warp / WR;
+  const uint32_t ring = smem_u32(smem) + (warp / WR) * L::kRing;
   pdl_wait();
   pdl_launch_dependents();
 
   // The worker's run: an equal share of all tiles.
   const long long per_tile = (long long)a.Hk * a.row_tiles;
   long long total = 0;
-  for (int b = lane; b < a.B; b += 32) total += tiles_of(sequence_len(a, b));
+  for (int b = lane; b < a.B; b += 32) total += tiles_of<KT>(sequence_len(a, b));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   total *= per_tile;
   const long long span = max((total + a.workers - 1) / a.workers, (long long)a.min_span);
   const long long u0 = worker * span, u1 = min(total, u0 + span);
-  int4 rec = make_int4(0, 0, 0, 0);
+  int4 rec = make_int4(0, 0, 0, worker);
   if (u0 < u1) {
-    Cursor at;
+    Cursor<KT> at;
     long long base = 0;
     for (int c = 0; c < a.B; c += 32) {
-      const long long mine = c + lane < a.B ? per_tile * tiles_of(sequence_len(a, c + lane)) : 0;
+      const long long mine = c + lane < a.B ? per_tile * tiles_of<KT>(sequence_len(a, c + lane)) : 0;
       long long upto = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -222,81 +214,75 @@ __global__ void __launch_bounds__(kWarps * 32, PagedLayout<DP>::kBlocks) attenti
       }
       base += shfl_ll(upto, 31);
     }
-    const int tiles0 = tiles_of(sequence_len(a, at.b));
+    const int tiles0 = tiles_of<KT>(sequence_len(a, at.b));
     at.rest = int((u0 - base) / tiles0);
     at.enter(a, int((u0 - base) - (long long)at.rest * tiles0), u1 - u0);
 
-    // ---- the loader: lanes 0-15 copy keys, 16-31 values; it runs `stages` tiles ahead
-    Cursor ld = at;
+    // ---- the loader, kStages - 1 tiles ahead: each lane looks up the page of one key (two of 64), the warps of a worker
+    // copy a share each
+    constexpr int kKeys = KT <= 32 ? 1 : 2;
+    Cursor<KT> ld = at;
     bool more = true;  // the loader has a tile
-    int ld_end = ld.visible_end(), page = -1;
-    const __nv_bfloat16* src = nullptr;
-    const bool is_v = lane >= 16;
-    const long long sp = is_v ? a.v_sp : a.k_sp, ss = is_v ? a.v_ss : a.k_ss;
-    const auto seek = [&]() {  // to the next tile with keys, and the page of this lane's key of it
+    int ld_end = ld.visible_end(), ld_stage = 0;
+    int page[kKeys];
+    const auto seek = [&]() {  // to the next tile with keys, and the pages of this lane's keys of it
       while (ld.t >= ld_end) {
         if (!ld.next(a)) {
           more = false;
           return;
         }
         ld_end = ld.visible_end();
-        src = nullptr;
       }
-      if (src == nullptr) {
+#pragma unroll
+      for (int x = 0; x < kKeys; ++x) {
+        const int j = ld.t * KT + lane + 32 * x;
+        page[x] = lane < KT && j < ld.seen ? a.table[ld.b * a.table_stride + j / a.page_size] : -1;
+      }
+    };
+    const auto issue = [&]() {
+      if (more) {
         const int kvh = ld.rest / a.row_tiles;
-        src = is_v ? a.v + kvh * a.v_sh : a.k + kvh * a.k_sh;
+        const __nv_bfloat16* src[2] = {a.k + kvh * a.k_sh, a.v + kvh * a.v_sh};
+        long long off[kKeys][2];  // of this lane's keys and values
+#pragma unroll
+        for (int x = 0; x < kKeys; ++x) {
+          const bool ok = page[x] >= 0 && page[x] < a.pages;
+          const uint32_t mask = __ballot_sync(0xffffffffu, ok);
+          if (lane == 0) s_valid[warp][ld_stage][x] = mask;
+          const int slot = (ld.t * KT + lane + 32 * x) % a.page_size;
+          off[x][0] = ok ? page[x] * a.k_sp + slot * a.k_ss : -1;
+          off[x][1] = ok ? page[x] * a.v_sp + slot * a.v_ss : -1;
+        }
+        constexpr int kChunks = DP / 8;  // 16-byte pieces of a row
+        const uint32_t stage = ring + ld_stage * L::kStage;
+#pragma unroll
+        for (int which = 0; which < 2; ++which)
+#pragma unroll
+          for (int i = 0; i < kSub * kChunks / 32; ++i) {
+            const int idx = (i * WR + role) * 32 + lane, row = idx / kChunks, c = idx - row * kChunks;
+            long long o = __shfl_sync(0xffffffffu, off[0][which], row & 31);
+            if constexpr (kKeys == 2) {
+              const long long hi = __shfl_sync(0xffffffffu, off[1][which], row & 31);
+              o = row >= 32 ? hi : o;
+            }
+            const bool ok = o >= 0 && c * 8 < a.D;
+            copy16(stage + (which * KT + row) * L::kRow + c * 16, src[which] + (ok ? o + c * 8 : 0), ok);
+          }
+        ld_stage = ld_stage + 1 == L::kStages ? 0 : ld_stage + 1;
+        ++ld.t;
+        seek();
       }
-      const int j = ld.t * kTileKeys + (lane & 15);
-      page = j < ld.seen ? a.table[ld.b * a.table_stride + j / a.page_size] : -1;
+      copy_commit();  // (an empty group behind the last tile: the waits count groups)
     };
-    int ld_stage = 0;
-    uint32_t ld_phase = 0;
-    int ahead = 0;  // tiles loaded and not yet used
-    const auto issue = [&]() -> bool {
-      if (a.wr > 1 && !mbar_wait_bounded_warp(&s_empty[ring0 + ld_stage], ld_phase ^ 1u, &s_abort, a.ctl,
-                                              kStatusTimeoutProducer))
-        return false;
-      const bool ok = page >= 0 && page < a.pages;
-      const uint32_t valid = __ballot_sync(0xffffffffu, ok) & 0xffffu;
-      uint64_t* bar = &s_full[ring0 + ld_stage];
-      if (lane == 0) {
-        s_valid[ring0 + ld_stage] = valid;
-        mbar_arrive_expect_tx(bar, uint32_t(__popc(valid)) * uint32_t(a.D) * 4u);
-      }
-      __syncwarp();
-      if (ok) {
-        const int j = ld.t * kTileKeys + (lane & 15);
-        bulk_load(smem_u32(smem + (ring0 + ld_stage) * L::kStage + lane * L::kRow),
-                  src + (long long)page * sp + (j % a.page_size) * ss, uint32_t(a.D) * 2u, bar);
-      }
-      if (++ld_stage == a.stages) {
-        ld_stage = 0;
-        ld_phase ^= 1u;
-      }
-      ++ahead;
-      ++ld.t;
-      seek();
-      return true;
-    };
-    bool good = true;
-    // With more warps the stage used last may still be read by another: the loader stays one tile further behind.
-    const int depth = a.wr > 1 ? a.stages - 1 : a.stages;
-    const auto fill = [&]() {
-      while (good && more && ahead < depth) good = issue();
-    };
-    if (role == 0) {
-      seek();
-      fill();
-    }
+    seek();
+#pragma unroll
+    for (int i = 0; i < L::kStages - 1; ++i) issue();
 
     // ---- the items of the run
     const int g = lane >> 2, c2 = (lane & 3) * 2;
     int stage = 0;
-    uint32_t phase = 0;
-    if (a.ctl.debug & 1u) good = mbar_wait_bounded_warp(&s_never, 0, &s_abort, a.ctl, kStatusForced);
-    bool again = good;
-    while (again) {
-      const int kvh = at.rest / a.row_tiles, r0 = (at.rest % a.row_tiles) * 16 * a.wr + role * 16;
+    do {
+      const int kvh = at.rest / a.row_tiles, r0 = (at.rest % a.row_tiles) * 16 * WR + role * 16;
       int lim[2];
       long long p[2];
       float slope[2];
@@ -332,13 +318,20 @@ __global__ void __launch_bounds__(kWarps * 32, PagedLayout<DP>::kBlocks) attenti
         for (int e = 0; e < 4; ++e) o[n][e] = 0.0f;
 
       const int first = at.t, end = at.visible_end();
-      for (int t = first; t < end && good; ++t) {
-        if (!mbar_wait_bounded_warp(&s_full[ring0 + stage], phase, &s_abort, a.ctl, kStatusTimeoutEpilogue)) {
-          good = false;
-          break;
+      for (int t = first; t < end; ++t) {
+        copy_wait<L::kStages - 2>();
+        if constexpr (WR == 1) {
+          __syncwarp();
+        } else {  // the other warps' copies of this tile are there, and they are done with the tile before
+          named_barrier_sync(1 + warp / WR, WR * 32);
         }
-        const uint32_t valid = s_valid[ring0 + stage];
-        const uint32_t base_k = smem_u32(smem + (ring0 + stage) * L::kStage);
+        issue();
+        const uint32_t stage_k = ring + stage * L::kStage;
+#pragma unroll 1
+        for (int sub = 0; sub < WR; ++sub) {
+        const int j0 = t * KT + sub * kSub;
+        const uint32_t valid = (s_valid[warp][stage][sub >> 1] >> ((sub & 1) * 16)) & 0xffffu;
+        const uint32_t base_k = stage_k + sub * kSub * L::kRow;
         // S = Q K^T: two blocks of 8 keys, even and odd steps in sums of their own (half the chain)
         float s4[2][2][4];
 #pragma unroll
@@ -364,20 +357,20 @@ __global__ void __launch_bounds__(kWarps * 32, PagedLayout<DP>::kBlocks) attenti
             if constexpr (MODS) {
               x[n][e] = a.cap_out != 0.0f ? a.cap_out * tanhf(dot * a.cap_in) : dot * a.scale_log2;
               if (a.slopes != nullptr) {
-                const long long j = t * kTileKeys + n * 8 + c2 + (e & 1);
+                const long long j = j0 + n * 8 + c2 + (e & 1);
                 x[n][e] = fmaf(-slope[e >> 1], fabsf(float(p[e >> 1] - j)), x[n][e]);
               }
             } else {
               x[n][e] = dot * a.scale_log2;
             }
           }
-        if (valid != 0xffffu || (t + 1) * kTileKeys > lim_min) {
+        if (valid != 0xffffu || j0 + kSub > lim_min) {
 #pragma unroll
           for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int j = n * 8 + c2 + (e & 1);
-              if (t * kTileKeys + j >= lim[e >> 1] || ((valid >> j) & 1u) == 0) x[n][e] = -INFINITY;
+              if (j0 + j >= lim[e >> 1] || ((valid >> j) & 1u) == 0) x[n][e] = -INFINITY;
             }
         }
         float top[2];
@@ -425,38 +418,17 @@ __global__ void __launch_bounds__(kWarps * 32, PagedLayout<DP>::kBlocks) attenti
           }
         }
         // O += P V
-        const uint32_t va = base_k + kTileKeys * L::kRow + ((lane & 7) + ((lane >> 3) & 1) * 8) * L::kRow + ((lane >> 4) & 1) * 16;
-        if (valid == 0xffffu) {
+        const uint32_t va = base_k + KT * L::kRow + ((lane & 7) + ((lane >> 3) & 1) * 8) * L::kRow + ((lane >> 4) & 1) * 16;
 #pragma unroll
-          for (int n = 0; n < DP / 16; ++n) {
-            uint32_t vf[4];
-            ldmatrix_x4_trans(va + n * 32, vf);
-            mma_bf16(o[2 * n], pf, vf[0], vf[1]);
-            mma_bf16(o[2 * n + 1], pf, vf[2], vf[3]);
-          }
-        } else {  // values that no copy brought: zeros instead of what the stage held (0 times NaN is NaN)
-          const uint32_t k0 = ((valid >> c2) & 1u ? 0xffffu : 0u) | ((valid >> (c2 + 1)) & 1u ? 0xffff0000u : 0u);
-          const uint32_t k1 = ((valid >> (c2 + 8)) & 1u ? 0xffffu : 0u) | ((valid >> (c2 + 9)) & 1u ? 0xffff0000u : 0u);
-#pragma unroll
-          for (int n = 0; n < DP / 16; ++n) {
-            uint32_t vf[4];
-            ldmatrix_x4_trans(va + n * 32, vf);
-            mma_bf16(o[2 * n], pf, vf[0] & k0, vf[1] & k1);
-            mma_bf16(o[2 * n + 1], pf, vf[2] & k0, vf[3] & k1);
-          }
+        for (int n = 0; n < DP / 16; ++n) {
+          uint32_t vf[4];
+          ldmatrix_x4_trans(va + n * 32, vf);
+          mma_bf16(o[2 * n], pf, vf[0], vf[1]);
+          mma_bf16(o[2 * n + 1], pf, vf[2], vf[3]);
         }
-        __syncwarp();
-        if (a.wr > 1 && lane == 0) mbar_arrive(&s_empty[ring0 + stage]);
-        if (++stage == a.stages) {
-          stage = 0;
-          phase ^= 1u;
         }
-        if (role == 0) {
-          --ahead;
-          fill();
-        }
+        stage = stage + 1 == L::kStages ? 0 : stage + 1;
       }
-      if (!good) break;
 
       // ---- the item's rows, or the run's part of them
 #pragma unroll
@@ -467,8 +439,10 @@ __global__ void __launch_bounds__(kWarps * 32, PagedLayout<DP>::kBlocks) attenti
       const bool whole = first == 0 && at.t1 == at.tiles;
       if (first == 0 && !whole) {
         const long long item_end = u1 - (at.t1 - first) + at.tiles;  // the run ends in this item
-        rec = make_int4(at.b, at.rest, int((item_end - 1) / span) - worker + 1, 0);
+        rec = make_int4(at.b, at.rest, int((item_end - 1) / span) - worker + 1, worker);
       }
+      if (a.rec_items && first == 0 && role == 0 && lane == 0)
+        a.rec[at.b * (a.Hk * a.row_tiles) + at.rest] = whole ? make_int4(0, 0, 0, 0) : rec;
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
         const int r = r0 + g + 8 * y;
@@ -509,38 +483,23 @@ __global__ void __launch_bounds__(kWarps * 32, PagedLayout<DP>::kBlocks) attenti
           }
         }
       }
-      again = at.next(a);
-    }
-    if (!good) {  // copies in flight write to this block's memory: it stays until they are done
-      rec = make_int4(0, 0, 0, 0);
-      if (role == 0) {
-        for (; ahead > 0; --ahead) {
-          mbar_wait_drain(&s_full[ring0 + stage], phase, a.ctl);
-          if (++stage == a.stages) {
-            stage = 0;
-            phase ^= 1u;
-          }
-        }
-      }
-    }
+    } while (at.next(a));
   }
-  if (role == 0 && lane == 0) a.rec[worker] = rec;
+  if (!a.rec_items && role == 0 && lane == 0) a.rec[worker] = rec;
 }
 
-// Joins the parts of the item that begins in worker blockIdx.x's run and ends in a later one. Eight warps take the parts in
-// turn, a lane 4 (8 above 128) columns of them.
-__global__ void __launch_bounds__(kJoinWarps * 32) attention_paged_join_kernel(const PagedArgs a) {
+// Joins the parts of the item of record blockIdx.x. Eight warps take the parts in turn, a lane 4 (8 above 128) columns.
+__global__ void __launch_bounds__(kJoinWarps * 32) attention_paged_join_kernel(const PagedArgs a, int row_tile) {
   __shared__ float s_acc[kJoinWarps][256];
   __shared__ float s_inv;
   const int lane = int(threadIdx.x) & 31, warp = int(threadIdx.x) >> 5;
-  const int w = int(blockIdx.x);
   pdl_wait();
   pdl_launch_dependents();
-  const int4 rec = a.rec[w];
-  const int parts = rec.z;
+  const int4 rec = a.rec[blockIdx.x];
+  const int parts = rec.z, w = rec.w;
   if (parts == 0) return;
-  const int kvh = rec.y / a.row_tiles, r0 = (rec.y % a.row_tiles) * 16 * a.wr;
-  const int rows = min(a.rows - r0, 16 * a.wr);
+  const int kvh = rec.y / a.row_tiles, r0 = (rec.y % a.row_tiles) * row_tile;
+  const int rows = min(a.rows - r0, row_tile);
   const auto part_row = [&](int z) { return ((long long)(w + z) * 2 + (z == 0)) * a.slot_rows; };
   for (int row = int(blockIdx.y); row < rows; row += int(gridDim.y)) {
     float top = -INFINITY;
@@ -633,31 +592,38 @@ PagedPlan plan_paged(int64_t H, int64_t Hk, int64_t Sq, int64_t D, int sms) {
   return p;
 }
 
-template <int DP, bool MODS>
-int launch_paged(PagedArgs& a, int blocks, cudaStream_t stream, int device) {
-  using L = PagedLayout<DP>;
+template <int DP, int WR, bool MODS>
+int launch_paged(const PagedArgs& a, int blocks, cudaStream_t stream, int device) {
+  using L = PagedLayout<DP, WR>;
   static_assert(L::kStages <= kMaxStages && L::kSmem + 2048 <= 227 * 1024 / L::kBlocks, "shared memory of the SM");
-  static bool ready[64] = {};
+  static std::atomic<bool> ready[64] = {};
   if (!ready[device]) {
-    if (int rc = check_cuda(cudaFuncSetAttribute(attention_paged_kernel<DP, MODS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 L::kSmem),
+    if (int rc = check_cuda(cudaFuncSetAttribute(attention_paged_kernel<DP, WR, MODS>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem),
                             "paged attention shared memory"))
       return rc;
     ready[device] = true;
   }
-  a.stages = L::kStages * a.wr;
-  return check_cuda(launch_pdl(attention_paged_kernel<DP, MODS>, dim3(unsigned(blocks)), dim3(kWarps * 32), L::kSmem, stream, a),
+  return check_cuda(launch_pdl(attention_paged_kernel<DP, WR, MODS>, dim3(unsigned(blocks)), dim3(kWarps * 32), L::kSmem,
+                               stream, a),
                     "paged attention kernel launch");
 }
 
+template <int WR, bool MODS>
+int launch_paged_dim(const PagedArgs& a, int blocks, cudaStream_t stream, int device) {
+  if (a.D <= 64) return launch_paged<64, WR, MODS>(a, blocks, stream, device);
+  if (a.D <= 96) return launch_paged<96, WR, MODS>(a, blocks, stream, device);
+  if (a.D <= 128) return launch_paged<128, WR, MODS>(a, blocks, stream, device);
+  if (a.D <= 160) return launch_paged<160, WR, MODS>(a, blocks, stream, device);
+  if (a.D <= 192) return launch_paged<192, WR, MODS>(a, blocks, stream, device);
+  return launch_paged<256, WR, MODS>(a, blocks, stream, device);
+}
+
 template <bool MODS>
-int launch_paged_for(PagedArgs& a, int blocks, cudaStream_t stream, int device) {
-  if (a.D <= 64) return launch_paged<64, MODS>(a, blocks, stream, device);
-  if (a.D <= 96) return launch_paged<96, MODS>(a, blocks, stream, device);
-  if (a.D <= 128) return launch_paged<128, MODS>(a, blocks, stream, device);
-  if (a.D <= 160) return launch_paged<160, MODS>(a, blocks, stream, device);
-  if (a.D <= 192) return launch_paged<192, MODS>(a, blocks, stream, device);
-  return launch_paged<256, MODS>(a, blocks, stream, device);
+int launch_paged_for(const PagedArgs& a, int wr, int blocks, cudaStream_t stream, int device) {
+  if (wr == 1) return launch_paged_dim<1, MODS>(a, blocks, stream, device);
+  if (wr == 2) return launch_paged_dim<2, MODS>(a, blocks, stream, device);
+  return launch_paged_dim<4, MODS>(a, blocks, stream, device);
 }
 
 }  // namespace
@@ -740,28 +706,25 @@ int attention_paged_launch(const AttnPagedProblem& p, cudaStream_t stream) {
   a.cap_in = cap_in;
   a.cap_out = p.softcap * kLog2e;
   a.slopes = p.slopes;
-  a.wr = plan.wr;
   a.workers = plan.workers;
   a.rows = int(plan.rows);
   a.row_tiles = int(plan.row_tiles);
   a.slot_rows = int(plan.slot_rows);
   a.min_span = p.variant > 0 ? p.variant : 4;
+  const int64_t items = p.batch * c.kv_heads * plan.row_tiles;
+  a.rec_items = items <= plan.workers;
   uint8_t* ws = static_cast<uint8_t*>(p.workspace);
   a.rec = reinterpret_cast<int4*>(ws);
   a.part_ml = reinterpret_cast<float2*>(ws + plan.ml_offset);
   a.part_o = reinterpret_cast<float*>(ws + plan.o_offset);
-  a.ctl.status = dev->status;
-  a.ctl.timeout_ns = wait_timeout_ns();
-  a.ctl.debug = p.debug;
   const bool mods = p.softcap > 0.0f || p.slopes != nullptr;
-  if (int rc = mods ? launch_paged_for<true>(a, plan.blocks, stream, dev->device)
-                    : launch_paged_for<false>(a, plan.blocks, stream, dev->device))
+  if (int rc = mods ? launch_paged_for<true>(a, plan.wr, plan.blocks, stream, dev->device)
+                    : launch_paged_for<false>(a, plan.wr, plan.blocks, stream, dev->device))
     return rc;
-  // A block joins one item, all of its rows when there are items enough to fill the GPU.
-  const int64_t items = p.batch * c.kv_heads * plan.row_tiles;
+  // A block joins one row of an item, or all of them when there are items enough to fill the GPU.
   const int64_t split = items >= dev->sms ? 1 : plan.slot_rows;
-  return check_cuda(launch_pdl(attention_paged_join_kernel, dim3(unsigned(plan.workers), unsigned(split)),
-                               dim3(kJoinWarps * 32), 0, stream, a),
+  return check_cuda(launch_pdl(attention_paged_join_kernel, dim3(unsigned(std::min<int64_t>(items, plan.workers)), unsigned(split)),
+                               dim3(kJoinWarps * 32), 0, stream, a, 16 * plan.wr),
                     "paged attention join kernel launch");
 }
 
