@@ -7,25 +7,28 @@
 // and parts (m, l, o) of one row's keys join the same way. Scores are kept in log2 units.
 //
 // Bound by memory: each key and value is read once and does 4 G flops a value for the G query heads of its head, far below
-// what the tensor cores need to be busy. So the design is about loads in flight and an even split:
-//   * A worker is WR warps, 16 rows each; the rows of a (sequence, key/value head) are its G heads x the new tokens. Few
-//     rows take one warp, more share the keys of one load among 2 or 4 warps. Rows of 16 waste the matrix instruction's
-//     rows, not time: mma.sync m16n8k16 on registers keeps the whole softmax in one warp, without the round trips through
-//     TMEM and shared memory that a tcgen05 tile of 128 rows would add to each tile of keys.
-//   * One block an SM. Every block takes an equal run of tiles of the whole batch, found on the device from kv_lens, so
-//     ragged lengths leave no SM idle and a captured graph follows them, and its workers equal shares of it. Shares start
-//     and end anywhere in a sequence; the parts of a row's keys are joined in order of keys, first those of a block through
-//     its shared memory, then those of several blocks through the workspace by the join kernel.
-//   * A tile's keys and values are rows anywhere in memory: cp.async of 16 bytes a lane takes any page size and layout.
-//     (A bulk copy a row, one instruction a lane, was the first form: the copy engine takes one in about 17 cycles, 16
-//     bytes a cycle at 128 columns where 23 are the memory's rate.) Keys and values wait in one ring, a half tile each.
-//     Rows in shared memory are 16 bytes longer than the head, so that ldmatrix reads 8 of them without a bank conflict.
+// what the tensor cores need to be busy. So the design is about loads in flight, few instructions a key and an even split:
+//   * Keys are the rows of the matrix instructions: S^T = K Q^T and O^T = V^T P^T with mma.sync m16n8k16, 16 keys (16
+//     columns of the head) against 8 rows of queries. The rows of a (sequence, key/value head) are its G heads x the new
+//     tokens, mostly 8 or fewer, so nothing is padded to the 64 or 128 rows of a tcgen05 tile, and the softmax of a tile
+//     stays in one warp's registers without round trips through TMEM and shared memory. A warp takes one or two such blocks
+//     of 8 rows; more rows share the keys of one load among the 2 or 4 warps of a worker.
+//   * Every block takes an equal run of tiles of the whole batch, found on the device from kv_lens, so ragged lengths leave
+//     no SM idle and a captured graph follows them, and its workers equal shares of it. Shares start and end anywhere in a
+//     sequence; the parts of a row's keys are joined in order of keys, first those of a block through its shared memory,
+//     then those of several blocks through the workspace by the join kernel.
+//   * Pages of a multiple of 16 slots are read by TMA, a box of 64 columns x 16 (32) slots a copy; other pages and layouts
+//     that a tensor map does not take by cp.async, 16 bytes a lane, which costs as many instructions as all the arithmetic.
+//     (A bulk copy a row was the first form: the copy engine takes one in about 17 cycles, 16 bytes a cycle at 128 columns
+//     where 23 are the memory's rate.) Keys and values wait in one ring, a half tile each, swizzled in 128-byte rows, which
+//     ldmatrix reads without a bank conflict.
 #include <algorithm>
 #include <atomic>
 #include <cfloat>
 #include <cmath>
 #include <cstring>
 
+#include "attention_sm100.cuh"
 #include "internal.h"
 
 namespace npub200 {
@@ -33,11 +36,27 @@ namespace npub200 {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kWarps = 8;  // of a block
+constexpr int kWarps = 4;  // of a block
+constexpr int kBlocks = 2;  // resident on an SM
+constexpr int kWaves = 1;  // blocks of the grid for each that is resident
+constexpr int kMaxHalves = 8;  // of a ring
 constexpr int kJoinWarps = 8;
+constexpr int kJoinMaxRecs = 1024;  // blocks whose records the join kernel looks through
 // The row maximum moves only when a tile's beats it by this much (log2 units): P stays within 2^8 of 1, which bf16 holds
 // with the same relative rounding, and the O registers are rescaled once in a while instead of once a tile.
 constexpr float kRescale = 8.0f;
+
+// n / d for 0 <= n < 2^31 by a multiplication: with p = 31 + ceil(log2 d) and mul = ceil(2^p / d), n mul / 2^p is above
+// n / d by less than 1 / d.
+struct Divisor {
+  uint32_t mul, shift;
+  __device__ __forceinline__ int operator()(int n) const { return int((uint64_t(uint32_t(n)) * mul) >> shift); }
+};
+Divisor divisor(int64_t d) {
+  int log = 0;
+  while ((int64_t(1) << log) < d) ++log;
+  return Divisor{uint32_t(((uint64_t(1) << (31 + log)) + uint64_t(d) - 1) / uint64_t(d)), uint32_t(31 + log)};
+}
 
 struct PagedArgs {
   const __nv_bfloat16* q;
@@ -46,30 +65,37 @@ struct PagedArgs {
   long long k_sp, k_ss, k_sh;
   const __nv_bfloat16* v;
   long long v_sp, v_ss, v_sh;
+  MapPos pk, pv;  // where the slot, head and page are among the coordinates of the tensor maps
+  int tma;        // 1: the maps are there
   const int32_t* table;
   long long table_stride;
   int pages, page_size, capacity;
+  Divisor by_page;
   const int32_t* lens;
   const int32_t* q_starts;
   void* out;
   long long o_sb, o_ss, o_sh;
-  int out_f32, out_vec;  // out_vec: pairs (1) or four (2) output columns may be written together
+  int out_f32, out_vec;  // out_vec: four output columns may be written together
   int B, Hk, G, Sq, D;
+  Divisor by_g;
   int causal;
   float scale_log2;       // scores to log2 units
   float cap_in, cap_out;  // softcap: cap_out tanh(cap_in q.k), cap_out 0: none
   const float* slopes;
-  int rows, row_tiles, slot_rows;  // rows of a (sequence, kv head), tiles of 16 WR rows, rows of a part
+  int rows, row_tiles, slot_rows;  // rows of a (sequence, kv head), tiles of a worker's rows, rows of a part
+  Divisor by_row_tiles, by_slot_rows;
   int min_span;           // least tiles of a block's run
-  // What there is to join: of each item where there are no more items than blocks, else of the item that begins in each
-  // block's run and goes on behind it. (sequence, kv head and row tile, parts or 0, block of the first)
+  float per_block;        // 1 / blocks
+  // What there is to join: of the item that begins in each block's run and goes on behind it. (sequence, kv head and row
+  // tile, parts or 0, -)
   int4* rec;
-  int rec_items;
   float2* part_ml;  // [2 blocks][slot_rows] (m, l); part 0 of a block continues an item, part 1 begins one
   float* part_o;    // [2 blocks][slot_rows][D]
   float* head_o;    // [blocks][workers][slot_rows][D] O of the items that end within a worker's share
+  KernelCtl ctl;
 };
 
+// Four 8 x 8 matrices, a row of one at each lane's address.
 __device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -82,6 +108,12 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t (&r)[4
                : "r"(addr)
                : "memory");
 }
+// An 8 x 8 matrix of two-byte values across the warp, transposed.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
@@ -93,35 +125,35 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool ok) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() {  // all but the last N groups of this thread are there
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// Arrives on the barrier when this thread's copies so far are there.
+__device__ __forceinline__ void copy_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+__device__ __forceinline__ void copy_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// Layout of a block's shared memory for head dims up to DP and workers of WR warps.
-template <int DP, int WR>
+// Layout for head dims up to DP, workers of WR warps and NB blocks of 8 rows a warp.
+template <int DP, int WR, int NB>
 struct PagedLayout {
-  // Keys of a tile: what keeps its scores in registers next to O and Q. 16 for one warp took 30% longer at 64 columns,
-  // where the softmax of a tile and not its load decided.
-  static constexpr int kTile = WR == 1 ? (DP <= 128 ? 32 : 16) : 16 * WR;
-  static constexpr int kRow = DP * 2 + 16;  // bytes of a key's (value's) row
-  static constexpr int kHalf = kTile * kRow;  // the keys or the values of a tile
+  static constexpr int kAtoms = (DP + 63) / 64;           // 128-byte columns of a row
+  static constexpr int kTile = DP <= 128 ? 32 : 16;       // keys of a tile
+  static constexpr int kAtom = kTile * 128;               // bytes of one column of the keys (values) of a tile
+  static constexpr int kHalf = kAtoms * kAtom;
   static constexpr int kWorkers = kWarps / WR;
-  // As many as an SM holds next to the static tables: 130 to 170 KB in flight, of which some 40 KB cover the latency at the
-  // full rate.
-  static constexpr int kFit = 219 * 1000 / (kWorkers * kHalf);
-  static constexpr int kHalves = kFit < 8 ? kFit : 8;
+  static constexpr int kRows = 8 * NB * WR;
+  // As many as half an SM holds next to the static tables: up to 130 KB in flight on the SM, of which some 40 KB cover the
+  // latency at the full rate.
+  static constexpr int kFit = 104 * 1024 / (kWorkers * kHalf);
+  static constexpr int kHalves = kFit < kMaxHalves ? kFit : kMaxHalves;
   static constexpr int kRing = kHalves * kHalf;
-  static constexpr int kSmem = kWorkers * kRing;
-  // The ring takes the O rows of the share's last part, 8 floats longer so that their stores spread over the banks.
-  static_assert(kHalves >= 3 && kRing >= 16 * WR * (DP + 8) * 4, "ring");
+  static constexpr int kSmem = kWorkers * kRing + 1024;   // (the swizzle wants 1024-byte boundaries)
+  // The ring takes the O rows of the share's last part, 4 floats longer so that their stores spread over the banks.
+  static_assert(kHalves >= 3 && kRing >= kRows * (DP + 4) * 4, "ring");
 };
 
-// The keys that row tile `rt` of a sequence sees at most, and the row's own bounds.
+// The keys of a sequence.
 struct Sequence {
-  int len;         // valid keys
-  long long p0;    // position of query 0
+  int len;       // valid keys
+  long long p0;  // position of query 0
 };
 __device__ __forceinline__ int sequence_len(const PagedArgs& a, int b) { return min(max(a.lens[b], 0), a.capacity); }
 __device__ __forceinline__ Sequence sequence_of(const PagedArgs& a, int b) {
@@ -157,8 +189,8 @@ struct Cursor {
     t = t0;
     t1 = int(min((long long)tiles, t0 + run));
     left = run - (t1 - t0);
-    const int last = min(a.rows, (rest % a.row_tiles + 1) * row_tile) - 1;
-    seen = keys_seen(a, seq.len, seq.p0 + last / a.G);
+    const int last = min(a.rows, (rest - a.by_row_tiles(rest) * a.row_tiles + 1) * row_tile) - 1;
+    seen = keys_seen(a, seq.len, seq.p0 + a.by_g(last));
   }
   // The next item of the share; false when there is none.
   __device__ __forceinline__ bool next(const PagedArgs& a, int row_tile) {
@@ -193,66 +225,67 @@ __device__ __forceinline__ float capped(float y, float cap_out) {
   return cap_out * (z <= 1.0f ? p * y : far);
 }
 
-// Output columns col ... col + N - 1 (N = 2 or 4) of the row that starts at `base`.
-template <int N>
-__device__ __forceinline__ void write_out(const PagedArgs& a, long long base, int col, const float (&x)[N]) {
-  if (a.out_f32) {
-    float* d = static_cast<float*>(a.out) + base + col;
-    if (N == 4 && a.out_vec == 2) {
-      *reinterpret_cast<float4*>(d) = make_float4(x[0], x[1], x[N - 2], x[N - 1]);
-    } else if (N == 2 && a.out_vec) {
-      *reinterpret_cast<float2*>(d) = make_float2(x[0], x[1]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) d[i] = x[i];
-    }
-  } else {
-    __nv_bfloat16* d = static_cast<__nv_bfloat16*>(a.out) + base + col;
-    if (N == 4 && a.out_vec == 2) {
-      *reinterpret_cast<uint2*>(d) = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[N - 2], x[N - 1]));
-    } else if (N == 2 && a.out_vec) {
-      *reinterpret_cast<uint32_t*>(d) = pack_bf16x2(x[0], x[1]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) d[i] = __float2bfloat16_rn(x[i]);
-    }
-  }
-}
 __device__ __forceinline__ long long out_row(const PagedArgs& a, int b, int kvh, int r) {
-  const int i = r / a.G, h = kvh * a.G + (r - i * a.G);
+  const int i = a.by_g(r), h = kvh * a.G + (r - i * a.G);
   return (long long)b * a.o_sb + (long long)i * a.o_ss + (long long)h * a.o_sh;
+}
+__device__ __forceinline__ void write_out(const PagedArgs& a, long long at, float x) {
+  if (a.out_f32)
+    static_cast<float*>(a.out)[at] = x;
+  else
+    static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(x);
+}
+__device__ __forceinline__ void write_out4(const PagedArgs& a, long long at, const float (&x)[4]) {
+  if (!a.out_vec) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) write_out(a, at + i, x[i]);
+  } else if (a.out_f32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = make_float4(x[0], x[1], x[2], x[3]);
+  } else {
+    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + at) =
+        make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
+  }
 }
 
 // A part of an item's keys that a worker is done with, or nothing (b < 0).
 struct Part {
   int b, rest;
-  int rem;            // tiles of the item behind it
+  int rem;                        // tiles of the item behind it
   uint8_t begins, ends, in_ring;  // holds the item's first tile, its last; where its O rows are
 };
 
-template <int DP, int WR, bool MODS>
-__global__ void __launch_bounds__(kWarps * 32, 1) attention_paged_kernel(const PagedArgs a) {
-  using L = PagedLayout<DP, WR>;
-  constexpr int KT = L::kTile, H = L::kHalves, NW = L::kWorkers, ROWS = 16 * WR;
-  constexpr int kKeys = KT <= 32 ? 1 : 2;  // keys of a tile a lane looks up
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ long long s_off[kWarps][KT][2];      // where the keys and values of the tile in issue are; < 0: nowhere
-  __shared__ uint32_t s_valid[kWarps][H][kKeys];  // which of a tile's keys are there, as each warp found
-  __shared__ Part s_part[NW][2];                  // parts to join: of the item a share continues, of the one it begins
-  __shared__ float2 s_ml[NW][2][ROWS];
+template <int DP, int WR, int NB, bool MODS>
+__global__ void __launch_bounds__(kWarps * 32, kBlocks)
+    attention_paged_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                           const PagedArgs a) {
+  using L = PagedLayout<DP, WR, NB>;
+  constexpr int KT = L::kTile, H = L::kHalves, NW = L::kWorkers, ROWS = L::kRows;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t s_full[NW][H], s_empty[NW][H], s_never;
+  __shared__ uint32_t s_valid[NW][H];      // which keys of a tile are there
+  __shared__ Part s_part[NW][2];           // parts to join: of the item a share continues, of the one it begins
+  __shared__ float2 s_ml[NW][2][ROWS];     // (m, l) of their rows, later (weight, l)
+  __shared__ int4 s_rec;
+  __shared__ int s_abort;
   const int lane = int(threadIdx.x) & 31, warp = int(threadIdx.x) >> 5;
-  const int role = warp % WR, wk = warp / WR;  // this warp's 16 rows of its worker's
+  const int role = warp % WR, wk = warp / WR;  // this warp's rows of its worker's
+  uint8_t* const smem = smem_raw + ((0u - smem_u32(smem_raw)) & 1023u);
   uint8_t* const ring = smem + wk * L::kRing;
   const uint32_t ring_at = smem_u32(ring);
-  const auto worker_sync = [&]() {
-    if constexpr (WR == 1) {
-      __syncwarp();
-    } else {
-      named_barrier_sync(1 + wk, WR * 32);
-    }
-  };
-  if (role == 0 && lane < 2) s_part[wk][lane].b = -1;
-  __syncwarp();
+  if (threadIdx.x < NW * H) {
+    // A tile's half is there when its copies are: TMA's bytes, or the copies of each lane, and the word of the lane that
+    // says which keys are valid.
+    mbar_init(&s_full[0][threadIdx.x], a.tma ? 1u : 32u * WR + 1u);
+    mbar_init(&s_empty[0][threadIdx.x], WR);
+  }
+  if (threadIdx.x < 2 * NW) s_part[threadIdx.x >> 1][threadIdx.x & 1].b = -1;
+  if (threadIdx.x == 0) {
+    s_rec = make_int4(0, 0, 0, 0);
+    s_abort = 0;
+    mbar_init(&s_never, 1);
+    fence_barrier_init();
+  }
+  __syncthreads();
   pdl_wait();
   pdl_launch_dependents();
 
@@ -279,7 +312,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attention_paged_kernel(const P
     total += more;
   }
   total *= per_tile;
-  const long long span = max(divide(total + gridDim.x - 1, gridDim.x), (long long)a.min_span);
+  // (a f32 product is off by less than 1 / blocks below 2^20 tiles: one more than its whole part is never short)
+  const long long span =
+      max(total < (1 << 20) ? (long long)(float(int(total)) * a.per_block) + 1 : (total + gridDim.x - 1) / gridDim.x,
+          (long long)a.min_span);
   const long long c0 = blockIdx.x * span, run = max(0ll, min(total, c0 + span) - c0);
   const long long u0 = c0 + run * wk / NW, u1 = c0 + run * (wk + 1) / NW;
   if (u0 < u1) {
@@ -301,392 +337,487 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attention_paged_kernel(const P
     at.rest = int(divide(u0 - base, tiles0));
     at.enter(a, ROWS, int((u0 - base) - (long long)at.rest * tiles0), u1 - u0);
 
-    // ---- the loader, H - 1 halves ahead: each lane looks up the page of a key, the warps of a worker copy a share each
-    struct Ahead {
-      int page[kKeys];
-      int t, kvh;  // t < 0: behind the last tile
-    };
+    // ---- the loader, H - 1 halves ahead: by TMA the worker's first warp, else all of its warps a share each. A lane looks
+    // up the page of its key.
     Cursor<KT> ld = at;
     int ld_end = ld.visible_end();
-    const auto seek = [&]() {  // to the next tile with keys, if any
+    const bool loads = role == 0 || !a.tma;
+    int page = -1, next_t = -1;  // of the tile that goes out next; next_t < 0: behind the last
+    int next_head = 0;
+    int ahead = 0;               // halves issued and not used (of the warp that loads)
+    const auto peek = [&]() {    // takes the next tile with keys, if any, and has its pages looked up
       while (ld.t >= ld_end) {
         if (!ld.next(a, ROWS)) {
-          ld_end = INT32_MAX;
-          ld.t = -1;
+          next_t = -1;
+          ld_end = 0;
+          ld.t = 0;
+          ld.left = 0;
           return;
         }
         ld_end = ld.visible_end();
       }
+      next_t = ld.t++;
+      next_head = a.by_row_tiles(ld.rest);
+      const int j = next_t * KT + lane;
+      page = lane < KT && j < ld.seen ? a.table[ld.b * a.table_stride + a.by_page(j)] : -1;
     };
-    const auto peek = [&](Ahead& x) {  // takes that tile and has its pages looked up
-      x.t = ld.t;
-      if (x.t < 0) return;
-      x.kvh = ld.rest / a.row_tiles;
-#pragma unroll
-      for (int y = 0; y < kKeys; ++y) {
-        const int key = lane + 32 * y, j = x.t * KT + key;
-        x.page[y] = key < KT && j < ld.seen ? a.table[ld.b * a.table_stride + j / a.page_size] : -1;
+    int in = 0, in_values = 0;  // the half of the ring that is filled next, with keys or values
+    uint32_t in_phase = 0;
+    // (Its code stands once: with the fill of the ring written out in front of the loop the start took 2 us more for
+    // fetching instructions.)
+    const auto issue = [&]() -> bool {
+      if (next_t < 0) return true;
+      if (WR > 1 && !mbar_wait_bounded_warp(&s_empty[wk][in], in_phase ^ 1u, &s_abort, a.ctl, kStatusTimeoutProducer))
+        return false;
+      uint64_t* const bar = &s_full[wk][in];
+      const bool ok = page >= 0 && page < a.pages;
+      const uint32_t valid = __ballot_sync(0xffffffffu, ok);
+      if (role == 0 && lane == 0) {
+        s_valid[wk][in] = valid;
+        if (a.tma)
+          mbar_arrive_expect_tx(bar, L::kHalf);
+        else
+          mbar_arrive(bar);
       }
-      ++ld.t;
-      seek();
-    };
-    constexpr int kChunks = DP / 8;  // 16-byte pieces of a row
-    int in = 0;                      // the half of the ring that the next copy goes to
-    const auto copy_half = [&](const Ahead& x, int which) {
-      if (x.t >= 0) {
-        const __nv_bfloat16* src = which ? a.v + x.kvh * a.v_sh : a.k + x.kvh * a.k_sh;
-        const uint32_t dst = ring_at + in * L::kHalf;
-#pragma unroll
-        for (int i = 0; i < KT * kChunks / (32 * WR); ++i) {
-          const int idx = (i * WR + role) * 32 + lane, row = idx / kChunks, c = idx - row * kChunks;
-          const long long o = s_off[warp][row][which];
-          const bool ok = o >= 0 && c * 8 < a.D;
-          copy16(dst + row * L::kRow + c * 16, src + (ok ? o + c * 8 : 0), ok);
-        }
-        in = in + 1 == H ? 0 : in + 1;
-      }
-      copy_commit();  // (an empty group behind the last tile: the waits count groups)
-    };
-    const auto issue_k = [&](const Ahead& x) {
-      if (x.t >= 0) {
-        __syncwarp();  // the table's last reads
-#pragma unroll
-        for (int y = 0; y < kKeys; ++y) {
-          const int key = lane + 32 * y, slot = (x.t * KT + key) % a.page_size;
-          const bool ok = x.page[y] >= 0 && x.page[y] < a.pages;
-          const uint32_t valid = __ballot_sync(0xffffffffu, ok);
-          if (lane == 0) s_valid[warp][in][y] = valid;
-          if (key < KT) {
-            s_off[warp][key][0] = ok ? x.page[y] * a.k_sp + slot * a.k_ss : -1;
-            s_off[warp][key][1] = ok ? x.page[y] * a.v_sp + slot * a.v_ss : -1;
-          }
-        }
+      if (a.tma) {
         __syncwarp();
-      }
-      copy_half(x, 0);
-    };
-    const auto issue_v = [&](const Ahead& x) { copy_half(x, 1); };
-
-    Ahead next;
-    {
-      Ahead pre[(H - 1) / 2];  // all look-ups of the start in flight together
-      seek();
+        // 16 slots and 64 columns a lane; a page that is not there is outside the map, zeros
+        constexpr int kBoxes = L::kAtoms * (KT / 16);
+        const int group = lane / L::kAtoms, atom = lane - group * L::kAtoms;
+        const int p = __shfl_sync(0xffffffffu, page, (group * 16) & 31);
+        if (lane < kBoxes) {
+          const int j = next_t * KT + group * 16, slot = j - a.by_page(j) * a.page_size;
+          const MapPos& pos = in_values ? a.pv : a.pk;
+          int c[4] = {atom * 64, 0, 0, 0};
+          const int page_at = p >= 0 && p < a.pages ? p : a.pages;
 #pragma unroll
-      for (int i = 0; i < (H - 1) / 2; ++i) peek(pre[i]);
-      peek(next);
-#pragma unroll
-      for (int i = 0; i < (H - 1) / 2; ++i) {
-        issue_k(pre[i]);
-        issue_v(pre[i]);
-      }
-      if constexpr (H % 2 == 0) issue_k(next);
-    }
-    // The half that is loaded where the keys of a tile (the values) have been waited for: H - 1 behind them.
-    const auto issue_at_keys = [&]() {
-      if constexpr (H % 2 == 1) {
-        issue_k(next);
+          for (int i = 1; i < 4; ++i) c[i] = pos.s == i ? slot : pos.h == i ? next_head : page_at;
+          tma_load_4d(in_values ? &map_v : &map_k, bar, ring + in * L::kHalf + atom * L::kAtom + group * 2048, c[0], c[1],
+                      c[2], c[3]);
+        }
       } else {
-        issue_v(next);
-        peek(next);
+        const long long sp = in_values ? a.v_sp : a.k_sp, ss = in_values ? a.v_ss : a.k_ss;
+        const __nv_bfloat16* src = in_values ? a.v + next_head * a.v_sh : a.k + next_head * a.k_sh;
+        const int j = next_t * KT + lane;
+        const long long off = ok ? page * sp + (j - a.by_page(j) * a.page_size) * ss : -1;  // < 0: nowhere
+        const uint32_t dst = ring_at + in * L::kHalf;
+        constexpr int kChunks = L::kAtoms * 8;  // 16-byte pieces of a row
+#pragma unroll 4
+        for (int i = role; i < KT * kChunks / 32; i += WR) {
+          const int idx = i * 32 + lane, row = idx / kChunks, c = idx - row * kChunks;
+          const long long o = __shfl_sync(0xffffffffu, off, row);
+          const bool there = o >= 0 && c * 8 < a.D;
+          copy16(dst + (c >> 3) * L::kAtom + row * 128 + (((c ^ row) & 7) << 4), src + (there ? o + c * 8 : 0), there);
+        }
+        copy_arrive(bar);
       }
-    };
-    const auto issue_at_values = [&]() {
-      if constexpr (H % 2 == 1) {
-        issue_v(next);
-        peek(next);
-      } else {
-        issue_k(next);
+      ++ahead;
+      if (++in == H) {
+        in = 0;
+        in_phase ^= 1u;
       }
+      if (in_values) peek();
+      in_values ^= 1;
+      return true;
     };
+    bool good = true;
+    if (loads) peek();
+    int filled = 0;  // halves issued ahead of the first that is used, up to H - 1
+    if (a.ctl.debug & 1u) good = mbar_wait_bounded_warp(&s_never, 0, &s_abort, a.ctl, kStatusForced);
 
     // ---- the items of the share
     const int g = lane >> 2, c2 = (lane & 3) * 2;
-    int out_half = 0;  // the half of the ring that is used next
-    do {
-      const int kvh = at.rest / a.row_tiles, r0 = (at.rest % a.row_tiles) * ROWS + role * 16;
-      int lim[2];
-      long long p[2];
-      float slope[2];
-      uint32_t qf[DP / 16][4];
-      {
-        const __nv_bfloat16* qp[2];
+    // ldmatrix: this lane's row of a half, and the four swizzled 16-byte columns that it reads of each 64
+    const int k_row = (lane & 7) + ((lane >> 3) & 1) * 8, v_row = (lane & 7) + (lane >> 4) * 8;
+    uint32_t k_col[4], v_col[4];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int r = r0 + g + 8 * x;
-          const bool ok = r < a.rows;
-          const int i = ok ? r / a.G : 0, h = kvh * a.G + (ok ? r - i * a.G : 0);
-          p[x] = at.seq.p0 + i;
-          lim[x] = ok ? keys_seen(a, at.seq.len, p[x]) : at.seq.len;
-          slope[x] = MODS && a.slopes != nullptr ? a.slopes[h] * kLog2e : 0.0f;
-          qp[x] = ok ? a.q + ((long long)at.b * a.q_sb + (long long)i * a.q_ss + (long long)h * a.q_sh + c2) : nullptr;
-        }
+    for (int i = 0; i < 4; ++i) {
+      k_col[i] = k_row * 128 + (((2 * i + (lane >> 4)) ^ (lane & 7)) << 4);
+      v_col[i] = v_row * 128 + (((2 * i + ((lane >> 3) & 1)) ^ (lane & 7)) << 4);
+    }
+    int used = 0;  // the half of the ring that is used next
+    uint32_t phase = 0;
+    while (good) {
+      const int kvh = a.by_row_tiles(at.rest), r0 = (at.rest - kvh * a.row_tiles) * ROWS + role * 8 * NB;
+      uint32_t qf[DP / 16][NB][2];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const int r = r0 + nb * 8 + g;
+        const bool ok = r < a.rows;
+        const int i = ok ? a.by_g(r) : 0, h = kvh * a.G + (ok ? r - i * a.G : 0);
+        const __nv_bfloat16* qp = a.q + ((long long)at.b * a.q_sb + (long long)i * a.q_ss + (long long)h * a.q_sh + c2);
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int col = s * 16 + (e >> 1) * 8;
-            qf[s][e] = qp[e & 1] != nullptr && col < a.D ? *reinterpret_cast<const uint32_t*>(qp[e & 1] + col) : 0u;
+          for (int e = 0; e < 2; ++e) {
+            const int col = s * 16 + e * 8;
+            qf[s][nb][e] = ok && col < a.D ? *reinterpret_cast<const uint32_t*>(qp + col) : 0u;
           }
       }
-      int lim_min = min(lim[0], lim[1]);
+      // this lane's rows of the scores: c2 and c2 + 1 of each block of 8
+      int lim[NB][2], lim_min = INT32_MAX;
+      long long p[NB][2];
+      float slope[NB][2];
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, o));
-      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-      float o[DP / 8][4];
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-      for (int n = 0; n < DP / 8; ++n)
+        for (int y = 0; y < 2; ++y) {
+          const int r = r0 + nb * 8 + c2 + y;
+          const bool ok = r < a.rows;
+          const int i = ok ? a.by_g(r) : 0;
+          p[nb][y] = at.seq.p0 + i;
+          lim[nb][y] = ok ? keys_seen(a, at.seq.len, p[nb][y]) : at.seq.len;
+          lim_min = min(lim_min, lim[nb][y]);
+          slope[nb][y] = MODS && a.slopes != nullptr ? a.slopes[kvh * a.G + (ok ? r - i * a.G : 0)] * kLog2e : 0.0f;
+        }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[n][e] = 0.0f;
+      for (int o = 1; o < 4; o <<= 1) lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, o));
+      float m[NB][2], l[NB][2];
+      float o[DP / 16][NB][4];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        m[nb][0] = m[nb][1] = -INFINITY;
+        l[nb][0] = l[nb][1] = 0.0f;
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[s][nb][e] = 0.0f;
+      }
 
-      const int first = at.t, end = at.visible_end();
-      for (int t = first; t < end; ++t) {
-        // S = Q K^T, 8 keys a block of x
-        copy_wait<H - 2>();
-        worker_sync();  // the tile's keys are there, whoever copied them, and all are done with the half before
-        uint32_t valid[kKeys];
+      const int first = at.t, halves = 2 * max(0, at.visible_end() - first);
+      uint32_t valid = 0;
+      float x[KT / 16][NB][4];
+#pragma unroll 1
+      for (int half = 0; half < halves && good; ++half) {  // a tile's keys, then its values
+#pragma unroll 1
+        for (;;) {
+          const bool full = filled == H - 1;
+          if (full) {
+            good = mbar_wait_bounded_warp(&s_full[wk][used], phase, &s_abort, a.ctl, kStatusTimeoutEpilogue);
+            if (!good) break;
+          }
+          if (loads && !issue()) good = false;
+          if (full || !good) break;
+          ++filled;
+        }
+        if (!good) break;
+        const uint32_t half_at = ring_at + used * L::kHalf;
+        if ((half & 1) == 0) {
+          valid = s_valid[wk][used];
+          // S^T = K Q^T, 16 keys a block of x
 #pragma unroll
-        for (int y = 0; y < kKeys; ++y) valid[y] = s_valid[warp][out_half][y];
-        issue_at_keys();
-        float x[KT / 8][4];
+          for (int n = 0; n < KT / 16; ++n)
 #pragma unroll
-        for (int n = 0; n < KT / 8; ++n)
+            for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[n][e] = 0.0f;
-        {
-          const uint32_t ka = ring_at + out_half * L::kHalf + ((lane & 7) + ((lane >> 4) & 1) * 8) * L::kRow + ((lane >> 3) & 1) * 16;
+              for (int e = 0; e < 4; ++e) x[n][nb][e] = 0.0f;
 #pragma unroll
           for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
             for (int n = 0; n < KT / 16; ++n) {
               uint32_t kf[4];
-              ldmatrix_x4(ka + n * 16 * L::kRow + s * 32, kf);
-              mma_bf16(x[2 * n], qf[s], kf[0], kf[1]);
-              mma_bf16(x[2 * n + 1], qf[s], kf[2], kf[3]);
+              ldmatrix_x4(half_at + k_col[s & 3] + (s >> 2) * L::kAtom + n * 2048, kf);
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) mma_bf16(x[n][nb], kf, qf[s][nb][0], qf[s][nb][1]);
             }
-        }
-        out_half = out_half + 1 == H ? 0 : out_half + 1;
-        const int j0 = t * KT;
+          const int j0 = (first + (half >> 1)) * KT;
+          if constexpr (MODS) {
 #pragma unroll
-        for (int n = 0; n < KT / 8; ++n)
+            for (int n = 0; n < KT / 16; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if constexpr (MODS) {
-              x[n][e] = a.cap_out != 0.0f ? capped(x[n][e] * a.cap_in, a.cap_out) : x[n][e] * a.scale_log2;
-              if (a.slopes != nullptr) {
-                const long long j = j0 + n * 8 + c2 + (e & 1);
-                x[n][e] = fmaf(-slope[e >> 1], fabsf(float(p[e >> 1] - j)), x[n][e]);
+              for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  float& s = x[n][nb][e];
+                  s = a.cap_out != 0.0f ? capped(s * a.cap_in, a.cap_out) : s * a.scale_log2;
+                  const long long j = j0 + n * 16 + g + (e >> 1) * 8;
+                  if (a.slopes != nullptr) s = fmaf(-slope[nb][e & 1], fabsf(float(p[nb][e & 1] - j)), s);
+                }
+          }
+          if (j0 + KT > lim_min || valid != (KT < 32 ? (1u << (KT & 31)) - 1u : 0xffffffffu)) {
+#pragma unroll
+            for (int n = 0; n < KT / 16; ++n)
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const int j = n * 16 + g + (e >> 1) * 8;
+                  if (j0 + j >= lim[nb][e & 1] || ((valid >> j) & 1u) == 0) x[n][nb][e] = -INFINITY;
+                }
+          }
+          const float sc = MODS ? 1.0f : a.scale_log2;
+          float top[NB][2];
+          bool moved = false;
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              float& w = top[nb][y];
+              w = fmaxf(x[0][nb][y], x[0][nb][2 + y]);
+#pragma unroll
+              for (int n = 1; n < KT / 16; ++n) w = fmax3(w, x[n][nb][y], x[n][nb][2 + y]);
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, d));
+              w *= sc;
+              moved = moved || w > m[nb][y] + kRescale;
+            }
+          if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+              for (int y = 0; y < 2; ++y) {
+                const float to = top[nb][y] > m[nb][y] + kRescale ? top[nb][y] : m[nb][y];
+                const float f = to == m[nb][y] ? 1.0f : fast_exp2(m[nb][y] - to);
+                m[nb][y] = to;
+                l[nb][y] *= f;
+#pragma unroll
+                for (int s = 0; s < DP / 16; ++s) {
+                  o[s][nb][y] *= f;
+                  o[s][nb][2 + y] *= f;
+                }
               }
-            } else {
-              x[n][e] *= a.scale_log2;
+          }
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const float mu = m[nb][y] == -INFINITY ? 0.0f : m[nb][y];  // nothing seen yet: every weight is 0
+#pragma unroll
+              for (int n = 0; n < KT / 16; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; e += 2) {
+                  float& w = x[n][nb][e + y];
+                  w = fast_exp2(fmaf(w, sc, -mu));
+                  l[nb][y] += w;
+                }
+            }
+        } else {
+          // O^T += V^T P^T; P rounded to bf16 for the tensor core, 2^-8 relative at most, the sum takes the unrounded
+          // weights
+          uint32_t pf[KT / 16][NB][2];
+#pragma unroll
+          for (int n = 0; n < KT / 16; ++n)
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+              pf[n][nb][0] = transposed(pack_bf16x2(x[n][nb][0], x[n][nb][1]));
+              pf[n][nb][1] = transposed(pack_bf16x2(x[n][nb][2], x[n][nb][3]));
+            }
+          const bool all = valid == (KT < 32 ? (1u << (KT & 31)) - 1u : 0xffffffffu);
+#pragma unroll
+          for (int n = 0; n < KT / 16; ++n) {
+            const uint32_t w = valid >> (n * 16 + c2);
+            const uint32_t k0 = (w & 1u ? 0xffffu : 0u) | (w & 2u ? 0xffff0000u : 0u);
+            const uint32_t k1 = (w & 0x100u ? 0xffffu : 0u) | (w & 0x200u ? 0xffff0000u : 0u);
+#pragma unroll
+            for (int s = 0; s < DP / 16; ++s) {
+              uint32_t vf[4];
+              ldmatrix_x4_trans(half_at + v_col[s & 3] + (s >> 2) * L::kAtom + n * 2048, vf);
+              if (!all) {  // slots behind the last key may hold anything: zeros, for 0 times NaN is NaN
+                vf[0] &= k0;
+                vf[1] &= k0;
+                vf[2] &= k1;
+                vf[3] &= k1;
+              }
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) mma_bf16(o[s][nb], vf, pf[n][nb][0], pf[n][nb][1]);
             }
           }
-        bool all = j0 + KT <= lim_min;
-#pragma unroll
-        for (int y = 0; y < kKeys; ++y) all = all && valid[y] == (KT < 32 ? (1u << (KT & 31)) - 1u : 0xffffffffu);
-        if (!all) {
-#pragma unroll
-          for (int n = 0; n < KT / 8; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int j = n * 8 + c2 + (e & 1);
-              if (j0 + j >= lim[e >> 1] || ((valid[n / 4] >> (j & 31)) & 1u) == 0) x[n][e] = -INFINITY;
-            }
         }
-        float top[2];
-        bool moved = false;
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          top[r] = fmaxf(x[0][2 * r], x[0][2 * r + 1]);
-#pragma unroll
-          for (int n = 1; n < KT / 8; ++n) top[r] = fmax3(top[r], x[n][2 * r], x[n][2 * r + 1]);
-          top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-          top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-          moved = moved || top[r] > m[r] + kRescale;
+        __syncwarp();  // all lanes are done with the half
+        if (WR > 1 && lane == 0) mbar_arrive(&s_empty[wk][used]);
+        if (++used == H) {
+          used = 0;
+          phase ^= 1u;
         }
-        if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const float mr = top[r] > m[r] + kRescale ? top[r] : m[r];
-            const float f = mr == m[r] ? 1.0f : fast_exp2(m[r] - mr);
-            m[r] = mr;
-            l[r] *= f;
-#pragma unroll
-            for (int n = 0; n < DP / 8; ++n) {
-              o[n][2 * r] *= f;
-              o[n][2 * r + 1] *= f;
-            }
-          }
-        }
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float mu = m[r] == -INFINITY ? 0.0f : m[r];  // nothing seen yet: every weight is 0
-#pragma unroll
-          for (int n = 0; n < KT / 8; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              x[n][2 * r + e] = fast_exp2(x[n][2 * r + e] - mu);
-              l[r] += x[n][2 * r + e];
-            }
-        }
-        // O += P V; P rounded to bf16 for the tensor core, 2^-8 relative at most, the sum takes the unrounded weights
-        copy_wait<H - 2>();
-        worker_sync();
-        issue_at_values();
-        const uint32_t va = ring_at + out_half * L::kHalf + ((lane & 7) + ((lane >> 3) & 1) * 8) * L::kRow + ((lane >> 4) & 1) * 16;
-#pragma unroll
-        for (int n = 0; n < KT / 16; ++n) {
-          const uint32_t pf[4] = {pack_bf16x2(x[2 * n][0], x[2 * n][1]), pack_bf16x2(x[2 * n][2], x[2 * n][3]),
-                                  pack_bf16x2(x[2 * n + 1][0], x[2 * n + 1][1]),
-                                  pack_bf16x2(x[2 * n + 1][2], x[2 * n + 1][3])};
-#pragma unroll
-          for (int c = 0; c < DP / 16; ++c) {
-            uint32_t vf[4];
-            ldmatrix_x4_trans(va + n * 16 * L::kRow + c * 32, vf);
-            mma_bf16(o[2 * c], pf, vf[0], vf[1]);
-            mma_bf16(o[2 * c + 1], pf, vf[2], vf[3]);
-          }
-        }
-        out_half = out_half + 1 == H ? 0 : out_half + 1;
+        --ahead;
       }
+      if (!good) break;
 
       // ---- the item's rows, or the share's part of them
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-      }
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) l[nb][y] += __shfl_xor_sync(0xffffffffu, l[nb][y], d);
       const bool begins = first == 0, ends = at.t1 == at.tiles, last = at.left <= 0;
       if (begins && ends) {
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const int r = r0 + g + 8 * y;
-          if (r >= a.rows) continue;
-          const float inv = l[y] == 0.0f ? 0.0f : 1.0f / l[y];  // (a NaN sum makes the row NaN)
-          const long long row = out_row(a, at.b, kvh, r);
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-          for (int n = 0; n < DP / 8; ++n) {
-            if (n * 8 >= a.D) break;
-            write_out<2>(a, row, n * 8 + c2, {o[n][2 * y] * inv, o[n][2 * y + 1] * inv});
+          for (int y = 0; y < 2; ++y) {
+            const int r = r0 + nb * 8 + c2 + y;
+            if (r >= a.rows) continue;
+            const float inv = l[nb][y] == 0.0f ? 0.0f : 1.0f / l[nb][y];  // (a NaN sum makes the row NaN)
+            const long long row = out_row(a, at.b, kvh, r) + g;
+#pragma unroll
+            for (int s = 0; s < DP / 16; ++s)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if (s * 16 + e * 8 < a.D) write_out(a, row + s * 16 + e * 8, o[s][nb][2 * e + y] * inv);
           }
-        }
-        if (a.rec_items && role == 0 && lane == 0)
-          a.rec[at.b * (a.Hk * a.row_tiles) + at.rest] = make_int4(0, 0, 0, 0);
       } else {
         // The share's last part waits in the ring, which nobody needs any more; the end of an item before it does not.
-        if (last) worker_sync();
+        if (WR > 1 && last) {  // (once the worker's other warps are done with the half used last)
+          const int before = used == 0 ? H - 1 : used - 1;
+          good = mbar_wait_bounded_warp(&s_empty[wk][before], used == 0 ? phase ^ 1u : phase, &s_abort, a.ctl,
+                                        kStatusTimeoutEpilogue);
+          if (!good) break;
+        }
         float* const dst = last ? reinterpret_cast<float*>(ring)
                                 : a.head_o + ((long long)blockIdx.x * NW + wk) * a.slot_rows * a.D;
-        const int ld_o = last ? DP + 8 : a.D;
+        const int ld_o = last ? DP + 4 : a.D;
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const int r = role * 16 + g + 8 * y;
-          if (r >= a.slot_rows) continue;
-          if (c2 == 0) s_ml[wk][begins][r] = make_float2(m[y], l[y]);
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-          for (int n = 0; n < DP / 8; ++n) {
-            if (n * 8 >= a.D) break;
-            *reinterpret_cast<float2*>(dst + (long long)r * ld_o + n * 8 + c2) = make_float2(o[n][2 * y], o[n][2 * y + 1]);
+          for (int y = 0; y < 2; ++y) {
+            const int r = (role * NB + nb) * 8 + c2 + y;
+            if (r >= a.slot_rows) continue;
+            if (g == 0) s_ml[wk][begins][r] = make_float2(m[nb][y], l[nb][y]);
+#pragma unroll
+            for (int s = 0; s < DP / 16; ++s)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if (s * 16 + e * 8 < a.D) dst[(long long)r * ld_o + s * 16 + e * 8 + g] = o[s][nb][2 * e + y];
           }
-        }
         if (role == 0 && lane == 0)
           s_part[wk][begins] = Part{at.b, at.rest, at.tiles - at.t1, uint8_t(begins), uint8_t(ends), uint8_t(last)};
       }
-    } while (at.next(a, ROWS));
+      if (!at.next(a, ROWS)) break;
+    }
+    if (!good) {  // copies in flight write to this block's memory: it stays until they are done
+      copy_wait_all();
+      if (a.tma && loads)
+        for (; ahead > 0; --ahead) {
+          mbar_wait_drain(&s_full[wk][used], phase, a.ctl);
+          if (++used == H) {
+            used = 0;
+            phase ^= 1u;
+          }
+        }
+    }
   }
   __syncthreads();
 
   // ---- the block's parts, in order of keys: chains of one item each, joined here; what goes on in another block, or came
   // from one, is a part of the block's
   const Part mine_p = lane < 2 * NW ? s_part[lane >> 1][lane & 1] : Part{-1, 0, 0, 0, 0, 0};
-  const uint32_t present = __ballot_sync(0xffffffffu, mine_p.b >= 0);
+  const uint32_t present = s_abort ? 0u : __ballot_sync(0xffffffffu, mine_p.b >= 0);
   const uint32_t starts = (__ballot_sync(0xffffffffu, mine_p.begins) & present) | (present & (0u - present));
-  const int chains = __popc(starts), units = a.slot_rows * (a.D / 4);
-  for (int i = int(threadIdx.x); i < chains * units; i += kWarps * 32) {
-    int c = i / units;
-    const int u = i - c * units, r = u / (a.D / 4), col = (u - r * (a.D / 4)) * 4;
+  if (present == 0) {
+    if (threadIdx.x == 0) a.rec[blockIdx.x] = make_int4(0, 0, 0, 0);
+    return;
+  }
+  // The parts' weights, a thread for each row of each chain: over the sum where the chain is the whole item.
+  for (int i = int(threadIdx.x); i < __popc(starts) * a.slot_rows; i += kWarps * 32) {
+    const int c = a.by_slot_rows(i), r = i - c * a.slot_rows;
     uint32_t rest = starts;
-    for (; c > 0; --c) rest &= rest - 1;
+    for (int k = 0; k < c; ++k) rest &= rest - 1;
     const int z0 = __ffs(int(rest)) - 1;
     rest &= rest - 1;
-    const int z1 = rest != 0 ? __ffs(int(rest)) - 1 : 32;  // the chain's parts are those present in [z0, z1)
-    const uint32_t parts = present & (0xffffffffu << z0) & (z1 < 32 ? (1u << z1) - 1u : 0xffffffffu);
+    const uint32_t parts = present & (0xffffffffu << z0) & (rest != 0 ? (rest & (0u - rest)) - 1u : 0xffffffffu);
     const Part head = s_part[z0 >> 1][z0 & 1];
     const int zl = 31 - __clz(int(parts));
     const Part tail = s_part[zl >> 1][zl & 1];
-    float top = -INFINITY;
+    float top = -INFINITY, sum = 0.0f;
     for (uint32_t w = parts; w != 0; w &= w - 1) {
       const int z = __ffs(int(w)) - 1;
       top = fmaxf(top, s_ml[z >> 1][z & 1][r].x);
     }
-    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f;
     for (uint32_t w = parts; w != 0; w &= w - 1) {
       const int z = __ffs(int(w)) - 1;
-      const float2 ml = s_ml[z >> 1][z & 1][r];
-      const float wt = ml.x == -INFINITY ? 0.0f : fast_exp2(ml.x - top);
-      sum = fmaf(wt, ml.y, sum);
-      const float4 v = s_part[z >> 1][z & 1].in_ring
-                           ? *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + (z >> 1) * L::kRing) +
-                                                              r * (DP + 8) + col)
-                           : *reinterpret_cast<const float4*>(
-                                 a.head_o + (((long long)blockIdx.x * NW + (z >> 1)) * a.slot_rows + r) * a.D + col);
-      acc[0] = fmaf(wt, v.x, acc[0]);
-      acc[1] = fmaf(wt, v.y, acc[1]);
-      acc[2] = fmaf(wt, v.z, acc[2]);
-      acc[3] = fmaf(wt, v.w, acc[3]);
+      float2& ml = s_ml[z >> 1][z & 1][r];
+      ml.x = ml.x == -INFINITY ? 0.0f : fast_exp2(ml.x - top);
+      sum = fmaf(ml.x, ml.y, sum);
     }
-    const int kvh = head.rest / a.row_tiles, row = (head.rest % a.row_tiles) * ROWS + r;
-    if (row < a.rows) {
-      if (head.begins && tail.ends) {
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        write_out<4>(a, out_row(a, head.b, kvh, row), col, {acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv});
-      } else {
-        const long long part = ((long long)blockIdx.x * 2 + head.begins) * a.slot_rows + r;
-        if (col == 0) a.part_ml[part] = make_float2(top, sum);
-        *reinterpret_cast<float4*>(a.part_o + part * a.D + col) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    if (head.begins && tail.ends) {
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      for (uint32_t w = parts; w != 0; w &= w - 1) {
+        const int z = __ffs(int(w)) - 1;
+        s_ml[z >> 1][z & 1][r].x *= inv;
+      }
+    } else {
+      a.part_ml[((long long)blockIdx.x * 2 + head.begins) * a.slot_rows + r] = make_float2(top, sum);
+      if (r == 0 && head.begins)  // (only the last chain goes on in another block)
+        s_rec = make_int4(head.b, head.rest, int(divide(c0 + run + tail.rem - 1, span)) - int(blockIdx.x) + 1, 0);
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) a.rec[blockIdx.x] = s_rec;
+  for (int r = warp; r < a.slot_rows; r += kWarps)
+    for (int col = lane * 4; col < a.D; col += 128) {
+      float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      int begins = 0;
+      for (uint32_t w = present; w != 0; w &= w - 1) {
+        const int z = __ffs(int(w)) - 1;
+        const Part part = s_part[z >> 1][z & 1];
+        const float wt = s_ml[z >> 1][z & 1][r].x;
+        const float4 v = *reinterpret_cast<const float4*>(
+            part.in_ring ? reinterpret_cast<const float*>(smem + (z >> 1) * L::kRing) + r * (DP + 4) + col
+                         : a.head_o + (((long long)blockIdx.x * NW + (z >> 1)) * a.slot_rows + r) * a.D + col);
+        if ((starts >> z) & 1u) {
+          begins = part.begins;
+          acc[0] = wt * v.x, acc[1] = wt * v.y, acc[2] = wt * v.z, acc[3] = wt * v.w;
+        } else {
+          acc[0] = fmaf(wt, v.x, acc[0]);
+          acc[1] = fmaf(wt, v.y, acc[1]);
+          acc[2] = fmaf(wt, v.z, acc[2]);
+          acc[3] = fmaf(wt, v.w, acc[3]);
+        }
+        const uint32_t behind = w & (w - 1);
+        if (behind != 0 && (starts & behind & (0u - behind)) == 0) continue;  // the chain goes on
+        const int kvh = a.by_row_tiles(part.rest), row = (part.rest - kvh * a.row_tiles) * ROWS + r;
+        if (row >= a.rows) continue;
+        if (begins && part.ends)
+          write_out4(a, out_row(a, part.b, kvh, row) + col, acc);
+        else
+          *reinterpret_cast<float4*>(a.part_o + (((long long)blockIdx.x * 2 + begins) * a.slot_rows + r) * a.D + col) =
+              make_float4(acc[0], acc[1], acc[2], acc[3]);
       }
     }
-    if (u == 0 && head.begins) {
-      const int4 mine_rec =
-          tail.ends ? make_int4(0, 0, 0, 0)
-                    : make_int4(head.b, head.rest, int(divide(c0 + run + tail.rem - 1, span)) - int(blockIdx.x) + 1,
-                                int(blockIdx.x));
-      if (a.rec_items)
-        a.rec[head.b * (a.Hk * a.row_tiles) + head.rest] = mine_rec;
-      else if (!tail.ends)
-        a.rec[blockIdx.x] = mine_rec;
-    }
-  }
-  // The block begins no item that goes on behind it: its record says so.
-  if (!a.rec_items && threadIdx.x == 0) {
-    const int zl = present != 0 ? 31 - __clz(int(present)) : 0;
-    const Part tail = s_part[zl >> 1][zl & 1];
-    const uint32_t z0 = starts != 0 ? 31 - __clz(int(starts)) : 0;  // the last chain's first part
-    if (present == 0 || tail.ends || !s_part[z0 >> 1][z0 & 1].begins) a.rec[blockIdx.x] = make_int4(0, 0, 0, 0);
-  }
 }
 
-// Joins the parts of the item of record blockIdx.x. Eight warps take the parts in turn, a lane 4 (8 above 128) columns.
-__global__ void __launch_bounds__(kJoinWarps * 32) attention_paged_join_kernel(const PagedArgs a, int row_tile) {
+// Joins the parts of the items that go on from block to block, a row of one at a time: eight warps take the parts in turn, a
+// lane 4 (8 above 128) columns. A block looks through all records for the rows that are its own.
+__global__ void __launch_bounds__(kJoinWarps * 32) attention_paged_join_kernel(const PagedArgs a, int recs, int row_tile) {
   __shared__ float s_acc[kJoinWarps][256];
   __shared__ float s_inv;
+  __shared__ int s_list[kJoinMaxRecs], s_count[kJoinWarps];
   const int lane = int(threadIdx.x) & 31, warp = int(threadIdx.x) >> 5;
   pdl_wait();
   pdl_launch_dependents();
-  const int4 rec = a.rec[blockIdx.x];
-  const int parts = rec.z, blk = rec.w;
-  if (parts == 0) return;
-  const int kvh = rec.y / a.row_tiles, r0 = (rec.y % a.row_tiles) * row_tile;
-  const int rows = min(a.rows - r0, row_tile);
-  const auto part_row = [&](int z) { return ((long long)(blk + z) * 2 + (z == 0)) * a.slot_rows; };
-  for (int row = int(blockIdx.y); row < rows; row += int(gridDim.y)) {
+  int items = 0;
+  for (int i0 = 0; i0 < recs; i0 += kJoinWarps * 32) {  // the records with something to join, in order
+    const int i = i0 + int(threadIdx.x);
+    const bool some = i < recs && a.rec[i].z != 0;
+    const unsigned mask = __ballot_sync(0xffffffffu, some);
+    if (lane == 0) s_count[warp] = __popc(mask);
+    __syncthreads();
+    int before = items;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) {
+      before += w < warp ? s_count[w] : 0;
+      items += s_count[w];
+    }
+    if (some) s_list[before + __popc(mask & ((1u << lane) - 1u))] = i;
+    __syncthreads();
+  }
+  for (int task = int(blockIdx.x); task < items * a.slot_rows; task += int(gridDim.x)) {
+    const int item = a.by_slot_rows(task), row = task - item * a.slot_rows;
+    const int blk = s_list[item];
+    const int4 rec = a.rec[blk];
+    const int parts = rec.z;
+    const int kvh = a.by_row_tiles(rec.y), r = (rec.y - kvh * a.row_tiles) * row_tile + row;
+    if (r >= a.rows) continue;
+    const auto part_row = [&](int z) { return ((long long)(blk + z) * 2 + (z == 0)) * a.slot_rows + row; };
     float top = -INFINITY;
-    for (int z = lane; z < parts; z += 32) top = fmaxf(top, a.part_ml[part_row(z) + row].x);
+    for (int z = lane; z < parts; z += 32) top = fmaxf(top, a.part_ml[part_row(z)].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     float sum = 0.0f;
     if (warp == 0) {
       for (int z = lane; z < parts; z += 32) {
-        const float2 ml = a.part_ml[part_row(z) + row];
+        const float2 ml = a.part_ml[part_row(z)];
         sum = fmaf(ml.x == -INFINITY ? 0.0f : fast_exp2(ml.x - top), ml.y, sum);
       }
 #pragma unroll
@@ -694,8 +825,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_paged_join_kernel(c
       if (lane == 0) s_inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     }
     float acc[2][4] = {};
+#pragma unroll 4
     for (int z = warp; z < parts; z += kJoinWarps) {
-      const long long at = part_row(z) + row;
+      const long long at = part_row(z);
       const float mz = a.part_ml[at].x;
       const float wt = mz == -INFINITY ? 0.0f : fast_exp2(mz - top);
 #pragma unroll
@@ -720,12 +852,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_paged_join_kernel(c
       float x = 0.0f;
 #pragma unroll
       for (int k = 0; k < kJoinWarps; ++k) x += s_acc[k][col];
-      x *= s_inv;
-      const long long at = out_row(a, rec.x, kvh, r0 + row) + col;
-      if (a.out_f32)
-        static_cast<float*>(a.out)[at] = x;
-      else
-        static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(x);
+      write_out(a, out_row(a, rec.x, kvh, r) + col, x * s_inv);
     }
     __syncthreads();  // s_acc and s_inv are written again for the next row
   }
@@ -735,7 +862,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_paged_join_kernel(c
 // Host side
 // ---------------------------------------------------------------------------------------------------------------
 struct PagedPlan {
-  int wr, blocks;
+  int wr, nb, blocks;
   int64_t rows, row_tiles, slot_rows;
   size_t ml_offset, o_offset, head_offset, bytes;
 };
@@ -756,11 +883,13 @@ int check_paged_sizes(int64_t H, int64_t Hk, int64_t Sq, int64_t D) {
 PagedPlan plan_paged(int64_t H, int64_t Hk, int64_t Sq, int64_t D, int sms) {
   PagedPlan p;
   p.rows = H / Hk * Sq;
-  // The scores of 64 keys next to O and Q of more than 128 columns do not fit a thread's registers.
+  p.nb = p.rows <= 8 ? 1 : 2;
+  // (four warps' rows share keys up to 128 columns only: above, two blocks of them fit an SM no more)
   p.wr = p.rows <= 16 ? 1 : p.rows <= 32 || D > 128 ? 2 : 4;
-  p.row_tiles = (p.rows + 16 * p.wr - 1) / (16 * p.wr);
-  p.slot_rows = p.rows < 16 * p.wr ? p.rows : 16 * p.wr;
-  p.blocks = sms;
+  const int64_t tile = 8 * p.nb * p.wr;
+  p.row_tiles = (p.rows + tile - 1) / tile;
+  p.slot_rows = p.rows < tile ? p.rows : tile;
+  p.blocks = sms * kBlocks * kWaves;
   const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   const size_t row = size_t(p.slot_rows) * size_t(D) * sizeof(float);
   p.ml_offset = up(size_t(p.blocks) * sizeof(int4));
@@ -770,40 +899,44 @@ PagedPlan plan_paged(int64_t H, int64_t Hk, int64_t Sq, int64_t D, int sms) {
   return p;
 }
 
-template <int DP, int WR, bool MODS>
-int launch_paged(const PagedArgs& a, int blocks, cudaStream_t stream, int device) {
-  using L = PagedLayout<DP, WR>;
+template <int DP, int WR, int NB, bool MODS>
+int launch_paged(const CUtensorMap& mk, const CUtensorMap& mv, const PagedArgs& a, int blocks, cudaStream_t stream,
+                 int device) {
+  constexpr int smem = PagedLayout<DP, WR, NB>::kSmem;
   static std::atomic<bool> ready[64] = {};
   if (!ready[device]) {
-    if (int rc = check_cuda(cudaFuncSetAttribute(attention_paged_kernel<DP, WR, MODS>,
-                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem),
+    if (int rc = check_cuda(cudaFuncSetAttribute(attention_paged_kernel<DP, WR, NB, MODS>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
                             "paged attention shared memory"))
       return rc;
     ready[device] = true;
   }
-  return check_cuda(launch_pdl(attention_paged_kernel<DP, WR, MODS>, dim3(unsigned(blocks)), dim3(kWarps * 32), L::kSmem,
-                               stream, a),
+  return check_cuda(launch_pdl(attention_paged_kernel<DP, WR, NB, MODS>, dim3(unsigned(blocks)), dim3(kWarps * 32), smem,
+                               stream, mk, mv, a),
                     "paged attention kernel launch");
 }
 
-template <int WR, bool MODS>
-int launch_paged_dim(const PagedArgs& a, int blocks, cudaStream_t stream, int device) {
-  if (a.D <= 64) return launch_paged<64, WR, MODS>(a, blocks, stream, device);
-  if (a.D <= 96) return launch_paged<96, WR, MODS>(a, blocks, stream, device);
-  if (a.D <= 128) return launch_paged<128, WR, MODS>(a, blocks, stream, device);
+template <int WR, int NB, bool MODS>
+int launch_paged_dim(const CUtensorMap& mk, const CUtensorMap& mv, const PagedArgs& a, int blocks, cudaStream_t stream,
+                     int device) {
+  if (a.D <= 64) return launch_paged<64, WR, NB, MODS>(mk, mv, a, blocks, stream, device);
+  if (a.D <= 96) return launch_paged<96, WR, NB, MODS>(mk, mv, a, blocks, stream, device);
+  if (a.D <= 128) return launch_paged<128, WR, NB, MODS>(mk, mv, a, blocks, stream, device);
   if constexpr (WR <= 2) {
-    if (a.D <= 160) return launch_paged<160, WR, MODS>(a, blocks, stream, device);
-    if (a.D <= 192) return launch_paged<192, WR, MODS>(a, blocks, stream, device);
-    return launch_paged<256, WR, MODS>(a, blocks, stream, device);
+    if (a.D <= 160) return launch_paged<160, WR, NB, MODS>(mk, mv, a, blocks, stream, device);
+    if (a.D <= 192) return launch_paged<192, WR, NB, MODS>(mk, mv, a, blocks, stream, device);
+    return launch_paged<256, WR, NB, MODS>(mk, mv, a, blocks, stream, device);
   }
   return fail(kErrUnsupported, "paged attention: no kernel for these rows");  // (plan_paged asks for none)
 }
 
 template <bool MODS>
-int launch_paged_for(const PagedArgs& a, int wr, int blocks, cudaStream_t stream, int device) {
-  if (wr == 1) return launch_paged_dim<1, MODS>(a, blocks, stream, device);
-  if (wr == 2) return launch_paged_dim<2, MODS>(a, blocks, stream, device);
-  return launch_paged_dim<4, MODS>(a, blocks, stream, device);
+int launch_paged_for(const CUtensorMap& mk, const CUtensorMap& mv, const PagedArgs& a, const PagedPlan& p,
+                     cudaStream_t stream, int device) {
+  if (p.nb == 1) return launch_paged_dim<1, 1, MODS>(mk, mv, a, p.blocks, stream, device);
+  if (p.wr == 1) return launch_paged_dim<1, 2, MODS>(mk, mv, a, p.blocks, stream, device);
+  if (p.wr == 2) return launch_paged_dim<2, 2, MODS>(mk, mv, a, p.blocks, stream, device);
+  return launch_paged_dim<4, 2, MODS>(mk, mv, a, p.blocks, stream, device);
 }
 
 }  // namespace
@@ -850,6 +983,7 @@ int attention_paged_launch(const AttnPagedProblem& p, cudaStream_t stream) {
   if (reinterpret_cast<uintptr_t>(p.out) % uintptr_t(esize)) return fail(kErrInvalid, "paged attention: out is misaligned");
   const DeviceInfo* dev = nullptr;
   if (int rc = current_device_info(&dev)) return rc;
+  if (dev->sms > 160) return fail(kErrUnsupported, "paged attention: more than 160 SMs");
   const PagedPlan plan = plan_paged(p.heads, c.kv_heads, p.sq, c.head_dim, dev->sms);
   if (p.workspace == nullptr || p.workspace_bytes < plan.bytes)
     return fail(kErrInvalid, "paged attention needs a %zu-byte workspace, got %zu", plan.bytes, p.workspace_bytes);
@@ -873,9 +1007,9 @@ int attention_paged_launch(const AttnPagedProblem& p, cudaStream_t stream) {
   a.out = p.out;
   a.o_sb = p.o_sb, a.o_ss = p.o_ss, a.o_sh = p.o_sh;
   a.out_f32 = p.out_dtype == NPUB200_DTYPE_F32;
-  const uintptr_t out_align = reinterpret_cast<uintptr_t>(p.out) | uintptr_t(p.o_sb * esize) | uintptr_t(p.o_ss * esize) |
-                              uintptr_t(p.o_sh * esize);
-  a.out_vec = out_align % uintptr_t(4 * esize) == 0 ? 2 : out_align % uintptr_t(2 * esize) == 0 ? 1 : 0;
+  a.out_vec = ((reinterpret_cast<uintptr_t>(p.out) | uintptr_t(p.o_sb * esize) | uintptr_t(p.o_ss * esize) |
+                uintptr_t(p.o_sh * esize)) &
+               uintptr_t(4 * esize - 1)) == 0;
   a.B = int(p.batch);
   a.Hk = int(c.kv_heads);
   a.G = int(p.heads / c.kv_heads);
@@ -889,22 +1023,44 @@ int attention_paged_launch(const AttnPagedProblem& p, cudaStream_t stream) {
   a.rows = int(plan.rows);
   a.row_tiles = int(plan.row_tiles);
   a.slot_rows = int(plan.slot_rows);
+  a.by_page = divisor(c.page_size);
+  a.by_g = divisor(a.G);
+  a.by_row_tiles = divisor(a.row_tiles);
+  a.by_slot_rows = divisor(a.slot_rows);
   a.min_span = p.variant > 0 ? p.variant : 8;
-  const int64_t items = p.batch * c.kv_heads * plan.row_tiles;
-  a.rec_items = items <= plan.blocks;
+  a.per_block = 1.0f / float(plan.blocks);
   uint8_t* ws = static_cast<uint8_t*>(p.workspace);
   a.rec = reinterpret_cast<int4*>(ws);
   a.part_ml = reinterpret_cast<float2*>(ws + plan.ml_offset);
   a.part_o = reinterpret_cast<float*>(ws + plan.o_offset);
   a.head_o = reinterpret_cast<float*>(ws + plan.head_offset);
+  a.ctl.status = dev->status;
+  a.ctl.timeout_ns = wait_timeout_ns();
+  a.ctl.debug = p.debug;
+  // TMA takes 16 slots of a page at a time, and maps of positive strides below 2^40 bytes.
+  CUtensorMap mk, mv;
+  memset(&mk, 0, sizeof(mk));
+  memset(&mv, 0, sizeof(mv));
+  const auto strided = [&](int64_t sp, int64_t ss, int64_t sh) {
+    const auto fits = [](int64_t n, int64_t s) { return n == 1 || (s > 0 && s < (int64_t(1) << 38)); };
+    return fits(c.pages, sp) && fits(c.page_size, ss) && fits(c.kv_heads, sh);
+  };
+  a.tma = c.page_size % 16 == 0 && c.pages > 0 && strided(c.k_sp, c.k_ss, c.k_sh) && strided(c.v_sp, c.v_ss, c.v_sh);
+  if (a.tma) {
+    if (int rc = encode_bshd_map(c.k, c.head_dim, c.page_size, c.kv_heads, c.pages, c.k_ss, c.k_sh, c.k_sp, 16, &mk, &a.pk))
+      return rc;
+    if (int rc = encode_bshd_map(c.v, c.head_dim, c.page_size, c.kv_heads, c.pages, c.v_ss, c.v_sh, c.v_sp, 16, &mv, &a.pv))
+      return rc;
+  }
   const bool mods = p.softcap > 0.0f || p.slopes != nullptr;
-  if (int rc = mods ? launch_paged_for<true>(a, plan.wr, plan.blocks, stream, dev->device)
-                    : launch_paged_for<false>(a, plan.wr, plan.blocks, stream, dev->device))
+  if (int rc = mods ? launch_paged_for<true>(mk, mv, a, plan, stream, dev->device)
+                    : launch_paged_for<false>(mk, mv, a, plan, stream, dev->device))
     return rc;
-  // A block joins one row of an item, or all of them when there are items enough to fill the GPU.
-  const int64_t split = items >= dev->sms ? 1 : plan.slot_rows;
-  return check_cuda(launch_pdl(attention_paged_join_kernel, dim3(unsigned(std::min<int64_t>(items, plan.blocks)), unsigned(split)),
-                               dim3(kJoinWarps * 32), 0, stream, a, 16 * plan.wr),
+  // As many rows can be left to join as items begin, one a block at most.
+  const int64_t items = std::min<int64_t>(p.batch * c.kv_heads * plan.row_tiles, plan.blocks);
+  static_assert(kBlocks * kWaves * 160 <= kJoinMaxRecs, "records of the join kernel");
+  return check_cuda(launch_pdl(attention_paged_join_kernel, dim3(unsigned(std::min<int64_t>(items * plan.slot_rows, dev->sms))),
+                               dim3(kJoinWarps * 32), 0, stream, a, plan.blocks, 8 * plan.nb * plan.wr),
                     "paged attention join kernel launch");
 }
 

@@ -549,7 +549,7 @@ int npub200_attention_paged(const void* q, int64_t q_sb, int64_t q_ss, int64_t q
                             void* stream) {
   const AttnPagedProblem p = {q,     q_sb,   q_ss,     q_sh,    cache,  kv_lens,   out,             o_sb,
                               o_ss,  o_sh,   out_dtype, batch,  heads,  sq,        scale,           causal,
-                              q_starts, softcap, slopes, workspace, workspace_bytes, variant};
+                              q_starts, softcap, slopes, workspace, workspace_bytes, variant, g_debug_flags.load()};
   return attention_paged_launch(p, static_cast<cudaStream_t>(stream));
 }
 

@@ -237,6 +237,7 @@ struct AttnPagedProblem {
   void* workspace;
   size_t workspace_bytes;
   int variant;
+  uint32_t debug;
 };
 int attention_paged_launch(const AttnPagedProblem& p, cudaStream_t stream);
 int attention_paged_workspace(int64_t heads, int64_t kv_heads, int64_t sq, int64_t head_dim, size_t* bytes);

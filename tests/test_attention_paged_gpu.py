@@ -283,6 +283,25 @@ def test_graphs_follow_the_lengths(cuda_device):
     kernels.check_status(d)
 
 
+@pytest.mark.parametrize("page", [16, 7])
+@pytest.mark.parametrize("H,Sq", [(4, 1), (4, 8), (4, 16), (4, 40)])
+def test_forced_timeout_reports_and_recovers(cuda_device, H, Sq, page):
+    from npu_ai_b200 import kernels
+    c = Cache(cuda_device, [500, 40], 2, 64, page)
+    q = torch.zeros(2, Sq, H * 64, dtype=BF16, device=cuda_device)
+    kernels.status(cuda_device)
+    kernels.set_wait_timeout_ns(2_000_000)
+    kernels.set_debug_flags(1)
+    try:
+        kernels.paged_attention(q, c.k, c.v, c.table, c.lens, H)
+        with pytest.raises(RuntimeError, match="failure status"):
+            kernels.check_status(cuda_device)
+    finally:
+        kernels.set_debug_flags(0)
+        kernels.set_wait_timeout_ns(0)
+    run(cuda_device, None, H, 2, 64, page, Sq=Sq, cache=c)
+
+
 def test_c_entry_and_its_workspace(cuda_device):
     """Straight through the C ABI, with a workspace of garbage; one that is too small, missing or misaligned is refused."""
     from npu_ai_b200 import _lib, kernels
