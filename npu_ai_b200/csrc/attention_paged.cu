@@ -11,8 +11,8 @@
 //   * Keys are the rows of the matrix instructions: S^T = K Q^T and O^T = V^T P^T with mma.sync m16n8k16, 16 keys (16
 //     columns of the head) against 8 rows of queries. The rows of a (sequence, key/value head) are its G heads x the new
 //     tokens, mostly 8 or fewer, so nothing is padded to the 64 or 128 rows of a tcgen05 tile, and the softmax of a tile
-//     stays in one warp's registers without round trips through TMEM and shared memory. A warp takes one or two such blocks
-//     of 8 rows; more rows share the keys of one load among the 2 or 4 warps of a worker.
+//     stays in one warp's registers without round trips through TMEM and shared memory. More rows share the keys of one
+//     load among the 2 or 4 warps of a worker.
 //   * Every block takes an equal run of tiles of the whole batch, found on the device from kv_lens, so ragged lengths leave
 //     no SM idle and a captured graph follows them, and its workers equal shares of it. Shares start and end anywhere in a
 //     sequence; the parts of a row's keys are joined in order of keys, first those of a block through its shared memory,
@@ -27,6 +27,7 @@
 #include <cfloat>
 #include <cmath>
 #include <cstring>
+#include <type_traits>
 
 #include "attention_sm100.cuh"
 #include "internal.h"
@@ -66,7 +67,7 @@ struct PagedArgs {
   const __nv_bfloat16* v;
   long long v_sp, v_ss, v_sh;
   MapPos pk, pv;  // where the slot, head and page are among the coordinates of the tensor maps
-  int tma;        // 1: the maps are there
+  int box_rows;   // slots of a box: a whole tile's where the page is a multiple of it, else 16
   const int32_t* table;
   long long table_stride;
   int pages, page_size, capacity;
@@ -131,15 +132,15 @@ __device__ __forceinline__ void copy_arrive(uint64_t* bar) {
 }
 __device__ __forceinline__ void copy_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// Layout for head dims up to DP, workers of WR warps and NB blocks of 8 rows a warp.
-template <int DP, int WR, int NB>
+// Layout for head dims up to DP and workers of WR warps, 8 rows a warp.
+template <int DP, int WR>
 struct PagedLayout {
   static constexpr int kAtoms = (DP + 63) / 64;           // 128-byte columns of a row
   static constexpr int kTile = DP <= 128 ? 32 : 16;       // keys of a tile
   static constexpr int kAtom = kTile * 128;               // bytes of one column of the keys (values) of a tile
   static constexpr int kHalf = kAtoms * kAtom;
   static constexpr int kWorkers = kWarps / WR;
-  static constexpr int kRows = 8 * NB * WR;
+  static constexpr int kRows = 8 * WR;
   // As many as half an SM holds next to the static tables: up to 130 KB in flight on the SM, of which some 40 KB cover the
   // latency at the full rate.
   static constexpr int kFit = 104 * 1024 / (kWorkers * kHalf);
@@ -254,18 +255,118 @@ struct Part {
   uint8_t begins, ends, in_ring;  // holds the item's first tile, its last; where its O rows are
 };
 
-template <int DP, int WR, int NB, bool MODS>
-__global__ void __launch_bounds__(kWarps * 32, kBlocks)
+// A worker's share of tiles, as its warps hand it to the one that loads.
+struct Share {
+  int b, rest, t;
+  long long tiles;
+};
+
+// The loads of a block by TMA: one warp, a lane for each worker, H halves ahead of it. Boxes of 64 columns and box_rows slots;
+// a page that is not there is outside the map, which reads as zeros. (The warps that use the tiles spent 480 cycles on each
+// half where they issued the loads themselves, as much as on its arithmetic.)
+template <typename L, int WR>
+__device__ __forceinline__ void load_pages(const PagedArgs& a, const CUtensorMap* map_k, const CUtensorMap* map_v,
+                                           const Share* shares, uint8_t* smem, uint64_t (*full)[L::kHalves],
+                                           uint64_t (*empty)[L::kHalves], uint32_t (*valid)[L::kHalves], int* abort) {
+  constexpr int KT = L::kTile, H = L::kHalves;
+  const int lane = int(threadIdx.x) & 31;
+  Cursor<KT> ld = {};
+  bool more = lane < L::kWorkers && shares[lane].tiles > 0;
+  int end = 0, t = 0, head = 0, seen = 0, page[KT / 16];
+  const auto peek = [&]() {  // takes the next tile with keys, if any, and has its pages looked up
+    while (ld.t >= end) {
+      if (!ld.next(a, L::kRows)) {
+        more = false;
+        return;
+      }
+      end = ld.visible_end();
+    }
+    t = ld.t++;
+    head = a.by_row_tiles(ld.rest);
+    seen = ld.seen;
+    const int32_t* const row = a.table + ld.b * a.table_stride;
+#pragma unroll
+    for (int i = 0; i < KT / 16; ++i) page[i] = t * KT + i * 16 < seen ? row[a.by_page(t * KT + i * 16)] : -1;
+  };
+  if (more) {
+    ld.b = shares[lane].b;
+    ld.rest = shares[lane].rest;
+    ld.enter(a, L::kRows, shares[lane].t, shares[lane].tiles);
+    end = ld.visible_end();
+    peek();
+  }
+  int in = 0, in_values = 0, issued = 0;
+  uint32_t phase = 0;
+  uint64_t since = globaltimer_ns();
+  uint32_t polls = 0;
+  while (__any_sync(0xffffffffu, more)) {
+    const bool ready = more && (issued < H || mbar_test_wait(&empty[lane][in], phase ^ 1u));
+    if (ready) {
+      uint64_t* const bar = &full[lane][in];
+      uint32_t bits = 0;
+      int c[KT / 16][3];
+      const int slot0 = t * KT - a.by_page(t * KT) * a.page_size;
+      const MapPos& pos = in_values ? a.pv : a.pk;
+#pragma unroll
+      for (int i = 0; i < KT / 16; ++i) {
+        const bool ok = page[i] >= 0 && page[i] < a.pages;
+        const int n = min(16, seen - t * KT - i * 16);  // (no page was looked up where there is no key)
+        bits |= ok ? ((1u << n) - 1u) << (16 * i) : 0u;
+        int slot = slot0 + 16 * i;
+        slot -= slot >= a.page_size ? a.by_page(slot) * a.page_size : 0;
+        const int at = ok ? page[i] : a.pages;
+        c[i][0] = pos.s == 1 ? slot : pos.h == 1 ? head : at;
+        c[i][1] = pos.s == 2 ? slot : pos.h == 2 ? head : at;
+        c[i][2] = pos.s == 3 ? slot : pos.h == 3 ? head : at;
+      }
+      valid[lane][in] = bits;
+      mbar_arrive_expect_tx(bar, L::kHalf);
+      uint8_t* const dst = smem + lane * L::kRing + in * L::kHalf;
+#pragma unroll
+      for (int i = 0; i < KT / 16; ++i)
+        if (i % (a.box_rows / 16) == 0)
+#pragma unroll
+          for (int k = 0; k < L::kAtoms; ++k)
+            tma_load_4d(in_values ? map_v : map_k, bar, dst + k * L::kAtom + i * 2048, k * 64, c[i][0], c[i][1], c[i][2]);
+      ++issued;
+      if (++in == H) {
+        in = 0;
+        phase ^= 1u;
+      }
+      if (in_values) peek();
+      in_values ^= 1;
+    }
+    if (__any_sync(0xffffffffu, ready)) {
+      polls = 0;
+    } else if ((++polls & 63u) == 0) {
+      if (polls == 64) since = globaltimer_ns();
+      const bool late = globaltimer_ns() - since > a.ctl.timeout_ns;
+      if (late && lane == 0) atomicOr(a.ctl.status, kStatusTimeoutProducer);
+      if (late) *reinterpret_cast<volatile int*>(abort) = 1;
+      if (__any_sync(0xffffffffu, late || *reinterpret_cast<volatile int*>(abort))) break;
+    }
+  }
+  // The copies in flight write to this block's memory: it stays until they are done, whether they are used or not (the others
+  // may have given up).
+  for (int i = 0; i < min(issued, H); ++i) {
+    in = in == 0 ? H - 1 : in - 1;
+    phase ^= in == H - 1 ? 1u : 0u;
+    mbar_wait_drain(&full[lane][in], phase, a.ctl);
+  }
+}
+
+template <int DP, int WR, bool MODS, bool TMA>
+__global__ void __launch_bounds__(kWarps * 32 + (TMA ? 32 : 0), kBlocks)
     attention_paged_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                            const PagedArgs a) {
-  using L = PagedLayout<DP, WR, NB>;
+  using L = PagedLayout<DP, WR>;
   constexpr int KT = L::kTile, H = L::kHalves, NW = L::kWorkers, ROWS = L::kRows;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t s_full[NW][H], s_empty[NW][H], s_never;
   __shared__ uint32_t s_valid[NW][H];      // which keys of a tile are there
+  __shared__ Share s_share[NW];
   __shared__ Part s_part[NW][2];           // parts to join: of the item a share continues, of the one it begins
-  __shared__ float2 s_ml[NW][2][ROWS];     // (m, l) of their rows, later (weight, l)
-  __shared__ int4 s_rec;
+  __shared__ float2 s_ml[NW][2][ROWS];     // (m, l) of their rows
   __shared__ int s_abort;
   const int lane = int(threadIdx.x) & 31, warp = int(threadIdx.x) >> 5;
   const int role = warp % WR, wk = warp / WR;  // this warp's rows of its worker's
@@ -275,12 +376,11 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocks)
   if (threadIdx.x < NW * H) {
     // A tile's half is there when its copies are: TMA's bytes, or the copies of each lane, and the word of the lane that
     // says which keys are valid.
-    mbar_init(&s_full[0][threadIdx.x], a.tma ? 1u : 32u * WR + 1u);
+    mbar_init(&s_full[0][threadIdx.x], TMA ? 1u : 32u * WR + 1u);
     mbar_init(&s_empty[0][threadIdx.x], WR);
   }
   if (threadIdx.x < 2 * NW) s_part[threadIdx.x >> 1][threadIdx.x & 1].b = -1;
   if (threadIdx.x == 0) {
-    s_rec = make_int4(0, 0, 0, 0);
     s_abort = 0;
     mbar_init(&s_never, 1);
     fence_barrier_init();
@@ -301,57 +401,61 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocks)
     }
     return upto;
   };
-  int mine;
-  int upto = scan(0, mine);
-  long long total = __shfl_sync(0xffffffffu, upto, 31);
-  if (a.B > 32) {
-    long long more = 0;
-    for (int b = 32 + lane; b < a.B; b += 32) more += tiles_of<KT>(sequence_len(a, b));
+  long long span = 0, c0 = 0, run = 0;
+  if (TMA && warp == kWarps) {
+    __syncthreads();
+    load_pages<L, WR>(a, &map_k, &map_v, s_share, smem, s_full, s_empty, s_valid, &s_abort);
+  } else {
+    int mine;
+    int upto = scan(0, mine);
+    long long total = __shfl_sync(0xffffffffu, upto, 31);
+    if (a.B > 32) {
+      long long more = 0;
+      for (int b = 32 + lane; b < a.B; b += 32) more += tiles_of<KT>(sequence_len(a, b));
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) more += __shfl_xor_sync(0xffffffffu, more, o);
-    total += more;
-  }
-  total *= per_tile;
-  // (a f32 product is off by less than 1 / blocks below 2^20 tiles: one more than its whole part is never short)
-  const long long span =
-      max(total < (1 << 20) ? (long long)(float(int(total)) * a.per_block) + 1 : (total + gridDim.x - 1) / gridDim.x,
-          (long long)a.min_span);
-  const long long c0 = blockIdx.x * span, run = max(0ll, min(total, c0 + span) - c0);
-  const long long u0 = c0 + run * wk / NW, u1 = c0 + run * (wk + 1) / NW;
-  if (u0 < u1) {
-    Cursor<KT> at;
-    long long base = 0;
-    for (int c = 0;;) {
-      const unsigned hit = __ballot_sync(0xffffffffu, base + upto * per_tile > u0);
-      if (hit != 0) {
-        const int f = __ffs(int(hit)) - 1;
-        at.b = c + f;
-        base += __shfl_sync(0xffffffffu, upto - mine, f) * per_tile;
-        break;
-      }
-      base += __shfl_sync(0xffffffffu, upto, 31) * per_tile;
-      c += 32;
-      upto = scan(c, mine);
+      for (int o = 16; o > 0; o >>= 1) more += __shfl_xor_sync(0xffffffffu, more, o);
+      total += more;
     }
-    const int tiles0 = tiles_of<KT>(sequence_len(a, at.b));
-    at.rest = int(divide(u0 - base, tiles0));
-    at.enter(a, ROWS, int((u0 - base) - (long long)at.rest * tiles0), u1 - u0);
-
-    // ---- the loader, H - 1 halves ahead: by TMA the worker's first warp, else all of its warps a share each. A lane looks
-    // up the page of its key.
+    total *= per_tile;
+    // (a f32 product is off by less than 1 / blocks below 2^20 tiles: one more than its whole part is never short)
+    span = max(total < (1 << 20) ? (long long)(float(int(total)) * a.per_block) + 1 : (total + gridDim.x - 1) / gridDim.x,
+               (long long)a.min_span);
+    c0 = blockIdx.x * span;
+    run = max(0ll, min(total, c0 + span) - c0);
+    const long long u0 = c0 + run * wk / NW, u1 = c0 + run * (wk + 1) / NW;
+    Cursor<KT> at = {};
+    if (u0 < u1) {
+      long long base = 0;
+      for (int c = 0;;) {
+        const unsigned hit = __ballot_sync(0xffffffffu, base + upto * per_tile > u0);
+        if (hit != 0) {
+          const int f = __ffs(int(hit)) - 1;
+          at.b = c + f;
+          base += __shfl_sync(0xffffffffu, upto - mine, f) * per_tile;
+          break;
+        }
+        base += __shfl_sync(0xffffffffu, upto, 31) * per_tile;
+        c += 32;
+        upto = scan(c, mine);
+      }
+      const int tiles0 = tiles_of<KT>(sequence_len(a, at.b));
+      at.rest = int(divide(u0 - base, tiles0));
+      at.enter(a, ROWS, int((u0 - base) - (long long)at.rest * tiles0), u1 - u0);
+    }
+    if constexpr (TMA) {
+      if (role == 0 && lane == 0) s_share[wk] = Share{at.b, at.rest, at.t, u1 - u0};
+      __syncthreads();
+    }
+    if (u0 < u1) {
+    // ---- loads by cp.async: H - 1 halves ahead, the warps of a worker a share each. A lane looks up the page of its key.
     Cursor<KT> ld = at;
     int ld_end = ld.visible_end();
-    const bool loads = role == 0 || !a.tma;
     int page = -1, next_t = -1;  // of the tile that goes out next; next_t < 0: behind the last
     int next_head = 0;
-    int ahead = 0;               // halves issued and not used (of the warp that loads)
     const auto peek = [&]() {    // takes the next tile with keys, if any, and has its pages looked up
       while (ld.t >= ld_end) {
         if (!ld.next(a, ROWS)) {
           next_t = -1;
-          ld_end = 0;
-          ld.t = 0;
-          ld.left = 0;
           return;
         }
         ld_end = ld.visible_end();
@@ -361,7 +465,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocks)
       const int j = next_t * KT + lane;
       page = lane < KT && j < ld.seen ? a.table[ld.b * a.table_stride + a.by_page(j)] : -1;
     };
-    int in = 0, in_values = 0;  // the half of the ring that is filled next, with keys or values
+    int in = 0, in_values = 0, filled = 0;  // the half of the ring that is filled next, with keys or values; how many are ahead
     uint32_t in_phase = 0;
     // (Its code stands once: with the fill of the ring written out in front of the loop the start took 2 us more for
     // fetching instructions.)
@@ -374,44 +478,27 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocks)
       const uint32_t valid = __ballot_sync(0xffffffffu, ok);
       if (role == 0 && lane == 0) {
         s_valid[wk][in] = valid;
-        if (a.tma)
-          mbar_arrive_expect_tx(bar, L::kHalf);
-        else
-          mbar_arrive(bar);
+        mbar_arrive(bar);
       }
-      if (a.tma) {
-        __syncwarp();
-        // 16 slots and 64 columns a lane; a page that is not there is outside the map, zeros
-        constexpr int kBoxes = L::kAtoms * (KT / 16);
-        const int group = lane / L::kAtoms, atom = lane - group * L::kAtoms;
-        const int p = __shfl_sync(0xffffffffu, page, (group * 16) & 31);
-        if (lane < kBoxes) {
-          const int j = next_t * KT + group * 16, slot = j - a.by_page(j) * a.page_size;
-          const MapPos& pos = in_values ? a.pv : a.pk;
-          int c[4] = {atom * 64, 0, 0, 0};
-          const int page_at = p >= 0 && p < a.pages ? p : a.pages;
+      const long long sp = in_values ? a.v_sp : a.k_sp, ss = in_values ? a.v_ss : a.k_ss;
+      const __nv_bfloat16* src = in_values ? a.v + next_head * a.v_sh : a.k + next_head * a.k_sh;
+      const int j = next_t * KT + lane;
+      const long long off = ok ? page * sp + (j - a.by_page(j) * a.page_size) * ss : -1;  // < 0: nowhere
+      // Eight lanes a row, four rows a copy, the columns of 64 after each other.
+      const uint32_t dst = ring_at + in * L::kHalf + (lane >> 3) * 128;
 #pragma unroll
-          for (int i = 1; i < 4; ++i) c[i] = pos.s == i ? slot : pos.h == i ? next_head : page_at;
-          tma_load_4d(in_values ? &map_v : &map_k, bar, ring + in * L::kHalf + atom * L::kAtom + group * 2048, c[0], c[1],
-                      c[2], c[3]);
+      for (int i = 0; i < KT / (4 * WR); ++i) {
+        const int row4 = i * WR + role;  // rows 4 row4 ... 4 row4 + 3
+        const long long o = __shfl_sync(0xffffffffu, off, row4 * 4 + (lane >> 3));
+        const uint32_t to = dst + row4 * 512 + (((lane & 7) ^ ((row4 & 1) * 4 + (lane >> 3))) << 4);
+#pragma unroll
+        for (int c = 0; c < L::kAtoms; ++c) {
+          const int col = c * 64 + (lane & 7) * 8;
+          const bool there = o >= 0 && col < a.D;
+          copy16(to + c * L::kAtom, src + (there ? o + col : 0), there);
         }
-      } else {
-        const long long sp = in_values ? a.v_sp : a.k_sp, ss = in_values ? a.v_ss : a.k_ss;
-        const __nv_bfloat16* src = in_values ? a.v + next_head * a.v_sh : a.k + next_head * a.k_sh;
-        const int j = next_t * KT + lane;
-        const long long off = ok ? page * sp + (j - a.by_page(j) * a.page_size) * ss : -1;  // < 0: nowhere
-        const uint32_t dst = ring_at + in * L::kHalf;
-        constexpr int kChunks = L::kAtoms * 8;  // 16-byte pieces of a row
-#pragma unroll 4
-        for (int i = role; i < KT * kChunks / 32; i += WR) {
-          const int idx = i * 32 + lane, row = idx / kChunks, c = idx - row * kChunks;
-          const long long o = __shfl_sync(0xffffffffu, off, row);
-          const bool there = o >= 0 && c * 8 < a.D;
-          copy16(dst + (c >> 3) * L::kAtom + row * 128 + (((c ^ row) & 7) << 4), src + (there ? o + c * 8 : 0), there);
-        }
-        copy_arrive(bar);
       }
-      ++ahead;
+      copy_arrive(bar);
       if (++in == H) {
         in = 0;
         in_phase ^= 1u;
@@ -420,9 +507,8 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocks)
       in_values ^= 1;
       return true;
     };
+    if constexpr (!TMA) peek();
     bool good = true;
-    if (loads) peek();
-    int filled = 0;  // halves issued ahead of the first that is used, up to H - 1
     if (a.ctl.debug & 1u) good = mbar_wait_bounded_warp(&s_never, 0, &s_abort, a.ctl, kStatusForced);
 
     // ---- the items of the share
@@ -435,14 +521,14 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocks)
       k_col[i] = k_row * 128 + (((2 * i + (lane >> 4)) ^ (lane & 7)) << 4);
       v_col[i] = v_row * 128 + (((2 * i + ((lane >> 3) & 1)) ^ (lane & 7)) << 4);
     }
+    const float sc = MODS ? 1.0f : a.scale_log2;
     int used = 0;  // the half of the ring that is used next
     uint32_t phase = 0;
     while (good) {
-      const int kvh = a.by_row_tiles(at.rest), r0 = (at.rest - kvh * a.row_tiles) * ROWS + role * 8 * NB;
-      uint32_t qf[DP / 16][NB][2];
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const int r = r0 + nb * 8 + g;
+      const int kvh = a.by_row_tiles(at.rest), r0 = (at.rest - kvh * a.row_tiles) * ROWS + role * 8;
+      uint32_t qf[DP / 16][2];
+      {
+        const int r = r0 + g;
         const bool ok = r < a.rows;
         const int i = ok ? a.by_g(r) : 0, h = kvh * a.G + (ok ? r - i * a.G : 0);
         const __nv_bfloat16* qp = a.q + ((long long)at.b * a.q_sb + (long long)i * a.q_ss + (long long)h * a.q_sh + c2);
@@ -451,160 +537,142 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocks)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int col = s * 16 + e * 8;
-            qf[s][nb][e] = ok && col < a.D ? *reinterpret_cast<const uint32_t*>(qp + col) : 0u;
+            qf[s][e] = ok && col < a.D ? *reinterpret_cast<const uint32_t*>(qp + col) : 0u;
           }
       }
-      // this lane's rows of the scores: c2 and c2 + 1 of each block of 8
-      int lim[NB][2], lim_min = INT32_MAX;
-      long long p[NB][2];
-      float slope[NB][2];
+      // this lane's rows of the scores: c2 and c2 + 1
+      int lim[2], lim_min = INT32_MAX;
+      long long p[2];
+      float slope[2];
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const int r = r0 + nb * 8 + c2 + y;
-          const bool ok = r < a.rows;
-          const int i = ok ? a.by_g(r) : 0;
-          p[nb][y] = at.seq.p0 + i;
-          lim[nb][y] = ok ? keys_seen(a, at.seq.len, p[nb][y]) : at.seq.len;
-          lim_min = min(lim_min, lim[nb][y]);
-          slope[nb][y] = MODS && a.slopes != nullptr ? a.slopes[kvh * a.G + (ok ? r - i * a.G : 0)] * kLog2e : 0.0f;
-        }
+      for (int y = 0; y < 2; ++y) {
+        const int r = r0 + c2 + y;
+        const bool ok = r < a.rows;
+        const int i = ok ? a.by_g(r) : 0;
+        p[y] = at.seq.p0 + i;
+        lim[y] = ok ? keys_seen(a, at.seq.len, p[y]) : at.seq.len;
+        lim_min = min(lim_min, lim[y]);
+        slope[y] = MODS && a.slopes != nullptr ? a.slopes[kvh * a.G + (ok ? r - i * a.G : 0)] * kLog2e : 0.0f;
+      }
 #pragma unroll
       for (int o = 1; o < 4; o <<= 1) lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, o));
-      float m[NB][2], l[NB][2];
-      float o[DP / 16][NB][4];
+      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+      float o[DP / 16][4];
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        m[nb][0] = m[nb][1] = -INFINITY;
-        l[nb][0] = l[nb][1] = 0.0f;
+      for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[s][nb][e] = 0.0f;
-      }
+        for (int e = 0; e < 4; ++e) o[s][e] = 0.0f;
 
       const int first = at.t, halves = 2 * max(0, at.visible_end() - first);
+      constexpr uint32_t kAll = 0xffffffffu >> (32 - KT);
       uint32_t valid = 0;
-      float x[KT / 16][NB][4];
+      float x[KT / 16][4];
 #pragma unroll 1
       for (int half = 0; half < halves && good; ++half) {  // a tile's keys, then its values
+        if constexpr (TMA) {
+          good = mbar_wait_bounded_warp(&s_full[wk][used], phase, &s_abort, a.ctl, kStatusTimeoutEpilogue);
+        } else {
 #pragma unroll 1
-        for (;;) {
-          const bool full = filled == H - 1;
-          if (full) {
-            good = mbar_wait_bounded_warp(&s_full[wk][used], phase, &s_abort, a.ctl, kStatusTimeoutEpilogue);
-            if (!good) break;
+          for (;;) {
+            const bool full = filled == H - 1;
+            if (full) {
+              good = mbar_wait_bounded_warp(&s_full[wk][used], phase, &s_abort, a.ctl, kStatusTimeoutEpilogue);
+              if (!good) break;
+            }
+            good = issue();
+            if (full || !good) break;
+            ++filled;
           }
-          if (loads && !issue()) good = false;
-          if (full || !good) break;
-          ++filled;
         }
         if (!good) break;
         const uint32_t half_at = ring_at + used * L::kHalf;
         if ((half & 1) == 0) {
           valid = s_valid[wk][used];
-          // S^T = K Q^T, 16 keys a block of x
+          // S^T = K Q^T, 16 keys a block of x; even and odd steps are sums of their own, half the chain of instructions that
+          // wait for each other
+          float odd[KT / 16][4];
 #pragma unroll
           for (int n = 0; n < KT / 16; ++n)
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) x[n][nb][e] = 0.0f;
+            for (int e = 0; e < 4; ++e) x[n][e] = odd[n][e] = 0.0f;
 #pragma unroll
           for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
             for (int n = 0; n < KT / 16; ++n) {
               uint32_t kf[4];
               ldmatrix_x4(half_at + k_col[s & 3] + (s >> 2) * L::kAtom + n * 2048, kf);
-#pragma unroll
-              for (int nb = 0; nb < NB; ++nb) mma_bf16(x[n][nb], kf, qf[s][nb][0], qf[s][nb][1]);
+              mma_bf16(s & 1 ? odd[n] : x[n], kf, qf[s][0], qf[s][1]);
             }
+#pragma unroll
+          for (int n = 0; n < KT / 16; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[n][e] += odd[n][e];
           const int j0 = (first + (half >> 1)) * KT;
           if constexpr (MODS) {
 #pragma unroll
             for (int n = 0; n < KT / 16; ++n)
 #pragma unroll
-              for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  float& s = x[n][nb][e];
-                  s = a.cap_out != 0.0f ? capped(s * a.cap_in, a.cap_out) : s * a.scale_log2;
-                  const long long j = j0 + n * 16 + g + (e >> 1) * 8;
-                  if (a.slopes != nullptr) s = fmaf(-slope[nb][e & 1], fabsf(float(p[nb][e & 1] - j)), s);
-                }
+              for (int e = 0; e < 4; ++e) {
+                float& s = x[n][e];
+                s = a.cap_out != 0.0f ? capped(s * a.cap_in, a.cap_out) : s * a.scale_log2;
+                const long long j = j0 + n * 16 + g + (e >> 1) * 8;
+                if (a.slopes != nullptr) s = fmaf(-slope[e & 1], fabsf(float(p[e & 1] - j)), s);
+              }
           }
-          if (j0 + KT > lim_min || valid != (KT < 32 ? (1u << (KT & 31)) - 1u : 0xffffffffu)) {
+          if (j0 + KT > lim_min || valid != kAll) {
 #pragma unroll
             for (int n = 0; n < KT / 16; ++n)
 #pragma unroll
-              for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const int j = n * 16 + g + (e >> 1) * 8;
-                  if (j0 + j >= lim[nb][e & 1] || ((valid >> j) & 1u) == 0) x[n][nb][e] = -INFINITY;
-                }
-          }
-          const float sc = MODS ? 1.0f : a.scale_log2;
-          float top[NB][2];
-          bool moved = false;
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              float& w = top[nb][y];
-              w = fmaxf(x[0][nb][y], x[0][nb][2 + y]);
-#pragma unroll
-              for (int n = 1; n < KT / 16; ++n) w = fmax3(w, x[n][nb][y], x[n][nb][2 + y]);
-#pragma unroll
-              for (int d = 4; d < 32; d <<= 1) w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, d));
-              w *= sc;
-              moved = moved || w > m[nb][y] + kRescale;
-            }
-          if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-              for (int y = 0; y < 2; ++y) {
-                const float to = top[nb][y] > m[nb][y] + kRescale ? top[nb][y] : m[nb][y];
-                const float f = to == m[nb][y] ? 1.0f : fast_exp2(m[nb][y] - to);
-                m[nb][y] = to;
-                l[nb][y] *= f;
-#pragma unroll
-                for (int s = 0; s < DP / 16; ++s) {
-                  o[s][nb][y] *= f;
-                  o[s][nb][2 + y] *= f;
-                }
+              for (int e = 0; e < 4; ++e) {
+                const int j = n * 16 + g + (e >> 1) * 8;
+                if (j0 + j >= lim[e & 1] || ((valid >> j) & 1u) == 0) x[n][e] = -INFINITY;
               }
           }
+          float top[2];
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
+          for (int y = 0; y < 2; ++y) {
+            top[y] = fmaxf(x[0][y], x[0][2 + y]);
+#pragma unroll
+            for (int n = 1; n < KT / 16; ++n) top[y] = fmax3(top[y], x[n][y], x[n][2 + y]);
+          }
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) top[y] = fmaxf(top[y], __shfl_xor_sync(0xffffffffu, top[y], d));
+          top[0] *= sc;
+          top[1] *= sc;
+          if (__any_sync(0xffffffffu, top[0] > m[0] + kRescale || top[1] > m[1] + kRescale)) {
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
-              const float mu = m[nb][y] == -INFINITY ? 0.0f : m[nb][y];  // nothing seen yet: every weight is 0
+              const float to = top[y] > m[y] + kRescale ? top[y] : m[y];
+              const float f = to == m[y] ? 1.0f : fast_exp2(m[y] - to);
+              m[y] = to;
+              l[y] *= f;
 #pragma unroll
-              for (int n = 0; n < KT / 16; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; e += 2) {
-                  float& w = x[n][nb][e + y];
-                  w = fast_exp2(fmaf(w, sc, -mu));
-                  l[nb][y] += w;
-                }
+              for (int s = 0; s < DP / 16; ++s) {
+                o[s][y] *= f;
+                o[s][2 + y] *= f;
+              }
             }
+          }
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const float mu = m[y] == -INFINITY ? 0.0f : m[y];  // nothing seen yet: every weight is 0
+#pragma unroll
+            for (int n = 0; n < KT / 16; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; e += 2) {
+                x[n][e + y] = fast_exp2(fmaf(x[n][e + y], sc, -mu));
+                l[y] += x[n][e + y];
+              }
+          }
         } else {
           // O^T += V^T P^T; P rounded to bf16 for the tensor core, 2^-8 relative at most, the sum takes the unrounded
           // weights
-          uint32_t pf[KT / 16][NB][2];
-#pragma unroll
-          for (int n = 0; n < KT / 16; ++n)
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-              pf[n][nb][0] = transposed(pack_bf16x2(x[n][nb][0], x[n][nb][1]));
-              pf[n][nb][1] = transposed(pack_bf16x2(x[n][nb][2], x[n][nb][3]));
-            }
-          const bool all = valid == (KT < 32 ? (1u << (KT & 31)) - 1u : 0xffffffffu);
+          const bool all = valid == kAll;
 #pragma unroll
           for (int n = 0; n < KT / 16; ++n) {
+            const uint32_t p0 = transposed(pack_bf16x2(x[n][0], x[n][1])), p1 = transposed(pack_bf16x2(x[n][2], x[n][3]));
             const uint32_t w = valid >> (n * 16 + c2);
             const uint32_t k0 = (w & 1u ? 0xffffu : 0u) | (w & 2u ? 0xffff0000u : 0u);
             const uint32_t k1 = (w & 0x100u ? 0xffffu : 0u) | (w & 0x200u ? 0xffff0000u : 0u);
@@ -618,44 +686,38 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocks)
                 vf[2] &= k1;
                 vf[3] &= k1;
               }
-#pragma unroll
-              for (int nb = 0; nb < NB; ++nb) mma_bf16(o[s][nb], vf, pf[n][nb][0], pf[n][nb][1]);
+              mma_bf16(o[s], vf, p0, p1);
             }
           }
         }
         __syncwarp();  // all lanes are done with the half
-        if (WR > 1 && lane == 0) mbar_arrive(&s_empty[wk][used]);
+        if ((TMA || WR > 1) && lane == 0) mbar_arrive(&s_empty[wk][used]);
         if (++used == H) {
           used = 0;
           phase ^= 1u;
         }
-        --ahead;
       }
       if (!good) break;
 
       // ---- the item's rows, or the share's part of them
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
+      for (int d = 4; d < 32; d <<= 1)
 #pragma unroll
-        for (int y = 0; y < 2; ++y)
-#pragma unroll
-          for (int d = 4; d < 32; d <<= 1) l[nb][y] += __shfl_xor_sync(0xffffffffu, l[nb][y], d);
+        for (int y = 0; y < 2; ++y) l[y] += __shfl_xor_sync(0xffffffffu, l[y], d);
       const bool begins = first == 0, ends = at.t1 == at.tiles, last = at.left <= 0;
       if (begins && ends) {
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
+        for (int y = 0; y < 2; ++y) {
+          const int r = r0 + c2 + y;
+          if (r >= a.rows) continue;
+          const float inv = l[y] == 0.0f ? 0.0f : 1.0f / l[y];  // (a NaN sum makes the row NaN)
+          const long long row = out_row(a, at.b, kvh, r) + g;
 #pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const int r = r0 + nb * 8 + c2 + y;
-            if (r >= a.rows) continue;
-            const float inv = l[nb][y] == 0.0f ? 0.0f : 1.0f / l[nb][y];  // (a NaN sum makes the row NaN)
-            const long long row = out_row(a, at.b, kvh, r) + g;
+          for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
-            for (int s = 0; s < DP / 16; ++s)
-#pragma unroll
-              for (int e = 0; e < 2; ++e)
-                if (s * 16 + e * 8 < a.D) write_out(a, row + s * 16 + e * 8, o[s][nb][2 * e + y] * inv);
-          }
+            for (int e = 0; e < 2; ++e)
+              if (s * 16 + e * 8 < a.D) write_out(a, row + s * 16 + e * 8, o[s][2 * e + y] * inv);
+        }
       } else {
         // The share's last part waits in the ring, which nobody needs any more; the end of an item before it does not.
         if (WR > 1 && last) {  // (once the worker's other warps are done with the half used last)
@@ -664,117 +726,115 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocks)
                                         kStatusTimeoutEpilogue);
           if (!good) break;
         }
-        float* const dst = last ? reinterpret_cast<float*>(ring)
-                                : a.head_o + ((long long)blockIdx.x * NW + wk) * a.slot_rows * a.D;
-        const int ld_o = last ? DP + 4 : a.D;
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
+        const auto put = [&](float* dst, int ld_o) {
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            const int r = (role * NB + nb) * 8 + c2 + y;
+            const int r = role * 8 + c2 + y;
             if (r >= a.slot_rows) continue;
-            if (g == 0) s_ml[wk][begins][r] = make_float2(m[nb][y], l[nb][y]);
+            if (g == 0) s_ml[wk][begins][r] = make_float2(m[y], l[y]);
+            float* const row = dst + r * ld_o + g;
 #pragma unroll
             for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
               for (int e = 0; e < 2; ++e)
-                if (s * 16 + e * 8 < a.D) dst[(long long)r * ld_o + s * 16 + e * 8 + g] = o[s][nb][2 * e + y];
+                if (s * 16 + e * 8 < a.D) row[s * 16 + e * 8] = o[s][2 * e + y];
           }
+        };
+        if (last)
+          put(reinterpret_cast<float*>(ring), DP + 4);
+        else
+          put(a.head_o + ((long long)blockIdx.x * NW + wk) * a.slot_rows * a.D, a.D);
         if (role == 0 && lane == 0)
           s_part[wk][begins] = Part{at.b, at.rest, at.tiles - at.t1, uint8_t(begins), uint8_t(ends), uint8_t(last)};
       }
       if (!at.next(a, ROWS)) break;
     }
-    if (!good) {  // copies in flight write to this block's memory: it stays until they are done
-      copy_wait_all();
-      if (a.tma && loads)
-        for (; ahead > 0; --ahead) {
-          mbar_wait_drain(&s_full[wk][used], phase, a.ctl);
-          if (++used == H) {
-            used = 0;
-            phase ^= 1u;
-          }
-        }
+    if (!TMA && !good) copy_wait_all();  // copies in flight write to this block's memory: it stays until they are done
     }
   }
   __syncthreads();
 
-  // ---- the block's parts, in order of keys: chains of one item each, joined here; what goes on in another block, or came
-  // from one, is a part of the block's
-  const Part mine_p = lane < 2 * NW ? s_part[lane >> 1][lane & 1] : Part{-1, 0, 0, 0, 0, 0};
-  const uint32_t present = s_abort ? 0u : __ballot_sync(0xffffffffu, mine_p.b >= 0);
-  const uint32_t starts = (__ballot_sync(0xffffffffu, mine_p.begins) & present) | (present & (0u - present));
-  if (present == 0) {
-    if (threadIdx.x == 0) a.rec[blockIdx.x] = make_int4(0, 0, 0, 0);
-    return;
+  // ---- the block's parts, in order of keys: chains of one item each, joined here, a warp a row; what goes on in another
+  // block, or came from one, is a part of the block's. A lane holds a part.
+  constexpr int PARTS = 2 * NW;
+  const Part part = lane < PARTS ? s_part[lane / 2][lane & 1] : Part{-1, 0, 0, 0, 0, 0};
+  const uint32_t present = s_abort ? 0u : __ballot_sync(0xffffffffu, part.b >= 0);
+  const uint32_t begin_bits = __ballot_sync(0xffffffffu, part.begins) & present;
+  const uint32_t starts = begin_bits | (present & (0u - present));
+  const uint32_t end_bits = __ballot_sync(0xffffffffu, part.ends) & present;
+  const uint32_t ring_bits = __ballot_sync(0xffffffffu, part.in_ring) & present;
+  // (only the last chain goes on in another block: when it begins here, it is the block's to join)
+  const int final = 31 - __clz(int(present)), opens = 31 - __clz(int(starts));
+  if (warp == 0 && lane == (present != 0 ? final : 0)) {
+    const bool joins = present != 0 && !part.ends && ((begin_bits >> opens) & 1u);
+    a.rec[blockIdx.x] = joins ? make_int4(part.b, part.rest, int(divide(c0 + run + part.rem - 1, span)) - int(blockIdx.x) + 1, 0)
+                              : make_int4(0, 0, 0, 0);
   }
-  // The parts' weights, a thread for each row of each chain: over the sum where the chain is the whole item.
-  for (int i = int(threadIdx.x); i < __popc(starts) * a.slot_rows; i += kWarps * 32) {
-    const int c = a.by_slot_rows(i), r = i - c * a.slot_rows;
-    uint32_t rest = starts;
-    for (int k = 0; k < c; ++k) rest &= rest - 1;
-    const int z0 = __ffs(int(rest)) - 1;
-    rest &= rest - 1;
-    const uint32_t parts = present & (0xffffffffu << z0) & (rest != 0 ? (rest & (0u - rest)) - 1u : 0xffffffffu);
-    const Part head = s_part[z0 >> 1][z0 & 1];
-    const int zl = 31 - __clz(int(parts));
-    const Part tail = s_part[zl >> 1][zl & 1];
+  if (present == 0 || warp >= kWarps) return;
+  const int chain = __popc(starts & (0xffffffffu >> (31 - lane)));  // of this lane's part
+  const int kvh = a.by_row_tiles(part.b >= 0 ? part.rest : 0), tile_row = (part.rest - kvh * a.row_tiles) * ROWS;
+  const uint32_t same = __match_any_sync(0xffffffffu, part.b >= 0 ? chain : -1);  // the parts of this lane's chain
+  const bool whole = part.b >= 0 && (same & begin_bits) != 0 && (same & end_bits) != 0;
+  const uint32_t whole_bits = __ballot_sync(0xffffffffu, whole);
+  for (int r = warp; r < a.slot_rows; r += kWarps) {
+    float4 v[PARTS];
+    const auto load = [&](int col) {
+#pragma unroll
+      for (int z = 0; z < PARTS; ++z)
+        if ((present >> z) & 1u)
+          v[z] = (ring_bits >> z) & 1u
+                     ? *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + (z / 2) * L::kRing) +
+                                                        r * (DP + 4) + col)
+                     : *reinterpret_cast<const float4*>(
+                           a.head_o + (((long long)blockIdx.x * NW + z / 2) * a.slot_rows + r) * a.D + col);
+    };
+    if (lane * 4 < a.D) load(lane * 4);
+    const float2 ml = part.b >= 0 ? s_ml[lane / 2][lane & 1][r] : make_float2(-INFINITY, 0.0f);
     float top = -INFINITY, sum = 0.0f;
-    for (uint32_t w = parts; w != 0; w &= w - 1) {
-      const int z = __ffs(int(w)) - 1;
-      top = fmaxf(top, s_ml[z >> 1][z & 1][r].x);
+#pragma unroll
+    for (int z = 0; z < PARTS; ++z) {
+      const float mz = __shfl_sync(0xffffffffu, ml.x, z);
+      if (__shfl_sync(0xffffffffu, chain, z) == chain) top = fmaxf(top, mz);
     }
-    for (uint32_t w = parts; w != 0; w &= w - 1) {
-      const int z = __ffs(int(w)) - 1;
-      float2& ml = s_ml[z >> 1][z & 1][r];
-      ml.x = ml.x == -INFINITY ? 0.0f : fast_exp2(ml.x - top);
-      sum = fmaf(ml.x, ml.y, sum);
+    float wt = ml.x == -INFINITY ? 0.0f : fast_exp2(ml.x - top);
+    const float lw = part.b >= 0 ? wt * ml.y : 0.0f;
+#pragma unroll
+    for (int z = 0; z < PARTS; ++z) {
+      const float lz = __shfl_sync(0xffffffffu, lw, z);
+      if (__shfl_sync(0xffffffffu, chain, z) == chain) sum += lz;
     }
-    if (head.begins && tail.ends) {
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      for (uint32_t w = parts; w != 0; w &= w - 1) {
-        const int z = __ffs(int(w)) - 1;
-        s_ml[z >> 1][z & 1][r].x *= inv;
-      }
-    } else {
-      a.part_ml[((long long)blockIdx.x * 2 + head.begins) * a.slot_rows + r] = make_float2(top, sum);
-      if (r == 0 && head.begins)  // (only the last chain goes on in another block)
-        s_rec = make_int4(head.b, head.rest, int(divide(c0 + run + tail.rem - 1, span)) - int(blockIdx.x) + 1, 0);
-    }
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) a.rec[blockIdx.x] = s_rec;
-  for (int r = warp; r < a.slot_rows; r += kWarps)
-    for (int col = lane * 4; col < a.D; col += 128) {
+    // over the sum where the chain is the whole item; (a NaN sum makes the row NaN)
+    if (whole)
+      wt *= sum == 0.0f ? 0.0f : 1.0f / sum;
+    else if ((starts >> lane) & 1u)
+      a.part_ml[((long long)blockIdx.x * 2 + part.begins) * a.slot_rows + r] = make_float2(top, sum);
+    const bool inside = part.b >= 0 && tile_row + r < a.rows;
+    const long long at = inside ? out_row(a, part.b, kvh, tile_row + r) : -1;
+    for (int col = lane * 4; col < (a.D + 127) / 128 * 128; col += 128) {
+      if (col >= 128 && col < a.D) load(col);
       float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      int begins = 0;
-      for (uint32_t w = present; w != 0; w &= w - 1) {
-        const int z = __ffs(int(w)) - 1;
-        const Part part = s_part[z >> 1][z & 1];
-        const float wt = s_ml[z >> 1][z & 1][r].x;
-        const float4 v = *reinterpret_cast<const float4*>(
-            part.in_ring ? reinterpret_cast<const float*>(smem + (z >> 1) * L::kRing) + r * (DP + 4) + col
-                         : a.head_o + (((long long)blockIdx.x * NW + (z >> 1)) * a.slot_rows + r) * a.D + col);
-        if ((starts >> z) & 1u) {
-          begins = part.begins;
-          acc[0] = wt * v.x, acc[1] = wt * v.y, acc[2] = wt * v.z, acc[3] = wt * v.w;
-        } else {
-          acc[0] = fmaf(wt, v.x, acc[0]);
-          acc[1] = fmaf(wt, v.y, acc[1]);
-          acc[2] = fmaf(wt, v.z, acc[2]);
-          acc[3] = fmaf(wt, v.w, acc[3]);
-        }
-        const uint32_t behind = w & (w - 1);
+#pragma unroll
+      for (int z = 0; z < PARTS; ++z) {
+        if (((present >> z) & 1u) == 0) continue;
+        const float w = __shfl_sync(0xffffffffu, wt, z);
+        if ((starts >> z) & 1u) acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
+        acc[0] = fmaf(w, v[z].x, acc[0]);
+        acc[1] = fmaf(w, v[z].y, acc[1]);
+        acc[2] = fmaf(w, v[z].z, acc[2]);
+        acc[3] = fmaf(w, v[z].w, acc[3]);
+        const uint32_t behind = present & ~((2u << z) - 1u);
         if (behind != 0 && (starts & behind & (0u - behind)) == 0) continue;  // the chain goes on
-        const int kvh = a.by_row_tiles(part.rest), row = (part.rest - kvh * a.row_tiles) * ROWS + r;
-        if (row >= a.rows) continue;
-        if (begins && part.ends)
-          write_out4(a, out_row(a, part.b, kvh, row) + col, acc);
+        const long long to = __shfl_sync(0xffffffffu, at, z);
+        const int slot = (begin_bits >> (31 - __clz(int(starts & ((2u << z) - 1u))))) & 1u;
+        if (to < 0 || col >= a.D) continue;
+        if ((whole_bits >> z) & 1u)
+          write_out4(a, to + col, acc);
         else
-          *reinterpret_cast<float4*>(a.part_o + (((long long)blockIdx.x * 2 + begins) * a.slot_rows + r) * a.D + col) =
+          *reinterpret_cast<float4*>(a.part_o + (((long long)blockIdx.x * 2 + slot) * a.slot_rows + r) * a.D + col) =
               make_float4(acc[0], acc[1], acc[2], acc[3]);
       }
     }
+  }
 }
 
 // Joins the parts of the items that go on from block to block, a row of one at a time: eight warps take the parts in turn, a
@@ -862,7 +922,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_paged_join_kernel(c
 // Host side
 // ---------------------------------------------------------------------------------------------------------------
 struct PagedPlan {
-  int wr, nb, blocks;
+  int wr, blocks;
   int64_t rows, row_tiles, slot_rows;
   size_t ml_offset, o_offset, head_offset, bytes;
 };
@@ -883,10 +943,8 @@ int check_paged_sizes(int64_t H, int64_t Hk, int64_t Sq, int64_t D) {
 PagedPlan plan_paged(int64_t H, int64_t Hk, int64_t Sq, int64_t D, int sms) {
   PagedPlan p;
   p.rows = H / Hk * Sq;
-  p.nb = p.rows <= 8 ? 1 : 2;
-  // (four warps' rows share keys up to 128 columns only: above, two blocks of them fit an SM no more)
-  p.wr = p.rows <= 16 ? 1 : p.rows <= 32 || D > 128 ? 2 : 4;
-  const int64_t tile = 8 * p.nb * p.wr;
+  p.wr = p.rows <= 8 ? 1 : p.rows <= 16 ? 2 : 4;
+  const int64_t tile = 8 * p.wr;
   p.row_tiles = (p.rows + tile - 1) / tile;
   p.slot_rows = p.rows < tile ? p.rows : tile;
   p.blocks = sms * kBlocks * kWaves;
@@ -899,44 +957,47 @@ PagedPlan plan_paged(int64_t H, int64_t Hk, int64_t Sq, int64_t D, int sms) {
   return p;
 }
 
-template <int DP, int WR, int NB, bool MODS>
+template <int DP, int WR, bool MODS, bool TMA>
 int launch_paged(const CUtensorMap& mk, const CUtensorMap& mv, const PagedArgs& a, int blocks, cudaStream_t stream,
                  int device) {
-  constexpr int smem = PagedLayout<DP, WR, NB>::kSmem;
+  constexpr int smem = PagedLayout<DP, WR>::kSmem;
   static std::atomic<bool> ready[64] = {};
   if (!ready[device]) {
-    if (int rc = check_cuda(cudaFuncSetAttribute(attention_paged_kernel<DP, WR, NB, MODS>,
+    if (int rc = check_cuda(cudaFuncSetAttribute(attention_paged_kernel<DP, WR, MODS, TMA>,
                                                  cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
                             "paged attention shared memory"))
       return rc;
     ready[device] = true;
   }
-  return check_cuda(launch_pdl(attention_paged_kernel<DP, WR, NB, MODS>, dim3(unsigned(blocks)), dim3(kWarps * 32), smem,
-                               stream, mk, mv, a),
+  return check_cuda(launch_pdl(attention_paged_kernel<DP, WR, MODS, TMA>, dim3(unsigned(blocks)),
+                               dim3(kWarps * 32 + (TMA ? 32 : 0)), smem, stream, mk, mv, a),
                     "paged attention kernel launch");
 }
 
-template <int WR, int NB, bool MODS>
+template <int WR, bool MODS, bool TMA>
 int launch_paged_dim(const CUtensorMap& mk, const CUtensorMap& mv, const PagedArgs& a, int blocks, cudaStream_t stream,
                      int device) {
-  if (a.D <= 64) return launch_paged<64, WR, NB, MODS>(mk, mv, a, blocks, stream, device);
-  if (a.D <= 96) return launch_paged<96, WR, NB, MODS>(mk, mv, a, blocks, stream, device);
-  if (a.D <= 128) return launch_paged<128, WR, NB, MODS>(mk, mv, a, blocks, stream, device);
-  if constexpr (WR <= 2) {
-    if (a.D <= 160) return launch_paged<160, WR, NB, MODS>(mk, mv, a, blocks, stream, device);
-    if (a.D <= 192) return launch_paged<192, WR, NB, MODS>(mk, mv, a, blocks, stream, device);
-    return launch_paged<256, WR, NB, MODS>(mk, mv, a, blocks, stream, device);
-  }
-  return fail(kErrUnsupported, "paged attention: no kernel for these rows");  // (plan_paged asks for none)
+  if (a.D <= 64) return launch_paged<64, WR, MODS, TMA>(mk, mv, a, blocks, stream, device);
+  if (TMA && a.D <= 96) return launch_paged<96, WR, MODS, true>(mk, mv, a, blocks, stream, device);
+  if (a.D <= 128) return launch_paged<128, WR, MODS, TMA>(mk, mv, a, blocks, stream, device);
+  if (TMA && a.D <= 160) return launch_paged<160, WR, MODS, true>(mk, mv, a, blocks, stream, device);
+  if (a.D <= 192) return launch_paged<192, WR, MODS, TMA>(mk, mv, a, blocks, stream, device);
+  return launch_paged<256, WR, MODS, TMA>(mk, mv, a, blocks, stream, device);
+}
+
+template <bool MODS, bool TMA>
+int launch_paged_rows(const CUtensorMap& mk, const CUtensorMap& mv, const PagedArgs& a, const PagedPlan& p,
+                      cudaStream_t stream, int device) {
+  if (p.wr == 1) return launch_paged_dim<1, MODS, TMA>(mk, mv, a, p.blocks, stream, device);
+  if (p.wr == 2) return launch_paged_dim<2, MODS, TMA>(mk, mv, a, p.blocks, stream, device);
+  return launch_paged_dim<4, MODS, TMA>(mk, mv, a, p.blocks, stream, device);
 }
 
 template <bool MODS>
-int launch_paged_for(const CUtensorMap& mk, const CUtensorMap& mv, const PagedArgs& a, const PagedPlan& p,
+int launch_paged_for(const CUtensorMap& mk, const CUtensorMap& mv, const PagedArgs& a, const PagedPlan& p, bool tma,
                      cudaStream_t stream, int device) {
-  if (p.nb == 1) return launch_paged_dim<1, 1, MODS>(mk, mv, a, p.blocks, stream, device);
-  if (p.wr == 1) return launch_paged_dim<1, 2, MODS>(mk, mv, a, p.blocks, stream, device);
-  if (p.wr == 2) return launch_paged_dim<2, 2, MODS>(mk, mv, a, p.blocks, stream, device);
-  return launch_paged_dim<4, 2, MODS>(mk, mv, a, p.blocks, stream, device);
+  return tma ? launch_paged_rows<MODS, true>(mk, mv, a, p, stream, device)
+             : launch_paged_rows<MODS, false>(mk, mv, a, p, stream, device);
 }
 
 }  // namespace
@@ -1045,22 +1106,24 @@ int attention_paged_launch(const AttnPagedProblem& p, cudaStream_t stream) {
     const auto fits = [](int64_t n, int64_t s) { return n == 1 || (s > 0 && s < (int64_t(1) << 38)); };
     return fits(c.pages, sp) && fits(c.page_size, ss) && fits(c.kv_heads, sh);
   };
-  a.tma = c.page_size % 16 == 0 && c.pages > 0 && strided(c.k_sp, c.k_ss, c.k_sh) && strided(c.v_sp, c.v_ss, c.v_sh);
-  if (a.tma) {
-    if (int rc = encode_bshd_map(c.k, c.head_dim, c.page_size, c.kv_heads, c.pages, c.k_ss, c.k_sh, c.k_sp, 16, &mk, &a.pk))
+  const bool tma = c.page_size % 16 == 0 && c.pages > 0 && strided(c.k_sp, c.k_ss, c.k_sh) && strided(c.v_sp, c.v_ss, c.v_sh);
+  const int tile = c.head_dim <= 128 ? 32 : 16;  // (PagedLayout::kTile)
+  a.box_rows = c.page_size % tile == 0 ? tile : 16;
+  if (tma) {
+    if (int rc = encode_bshd_map(c.k, c.head_dim, c.page_size, c.kv_heads, c.pages, c.k_ss, c.k_sh, c.k_sp, a.box_rows, &mk, &a.pk))
       return rc;
-    if (int rc = encode_bshd_map(c.v, c.head_dim, c.page_size, c.kv_heads, c.pages, c.v_ss, c.v_sh, c.v_sp, 16, &mv, &a.pv))
+    if (int rc = encode_bshd_map(c.v, c.head_dim, c.page_size, c.kv_heads, c.pages, c.v_ss, c.v_sh, c.v_sp, a.box_rows, &mv, &a.pv))
       return rc;
   }
   const bool mods = p.softcap > 0.0f || p.slopes != nullptr;
-  if (int rc = mods ? launch_paged_for<true>(mk, mv, a, plan, stream, dev->device)
-                    : launch_paged_for<false>(mk, mv, a, plan, stream, dev->device))
+  if (int rc = mods ? launch_paged_for<true>(mk, mv, a, plan, tma, stream, dev->device)
+                    : launch_paged_for<false>(mk, mv, a, plan, tma, stream, dev->device))
     return rc;
   // As many rows can be left to join as items begin, one a block at most.
   const int64_t items = std::min<int64_t>(p.batch * c.kv_heads * plan.row_tiles, plan.blocks);
   static_assert(kBlocks * kWaves * 160 <= kJoinMaxRecs, "records of the join kernel");
   return check_cuda(launch_pdl(attention_paged_join_kernel, dim3(unsigned(std::min<int64_t>(items * plan.slot_rows, dev->sms))),
-                               dim3(kJoinWarps * 32), 0, stream, a, plan.blocks, 8 * plan.nb * plan.wr),
+                               dim3(kJoinWarps * 32), 0, stream, a, plan.blocks, 8 * plan.wr),
                     "paged attention join kernel launch");
 }
 
