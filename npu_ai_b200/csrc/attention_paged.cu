@@ -132,15 +132,15 @@ __device__ __forceinline__ void copy_arrive(uint64_t* bar) {
 }
 __device__ __forceinline__ void copy_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// Layout for head dims up to DP and workers of WR warps, 8 rows a warp.
-template <int DP, int WR>
+// Layout for head dims up to DP, workers of WR warps and NB blocks of 8 rows a warp.
+template <int DP, int WR, int NB>
 struct PagedLayout {
   static constexpr int kAtoms = (DP + 63) / 64;           // 128-byte columns of a row
   static constexpr int kTile = DP <= 128 ? 32 : 16;       // keys of a tile
   static constexpr int kAtom = kTile * 128;               // bytes of one column of the keys (values) of a tile
   static constexpr int kHalf = kAtoms * kAtom;
   static constexpr int kWorkers = kWarps / WR;
-  static constexpr int kRows = 8 * WR;
+  static constexpr int kRows = 8 * NB * WR;
   // As many as half an SM holds next to the static tables: up to 130 KB in flight on the SM, of which some 40 KB cover the
   // latency at the full rate.
   static constexpr int kFit = 104 * 1024 / (kWorkers * kHalf);
@@ -355,11 +355,11 @@ __device__ __forceinline__ void load_pages(const PagedArgs& a, const CUtensorMap
   }
 }
 
-template <int DP, int WR, bool MODS, bool TMA>
+template <int DP, int WR, int NB, bool MODS, bool TMA>
 __global__ void __launch_bounds__(kWarps * 32 + (TMA ? 32 : 0), kBlocks)
     attention_paged_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                            const PagedArgs a) {
-  using L = PagedLayout<DP, WR>;
+  using L = PagedLayout<DP, WR, NB>;
   constexpr int KT = L::kTile, H = L::kHalves, NW = L::kWorkers, ROWS = L::kRows;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t s_full[NW][H], s_empty[NW][H], s_never;
@@ -522,13 +522,18 @@ __global__ void __launch_bounds__(kWarps * 32 + (TMA ? 32 : 0), kBlocks)
       v_col[i] = v_row * 128 + (((2 * i + ((lane >> 3) & 1)) ^ (lane & 7)) << 4);
     }
     const float sc = MODS ? 1.0f : a.scale_log2;
+    constexpr uint32_t kAll = 0xffffffffu >> (32 - KT);
     int used = 0;  // the half of the ring that is used next
     uint32_t phase = 0;
+    // The first tile's instructions run once ahead of its data, with every key hidden: fetching them takes as long as the
+    // first load, and so they pass together.
+    int from = -2;
     while (good) {
-      const int kvh = a.by_row_tiles(at.rest), r0 = (at.rest - kvh * a.row_tiles) * ROWS + role * 8;
-      uint32_t qf[DP / 16][2];
-      {
-        const int r = r0 + g;
+      const int kvh = a.by_row_tiles(at.rest), r0 = (at.rest - kvh * a.row_tiles) * ROWS + role * 8 * NB;
+      uint32_t qf[DP / 16][NB][2];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const int r = r0 + nb * 8 + g;
         const bool ok = r < a.rows;
         const int i = ok ? a.by_g(r) : 0, h = kvh * a.G + (ok ? r - i * a.G : 0);
         const __nv_bfloat16* qp = a.q + ((long long)at.b * a.q_sb + (long long)i * a.q_ss + (long long)h * a.q_sh + c2);
@@ -537,43 +542,45 @@ __global__ void __launch_bounds__(kWarps * 32 + (TMA ? 32 : 0), kBlocks)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int col = s * 16 + e * 8;
-            qf[s][e] = ok && col < a.D ? *reinterpret_cast<const uint32_t*>(qp + col) : 0u;
+            qf[s][nb][e] = ok && col < a.D ? *reinterpret_cast<const uint32_t*>(qp + col) : 0u;
           }
       }
-      // this lane's rows of the scores: c2 and c2 + 1
-      int lim[2], lim_min = INT32_MAX;
-      long long p[2];
-      float slope[2];
+      // this lane's rows of the scores: c2 and c2 + 1 of each block
+      int lim[NB][2], lim_min = INT32_MAX;
+      long long p[NB][2];
+      float slope[NB][2], m[NB][2], l[NB][2], o[DP / 16][NB][4];
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        const int r = r0 + c2 + y;
-        const bool ok = r < a.rows;
-        const int i = ok ? a.by_g(r) : 0;
-        p[y] = at.seq.p0 + i;
-        lim[y] = ok ? keys_seen(a, at.seq.len, p[y]) : at.seq.len;
-        lim_min = min(lim_min, lim[y]);
-        slope[y] = MODS && a.slopes != nullptr ? a.slopes[kvh * a.G + (ok ? r - i * a.G : 0)] * kLog2e : 0.0f;
+      for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const int r = r0 + nb * 8 + c2 + y;
+          const bool ok = r < a.rows;
+          const int i = ok ? a.by_g(r) : 0;
+          p[nb][y] = at.seq.p0 + i;
+          lim[nb][y] = ok ? keys_seen(a, at.seq.len, p[nb][y]) : at.seq.len;
+          lim_min = min(lim_min, lim[nb][y]);
+          slope[nb][y] = MODS && a.slopes != nullptr ? a.slopes[kvh * a.G + (ok ? r - i * a.G : 0)] * kLog2e : 0.0f;
+          m[nb][y] = -INFINITY;
+          l[nb][y] = 0.0f;
+        }
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[s][nb][e] = 0.0f;
       }
 #pragma unroll
-      for (int o = 1; o < 4; o <<= 1) lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, o));
-      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-      float o[DP / 16][4];
-#pragma unroll
-      for (int s = 0; s < DP / 16; ++s)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[s][e] = 0.0f;
+      for (int d = 1; d < 4; d <<= 1) lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, d));
 
       const int first = at.t, halves = 2 * max(0, at.visible_end() - first);
-      constexpr uint32_t kAll = 0xffffffffu >> (32 - KT);
       uint32_t valid = 0;
-      float x[KT / 16][4];
+      float x[KT / 16][NB][4];
 #pragma unroll 1
-      for (int half = 0; half < halves && good; ++half) {  // a tile's keys, then its values
+      for (int half = from; half < halves && good; ++half) {  // a tile's keys, then its values
         if constexpr (TMA) {
-          good = mbar_wait_bounded_warp(&s_full[wk][used], phase, &s_abort, a.ctl, kStatusTimeoutEpilogue);
+          if (half >= 0) good = mbar_wait_bounded_warp(&s_full[wk][used], phase, &s_abort, a.ctl, kStatusTimeoutEpilogue);
         } else {
 #pragma unroll 1
-          for (;;) {
+          for (; half >= 0;) {
             const bool full = filled == H - 1;
             if (full) {
               good = mbar_wait_bounded_warp(&s_full[wk][used], phase, &s_abort, a.ctl, kStatusTimeoutEpilogue);
@@ -587,92 +594,123 @@ __global__ void __launch_bounds__(kWarps * 32 + (TMA ? 32 : 0), kBlocks)
         if (!good) break;
         const uint32_t half_at = ring_at + used * L::kHalf;
         if ((half & 1) == 0) {
-          valid = s_valid[wk][used];
-          // S^T = K Q^T, 16 keys a block of x; even and odd steps are sums of their own, half the chain of instructions that
-          // wait for each other
+          if (half >= 0) valid = s_valid[wk][used];
+          // S^T = K Q^T, 16 keys a block of x; with one block of rows even and odd steps are sums of their own, half the
+          // chain of instructions that wait for each other
           float odd[KT / 16][4];
 #pragma unroll
           for (int n = 0; n < KT / 16; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[n][e] = odd[n][e] = 0.0f;
+            for (int e = 0; e < 4; ++e) {
+              odd[n][e] = 0.0f;
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) x[n][nb][e] = 0.0f;
+            }
 #pragma unroll
           for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
             for (int n = 0; n < KT / 16; ++n) {
               uint32_t kf[4];
               ldmatrix_x4(half_at + k_col[s & 3] + (s >> 2) * L::kAtom + n * 2048, kf);
-              mma_bf16(s & 1 ? odd[n] : x[n], kf, qf[s][0], qf[s][1]);
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb)
+                mma_bf16(NB == 1 && (s & 1) ? odd[n] : x[n][nb], kf, qf[s][nb][0], qf[s][nb][1]);
             }
+          if constexpr (NB == 1) {
 #pragma unroll
-          for (int n = 0; n < KT / 16; ++n)
+            for (int n = 0; n < KT / 16; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[n][e] += odd[n][e];
+              for (int e = 0; e < 4; ++e) x[n][0][e] += odd[n][e];
+          }
           const int j0 = (first + (half >> 1)) * KT;
           if constexpr (MODS) {
 #pragma unroll
             for (int n = 0; n < KT / 16; ++n)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                float& s = x[n][e];
-                s = a.cap_out != 0.0f ? capped(s * a.cap_in, a.cap_out) : s * a.scale_log2;
-                const long long j = j0 + n * 16 + g + (e >> 1) * 8;
-                if (a.slopes != nullptr) s = fmaf(-slope[e & 1], fabsf(float(p[e & 1] - j)), s);
-              }
+              for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  float& s = x[n][nb][e];
+                  s = a.cap_out != 0.0f ? capped(s * a.cap_in, a.cap_out) : s * a.scale_log2;
+                  const long long j = j0 + n * 16 + g + (e >> 1) * 8;
+                  if (a.slopes != nullptr) s = fmaf(-slope[nb][e & 1], fabsf(float(p[nb][e & 1] - j)), s);
+                }
           }
           if (j0 + KT > lim_min || valid != kAll) {
 #pragma unroll
             for (int n = 0; n < KT / 16; ++n)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int j = n * 16 + g + (e >> 1) * 8;
-                if (j0 + j >= lim[e & 1] || ((valid >> j) & 1u) == 0) x[n][e] = -INFINITY;
-              }
-          }
-          float top[2];
+              for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            top[y] = fmaxf(x[0][y], x[0][2 + y]);
-#pragma unroll
-            for (int n = 1; n < KT / 16; ++n) top[y] = fmax3(top[y], x[n][y], x[n][2 + y]);
+                for (int e = 0; e < 4; ++e) {
+                  const int j = n * 16 + g + (e >> 1) * 8;
+                  if (j0 + j >= lim[nb][e & 1] || ((valid >> j) & 1u) == 0) x[n][nb][e] = -INFINITY;
+                }
           }
+          float top[NB][2];
+          bool moved = false;
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              top[nb][y] = fmaxf(x[0][nb][y], x[0][nb][2 + y]);
+#pragma unroll
+              for (int n = 1; n < KT / 16; ++n) top[nb][y] = fmax3(top[nb][y], x[n][nb][y], x[n][nb][2 + y]);
+            }
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1)
 #pragma unroll
-            for (int y = 0; y < 2; ++y) top[y] = fmaxf(top[y], __shfl_xor_sync(0xffffffffu, top[y], d));
-          top[0] *= sc;
-          top[1] *= sc;
-          if (__any_sync(0xffffffffu, top[0] > m[0] + kRescale || top[1] > m[1] + kRescale)) {
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+              for (int y = 0; y < 2; ++y) top[nb][y] = fmaxf(top[nb][y], __shfl_xor_sync(0xffffffffu, top[nb][y], d));
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
-              const float to = top[y] > m[y] + kRescale ? top[y] : m[y];
-              const float f = to == m[y] ? 1.0f : fast_exp2(m[y] - to);
-              m[y] = to;
-              l[y] *= f;
-#pragma unroll
-              for (int s = 0; s < DP / 16; ++s) {
-                o[s][y] *= f;
-                o[s][2 + y] *= f;
-              }
+              top[nb][y] *= sc;
+              moved = moved || top[nb][y] > m[nb][y] + kRescale;
             }
-          }
+          if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const float mu = m[y] == -INFINITY ? 0.0f : m[y];  // nothing seen yet: every weight is 0
+            for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-            for (int n = 0; n < KT / 16; ++n)
+              for (int y = 0; y < 2; ++y) {
+                const float to = top[nb][y] > m[nb][y] + kRescale ? top[nb][y] : m[nb][y];
+                const float f = to == m[nb][y] ? 1.0f : fast_exp2(m[nb][y] - to);
+                m[nb][y] = to;
+                l[nb][y] *= f;
 #pragma unroll
-              for (int e = 0; e < 4; e += 2) {
-                x[n][e + y] = fast_exp2(fmaf(x[n][e + y], sc, -mu));
-                l[y] += x[n][e + y];
+                for (int s = 0; s < DP / 16; ++s) {
+                  o[s][nb][y] *= f;
+                  o[s][nb][2 + y] *= f;
+                }
               }
           }
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const float mu = m[nb][y] == -INFINITY ? 0.0f : m[nb][y];  // nothing seen yet: every weight is 0
+#pragma unroll
+              for (int n = 0; n < KT / 16; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; e += 2) {
+                  x[n][nb][e + y] = fast_exp2(fmaf(x[n][nb][e + y], sc, -mu));
+                  l[nb][y] += x[n][nb][e + y];
+                }
+            }
         } else {
           // O^T += V^T P^T; P rounded to bf16 for the tensor core, 2^-8 relative at most, the sum takes the unrounded
           // weights
           const bool all = valid == kAll;
 #pragma unroll
           for (int n = 0; n < KT / 16; ++n) {
-            const uint32_t p0 = transposed(pack_bf16x2(x[n][0], x[n][1])), p1 = transposed(pack_bf16x2(x[n][2], x[n][3]));
+            uint32_t pf[NB][2];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+              pf[nb][0] = transposed(pack_bf16x2(x[n][nb][0], x[n][nb][1]));
+              pf[nb][1] = transposed(pack_bf16x2(x[n][nb][2], x[n][nb][3]));
+            }
             const uint32_t w = valid >> (n * 16 + c2);
             const uint32_t k0 = (w & 1u ? 0xffffu : 0u) | (w & 2u ? 0xffff0000u : 0u);
             const uint32_t k1 = (w & 0x100u ? 0xffffu : 0u) | (w & 0x200u ? 0xffff0000u : 0u);
@@ -686,10 +724,12 @@ __global__ void __launch_bounds__(kWarps * 32 + (TMA ? 32 : 0), kBlocks)
                 vf[2] &= k1;
                 vf[3] &= k1;
               }
-              mma_bf16(o[s], vf, p0, p1);
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) mma_bf16(o[s][nb], vf, pf[nb][0], pf[nb][1]);
             }
           }
         }
+        if (half < 0) continue;
         __syncwarp();  // all lanes are done with the half
         if ((TMA || WR > 1) && lane == 0) mbar_arrive(&s_empty[wk][used]);
         if (++used == H) {
@@ -697,27 +737,38 @@ __global__ void __launch_bounds__(kWarps * 32 + (TMA ? 32 : 0), kBlocks)
           phase ^= 1u;
         }
       }
+      from = 0;
       if (!good) break;
 
       // ---- the item's rows, or the share's part of them
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1)
 #pragma unroll
-        for (int y = 0; y < 2; ++y) l[y] += __shfl_xor_sync(0xffffffffu, l[y], d);
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) l[nb][y] += __shfl_xor_sync(0xffffffffu, l[nb][y], d);
       const bool begins = first == 0, ends = at.t1 == at.tiles, last = at.left <= 0;
       if (begins && ends) {
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const int r = r0 + c2 + y;
-          if (r >= a.rows) continue;
-          const float inv = l[y] == 0.0f ? 0.0f : 1.0f / l[y];  // (a NaN sum makes the row NaN)
-          const long long row = out_row(a, at.b, kvh, r) + g;
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-          for (int s = 0; s < DP / 16; ++s)
+          for (int y = 0; y < 2; ++y) {
+            const int r = r0 + nb * 8 + c2 + y;
+            if (r >= a.rows) continue;
+            const float inv = l[nb][y] == 0.0f ? 0.0f : 1.0f / l[nb][y];  // (a NaN sum makes the row NaN)
+            const long long row = out_row(a, at.b, kvh, r) + g;
+            if (a.out_f32) {
+              float* const d = static_cast<float*>(a.out) + row;
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-              if (s * 16 + e * 8 < a.D) write_out(a, row + s * 16 + e * 8, o[s][2 * e + y] * inv);
-        }
+              for (int s = 0; s < DP / 8; ++s)
+                if (s * 8 < a.D) d[s * 8] = o[s / 2][nb][(s & 1) * 2 + y] * inv;
+            } else {
+              __nv_bfloat16* const d = static_cast<__nv_bfloat16*>(a.out) + row;
+#pragma unroll
+              for (int s = 0; s < DP / 8; ++s)
+                if (s * 8 < a.D) d[s * 8] = __float2bfloat16_rn(o[s / 2][nb][(s & 1) * 2 + y] * inv);
+            }
+          }
       } else {
         // The share's last part waits in the ring, which nobody needs any more; the end of an item before it does not.
         if (WR > 1 && last) {  // (once the worker's other warps are done with the half used last)
@@ -726,24 +777,21 @@ __global__ void __launch_bounds__(kWarps * 32 + (TMA ? 32 : 0), kBlocks)
                                         kStatusTimeoutEpilogue);
           if (!good) break;
         }
-        const auto put = [&](float* dst, int ld_o) {
+        float* const dst = last ? reinterpret_cast<float*>(ring)
+                                : a.head_o + ((long long)blockIdx.x * NW + wk) * a.slot_rows * a.D;
+        const int ld_o = last ? DP + 4 : a.D;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            const int r = role * 8 + c2 + y;
+            const int r = (role * NB + nb) * 8 + c2 + y;
             if (r >= a.slot_rows) continue;
-            if (g == 0) s_ml[wk][begins][r] = make_float2(m[y], l[y]);
+            if (g == 0) s_ml[wk][begins][r] = make_float2(m[nb][y], l[nb][y]);
             float* const row = dst + r * ld_o + g;
 #pragma unroll
-            for (int s = 0; s < DP / 16; ++s)
-#pragma unroll
-              for (int e = 0; e < 2; ++e)
-                if (s * 16 + e * 8 < a.D) row[s * 16 + e * 8] = o[s][2 * e + y];
+            for (int s = 0; s < DP / 8; ++s)
+              if (s * 8 < a.D) row[s * 8] = o[s / 2][nb][(s & 1) * 2 + y];
           }
-        };
-        if (last)
-          put(reinterpret_cast<float*>(ring), DP + 4);
-        else
-          put(a.head_o + ((long long)blockIdx.x * NW + wk) * a.slot_rows * a.D, a.D);
         if (role == 0 && lane == 0)
           s_part[wk][begins] = Part{at.b, at.rest, at.tiles - at.t1, uint8_t(begins), uint8_t(ends), uint8_t(last)};
       }
@@ -755,86 +803,64 @@ __global__ void __launch_bounds__(kWarps * 32 + (TMA ? 32 : 0), kBlocks)
   __syncthreads();
 
   // ---- the block's parts, in order of keys: chains of one item each, joined here, a warp a row; what goes on in another
-  // block, or came from one, is a part of the block's. A lane holds a part.
+  // block, or came from one, is a part of the block's. (Loops, for the code that runs once is as slow as it is long.)
   constexpr int PARTS = 2 * NW;
-  const Part part = lane < PARTS ? s_part[lane / 2][lane & 1] : Part{-1, 0, 0, 0, 0, 0};
-  const uint32_t present = s_abort ? 0u : __ballot_sync(0xffffffffu, part.b >= 0);
-  const uint32_t begin_bits = __ballot_sync(0xffffffffu, part.begins) & present;
+  const Part mine_p = lane < PARTS ? s_part[lane / 2][lane & 1] : Part{-1, 0, 0, 0, 0, 0};
+  const uint32_t present = s_abort ? 0u : __ballot_sync(0xffffffffu, mine_p.b >= 0);
+  const uint32_t begin_bits = __ballot_sync(0xffffffffu, mine_p.begins) & present;
   const uint32_t starts = begin_bits | (present & (0u - present));
-  const uint32_t end_bits = __ballot_sync(0xffffffffu, part.ends) & present;
-  const uint32_t ring_bits = __ballot_sync(0xffffffffu, part.in_ring) & present;
-  // (only the last chain goes on in another block: when it begins here, it is the block's to join)
-  const int final = 31 - __clz(int(present)), opens = 31 - __clz(int(starts));
-  if (warp == 0 && lane == (present != 0 ? final : 0)) {
-    const bool joins = present != 0 && !part.ends && ((begin_bits >> opens) & 1u);
-    a.rec[blockIdx.x] = joins ? make_int4(part.b, part.rest, int(divide(c0 + run + part.rem - 1, span)) - int(blockIdx.x) + 1, 0)
-                              : make_int4(0, 0, 0, 0);
+  if (warp == 0 && lane == (present != 0 ? 31 - __clz(int(present)) : 0)) {
+    // Only the last chain goes on in another block: when it begins here, it is the block's to join.
+    const bool joins = present != 0 && !mine_p.ends && ((begin_bits >> (31 - __clz(int(starts)))) & 1u);
+    a.rec[blockIdx.x] =
+        joins ? make_int4(mine_p.b, mine_p.rest, int(divide(c0 + run + mine_p.rem - 1, span)) - int(blockIdx.x) + 1, 0)
+              : make_int4(0, 0, 0, 0);
   }
   if (present == 0 || warp >= kWarps) return;
-  const int chain = __popc(starts & (0xffffffffu >> (31 - lane)));  // of this lane's part
-  const int kvh = a.by_row_tiles(part.b >= 0 ? part.rest : 0), tile_row = (part.rest - kvh * a.row_tiles) * ROWS;
-  const uint32_t same = __match_any_sync(0xffffffffu, part.b >= 0 ? chain : -1);  // the parts of this lane's chain
-  const bool whole = part.b >= 0 && (same & begin_bits) != 0 && (same & end_bits) != 0;
-  const uint32_t whole_bits = __ballot_sync(0xffffffffu, whole);
-  for (int r = warp; r < a.slot_rows; r += kWarps) {
-    float4 v[PARTS];
-    const auto load = [&](int col) {
-#pragma unroll
-      for (int z = 0; z < PARTS; ++z)
-        if ((present >> z) & 1u)
-          v[z] = (ring_bits >> z) & 1u
-                     ? *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + (z / 2) * L::kRing) +
-                                                        r * (DP + 4) + col)
-                     : *reinterpret_cast<const float4*>(
-                           a.head_o + (((long long)blockIdx.x * NW + z / 2) * a.slot_rows + r) * a.D + col);
-    };
-    if (lane * 4 < a.D) load(lane * 4);
-    const float2 ml = part.b >= 0 ? s_ml[lane / 2][lane & 1][r] : make_float2(-INFINITY, 0.0f);
-    float top = -INFINITY, sum = 0.0f;
-#pragma unroll
-    for (int z = 0; z < PARTS; ++z) {
-      const float mz = __shfl_sync(0xffffffffu, ml.x, z);
-      if (__shfl_sync(0xffffffffu, chain, z) == chain) top = fmaxf(top, mz);
-    }
-    float wt = ml.x == -INFINITY ? 0.0f : fast_exp2(ml.x - top);
-    const float lw = part.b >= 0 ? wt * ml.y : 0.0f;
-#pragma unroll
-    for (int z = 0; z < PARTS; ++z) {
-      const float lz = __shfl_sync(0xffffffffu, lw, z);
-      if (__shfl_sync(0xffffffffu, chain, z) == chain) sum += lz;
-    }
-    // over the sum where the chain is the whole item; (a NaN sum makes the row NaN)
-    if (whole)
-      wt *= sum == 0.0f ? 0.0f : 1.0f / sum;
-    else if ((starts >> lane) & 1u)
-      a.part_ml[((long long)blockIdx.x * 2 + part.begins) * a.slot_rows + r] = make_float2(top, sum);
-    const bool inside = part.b >= 0 && tile_row + r < a.rows;
-    const long long at = inside ? out_row(a, part.b, kvh, tile_row + r) : -1;
-    for (int col = lane * 4; col < (a.D + 127) / 128 * 128; col += 128) {
-      if (col >= 128 && col < a.D) load(col);
-      float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int z = 0; z < PARTS; ++z) {
-        if (((present >> z) & 1u) == 0) continue;
-        const float w = __shfl_sync(0xffffffffu, wt, z);
-        if ((starts >> z) & 1u) acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
-        acc[0] = fmaf(w, v[z].x, acc[0]);
-        acc[1] = fmaf(w, v[z].y, acc[1]);
-        acc[2] = fmaf(w, v[z].z, acc[2]);
-        acc[3] = fmaf(w, v[z].w, acc[3]);
-        const uint32_t behind = present & ~((2u << z) - 1u);
+#pragma unroll 1
+  for (int r = warp; r < a.slot_rows; r += kWarps)
+#pragma unroll 1
+    for (int col = lane * 4; col < a.D; col += 128) {
+      float acc[4], top = -INFINITY, sum = 0.0f;
+      int begins = 0;
+#pragma unroll 1
+      for (uint32_t w = present; w != 0; w &= w - 1) {
+        const int z = __ffs(int(w)) - 1;
+        const Part part = s_part[z / 2][z & 1];
+        const float2 ml = s_ml[z / 2][z & 1][r];
+        const float* const src = part.in_ring
+                                     ? reinterpret_cast<const float*>(smem + (z / 2) * L::kRing) + r * (DP + 4)
+                                     : a.head_o + (((long long)blockIdx.x * NW + z / 2) * a.slot_rows + r) * a.D;
+        const float4 v = *reinterpret_cast<const float4*>(src + col);
+        if ((starts >> z) & 1u) {
+          begins = part.begins;
+          top = -INFINITY;
+          sum = acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
+        }
+        const float to = fmaxf(top, ml.x), base = to == -INFINITY ? 0.0f : to;
+        const float f0 = fast_exp2(top - base), f1 = fast_exp2(ml.x - base);
+        top = to;
+        sum = fmaf(f1, ml.y, sum * f0);
+        acc[0] = fmaf(f1, v.x, acc[0] * f0);
+        acc[1] = fmaf(f1, v.y, acc[1] * f0);
+        acc[2] = fmaf(f1, v.z, acc[2] * f0);
+        acc[3] = fmaf(f1, v.w, acc[3] * f0);
+        const uint32_t behind = w & (w - 1);
         if (behind != 0 && (starts & behind & (0u - behind)) == 0) continue;  // the chain goes on
-        const long long to = __shfl_sync(0xffffffffu, at, z);
-        const int slot = (begin_bits >> (31 - __clz(int(starts & ((2u << z) - 1u))))) & 1u;
-        if (to < 0 || col >= a.D) continue;
-        if ((whole_bits >> z) & 1u)
-          write_out4(a, to + col, acc);
-        else
-          *reinterpret_cast<float4*>(a.part_o + (((long long)blockIdx.x * 2 + slot) * a.slot_rows + r) * a.D + col) =
-              make_float4(acc[0], acc[1], acc[2], acc[3]);
+        const int kvh = a.by_row_tiles(part.rest), row = (part.rest - kvh * a.row_tiles) * ROWS + r;
+        if (row >= a.rows) continue;
+        if (begins && part.ends) {
+          const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // (a NaN sum makes the row NaN)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] *= inv;
+          write_out4(a, out_row(a, part.b, kvh, row) + col, acc);
+        } else {
+          const long long at = ((long long)blockIdx.x * 2 + begins) * a.slot_rows + r;
+          if (col == 0) a.part_ml[at] = make_float2(top, sum);
+          *reinterpret_cast<float4*>(a.part_o + at * a.D + col) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        }
       }
     }
-  }
 }
 
 // Joins the parts of the items that go on from block to block, a row of one at a time: eight warps take the parts in turn, a
@@ -922,7 +948,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_paged_join_kernel(c
 // Host side
 // ---------------------------------------------------------------------------------------------------------------
 struct PagedPlan {
-  int wr, blocks;
+  int wr, nb, blocks;
   int64_t rows, row_tiles, slot_rows;
   size_t ml_offset, o_offset, head_offset, bytes;
 };
@@ -943,8 +969,11 @@ int check_paged_sizes(int64_t H, int64_t Hk, int64_t Sq, int64_t D) {
 PagedPlan plan_paged(int64_t H, int64_t Hk, int64_t Sq, int64_t D, int sms) {
   PagedPlan p;
   p.rows = H / Hk * Sq;
-  p.wr = p.rows <= 8 ? 1 : p.rows <= 16 ? 2 : 4;
-  const int64_t tile = 8 * p.wr;
+  // Two blocks of rows a warp from 17 rows on, where reading the keys from shared memory for each block decides; above 128
+  // columns their O does not fit the registers.
+  p.nb = p.rows > 16 && D <= 128 ? 2 : 1;
+  p.wr = p.rows <= 8 ? 1 : p.rows <= 16 * p.nb ? 2 : 4;
+  const int64_t tile = 8 * p.nb * p.wr;
   p.row_tiles = (p.rows + tile - 1) / tile;
   p.slot_rows = p.rows < tile ? p.rows : tile;
   p.blocks = sms * kBlocks * kWaves;
@@ -957,40 +986,46 @@ PagedPlan plan_paged(int64_t H, int64_t Hk, int64_t Sq, int64_t D, int sms) {
   return p;
 }
 
-template <int DP, int WR, bool MODS, bool TMA>
+template <int DP, int WR, int NB, bool MODS, bool TMA>
 int launch_paged(const CUtensorMap& mk, const CUtensorMap& mv, const PagedArgs& a, int blocks, cudaStream_t stream,
                  int device) {
-  constexpr int smem = PagedLayout<DP, WR>::kSmem;
+  constexpr int smem = PagedLayout<DP, WR, NB>::kSmem;
   static std::atomic<bool> ready[64] = {};
   if (!ready[device]) {
-    if (int rc = check_cuda(cudaFuncSetAttribute(attention_paged_kernel<DP, WR, MODS, TMA>,
+    if (int rc = check_cuda(cudaFuncSetAttribute(attention_paged_kernel<DP, WR, NB, MODS, TMA>,
                                                  cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
                             "paged attention shared memory"))
       return rc;
     ready[device] = true;
   }
-  return check_cuda(launch_pdl(attention_paged_kernel<DP, WR, MODS, TMA>, dim3(unsigned(blocks)),
+  return check_cuda(launch_pdl(attention_paged_kernel<DP, WR, NB, MODS, TMA>, dim3(unsigned(blocks)),
                                dim3(kWarps * 32 + (TMA ? 32 : 0)), smem, stream, mk, mv, a),
                     "paged attention kernel launch");
 }
 
-template <int WR, bool MODS, bool TMA>
+template <int WR, int NB, bool MODS, bool TMA>
 int launch_paged_dim(const CUtensorMap& mk, const CUtensorMap& mv, const PagedArgs& a, int blocks, cudaStream_t stream,
                      int device) {
-  if (a.D <= 64) return launch_paged<64, WR, MODS, TMA>(mk, mv, a, blocks, stream, device);
-  if (TMA && a.D <= 96) return launch_paged<96, WR, MODS, true>(mk, mv, a, blocks, stream, device);
-  if (a.D <= 128) return launch_paged<128, WR, MODS, TMA>(mk, mv, a, blocks, stream, device);
-  if (TMA && a.D <= 160) return launch_paged<160, WR, MODS, true>(mk, mv, a, blocks, stream, device);
-  if (a.D <= 192) return launch_paged<192, WR, MODS, TMA>(mk, mv, a, blocks, stream, device);
-  return launch_paged<256, WR, MODS, TMA>(mk, mv, a, blocks, stream, device);
+  if (a.D <= 64) return launch_paged<64, WR, NB, MODS, TMA>(mk, mv, a, blocks, stream, device);
+  if (TMA && a.D <= 96) return launch_paged<96, WR, NB, MODS, true>(mk, mv, a, blocks, stream, device);
+  if (a.D <= 128) return launch_paged<128, WR, NB, MODS, TMA>(mk, mv, a, blocks, stream, device);
+  if constexpr (NB == 1) {
+    if (TMA && a.D <= 160) return launch_paged<160, WR, 1, MODS, true>(mk, mv, a, blocks, stream, device);
+    if (a.D <= 192) return launch_paged<192, WR, 1, MODS, TMA>(mk, mv, a, blocks, stream, device);
+    return launch_paged<256, WR, 1, MODS, TMA>(mk, mv, a, blocks, stream, device);
+  }
+  return fail(kErrUnsupported, "paged attention: no kernel for these rows");  // (plan_paged asks for none)
 }
 
 template <bool MODS, bool TMA>
 int launch_paged_rows(const CUtensorMap& mk, const CUtensorMap& mv, const PagedArgs& a, const PagedPlan& p,
                       cudaStream_t stream, int device) {
-  if (p.wr == 1) return launch_paged_dim<1, MODS, TMA>(mk, mv, a, p.blocks, stream, device);
-  if (p.wr == 2) return launch_paged_dim<2, MODS, TMA>(mk, mv, a, p.blocks, stream, device);
-  return launch_paged_dim<4, MODS, TMA>(mk, mv, a, p.blocks, stream, device);
+  if (p.nb == 2)
+    return p.wr == 2 ? launch_paged_dim<2, 2, MODS, TMA>(mk, mv, a, p.blocks, stream, device)
+                     : launch_paged_dim<4, 2, MODS, TMA>(mk, mv, a, p.blocks, stream, device);
+  if (p.wr == 1) return launch_paged_dim<1, 1, MODS, TMA>(mk, mv, a, p.blocks, stream, device);
+  if (p.wr == 2) return launch_paged_dim<2, 1, MODS, TMA>(mk, mv, a, p.blocks, stream, device);
+  return launch_paged_dim<4, 1, MODS, TMA>(mk, mv, a, p.blocks, stream, device);
 }
 
 template <bool MODS>
@@ -1123,7 +1158,7 @@ int attention_paged_launch(const AttnPagedProblem& p, cudaStream_t stream) {
   const int64_t items = std::min<int64_t>(p.batch * c.kv_heads * plan.row_tiles, plan.blocks);
   static_assert(kBlocks * kWaves * 160 <= kJoinMaxRecs, "records of the join kernel");
   return check_cuda(launch_pdl(attention_paged_join_kernel, dim3(unsigned(std::min<int64_t>(items * plan.slot_rows, dev->sms))),
-                               dim3(kJoinWarps * 32), 0, stream, a, plan.blocks, 8 * plan.wr),
+                               dim3(kJoinWarps * 32), 0, stream, a, plan.blocks, 8 * plan.nb * plan.wr),
                     "paged attention join kernel launch");
 }
 
