@@ -37,7 +37,8 @@ namespace npub200 {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kWarps = 4;  // of a block
+constexpr int kWarps = 4;  // of a block that use the tiles
+constexpr int kLoadWarps = 2;  // that load them by TMA: each the half of the workers
 constexpr int kBlocks = 2;  // resident on an SM
 constexpr int kWaves = 1;  // blocks of the grid for each that is resident
 constexpr int kMaxHalves = 8;  // of a ring
@@ -124,7 +125,7 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
 }
 // 16 bytes from global to shared memory, or zeros where `ok` is false.
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool ok) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0));
 }
 // Arrives on the barrier when this thread's copies so far are there.
 __device__ __forceinline__ void copy_arrive(uint64_t* bar) {
@@ -261,7 +262,7 @@ struct Share {
   long long tiles;
 };
 
-// The loads of a block by TMA: one warp, a lane for each worker, H halves ahead of it. Boxes of 64 columns and box_rows slots;
+// The loads of half a block's workers by TMA: a warp, a lane for each worker, H halves ahead of it. Boxes of 64 columns and box_rows slots;
 // a page that is not there is outside the map, which reads as zeros. (The warps that use the tiles spent 480 cycles on each
 // half where they issued the loads themselves, as much as on its arithmetic.)
 template <typename L, int WR>
@@ -271,7 +272,8 @@ __device__ __forceinline__ void load_pages(const PagedArgs& a, const CUtensorMap
   constexpr int KT = L::kTile, H = L::kHalves;
   const int lane = int(threadIdx.x) & 31;
   Cursor<KT> ld = {};
-  bool more = lane < L::kWorkers && shares[lane].tiles > 0;
+  const int half = int(threadIdx.x) / 32 - kWarps;  // (a box takes a lane some 80 cycles, and lanes take turns)
+  bool more = lane < L::kWorkers && lane % kLoadWarps == half && shares[lane].tiles > 0;
   int end = 0, t = 0, head = 0, seen = 0, page[KT / 16];
   const auto peek = [&]() {  // takes the next tile with keys, if any, and has its pages looked up
     while (ld.t >= end) {
@@ -356,7 +358,7 @@ __device__ __forceinline__ void load_pages(const PagedArgs& a, const CUtensorMap
 }
 
 template <int DP, int WR, int NB, bool MODS, bool TMA>
-__global__ void __launch_bounds__(kWarps * 32 + (TMA ? 32 : 0), kBlocks)
+__global__ void __launch_bounds__((kWarps + (TMA ? kLoadWarps : 0)) * 32, kBlocks)
     attention_paged_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                            const PagedArgs a) {
   using L = PagedLayout<DP, WR, NB>;
@@ -402,7 +404,7 @@ __global__ void __launch_bounds__(kWarps * 32 + (TMA ? 32 : 0), kBlocks)
     return upto;
   };
   long long span = 0, c0 = 0, run = 0;
-  if (TMA && warp == kWarps) {
+  if (TMA && warp >= kWarps) {
     __syncthreads();
     load_pages<L, WR>(a, &map_k, &map_v, s_share, smem, s_full, s_empty, s_valid, &s_abort);
   } else {
@@ -486,16 +488,18 @@ __global__ void __launch_bounds__(kWarps * 32 + (TMA ? 32 : 0), kBlocks)
       const long long off = ok ? page * sp + (j - a.by_page(j) * a.page_size) * ss : -1;  // < 0: nowhere
       // Eight lanes a row, four rows a copy, the columns of 64 after each other.
       const uint32_t dst = ring_at + in * L::kHalf + (lane >> 3) * 128;
+      long long o[KT / (4 * WR)];  // (all of them first: between the copies each would wait for the copy before it)
+#pragma unroll
+      for (int i = 0; i < KT / (4 * WR); ++i) o[i] = __shfl_sync(0xffffffffu, off, (i * WR + role) * 4 + (lane >> 3));
 #pragma unroll
       for (int i = 0; i < KT / (4 * WR); ++i) {
         const int row4 = i * WR + role;  // rows 4 row4 ... 4 row4 + 3
-        const long long o = __shfl_sync(0xffffffffu, off, row4 * 4 + (lane >> 3));
         const uint32_t to = dst + row4 * 512 + (((lane & 7) ^ ((row4 & 1) * 4 + (lane >> 3))) << 4);
 #pragma unroll
         for (int c = 0; c < L::kAtoms; ++c) {
           const int col = c * 64 + (lane & 7) * 8;
-          const bool there = o >= 0 && col < a.D;
-          copy16(to + c * L::kAtom, src + (there ? o + col : 0), there);
+          const bool there = o[i] >= 0 && col < a.D;
+          copy16(to + c * L::kAtom, src + (there ? o[i] + col : 0), there);
         }
       }
       copy_arrive(bar);
@@ -771,22 +775,25 @@ __global__ void __launch_bounds__(kWarps * 32 + (TMA ? 32 : 0), kBlocks)
           }
       } else {
         // The share's last part waits in the ring, which nobody needs any more; the end of an item before it does not.
-        if (WR > 1 && last) {  // (once the worker's other warps are done with the half used last)
+        if (WR > 1 && NW > 1 && last) {  // (once the worker's other warps are done with the half used last)
           const int before = used == 0 ? H - 1 : used - 1;
           good = mbar_wait_bounded_warp(&s_empty[wk][before], used == 0 ? phase ^ 1u : phase, &s_abort, a.ctl,
                                         kStatusTimeoutEpilogue);
           if (!good) break;
         }
-        float* const dst = last ? reinterpret_cast<float*>(ring)
-                                : a.head_o + ((long long)blockIdx.x * NW + wk) * a.slot_rows * a.D;
-        const int ld_o = last ? DP + 4 : a.D;
+        // (The only worker's parts are the block's.)
+        const long long slot = ((long long)blockIdx.x * 2 + begins) * a.slot_rows;
+        float* const dst = NW == 1 ? a.part_o + slot * a.D
+                           : last  ? reinterpret_cast<float*>(ring)
+                                   : a.head_o + ((long long)blockIdx.x * NW + wk) * a.slot_rows * a.D;
+        const int ld_o = NW > 1 && last ? DP + 4 : a.D;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
             const int r = (role * NB + nb) * 8 + c2 + y;
             if (r >= a.slot_rows) continue;
-            if (g == 0) s_ml[wk][begins][r] = make_float2(m[nb][y], l[nb][y]);
+            if (g == 0) (NW == 1 ? a.part_ml[slot + r] : s_ml[wk][begins][r]) = make_float2(m[nb][y], l[nb][y]);
             float* const row = dst + r * ld_o + g;
 #pragma unroll
             for (int s = 0; s < DP / 8; ++s)
@@ -816,7 +823,7 @@ __global__ void __launch_bounds__(kWarps * 32 + (TMA ? 32 : 0), kBlocks)
         joins ? make_int4(mine_p.b, mine_p.rest, int(divide(c0 + run + mine_p.rem - 1, span)) - int(blockIdx.x) + 1, 0)
               : make_int4(0, 0, 0, 0);
   }
-  if (present == 0 || warp >= kWarps) return;
+  if (NW == 1 || present == 0 || warp >= kWarps) return;
 #pragma unroll 1
   for (int r = warp; r < a.slot_rows; r += kWarps)
 #pragma unroll 1
@@ -863,10 +870,12 @@ __global__ void __launch_bounds__(kWarps * 32 + (TMA ? 32 : 0), kBlocks)
     }
 }
 
-// Joins the parts of the items that go on from block to block, a row of one at a time: eight warps take the parts in turn, a
-// lane 4 (8 above 128) columns. A block looks through all records for the rows that are its own.
+// Joins the parts of the items that go on from block to block. WARPS warps share a row, the parts in turn: all eight of a
+// block where there are few rows, each with many parts, one where there are many rows. A lane takes 4 (8 above 128) columns.
+// A block looks through all records for its rows.
+template <int WARPS>
 __global__ void __launch_bounds__(kJoinWarps * 32) attention_paged_join_kernel(const PagedArgs a, int recs, int row_tile) {
-  __shared__ float s_acc[kJoinWarps][256];
+  __shared__ float s_acc[WARPS > 1 ? WARPS : 1][256];
   __shared__ float s_inv;
   __shared__ int s_list[kJoinMaxRecs], s_count[kJoinWarps];
   const int lane = int(threadIdx.x) & 31, warp = int(threadIdx.x) >> 5;
@@ -888,7 +897,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_paged_join_kernel(c
     if (some) s_list[before + __popc(mask & ((1u << lane) - 1u))] = i;
     __syncthreads();
   }
-  for (int task = int(blockIdx.x); task < items * a.slot_rows; task += int(gridDim.x)) {
+  constexpr int kTeams = kJoinWarps / WARPS;  // of a block
+  for (int task = int(blockIdx.x) * kTeams + warp / WARPS; task < items * a.slot_rows; task += int(gridDim.x) * kTeams) {
     const int item = a.by_slot_rows(task), row = task - item * a.slot_rows;
     const int blk = s_list[item];
     const int4 rec = a.rec[blk];
@@ -901,18 +911,19 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_paged_join_kernel(c
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     float sum = 0.0f;
-    if (warp == 0) {
+    if (WARPS == 1 || warp == 0) {
       for (int z = lane; z < parts; z += 32) {
         const float2 ml = a.part_ml[part_row(z)];
         sum = fmaf(ml.x == -INFINITY ? 0.0f : fast_exp2(ml.x - top), ml.y, sum);
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (lane == 0) s_inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // (a NaN sum makes the row NaN)
+    if (WARPS > 1 && threadIdx.x == 0) s_inv = inv;
     float acc[2][4] = {};
 #pragma unroll 4
-    for (int z = warp; z < parts; z += kJoinWarps) {
+    for (int z = WARPS == 1 ? 0 : warp; z < parts; z += WARPS) {
       const long long at = part_row(z);
       const float mz = a.part_ml[at].x;
       const float wt = mz == -INFINITY ? 0.0f : fast_exp2(mz - top);
@@ -928,19 +939,29 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_paged_join_kernel(c
         }
       }
     }
+    if constexpr (WARPS == 1) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+      for (int k = 0; k < 2; ++k) {
+        const int col = lane * 4 + k * 128;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s_acc[warp][k * 128 + lane * 4 + e] = acc[k][e];
-    __syncthreads();
-    const int col = int(threadIdx.x);
-    if (col < a.D) {
-      float x = 0.0f;
+        for (int e = 0; e < 4; ++e) acc[k][e] *= inv;
+        if (col < a.D) write_out4(a, out_row(a, rec.x, kvh, r) + col, acc[k]);
+      }
+    } else {
 #pragma unroll
-      for (int k = 0; k < kJoinWarps; ++k) x += s_acc[k][col];
-      write_out(a, out_row(a, rec.x, kvh, r) + col, x * s_inv);
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s_acc[warp][k * 128 + lane * 4 + e] = acc[k][e];
+      __syncthreads();
+      const int col = int(threadIdx.x);
+      if (col < a.D) {
+        float x = 0.0f;
+#pragma unroll
+        for (int k = 0; k < WARPS; ++k) x += s_acc[k][col];
+        write_out(a, out_row(a, rec.x, kvh, r) + col, x * s_inv);
+      }
+      __syncthreads();  // s_acc and s_inv are written again for the next row
     }
-    __syncthreads();  // s_acc and s_inv are written again for the next row
   }
 }
 
@@ -999,7 +1020,7 @@ int launch_paged(const CUtensorMap& mk, const CUtensorMap& mv, const PagedArgs& 
     ready[device] = true;
   }
   return check_cuda(launch_pdl(attention_paged_kernel<DP, WR, NB, MODS, TMA>, dim3(unsigned(blocks)),
-                               dim3(kWarps * 32 + (TMA ? 32 : 0)), smem, stream, mk, mv, a),
+                               dim3((kWarps + (TMA ? kLoadWarps : 0)) * 32), smem, stream, mk, mv, a),
                     "paged attention kernel launch");
 }
 
@@ -1157,7 +1178,10 @@ int attention_paged_launch(const AttnPagedProblem& p, cudaStream_t stream) {
   // As many rows can be left to join as items begin, one a block at most.
   const int64_t items = std::min<int64_t>(p.batch * c.kv_heads * plan.row_tiles, plan.blocks);
   static_assert(kBlocks * kWaves * 160 <= kJoinMaxRecs, "records of the join kernel");
-  return check_cuda(launch_pdl(attention_paged_join_kernel, dim3(unsigned(std::min<int64_t>(items * plan.slot_rows, dev->sms))),
+  const int64_t rows = items * plan.slot_rows;
+  const bool few = rows <= 2 * dev->sms;
+  return check_cuda(launch_pdl(few ? attention_paged_join_kernel<kJoinWarps> : attention_paged_join_kernel<1>,
+                               dim3(unsigned(std::min<int64_t>(few ? rows : (rows + kJoinWarps - 1) / kJoinWarps, 2 * dev->sms))),
                                dim3(kJoinWarps * 32), 0, stream, a, plan.blocks, 8 * plan.nb * plan.wr),
                     "paged attention join kernel launch");
 }
