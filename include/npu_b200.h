@@ -315,7 +315,7 @@ int npub200_paged_append(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh
  * kv_lens: nothing but the sizes given here decides the launch, so a captured graph follows growing lengths. Partial results
  * go to `workspace` (npub200_attention_paged_workspace_size() bytes, 16-byte aligned, contents irrelevant) and a second
  * kernel joins them in a fixed order: deterministic. Calls that can run at the same time must not share a workspace.
- * variant: 0, or the least number of 16-key tiles of one split (1 ... 2^20). Allocates nothing. */
+ * variant: 0, or the least number of key tiles (32 keys, 16 above 128 columns) of one split (1 ... 2^20). Allocates nothing. */
 int npub200_attention_paged_workspace_size(int64_t heads, int64_t kv_heads, int64_t sq, int64_t head_dim,
                                            size_t* bytes_out);
 int npub200_attention_paged(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, const npub200_paged_cache* cache,

@@ -86,7 +86,7 @@ struct PagedArgs {
   const float* slopes;
   int rows, row_tiles, slot_rows;  // rows of a (sequence, kv head), tiles of a worker's rows, rows of a part
   Divisor by_row_tiles, by_slot_rows;
-  int min_span;           // least tiles of a block's run
+  int min_span, round_span;  // least tiles of a block's run; 1: a whole number of them for each worker
   float per_block;        // 1 / blocks
   // What there is to join: of the item that begins in each block's run and goes on behind it. (sequence, kv head and row
   // tile, parts or 0, -)
@@ -213,18 +213,21 @@ __device__ __forceinline__ long long divide(long long a, long long b) {
   return ((a | b) >> 32) == 0 ? (long long)(uint32_t(a) / uint32_t(b)) : a / b;
 }
 
-// cap_out tanh(y): below 1 tanh(y) / y as a polynomial in y^2 (fit_tanh_poly.py beside this file; relative error 7e-7), which
-// keeps small values' relative accuracy, e^2y above.
-__device__ __forceinline__ float capped(float y, float cap_out) {
+// tanh(y) for |y| <= 1: y times a polynomial in y^2 (fit_tanh_poly.py beside this file; relative error 7e-7), which keeps small
+// values' relative accuracy; and for any y, by e^2y above 1.
+__device__ __forceinline__ float tanh_small(float y) {
   constexpr float kTanhRatio[6] = {9.999994040e-01f, -3.332909346e-01f, 1.328188479e-01f,
                                    -5.161965266e-02f, 1.676048711e-02f, -3.074449487e-03f};
   const float z = y * y;
   float p = kTanhRatio[5];
 #pragma unroll
   for (int i = 4; i >= 0; --i) p = fmaf(p, z, kTanhRatio[i]);
+  return p * y;
+}
+__device__ __forceinline__ float tanh_any(float y) {
   const float e = fast_exp2(2.0f * kLog2e * fabsf(y));  // (infinity ends at 1)
   const float far = copysignf(1.0f - 2.0f * fast_rcp(1.0f + e), y);
-  return cap_out * (z <= 1.0f ? p * y : far);
+  return fabsf(y) <= 1.0f ? tanh_small(y) : far;
 }
 
 __device__ __forceinline__ long long out_row(const PagedArgs& a, int b, int kvh, int r) {
@@ -419,9 +422,12 @@ __global__ void __launch_bounds__((kWarps + (TMA ? kLoadWarps : 0)) * 32, kBlock
       total += more;
     }
     total *= per_tile;
-    // (a f32 product is off by less than 1 / blocks below 2^20 tiles: one more than its whole part is never short)
+    // Whole tiles for every worker: 7 for four took as long as 8, and there were more parts to join (1 x 8192 keys, 8 heads
+    // 15.9 us, 14.4 with 8). (A f32 product is off by less than 1 / blocks below 2^20 tiles: one more than its whole part is
+    // never short.)
     span = max(total < (1 << 20) ? (long long)(float(int(total)) * a.per_block) + 1 : (total + gridDim.x - 1) / gridDim.x,
                (long long)a.min_span);
+    if (a.round_span) span = (span + NW - 1) / NW * NW;
     c0 = blockIdx.x * span;
     run = max(0ll, min(total, c0 + span) - c0);
     const long long u0 = c0 + run * wk / NW, u1 = c0 + run * (wk + 1) / NW;
@@ -628,17 +634,47 @@ __global__ void __launch_bounds__((kWarps + (TMA ? kLoadWarps : 0)) * 32, kBlock
           }
           const int j0 = (first + (half >> 1)) * KT;
           if constexpr (MODS) {
+            if (a.cap_out != 0.0f) {
+              float big = 0.0f;
 #pragma unroll
-            for (int n = 0; n < KT / 16; ++n)
+              for (int n = 0; n < KT / 16; ++n)
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    x[n][nb][e] *= a.cap_in;
+                    big = max_nan(big, fabsf(x[n][nb][e]));
+                  }
+              const bool small = __all_sync(0xffffffffu, big <= 1.0f);  // (mostly: the cap is for the rare large score)
+#pragma unroll
+              for (int n = 0; n < KT / 16; ++n)
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e)
+                    x[n][nb][e] = a.cap_out * (small ? tanh_small(x[n][nb][e]) : tanh_any(x[n][nb][e]));
+            } else {
+#pragma unroll
+              for (int n = 0; n < KT / 16; ++n)
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) x[n][nb][e] *= a.scale_log2;
+            }
+            if (a.slopes != nullptr) {
+              // The distance from f32: exact up to 2^24, rounded to a step of itself beyond.
 #pragma unroll
               for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  float& s = x[n][nb][e];
-                  s = a.cap_out != 0.0f ? capped(s * a.cap_in, a.cap_out) : s * a.scale_log2;
-                  const long long j = j0 + n * 16 + g + (e >> 1) * 8;
-                  if (a.slopes != nullptr) s = fmaf(-slope[nb][e & 1], fabsf(float(p[nb][e & 1] - j)), s);
+                for (int y = 0; y < 2; ++y) {
+                  const float ahead = float(p[nb][y] - j0 - g);
+#pragma unroll
+                  for (int n = 0; n < KT / 16; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; e += 2)
+                      x[n][nb][e + y] = fmaf(-slope[nb][y], fabsf(ahead - float(n * 16 + e * 4)), x[n][nb][e + y]);
                 }
+            }
           }
           if (j0 + KT > lim_min || valid != kAll) {
 #pragma unroll
@@ -1028,10 +1064,10 @@ template <int WR, int NB, bool MODS, bool TMA>
 int launch_paged_dim(const CUtensorMap& mk, const CUtensorMap& mv, const PagedArgs& a, int blocks, cudaStream_t stream,
                      int device) {
   if (a.D <= 64) return launch_paged<64, WR, NB, MODS, TMA>(mk, mv, a, blocks, stream, device);
-  if (TMA && a.D <= 96) return launch_paged<96, WR, NB, MODS, true>(mk, mv, a, blocks, stream, device);
+  if (a.D <= 96) return launch_paged<96, WR, NB, MODS, TMA>(mk, mv, a, blocks, stream, device);
   if (a.D <= 128) return launch_paged<128, WR, NB, MODS, TMA>(mk, mv, a, blocks, stream, device);
   if constexpr (NB == 1) {
-    if (TMA && a.D <= 160) return launch_paged<160, WR, 1, MODS, true>(mk, mv, a, blocks, stream, device);
+    if (a.D <= 160) return launch_paged<160, WR, 1, MODS, TMA>(mk, mv, a, blocks, stream, device);
     if (a.D <= 192) return launch_paged<192, WR, 1, MODS, TMA>(mk, mv, a, blocks, stream, device);
     return launch_paged<256, WR, 1, MODS, TMA>(mk, mv, a, blocks, stream, device);
   }
@@ -1144,7 +1180,8 @@ int attention_paged_launch(const AttnPagedProblem& p, cudaStream_t stream) {
   a.by_g = divisor(a.G);
   a.by_row_tiles = divisor(a.row_tiles);
   a.by_slot_rows = divisor(a.slot_rows);
-  a.min_span = p.variant > 0 ? p.variant : 8;
+  a.min_span = p.variant > 0 ? p.variant : 1;
+  a.round_span = p.variant == 0;
   a.per_block = 1.0f / float(plan.blocks);
   uint8_t* ws = static_cast<uint8_t*>(p.workspace);
   a.rec = reinterpret_cast<int4*>(ws);

@@ -709,7 +709,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     softcap, slopes: as in attention. A row that may see no key is zero, one that sees a NaN score NaN; v has to be finite
                 at every key that some row sees.
     The batch's keys are split evenly over the GPU whatever the lengths. Made for few tokens; the attention of a prompt is
-    `attention`, on its own keys. variant: the least number of 16-key tiles of one split (0 = automatic).
+    `attention`, on its own keys. variant: the least number of key tiles of one split (0 = automatic).
     """
     _require_cuda(q, "q")
     if softcap is not None and not 1e-30 <= softcap <= 1e30:
