@@ -30,6 +30,7 @@
 #include <type_traits>
 
 #include "attention_sm100.cuh"
+#include "fast_div.cuh"
 #include "internal.h"
 
 namespace npub200 {
@@ -47,18 +48,6 @@ constexpr int kJoinMaxRecs = 1024;  // blocks whose records the join kernel look
 // The row maximum moves only when a tile's beats it by this much (log2 units): P stays within 2^8 of 1, which bf16 holds
 // with the same relative rounding, and the O registers are rescaled once in a while instead of once a tile.
 constexpr float kRescale = 8.0f;
-
-// n / d for 0 <= n < 2^31 by a multiplication: with p = 31 + ceil(log2 d) and mul = ceil(2^p / d), n mul / 2^p is above
-// n / d by less than 1 / d.
-struct Divisor {
-  uint32_t mul, shift;
-  __device__ __forceinline__ int operator()(int n) const { return int((uint64_t(uint32_t(n)) * mul) >> shift); }
-};
-Divisor divisor(int64_t d) {
-  int log = 0;
-  while ((int64_t(1) << log) < d) ++log;
-  return Divisor{uint32_t(((uint64_t(1) << (31 + log)) + uint64_t(d) - 1) / uint64_t(d)), uint32_t(31 + log)};
-}
 
 struct PagedArgs {
   const __nv_bfloat16* q;

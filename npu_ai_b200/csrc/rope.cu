@@ -13,6 +13,7 @@
 #include <cmath>
 #include <cstring>
 
+#include "fast_div.cuh"
 #include "internal.h"
 
 namespace npub200 {
@@ -22,7 +23,7 @@ namespace {
 constexpr int kRopeThreads = 256;
 constexpr int kRopeMaxTokens = 16;         // tokens of a block
 constexpr int kRopeTableBytes = 32 * 1024;  // (cos, sin) of a block's tokens
-constexpr int kRopeBlockBytes = 32 * 1024;  // source bytes of a block where there are enough tokens
+constexpr int kRopeBlockBytes = 128 * 1024;  // source bytes of a block, at most, where there are enough tokens
 
 // Element (b, s, h, e) at b*sb + s*ss + h*sh + e.
 struct RopeRows {
@@ -37,6 +38,8 @@ struct RopeArgs {
   long long tokens;
   int seq, dim, half, rot_units, units;  // units of a head: rot_units rotated ones, the rest copied
   int block_tokens, chunk;               // tokens and heads of a block
+  int places, groups;                    // units of a block's tokens, threads that share the heads of one
+  Divisor by_units, by_places, by_seq, by_half;
   int inverse;
   float magnitude;
   const double* freqs;
@@ -51,39 +54,42 @@ struct RopeArgs {
   int page_size;
 };
 
+// V values as they lie in memory, and as f32.
 template <typename T, int V>
-__device__ __forceinline__ void load_values(const T* p, float (&f)[V]) {
-  if constexpr (sizeof(T) == 4) {
-    if constexpr (V >= 4) {
+struct Values {
+  static constexpr int kWords = V * int(sizeof(T)) / 4 > 0 ? V * int(sizeof(T)) / 4 : 1;
+  uint32_t w[kWords];
+
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (sizeof(T) == 4) {
+      if constexpr (V >= 4) {
 #pragma unroll
-      for (int i = 0; i < V; i += 4) {
-        const float4 x = *reinterpret_cast<const float4*>(p + i);
-        f[i] = x.x, f[i + 1] = x.y, f[i + 2] = x.z, f[i + 3] = x.w;
+        for (int i = 0; i < V; i += 4) {
+          const uint4 x = *reinterpret_cast<const uint4*>(p + i);
+          w[i] = x.x, w[i + 1] = x.y, w[i + 2] = x.z, w[i + 3] = x.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) w[i] = __float_as_uint(p[i]);
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) f[i] = p[i];
-    }
-  } else if constexpr (V == 1) {
-    f[0] = __bfloat162float(*p);
-  } else {
-    uint32_t w[V / 2];
-    if constexpr (V == 8) {
+    } else if constexpr (V == 8) {
       const uint4 x = *reinterpret_cast<const uint4*>(p);
       w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
     } else if constexpr (V == 4) {
       const uint2 x = *reinterpret_cast<const uint2*>(p);
       w[0] = x.x, w[1] = x.y;
-    } else {  // two values, which need not lie on a 4-byte boundary
-      w[0] = uint32_t(*reinterpret_cast<const uint16_t*>(p)) | uint32_t(*reinterpret_cast<const uint16_t*>(p + 1)) << 16;
-    }
-#pragma unroll
-    for (int i = 0; i < V / 2; ++i) {
-      f[2 * i] = __uint_as_float(w[i] << 16);
-      f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    } else {  // one or two values, which need not lie on a 4-byte boundary
+      w[0] = *reinterpret_cast<const uint16_t*>(p);
+      if constexpr (V == 2) w[0] |= uint32_t(*reinterpret_cast<const uint16_t*>(p + 1)) << 16;
     }
   }
-}
+  __device__ __forceinline__ void unpack(float (&f)[V]) const {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      f[i] = sizeof(T) == 4 ? __uint_as_float(w[i])
+                            : __uint_as_float(i & 1 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+  }
+};
 
 template <typename T, int V>
 __device__ __forceinline__ void store_values(T* p, const float (&f)[V]) {
@@ -108,7 +114,7 @@ __device__ __forceinline__ void store_values(T* p, const float (&f)[V]) {
 
 // What a block keeps of each of its tokens.
 struct RopeToken {
-  long long src[3], dst[3];  // offsets of the token's first head; dst < 0: nothing is written
+  long long dst[3];  // offset of the token's first head in each destination; < 0: nothing is written
 };
 
 // V values a vector. Half layout: a rotated unit is the vectors at j and j + r/2; interleaved: one vector of V/2 pairs.
@@ -116,13 +122,11 @@ template <typename TIn, typename TOut, int V, bool IL, bool PAGED>
 __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
   extern __shared__ float2 s_turn[];  // [block_tokens][half] (m cos, m sin)
   __shared__ RopeToken s_token[kRopeMaxTokens];
-  constexpr int TENSORS = PAGED ? 3 : 1;
   const int tid = int(threadIdx.x);
   const long long first = (long long)blockIdx.x * a.block_tokens;
   const int n = int(min((long long)a.block_tokens, a.tokens - first));
   pdl_wait();
   pdl_launch_dependents();
-
   __shared__ long long s_pos[kRopeMaxTokens];
   if (tid < n) {
     const long long token = first + tid, b = token / a.seq, s = token - b * a.seq;
@@ -133,8 +137,6 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
   if (tid < n) {
     const long long token = first + tid, b = token / a.seq, s = token - b * a.seq;
     RopeToken t;
-#pragma unroll
-    for (int k = 0; k < TENSORS; ++k) t.src[k] = b * a.src[k].sb + s * a.src[k].ss;
     t.dst[0] = b * a.dst[0].sb + s * a.dst[0].ss;
     if constexpr (PAGED) {
       const long long p = s_pos[tid];
@@ -151,7 +153,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
     s_token[tid] = t;
   }
   for (int i = tid; i < n * a.half; i += kRopeThreads) {
-    const int t = i / a.half, j = i - t * a.half;
+    const int t = a.by_half(i), j = i - t * a.half;
     double turns = double(s_pos[t]) * (a.freqs[j] * 0.15915494309189535);  // 1 / (2 pi)
     turns -= rint(turns);
     float sn, cs;
@@ -160,73 +162,94 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
   }
   __syncthreads();
 
+  // A thread keeps one place of a head (a token's unit: V or 2 V values) with its angles in registers and walks over the
+  // heads, the threads with the same place sharing them.
+  constexpr int TENSORS = PAGED ? 3 : 1;
   const int h0 = int(blockIdx.y) * a.chunk;
   const int heads = min(a.chunk, a.heads[0] + (PAGED ? a.heads[1] + a.heads[2] : 0) - h0);
-  const int total = n * heads * a.units;
-  constexpr int UN = 2;  // units whose loads are in flight together
-  for (int u0 = tid; u0 < total; u0 += UN * kRopeThreads) {
-    float lo[UN][V], hi[UN][V];
-    TOut* out[UN];
-    int unit[UN], tok[UN];
-    bool turn[UN];
+  for (int place = tid - a.by_places(tid) * min(a.places, kRopeThreads), group = a.by_places(tid); place < a.places && group < a.groups;
+       place += a.places > kRopeThreads ? kRopeThreads : a.places) {
+    const int tok = a.by_units(place), unit = place - tok * a.units;
+    if (tok >= n) break;
+    const bool rotated = unit < a.rot_units, pair = !IL && rotated;
+    const int e = IL || rotated ? unit * V : 2 * a.half + (unit - a.rot_units) * V;  // the unit's first value
+    constexpr int ANGLES = IL ? V / 2 : V;
+    float cs[ANGLES], sn[ANGLES];
+    if (rotated) {
 #pragma unroll
-    for (int k = 0; k < UN; ++k) {
-      out[k] = nullptr;
-      const int u = u0 + k * kRopeThreads;
-      if (u >= total) continue;
-      const int row = u / a.units;
-      unit[k] = u - row * a.units;
-      tok[k] = row / heads;
-      int h = h0 + row - tok[k] * heads;
-      int which = 0;
-      if constexpr (PAGED) {
-        if (h >= a.heads[0]) {
-          h -= a.heads[0];
-          which = 1;
-          if (h >= a.heads[1]) {
-            h -= a.heads[1];
-            which = 2;
-          }
-        }
+      for (int i = 0; i < ANGLES; ++i) {
+        const float2 w = s_turn[tok * a.half + unit * ANGLES + i];
+        cs[i] = w.x;
+        sn[i] = w.y;
       }
-      const RopeToken& t = s_token[tok[k]];
-      const long long dst = t.dst[which];
-      if (PAGED && dst < 0) continue;
-      turn[k] = which != 2 && unit[k] < a.rot_units;
-      // the first value of the unit; units behind the rotated ones are single vectors of the rest
-      const int e = IL || unit[k] < a.rot_units ? unit[k] * V : 2 * a.half + (unit[k] - a.rot_units) * V;
-      const RopeRows& from = a.src[which];
-      const TIn* x = static_cast<const TIn*>(from.p) + (t.src[which] + h * from.sh + e);
-      out[k] = static_cast<TOut*>(const_cast<void*>(a.dst[which].p)) + (dst + h * a.dst[which].sh + e);
-      load_values<TIn, V>(x, lo[k]);
-      if (!IL && unit[k] < a.rot_units) load_values<TIn, V>(x + a.half, hi[k]);
     }
+    const int token = int(first) + tok;  // (fewer than 2^31 tokens)
+    const long long b = a.by_seq(token), s = token - b * a.seq;
+    const TIn* src[TENSORS];
+    TOut* dst[TENSORS];  // null: nothing is written
 #pragma unroll
-    for (int k = 0; k < UN; ++k) {
-      if (out[k] == nullptr) continue;
-      const bool pair = !IL && unit[k] < a.rot_units;
-      if (turn[k]) {
-        const float2* cs = s_turn + tok[k] * a.half + (IL ? unit[k] * (V / 2) : unit[k] * V);
-        if constexpr (IL) {
+    for (int k = 0; k < TENSORS; ++k) {
+      const long long at = s_token[tok].dst[k];
+      src[k] = static_cast<const TIn*>(a.src[k].p) + (b * a.src[k].sb + s * a.src[k].ss + e);
+      dst[k] = at < 0 ? nullptr : static_cast<TOut*>(const_cast<void*>(a.dst[k].p)) + (at + e);
+    }
+    // Units whose loads are in flight together, of one tensor or the next: 64 bytes a thread.
+    constexpr int UNIT = V * int(sizeof(TIn)) * (IL ? 1 : 2), UN = UNIT >= 64 ? 1 : UNIT >= 16 ? 64 / UNIT : 4;
+    for (int h = h0 + group; h < h0 + heads; h += UN * a.groups) {
+      Values<TIn, V> lo[UN], hi[UN];
+      TOut* out[UN];
+      bool turn[UN];
 #pragma unroll
-          for (int i = 0; i < V / 2; ++i) {
-            const float2 w = cs[i];
-            const float x = lo[k][2 * i], y = lo[k][2 * i + 1];
-            lo[k][2 * i] = x * w.x - y * w.y;
-            lo[k][2 * i + 1] = y * w.x + x * w.y;
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float2 w = cs[i];
-            const float x = lo[k][i], y = hi[k][i];
-            lo[k][i] = x * w.x - y * w.y;
-            hi[k][i] = y * w.x + x * w.y;
+      for (int k = 0; k < UN; ++k) {
+        int hk = h + k * a.groups;
+        out[k] = nullptr;
+        if (hk >= h0 + heads) continue;
+        const TIn* in = src[0];
+        long long in_sh = a.src[0].sh, out_sh = a.dst[0].sh;
+        out[k] = dst[0];
+        turn[k] = rotated;
+        if constexpr (PAGED) {
+          if (hk >= a.heads[0]) {
+            const bool value = hk >= a.heads[0] + a.heads[1];
+            hk -= a.heads[0] + (value ? a.heads[1] : 0);
+            in = src[value ? 2 : 1];
+            in_sh = value ? a.src[2].sh : a.src[1].sh;
+            out[k] = dst[value ? 2 : 1];
+            out_sh = value ? a.dst[2].sh : a.dst[1].sh;
+            turn[k] = rotated && !value;
           }
         }
+        if (out[k] == nullptr) continue;
+        out[k] += hk * out_sh;
+        lo[k].load(in + hk * in_sh);
+        if (pair) hi[k].load(in + hk * in_sh + a.half);
       }
-      store_values<TOut, V>(out[k], lo[k]);
-      if (pair) store_values<TOut, V>(out[k] + a.half, hi[k]);
+#pragma unroll
+      for (int k = 0; k < UN; ++k) {
+        if (out[k] == nullptr) continue;
+        float u[V], v[V];
+        lo[k].unpack(u);
+        if (pair) hi[k].unpack(v);
+        if (turn[k]) {
+          if constexpr (IL) {
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+              const float x = u[2 * i], y = u[2 * i + 1];
+              u[2 * i] = x * cs[i] - y * sn[i];
+              u[2 * i + 1] = y * cs[i] + x * sn[i];
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              const float x = u[i], y = v[i];
+              u[i] = x * cs[i] - y * sn[i];
+              v[i] = y * cs[i] + x * sn[i];
+            }
+          }
+        }
+        store_values<TOut, V>(out[k], u);
+        if (pair) store_values<TOut, V>(out[k] + a.half, v);
+      }
     }
   }
 }
@@ -248,7 +271,9 @@ template <typename TIn, typename TOut, bool PAGED>
 int launch_rope_for(RopeArgs& a, int rot, bool interleaved, cudaStream_t stream, int sms) {
   // The widest vectors that every tensor's alignment and the rotated part's width allow; pairs lie within a vector or in
   // two of them, so a rotated part that is no whole number of vectors takes narrower ones.
-  int V = 8;
+  // (Half layout: two vectors a unit, and angles for each: with 8 values 80 registers and three blocks an SM, 16384 x 40 x 128
+  // 64 us, with 4 values 58.)
+  int V = interleaved ? 8 : 4;
   for (; V > (interleaved ? 2 : 1); V = V == 8 ? 4 : interleaved ? 2 : 1) {
     bool fit = a.dim % V == 0 && (interleaved ? rot : rot / 2) % V == 0;
     for (int k = 0; k < (PAGED ? 3 : 1); ++k)
@@ -262,6 +287,7 @@ int launch_rope_for(RopeArgs& a, int rot, bool interleaved, cudaStream_t stream,
   long long tb = kRopeBlockBytes / ((long long)heads * a.dim * (int)sizeof(TIn));
   if (a.half > 0) tb = std::min<long long>(tb, kRopeTableBytes / (a.half * (int)sizeof(float2)));
   tb = std::max<long long>(1, std::min<long long>(tb, kRopeMaxTokens));
+  while (tb & (tb - 1)) tb &= tb - 1;  // a power of two, whose units mostly divide the threads: with 9 tokens 144 of 256 worked
   while (tb > 1 && (a.tokens + tb - 1) / tb < 2 * sms) tb /= 2;
   a.block_tokens = int(tb);
   const long long blocks = (a.tokens + tb - 1) / tb;
@@ -269,6 +295,12 @@ int launch_rope_for(RopeArgs& a, int rot, bool interleaved, cudaStream_t stream,
   const long long wish = std::min<long long>(std::max<long long>(1, sms / blocks),
                                              std::max<long long>(1, (long long)heads * a.units * tb / kRopeThreads));
   a.chunk = int((heads + wish - 1) / wish);
+  a.places = a.block_tokens * a.units;
+  a.groups = std::max(1, kRopeThreads / a.places);
+  a.by_units = divisor(a.units);
+  a.by_places = divisor(std::min(a.places, kRopeThreads));
+  a.by_seq = divisor(a.seq);
+  a.by_half = divisor(std::max(1, a.half));
   const dim3 grid(unsigned(blocks), unsigned((heads + a.chunk - 1) / a.chunk));
   const size_t smem = size_t(tb) * a.half * sizeof(float2);
   if (interleaved) {
@@ -276,7 +308,6 @@ int launch_rope_for(RopeArgs& a, int rot, bool interleaved, cudaStream_t stream,
     if (V == 4) return launch_rope<TIn, TOut, 4, true, PAGED>(a, grid, smem, stream);
     return launch_rope<TIn, TOut, 2, true, PAGED>(a, grid, smem, stream);
   }
-  if (V == 8) return launch_rope<TIn, TOut, 8, false, PAGED>(a, grid, smem, stream);
   if (V == 4) return launch_rope<TIn, TOut, 4, false, PAGED>(a, grid, smem, stream);
   return launch_rope<TIn, TOut, 1, false, PAGED>(a, grid, smem, stream);
 }
