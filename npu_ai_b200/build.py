@@ -6,7 +6,7 @@
 The libraries land next to this file so they travel with the source tree; no JIT cache, no site-packages install:
   * ``npu_ai_b200/libnpub200.so``: every ``csrc/*.cu`` (kernels + C ABI), objects in ``npu_ai_b200/_build/``;
   * ``npu_ai_b200/libnpub200_torch.so``: ``csrc/torch_ops.cpp``, the TORCH_LIBRARY(npub200) operators
-    (torch.ops.npub200.gemm / .attention / .attention_masked), linked against libnpub200.so and torch.
+    (torch.ops.npub200.gemm / .attention / .attention_masked / .rope / .paged_append / .attention_paged), linked against libnpub200.so and torch.
 """
 from __future__ import annotations
 

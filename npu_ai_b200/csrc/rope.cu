@@ -8,7 +8,11 @@
 // input's type) and is rounded once.
 //
 // Bound by memory: each value is read once and written once. A block owns a few tokens and a chunk of their heads; it works
-// out its tokens' (cos, sin) once into shared memory, for all heads, then streams the heads in vectors of up to 8 values.
+// out its tokens' (cos, sin) once into shared memory, a thread takes those of one place of a head into registers and walks over
+// the heads. (With a table read for each vector 16384 x 40 x 128 took 72 us instead of 58: eight lanes' reads of it met in the
+// same banks.) 58 us are 5.8 TB/s, 88% of the measured copy rate; pairs next to each other 56.8 us; 8192 tokens of f32 to bf16
+// 42.6 us, 90%; the append of 2 x 8192 tokens with 32 + 8 + 8 heads of 128 76 us, 80%: its start (positions, the page table,
+// the angles) passes without loads in flight.
 #include <algorithm>
 #include <cmath>
 #include <cstring>

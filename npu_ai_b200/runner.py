@@ -10,6 +10,7 @@ the NPU runner (its ComfyUI node, its test scripts) run unchanged:
   prepare(shapes), dispatch_shapes(M,K,N)   xdna1_gemm.py:295-308
   attention(q, k, v, heads, scale=None, skip_reshape=False, skip_output_reshape=False)   xdna1_gemm.py:499-600
                                             (also masked and with grouped key/value heads: kernels.attention)
+  rope / paged_append / paged_attention   (beyond the reference: a text model's cached steps, kernels.py)
   attention_fits / attention_warmup / attention_fused_fits                              xdna1_gemm.py:451-497
   summary(), stats, pool                    xdna1_gemm.py:201-209, :755-773
 
@@ -404,6 +405,49 @@ class NpuGemm:
             self.stats["attn_fused_flops"] += 4.0 * b * h * tq * tk * d
             self.stats["attn_fused_seconds"] += wall
         return y
+
+    # -- a text model's cached steps ------------------------------------------------------------
+    def _on_device(self, t, dtype: torch.dtype | None = None):
+        """Tensors go to this runner's device (and type); anything else (ints, None) is passed on."""
+        return t.detach().to(self.device, dtype) if isinstance(t, torch.Tensor) else t
+
+    def _turned(self, t) -> torch.Tensor:
+        """An operand of a rotation on this device: bf16 and f32 as they are, other types as f32."""
+        t = self._on_device(_as_tensor(t))
+        if t.dtype not in (torch.bfloat16, torch.float32):
+            t = t.float()
+        return t if t.stride(-1) == 1 else t.contiguous()
+
+    def rope(self, x, freqs: torch.Tensor, heads: int, positions: int | torch.Tensor = 0, **rotation) -> torch.Tensor:
+        """Rotary positions (kernels.rope and its keywords): x (B, S, heads*D), or (B, heads, S, D) with head_major, on any
+        device -> a CUDA tensor of its type (other float types than bf16 become f32) unless `out_dtype` says otherwise."""
+        return kernels.rope(self._turned(x), self._on_device(freqs, torch.float64), heads,
+                            self._on_device(positions, torch.int32), **rotation)
+
+    def paged_append(self, k, v, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                     starts: torch.Tensor, *, counts: torch.Tensor | None = None, q=None, freqs: torch.Tensor | None = None,
+                     **more) -> torch.Tensor | None:
+        """New keys and values into the pages of a cache, keys and queries rotated on the way (kernels.paged_append and its
+        keywords). k, v and q may lie on any device; the pages are this device's bf16 tensors, written in place."""
+        ops = [self._turned(t) if t is not None else None for t in (k, v, q)]
+        if any(t is not None and t.dtype != ops[0].dtype for t in ops):
+            ops = [t.float() if t is not None else None for t in ops]
+        k, v, q = ops
+        return kernels.paged_append(k, v, k_pages, v_pages, self._on_device(page_table, torch.int32),
+                                    self._on_device(starts, torch.int32), counts=self._on_device(counts, torch.int32), q=q,
+                                    freqs=self._on_device(freqs, torch.float64), **more)
+
+    def paged_attention(self, q, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                        kv_lens: torch.Tensor, heads: int, scale: float | None = None, *,
+                        q_start: torch.Tensor | None = None, slopes: torch.Tensor | None = None,
+                        out_dtype: torch.dtype | None = None, **more) -> torch.Tensor:
+        """Attention of a few new tokens of each sequence over its pages (kernels.paged_attention and its keywords); q on any
+        device and of any float type (bf16 in the kernel), f32 out unless `out_dtype` says otherwise."""
+        return kernels.paged_attention(self._attn_operand(q), k_pages, v_pages, self._on_device(page_table, torch.int32),
+                                       self._on_device(kv_lens, torch.int32), heads, scale,
+                                       q_start=self._on_device(q_start, torch.int32),
+                                       slopes=self._on_device(slopes, torch.float32),
+                                       out_dtype=out_dtype or self.out_dtype, **more)
 
     # -- reporting ------------------------------------------------------------------------------
     def summary(self) -> str:

@@ -182,3 +182,24 @@ def test_frequencies():
 def test_frequencies_refuse(kw):
     with pytest.raises(ValueError):
         kernels.rope_frequencies(**{"rot_dim": 64, **kw})
+
+
+def test_tanh_of_the_cap_is_the_fitted_polynomial():
+    """The cap's coefficients are those of the masked attention, which are fitted and checked by their own test."""
+    csrc = os.path.join(ROOT, "npu_ai_b200", "csrc")
+    found = [re.search(r"kTanhRatio\[6\] = \{(.*?)\}", open(os.path.join(csrc, f)).read(), re.S).group(1)
+             for f in ("attention_masked.cuh", "attention_paged.cu")]
+    a, b = ([float(x.rstrip("f")) for x in re.findall(r"-?\d[\d.e+-]*f", s)] for s in found)
+    assert a == b and len(a) == 6
+
+
+@pytest.mark.parametrize("d", list(range(1, 70)) + [127, 128, 129, 1000, 65535, 2 ** 20 + 1, 2 ** 30 - 1, 2 ** 30])
+def test_division_by_multiplication(d):
+    """csrc/fast_div.cuh: the same arithmetic on whole numbers, at the quotients' borders over its range."""
+    log = max(0, (d - 1).bit_length())
+    mul, shift = -(-2 ** (31 + log) // d), 31 + log
+    assert mul < 2 ** 32
+    for q in {0, 1, 2, (2 ** 31 - 1) // d // 2, (2 ** 31 - 1) // d}:
+        for n in (q * d - 1, q * d, q * d + d - 1):
+            if 0 <= n < 2 ** 31:
+                assert (n * mul) >> shift == n // d

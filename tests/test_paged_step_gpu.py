@@ -82,3 +82,32 @@ def test_prompt_and_continuation(cuda_device, heads, kv_heads, page, interleaved
             tok.copy_(t)
             graph.replay()
             assert torch.equal(out, want)
+
+
+def test_runner_methods(cuda_device):
+    """NpuGemm's methods take tensors of any device and float type; the same results as the functions they wrap."""
+    from npu_ai_b200 import kernels
+    from npu_ai_b200.runner import NpuGemm
+    g = NpuGemm()
+    dev, H, hk, D, page = g.device, 4, 2, 64, 16
+    f, m = kernels.rope_frequencies(D)
+    x = torch.randn(2, 3, H * D, dtype=torch.float64)
+    y = g.rope(x, f, H, torch.tensor([5, 9]), magnitude=1.5)
+    assert y.is_cuda and y.dtype == torch.float32
+    assert torch.equal(y, kernels.rope(x.float().to(dev), f.to(dev), H, torch.tensor([5, 9], dtype=torch.int32, device=dev),
+                                       magnitude=1.5))
+    table = torch.arange(4).view(2, 2)
+    starts = torch.tensor([0, 20])
+    q, k, v = (torch.randn(2, 3, n * D) for n in (H, hk, hk))
+    pools = [torch.zeros(4, page, hk, D, dtype=BF16, device=dev) for _ in range(4)]
+    turned = g.paged_append(k, v.to(BF16), pools[0], pools[1], table, starts, q=q, heads=H, freqs=f)
+    i32 = [t.to(dev, torch.int32) for t in (table, starts)]
+    want = kernels.paged_append(k.to(dev), v.to(BF16).float().to(dev), pools[2], pools[3], *i32, q=q.to(dev), heads=H,
+                                freqs=f.to(dev))
+    assert torch.equal(turned, want) and torch.equal(pools[0], pools[2]) and torch.equal(pools[1], pools[3])
+    o = g.paged_attention(turned.cpu(), pools[0], pools[1], table, starts + 3, H, softcap=20.0)
+    assert o.dtype == torch.float32
+    assert torch.equal(o, kernels.paged_attention(want, pools[2], pools[3], i32[0], i32[1] + 3, H, softcap=20.0))
+    assert torch.equal(g.paged_attention(turned, pools[0], pools[1], table, starts + 3, H, q_start=starts, out_dtype=BF16),
+                       kernels.paged_attention(want, pools[2], pools[3], i32[0], i32[1] + 3, H, q_start=i32[1], out_dtype=BF16))
+    kernels.check_status(dev)
