@@ -1180,7 +1180,11 @@ int attention_paged_launch(const AttnPagedProblem& p, cudaStream_t stream) {
   a.ctl.status = dev->status;
   a.ctl.timeout_ns = wait_timeout_ns();
   a.ctl.debug = p.debug;
-  // TMA takes 16 slots of a page at a time, and maps of positive strides below 2^40 bytes.
+  // TMA takes 16 slots of a page at a time, and maps of positive strides below 2^40 bytes. It moves 128 bytes of a row a step,
+  // whatever part of them the head fills, so heads that are no multiple of 128 are copied faster by cp.async where there is much
+  // to read (16 x 16384 keys of 64: 96 us, by TMA 104; 16 x 8000 of 80: 126 and 143; of 128: 137 and 133), while it starts sooner
+  // (777 keys of 64: 9.0 us, by cp.async 11).
+  const bool few_keys = p.batch * c.kv_heads * (a.capacity / 32 + 1) <= int64_t(plan.blocks) * 8;
   CUtensorMap mk, mv;
   memset(&mk, 0, sizeof(mk));
   memset(&mv, 0, sizeof(mv));
@@ -1188,7 +1192,7 @@ int attention_paged_launch(const AttnPagedProblem& p, cudaStream_t stream) {
     const auto fits = [](int64_t n, int64_t s) { return n == 1 || (s > 0 && s < (int64_t(1) << 38)); };
     return fits(c.pages, sp) && fits(c.page_size, ss) && fits(c.kv_heads, sh);
   };
-  const bool tma = c.page_size % 16 == 0 && c.pages > 0 && strided(c.k_sp, c.k_ss, c.k_sh) && strided(c.v_sp, c.v_ss, c.v_sh);
+  const bool tma = (c.head_dim % 128 == 0 || few_keys) && c.page_size % 16 == 0 && c.pages > 0 && strided(c.k_sp, c.k_ss, c.k_sh) && strided(c.v_sp, c.v_ss, c.v_sh);
   const int tile = c.head_dim <= 128 ? 32 : 16;  // (PagedLayout::kTile)
   a.box_rows = c.page_size % tile == 0 ? tile : 16;
   if (tma) {
