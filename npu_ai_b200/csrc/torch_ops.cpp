@@ -371,6 +371,13 @@ void check_written(const at::Tensor& t, const char* name, const at::Tensor* from
                     " must be the input itself or share no element with it");
 }
 
+// Two tensors of which one is written while the other is read, or both are written: nothing in common, as far as their strides
+// tell.
+void check_apart(const at::Tensor& a, const at::Tensor& b, const char* names) {
+  const auto s = at::get_overlap_status(a, b);
+  TORCH_CHECK_VALUE(s != at::MemOverlapStatus::Full && s != at::MemOverlapStatus::Partial, names, " must not overlap");
+}
+
 // Rotary positions (npub200_rope): x (B, S, heads * d), or (B, heads, S, d) when head-major, like the result.
 at::Tensor rope(const at::Tensor& x, const at::Tensor& freqs, int64_t heads, const std::optional<at::Tensor>& out_arg,
                 std::optional<at::ScalarType> out_dtype, int64_t start, const std::optional<at::Tensor>& positions,
@@ -448,6 +455,7 @@ std::optional<at::Tensor> paged_append(const at::Tensor& k, const at::Tensor& v,
                     v.scalar_type(), " ", v.sizes());
   check_written(k_pages, "k_pages");
   check_written(v_pages, "v_pages");
+  check_apart(k_pages, v_pages, "k_pages and v_pages");
   const int32_t* starts_ptr = vector_ptr<int32_t>(starts, k_pages, B, "starts");
   const int32_t* counts_ptr = vector_ptr<int32_t>(counts, k_pages, B, "counts");
   npub200_rotation r = {};
@@ -464,6 +472,8 @@ std::optional<at::Tensor> paged_append(const at::Tensor& k, const at::Tensor& v,
       TORCH_CHECK_VALUE(q_out->sizes() == q->sizes() && q_out->scalar_type() == at::kBFloat16,
                         "q_out must be bf16 with q's shape ", q->sizes(), ", got ", q_out->scalar_type(), " ", q_out->sizes());
       check_written(*q_out, "q_out", &*q);
+      check_apart(*q_out, k, "q_out and k");
+      check_apart(*q_out, v, "q_out and v");
       out = *q_out;
     } else {
       out = at::empty(q->sizes(), k_pages.options());

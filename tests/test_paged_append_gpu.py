@@ -167,7 +167,11 @@ def test_empty_calls_and_refusals(cuda_device):
                 dict(q=q, heads=3, freqs=f), dict(q=q.float(), heads=H, freqs=f), dict(q=q[:1], heads=H, freqs=f),
                 dict(q_out=q, freqs=f), dict(q=q, heads=H, freqs=f, q_out=q.float()), dict(freqs=f.float()),
                 dict(freqs=torch.cat((f, f))), dict(k=torch.cat((k, k), -1)), dict(kp=kp[:1].expand(4, 8, hk, D)),
-                dict(k=k.cpu()), dict(vp=vp.cpu()), dict(kp=kp.mT), dict(freqs=f, magnitude=float("inf"))):
+                dict(k=k.cpu()), dict(vp=vp.cpu()), dict(kp=kp.mT), dict(freqs=f, magnitude=float("inf")), dict(vp=kp)):
         with pytest.raises(ValueError):
             call(**bad)
     assert bool((kp == 0).all()) and bool((vp == 0).all())
+    mha = make(dev, B, S, H, D, BF16, False)
+    kp4, vp4 = pool(dev, 4, 8, H, D, fill=0.0)
+    with pytest.raises(ValueError, match="overlap"):
+        kernels.paged_append(mha, mha.clone(), kp4, vp4, table, ints, q=mha.clone(), heads=H, freqs=f, q_out=mha)
