@@ -1018,10 +1018,11 @@ int check_paged_sizes(int64_t H, int64_t Hk, int64_t Sq, int64_t D) {
 PagedPlan plan_paged(int64_t H, int64_t Hk, int64_t Sq, int64_t D, int sms) {
   PagedPlan p;
   p.rows = H / Hk * Sq;
-  // Two blocks of rows a warp from 17 rows on, where reading the keys from shared memory for each block decides; above 128
-  // columns their O does not fit the registers.
-  p.nb = p.rows > 16 && D <= 128 ? 2 : 1;
-  p.wr = p.rows <= 8 ? 1 : p.rows <= 16 * p.nb ? 2 : 4;
+  // Two blocks of rows a warp from 33 rows on, where reading the keys from shared memory for each block decides (4 x 16 tokens,
+  // 32/8 heads, 9000 keys: 73 us, 110 with one); above 128 columns their O does not fit the registers. With 20 rows two warps
+  // of two blocks took 25 us, four of one 17.
+  p.nb = p.rows > 32 && D <= 128 ? 2 : 1;
+  p.wr = p.rows <= 8 ? 1 : p.rows <= 16 ? 2 : 4;
   const int64_t tile = 8 * p.nb * p.wr;
   p.row_tiles = (p.rows + tile - 1) / tile;
   p.slot_rows = p.rows < tile ? p.rows : tile;
@@ -1069,9 +1070,7 @@ int launch_paged_dim(const CUtensorMap& mk, const CUtensorMap& mv, const PagedAr
 template <bool MODS, bool TMA>
 int launch_paged_rows(const CUtensorMap& mk, const CUtensorMap& mv, const PagedArgs& a, const PagedPlan& p,
                       cudaStream_t stream, int device) {
-  if (p.nb == 2)
-    return p.wr == 2 ? launch_paged_dim<2, 2, MODS, TMA>(mk, mv, a, p.blocks, stream, device)
-                     : launch_paged_dim<4, 2, MODS, TMA>(mk, mv, a, p.blocks, stream, device);
+  if (p.nb == 2) return launch_paged_dim<4, 2, MODS, TMA>(mk, mv, a, p.blocks, stream, device);
   if (p.wr == 1) return launch_paged_dim<1, 1, MODS, TMA>(mk, mv, a, p.blocks, stream, device);
   if (p.wr == 2) return launch_paged_dim<2, 1, MODS, TMA>(mk, mv, a, p.blocks, stream, device);
   return launch_paged_dim<4, 1, MODS, TMA>(mk, mv, a, p.blocks, stream, device);
