@@ -280,7 +280,7 @@ int npub200_rope(const void* x, int64_t x_sb, int64_t x_ss, int64_t x_sh, int x_
  * page table[b * table_stride + p / page_size]. Element (page, slot, head, e) of the keys at page*k_sp + slot*k_ss +
  * head*k_sh + e, so both orders of slots and heads are strided views; bf16. A page may stand in several tables. A page id
  * outside [0, pages) is a page that is not there: nothing is written to it and its keys are seen by no row. A sequence's
- * pages hold at most 2^30 tokens.
+ * pages hold at most 2^30 - 32 tokens.
  * ---------------------------------------------------------------------------------------------------------- */
 typedef struct npub200_paged_cache {
   void* k;

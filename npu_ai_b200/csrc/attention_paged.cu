@@ -44,7 +44,8 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kWarps = 4;  // of a block that use the tiles
 constexpr int kLoadWarps = 2;  // that load them by TMA: each the half of the workers
-constexpr int kBlocks = 2;  // on an SM; the grid is as many as are resident (three times as many took 15% longer at 131072 keys)
+// On an SM; the grid is as many as are resident (three times as many took 15% longer at 131072 keys).
+constexpr int kBlocks = 2;
 constexpr int kMaxHalves = 8;  // of a ring
 constexpr int kJoinWarps = 8;
 constexpr int kJoinMaxRecs = 1024;  // blocks whose records the join kernel looks through
@@ -447,392 +448,395 @@ __global__ void __launch_bounds__((kWarps + (TMA ? kLoadWarps : 0)) * 32, kBlock
       __syncthreads();
     }
     if (u0 < u1) {
-    // ---- loads by cp.async: H - 1 halves ahead, the warps of a worker a share each. A lane looks up the page of its key.
-    Cursor<KT> ld = at;
-    int ld_end = ld.visible_end();
-    int page = -1, next_t = -1;  // of the tile that goes out next; next_t < 0: behind the last
-    int next_head = 0;
-    const auto peek = [&]() {    // takes the next tile with keys, if any, and has its pages looked up
-      while (ld.t >= ld_end) {
-        if (!ld.next(a, ROWS)) {
-          next_t = -1;
-          return;
-        }
-        ld_end = ld.visible_end();
-      }
-      next_t = ld.t++;
-      next_head = a.by_row_tiles(ld.rest);
-      const int j = next_t * KT + lane;
-      page = lane < KT && j < ld.seen ? a.table[ld.b * a.table_stride + a.by_page(j)] : -1;
-    };
-    int in = 0, in_values = 0, filled = 0;  // the half of the ring that is filled next, with keys or values; how many are ahead
-    uint32_t in_phase = 0;
-    // (Its code stands once: with the fill of the ring written out in front of the loop the start took 2 us more for
-    // fetching instructions.)
-    const auto issue = [&]() -> bool {
-      if (next_t < 0) return true;
-      if (WR > 1 && !mbar_wait_bounded_warp(&s_empty[wk][in], in_phase ^ 1u, &s_abort, a.ctl, kStatusTimeoutProducer))
-        return false;
-      uint64_t* const bar = &s_full[wk][in];
-      const bool ok = page >= 0 && page < a.pages;
-      const uint32_t valid = __ballot_sync(0xffffffffu, ok);
-      if (role == 0 && lane == 0) {
-        s_valid[wk][in] = valid;
-        mbar_arrive(bar);
-      }
-      const long long sp = in_values ? a.v_sp : a.k_sp, ss = in_values ? a.v_ss : a.k_ss;
-      const __nv_bfloat16* src = in_values ? a.v + next_head * a.v_sh : a.k + next_head * a.k_sh;
-      const int j = next_t * KT + lane;
-      const long long off = ok ? page * sp + (j - a.by_page(j) * a.page_size) * ss : -1;  // < 0: nowhere
-      // Eight lanes a row, four rows a copy, the columns of 64 after each other.
-      const uint32_t dst = ring_at + in * L::kHalf + (lane >> 3) * 128;
-      long long o[KT / (4 * WR)];  // (all of them first: between the copies each would wait for the copy before it)
-#pragma unroll
-      for (int i = 0; i < KT / (4 * WR); ++i) o[i] = __shfl_sync(0xffffffffu, off, (i * WR + role) * 4 + (lane >> 3));
-#pragma unroll
-      for (int i = 0; i < KT / (4 * WR); ++i) {
-        const int row4 = i * WR + role;  // rows 4 row4 ... 4 row4 + 3
-        const uint32_t to = dst + row4 * 512 + (((lane & 7) ^ ((row4 & 1) * 4 + (lane >> 3))) << 4);
-#pragma unroll
-        for (int c = 0; c < L::kAtoms; ++c) {
-          const int col = c * 64 + (lane & 7) * 8;
-          const bool there = o[i] >= 0 && col < a.D;
-          copy16(to + c * L::kAtom, src + (there ? o[i] + col : 0), there);
-        }
-      }
-      copy_arrive(bar);
-      if (++in == H) {
-        in = 0;
-        in_phase ^= 1u;
-      }
-      if (in_values) peek();
-      in_values ^= 1;
-      return true;
-    };
-    if constexpr (!TMA) peek();
-    bool good = true;
-    if (a.ctl.debug & 1u) good = mbar_wait_bounded_warp(&s_never, 0, &s_abort, a.ctl, kStatusForced);
-
-    // ---- the items of the share
-    const int g = lane >> 2, c2 = (lane & 3) * 2;
-    // ldmatrix: this lane's row of a half, and the four swizzled 16-byte columns that it reads of each 64
-    const int k_row = (lane & 7) + ((lane >> 3) & 1) * 8, v_row = (lane & 7) + (lane >> 4) * 8;
-    uint32_t k_col[4], v_col[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      k_col[i] = k_row * 128 + (((2 * i + (lane >> 4)) ^ (lane & 7)) << 4);
-      v_col[i] = v_row * 128 + (((2 * i + ((lane >> 3) & 1)) ^ (lane & 7)) << 4);
-    }
-    const float sc = MODS ? 1.0f : a.scale_log2;
-    constexpr uint32_t kAll = 0xffffffffu >> (32 - KT);
-    int used = 0;  // the half of the ring that is used next
-    uint32_t phase = 0;
-    // The first tile's instructions run once ahead of its data, with every key hidden: fetching them takes as long as the
-    // first load, and so they pass together.
-    int from = -2;
-    while (good) {
-      const int kvh = a.by_row_tiles(at.rest), r0 = (at.rest - kvh * a.row_tiles) * ROWS + role * 8 * NB;
-      uint32_t qf[DP / 16][NB][2];
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const int r = r0 + nb * 8 + g;
-        const bool ok = r < a.rows;
-        const int i = ok ? a.by_g(r) : 0, h = kvh * a.G + (ok ? r - i * a.G : 0);
-        const __nv_bfloat16* qp = a.q + ((long long)at.b * a.q_sb + (long long)i * a.q_ss + (long long)h * a.q_sh + c2);
-#pragma unroll
-        for (int s = 0; s < DP / 16; ++s)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int col = s * 16 + e * 8;
-            qf[s][nb][e] = ok && col < a.D ? *reinterpret_cast<const uint32_t*>(qp + col) : 0u;
+      // ---- loads by cp.async: H - 1 halves ahead, the warps of a worker a share each. A lane looks up the page of its key.
+      Cursor<KT> ld = at;
+      int ld_end = ld.visible_end();
+      int page = -1, next_t = -1;  // of the tile that goes out next; next_t < 0: behind the last
+      int next_head = 0;
+      const auto peek = [&]() {    // takes the next tile with keys, if any, and has its pages looked up
+        while (ld.t >= ld_end) {
+          if (!ld.next(a, ROWS)) {
+            next_t = -1;
+            return;
           }
+          ld_end = ld.visible_end();
+        }
+        next_t = ld.t++;
+        next_head = a.by_row_tiles(ld.rest);
+        const int j = next_t * KT + lane;
+        page = lane < KT && j < ld.seen ? a.table[ld.b * a.table_stride + a.by_page(j)] : -1;
+      };
+      int in = 0, in_values = 0;  // the half of the ring that is filled next, with keys or values
+      int filled = 0;             // how many are ahead of the one that is used, up to H - 1
+      uint32_t in_phase = 0;
+      // (Its code stands once: with the fill of the ring written out in front of the loop the start took 2 us more for
+      // fetching instructions.)
+      const auto issue = [&]() -> bool {
+        if (next_t < 0) return true;
+        if (WR > 1 && !mbar_wait_bounded_warp(&s_empty[wk][in], in_phase ^ 1u, &s_abort, a.ctl, kStatusTimeoutProducer))
+          return false;
+        uint64_t* const bar = &s_full[wk][in];
+        const bool ok = page >= 0 && page < a.pages;
+        const uint32_t valid = __ballot_sync(0xffffffffu, ok);
+        if (role == 0 && lane == 0) {
+          s_valid[wk][in] = valid;
+          mbar_arrive(bar);
+        }
+        const long long sp = in_values ? a.v_sp : a.k_sp, ss = in_values ? a.v_ss : a.k_ss;
+        const __nv_bfloat16* src = in_values ? a.v + next_head * a.v_sh : a.k + next_head * a.k_sh;
+        const int j = next_t * KT + lane;
+        const long long off = ok ? page * sp + (j - a.by_page(j) * a.page_size) * ss : -1;  // < 0: nowhere
+        // Eight lanes a row, four rows a copy, the columns of 64 after each other; of the last 64 only what the head's columns
+        // reach, where that is half of them four lanes a row.
+        constexpr int kLast = DP % 64 == 32 && KT >= 8 * WR ? 4 : 8, kFull = kLast == 8 ? L::kAtoms : L::kAtoms - 1;
+        const uint32_t dst = ring_at + in * L::kHalf;
+        const auto copy = [&](auto lanes, int first, int last) {  // lanes a row; columns of 64
+          constexpr int N = decltype(lanes)::value, ROWS4 = 32 / N;
+          long long o[KT / (ROWS4 * WR)];  // (all of them first: between the copies each would wait for the copy before it)
+#pragma unroll
+          for (int i = 0; i < KT / (ROWS4 * WR); ++i) o[i] = __shfl_sync(0xffffffffu, off, (i * WR + role) * ROWS4 + lane / N);
+#pragma unroll
+          for (int i = 0; i < KT / (ROWS4 * WR); ++i) {
+            const int row = (i * WR + role) * ROWS4 + lane / N;
+            const uint32_t to = dst + row * 128 + (((lane % N) ^ (row & 7)) << 4);
+#pragma unroll
+            for (int c = first; c < last; ++c) {
+              const int col = c * 64 + (lane % N) * 8;
+              const bool there = o[i] >= 0 && col < a.D;
+              copy16(to + c * L::kAtom, src + (there ? o[i] + col : 0), there);
+            }
+          }
+        };
+        copy(std::integral_constant<int, 8>{}, 0, kFull);
+        if constexpr (kLast == 4) copy(std::integral_constant<int, 4>{}, kFull, L::kAtoms);
+        copy_arrive(bar);
+        if (++in == H) {
+          in = 0;
+          in_phase ^= 1u;
+        }
+        if (in_values) peek();
+        in_values ^= 1;
+        return true;
+      };
+      if constexpr (!TMA) peek();
+      bool good = true;
+      if (a.ctl.debug & 1u) good = mbar_wait_bounded_warp(&s_never, 0, &s_abort, a.ctl, kStatusForced);
+
+      // ---- the items of the share
+      const int g = lane >> 2, c2 = (lane & 3) * 2;
+      // ldmatrix: this lane's row of a half, and the four swizzled 16-byte columns that it reads of each 64
+      const int k_row = (lane & 7) + ((lane >> 3) & 1) * 8, v_row = (lane & 7) + (lane >> 4) * 8;
+      uint32_t k_col[4], v_col[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        k_col[i] = k_row * 128 + (((2 * i + (lane >> 4)) ^ (lane & 7)) << 4);
+        v_col[i] = v_row * 128 + (((2 * i + ((lane >> 3) & 1)) ^ (lane & 7)) << 4);
       }
-      // this lane's rows of the scores: c2 and c2 + 1 of each block
-      int lim[NB][2], lim_min = INT32_MAX;
-      long long p[NB][2];
-      float slope[NB][2], m[NB][2], l[NB][2], o[DP / 16][NB][4];
+      const float sc = MODS ? 1.0f : a.scale_log2;
+      constexpr uint32_t kAll = 0xffffffffu >> (32 - KT);
+      int used = 0;  // the half of the ring that is used next
+      uint32_t phase = 0;
+      while (good) {
+        const int kvh = a.by_row_tiles(at.rest), r0 = (at.rest - kvh * a.row_tiles) * ROWS + role * 8 * NB;
+        uint32_t qf[DP / 16][NB][2];
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const int r = r0 + nb * 8 + c2 + y;
+        for (int nb = 0; nb < NB; ++nb) {
+          const int r = r0 + nb * 8 + g;
           const bool ok = r < a.rows;
-          const int i = ok ? a.by_g(r) : 0;
-          p[nb][y] = at.seq.p0 + i;
-          lim[nb][y] = ok ? keys_seen(a, at.seq.len, p[nb][y]) : at.seq.len;
-          lim_min = min(lim_min, lim[nb][y]);
-          slope[nb][y] = MODS && a.slopes != nullptr ? a.slopes[kvh * a.G + (ok ? r - i * a.G : 0)] * kLog2e : 0.0f;
-          m[nb][y] = -INFINITY;
-          l[nb][y] = 0.0f;
-        }
-#pragma unroll
-        for (int s = 0; s < DP / 16; ++s)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[s][nb][e] = 0.0f;
-      }
-#pragma unroll
-      for (int d = 1; d < 4; d <<= 1) lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, d));
-
-      const int first = at.t, halves = 2 * max(0, at.visible_end() - first);
-      uint32_t valid = 0;
-      float x[KT / 16][NB][4];
-#pragma unroll 1
-      for (int half = from; half < halves && good; ++half) {  // a tile's keys, then its values
-        if constexpr (TMA) {
-          if (half >= 0) good = mbar_wait_bounded_warp(&s_full[wk][used], phase, &s_abort, a.ctl, kStatusTimeoutEpilogue);
-        } else {
-#pragma unroll 1
-          for (; half >= 0;) {
-            const bool full = filled == H - 1;
-            if (full) {
-              good = mbar_wait_bounded_warp(&s_full[wk][used], phase, &s_abort, a.ctl, kStatusTimeoutEpilogue);
-              if (!good) break;
-            }
-            good = issue();
-            if (full || !good) break;
-            ++filled;
-          }
-        }
-        if (!good) break;
-        const uint32_t half_at = ring_at + used * L::kHalf;
-        if ((half & 1) == 0) {
-          if (half >= 0) valid = s_valid[wk][used];
-          // S^T = K Q^T, 16 keys a block of x; with one block of rows even and odd steps are sums of their own, half the
-          // chain of instructions that wait for each other
-          float odd[KT / 16][4];
-#pragma unroll
-          for (int n = 0; n < KT / 16; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              odd[n][e] = 0.0f;
-#pragma unroll
-              for (int nb = 0; nb < NB; ++nb) x[n][nb][e] = 0.0f;
-            }
+          const int i = ok ? a.by_g(r) : 0, h = kvh * a.G + (ok ? r - i * a.G : 0);
+          const __nv_bfloat16* qp = a.q + ((long long)at.b * a.q_sb + (long long)i * a.q_ss + (long long)h * a.q_sh + c2);
 #pragma unroll
           for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
-            for (int n = 0; n < KT / 16; ++n) {
-              uint32_t kf[4];
-              ldmatrix_x4(half_at + k_col[s & 3] + (s >> 2) * L::kAtom + n * 2048, kf);
-#pragma unroll
-              for (int nb = 0; nb < NB; ++nb)
-                mma_bf16(NB == 1 && (s & 1) ? odd[n] : x[n][nb], kf, qf[s][nb][0], qf[s][nb][1]);
+            for (int e = 0; e < 2; ++e) {
+              const int col = s * 16 + e * 8;
+              qf[s][nb][e] = ok && col < a.D ? *reinterpret_cast<const uint32_t*>(qp + col) : 0u;
             }
-          if constexpr (NB == 1) {
+        }
+        // this lane's rows of the scores: c2 and c2 + 1 of each block
+        int lim[NB][2], lim_min = INT32_MAX;
+        long long p[NB][2];
+        float slope[NB][2], m[NB][2], l[NB][2], o[DP / 16][NB][4];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const int r = r0 + nb * 8 + c2 + y;
+            const bool ok = r < a.rows;
+            const int i = ok ? a.by_g(r) : 0;
+            p[nb][y] = at.seq.p0 + i;
+            lim[nb][y] = ok ? keys_seen(a, at.seq.len, p[nb][y]) : at.seq.len;
+            lim_min = min(lim_min, lim[nb][y]);
+            slope[nb][y] = MODS && a.slopes != nullptr ? a.slopes[kvh * a.G + (ok ? r - i * a.G : 0)] * kLog2e : 0.0f;
+            m[nb][y] = -INFINITY;
+            l[nb][y] = 0.0f;
+          }
+#pragma unroll
+          for (int s = 0; s < DP / 16; ++s)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[s][nb][e] = 0.0f;
+        }
+#pragma unroll
+        for (int d = 1; d < 4; d <<= 1) lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, d));
+
+        const int first = at.t, halves = 2 * max(0, at.visible_end() - first);
+        uint32_t valid = 0;
+        float x[KT / 16][NB][4];
+#pragma unroll 1
+        for (int half = 0; half < halves && good; ++half) {  // a tile's keys, then its values
+          if constexpr (TMA) {
+            good = mbar_wait_bounded_warp(&s_full[wk][used], phase, &s_abort, a.ctl, kStatusTimeoutEpilogue);
+          } else {
+#pragma unroll 1
+            for (;;) {
+              const bool full = filled == H - 1;
+              if (full) {
+                good = mbar_wait_bounded_warp(&s_full[wk][used], phase, &s_abort, a.ctl, kStatusTimeoutEpilogue);
+                if (!good) break;
+              }
+              good = issue();
+              if (full || !good) break;
+              ++filled;
+            }
+          }
+          if (!good) break;
+          const uint32_t half_at = ring_at + used * L::kHalf;
+          if ((half & 1) == 0) {
+            valid = s_valid[wk][used];
+            // S^T = K Q^T, 16 keys a block of x; with one block of rows even and odd steps are sums of their own, half the
+            // chain of instructions that wait for each other
+            float odd[KT / 16][4];
 #pragma unroll
             for (int n = 0; n < KT / 16; ++n)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) x[n][0][e] += odd[n][e];
-          }
-          const int j0 = (first + (half >> 1)) * KT;
-          if constexpr (MODS) {
-            if (a.cap_out != 0.0f) {
-              float big = 0.0f;
+              for (int e = 0; e < 4; ++e) {
+                odd[n][e] = 0.0f;
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) x[n][nb][e] = 0.0f;
+              }
+#pragma unroll
+            for (int s = 0; s < DP / 16; ++s)
+#pragma unroll
+              for (int n = 0; n < KT / 16; ++n) {
+                uint32_t kf[4];
+                ldmatrix_x4(half_at + k_col[s & 3] + (s >> 2) * L::kAtom + n * 2048, kf);
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+                  mma_bf16(NB == 1 && (s & 1) ? odd[n] : x[n][nb], kf, qf[s][nb][0], qf[s][nb][1]);
+              }
+            if constexpr (NB == 1) {
+#pragma unroll
+              for (int n = 0; n < KT / 16; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[n][0][e] += odd[n][e];
+            }
+            const int j0 = (first + (half >> 1)) * KT;
+            if constexpr (MODS) {
+              if (a.cap_out != 0.0f) {
+                float big = 0.0f;
+#pragma unroll
+                for (int n = 0; n < KT / 16; ++n)
+#pragma unroll
+                  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                      x[n][nb][e] *= a.cap_in;
+                      big = max_nan(big, fabsf(x[n][nb][e]));
+                    }
+                const bool small = __all_sync(0xffffffffu, big <= 1.0f);  // (mostly: the cap is for the rare large score)
+#pragma unroll
+                for (int n = 0; n < KT / 16; ++n)
+#pragma unroll
+                  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                      x[n][nb][e] = a.cap_out * (small ? tanh_small(x[n][nb][e]) : tanh_any(x[n][nb][e]));
+              } else {
+#pragma unroll
+                for (int n = 0; n < KT / 16; ++n)
+#pragma unroll
+                  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[n][nb][e] *= a.scale_log2;
+              }
+              if (a.slopes != nullptr) {
+                // The distance from f32: exact up to 2^24, rounded to a step of itself beyond.
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                  for (int y = 0; y < 2; ++y) {
+                    const float ahead = float(p[nb][y] - j0 - g);
+#pragma unroll
+                    for (int n = 0; n < KT / 16; ++n)
+#pragma unroll
+                      for (int e = 0; e < 4; e += 2)
+                        x[n][nb][e + y] = fmaf(-slope[nb][y], fabsf(ahead - float(n * 16 + e * 4)), x[n][nb][e + y]);
+                  }
+              }
+            }
+            if (j0 + KT > lim_min || valid != kAll) {
 #pragma unroll
               for (int n = 0; n < KT / 16; ++n)
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                   for (int e = 0; e < 4; ++e) {
-                    x[n][nb][e] *= a.cap_in;
-                    big = max_nan(big, fabsf(x[n][nb][e]));
+                    const int j = n * 16 + g + (e >> 1) * 8;
+                    if (j0 + j >= lim[nb][e & 1] || ((valid >> j) & 1u) == 0) x[n][nb][e] = -INFINITY;
                   }
-              const bool small = __all_sync(0xffffffffu, big <= 1.0f);  // (mostly: the cap is for the rare large score)
-#pragma unroll
-              for (int n = 0; n < KT / 16; ++n)
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                  for (int e = 0; e < 4; ++e)
-                    x[n][nb][e] = a.cap_out * (small ? tanh_small(x[n][nb][e]) : tanh_any(x[n][nb][e]));
-            } else {
-#pragma unroll
-              for (int n = 0; n < KT / 16; ++n)
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) x[n][nb][e] *= a.scale_log2;
             }
-            if (a.slopes != nullptr) {
-              // The distance from f32: exact up to 2^24, rounded to a step of itself beyond.
-#pragma unroll
-              for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                  const float ahead = float(p[nb][y] - j0 - g);
-#pragma unroll
-                  for (int n = 0; n < KT / 16; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; e += 2)
-                      x[n][nb][e + y] = fmaf(-slope[nb][y], fabsf(ahead - float(n * 16 + e * 4)), x[n][nb][e + y]);
-                }
-            }
-          }
-          if (j0 + KT > lim_min || valid != kAll) {
-#pragma unroll
-            for (int n = 0; n < KT / 16; ++n)
-#pragma unroll
-              for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const int j = n * 16 + g + (e >> 1) * 8;
-                  if (j0 + j >= lim[nb][e & 1] || ((valid >> j) & 1u) == 0) x[n][nb][e] = -INFINITY;
-                }
-          }
-          float top[NB][2];
-          bool moved = false;
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              top[nb][y] = fmaxf(x[0][nb][y], x[0][nb][2 + y]);
-#pragma unroll
-              for (int n = 1; n < KT / 16; ++n) top[nb][y] = fmax3(top[nb][y], x[n][nb][y], x[n][nb][2 + y]);
-            }
-#pragma unroll
-          for (int d = 4; d < 32; d <<= 1)
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-              for (int y = 0; y < 2; ++y) top[nb][y] = fmaxf(top[nb][y], __shfl_xor_sync(0xffffffffu, top[nb][y], d));
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              top[nb][y] *= sc;
-              moved = moved || top[nb][y] > m[nb][y] + kRescale;
-            }
-          if (__any_sync(0xffffffffu, moved)) {
+            float top[NB][2];
+            bool moved = false;
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
               for (int y = 0; y < 2; ++y) {
-                const float to = top[nb][y] > m[nb][y] + kRescale ? top[nb][y] : m[nb][y];
-                const float f = to == m[nb][y] ? 1.0f : fast_exp2(m[nb][y] - to);
-                m[nb][y] = to;
-                l[nb][y] *= f;
+                top[nb][y] = fmaxf(x[0][nb][y], x[0][nb][2 + y]);
 #pragma unroll
-                for (int s = 0; s < DP / 16; ++s) {
-                  o[s][nb][y] *= f;
-                  o[s][nb][2 + y] *= f;
-                }
+                for (int n = 1; n < KT / 16; ++n) top[nb][y] = fmax3(top[nb][y], x[n][nb][y], x[n][nb][2 + y]);
               }
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1)
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) top[nb][y] = fmaxf(top[nb][y], __shfl_xor_sync(0xffffffffu, top[nb][y], d));
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+              for (int y = 0; y < 2; ++y) {
+                top[nb][y] *= sc;
+                moved = moved || top[nb][y] > m[nb][y] + kRescale;
+              }
+            if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                  const float to = top[nb][y] > m[nb][y] + kRescale ? top[nb][y] : m[nb][y];
+                  const float f = to == m[nb][y] ? 1.0f : fast_exp2(m[nb][y] - to);
+                  m[nb][y] = to;
+                  l[nb][y] *= f;
+#pragma unroll
+                  for (int s = 0; s < DP / 16; ++s) {
+                    o[s][nb][y] *= f;
+                    o[s][nb][2 + y] *= f;
+                  }
+                }
+            }
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+              for (int y = 0; y < 2; ++y) {
+                const float mu = m[nb][y] == -INFINITY ? 0.0f : m[nb][y];  // nothing seen yet: every weight is 0
+#pragma unroll
+                for (int n = 0; n < KT / 16; ++n)
+#pragma unroll
+                  for (int e = 0; e < 4; e += 2) {
+                    x[n][nb][e + y] = fast_exp2(fmaf(x[n][nb][e + y], sc, -mu));
+                    l[nb][y] += x[n][nb][e + y];
+                  }
+              }
+          } else {
+            // O^T += V^T P^T; P rounded to bf16 for the tensor core, 2^-8 relative at most, the sum takes the unrounded
+            // weights
+            const bool all = valid == kAll;
+#pragma unroll
+            for (int n = 0; n < KT / 16; ++n) {
+              uint32_t pf[NB][2];
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) {
+                pf[nb][0] = transposed(pack_bf16x2(x[n][nb][0], x[n][nb][1]));
+                pf[nb][1] = transposed(pack_bf16x2(x[n][nb][2], x[n][nb][3]));
+              }
+              const uint32_t w = valid >> (n * 16 + c2);
+              const uint32_t k0 = (w & 1u ? 0xffffu : 0u) | (w & 2u ? 0xffff0000u : 0u);
+              const uint32_t k1 = (w & 0x100u ? 0xffffu : 0u) | (w & 0x200u ? 0xffff0000u : 0u);
+#pragma unroll
+              for (int s = 0; s < DP / 16; ++s) {
+                uint32_t vf[4];
+                ldmatrix_x4_trans(half_at + v_col[s & 3] + (s >> 2) * L::kAtom + n * 2048, vf);
+                if (!all) {  // slots behind the last key may hold anything: zeros, for 0 times NaN is NaN
+                  vf[0] &= k0;
+                  vf[1] &= k0;
+                  vf[2] &= k1;
+                  vf[3] &= k1;
+                }
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) mma_bf16(o[s][nb], vf, pf[nb][0], pf[nb][1]);
+              }
+            }
           }
+          __syncwarp();  // all lanes are done with the half
+          if ((TMA || WR > 1) && lane == 0) mbar_arrive(&s_empty[wk][used]);
+          if (++used == H) {
+            used = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!good) break;
+
+        // ---- the item's rows, or the share's part of them
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1)
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) l[nb][y] += __shfl_xor_sync(0xffffffffu, l[nb][y], d);
+        const bool begins = first == 0, ends = at.t1 == at.tiles, last = at.left <= 0;
+        if (begins && ends) {
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
-              const float mu = m[nb][y] == -INFINITY ? 0.0f : m[nb][y];  // nothing seen yet: every weight is 0
+              const int r = r0 + nb * 8 + c2 + y;
+              if (r >= a.rows) continue;
+              const float inv = l[nb][y] == 0.0f ? 0.0f : 1.0f / l[nb][y];  // (a NaN sum makes the row NaN)
+              const long long row = out_row(a, at.b, kvh, r) + g;
+              if (a.out_f32) {
+                float* const d = static_cast<float*>(a.out) + row;
 #pragma unroll
-              for (int n = 0; n < KT / 16; ++n)
+                for (int s = 0; s < DP / 8; ++s)
+                  if (s * 8 < a.D) d[s * 8] = o[s / 2][nb][(s & 1) * 2 + y] * inv;
+              } else {
+                __nv_bfloat16* const d = static_cast<__nv_bfloat16*>(a.out) + row;
 #pragma unroll
-                for (int e = 0; e < 4; e += 2) {
-                  x[n][nb][e + y] = fast_exp2(fmaf(x[n][nb][e + y], sc, -mu));
-                  l[nb][y] += x[n][nb][e + y];
-                }
+                for (int s = 0; s < DP / 8; ++s)
+                  if (s * 8 < a.D) d[s * 8] = __float2bfloat16_rn(o[s / 2][nb][(s & 1) * 2 + y] * inv);
+              }
             }
         } else {
-          // O^T += V^T P^T; P rounded to bf16 for the tensor core, 2^-8 relative at most, the sum takes the unrounded
-          // weights
-          const bool all = valid == kAll;
-#pragma unroll
-          for (int n = 0; n < KT / 16; ++n) {
-            uint32_t pf[NB][2];
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-              pf[nb][0] = transposed(pack_bf16x2(x[n][nb][0], x[n][nb][1]));
-              pf[nb][1] = transposed(pack_bf16x2(x[n][nb][2], x[n][nb][3]));
-            }
-            const uint32_t w = valid >> (n * 16 + c2);
-            const uint32_t k0 = (w & 1u ? 0xffffu : 0u) | (w & 2u ? 0xffff0000u : 0u);
-            const uint32_t k1 = (w & 0x100u ? 0xffffu : 0u) | (w & 0x200u ? 0xffff0000u : 0u);
-#pragma unroll
-            for (int s = 0; s < DP / 16; ++s) {
-              uint32_t vf[4];
-              ldmatrix_x4_trans(half_at + v_col[s & 3] + (s >> 2) * L::kAtom + n * 2048, vf);
-              if (!all) {  // slots behind the last key may hold anything: zeros, for 0 times NaN is NaN
-                vf[0] &= k0;
-                vf[1] &= k0;
-                vf[2] &= k1;
-                vf[3] &= k1;
-              }
-#pragma unroll
-              for (int nb = 0; nb < NB; ++nb) mma_bf16(o[s][nb], vf, pf[nb][0], pf[nb][1]);
-            }
+          // The share's last part waits in the ring, which nobody needs any more; the end of an item before it does not.
+          if (WR > 1 && NW > 1 && last) {  // (once the worker's other warps are done with the half used last)
+            const int before = used == 0 ? H - 1 : used - 1;
+            good = mbar_wait_bounded_warp(&s_empty[wk][before], used == 0 ? phase ^ 1u : phase, &s_abort, a.ctl,
+                                          kStatusTimeoutEpilogue);
+            if (!good) break;
           }
-        }
-        if (half < 0) continue;
-        __syncwarp();  // all lanes are done with the half
-        if ((TMA || WR > 1) && lane == 0) mbar_arrive(&s_empty[wk][used]);
-        if (++used == H) {
-          used = 0;
-          phase ^= 1u;
-        }
-      }
-      from = 0;
-      if (!good) break;
-
-      // ---- the item's rows, or the share's part of them
+          // (The only worker's parts are the block's.)
+          const long long slot = ((long long)blockIdx.x * 2 + begins) * a.slot_rows;
+          float* const dst = NW == 1 ? a.part_o + slot * a.D
+                             : last  ? reinterpret_cast<float*>(ring)
+                                     : a.head_o + ((long long)blockIdx.x * NW + wk) * a.slot_rows * a.D;
+          const int ld_o = NW > 1 && last ? DP + 4 : a.D;
 #pragma unroll
-      for (int d = 4; d < 32; d <<= 1)
+          for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-          for (int y = 0; y < 2; ++y) l[nb][y] += __shfl_xor_sync(0xffffffffu, l[nb][y], d);
-      const bool begins = first == 0, ends = at.t1 == at.tiles, last = at.left <= 0;
-      if (begins && ends) {
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const int r = r0 + nb * 8 + c2 + y;
-            if (r >= a.rows) continue;
-            const float inv = l[nb][y] == 0.0f ? 0.0f : 1.0f / l[nb][y];  // (a NaN sum makes the row NaN)
-            const long long row = out_row(a, at.b, kvh, r) + g;
-            if (a.out_f32) {
-              float* const d = static_cast<float*>(a.out) + row;
+            for (int y = 0; y < 2; ++y) {
+              const int r = (role * NB + nb) * 8 + c2 + y;
+              if (r >= a.slot_rows) continue;
+              if (g == 0) (NW == 1 ? a.part_ml[slot + r] : s_ml[wk][begins][r]) = make_float2(m[nb][y], l[nb][y]);
+              float* const row = dst + r * ld_o + g;
 #pragma unroll
               for (int s = 0; s < DP / 8; ++s)
-                if (s * 8 < a.D) d[s * 8] = o[s / 2][nb][(s & 1) * 2 + y] * inv;
-            } else {
-              __nv_bfloat16* const d = static_cast<__nv_bfloat16*>(a.out) + row;
-#pragma unroll
-              for (int s = 0; s < DP / 8; ++s)
-                if (s * 8 < a.D) d[s * 8] = __float2bfloat16_rn(o[s / 2][nb][(s & 1) * 2 + y] * inv);
+                if (s * 8 < a.D) row[s * 8] = o[s / 2][nb][(s & 1) * 2 + y];
             }
-          }
-      } else {
-        // The share's last part waits in the ring, which nobody needs any more; the end of an item before it does not.
-        if (WR > 1 && NW > 1 && last) {  // (once the worker's other warps are done with the half used last)
-          const int before = used == 0 ? H - 1 : used - 1;
-          good = mbar_wait_bounded_warp(&s_empty[wk][before], used == 0 ? phase ^ 1u : phase, &s_abort, a.ctl,
-                                        kStatusTimeoutEpilogue);
-          if (!good) break;
+          if (role == 0 && lane == 0)
+            s_part[wk][begins] = Part{at.b, at.rest, at.tiles - at.t1, uint8_t(begins), uint8_t(ends), uint8_t(last)};
         }
-        // (The only worker's parts are the block's.)
-        const long long slot = ((long long)blockIdx.x * 2 + begins) * a.slot_rows;
-        float* const dst = NW == 1 ? a.part_o + slot * a.D
-                           : last  ? reinterpret_cast<float*>(ring)
-                                   : a.head_o + ((long long)blockIdx.x * NW + wk) * a.slot_rows * a.D;
-        const int ld_o = NW > 1 && last ? DP + 4 : a.D;
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const int r = (role * NB + nb) * 8 + c2 + y;
-            if (r >= a.slot_rows) continue;
-            if (g == 0) (NW == 1 ? a.part_ml[slot + r] : s_ml[wk][begins][r]) = make_float2(m[nb][y], l[nb][y]);
-            float* const row = dst + r * ld_o + g;
-#pragma unroll
-            for (int s = 0; s < DP / 8; ++s)
-              if (s * 8 < a.D) row[s * 8] = o[s / 2][nb][(s & 1) * 2 + y];
-          }
-        if (role == 0 && lane == 0)
-          s_part[wk][begins] = Part{at.b, at.rest, at.tiles - at.t1, uint8_t(begins), uint8_t(ends), uint8_t(last)};
+        if (!at.next(a, ROWS)) break;
       }
-      if (!at.next(a, ROWS)) break;
-    }
-    if (!TMA && !good) copy_wait_all();  // copies in flight write to this block's memory: it stays until they are done
+      if (!TMA && !good) copy_wait_all();  // copies in flight write to this block's memory: it stays until they are done
     }
   }
   __syncthreads();
@@ -851,51 +855,53 @@ __global__ void __launch_bounds__((kWarps + (TMA ? kLoadWarps : 0)) * 32, kBlock
         joins ? make_int4(mine_p.b, mine_p.rest, int(divide(c0 + run + mine_p.rem - 1, span)) - int(blockIdx.x) + 1, 0)
               : make_int4(0, 0, 0, 0);
   }
-  if (NW == 1 || present == 0 || warp >= kWarps) return;
+  if constexpr (NW > 1) {
+    if (present == 0 || warp >= kWarps) return;
 #pragma unroll 1
-  for (int r = warp; r < a.slot_rows; r += kWarps)
+    for (int r = warp; r < a.slot_rows; r += kWarps)
 #pragma unroll 1
-    for (int col = lane * 4; col < a.D; col += 128) {
-      float acc[4], top = -INFINITY, sum = 0.0f;
-      int begins = 0;
+      for (int col = lane * 4; col < a.D; col += 128) {
+        float acc[4], top = -INFINITY, sum = 0.0f;
+        int begins = 0;
 #pragma unroll 1
-      for (uint32_t w = present; w != 0; w &= w - 1) {
-        const int z = __ffs(int(w)) - 1;
-        const Part part = s_part[z / 2][z & 1];
-        const float2 ml = s_ml[z / 2][z & 1][r];
-        const float* const src = part.in_ring
-                                     ? reinterpret_cast<const float*>(smem + (z / 2) * L::kRing) + r * (DP + 4)
-                                     : a.head_o + (((long long)blockIdx.x * NW + z / 2) * a.slot_rows + r) * a.D;
-        const float4 v = *reinterpret_cast<const float4*>(src + col);
-        if ((starts >> z) & 1u) {
-          begins = part.begins;
-          top = -INFINITY;
-          sum = acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
-        }
-        const float to = fmaxf(top, ml.x), base = to == -INFINITY ? 0.0f : to;
-        const float f0 = fast_exp2(top - base), f1 = fast_exp2(ml.x - base);
-        top = to;
-        sum = fmaf(f1, ml.y, sum * f0);
-        acc[0] = fmaf(f1, v.x, acc[0] * f0);
-        acc[1] = fmaf(f1, v.y, acc[1] * f0);
-        acc[2] = fmaf(f1, v.z, acc[2] * f0);
-        acc[3] = fmaf(f1, v.w, acc[3] * f0);
-        const uint32_t behind = w & (w - 1);
-        if (behind != 0 && (starts & behind & (0u - behind)) == 0) continue;  // the chain goes on
-        const int kvh = a.by_row_tiles(part.rest), row = (part.rest - kvh * a.row_tiles) * ROWS + r;
-        if (row >= a.rows) continue;
-        if (begins && part.ends) {
-          const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // (a NaN sum makes the row NaN)
+        for (uint32_t w = present; w != 0; w &= w - 1) {
+          const int z = __ffs(int(w)) - 1;
+          const Part part = s_part[z / 2][z & 1];
+          const float2 ml = s_ml[z / 2][z & 1][r];
+          const float* const src = part.in_ring
+                                       ? reinterpret_cast<const float*>(smem + (z / 2) * L::kRing) + r * (DP + 4)
+                                       : a.head_o + (((long long)blockIdx.x * NW + z / 2) * a.slot_rows + r) * a.D;
+          const float4 v = *reinterpret_cast<const float4*>(src + col);
+          if ((starts >> z) & 1u) {
+            begins = part.begins;
+            top = -INFINITY;
+            sum = acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
+          }
+          const float to = fmaxf(top, ml.x), base = to == -INFINITY ? 0.0f : to;
+          const float f0 = fast_exp2(top - base), f1 = fast_exp2(ml.x - base);
+          top = to;
+          sum = fmaf(f1, ml.y, sum * f0);
+          acc[0] = fmaf(f1, v.x, acc[0] * f0);
+          acc[1] = fmaf(f1, v.y, acc[1] * f0);
+          acc[2] = fmaf(f1, v.z, acc[2] * f0);
+          acc[3] = fmaf(f1, v.w, acc[3] * f0);
+          const uint32_t behind = w & (w - 1);
+          if (behind != 0 && (starts & behind & (0u - behind)) == 0) continue;  // the chain goes on
+          const int kvh = a.by_row_tiles(part.rest), row = (part.rest - kvh * a.row_tiles) * ROWS + r;
+          if (row >= a.rows) continue;
+          if (begins && part.ends) {
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // (a NaN sum makes the row NaN)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[e] *= inv;
-          write_out4(a, out_row(a, part.b, kvh, row) + col, acc);
-        } else {
-          const long long at = ((long long)blockIdx.x * 2 + begins) * a.slot_rows + r;
-          if (col == 0) a.part_ml[at] = make_float2(top, sum);
-          *reinterpret_cast<float4*>(a.part_o + at * a.D + col) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+            for (int e = 0; e < 4; ++e) acc[e] *= inv;
+            write_out4(a, out_row(a, part.b, kvh, row) + col, acc);
+          } else {
+            const long long at = ((long long)blockIdx.x * 2 + begins) * a.slot_rows + r;
+            if (col == 0) a.part_ml[at] = make_float2(top, sum);
+            *reinterpret_cast<float4*>(a.part_o + at * a.D + col) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+          }
         }
       }
-    }
+  }
 }
 
 // Joins the parts of the items that go on from block to block. WARPS warps share a row, the parts in turn: all eight of a
@@ -1194,13 +1200,16 @@ int attention_paged_launch(const AttnPagedProblem& p, cudaStream_t stream) {
     const auto fits = [](int64_t n, int64_t s) { return n == 1 || (s > 0 && s < (int64_t(1) << 38)); };
     return fits(c.pages, sp) && fits(c.page_size, ss) && fits(c.kv_heads, sh);
   };
-  const bool tma = (c.head_dim % 128 == 0 || few_keys) && c.page_size % 16 == 0 && c.pages > 0 && strided(c.k_sp, c.k_ss, c.k_sh) && strided(c.v_sp, c.v_ss, c.v_sh);
+  const bool tma = (c.head_dim % 128 == 0 || few_keys) && c.page_size % 16 == 0 && c.pages > 0 &&
+                   strided(c.k_sp, c.k_ss, c.k_sh) && strided(c.v_sp, c.v_ss, c.v_sh);
   const int tile = c.head_dim <= 128 ? 32 : 16;  // (PagedLayout::kTile)
   a.box_rows = c.page_size % tile == 0 ? tile : 16;
   if (tma) {
-    if (int rc = encode_bshd_map(c.k, c.head_dim, c.page_size, c.kv_heads, c.pages, c.k_ss, c.k_sh, c.k_sp, a.box_rows, &mk, &a.pk))
+    if (int rc = encode_bshd_map(c.k, c.head_dim, c.page_size, c.kv_heads, c.pages, c.k_ss, c.k_sh, c.k_sp, a.box_rows, &mk,
+                                 &a.pk))
       return rc;
-    if (int rc = encode_bshd_map(c.v, c.head_dim, c.page_size, c.kv_heads, c.pages, c.v_ss, c.v_sh, c.v_sp, a.box_rows, &mv, &a.pv))
+    if (int rc = encode_bshd_map(c.v, c.head_dim, c.page_size, c.kv_heads, c.pages, c.v_ss, c.v_sh, c.v_sp, a.box_rows, &mv,
+                                 &a.pv))
       return rc;
   }
   const bool mods = p.softcap > 0.0f || p.slopes != nullptr;
@@ -1212,9 +1221,9 @@ int attention_paged_launch(const AttnPagedProblem& p, cudaStream_t stream) {
   static_assert(kBlocks * 160 <= kJoinMaxRecs, "records of the join kernel");
   const int64_t rows = items * plan.slot_rows;
   const bool few = rows <= 2 * dev->sms;
+  const int64_t join_blocks = std::min<int64_t>(few ? rows : (rows + kJoinWarps - 1) / kJoinWarps, 2 * dev->sms);
   return check_cuda(launch_pdl(few ? attention_paged_join_kernel<kJoinWarps> : attention_paged_join_kernel<1>,
-                               dim3(unsigned(std::min<int64_t>(few ? rows : (rows + kJoinWarps - 1) / kJoinWarps, 2 * dev->sms))),
-                               dim3(kJoinWarps * 32), 0, stream, a, plan.blocks, 8 * plan.nb * plan.wr),
+                               dim3(unsigned(join_blocks)), dim3(kJoinWarps * 32), 0, stream, a, plan.blocks, 8 * plan.nb * plan.wr),
                     "paged attention join kernel launch");
 }
 

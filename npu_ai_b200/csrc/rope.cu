@@ -397,9 +397,9 @@ int check_paged_cache(const npub200_paged_cache* c, int64_t batch, const char* w
     return fail(kErrInvalid, "%s: bad cache sizes (pages=%lld page_size=%lld kv_heads=%lld head_dim=%lld table=%lld/%lld)",
                 what, (long long)c->pages, (long long)c->page_size, (long long)c->kv_heads, (long long)c->head_dim,
                 (long long)c->table_width, (long long)c->table_stride);
-  constexpr int64_t most = int64_t(1) << 30;
+  constexpr int64_t most = (int64_t(1) << 30) - 32;  // (32 sequences have fewer than 2^31 tiles of 16)
   if (c->pages > INT32_MAX || c->page_size > most || (c->table_width > 0 && c->page_size > most / c->table_width))
-    return fail(kErrUnsupported, "%s: more than 2^31 - 1 pages (%lld) or 2^30 tokens in a sequence's pages (%lld x %lld)",
+    return fail(kErrUnsupported, "%s: more than 2^31 - 1 pages (%lld) or 2^30 - 32 tokens in a sequence's pages (%lld x %lld)",
                 what, (long long)c->pages, (long long)c->table_width, (long long)c->page_size);
   if (c->kv_heads > 65535) return fail(kErrUnsupported, "%s: more than 65535 heads (%lld)", what, (long long)c->kv_heads);
   if (c->pages > 0) {

@@ -214,6 +214,24 @@ def test_strides(cuda_device):
     assert torch.equal(o, kernels.paged_attention(one.contiguous(), c.k, c.v, c.table, c.lens, H, out_dtype=BF16))
 
 
+@pytest.mark.parametrize("D", [64, 80, 128, 256])
+def test_both_kinds_of_loads(cuda_device, D):
+    """Pools whose heads are one head expanded (no tensor map takes a stride of 0) give what a copy of them gives, and a wide
+    table (which decides between the kinds of loads below 128 columns) what a narrow one gives."""
+    from npu_ai_b200 import kernels
+    d = cuda_device
+    for Sq in (1, 4, 12):
+        c = Cache(d, [333, 40, 0], 1, D, 32)
+        q = torch.randn(3, Sq, 4 * D, device=d).to(BF16)
+        one = [t.expand(-1, -1, 2, -1) for t in (c.k, c.v)]
+        want = kernels.paged_attention(q, *(t.contiguous() for t in one), c.table, c.lens, 4)
+        assert torch.equal(kernels.paged_attention(q, *one, c.table, c.lens, 4), want)
+        wide = torch.full((3, 5000), -1, dtype=torch.int32, device=d)
+        wide[:, :c.width] = c.table
+        assert torch.equal(kernels.paged_attention(q, *(t.contiguous() for t in one), wide, c.lens, 4), want)
+    kernels.check_status(d)
+
+
 def test_shared_pages(cuda_device):
     """Two sequences with the same first pages, and one page many times in one table."""
     d = cuda_device
