@@ -11,6 +11,8 @@
 #include <ATen/ATen.h>
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
@@ -309,6 +311,13 @@ at::Tensor attention_masked(const at::Tensor& q, const at::Tensor& k, const at::
   return out;
 }
 
+// An uninitialised CUDA tensor, and a workspace of the current stream's, without the way through the dispatcher (1 us each on the
+// host, which is what a small call waits for).
+at::Tensor empty_like_device(at::IntArrayRef size, at::ScalarType dtype, const at::Tensor& ref) {
+  return at::Tensor(at::detail::empty_cuda(size, dtype, ref.device(), std::nullopt));
+}
+c10::DataPtr workspace(size_t bytes) { return c10::cuda::CUDACachingAllocator::get()->allocate(bytes); }
+
 // (batch, seq, head) element strides of a tensor of heads, and the checks of its shape: (B, S, heads * d), or (B, heads, S, d)
 // when head-major. A dimension of one element has no stride of its own.
 struct HeadRows {
@@ -398,7 +407,7 @@ at::Tensor rope(const at::Tensor& x, const at::Tensor& freqs, int64_t heads, con
     TORCH_CHECK_VALUE(out.sizes() == x.sizes(), "out must have x's shape ", x.sizes(), ", got ", out.sizes());
     check_written(out, "out", &x);
   } else {
-    out = at::empty(x.sizes(), x.options().dtype(out_dtype.value_or(x.scalar_type())));
+    out = empty_like_device(x.sizes(), out_dtype.value_or(x.scalar_type()), x);
   }
   const HeadRows orr = head_rows(out, x, head_major, heads, d, "out");
   check_rc(npub200_rope(x.data_ptr(), xr.sb, xr.ss, xr.sh, x_code, out.data_ptr(), orr.sb, orr.ss, orr.sh,
@@ -476,7 +485,7 @@ std::optional<at::Tensor> paged_append(const at::Tensor& k, const at::Tensor& v,
       check_apart(*q_out, v, "q_out and v");
       out = *q_out;
     } else {
-      out = at::empty(q->sizes(), k_pages.options());
+      out = empty_like_device(q->sizes(), at::kBFloat16, k_pages);
     }
     orr = head_rows(*out, k_pages, head_major, heads, c.head_dim, "q_out");
   } else {
@@ -515,7 +524,7 @@ at::Tensor attention_paged(const at::Tensor& q, const at::Tensor& k_pages, const
                       out.sizes());
     check_written(out, "out");
   } else {
-    out = at::empty(shape, q.options().dtype(out_dtype.value_or(at::kFloat)));
+    out = empty_like_device(shape, out_dtype.value_or(at::kFloat), k_pages);
   }
   const HeadRows orr = head_rows(out, k_pages, head_major_out, heads, d, "attention output");
   const int out_code = dtype_code(out, "attention output");
@@ -525,10 +534,10 @@ at::Tensor attention_paged(const at::Tensor& q, const at::Tensor& k_pages, const
   if (B == 0 || S == 0) return out;
   size_t ws_bytes = 0;
   check_rc(npub200_attention_paged_workspace_size(heads, c.kv_heads, S, d, &ws_bytes), "npub200::attention_paged");
-  const at::Tensor ws = at::empty({int64_t(ws_bytes)}, q.options().dtype(at::kByte));
+  const c10::DataPtr ws = workspace(ws_bytes);  // (of this call's own: calls on other streams and captured graphs share none)
   check_rc(npub200_attention_paged(q.data_ptr(), qr.sb, qr.ss, qr.sh, &c, lens, out.data_ptr(), orr.sb, orr.ss, orr.sh,
                                    out_code, B, heads, S, float(scale), causal ? 1 : 0, starts, float(softcap), slopes_ptr,
-                                   ws.data_ptr(), ws_bytes, int(variant), stream_of(k_pages)),
+                                   ws.get(), ws_bytes, int(variant), stream_of(k_pages)),
            "npub200::attention_paged");
   return out;
 }
