@@ -23,8 +23,8 @@
 //     (A bulk copy a row was the first form: the copy engine takes one in about 17 cycles, 16 bytes a cycle at 128 columns
 //     where 23 are the memory's rate.) Keys and values wait in one ring, a half tile each, swizzled in 128-byte rows, which
 //     ldmatrix reads without a bank conflict.
-// Measured (GPU time of a call with its join, a graph of calls): one token, 16 x 32/8 heads x 16384 keys (ragged) x 128 133 us,
-// 6.2 TB/s, 94% of the measured copy rate; 1 x 131071 keys 93 us, 5.7 TB/s; 777 keys x 64 9.0 us: launches, the run from
+// Measured (GPU time of a call with its join, a graph of calls): one token, 16 x 32/8 heads x 16384 keys (ragged) x 128 134 us,
+// 6.1 TB/s, 94% of the measured copy rate; 1 x 131071 keys 94 us, 5.7 TB/s; 777 keys x 64 8.3 us: launches, the run from
 // kv_lens, the page table, the first keys and the join's records after each other.
 #include <algorithm>
 #include <atomic>
@@ -1025,8 +1025,8 @@ PagedPlan plan_paged(int64_t H, int64_t Hk, int64_t Sq, int64_t D, int sms) {
   PagedPlan p;
   p.rows = H / Hk * Sq;
   // Two blocks of rows a warp from 33 rows on, where reading the keys from shared memory for each block decides (4 x 16 tokens,
-  // 32/8 heads, 9000 keys: 73 us, 110 with one); above 128 columns their O does not fit the registers. With 20 rows two warps
-  // of two blocks took 25 us, four of one 17.
+  // 32/8 heads, 9000 keys: 68 us, 110 with one); above 128 columns their O does not fit the registers. With 20 rows two warps
+  // of two blocks took 25 us, four of one 16.
   p.nb = p.rows > 32 && D <= 128 ? 2 : 1;
   p.wr = p.rows <= 8 ? 1 : p.rows <= 16 ? 2 : 4;
   const int64_t tile = 8 * p.nb * p.wr;
@@ -1190,8 +1190,8 @@ int attention_paged_launch(const AttnPagedProblem& p, cudaStream_t stream) {
   a.ctl.debug = p.debug;
   // TMA takes 16 slots of a page at a time, and maps of positive strides below 2^40 bytes. It moves 128 bytes of a row a step,
   // whatever part of them the head fills, so heads that are no multiple of 128 are copied faster by cp.async where there is much
-  // to read (16 x 16384 keys of 64: 96 us, by TMA 104; 16 x 8000 of 80: 126 and 143; of 128: 137 and 133), while it starts sooner
-  // (777 keys of 64: 9.0 us, by cp.async 11).
+  // to read (16 x 16384 keys of 64: 89 us, by TMA 104; 16 x 8000 of 80: 126 and 143; of 128: 137 and 133), while it starts sooner
+  // (777 keys of 64: 8.3 us, by cp.async 11).
   const bool few_keys = p.batch * c.kv_heads * (a.capacity / 32 + 1) <= int64_t(plan.blocks) * 8;
   CUtensorMap mk, mv;
   memset(&mk, 0, sizeof(mk));

@@ -9,9 +9,9 @@
 //
 // Bound by memory: each value is read once and written once. A block owns a few tokens and a chunk of their heads; it works
 // out its tokens' (cos, sin) once into shared memory, a thread takes those of one place of a head into registers and walks over
-// the heads. (With a table read for each vector 16384 x 40 x 128 took 72 us instead of 58: eight lanes' reads of it met in the
-// same banks.) 58 us are 5.8 TB/s, 88% of the measured copy rate; pairs next to each other 56.8 us; 8192 tokens of f32 to bf16
-// 42.6 us, 90%; the append of 2 x 8192 tokens with 32 + 8 + 8 heads of 128 76 us, 80%: its start (positions, the page table,
+// the heads. (With a table read for each vector 16384 x 40 x 128 took 72 us instead of 56: eight lanes' reads of it met in the
+// same banks.) 56.3 us are 6.0 TB/s, 91% of the measured copy rate; pairs next to each other 55.1 us; 8192 tokens of f32 to
+// bf16 42.0 us, 92%; the append of 2 x 8192 tokens with 32 + 8 + 8 heads of 128 75 us, 82%: its start (positions, the page table,
 // the angles) passes without loads in flight.
 #include <algorithm>
 #include <cmath>
@@ -276,7 +276,7 @@ int launch_rope_for(RopeArgs& a, int rot, bool interleaved, cudaStream_t stream,
   // The widest vectors that every tensor's alignment and the rotated part's width allow; pairs lie within a vector or in
   // two of them, so a rotated part that is no whole number of vectors takes narrower ones.
   // (Half layout: two vectors a unit, and angles for each: with 8 values 80 registers and three blocks an SM, 16384 x 40 x 128
-  // 64 us, with 4 values 58.)
+  // 64 us, with 4 values 56.)
   int V = interleaved ? 8 : 4;
   for (; V > (interleaved ? 2 : 1); V = V == 8 ? 4 : interleaved ? 2 : 1) {
     bool fit = a.dim % V == 0 && (interleaved ? rot : rot / 2) % V == 0;
