@@ -90,7 +90,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
 
 def build_torch_ops(force: bool = False, verbose: bool = False) -> str:
     """Compile csrc/torch_ops.cpp with the host compiler against torch's headers into libnpub200_torch.so."""
-    if not (force or _stale(TORCH_LIB, [TORCH_SRC, LIB, os.path.join(INCLUDE, "npu_b200.h")])):
+    if not (force or _stale(TORCH_LIB, [TORCH_SRC, LIB, *_headers()])):
         return TORCH_LIB
     import torch
     from torch.utils import cpp_extension as ce

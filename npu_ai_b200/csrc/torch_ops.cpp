@@ -22,6 +22,7 @@
 #include <vector>
 
 #include "npu_b200.h"
+#include "overlap.h"
 
 namespace {
 
@@ -373,11 +374,25 @@ npub200_rotation rotation_of(const at::Tensor& freqs, const at::Tensor& x, bool 
   return r;
 }
 
+// The bytes of a tensor of an operator (up to four dimensions).
+npub200::ByteRuns runs_of(const at::Tensor& t) {
+  TORCH_CHECK_VALUE(t.dim() <= npub200::kOverlapDims, "a tensor of ", t.dim(), " dimensions");
+  return npub200::byte_runs(t.data_ptr(), t.element_size(), int(t.dim()), t.sizes().data(), t.strides().data());
+}
+
+// Whether b is a itself: the same elements in the same places, so that who reads one of them is who writes it.
+bool same_tensor(const at::Tensor& a, const at::Tensor& b) {
+  if (a.data_ptr() != b.data_ptr() || a.scalar_type() != b.scalar_type() || a.sizes() != b.sizes()) return false;
+  for (int64_t i = 0; i < a.dim(); ++i)
+    if (a.size(i) > 1 && a.stride(i) != b.stride(i)) return false;
+  return true;
+}
+
 // A tensor that a kernel writes: no element twice, and `from` itself or nothing of it.
 void check_written(const at::Tensor& t, const char* name, const at::Tensor* from = nullptr) {
   TORCH_CHECK_VALUE(at::has_internal_overlap(t) != at::MemOverlap::Yes, name, " must not hold an element twice");
-  TORCH_CHECK_VALUE(from == nullptr || at::get_overlap_status(t, *from) != at::MemOverlapStatus::Partial, name,
-                    " must be the input itself or share no element with it");
+  TORCH_CHECK_VALUE(from == nullptr || same_tensor(t, *from) || !npub200::bytes_overlap(runs_of(t), runs_of(*from)), name,
+                    " must be the input itself or share no element with it: they overlap");
 }
 
 // Two tensors of which one is written while the other is read, or both are written: nothing in common, as far as their strides

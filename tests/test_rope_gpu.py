@@ -228,3 +228,22 @@ def test_many_tokens_and_heads(cuda_device):
         y = kernels.rope(x, f, H, starts, head_major=head_major)
         at = starts.long()[:, None] + torch.arange(S, device=dev)
         check(heads_of(y, H, head_major), *turned(heads_of(x, H, head_major), at, f))
+
+
+def test_outputs_that_overlap_are_refused(cuda_device):
+    """Columns of one buffer, which are no dense tensors: an output moved inside its input is refused, one next to it taken."""
+    from npu_ai_b200 import kernels
+    dev = cuda_device
+    B, S, H, D = 2, 5, 4, 64
+    f = frequencies(D, dev)
+    buf = make(dev, B, S, 3 * H, D, BF16, False, 4)
+    x, keep = buf[..., :H * D], buf.clone()
+    for out in (buf[..., D // 2:D // 2 + H * D], buf[..., H * D - 2:2 * H * D - 2], buf.view(torch.float32)[..., :H * D],
+                torch.as_strided(buf, x.shape, (x.stride(0), x.stride(1) - 8, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            kernels.rope(x, f, H, 7, out=out)
+    assert torch.equal(buf, keep)
+    want = kernels.rope(x, f, H, 7)
+    assert torch.equal(kernels.rope(x, f, H, 7, out=buf[..., H * D:2 * H * D]), want)
+    assert torch.equal(buf[..., :H * D], keep[..., :H * D]) and torch.equal(buf[..., 2 * H * D:], keep[..., 2 * H * D:])
+    assert torch.equal(kernels.rope(x, f, H, 7, out=x), want) and torch.equal(x, want)
