@@ -296,8 +296,10 @@ typedef struct npub200_paged_cache {
  * (counts NULL: all) and that position lies within the table (0 ... table_width * page_size - 1); other tokens write
  * nothing. With a rotation the keys turn by their positions first (as npub200_rope), and so do the queries in the same
  * launch: q_out [batch, seq, heads, head_dim] bf16, every row, whatever counts says (heads 0: no queries; q_out may be q
- * itself). q, k and v are of one type, bf16 or f32, strided as in npub200_attention; k and v hold the cache's heads. No two
- * tokens of a call may have the same slot (which of them stays is then undefined). Allocates nothing. */
+ * itself). q, k and v are of one type, bf16 or f32, strided as in npub200_attention; k and v hold the cache's heads. What is
+ * written has no element in common with anything else: the k pages, the v pages and q_out not with each other, nor with k, v
+ * and q (but q_out with q as said). No two tokens of a call may have the same slot (which of them stays is then undefined).
+ * Allocates nothing. */
 int npub200_paged_append(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, void* q_out, int64_t o_sb, int64_t o_ss,
                          int64_t o_sh, int64_t heads, const void* k, int64_t k_sb, int64_t k_ss, int64_t k_sh,
                          const void* v, int64_t v_sb, int64_t v_ss, int64_t v_sh, int dtype,

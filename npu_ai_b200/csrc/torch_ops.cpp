@@ -395,11 +395,9 @@ void check_written(const at::Tensor& t, const char* name, const at::Tensor* from
                     " must be the input itself or share no element with it: they overlap");
 }
 
-// Two tensors of which one is written while the other is read, or both are written: nothing in common, as far as their strides
-// tell.
-void check_apart(const at::Tensor& a, const at::Tensor& b, const char* names) {
-  const auto s = at::get_overlap_status(a, b);
-  TORCH_CHECK_VALUE(s != at::MemOverlapStatus::Full && s != at::MemOverlapStatus::Partial, names, " must not overlap");
+// Two tensors of which one is written while the other is read, or both are written: nothing in common.
+void check_apart(const npub200::ByteRuns& a, const npub200::ByteRuns& b, const char* names) {
+  TORCH_CHECK_VALUE(!npub200::bytes_overlap(a, b), names, " must not overlap");
 }
 
 // Rotary positions (npub200_rope): x (B, S, heads * d), or (B, heads, S, d) when head-major, like the result.
@@ -479,7 +477,12 @@ std::optional<at::Tensor> paged_append(const at::Tensor& k, const at::Tensor& v,
                     v.scalar_type(), " ", v.sizes());
   check_written(k_pages, "k_pages");
   check_written(v_pages, "v_pages");
-  check_apart(k_pages, v_pages, "k_pages and v_pages");
+  const npub200::ByteRuns kp = runs_of(k_pages), vp = runs_of(v_pages), k_runs = runs_of(k), v_runs = runs_of(v);
+  check_apart(kp, vp, "k_pages and v_pages");
+  check_apart(kp, k_runs, "k_pages and k");
+  check_apart(kp, v_runs, "k_pages and v");
+  check_apart(vp, k_runs, "v_pages and k");
+  check_apart(vp, v_runs, "v_pages and v");
   const int32_t* starts_ptr = vector_ptr<int32_t>(starts, k_pages, B, "starts");
   const int32_t* counts_ptr = vector_ptr<int32_t>(counts, k_pages, B, "counts");
   npub200_rotation r = {};
@@ -492,12 +495,18 @@ std::optional<at::Tensor> paged_append(const at::Tensor& k, const at::Tensor& v,
     qr = head_rows(*q, k_pages, head_major, heads, c.head_dim, "q");
     TORCH_CHECK_VALUE(q->size(0) == B && q->size(head_major ? 2 : 1) == S && q->scalar_type() == k.scalar_type(),
                       "q must have k's batch, tokens and type, got ", q->scalar_type(), " ", q->sizes());
+    const npub200::ByteRuns q_runs = runs_of(*q);
+    check_apart(kp, q_runs, "k_pages and q");
+    check_apart(vp, q_runs, "v_pages and q");
     if (q_out.has_value()) {
       TORCH_CHECK_VALUE(q_out->sizes() == q->sizes() && q_out->scalar_type() == at::kBFloat16,
                         "q_out must be bf16 with q's shape ", q->sizes(), ", got ", q_out->scalar_type(), " ", q_out->sizes());
       check_written(*q_out, "q_out", &*q);
-      check_apart(*q_out, k, "q_out and k");
-      check_apart(*q_out, v, "q_out and v");
+      const npub200::ByteRuns out_runs = runs_of(*q_out);
+      check_apart(out_runs, k_runs, "q_out and k");
+      check_apart(out_runs, v_runs, "q_out and v");
+      check_apart(out_runs, kp, "q_out and k_pages");
+      check_apart(out_runs, vp, "q_out and v_pages");
       out = *q_out;
     } else {
       out = empty_like_device(q->sizes(), at::kBFloat16, k_pages);

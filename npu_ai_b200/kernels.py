@@ -682,7 +682,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     freqs, interleaved, magnitude: as in rope; without freqs k is stored as it is.
     q, heads:         queries of k's type and layout with `heads` heads, rotated by the same positions (every row); needs
                       freqs. Returned in bf16, in `q_out` if given (which may be q itself).
-    Keys are rotated in f32 and rounded once. No two tokens may share a slot.
+    Keys are rotated in f32 and rounded once. No two tokens may share a slot, and the pools and q_out share no element with
+    each other or with k, v and q (a sequence's keys are copied out of a pool before they are appended to it).
     """
     _require_cuda(k, "k")
     if q is not None and heads is None:

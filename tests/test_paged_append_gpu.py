@@ -175,3 +175,43 @@ def test_empty_calls_and_refusals(cuda_device):
     kp4, vp4 = pool(dev, 4, 8, H, D, fill=0.0)
     with pytest.raises(ValueError, match="overlap"):
         kernels.paged_append(mha, mha.clone(), kp4, vp4, table, ints, q=mha.clone(), heads=H, freqs=f, q_out=mha)
+
+
+def test_operands_that_overlap_are_refused(cuda_device):
+    """Sources inside the pools, queries written into them, pools moved inside one buffer: refused, whatever the strides;
+    neighbours in one buffer are taken."""
+    from npu_ai_b200 import kernels
+    dev = cuda_device
+    B, S, H, hk, D, page = 2, 8, 4, 2, 64, 8
+    kp, vp = pool(dev, 6, page, hk, D, fill=1.0)
+    k, v = (make(dev, B, S, hk, D, BF16, False, i) for i in range(2))
+    q = make(dev, B, S, H, D, BF16, False, 2)
+    table = torch.tensor([[0], [1]], dtype=torch.int32, device=dev)
+    zero = torch.zeros(B, dtype=torch.int32, device=dev)
+    f = frequencies(D, dev)
+
+    def call(k=k, v=v, kp=kp, vp=vp, **kw):
+        return kernels.paged_append(k, v, kp, vp, table, zero, **kw)
+    tokens, wide = (t[2:4].flatten(2) for t in (kp, vp))  # whole pages of a pool as new tokens
+    inside = kp.flatten(0, 1).flatten(1).view(6, page, hk * D)
+    long = torch.zeros(6 * page * hk * D + 64, dtype=BF16, device=dev)
+    moved = [long[i:i + kp.numel()].view_as(kp) for i in (0, 64)]
+    rows = torch.zeros(6, page, 2 * hk, D, dtype=BF16, device=dev)  # views that are not dense
+    both = torch.zeros(B, S, (H + 2 * hk) * D, dtype=BF16, device=dev)
+    turned = dict(q=q, heads=H, freqs=f)
+    for bad in (dict(k=tokens), dict(v=tokens), dict(k=wide), dict(v=wide), dict(k=inside[:2], v=inside[3:5]),
+                dict(kp=moved[0], vp=moved[1]), dict(kp=rows[:, :, :hk], vp=rows[:, :, 1:1 + hk]),
+                dict(kp=rows[:, :, :hk], k=rows[2:4].flatten(2)[..., 64:192]),
+                dict(turned, q=torch.cat((kp, vp), 2)[:2].flatten(2), q_out=kp.view(3, page, 2 * hk, D)[:2].flatten(2)),
+                dict(turned, q=rows[:2].flatten(2), kp=rows[:, :, :hk]),
+                dict(turned, k=both[..., 64:64 + hk * D], q_out=both[..., :H * D]),
+                dict(turned, v=both[..., H * D - 8:(H + hk) * D - 8], q_out=both[..., :H * D])):
+        with pytest.raises(ValueError, match="overlap"):
+            call(**bad)
+    assert bool((kp == 1).all()) and bool((vp == 1).all())
+    kp2, vp2 = pool(dev, 6, page, hk, D, fill=0.0)
+    want = call(kp=kp2, vp=vp2, **turned)
+    both[..., H * D:(H + hk) * D], both[..., (H + hk) * D:] = k, v
+    got = call(kp=rows[:, :, :hk], vp=rows[:, :, hk:], k=both[..., H * D:(H + hk) * D], v=both[..., (H + hk) * D:],
+               q_out=both[..., :H * D], **turned)
+    assert torch.equal(got, want) and torch.equal(rows[:, :, :hk], kp2) and torch.equal(rows[:, :, hk:], vp2)
