@@ -546,7 +546,10 @@ at::Tensor attention_paged(const at::Tensor& q, const at::Tensor& k_pages, const
     out = *out_arg;
     TORCH_CHECK_VALUE(out.sizes() == at::IntArrayRef(shape), "attention output must be ", at::IntArrayRef(shape), ", got ",
                       out.sizes());
-    check_written(out, "out");
+    check_written(out, "out", &q);
+    const npub200::ByteRuns out_runs = runs_of(out);
+    check_apart(out_runs, runs_of(k_pages), "out and k_pages");
+    check_apart(out_runs, runs_of(v_pages), "out and v_pages");
   } else {
     out = empty_like_device(shape, out_dtype.value_or(at::kFloat), k_pages);
   }

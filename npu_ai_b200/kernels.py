@@ -700,7 +700,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     """softmax(q k^T * scale) v of a few new tokens of each sequence over its keys in the pages of a cache.
 
     q:          bf16 (B, Sq, heads*D), or (B, heads, Sq, D) when head_major_in; strides in multiples of 8 elements. The output
-                (B, Sq, heads*D), or (B, heads, Sq, D) when head_major_out, f32 unless `out_dtype` or `out` says otherwise.
+                (B, Sq, heads*D), or (B, heads, Sq, D) when head_major_out, f32 unless `out_dtype` or `out` says otherwise. `out`
+                may be q itself and shares no element with q or the pools otherwise.
     k_pages, v_pages, page_table: as in paged_append (strides in multiples of 8 elements); query head h reads head
                 h // (heads // kv_heads). Keys on a page that is not there are seen by no row.
     kv_lens:    int32 [B], the valid keys of each sequence, its new tokens among them (clamped to the table). Device tensors

@@ -370,3 +370,43 @@ def test_empty_calls_and_refusals(cuda_device):
             call(**bad)
     with pytest.raises(RuntimeError, match="variant"):
         call(variant=-1)
+
+
+def test_outputs_that_overlap_are_refused(cuda_device):
+    """An output that holds some of the queries elsewhere, or lies in a pool, is refused; one that is the queries is taken."""
+    from npu_ai_b200 import kernels
+    d = cuda_device
+    H, hk, D, page, Sq = 4, 2, 64, 16, 3
+    c = Cache(d, [700, 40], hk, D, page)
+    buf = torch.randn(2, Sq, 3 * H * D, device=d).to(BF16)
+    q, keep = buf[..., :H * D], buf.clone()
+    call = lambda q=q, **kw: kernels.paged_attention(q, c.k, c.v, c.table, c.lens, H, **kw)
+    pool = torch.empty(50, page, 2 * hk + 1, D, dtype=BF16, device=d)
+    dense = torch.randn(2, H, Sq, D, device=d).to(BF16)
+    for bad in (dict(out=buf[..., D:D + H * D]), dict(out=buf[..., H * D - 2:2 * H * D - 2]),
+                dict(out=buf.view(torch.float32)[..., :H * D]),
+                dict(q=dense, head_major_in=True, out=dense.view(2, Sq, H * D)),
+                dict(out=c.k.flatten()[:2 * Sq * H * D].view(2, Sq, H * D)),
+                dict(out=c.v.view(torch.float32).flatten()[-2 * Sq * H * D:].view(2, Sq, H * D))):
+        with pytest.raises(ValueError, match="overlap"):
+            call(**bad)
+    with pytest.raises(ValueError, match="overlap"):
+        kernels.paged_attention(q, pool[:, :, :hk], pool[:, :, hk:2 * hk], c.table, c.lens, H, out=pool[:2, :Sq].flatten(2)[..., 64:])
+    assert torch.equal(buf, keep)
+    want = call(out_dtype=BF16)
+    assert torch.equal(call(out=buf[..., H * D:2 * H * D]), want)
+
+
+@pytest.mark.parametrize("H,hk,Sq", [(4, 4, 1), (8, 2, 3), (8, 2, 5), (4, 2, 40)])
+def test_outputs_in_place_of_the_queries(cuda_device, H, hk, Sq):
+    """`out` may be q itself: bit for bit what a fresh output holds, over splits of one block and of many."""
+    from npu_ai_b200 import kernels
+    d = cuda_device
+    for lens, page, variant in (([9000, 77, 0], 16, 0), ([300, 20, 1], 7, 0), ([9000, 500, 40], 16, 1), ([300, 20, 0], 16, 1000)):
+        c = Cache(d, lens, hk, 64, page)
+        q = torch.randn(3, Sq, H * 64, device=d).to(BF16)
+        for _ in range(3):
+            x = q.clone()
+            want = kernels.paged_attention(q, c.k, c.v, c.table, c.lens, H, out_dtype=BF16, variant=variant)
+            assert torch.equal(kernels.paged_attention(x, c.k, c.v, c.table, c.lens, H, out=x, variant=variant), want)
+            assert torch.equal(x, want)
