@@ -400,6 +400,11 @@ void check_apart(const npub200::ByteRuns& a, const npub200::ByteRuns& b, const c
   TORCH_CHECK_VALUE(!npub200::bytes_overlap(a, b), names, " must not overlap");
 }
 
+// What was written has another version now, by which autograd and graph tools tell (inference tensors have none).
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // Rotary positions (npub200_rope): x (B, S, heads * d), or (B, heads, S, d) when head-major, like the result.
 at::Tensor rope(const at::Tensor& x, const at::Tensor& freqs, int64_t heads, const std::optional<at::Tensor>& out_arg,
                 std::optional<at::ScalarType> out_dtype, int64_t start, const std::optional<at::Tensor>& positions,
@@ -426,6 +431,7 @@ at::Tensor rope(const at::Tensor& x, const at::Tensor& freqs, int64_t heads, con
   check_rc(npub200_rope(x.data_ptr(), xr.sb, xr.ss, xr.sh, x_code, out.data_ptr(), orr.sb, orr.ss, orr.sh,
                         dtype_code(out, "out"), B, S, heads, d, &r, start, p.starts, p.each, p.sb, p.ss, stream_of(x)),
            "npub200::rope");
+  if (out_arg.has_value()) written(out);
   return out;
 }
 
@@ -520,6 +526,9 @@ std::optional<at::Tensor> paged_append(const at::Tensor& k, const at::Tensor& v,
                                 k.data_ptr(), kr.sb, kr.ss, kr.sh, v.data_ptr(), vr.sb, vr.ss, vr.sh, code, &c, starts_ptr,
                                 counts_ptr, B, S, freqs.has_value() ? &r : nullptr, stream_of(k_pages)),
            "npub200::paged_append");
+  written(k_pages);
+  written(v_pages);
+  if (q_out.has_value()) written(*out);
   return out;
 }
 
@@ -566,6 +575,7 @@ at::Tensor attention_paged(const at::Tensor& q, const at::Tensor& k_pages, const
                                    out_code, B, heads, S, float(scale), causal ? 1 : 0, starts, float(softcap), slopes_ptr,
                                    ws.get(), ws_bytes, int(variant), stream_of(k_pages)),
            "npub200::attention_paged");
+  if (out_arg.has_value()) written(out);
   return out;
 }
 
@@ -582,15 +592,15 @@ TORCH_LIBRARY(npub200, m) {
         "int? q_start=None, Tensor? q_starts=None, int prefix=0, Tensor? prefixes=None, Tensor? kv_lens=None, "
         "Tensor? doc_offsets=None, float softcap=0., Tensor? slopes=None, Tensor? distance_bias=None, "
         "Tensor? mask=None) -> Tensor");
-  m.def("rope(Tensor x, Tensor freqs, int heads, Tensor? out=None, ScalarType? out_dtype=None, int start=0, "
+  m.def("rope(Tensor x, Tensor freqs, int heads, Tensor(a!)? out=None, ScalarType? out_dtype=None, int start=0, "
         "Tensor? positions=None, bool interleaved=False, float magnitude=1., bool inverse=False, "
-        "bool head_major=False) -> Tensor");
-  m.def("paged_append(Tensor k, Tensor v, Tensor k_pages, Tensor v_pages, Tensor page_table, Tensor starts, "
-        "Tensor? counts=None, Tensor? q=None, int heads=0, Tensor? q_out=None, Tensor? freqs=None, "
-        "bool interleaved=False, float magnitude=1., bool head_major=False) -> Tensor?");
-  m.def("attention_paged(Tensor q, Tensor k_pages, Tensor v_pages, Tensor page_table, Tensor kv_lens, Tensor? out, "
+        "bool head_major=False) -> Tensor(a!)");
+  m.def("paged_append(Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor page_table, Tensor starts, "
+        "Tensor? counts=None, Tensor? q=None, int heads=0, Tensor(c!)? q_out=None, Tensor? freqs=None, "
+        "bool interleaved=False, float magnitude=1., bool head_major=False) -> Tensor(c!)?");
+  m.def("attention_paged(Tensor q, Tensor k_pages, Tensor v_pages, Tensor page_table, Tensor kv_lens, Tensor(a!)? out, "
         "ScalarType? out_dtype, int heads, float scale=0., bool causal=True, Tensor? q_starts=None, float softcap=0., "
-        "Tensor? slopes=None, bool head_major_in=False, bool head_major_out=False, int variant=0) -> Tensor");
+        "Tensor? slopes=None, bool head_major_in=False, bool head_major_out=False, int variant=0) -> Tensor(a!)");
 }
 
 TORCH_LIBRARY_IMPL(npub200, CUDA, m) {

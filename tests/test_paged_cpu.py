@@ -203,3 +203,15 @@ def test_division_by_multiplication(d):
         for n in (q * d - 1, q * d, q * d + d - 1):
             if 0 <= n < 2 ** 31:
                 assert (n * mul) >> shift == n // d
+
+
+def test_schemas_name_what_is_written():
+    """Tools that trust a schema would reorder or drop a call that says it writes nothing."""
+    _lib.torch_ops()
+
+    def written(name):
+        schema = getattr(torch.ops.npub200, name).default._schema
+        return schema.is_mutable, [a.name for a in schema.arguments if a.alias_info is not None and a.alias_info.is_write]
+    assert written("rope") == (True, ["out"])
+    assert written("paged_append") == (True, ["k_pages", "v_pages", "q_out"])
+    assert written("attention_paged") == (True, ["out"])

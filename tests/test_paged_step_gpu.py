@@ -111,3 +111,45 @@ def test_runner_methods(cuda_device):
     assert torch.equal(g.paged_attention(turned, pools[0], pools[1], table, starts + 3, H, q_start=starts, out_dtype=BF16),
                        kernels.paged_attention(want, pools[2], pools[3], i32[0], i32[1] + 3, H, q_start=i32[1], out_dtype=BF16))
     kernels.check_status(dev)
+
+
+def test_written_tensors_have_new_versions(cuda_device):
+    """What a call writes counts as written for autograd (a tensor saved before it may not be used after it); what it only
+    reads, and inference tensors, are left alone. Gradients are not tracked through the calls."""
+    from npu_ai_b200 import kernels
+    dev, H, hk, D = cuda_device, 4, 2, 64
+    f, _ = kernels.rope_frequencies(D, device=dev)
+
+    def operands():
+        return dict(q=torch.randn(2, 3, H * D, device=dev).to(BF16), k=torch.randn(2, 3, hk * D, device=dev).to(BF16),
+                    v=torch.randn(2, 3, hk * D, device=dev).to(BF16), kp=torch.zeros(4, 16, hk, D, dtype=BF16, device=dev),
+                    vp=torch.zeros(4, 16, hk, D, dtype=BF16, device=dev), o=torch.empty(2, 3, H * D, dtype=BF16, device=dev),
+                    table=torch.arange(4, dtype=torch.int32, device=dev).view(2, 2),
+                    starts=torch.zeros(2, dtype=torch.int32, device=dev))
+
+    def steps(t):
+        yield ["o"], kernels.rope(t["q"], f, H, out=t["o"])
+        yield [], kernels.rope(t["q"], f, H)
+        yield ["kp", "vp"], kernels.paged_append(t["k"], t["v"], t["kp"], t["vp"], t["table"], t["starts"], q=t["q"], heads=H,
+                                                 freqs=f)
+        yield ["kp", "vp", "q"], kernels.paged_append(t["k"], t["v"], t["kp"], t["vp"], t["table"], t["starts"], q=t["q"],
+                                                      heads=H, q_out=t["q"], freqs=f)
+        yield ["o"], kernels.paged_attention(t["q"], t["kp"], t["vp"], t["table"], t["starts"] + 3, H, out=t["o"])
+        yield [], kernels.paged_attention(t["q"], t["kp"], t["vp"], t["table"], t["starts"] + 3, H)
+    t = operands()
+    before = {n: x._version for n, x in t.items()}
+    for names, y in steps(t):
+        assert y._version == (0 if not names or names == ["kp", "vp"] else before[names[-1]] + 1)
+        for n in names:
+            before[n] += 1
+        assert {n: x._version for n, x in t.items()} == before
+    with torch.inference_mode():
+        for _ in steps(operands()):
+            pass
+    w = torch.ones(2, 3, H * D, device=dev, requires_grad=True)
+    x = torch.zeros(2, 3, H * D, device=dev)
+    loss = (w * x).sum()  # keeps x for w's gradient
+    kernels.rope(torch.ones_like(x), f, H, out=x)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    kernels.check_status(dev)
