@@ -44,6 +44,27 @@ def _as_tensor(x) -> torch.Tensor:
     return torch.from_numpy(np.ascontiguousarray(np.asarray(x, dtype=np.float32)))
 
 
+_INT32 = torch.iinfo(torch.int32)
+
+
+def _int32(t, device, name: str, exact: bool = False):
+    """A tensor of whole numbers as int32 on `device`; what is no tensor is passed on. Numbers that int32 does not hold end at
+    its limits: a page id stays outside every pool, a length or count stays all or nothing, where a cast would wrap them to
+    valid ones. With `exact` (positions, which angles depend on) such numbers are refused where the host has them."""
+    if not isinstance(t, torch.Tensor):
+        return t
+    t = t.detach()
+    if t.dtype.is_floating_point or t.dtype.is_complex or t.dtype in (torch.bool, torch.uint64):
+        raise ValueError(f"{name} must be whole numbers (int32 or a type that converts to it), got {t.dtype}")
+    if torch.iinfo(t.dtype).max > _INT32.max:
+        t = t.to(torch.int64)
+        kept = t.clamp(_INT32.min, _INT32.max)
+        if exact and t.device.type == "cpu" and not torch.equal(kept, t):
+            raise ValueError(f"{name} must fit 32 bits")
+        t = kept
+    return t.to(device, torch.int32)
+
+
 @dataclass
 class NpuWeight:
     """A weight resident in HBM (the reference's NpuWeight, npu/xdna1_gemm.py:89-99).
@@ -408,7 +429,7 @@ class NpuGemm:
 
     # -- a text model's cached steps ------------------------------------------------------------
     def _on_device(self, t, dtype: torch.dtype | None = None):
-        """Tensors go to this runner's device (and type); anything else (ints, None) is passed on."""
+        """Tensors go to this runner's device (and type); None is passed on."""
         return t.detach().to(self.device, dtype) if isinstance(t, torch.Tensor) else t
 
     def _turned(self, t) -> torch.Tensor:
@@ -420,21 +441,25 @@ class NpuGemm:
 
     def rope(self, x, freqs: torch.Tensor, heads: int, positions: int | torch.Tensor = 0, **rotation) -> torch.Tensor:
         """Rotary positions (kernels.rope and its keywords): x (B, S, heads*D), or (B, heads, S, D) with head_major, on any
-        device -> a CUDA tensor of its type (other float types than bf16 become f32) unless `out_dtype` says otherwise."""
+        device -> a CUDA tensor of its type (other float types than bf16 become f32) unless `out_dtype` says otherwise.
+        Positions of any integer type; those of a host tensor have to fit 32 bits, others end at int32's limits."""
         return kernels.rope(self._turned(x), self._on_device(freqs, torch.float64), heads,
-                            self._on_device(positions, torch.int32), **rotation)
+                            _int32(positions, self.device, "positions", exact=True), **rotation)
 
     def paged_append(self, k, v, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
                      starts: torch.Tensor, *, counts: torch.Tensor | None = None, q=None, freqs: torch.Tensor | None = None,
                      **more) -> torch.Tensor | None:
         """New keys and values into the pages of a cache, keys and queries rotated on the way (kernels.paged_append and its
-        keywords). k, v and q may lie on any device; the pages are this device's bf16 tensors, written in place."""
+        keywords). k, v and q may lie on any device; the pages are this device's bf16 tensors, written in place. The table,
+        starts and counts may be of any integer type: a page id that int32 does not hold is a page that is not there, starts
+        as the positions of `rope`."""
         ops = [self._turned(t) if t is not None else None for t in (k, v, q)]
         if any(t is not None and t.dtype != ops[0].dtype for t in ops):
             ops = [t.float() if t is not None else None for t in ops]
         k, v, q = ops
-        return kernels.paged_append(k, v, k_pages, v_pages, self._on_device(page_table, torch.int32),
-                                    self._on_device(starts, torch.int32), counts=self._on_device(counts, torch.int32), q=q,
+        return kernels.paged_append(k, v, k_pages, v_pages, _int32(page_table, self.device, "page_table"),
+                                    _int32(starts, self.device, "starts", exact=True),
+                                    counts=_int32(counts, self.device, "counts"), q=q,
                                     freqs=self._on_device(freqs, torch.float64), **more)
 
     def paged_attention(self, q, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -442,10 +467,11 @@ class NpuGemm:
                         q_start: torch.Tensor | None = None, slopes: torch.Tensor | None = None,
                         out_dtype: torch.dtype | None = None, **more) -> torch.Tensor:
         """Attention of a few new tokens of each sequence over its pages (kernels.paged_attention and its keywords); q on any
-        device and of any float type (bf16 in the kernel), f32 out unless `out_dtype` says otherwise."""
-        return kernels.paged_attention(self._attn_operand(q), k_pages, v_pages, self._on_device(page_table, torch.int32),
-                                       self._on_device(kv_lens, torch.int32), heads, scale,
-                                       q_start=self._on_device(q_start, torch.int32),
+        device and of any float type (bf16 in the kernel), f32 out unless `out_dtype` says otherwise. The table, lengths and
+        starts may be of any integer type; what int32 does not hold ends at its limits."""
+        return kernels.paged_attention(self._attn_operand(q), k_pages, v_pages, _int32(page_table, self.device, "page_table"),
+                                       _int32(kv_lens, self.device, "kv_lens"), heads, scale,
+                                       q_start=_int32(q_start, self.device, "q_start"),
                                        slopes=self._on_device(slopes, torch.float32),
                                        out_dtype=out_dtype or self.out_dtype, **more)
 

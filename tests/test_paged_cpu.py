@@ -215,3 +215,25 @@ def test_schemas_name_what_is_written():
     assert written("rope") == (True, ["out"])
     assert written("paged_append") == (True, ["k_pages", "v_pages", "q_out"])
     assert written("attention_paged") == (True, ["out"])
+
+
+def test_whole_numbers_of_the_runner():
+    """Numbers that int32 does not hold must not wrap to valid ones; types that hold no whole numbers are refused."""
+    from npu_ai_b200.runner import _int32
+    cpu = torch.device("cpu")
+    low, high = -2 ** 31, 2 ** 31 - 1
+    wide = torch.tensor([[-2 ** 63, 2 ** 32, 2 ** 32 + 5, -2 ** 32 + 3], [2 ** 63 - 1, low, high, 7]])
+    assert _int32(wide, cpu, "t").tolist() == [[low, high, high, low], [high, low, high, 7]]
+    assert _int32(torch.tensor([2 ** 32 - 1, 4], dtype=torch.uint32), cpu, "t").tolist() == [high, 4]
+    for t in (torch.int8, torch.uint8, torch.int16, torch.uint16, torch.int32, torch.int64):
+        for exact in (False, True):
+            got = _int32(torch.tensor([0, 5, 127]).to(t), cpu, "t", exact)
+            assert got.dtype == torch.int32 and got.tolist() == [0, 5, 127]
+    assert _int32(torch.tensor([low, high]), cpu, "t", exact=True).tolist() == [low, high]
+    for bad in (2 ** 31, low - 1, -2 ** 63):
+        with pytest.raises(ValueError, match="32 bits"):
+            _int32(torch.tensor([3, bad]), cpu, "t", exact=True)
+    for t in (torch.float32, torch.float64, torch.bfloat16, torch.bool, torch.complex64, torch.uint64):
+        with pytest.raises(ValueError, match="whole numbers"):
+            _int32(torch.ones(2, dtype=t), cpu, "t")
+    assert _int32(None, cpu, "t") is None and _int32(2 ** 40, cpu, "t", exact=True) == 2 ** 40

@@ -153,3 +153,37 @@ def test_written_tensors_have_new_versions(cuda_device):
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
     kernels.check_status(dev)
+
+
+def test_runner_numbers_past_32_bits(cuda_device):
+    """64-bit tables, lengths and positions of the runner's methods: a page id past 32 bits is a page that is not there, and
+    positions that do not fit are refused."""
+    from npu_ai_b200 import kernels
+    from npu_ai_b200.runner import NpuGemm
+    g = NpuGemm()
+    dev, H, hk, D, page = g.device, 4, 2, 64, 16
+    f, _ = kernels.rope_frequencies(D, device=dev)
+    pools = [torch.full((4, page, hk, D), 9.0, dtype=BF16, device=dev) for _ in range(4)]
+    k, v = (torch.randn(2, 3, hk * D, device=dev).to(BF16) for _ in range(2))
+    q = torch.randn(2, 3, H * D, device=dev).to(BF16)
+    starts = torch.zeros(2, dtype=torch.int64)
+    for place in ("cpu", dev):
+        table = torch.tensor([[1, -2 ** 63], [2 ** 32, 2 ** 32 + 5]], device=place)
+        near = torch.tensor([[1, -1], [-1, 99]], dtype=torch.int32, device=dev)
+        counts = torch.tensor([2 ** 40, -2 ** 40 + 3], device=place)
+        g.paged_append(k, v, pools[0], pools[1], table, starts, counts=counts, freqs=f)
+        kernels.paged_append(k, v, pools[2], pools[3], near, starts.to(dev, torch.int32),
+                             counts=torch.tensor([3, 0], dtype=torch.int32, device=dev), freqs=f)
+        assert torch.equal(pools[0], pools[2]) and torch.equal(pools[1], pools[3]) and bool((pools[0][[0, 2, 3]] == 9).all())
+        lens = torch.tensor([2 ** 33 + 1, 2 ** 32 + 7], device=place)
+        o = g.paged_attention(q, pools[0], pools[1], table, lens, H, q_start=torch.tensor([2 ** 40, 0], device=place))
+        want = kernels.paged_attention(q, pools[0], pools[1], near, torch.tensor([32, 32], dtype=torch.int32, device=dev), H,
+                                       q_start=torch.tensor([100, 0], dtype=torch.int32, device=dev))
+        assert torch.equal(o, want) and bool((o[1] == 0).all())
+    far = torch.tensor([0, 2 ** 31])
+    for bad in (lambda: g.rope(q, f, H, far), lambda: g.paged_append(k, v, pools[0], pools[1], table, far, freqs=f),
+                lambda: g.rope(q, f, H, far.float()), lambda: g.paged_attention(q, pools[0], pools[1], table.float(), lens, H),
+                lambda: g.rope(q, f, H, 2 ** 31)):
+        with pytest.raises(ValueError):
+            bad()
+    kernels.check_status(dev)
