@@ -555,7 +555,7 @@ __global__ void __launch_bounds__((kWarps + (TMA ? kLoadWarps : 0)) * 32, kBlock
         }
         // this lane's rows of the scores: c2 and c2 + 1 of each block
         int lim[NB][2], lim_min = INT32_MAX;
-        long long p[NB][2];
+        int near[NB][2];  // of the sequence's positions the one next to the row's: what distances are counted from
         float slope[NB][2], m[NB][2], l[NB][2], o[DP / 16][NB][4];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
@@ -564,8 +564,9 @@ __global__ void __launch_bounds__((kWarps + (TMA ? kLoadWarps : 0)) * 32, kBlock
             const int r = r0 + nb * 8 + c2 + y;
             const bool ok = r < a.rows;
             const int i = ok ? a.by_g(r) : 0;
-            p[nb][y] = at.seq.p0 + i;
-            lim[nb][y] = ok ? keys_seen(a, at.seq.len, p[nb][y]) : at.seq.len;
+            const long long p = at.seq.p0 + i;
+            lim[nb][y] = ok ? keys_seen(a, at.seq.len, p) : at.seq.len;
+            near[nb][y] = int(max(0ll, min(p, (long long)at.seq.len - 1)));
             lim_min = min(lim_min, lim[nb][y]);
             slope[nb][y] = MODS && a.slopes != nullptr ? a.slopes[kvh * a.G + (ok ? r - i * a.G : 0)] * kLog2e : 0.0f;
             m[nb][y] = -INFINITY;
@@ -660,12 +661,15 @@ __global__ void __launch_bounds__((kWarps + (TMA ? kLoadWarps : 0)) * 32, kBlock
                     for (int e = 0; e < 4; ++e) x[n][nb][e] *= a.scale_log2;
               }
               if (a.slopes != nullptr) {
-                // The distance from f32: exact up to 2^24, rounded to a step of itself beyond.
+                // Before the first key and behind the last all distances grow alike, which the softmax does not see: they
+                // are counted from the key next to the row, so that they stay below the number of keys (with p itself a row
+                // 2^30 past 1000 keys had the same distance, in f32, to 64 of them). Exact up to 2^24 keys, off by half a
+                // step of f32 beyond.
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                   for (int y = 0; y < 2; ++y) {
-                    const float ahead = float(p[nb][y] - j0 - g);
+                    const float ahead = float(near[nb][y] - j0 - g);
 #pragma unroll
                     for (int n = 0; n < KT / 16; ++n)
 #pragma unroll

@@ -410,3 +410,28 @@ def test_outputs_in_place_of_the_queries(cuda_device, H, hk, Sq):
             want = kernels.paged_attention(q, c.k, c.v, c.table, c.lens, H, out_dtype=BF16, variant=variant)
             assert torch.equal(kernels.paged_attention(x, c.k, c.v, c.table, c.lens, H, out=x, variant=variant), want)
             assert torch.equal(x, want)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("variant", [0, 1])
+def test_slopes_of_far_queries(cuda_device, causal, variant):
+    """Queries far from every key: the distances differ by less than a step of f32 there, and the softmax depends on their
+    differences. The part of a bias that all keys share drops out, so the tolerance is the one of a query next to them."""
+    from npu_ai_b200 import kernels
+    d = cuda_device
+    lens, H, hk, Sq = [200, 33, 1, 500], 4, 2, 3
+    slopes = torch.tensor([0.5, 0.011, 2.0 ** -8, 0.3], device=d)
+    g = torch.Generator(device=d).manual_seed(5)
+    c = Cache(d, lens, hk, 64, 16)
+    q = torch.randn(4, Sq, H * 64, generator=g, device=d).to(BF16)
+    for start in (2 ** 31 - 1, 2 ** 30 + 7, 2 ** 25 + 1) + (() if causal else (-2 ** 31, -2 ** 25 - 3)):
+        starts = ints(d, *(start,) * 4)
+        out = kernels.paged_attention(q, c.k, c.v, c.table, c.lens, H, causal=causal, q_start=starts, slopes=slopes,
+                                      variant=variant)
+        kernels.check_status(d)
+        near = c.lens - 1 if start > 0 else torch.zeros_like(c.lens)
+        for i in range(Sq):
+            row = (q[:, i:i + 1], c.k_flat, c.v_flat, H, hk)
+            ref, _ = oracle(*row, causal=causal, kv_lens=c.lens, slopes=slopes, q_start=starts.long() + i)
+            tol = oracle(*row, kv_lens=c.lens, slopes=slopes, q_start=near)[1]
+            check(out[:, i:i + 1], ref, tol, H, False)
