@@ -36,6 +36,7 @@
 #include "attention_sm100.cuh"
 #include "fast_div.cuh"
 #include "internal.h"
+#include "paged_split.cuh"
 
 namespace npub200 {
 
@@ -80,7 +81,7 @@ struct PagedArgs {
   int rows, row_tiles, slot_rows;  // rows of a (sequence, kv head), tiles of a worker's rows, rows of a part
   Divisor by_row_tiles, by_slot_rows;
   int min_span, round_span;  // least tiles of a block's run; 1: a whole number of them for each worker
-  float per_block;        // 1 / blocks
+  Divisor by_blocks;
   // What there is to join: of the item that begins in each block's run and goes on behind it. (sequence, kv head and row
   // tile, parts or 0, -)
   int4* rec;
@@ -416,11 +417,8 @@ __global__ void __launch_bounds__((kWarps + (TMA ? kLoadWarps : 0)) * 32, kBlock
     }
     total *= per_tile;
     // Whole tiles for every worker: 7 for four took as long as 8, and there were more parts to join (1 x 8192 keys, 8 heads
-    // 15.9 us, 14.4 with 8). (A f32 product is off by less than 1 / blocks below 2^20 tiles: one more than its whole part is
-    // never short.)
-    span = max(total < (1 << 20) ? (long long)(float(int(total)) * a.per_block) + 1 : (total + gridDim.x - 1) / gridDim.x,
-               (long long)a.min_span);
-    if (a.round_span) span = (span + NW - 1) / NW * NW;
+    // 15.9 us, 14.4 with 8).
+    span = tiles_of_run(total, int(gridDim.x), a.by_blocks, a.min_span, a.round_span ? NW : 1);
     c0 = blockIdx.x * span;
     run = max(0ll, min(total, c0 + span) - c0);
     const long long u0 = c0 + run * wk / NW, u1 = c0 + run * (wk + 1) / NW;
@@ -1183,7 +1181,7 @@ int attention_paged_launch(const AttnPagedProblem& p, cudaStream_t stream) {
   a.by_slot_rows = divisor(a.slot_rows);
   a.min_span = p.variant > 0 ? p.variant : 1;
   a.round_span = p.variant == 0;
-  a.per_block = 1.0f / float(plan.blocks);
+  a.by_blocks = divisor(plan.blocks);
   uint8_t* ws = static_cast<uint8_t*>(p.workspace);
   a.rec = reinterpret_cast<int4*>(ws);
   a.part_ml = reinterpret_cast<float2*>(ws + plan.ml_offset);

@@ -237,3 +237,43 @@ def test_whole_numbers_of_the_runner():
         with pytest.raises(ValueError, match="whole numbers"):
             _int32(torch.ones(2, dtype=t), cpu, "t")
     assert _int32(None, cpu, "t") is None and _int32(2 ** 40, cpu, "t", exact=True) == 2 ** 40
+
+
+@pytest.fixture(scope="module")
+def host_code(tmp_path_factory):
+    """csrc/fast_div.cuh and csrc/paged_split.cuh as the host compiler builds them."""
+    d = tmp_path_factory.mktemp("host")
+    (d / "h.cpp").write_text(
+        '#define __host__\n#define __device__\n#include "paged_split.cuh"\nusing namespace npub200;\n'
+        'extern "C" int quotient(int64_t d, int n) { return divisor(d)(n); }\n'
+        'extern "C" int64_t run(int64_t total, int blocks, int least, int workers) {\n'
+        '  return tiles_of_run(total, blocks, divisor(blocks), least, workers);\n}\n')
+    so = d / "h.so"
+    subprocess.run(["g++", "-O1", "-std=c++17", "-Wall", "-Werror", "-fPIC", "-shared", f"-I{ROOT}/npu_ai_b200/csrc",
+                    str(d / "h.cpp"), "-o", str(so)], check=True)
+    lib = ctypes.CDLL(str(so))
+    lib.quotient.argtypes = [ctypes.c_int64, ctypes.c_int]
+    lib.run.restype, lib.run.argtypes = ctypes.c_int64, [ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int]
+    return lib
+
+
+def test_division_as_it_is_compiled(host_code):
+    """Every quotient's borders over the divisors and the range that the kernels use."""
+    for d in [*range(1, 70), 127, 128, 129, 296, 320, 1000, 65535, 2 ** 20 + 1, 2 ** 30 - 1, 2 ** 30, 2 ** 31 - 1]:
+        for q in {0, 1, 2, 3, (2 ** 31 - 1) // d // 2, (2 ** 31 - 1) // d - 1, (2 ** 31 - 1) // d}:
+            for n in (q * d - 1, q * d, q * d + d // 2, q * d + d - 1):
+                if 0 <= n < 2 ** 31:
+                    assert host_code.quotient(d, n) == n // d, (d, n)
+
+
+@pytest.mark.parametrize("blocks", [1, 148, 264, 296, 320])
+@pytest.mark.parametrize("workers", [1, 2, 4])
+def test_runs_are_the_least_that_hold_all_tiles(host_code, blocks, workers):
+    for total in {*range(0, 40), *(k * blocks + e for k in (1, 2, 3, 4, 5, 8, 16, 31, 100, 2 ** 12) for e in (-1, 0, 1)),
+                  *(2 ** 31 - blocks + e for e in (-1, 0, 1, 2)), 2 ** 20 - 1, 2 ** 20, 2 ** 31, 2 ** 40 + 3}:
+        if total < 0:
+            continue
+        for least in (1, 3, 1000):
+            run = host_code.run(total, blocks, least, workers)
+            want = max(-(-total // blocks), least)
+            assert run == -(-want // workers) * workers, (total, least)
