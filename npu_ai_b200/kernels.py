@@ -608,7 +608,7 @@ def _operators():
 
 def rope_frequencies(rot_dim: int, base: float = 10000.0, scaling: str | None = None, factor: float = 1.0,
                      original_length: int = 4096, beta_fast: float = 32.0, beta_slow: float = 1.0,
-                     device: torch.device | str | None = None) -> tuple[torch.Tensor, float]:
+                     device: torch.device | str | None = None, *, whole_pairs: bool = False) -> tuple[torch.Tensor, float]:
     """(freqs, magnitude) of `rope` and `paged_append`: float64 [rot_dim / 2] radians a position, base^(-2j / rot_dim), and
     the factor of the rotated values.
 
@@ -619,6 +619,9 @@ def rope_frequencies(rot_dim: int, base: float = 10000.0, scaling: str | None = 
       "yarn"    pairs that turn more than beta_fast times over original_length keep their frequency, those that turn less
                 than beta_slow times have it divided by the factor, a linear ramp over the logarithm of their turns between;
                 magnitude 0.1 ln(factor) + 1 (for factors above 1).
+    whole_pairs: the ramp of "yarn" runs from one whole pair to another, the bounds above rounded outwards to them. Most weights
+                published with yarn were trained with this form and need it: the two differ by up to a third of a frequency
+                in the middle pairs.
     """
     if rot_dim <= 0 or rot_dim % 2:
         raise ValueError(f"rot_dim must be positive and even (got {rot_dim})")
@@ -634,12 +637,20 @@ def rope_frequencies(rot_dim: int, base: float = 10000.0, scaling: str | None = 
     if scaling == "linear":
         f = f / factor
     elif scaling == "yarn":
-        turns = original_length * f / (2.0 * math.pi)
-        keep = ((turns / beta_slow).log() / math.log(beta_fast / beta_slow)).clamp(0.0, 1.0)
+        if whole_pairs:
+            pair = [rot_dim * math.log(original_length / (2.0 * math.pi * b)) / (2.0 * math.log(base))
+                    for b in (beta_fast, beta_slow)]  # that turns b times
+            first, last = max(math.floor(pair[0]), 0), min(math.ceil(pair[1]), rot_dim - 1)
+            keep = 1.0 - ((j / 2 - first) / max(last - first, 0.001)).clamp(0.0, 1.0)
+        else:
+            turns = original_length * f / (2.0 * math.pi)
+            keep = ((turns / beta_slow).log() / math.log(beta_fast / beta_slow)).clamp(0.0, 1.0)
         f = f * keep + f / factor * (1.0 - keep)
         magnitude = 0.1 * math.log(factor) + 1.0
     elif scaling not in (None, "ntk"):
         raise ValueError(f"unknown scaling {scaling!r} (None, 'linear', 'ntk' or 'yarn')")
+    if whole_pairs and scaling != "yarn":
+        raise ValueError("whole_pairs is a form of the yarn scaling")
     return f.to(device) if device is not None else f, magnitude
 
 

@@ -277,3 +277,32 @@ def test_runs_are_the_least_that_hold_all_tiles(host_code, blocks, workers):
             run = host_code.run(total, blocks, least, workers)
             want = max(-(-total // blocks), least)
             assert run == -(-want // workers) * workers, (total, least)
+
+
+def test_yarn_frequencies_between_whole_pairs():
+    """The ramp from the 20th pair to the 46th (128 columns, base 10^4, 4096 tokens, turns of 32 and 1: the pairs 20.94 and
+    45.03), and at ends that the head does not have."""
+    f, _ = kernels.rope_frequencies(128)
+    got, m = kernels.rope_frequencies(128, scaling="yarn", factor=16.0, whole_pairs=True)
+    assert m == 0.1 * math.log(16.0) + 1.0
+    for j in range(64):
+        slow = min(1.0, max(0.0, (j - 20) / 26))
+        assert math.isclose(got[j], float(f[j]) * (1.0 - slow) + float(f[j]) / 16.0 * slow, rel_tol=1e-12)
+    plain = kernels.rope_frequencies(128, scaling="yarn", factor=16.0)[0]
+    assert 0.3 < float((plain / got - 1.0).abs().max()) < 0.4  # what separates the two forms
+    # 64 tokens: the pair of 32 turns lies before the first (-7.9), that of one turn at 16.1
+    short = kernels.rope_frequencies(128, scaling="yarn", factor=4.0, original_length=64, whole_pairs=True)[0]
+    for j in range(64):
+        slow = min(1.0, j / 17)
+        assert math.isclose(short[j], float(f[j]) * (1.0 - slow) + float(f[j]) / 4.0 * slow, rel_tol=1e-12)
+    # a million tokens, 8 columns: the ramp would go from the 3rd pair, the head's last, to the 6th
+    wide = kernels.rope_frequencies(8, scaling="yarn", factor=4.0, original_length=2 ** 20, whole_pairs=True)[0]
+    assert wide.tolist() == kernels.rope_frequencies(8)[0].tolist()
+    # both bounds behind the last column: nothing slows down; both before the first: everything from the second pair on
+    assert torch.equal(kernels.rope_frequencies(8, 1.5, "yarn", 4.0, 2 ** 20, whole_pairs=True)[0],
+                       kernels.rope_frequencies(8, 1.5)[0])
+    tiny = kernels.rope_frequencies(8, scaling="yarn", factor=4.0, original_length=1, whole_pairs=True)[0]
+    assert torch.allclose(tiny[1:], kernels.rope_frequencies(8)[0][1:] / 4.0, rtol=1e-12, atol=0.0) and tiny[0] == 1.0
+    for scaling in (None, "linear", "ntk"):
+        with pytest.raises(ValueError, match="whole_pairs"):
+            kernels.rope_frequencies(64, scaling=scaling, whole_pairs=True)
