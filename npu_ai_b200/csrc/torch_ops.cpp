@@ -16,6 +16,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <cmath>
 #include <optional>
 #include <type_traits>
@@ -548,6 +549,8 @@ at::Tensor attention_paged(const at::Tensor& q, const at::Tensor& k_pages, const
   const HeadRows qr = head_rows(q, k_pages, head_major_in, heads, d, "q");
   TORCH_CHECK_VALUE(scale >= 0, "attention scale must be positive (got ", scale, ")");
   if (scale == 0) scale = 1.0 / std::sqrt(double(d));
+  TORCH_CHECK_VALUE(softcap == 0 || float(softcap) != 0, "softcap must be 0 (none) or within [1e-30, 1e30] (got ", softcap, ")");
+  const int tiles = int(std::clamp<int64_t>(variant, -1, INT32_MAX));  // (what an int does not hold stays out of range)
   const c10::cuda::CUDAGuard guard(k_pages.device());
   at::Tensor out;
   const auto shape = head_major_out ? std::vector<int64_t>{B, heads, S, d} : std::vector<int64_t>{B, S, heads * d};
@@ -573,7 +576,7 @@ at::Tensor attention_paged(const at::Tensor& q, const at::Tensor& k_pages, const
   const c10::DataPtr ws = workspace(ws_bytes);  // (of this call's own: calls on other streams and captured graphs share none)
   check_rc(npub200_attention_paged(q.data_ptr(), qr.sb, qr.ss, qr.sh, &c, lens, out.data_ptr(), orr.sb, orr.ss, orr.sh,
                                    out_code, B, heads, S, float(scale), causal ? 1 : 0, starts, float(softcap), slopes_ptr,
-                                   ws.get(), ws_bytes, int(variant), stream_of(k_pages)),
+                                   ws.get(), ws_bytes, tiles, stream_of(k_pages)),
            "npub200::attention_paged");
   if (out_arg.has_value()) written(out);
   return out;

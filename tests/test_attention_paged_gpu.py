@@ -435,3 +435,17 @@ def test_slopes_of_far_queries(cuda_device, causal, variant):
             ref, _ = oracle(*row, causal=causal, kv_lens=c.lens, slopes=slopes, q_start=starts.long() + i)
             tol = oracle(*row, kv_lens=c.lens, slopes=slopes, q_start=near)[1]
             check(out[:, i:i + 1], ref, tol, H, False)
+
+
+def test_numbers_that_a_narrower_type_does_not_hold(cuda_device):
+    """A variant past 32 bits and a cap that is zero in f32 must not pass for the default."""
+    from npu_ai_b200 import _lib, kernels
+    d = cuda_device
+    c = Cache(d, [20], 2, 64, 8)
+    q = torch.randn(1, 1, 256, device=d).to(BF16)
+    for variant in (2 ** 32, -2 ** 32, 2 ** 63 - 1, -2 ** 63, 2 ** 32 + 1):
+        with pytest.raises(RuntimeError, match="variant"):
+            kernels.paged_attention(q, c.k, c.v, c.table, c.lens, 4, variant=variant)
+    for kw in (dict(softcap=1e-60), dict(softcap=-1e-60), dict(scale=1e-60), dict(scale=1e60), dict(softcap=1e60)):
+        with pytest.raises(ValueError, match="softcap|scale"):
+            _lib.torch_ops().attention_paged(q, c.k, c.v, c.table, c.lens, None, None, 4, **kw)
