@@ -553,7 +553,9 @@ __global__ void __launch_bounds__((kWarps + (TMA ? kLoadWarps : 0)) * 32, kBlock
         }
         // this lane's rows of the scores: c2 and c2 + 1 of each block
         int lim[NB][2], lim_min = INT32_MAX;
-        int near[NB][2];  // of the sequence's positions the one next to the row's: what distances are counted from
+        // Of the sequence's positions the one next to the row's: what distances are counted from. (An int would do; the capped
+        // form came out slower with it, 64 short caches 52.3 us instead of 51.5.)
+        long long near[NB][2];
         float slope[NB][2], m[NB][2], l[NB][2], o[DP / 16][NB][4];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
@@ -564,7 +566,7 @@ __global__ void __launch_bounds__((kWarps + (TMA ? kLoadWarps : 0)) * 32, kBlock
             const int i = ok ? a.by_g(r) : 0;
             const long long p = at.seq.p0 + i;
             lim[nb][y] = ok ? keys_seen(a, at.seq.len, p) : at.seq.len;
-            near[nb][y] = int(max(0ll, min(p, (long long)at.seq.len - 1)));
+            near[nb][y] = max(0ll, min(p, (long long)at.seq.len - 1));
             lim_min = min(lim_min, lim[nb][y]);
             slope[nb][y] = MODS && a.slopes != nullptr ? a.slopes[kvh * a.G + (ok ? r - i * a.G : 0)] * kLog2e : 0.0f;
             m[nb][y] = -INFINITY;
