@@ -313,8 +313,8 @@ int npub200_paged_append(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh
  * sees a NaN score is NaN. kv_lens are clamped to 0 ... table_width * page_size; keys behind them are not read. V has to be
  * finite at every key that some row sees. q: bf16, strides in multiples of 8 elements and a 16-byte aligned base, as the
  * pages'; out: bf16 or f32, any strides; it may be q itself (bf16, the same strides) and shares no element with q or the pages
- * otherwise. Head dims in multiples of 8 up to 256; any sq (made for few: a prompt's attention
- * belongs to npub200_attention_masked). The keys of the whole batch are split evenly over the GPU on the device, from
+ * otherwise. Head dims in multiples of 8 up to 256; any sq (made for few: a prompt's attention over
+ * its own keys belongs to npub200_attention_masked). The keys of the whole batch are split evenly over the GPU on the device, from
  * kv_lens: nothing but the sizes given here decides the launch, so a captured graph follows growing lengths. Partial results
  * go to `workspace` (npub200_attention_paged_workspace_size() bytes, 16-byte aligned, contents irrelevant) and a second
  * kernel joins them in a fixed order: deterministic. Calls that can run at the same time must not share a workspace.

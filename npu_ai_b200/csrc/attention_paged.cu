@@ -6,8 +6,9 @@
 //   m' = max(m, t), l' = l 2^(m - m') + sum_j 2^(s_j - m'), o' = o 2^(m - m') + sum_j 2^(s_j - m') v_j,
 // and parts (m, l, o) of one row's keys join the same way. Scores are kept in log2 units.
 //
-// Bound by memory: each key and value is read once and does 4 G flops a value for the G query heads of its head, far below
-// what the tensor cores need to be busy. So the design is about loads in flight, few instructions a key and an even split:
+// Bound by memory: each element of a key or value is read once and takes part in 2 G flops, a multiplication and an addition for
+// each of the G query heads of its head, far below what the tensor cores need to be busy. So the design is about loads in
+// flight, few instructions a key and an even split:
 //   * Keys are the rows of the matrix instructions: S^T = K Q^T and O^T = V^T P^T with mma.sync m16n8k16, 16 keys (16
 //     columns of the head) against 8 rows of queries. The rows of a (sequence, key/value head) are its G heads x the new
 //     tokens, mostly 8 or fewer, so nothing is padded to the 64 or 128 rows of a tcgen05 tile, and the softmax of a tile
@@ -16,15 +17,16 @@
 //   * Every block takes an equal run of tiles of the whole batch, found on the device from kv_lens, so ragged lengths leave
 //     no SM idle and a captured graph follows them, and its workers equal shares of it. Shares start and end anywhere in a
 //     sequence; the parts of a row's keys are joined in order of keys, first those of a block through its shared memory,
-//     then those of several blocks through the workspace by the join kernel. What is left: 24 of the 148 SMs read memory 15%
-//     slower than the others, and the equal runs wait for them.
+//     then those of several blocks through the workspace by the join kernel. What is left: 24 of the 148 SMs are done with equal
+//     runs 9% after the others (16 x 16384 keys: after 123 to 125 us, the median 114, by globaltimer stamps of each block;
+//     in a plain read of as many bytes the same SMs are not behind).
 //   * Pages of a multiple of 16 slots are read by TMA, a box of 64 columns x 16 (32) slots a copy; other pages and layouts
 //     that a tensor map does not take by cp.async, 16 bytes a lane, which costs as many instructions as all the arithmetic.
 //     (A bulk copy a row was the first form: the copy engine takes one in about 17 cycles, 16 bytes a cycle at 128 columns
 //     where 23 are the memory's rate.) Keys and values wait in one ring, a half tile each, swizzled in 128-byte rows, which
 //     ldmatrix reads without a bank conflict.
 // Measured (GPU time of a call with its join, a graph of calls): one token, 16 x 32/8 heads x 16384 keys (ragged) x 128 134 us,
-// 6.1 TB/s, 94% of the measured copy rate; 1 x 131071 keys 94 us, 5.7 TB/s; 777 keys x 64 8.3 us: launches, the run from
+// 6.1 TB/s, 94% of the measured copy rate; 1 x 131071 keys 94 us, 5.7 TB/s; 777 keys x 64 8.6 us: launches, the run from
 // kv_lens, the page table, the first keys and the join's records after each other.
 #include <algorithm>
 #include <atomic>
@@ -136,8 +138,9 @@ struct PagedLayout {
   static constexpr int kHalf = kAtoms * kAtom;
   static constexpr int kWorkers = kWarps / WR;
   static constexpr int kRows = 8 * NB * WR;
-  // As many as half an SM holds next to the static tables: up to 130 KB in flight on the SM, of which some 40 KB cover the
-  // latency at the full rate.
+  // As many as half an SM holds next to the static tables: 96 KB a block (64 KB with one worker), of which each worker uses one
+  // half while the others are on their way: 112 to 160 KB in flight on the SM, where some 40 KB cover the latency at the
+  // full rate.
   static constexpr int kFit = 104 * 1024 / (kWorkers * kHalf);
   static constexpr int kHalves = kFit < kMaxHalves ? kFit : kMaxHalves;
   static constexpr int kRing = kHalves * kHalf;
@@ -743,7 +746,8 @@ __global__ void __launch_bounds__((kWarps + (TMA ? kLoadWarps : 0)) * 32, kBlock
               }
           } else {
             // O^T += V^T P^T; P rounded to bf16 for the tensor core, 2^-8 relative at most, the sum takes the unrounded
-            // weights
+            // weights. (The error of a bf16 output against 64 bits, relative to its size, is 0.0023 on long caches, 0.0017 of it
+            // the output's own rounding; P in two bf16 parts would need twice the instructions of this product.)
             const bool all = valid == kAll;
 #pragma unroll
             for (int n = 0; n < KT / 16; ++n) {
@@ -1192,10 +1196,13 @@ int attention_paged_launch(const AttnPagedProblem& p, cudaStream_t stream) {
   a.ctl.status = dev->status;
   a.ctl.timeout_ns = wait_timeout_ns();
   a.ctl.debug = p.debug;
-  // TMA takes 16 slots of a page at a time, and maps of positive strides below 2^40 bytes. It moves 128 bytes of a row a step,
-  // whatever part of them the head fills, so heads that are no multiple of 128 are copied faster by cp.async where there is much
-  // to read (16 x 16384 keys of 64: 89 us, by TMA 104; 16 x 8000 of 80: 126 and 143; of 128: 137 and 133), while it starts sooner
-  // (777 keys of 64: 8.3 us, by cp.async 11).
+  // TMA takes 16 slots of a page at a time, and maps of positive strides below 2^40 bytes. Heads that are no multiple of 128
+  // columns are copied faster by cp.async where there is much to read: TMA moves the empty part of a column of 64 too (80, 96,
+  // 160), and its two warps have twice the half tiles to issue for the same bytes (64). One token, 32/8 heads, ragged, by TMA and by
+  // cp.async: 16 x 16384 keys of 64 99 and 89 us; 16 x 8000 of 80 72 and 65, of 96 77 and 70, of 160 113 and 108; of 128 and
+  // 256 level (72 and 73, 135 and 133). With little to read TMA starts sooner (777 keys of 64 8.7 us, 9.6 by cp.async; of 128
+  // 9.1 and 10.1). How much that is only the device knows: the table's width, which the lengths end at, stands for it here, so
+  // short caches under a table for long ones are copied by cp.async.
   const bool few_keys = p.batch * c.kv_heads * (a.capacity / 32 + 1) <= int64_t(plan.blocks) * 8;
   CUtensorMap mk, mv;
   memset(&mk, 0, sizeof(mk));
