@@ -1,4 +1,4 @@
-// overlap.h - whether two strided tensors have a byte in common. Host code without torch or CUDA.
+// overlap.h - whether two strided tensors have a byte in common, or one holds a byte twice. Host code without torch or CUDA.
 //
 // A tensor is its runs of contiguous bytes at base + sum_i x_i step_i, 0 <= x_i < n_i. Two of them are compared dimension by
 // dimension from the largest step down, where only those indices are followed whose bounds meet. Two dimensions of one step (views
@@ -72,6 +72,18 @@ inline bool bytes_overlap(const ByteRuns& a, const ByteRuns& b) {
   if (a.run == 0 || b.run == 0) return false;
   int left = kOverlapSteps;
   return bytes_meet(a, 0, b, 0, int64_t(b.base) - int64_t(a.base), left);
+}
+
+// Whether two elements of a tensor lie on the same bytes: windows that overlap (what a stride of 0 repeats is not asked here). Of
+// each dimension, whether what lies within it meets itself one or more steps on.
+inline bool bytes_repeat(const ByteRuns& a) {
+  int left = kOverlapSteps;
+  for (int i = 0; a.run != 0 && i < a.dims; ++i) {
+    const int64_t within = bytes_span(a, i + 1);
+    for (int64_t k = 1; k < a.n[i] && k * a.step[i] < within; ++k)
+      if (bytes_meet(a, i + 1, a, i + 1, k * a.step[i], left)) return true;
+  }
+  return false;
 }
 
 }  // namespace npub200

@@ -391,7 +391,8 @@ bool same_tensor(const at::Tensor& a, const at::Tensor& b) {
 
 // A tensor that a kernel writes: no element twice, and `from` itself or nothing of it.
 void check_written(const at::Tensor& t, const char* name, const at::Tensor* from = nullptr) {
-  TORCH_CHECK_VALUE(at::has_internal_overlap(t) != at::MemOverlap::Yes, name, " must not hold an element twice");
+  TORCH_CHECK_VALUE(at::has_internal_overlap(t) != at::MemOverlap::Yes && !npub200::bytes_repeat(runs_of(t)), name,
+                    " must not hold an element twice");
   TORCH_CHECK_VALUE(from == nullptr || same_tensor(t, *from) || !npub200::bytes_overlap(runs_of(t), runs_of(*from)), name,
                     " must be the input itself or share no element with it: they overlap");
 }

@@ -1,4 +1,5 @@
-"""csrc/overlap.h, compiled here: whether two strided tensors have a byte in common, against the sets of their bytes."""
+"""csrc/overlap.h, compiled here: whether two strided tensors have a byte in common, or one holds a byte twice, against the sets
+of their bytes."""
 import ctypes
 import itertools
 import os
@@ -18,18 +19,20 @@ def overlap(tmp_path_factory):
         '#include "overlap.h"\nusing namespace npub200;\n'
         'extern "C" int overlap(int64_t pa, int64_t ea, int da, const int64_t* na, const int64_t* sa, int64_t pb, int64_t eb, '
         'int db, const int64_t* nb, const int64_t* sb) {\n'
-        '  return bytes_overlap(byte_runs((const void*)pa, ea, da, na, sa), byte_runs((const void*)pb, eb, db, nb, sb));\n}\n')
+        '  return bytes_overlap(byte_runs((const void*)pa, ea, da, na, sa), byte_runs((const void*)pb, eb, db, nb, sb));\n}\n'
+        'extern "C" int repeats(int64_t p, int64_t e, int d, const int64_t* n, const int64_t* s) {\n'
+        '  return bytes_repeat(byte_runs((const void*)p, e, d, n, s));\n}\n')
     so = d / "o.so"
     subprocess.run(["g++", "-O1", "-std=c++17", "-Wall", "-Werror", "-fPIC", "-shared", f"-I{CSRC}", str(d / "o.cpp"), "-o",
                     str(so)], check=True)
     lib = ctypes.CDLL(str(so))
 
-    def call(a, b):
+    def call(*tensors):
         args = []
-        for base, element, sizes, strides in (a, b):
+        for base, element, sizes, strides in tensors:
             n = len(sizes)
             args += [I64(base), I64(element), n, (I64 * n)(*sizes), (I64 * n)(*strides)]
-        return bool(lib.overlap(*args))
+        return bool((lib.overlap if len(tensors) == 2 else lib.repeats)(*args))
     return call
 
 
@@ -97,3 +100,22 @@ def test_large_tensors(overlap):
     both_ways(overlap, (0, 4, [2 ** 20], [2]), (4, 4, [2 ** 20], [2]), False)
     both_ways(overlap, (0, 4, [2 ** 31], [1]), (2 ** 33, 4, [2 ** 31], [1]), False)
     both_ways(overlap, (0, 4, [2 ** 31], [1]), (2 ** 33 - 1, 4, [2 ** 31], [1]), True)
+
+
+def test_tensors_that_hold_a_byte_twice(overlap):
+    rng = random.Random(3)
+    found = 0
+    for _ in range(6000):
+        dims = rng.randint(0, 4)
+        t = (1000, rng.choice((2, 4)), [rng.choice((0, 1, 2, 2, 3, 4)) for _ in range(dims)],
+             [rng.choice((1, 2, 3, 5, 8, 12, 24, 30)) for _ in range(dims)])
+        elements = t[1]
+        for n in t[2]:
+            elements *= n
+        want = len(bytes_of(t)) < elements
+        assert overlap(t) == want, t
+        found += want
+    assert 300 < found < 5700
+    W, S = 6144, 8192
+    assert not overlap((0, 2, [64, S, 32, 128], [S * W, W, 128, 1])) and not overlap((0, 2, [2 ** 20, 8, 16, 128], [2 ** 15, 128, 1024, 1]))
+    assert overlap((0, 2, [64, S, 1024], [S * W, 1020, 1])) and overlap((0, 2, [64, S, 1024], [(S - 1) * W, W, 1]))

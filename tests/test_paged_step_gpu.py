@@ -187,3 +187,27 @@ def test_runner_numbers_past_32_bits(cuda_device):
         with pytest.raises(ValueError):
             bad()
     kernels.check_status(dev)
+
+
+def test_written_windows_that_overlap_are_refused(cuda_device):
+    """Outputs and pools whose rows, pages or heads reach into the next ones, as strides alone can make them."""
+    from npu_ai_b200 import kernels
+    dev, H, hk, D = cuda_device, 4, 2, 64
+    f, _ = kernels.rope_frequencies(D, device=dev)
+    q, (k, v) = torch.randn(2, 3, H * D, device=dev).to(BF16), (torch.randn(2, 3, hk * D, device=dev).to(BF16) for _ in range(2))
+    kp, vp = (torch.zeros(4, 16, hk, D, dtype=BF16, device=dev) for _ in range(2))
+    table, zero = torch.arange(4, dtype=torch.int32, device=dev).view(2, 2), torch.zeros(2, dtype=torch.int32, device=dev)
+    buf = torch.full((4, 20, 2 * H, D), 3.0, dtype=BF16, device=dev).view(-1)
+    for st in ((3 * H * D, H * D - 8, 1), (2 * H * D, H * D, 1), (8, 2048, 1)):
+        o = buf.as_strided((2, 3, H * D), st)
+        for call in (lambda: kernels.rope(q, f, H, out=o), lambda: kernels.paged_attention(q, kp, vp, table, zero + 3, H, out=o),
+                     lambda: kernels.paged_append(k, v, kp, vp, table, zero, q=q, heads=H, freqs=f, q_out=o)):
+            with pytest.raises(ValueError, match="twice"):
+                call()
+    for st in ((16 * hk * D - 64, hk * D, D, 1), (16 * hk * D, hk * D, D - 8, 1), (16 * hk * D, 64, D, 1)):
+        pages = buf.as_strided((4, 16, hk, D), st)
+        for pools in ((pages, vp), (kp, pages)):
+            with pytest.raises(ValueError, match="twice"):
+                kernels.paged_append(k, v, *pools, table, zero)
+    assert bool((buf == 3).all()) and bool((kp == 0).all())
+    kernels.check_status(dev)
