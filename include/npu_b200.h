@@ -306,19 +306,20 @@ int npub200_paged_append(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh
                          const npub200_paged_cache* cache, const int32_t* starts, const int32_t* counts, int64_t batch,
                          int64_t seq, const npub200_rotation* rotation, void* stream);
 
-/* Attention of a few new tokens of each sequence over its pages: npub200_attention_masked with key j of sequence b read from
- * position j of its table. Row i of sequence b stands at p_i = q_starts[b] + i (NULL: kv_lens[b] - sq + i) and sees the
- * keys j < kv_lens[b], with causal those of them with j <= p_i, on pages that are there; scores are scale q_i . k_j, then
- * softcap tanh(s / softcap) when softcap > 0, then - slopes[h] |p_i - j| when given. A row that sees no key is zeros, one that
- * sees a NaN score is NaN. kv_lens are clamped to 0 ... table_width * page_size; keys behind them are not read. V has to be
- * finite at every key that some row sees. q: bf16, strides in multiples of 8 elements and a 16-byte aligned base, as the
- * pages'; out: bf16 or f32, any strides; it may be q itself (bf16, the same strides) and shares no element with q or the pages
- * otherwise. Head dims in multiples of 8 up to 256; any sq (made for few: a prompt's attention over
- * its own keys belongs to npub200_attention_masked). The keys of the whole batch are split evenly over the GPU on the device, from
- * kv_lens: nothing but the sizes given here decides the launch, so a captured graph follows growing lengths. Partial results
- * go to `workspace` (npub200_attention_paged_workspace_size() bytes, 16-byte aligned, contents irrelevant) and a second
- * kernel joins them in a fixed order: deterministic. Calls that can run at the same time must not share a workspace.
- * variant: 0, or the least number of key tiles (32 keys, 16 above 128 columns) of one split (1 ... 2^20). Allocates nothing. */
+/* Attention of a few new tokens of each sequence over its pages: npub200_attention_masked with key j of sequence b
+ * read from position j of its table. Row i of sequence b stands at p_i = q_starts[b] + i (NULL: kv_lens[b] - sq + i)
+ * and sees the keys j < kv_lens[b], with causal those of them with j <= p_i, on pages that are there; scores are scale
+ * q_i . k_j, then softcap tanh(s / softcap) when softcap > 0, then - slopes[h] |p_i - j| when given. A row that sees
+ * no key is zeros, one that sees a NaN score is NaN; a score of -infinity hides its key. kv_lens are clamped to 0 ...
+ * table_width * page_size; keys behind them are not read. V has to be finite at every key that some row sees. q: bf16,
+ * strides in multiples of 8 elements and a 16-byte aligned base, as the pages'; out: bf16 or f32, any strides; it may
+ * be q itself (bf16, the same strides) and shares no element with q or the pages otherwise. Head dims in multiples of
+ * 8 up to 256; any sq (made for few: a prompt's attention over its own keys belongs to npub200_attention_masked). The
+ * keys of the whole batch are split evenly over the GPU on the device, from kv_lens: nothing but the sizes given here
+ * decides the launch, so a captured graph follows growing lengths. Partial results go to `workspace`
+ * (npub200_attention_paged_workspace_size() bytes, 16-byte aligned, contents irrelevant) and a second kernel joins
+ * them in a fixed order: deterministic. Calls that can run at the same time must not share a workspace. variant: 0, or
+ * the least number of key tiles (32 keys, 16 above 128 columns) of one split (1 ... 2^20). Allocates nothing. */
 int npub200_attention_paged_workspace_size(int64_t heads, int64_t kv_heads, int64_t sq, int64_t head_dim,
                                            size_t* bytes_out);
 int npub200_attention_paged(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, const npub200_paged_cache* cache,

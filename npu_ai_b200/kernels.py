@@ -719,8 +719,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                 are read when the call runs, so a captured graph follows their contents.
     q_start:    int32 [B], the position of query 0 (default kv_lens - Sq: the last query meets the last key).
     causal:     query i sees the keys up to its position q_start + i; otherwise all of kv_lens.
-    softcap, slopes: as in attention. A row that may see no key is zero, one that sees a NaN score NaN; v has to be finite
-                at every key that some row sees.
+    softcap, slopes: as in attention. A row that may see no key is zero, one that sees a NaN score NaN, and a score of -inf
+                hides its key; v has to be finite at every key that some row sees.
     The batch's keys are split evenly over the GPU whatever the lengths. Made for few tokens; the attention of a prompt is
     `attention`, on its own keys. variant: the least number of key tiles of one split (0 = automatic).
     """

@@ -449,3 +449,20 @@ def test_numbers_that_a_narrower_type_does_not_hold(cuda_device):
     for kw in (dict(softcap=1e-60), dict(softcap=-1e-60), dict(scale=1e-60), dict(scale=1e60), dict(softcap=1e60)):
         with pytest.raises(ValueError, match="softcap|scale"):
             _lib.torch_ops().attention_paged(q, c.k, c.v, c.table, c.lens, None, None, 4, **kw)
+
+
+@pytest.mark.parametrize("variant", [0, 1, 1000])
+def test_rows_with_nothing_but_minus_infinity_are_zeros(cuda_device, variant):
+    """As rows that see no key; the sequence's other heads and the batch's other rows are what they are without it."""
+    from npu_ai_b200 import kernels
+    d = cuda_device
+    lens = [200, 200, 33]
+    c = Cache(d, lens, 2, 64, 16)
+    q = torch.randn(3, 2, 256, device=d).abs().to(BF16)
+    want = kernels.paged_attention(q, c.k, c.v, c.table, c.lens, 4, variant=variant).view(3, 2, 4, 64)
+    at = torch.arange(200, device=d)
+    c.k[c.table[1].long()[at // 16], at % 16, 0] = float("-inf")  # key/value head 0 of sequence 1
+    o = kernels.paged_attention(q, c.k, c.v, c.table, c.lens, 4, variant=variant).view(3, 2, 4, 64)
+    kernels.check_status(d)
+    want[1, :, :2] = 0.0
+    assert torch.equal(o, want)
